@@ -200,7 +200,7 @@ def prepare(case, seed):
 # ---------------------------------------------------------------------------------------------- plain forms
 def _column(value, rows):
     """A setting as a 64-bit column, a value for each row."""
-    value = torch.as_tensor(value, device=DEVICE).double().reshape(-1, 1)
+    value = torch.as_tensor(value, dtype=torch.float64, device=DEVICE).reshape(-1, 1)
     return value.expand(rows, 1)
 
 
