@@ -60,6 +60,7 @@ enum trlk_scale_rewards { TRLK_SCALE_GROUP = 0, TRLK_SCALE_BATCH = 1, TRLK_SCALE
 
 /* bits of the int32 word the kernels OR into `d_error_flag` */
 #define TRLK_FLAG_INDEX_OUT_OF_RANGE 1
+#define TRLK_FLAG_NO_DISTRIBUTION 2 /* a row to draw from, or to score under, holds a NaN or +inf, nothing but -inf, or has a bad setting */
 
 int trlk_version(void);
 
@@ -430,6 +431,57 @@ int trlk_grpo_fused_fwd_bwd(const void* d_logits, int dtype, int64_t n_seq, int6
                             int64_t out_row_stride, int compute_masked_rows, int32_t* d_error_flag,
                             trlk_stream_t stream);
 int trlk_scale_unless_one(void* d_data, int dtype, int64_t n_elems, const float* d_scale, trlk_stream_t stream);
+
+/* ---------------------------------------------------------------------------------------
+ * K8  tokens drawn from, and scored under, softmax(logits / T) after top-k, top-p and min-p (the sampling settings of the
+ * trainers' generation: temperature, top_k, top_p, min_p, trl/trainer/grpo_config.py:522; the sampler's log-probs are
+ * `sampling_per_token_logps`, trl/trainer/grpo_trainer.py:2579-2623).
+ * A row's tokens are ordered by logit descending, index ascending; each filter keeps a prefix of that order:
+ *   top_k  > 0: the first top_k tokens
+ *   top_p  < 1: the tokens before which less than top_p of the mass lies that top-k kept (the first one always)
+ *   min_p  > 0: the tokens of at least min_p times the largest probability
+ * temperature 0 keeps the first token alone; -inf logits are never kept.  With w_v = exp((x_v - max) / T) for the kept tokens,
+ * 0 for the others, and C_v = w_0 + ... + w_v:
+ *   token = min { v : C_v > u C_last },  logp = log(w_token / C_last)
+ * Weights and their sums are held in 64 bits, so that a row's token is the same one whatever the number of rows.
+ * Each setting is one number for all rows (0 <= temperature < inf, top_k <= 0: none, 0 < top_p <= 1, 0 <= min_p <= 1) or, where
+ * d_temperature / d_top_k / d_top_p / d_min_p is not NULL, one for each row (top_p <= 0: the first token, > 1: 1, min_p < 0: 0,
+ * > 1: 1).  A row without a distribution (a NaN or +inf, nothing but -inf, or a temperature that is negative, infinite or NaN, a
+ * NaN top_p or min_p) gets the token -1 and a NaN log-prob, and sets TRLK_FLAG_NO_DISTRIBUTION in *d_error_flag (may be NULL).
+ * d_row_mask (optional, uint8 [rows]): rows whose mask is 0 are not read, and get the token fill_id and the log-prob 0.
+ * d_uniform: numbers in [0, 1), fp64 if uniform_f64 is non-zero, else fp32.  vocab <= trlk_token_filter_max_vocab().
+ * d_workspace: trlk_token_filter_workspace_bytes(rows, vocab, dtype) bytes, 16-byte aligned.
+ */
+int64_t trlk_token_filter_max_vocab(void);
+size_t trlk_token_filter_workspace_bytes(int64_t rows, int64_t vocab, int dtype);
+int trlk_sample_tokens(const void* d_logits, int dtype, int64_t n_seq, int64_t rows_per_seq, int64_t vocab,
+                       int64_t seq_stride, int64_t row_stride, const void* d_uniform, int32_t uniform_f64,
+                       double temperature, const float* d_temperature, int64_t top_k, const int32_t* d_top_k, double top_p,
+                       const float* d_top_p, double min_p, const float* d_min_p, const uint8_t* d_row_mask, int64_t fill_id,
+                       int64_t* d_out_ids, float* d_out_logp, int32_t* d_error_flag, void* d_workspace,
+                       size_t workspace_bytes, trlk_stream_t stream);
+
+/* trlk_filtered_logps_fwd: log(w_token / C_last) of given tokens (d_index int64 [rows]) under the same distribution; -inf for a
+ * token that the filters take away, NaN (and the flag TRLK_FLAG_INDEX_OUT_OF_RANGE) for one outside [0, vocab), 0 for a row
+ * whose mask is 0.  d_out_state fp32 [rows, 4] and d_out_block_max (in the logits' type, [rows, trlk_token_filter_blocks(vocab)];
+ * may be NULL) are what the backward needs; block maxima exist where trlk_token_filter_has_blocks(...) is 1.
+ * trlk_filtered_logps_bwd: the whole gradient of the logits, d_dlogits dense [rows, vocab],
+ *   dlogits[r, v] = g_logp[r] / T * (1[v == index[r]] - w_v / C_last)
+ * (the kept tokens are taken as given), 0 in rows whose token lies outside the support, whose mask is 0 or whose g_logp is 0.
+ * d_block_max NULL: every logit is read. */
+int64_t trlk_token_filter_blocks(int64_t vocab);
+int trlk_token_filter_has_blocks(double temperature, const float* d_temperature, int64_t top_k, const int32_t* d_top_k,
+                                 double top_p, const float* d_top_p, double min_p, const float* d_min_p);
+int trlk_filtered_logps_fwd(const void* d_logits, int dtype, int64_t n_seq, int64_t rows_per_seq, int64_t vocab,
+                            int64_t seq_stride, int64_t row_stride, const int64_t* d_index, double temperature,
+                            const float* d_temperature, int64_t top_k, const int32_t* d_top_k, double top_p,
+                            const float* d_top_p, double min_p, const float* d_min_p, const uint8_t* d_row_mask,
+                            float* d_out_logp, float* d_out_state, void* d_out_block_max, int32_t* d_error_flag,
+                            void* d_workspace, size_t workspace_bytes, trlk_stream_t stream);
+int trlk_filtered_logps_bwd(const void* d_logits, int dtype, int64_t n_seq, int64_t rows_per_seq, int64_t vocab,
+                            int64_t seq_stride, int64_t row_stride, const int64_t* d_index, double temperature,
+                            const float* d_temperature, const float* d_state, const void* d_block_max, const float* d_g_logp,
+                            void* d_dlogits, trlk_stream_t stream);
 
 #ifdef __cplusplus
 }

@@ -23,6 +23,7 @@ GRPO, BNPO, DR_GRPO, DAPO, LUSPO = 0, 1, 2, 3, 4
 TERM_CLIP, TERM_CISPO, TERM_SAPO, TERM_WEIGHTED_LOGP = 0, 1, 2, 3
 SCALE_GROUP, SCALE_BATCH, SCALE_NONE = 0, 1, 2
 FLAG_INDEX_OUT_OF_RANGE = 1
+FLAG_NO_DISTRIBUTION = 2
 GRPO_NUM_METRICS = 16
 GRPO_LOG_VALUES = 13
 DPO_NUM_METRICS = 8
@@ -133,6 +134,28 @@ SIGNATURES = {
         c_int32,
         [c_void_p, c_void_p, c_int32, c_int64, c_int64, c_int64, c_int64, c_int64, c_int64, c_int64, c_void_p, c_void_p,
          c_size_t, c_void_p],
+    ),
+    "trlk_token_filter_max_vocab": (c_int64, []),
+    "trlk_token_filter_workspace_bytes": (c_size_t, [c_int64, c_int64, c_int32]),
+    "trlk_token_filter_blocks": (c_int64, [c_int64]),
+    "trlk_token_filter_has_blocks": (
+        c_int32, [c_double, c_void_p, c_int64, c_void_p, c_double, c_void_p, c_double, c_void_p]),
+    "trlk_sample_tokens": (
+        c_int32,
+        [c_void_p, c_int32, c_int64, c_int64, c_int64, c_int64, c_int64, c_void_p, c_int32, c_double, c_void_p, c_int64,
+         c_void_p, c_double, c_void_p, c_double, c_void_p, c_void_p, c_int64, c_void_p, c_void_p, c_void_p, c_void_p,
+         c_size_t, c_void_p],
+    ),
+    "trlk_filtered_logps_fwd": (
+        c_int32,
+        [c_void_p, c_int32, c_int64, c_int64, c_int64, c_int64, c_int64, c_void_p, c_double, c_void_p, c_int64, c_void_p,
+         c_double, c_void_p, c_double, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_size_t,
+         c_void_p],
+    ),
+    "trlk_filtered_logps_bwd": (
+        c_int32,
+        [c_void_p, c_int32, c_int64, c_int64, c_int64, c_int64, c_int64, c_void_p, c_double, c_void_p, c_void_p, c_void_p,
+         c_void_p, c_void_p, c_void_p],
     ),
     "trlk_rloo_loss": (
         c_int32,

@@ -551,6 +551,143 @@ Tensor dpo_log_values(const Tensor& entropy_, const Tensor& row_stats_, const Te
                               fptr(ref_rejected), float(beta), error_word(mask), out(values), out(ws), stream_of(mask)));
     return values;
 }
+
+// ---- tokens drawn from, and scored under, a filtered distribution ------------------------------------------------------
+// The sampling settings: a number for all rows, or a tensor with a value for each.
+struct Settings {
+    double temperature, top_p, min_p;
+    int64_t top_k;
+    optional<Tensor> temperatures, top_ks, top_ps, min_ps;
+    const float* t() const { return fptr(temperatures); }
+    const float* p() const { return fptr(top_ps); }
+    const float* m() const { return fptr(min_ps); }
+    const int32_t* k() const { return top_ks ? static_cast<const int32_t*>(operand(*top_ks)) : nullptr; }
+};
+Settings settings(const char* op, int64_t rows, double temperature, int64_t top_k, double top_p, double min_p,
+                  const optional<Tensor>& temperatures, const optional<Tensor>& top_ks, const optional<Tensor>& top_ps,
+                  const optional<Tensor>& min_ps) {
+    for (const optional<Tensor>* t : {&temperatures, &top_ks, &top_ps, &min_ps})
+        TORCH_CHECK_VALUE(!*t || (*t)->numel() == rows, op, ": a setting has ", *t ? (*t)->numel() : 0, " values for ", rows, " rows");
+    return {temperature, top_p, min_p, top_k, f32c(temperatures),
+            top_ks ? optional<Tensor>(top_ks->contiguous().to(at::kInt)) : std::nullopt, f32c(top_ps), f32c(min_ps)};
+}
+const uint8_t* mask_ptr(const char* op, const optional<Tensor>& mask, int64_t rows) {
+    if (!mask) return nullptr;
+    TORCH_CHECK_VALUE(mask->numel() == rows && mask->element_size() == 1 && mask->is_contiguous(), op,
+                      ": the row mask must be one contiguous byte for each of ", rows, " rows");
+    return static_cast<const uint8_t*>(operand(*mask));
+}
+Tensor bytes(const Tensor& like, size_t n) { return at::empty({int64_t(n)}, like.options().dtype(at::kByte)); }
+
+std::tuple<Tensor, Tensor> sample_tokens(const Tensor& logits, const Tensor& uniforms_, double temperature, int64_t top_k, double top_p,
+                                         double min_p, const optional<Tensor>& temperatures, const optional<Tensor>& top_ks,
+                                         const optional<Tensor>& top_ps, const optional<Tensor>& min_ps,
+                                         const optional<Tensor>& row_mask, int64_t fill_id) {
+    check_logits3d(logits);
+    const int64_t n_seq = logits.size(0), length = logits.size(1), vocab = logits.size(2), rows = n_seq * length;
+    const c10::DeviceGuard guard(logits.device());
+    const int dtype = dtype_code(logits);
+    TORCH_CHECK_VALUE(uniforms_.numel() == rows, "sample_tokens: ", uniforms_.numel(), " uniform numbers for ", rows, " rows");
+    const Tensor ids = at::empty({rows}, logits.options().dtype(at::kLong)), logp = f32(logits, {rows});
+    const Settings s = settings("sample_tokens", rows, temperature, top_k, top_p, min_p, temperatures, top_ks, top_ps, min_ps);
+    const uint8_t* mask = mask_ptr("sample_tokens", row_mask, rows);
+    const bool f64 = uniforms_.scalar_type() == at::kDouble;
+    const Tensor uniforms = f64 ? uniforms_.contiguous() : f32c(uniforms_);
+    const size_t ws_bytes = trlk_token_filter_workspace_bytes(rows, vocab, dtype);
+    const Tensor ws = bytes(logits, ws_bytes);
+    check(trlk_sample_tokens(logits.const_data_ptr(), dtype, n_seq, length, vocab, logits.stride(0), logits.stride(1),
+                             operand(uniforms), f64 ? 1 : 0, s.temperature, s.t(), s.top_k, s.k(), s.top_p, s.p(), s.min_p, s.m(),
+                             mask, fill_id, static_cast<int64_t*>(ids.mutable_data_ptr()), out(logp), error_word(logits),
+                             ws.mutable_data_ptr(), ws_bytes, stream_of(logits)));
+    check_ids();
+    return {ids, logp};
+}
+
+Tensor3 filtered_logps_fwd(const Tensor& logits, const Tensor& index_, double temperature, int64_t top_k, double top_p, double min_p,
+                           const optional<Tensor>& temperatures, const optional<Tensor>& top_ks, const optional<Tensor>& top_ps,
+                           const optional<Tensor>& min_ps, const optional<Tensor>& row_mask) {
+    check_logits3d(logits);
+    const int64_t n_seq = logits.size(0), length = logits.size(1), vocab = logits.size(2), rows = n_seq * length;
+    const c10::DeviceGuard guard(logits.device());
+    const int dtype = dtype_code(logits);
+    TORCH_CHECK_VALUE(index_.numel() == rows && index_.scalar_type() == at::kLong, "filtered_logps: ", index_.numel(), " ", index_.scalar_type(),
+                      " token ids for ", rows, " rows of int64");
+    const Settings s = settings("filtered_logps", rows, temperature, top_k, top_p, min_p, temperatures, top_ks, top_ps, min_ps);
+    const uint8_t* mask = mask_ptr("filtered_logps", row_mask, rows);
+    const bool blocks = trlk_token_filter_has_blocks(s.temperature, s.t(), s.top_k, s.k(), s.top_p, s.p(), s.min_p, s.m()) != 0;
+    const Tensor logp = f32(logits, {rows}), state = f32(logits, {rows, 4});
+    const Tensor block_max = at::empty({blocks ? rows : 0, trlk_token_filter_blocks(vocab)}, logits.options());
+    const Tensor index = index_.contiguous();
+    const size_t ws_bytes = trlk_token_filter_workspace_bytes(rows, vocab, dtype);
+    const Tensor ws = bytes(logits, ws_bytes);
+    check(trlk_filtered_logps_fwd(logits.const_data_ptr(), dtype, n_seq, length, vocab, logits.stride(0), logits.stride(1), iptr(index),
+                                  s.temperature, s.t(), s.top_k, s.k(), s.top_p, s.p(), s.min_p, s.m(), mask, out(logp), out(state),
+                                  blocks ? block_max.mutable_data_ptr() : nullptr, error_word(logits), ws.mutable_data_ptr(), ws_bytes,
+                                  stream_of(logits)));
+    check_ids();
+    return {logp, state, block_max};
+}
+
+Tensor filtered_logps_bwd(const Tensor& logits, const Tensor& index_, double temperature, const optional<Tensor>& temperatures_,
+                          const Tensor& state, const Tensor& block_max, const Tensor& g_logp_) {
+    check_logits3d(logits);
+    const int64_t n_seq = logits.size(0), length = logits.size(1), vocab = logits.size(2), rows = n_seq * length;
+    const c10::DeviceGuard guard(logits.device());
+    const Tensor dlogits = at::empty({n_seq, length, vocab}, logits.options());
+    if (dlogits.numel() == 0) return dlogits;
+    TORCH_CHECK_VALUE(index_.numel() == rows && g_logp_.numel() == rows && state.numel() == 4 * rows && state.is_contiguous() &&
+                          (!temperatures_ || temperatures_->numel() == rows) &&
+                          (block_max.numel() == 0 || block_max.numel() == rows * trlk_token_filter_blocks(vocab)),
+                      "filtered_logps: the backward's operands do not match");
+    const Tensor index = index_.contiguous(), g_logp = f32c(g_logp_);
+    const optional<Tensor> temperatures = f32c(temperatures_);
+    check(trlk_filtered_logps_bwd(logits.const_data_ptr(), dtype_code(logits), n_seq, length, vocab, logits.stride(0), logits.stride(1),
+                                  iptr(index), temperature, fptr(temperatures), fptr(state),
+                                  block_max.numel() ? operand(block_max) : nullptr, fptr(g_logp), dlogits.mutable_data_ptr(),
+                                  stream_of(logits)));
+    return dlogits;
+}
+
+class FilteredLogps : public torch::autograd::Function<FilteredLogps> {
+  public:
+    static variable_list forward(AutogradContext* ctx, const Tensor& logits, const Tensor& index, double temperature, int64_t top_k,
+                                 double top_p, double min_p, const optional<Tensor>& temperatures, const optional<Tensor>& top_ks,
+                                 const optional<Tensor>& top_ps, const optional<Tensor>& min_ps, const optional<Tensor>& row_mask) {
+        variable_list result;
+        {
+            at::AutoDispatchBelowADInplaceOrView below;
+            static const auto op = handle<decltype(filtered_logps_fwd)>("trl_amd::filtered_logps_fwd");
+            auto [logp, state, block_max] =
+                op.call(logits, index, temperature, top_k, top_p, min_p, temperatures, top_ks, top_ps, min_ps, row_mask);
+            result = {logp, state, block_max};
+        }
+        ctx->save_for_backward({logits, index, result[1], result[2], temperatures ? *temperatures : Tensor()});
+        ctx->saved_data["temperature"] = temperature;
+        ctx->mark_non_differentiable({result[1], result[2]});
+        ctx->set_materialize_grads(false);
+        return result;
+    }
+    static variable_list backward(AutogradContext* ctx, const variable_list& grads) {
+        variable_list result(11);
+        if (!grads[0].defined()) return result;
+        const auto saved = ctx->get_saved_variables();
+        static const auto op = handle<decltype(filtered_logps_bwd)>("trl_amd::filtered_logps_bwd");
+        result[0] = op.call(saved[0], saved[1], ctx->saved_data["temperature"].toDouble(),
+                            saved[4].defined() ? optional<Tensor>(saved[4]) : std::nullopt, saved[2], saved[3], grads[0]);
+        return result;
+    }
+};
+Tensor3 filtered_logps_fwd_autograd(const Tensor& logits, const Tensor& index, double temperature, int64_t top_k, double top_p,
+                                    double min_p, const optional<Tensor>& temperatures, const optional<Tensor>& top_ks,
+                                    const optional<Tensor>& top_ps, const optional<Tensor>& min_ps, const optional<Tensor>& row_mask) {
+    if (needs_grad({&logits})) {
+        const auto r = FilteredLogps::apply(logits, index, temperature, top_k, top_p, min_p, temperatures, top_ks, top_ps, min_ps, row_mask);
+        return {r[0], r[1], r[2]};
+    }
+    at::AutoDispatchBelowADInplaceOrView below;
+    static const auto op = handle<decltype(filtered_logps_fwd)>("trl_amd::filtered_logps_fwd");
+    return op.call(logits, index, temperature, top_k, top_p, min_p, temperatures, top_ks, top_ps, min_ps, row_mask);
+}
 }  // namespace
 
 TORCH_LIBRARY_FRAGMENT(trl_amd, m) {
@@ -582,6 +719,12 @@ TORCH_LIBRARY_FRAGMENT(trl_amd, m) {
           "-> (Tensor, Tensor, Tensor, Tensor)");
     m.def("dpo_log_values(Tensor entropy, Tensor row_stats, Tensor mask, Tensor seq_logps, Tensor ref_chosen, "
           "Tensor ref_rejected, float beta) -> Tensor");
+    m.def("sample_tokens(Tensor logits, Tensor uniforms, float temperature, int top_k, float top_p, float min_p, "
+          "Tensor? temperatures, Tensor? top_ks, Tensor? top_ps, Tensor? min_ps, Tensor? row_mask, int fill_id) -> (Tensor, Tensor)");
+    m.def("filtered_logps_fwd(Tensor logits, Tensor index, float temperature, int top_k, float top_p, float min_p, "
+          "Tensor? temperatures, Tensor? top_ks, Tensor? top_ps, Tensor? min_ps, Tensor? row_mask) -> (Tensor, Tensor, Tensor)");
+    m.def("filtered_logps_bwd(Tensor logits, Tensor index, float temperature, Tensor? temperatures, Tensor state, Tensor block_max, "
+          "Tensor g_logp) -> Tensor");
 }
 TORCH_LIBRARY_IMPL(trl_amd, CUDA, m) {
     m.impl("logp_entropy_fwd", logp_entropy_fwd);
@@ -594,14 +737,18 @@ TORCH_LIBRARY_IMPL(trl_amd, CUDA, m) {
     m.impl("grpo_row_scale", grpo_row_scale);
     m.impl("dpo_loss", dpo_loss);
     m.impl("dpo_log_values", dpo_log_values);
+    m.impl("sample_tokens", sample_tokens);
+    m.impl("filtered_logps_fwd", filtered_logps_fwd);
+    m.impl("filtered_logps_bwd", filtered_logps_bwd);
 }
 TORCH_LIBRARY_IMPL(trl_amd, Autograd, m) {
     m.impl("logp_entropy_fwd", logp_entropy_fwd_autograd);
     m.impl("logp_entropy_stats_fwd", logp_entropy_stats_fwd_autograd);
     m.impl("grpo_loss", grpo_loss_autograd);
     m.impl("dpo_loss", dpo_loss_autograd);
-    for (const char* name : {"logp_entropy_bwd", "grpo_row_scale", "dpo_log_values"})
+    m.impl("filtered_logps_fwd", filtered_logps_fwd_autograd);
+    for (const char* name : {"logp_entropy_bwd", "grpo_row_scale", "dpo_log_values", "filtered_logps_bwd"})
         m.impl(name, torch::autograd::autogradNotImplementedFallback());
-    // (these hand out a gradient or scale one in place: their results belong to no graph, whatever the logits require)
-    for (const char* name : {"grpo_fused", "scale_unless_one_"}) m.impl(name, torch::CppFunction::makeFallthrough());
+    // (these hand out a gradient, scale one in place or draw: their results belong to no graph, whatever the logits require)
+    for (const char* name : {"grpo_fused", "scale_unless_one_", "sample_tokens"}) m.impl(name, torch::CppFunction::makeFallthrough());
 }

@@ -31,8 +31,18 @@ def _error_flag(device: torch.device) -> Tensor:
     return torch.ops.trl_amd.error_flag.default(device.index if device.index is not None else torch.cuda.current_device())
 
 
+def _raise_for(bits: int) -> None:
+    if bits & _lib.FLAG_INDEX_OUT_OF_RANGE:
+        raise IndexError("trl_amd: an index passed to a log-prob kernel was outside [0, vocab)")
+    if bits & _lib.FLAG_NO_DISTRIBUTION:
+        raise ValueError("trl_amd: a row of logits has no distribution to draw from (a NaN or +inf among them, nothing but -inf, "
+                         "or a temperature, top_p or min_p of its own that is none)")
+    raise RuntimeError(f"trl_amd: device error flag {bits:#x}")
+
+
 def check_device_errors() -> None:
-    """Raises IndexError if any kernel since the last call saw an index outside [0, vocab).
+    """Raises IndexError if any kernel since the last call saw an index outside [0, vocab), ValueError if one was to draw or
+    score a token in a row without a distribution.
 
     The reference raises synchronously on CPU and device-asserts on GPU
     (`torch.gather`, trl/trainer/utils.py:507,516); here the entry gets NaN, a flag is set on
@@ -43,9 +53,7 @@ def check_device_errors() -> None:
         bits = int(flag.item())
         if bits:
             flag.zero_()
-            if bits & _lib.FLAG_INDEX_OUT_OF_RANGE:
-                raise IndexError("trl_amd: an index passed to a log-prob kernel was outside [0, vocab)")
-            raise RuntimeError(f"trl_amd: device error flag {bits:#x}")
+            _raise_for(bits)
 
 
 def device_error_bits(device: torch.device) -> Tensor:
@@ -59,9 +67,7 @@ def raise_for_error_bits(bits: float, device: torch.device) -> None:
     bits = int(bits)
     if bits:
         _error_flag(device).zero_()
-        if bits & _lib.FLAG_INDEX_OUT_OF_RANGE:
-            raise IndexError("trl_amd: an index passed to a log-prob kernel was outside [0, vocab)")
-        raise RuntimeError(f"trl_amd: device error flag {bits:#x}")
+        _raise_for(bits)
 
 
 _library = torch.library.Library("trl_amd", "FRAGMENT")
@@ -224,6 +230,38 @@ def logp_entropy_forward(logits: Tensor, index: Tensor, temperature: float, keep
     """The forward op for these logits: the double-precision pair for float64, the streaming kernels otherwise."""
     op = logp_entropy_fwd_f64 if logits.dtype == torch.float64 else logp_entropy_fwd
     return op(logits, index, temperature, keep_start, keep_len, row_mask)
+
+
+# --------------------------------------------------------------------------------------------
+# tokens drawn from, and scored under, a filtered distribution (K8)
+# --------------------------------------------------------------------------------------------
+def _rows_of(logits) -> int:
+    return logits.shape[0] * logits.shape[1]
+
+
+# logits [n_seq, L, V] (strided view, last axis contiguous), uniforms fp32 or fp64 with an entry for each row.  A setting is a
+# number, or (the tensors behind them) a value for each row.  Returns (ids int64 [rows], logps fp32 [rows]).
+sample_tokens = _native_op(
+    "sample_tokens", lambda logits, uniforms, temperature, top_k, top_p, min_p, temperatures, top_ks, top_ps, min_ps, row_mask, fill_id:
+    (torch.empty((_rows_of(logits),), dtype=torch.int64, device=logits.device), _f32_like(logits, _rows_of(logits))))
+
+
+# As above for given tokens, index int64 [rows].  Returns (logps fp32 [rows], the backward's row state fp32 [rows, 4], block
+# maxima in the logits' type); the first carries the gradient.
+def _filtered_logps_fake(logits, index, temperature, top_k, top_p, min_p, temperatures, top_ks, top_ps, min_ps, row_mask):
+    rows, blocks = _rows_of(logits), -(-logits.shape[2] // 2048) * 32
+    per_row = any(t is not None for t in (temperatures, top_ks, top_ps, min_ps))
+    has = per_row or temperature == 0.0 or top_k > 0 or top_p < 1.0 or min_p > 0.0
+    return (_f32_like(logits, rows), _f32_like(logits, rows, 4),
+            torch.empty((rows if has else 0, blocks), dtype=logits.dtype, device=logits.device))
+
+
+filtered_logps_fwd = _native_op("filtered_logps_fwd", _filtered_logps_fake)
+
+# d(loss)/d(logits), contiguous [n_seq, L, V] in the logits' type.
+filtered_logps_bwd = _native_op(
+    "filtered_logps_bwd", lambda logits, index, temperature, temperatures, state, block_max, g_logp:
+    torch.empty(logits.shape, dtype=logits.dtype, device=logits.device))
 
 
 # --------------------------------------------------------------------------------------------

@@ -10,7 +10,7 @@ from torch import Tensor
 
 from .. import ops
 
-__all__ = ["selective_log_softmax", "entropy_from_logits", "logps_and_entropies", "nanstd", "nanmin", "nanmax",
+__all__ = ["selective_log_softmax", "entropy_from_logits", "logps_and_entropies", "sample_tokens", "filtered_logps", "nanstd", "nanmin", "nanmax",
            "_ChunkedLogProbFunction", "chunked_logprobs_from_hidden", "patch_chunked_lm_head"]
 
 
@@ -99,6 +99,82 @@ def entropy_from_logits(logits: Tensor, chunk_size: int = 128, out_dtype: torch.
     ent = ent.view(logits.shape[:-1])
     out_dtype = logits.dtype if out_dtype is None else out_dtype
     return ent if out_dtype == ent.dtype else ent.to(out_dtype)
+
+
+# ----------------------------------------------------------------------------------------------
+# tokens drawn from, and scored under, a filtered distribution
+# ----------------------------------------------------------------------------------------------
+def _settings(shape: torch.Size, temperature, top_k, top_p, min_p) -> tuple:
+    """The four settings as the operators take them: numbers, and tensors (or None) with a value for each row."""
+    numbers, tensors = [], []
+    for name, value, off in (("temperature", temperature, 1.0), ("top_k", top_k, 0), ("top_p", top_p, 1.0), ("min_p", min_p, 0.0)):
+        if isinstance(value, Tensor) and (value.dim() or value.is_cuda):
+            if value.numel() == 1 and value.shape != shape:
+                value = value.reshape(1).expand(shape)
+            if value.shape != shape:
+                raise ValueError(f"{name} of shape {tuple(value.shape)} for rows of shape {tuple(shape)}")
+            numbers.append(off)
+            tensors.append(value)
+        else:
+            numbers.append(off if value is None else type(off)(value))
+            tensors.append(None)
+    return (*numbers, *tensors)
+
+
+def _byte_mask(row_mask: Tensor | None, shape: torch.Size) -> Tensor | None:
+    if row_mask is None:
+        return None
+    if row_mask.shape != shape:
+        raise ValueError(f"row_mask of shape {tuple(row_mask.shape)} for rows of shape {tuple(shape)}")
+    if row_mask.dtype != torch.bool:
+        row_mask = row_mask != 0
+    return row_mask.contiguous().view(torch.uint8)
+
+
+def sample_tokens(logits: Tensor, uniforms: Tensor, temperature: float | Tensor = 1.0, top_k: int | Tensor | None = 0,
+                  top_p: float | Tensor | None = 1.0, min_p: float | Tensor | None = 0.0, row_mask: Tensor | None = None,
+                  pad_token_id: int = 0) -> tuple[Tensor, Tensor]:
+    """Draws one token per row of `logits` (`[..., V]`, bf16, fp16 or fp32, rows at any stride) from
+    `softmax(logits / temperature)` after top-k, top-p and min-p, with the given `uniforms` (`[...]`, numbers in [0, 1), fp32
+    or fp64).  Returns int64 ids and their fp32 log-probs under that filtered, renormalised distribution, both `[...]`: what
+    the reference's trainers get back from the sampler as `sampling_per_token_logps` (trl/trainer/grpo_trainer.py:2579-2623).
+
+    A row's tokens are ordered by logit, ties by index.  `top_k` > 0 keeps the first k of them, `top_p` < 1 those before which
+    less than `top_p` of the mass lies that top-k kept (one at least), `min_p` > 0 those of at least `min_p` times the largest
+    probability; `None`, and a `top_k` of 0 or less, switches a filter off.  A temperature of 0 takes the first token (log-prob 0).
+    The token is the first one in index order whose cumulative probability exceeds the uniform number.  All sums are held in 64
+    bits: a row's token depends on its logits, settings and number alone, not on the batch.  Each setting is a number, or a
+    tensor `[...]` with a value for each row.
+
+    Rows whose `row_mask` is 0 (finished sequences) are not read and return `pad_token_id` and 0.  A row without a distribution
+    (NaN or +inf, all -inf, a bad setting of its own) returns -1 and NaN, and `check_device_errors()` raises ValueError.
+    The log-probs carry no gradient: `filtered_logps` computes them with one."""
+    shape = logits.shape[:-1]
+    if uniforms.shape != shape:
+        raise ValueError(f"uniforms of shape {tuple(uniforms.shape)} for logits of shape {tuple(logits.shape)}")
+    ids, logps = ops.sample_tokens(_as_3d(logits), uniforms, *_settings(shape, temperature, top_k, top_p, min_p),
+                                   _byte_mask(row_mask, shape), pad_token_id)
+    return ids.view(shape), logps.view(shape)
+
+
+def filtered_logps(logits: Tensor, index: Tensor, temperature: float | Tensor = 1.0, top_k: int | Tensor | None = 0,
+                   top_p: float | Tensor | None = 1.0, min_p: float | Tensor | None = 0.0,
+                   row_mask: Tensor | None = None) -> Tensor:
+    """fp32 log-probs `[...]` of the tokens `index` (`[...]`, int64) under the distribution that `sample_tokens` draws from with
+    the same settings, differentiable w.r.t. `logits` (`[..., V]`).  `selective_log_softmax` scores under the whole
+    vocabulary: with top-k, top-p or min-p in generation, the ratio of the two would compare distributions of different support.
+
+    A token that the filters take away has log-prob -inf and its row no gradient.  The gradient takes the kept set as given:
+    `d logits[v] = g / temperature * (1[v = index] - kept_v p_v)`.  Rows whose `row_mask` is 0 are not read; they return 0 and
+    have no gradient.  Ids outside [0, V) give NaN and are reported by `check_device_errors()`, as are rows without a distribution."""
+    shape = logits.shape[:-1]
+    if index.shape != shape:
+        raise ValueError(f"index of shape {tuple(index.shape)} for logits of shape {tuple(logits.shape)}")
+    if index.dtype != torch.int64:
+        index = index.long()
+    logps, _, _ = ops.filtered_logps_fwd(_as_3d(logits), index, *_settings(shape, temperature, top_k, top_p, min_p),
+                                         _byte_mask(row_mask, shape))
+    return logps.view(shape)
 
 
 # ----------------------------------------------------------------------------------------------
