@@ -483,6 +483,47 @@ int trlk_filtered_logps_bwd(const void* d_logits, int dtype, int64_t n_seq, int6
                             const float* d_temperature, const float* d_state, const void* d_block_max, const float* d_g_logp,
                             void* d_dlogits, trlk_stream_t stream);
 
+/* ---------------------------------------------------------------------------------------
+ * K9  one AdamW step over many tensors (the optimiser of the trainers' training loop: `optim`, learning_rate, adam_beta1,
+ * adam_beta2, adam_epsilon, weight_decay and max_grad_norm of the training arguments), the global gradient norm clipped first:
+ *   clip = min(1, max_grad_norm / (norm + 1e-6)), norm over all tensors' gradients (64-bit sums)
+ *   t += 1;  m = beta1 m + (1 - beta1) clip g;  v = beta2 v + (1 - beta2) (clip g)^2
+ *   p = p (1 - lr weight_decay) - lr / (1 - beta1^t) * m / (sqrt(v) / sqrt(1 - beta2^t) + eps)
+ * in fp32, p rounded once to its type.  The tables are HOST memory, read before the call returns.  All operands of a tensor have
+ * `numel` entries in the same order; no two tensors share one.  d_step (fp32, device) counts the tensor's steps.
+ *   state_bits 32: d_exp_avg, d_exp_avg_sq fp32
+ *   state_bits 8:  codes of one byte in blocks of 256 entries, with fp32 scales (powers of two), one per block
+ *                  exp_avg: sign, 4 bits of exponent (bias 7), 3 of mantissa (e4m3);  exp_avg_sq: 4 bits of exponent (bias 7), 4
+ *                  of mantissa.  Rounded up or down by 16 random bits, a hash of (seed, t, the tensor's place, entry).
+ * max_grad_norm <= 0: no clipping.  d_out_norm (fp32, may be NULL) takes the norm.  A group's d_lr (fp32, device), if not NULL,
+ * is read in place of lr.  d_workspace: trlk_adamw_workspace_bytes(tensors, n_tensors) bytes, 16-byte aligned.
+ */
+typedef struct {
+    void* d_param;
+    const void* d_grad;
+    void* d_exp_avg;
+    void* d_exp_avg_sq;
+    float* d_exp_avg_scale;
+    float* d_exp_avg_sq_scale;
+    float* d_step;
+    int64_t numel;
+    int32_t dtype;      /* trlk_dtype of param and grad */
+    int32_t state_bits; /* 32 or 8 */
+    int32_t group;
+    int32_t reserved;
+} trlk_adamw_tensor;
+typedef struct {
+    double lr, beta1, beta2, eps, weight_decay;
+    const float* d_lr;
+} trlk_adamw_group;
+size_t trlk_adamw_workspace_bytes(const trlk_adamw_tensor* tensors, int32_t n_tensors);
+int trlk_adamw_step(const trlk_adamw_tensor* tensors, int32_t n_tensors, const trlk_adamw_group* groups, int32_t n_groups,
+                    double max_grad_norm, uint32_t seed, float* d_out_norm, void* d_workspace, size_t workspace_bytes,
+                    trlk_stream_t stream);
+/* The bf16 values (exact) of `n` 8-bit codes with their scales; has_sign: exp_avg's format, else exp_avg_sq's. */
+int trlk_adamw_state_values(const uint8_t* d_codes, const float* d_scales, int64_t n, int32_t has_sign, void* d_out_bf16,
+                            trlk_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -9,7 +9,7 @@ from __future__ import annotations
 
 import ctypes
 import os
-from ctypes import c_char_p, c_double, c_float, c_int32, c_int64, c_size_t, c_void_p
+from ctypes import c_char_p, c_double, c_float, c_int32, c_int64, c_size_t, c_uint32, c_void_p
 
 import torch  # (loads the HIP runtime the library binds to)
 
@@ -135,6 +135,10 @@ SIGNATURES = {
         [c_void_p, c_void_p, c_int32, c_int64, c_int64, c_int64, c_int64, c_int64, c_int64, c_int64, c_void_p, c_void_p,
          c_size_t, c_void_p],
     ),
+    "trlk_adamw_workspace_bytes": (c_size_t, [c_void_p, c_int32]),
+    "trlk_adamw_step": (
+        c_int32, [c_void_p, c_int32, c_void_p, c_int32, c_double, c_uint32, c_void_p, c_void_p, c_size_t, c_void_p]),
+    "trlk_adamw_state_values": (c_int32, [c_void_p, c_void_p, c_int64, c_int32, c_void_p, c_void_p]),
     "trlk_token_filter_max_vocab": (c_int64, []),
     "trlk_token_filter_workspace_bytes": (c_size_t, [c_int64, c_int64, c_int32]),
     "trlk_token_filter_blocks": (c_int64, [c_int64]),

@@ -8,6 +8,7 @@
 // current stream of the tensors' device to the library.  GPU tensors only: other devices have no kernel registered.
 #include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
 #include <ATen/ops/empty.h>
+#include <ATen/ops/empty_strided.h>
 #include <ATen/ops/zeros.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/core/InferenceMode.h>
@@ -17,6 +18,7 @@
 #include <torch/library.h>
 #include <torch/python.h>
 
+#include <algorithm>
 #include <cstdlib>
 #include <map>
 #include <mutex>
@@ -688,6 +690,116 @@ Tensor3 filtered_logps_fwd_autograd(const Tensor& logits, const Tensor& index, d
     static const auto op = handle<decltype(filtered_logps_fwd)>("trl_amd::filtered_logps_fwd");
     return op.call(logits, index, temperature, top_k, top_p, min_p, temperatures, top_ks, top_ps, min_ps, row_mask);
 }
+
+// ---- AdamW ------------------------------------------------------------------------------------------------------------
+constexpr int64_t kStateBlock = 256;  // entries of 8-bit moments that share a scale
+
+// whether two of the pointers are the same (the usual order is ascending or descending, and tells it at once)
+bool twice(std::vector<const void*> p) {
+    if (!std::is_sorted(p.begin(), p.end())) std::sort(p.begin(), p.end());
+    return std::adjacent_find(p.begin(), p.end()) != p.end();
+}
+
+Tensor adamw_step_(at::TensorList params, at::TensorList grads_, at::TensorList exp_avgs, at::TensorList exp_avg_sqs,
+                   at::TensorList steps, at::TensorList exp_avg_scales, at::TensorList exp_avg_sq_scales, at::IntArrayRef group_of,
+                   at::ArrayRef<double> hyper, at::TensorList lrs, double max_grad_norm, int64_t seed) {
+    const size_t n = params.size(), n_groups = hyper.size() / 5;
+    TORCH_CHECK_VALUE(grads_.size() == n && exp_avgs.size() == n && exp_avg_sqs.size() == n && steps.size() == n &&
+                          (group_of.empty() || group_of.size() == n) && (exp_avg_scales.empty() || exp_avg_scales.size() == n) &&
+                          exp_avg_scales.size() == exp_avg_sq_scales.size(),
+                      "adamw_step_: the lists differ in length");
+    TORCH_CHECK_VALUE(hyper.size() == 5 * n_groups && n_groups > 0 && (lrs.empty() || lrs.size() == n_groups),
+                      "adamw_step_: five numbers and one learning rate for each group are expected");
+    TORCH_CHECK_VALUE(n > 0, "adamw_step_: no parameters");
+    const at::Device device = params[0].device();
+    const c10::DeviceGuard guard(device);
+    std::vector<trlk_adamw_tensor> table(n);
+    std::vector<trlk_adamw_group> groups(n_groups);
+    std::vector<Tensor> copies;  // of gradients in another order than their parameters
+    std::vector<const void*> p_ptrs(n), step_ptrs(n);
+    const auto here = [&](const Tensor& t, size_t i, const char* what) {
+        TORCH_CHECK(t.device() == device, "adamw_step_: ", what, " ", i, " is on ", t.device(), ", the first parameter on ", device);
+    };
+    for (size_t g = 0; g < n_groups; ++g) {
+        groups[g] = {hyper[5 * g], hyper[5 * g + 1], hyper[5 * g + 2], hyper[5 * g + 3], hyper[5 * g + 4], nullptr};
+        if (lrs.empty() || lrs[g].numel() == 0) continue;
+        here(lrs[g], g, "learning rate");
+        TORCH_CHECK_VALUE(lrs[g].numel() == 1 && lrs[g].scalar_type() == at::kFloat, "adamw_step_: a learning rate on the GPU is one fp32 number");
+        groups[g].d_lr = static_cast<const float*>(lrs[g].const_data_ptr());
+    }
+    for (size_t i = 0; i < n; ++i) {
+        const Tensor &p = params[i], &m = exp_avgs[i], &v = exp_avg_sqs[i], &step = steps[i];
+        here(p, i, "parameter");
+        here(grads_[i], i, "gradient");
+        here(m, i, "exp_avg");
+        here(v, i, "exp_avg_sq");
+        here(step, i, "step");
+        const bool eight = m.scalar_type() == at::kFloat8_e4m3fn;
+        TORCH_CHECK_VALUE(grads_[i].sizes() == p.sizes() && m.sizes() == p.sizes() && v.sizes() == p.sizes(),
+                          "adamw_step_: parameter ", i, " of shape ", p.sizes(), " and its gradient or moments differ in shape");
+        TORCH_CHECK_TYPE(grads_[i].scalar_type() == p.scalar_type(), "adamw_step_: parameter ", i, " is ", p.scalar_type(), ", its gradient ",
+                         grads_[i].scalar_type());
+        TORCH_CHECK_TYPE(eight ? v.scalar_type() == at::kByte : m.scalar_type() == at::kFloat && v.scalar_type() == at::kFloat,
+                         "adamw_step_: moments are fp32 both, or float8_e4m3fn and uint8");
+        TORCH_CHECK_VALUE(step.numel() == 1 && step.scalar_type() == at::kFloat, "adamw_step_: a step is one fp32 number");
+        const bool plain = p.is_contiguous() && m.is_contiguous() && v.is_contiguous();
+        TORCH_CHECK_VALUE(plain || (p.is_non_overlapping_and_dense() && m.strides() == p.strides() && v.strides() == p.strides()),
+                          "adamw_step_: parameter ", i, " has gaps or its moments another order of entries");
+        Tensor g = grads_[i];
+        if (!(plain && g.is_contiguous()) && g.strides() != p.strides()) {
+            g = at::empty_strided(p.sizes(), p.strides(), p.options()).copy_(g);
+            copies.push_back(g);
+        }
+        trlk_adamw_tensor& t = table[i];
+        t = {};
+        t.numel = p.numel();
+        t.d_param = p.mutable_data_ptr();
+        t.d_grad = g.const_data_ptr();
+        t.d_exp_avg = m.mutable_data_ptr();
+        t.d_exp_avg_sq = v.mutable_data_ptr();
+        t.d_step = out(step);
+        t.dtype = dtype_code(p);
+        t.state_bits = eight ? 8 : 32;
+        t.group = group_of.empty() ? 0 : int32_t(group_of[i]);
+        if (eight) {
+            TORCH_CHECK_VALUE(!exp_avg_scales.empty(), "adamw_step_: 8-bit moments need their scales");
+            const int64_t blocks = (t.numel + kStateBlock - 1) / kStateBlock;
+            for (const Tensor* s : {&exp_avg_scales[i], &exp_avg_sq_scales[i]}) {
+                here(*s, i, "scales");
+                TORCH_CHECK_VALUE(s->numel() == blocks && s->scalar_type() == at::kFloat && s->is_contiguous(), "adamw_step_: parameter ", i,
+                                  " needs ", blocks, " contiguous fp32 scales for each moment");
+            }
+            t.d_exp_avg_scale = out(exp_avg_scales[i]);
+            t.d_exp_avg_sq_scale = out(exp_avg_sq_scales[i]);
+        }
+        p_ptrs[i] = t.numel ? t.d_param : static_cast<const void*>(&t);
+        step_ptrs[i] = t.d_step;
+    }
+    TORCH_CHECK_VALUE(!twice(p_ptrs) && !twice(step_ptrs), "adamw_step_: a parameter or a step is listed twice");
+    const Tensor norm = at::empty(max_grad_norm < 0 ? at::IntArrayRef({0}) : at::IntArrayRef(), params[0].options().dtype(at::kFloat));
+    const size_t ws_bytes = trlk_adamw_workspace_bytes(table.data(), int32_t(n));
+    const Tensor ws = bytes(params[0], ws_bytes);
+    check(trlk_adamw_step(table.data(), int32_t(n), groups.data(), int32_t(n_groups), max_grad_norm, uint32_t(seed),
+                          max_grad_norm < 0 ? nullptr : out(norm), ws.mutable_data_ptr(), ws_bytes, stream_of(params[0])));
+    for (at::TensorList list : {params, exp_avgs, exp_avg_sqs, steps, exp_avg_scales, exp_avg_sq_scales})
+        for (const Tensor& t : list)
+            if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();  // (graphs that saved one of them learn that it has changed)
+    return norm;
+}
+
+Tensor adamw_state_values(const Tensor& codes, const Tensor& scales) {
+    const bool has_sign = codes.scalar_type() == at::kFloat8_e4m3fn;
+    TORCH_CHECK_TYPE(has_sign || codes.scalar_type() == at::kByte, "adamw_state_values: codes are float8_e4m3fn (exp_avg) or uint8 (exp_avg_sq)");
+    TORCH_CHECK_VALUE(codes.is_non_overlapping_and_dense() && scales.is_contiguous() && scales.scalar_type() == at::kFloat &&
+                          scales.numel() == (codes.numel() + kStateBlock - 1) / kStateBlock,
+                      "adamw_state_values: one contiguous fp32 scale for each ", kStateBlock, " codes is expected");
+    TORCH_CHECK(codes.device() == scales.device(), "adamw_state_values: codes are on ", codes.device(), ", scales on ", scales.device());
+    const c10::DeviceGuard guard(codes.device());
+    const Tensor values = at::empty_strided(codes.sizes(), codes.strides(), codes.options().dtype(at::kBFloat16));
+    check(trlk_adamw_state_values(static_cast<const uint8_t*>(codes.const_data_ptr()), fptr(scales), codes.numel(), has_sign ? 1 : 0,
+                                  values.mutable_data_ptr(), stream_of(codes)));
+    return values;
+}
 }  // namespace
 
 TORCH_LIBRARY_FRAGMENT(trl_amd, m) {
@@ -725,6 +837,10 @@ TORCH_LIBRARY_FRAGMENT(trl_amd, m) {
           "Tensor? temperatures, Tensor? top_ks, Tensor? top_ps, Tensor? min_ps, Tensor? row_mask) -> (Tensor, Tensor, Tensor)");
     m.def("filtered_logps_bwd(Tensor logits, Tensor index, float temperature, Tensor? temperatures, Tensor state, Tensor block_max, "
           "Tensor g_logp) -> Tensor");
+    m.def("adamw_step_(Tensor(a!)[] params, Tensor[] grads, Tensor(b!)[] exp_avgs, Tensor(c!)[] exp_avg_sqs, Tensor(d!)[] steps, "
+          "Tensor(e!)[] exp_avg_scales, Tensor(f!)[] exp_avg_sq_scales, int[] group_of, float[] hyper, Tensor[] lrs, "
+          "float max_grad_norm, int seed) -> Tensor");
+    m.def("adamw_state_values(Tensor codes, Tensor scales) -> Tensor");
 }
 TORCH_LIBRARY_IMPL(trl_amd, CUDA, m) {
     m.impl("logp_entropy_fwd", logp_entropy_fwd);
@@ -740,6 +856,8 @@ TORCH_LIBRARY_IMPL(trl_amd, CUDA, m) {
     m.impl("sample_tokens", sample_tokens);
     m.impl("filtered_logps_fwd", filtered_logps_fwd);
     m.impl("filtered_logps_bwd", filtered_logps_bwd);
+    m.impl("adamw_step_", adamw_step_);
+    m.impl("adamw_state_values", adamw_state_values);
 }
 TORCH_LIBRARY_IMPL(trl_amd, Autograd, m) {
     m.impl("logp_entropy_fwd", logp_entropy_fwd_autograd);
@@ -749,6 +867,6 @@ TORCH_LIBRARY_IMPL(trl_amd, Autograd, m) {
     m.impl("filtered_logps_fwd", filtered_logps_fwd_autograd);
     for (const char* name : {"logp_entropy_bwd", "grpo_row_scale", "dpo_log_values", "filtered_logps_bwd"})
         m.impl(name, torch::autograd::autogradNotImplementedFallback());
-    // (these hand out a gradient, scale one in place or draw: their results belong to no graph, whatever the logits require)
-    for (const char* name : {"grpo_fused", "scale_unless_one_", "sample_tokens"}) m.impl(name, torch::CppFunction::makeFallthrough());
+    // (these hand out a gradient, scale one in place, draw or step: their results belong to no graph, whatever the operands require)
+    for (const char* name : {"grpo_fused", "scale_unless_one_", "sample_tokens", "adamw_step_", "adamw_state_values"}) m.impl(name, torch::CppFunction::makeFallthrough());
 }

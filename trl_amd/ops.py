@@ -265,6 +265,21 @@ filtered_logps_bwd = _native_op(
 
 
 # --------------------------------------------------------------------------------------------
+# AdamW over many tensors (K9)
+# --------------------------------------------------------------------------------------------
+# Lists with an entry for each parameter (the scales' may be empty; an empty tensor stands for none); `hyper` has lr, beta1,
+# beta2, eps and weight_decay of each group, `lrs` (may be empty) a learning rate on the GPU for each, `group_of` (may be empty) the
+# parameters' groups.  max_grad_norm > 0 clips, 0 only returns the norm (fp32 0-d), less than 0 does neither (an empty tensor).
+adamw_step_ = _native_op(
+    "adamw_step_", lambda params, grads, exp_avgs, exp_avg_sqs, steps, exp_avg_scales, exp_avg_sq_scales, group_of, hyper, lrs,
+    max_grad_norm, seed: torch.empty((0,) if max_grad_norm < 0 else (), dtype=torch.float32, device=params[0].device))
+
+# The bf16 values of 8-bit moments, in the codes' shape.
+adamw_state_values = _native_op(
+    "adamw_state_values", lambda codes, scales: torch.empty_like(codes, dtype=torch.bfloat16))
+
+
+# --------------------------------------------------------------------------------------------
 # group advantages (K2a)
 # --------------------------------------------------------------------------------------------
 _SCALE_MODES = {"group": _lib.SCALE_GROUP, "batch": _lib.SCALE_BATCH, "none": _lib.SCALE_NONE}

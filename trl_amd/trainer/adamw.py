@@ -1,0 +1,127 @@
+"""The optimiser's step of the reference's training loop (`transformers.Trainer` with `optim="adamw_torch"` or an 8-bit AdamW, and
+`max_grad_norm`): one call for all tensors of a model."""
+from __future__ import annotations
+
+import torch
+from torch import Tensor
+
+from .. import ops
+
+__all__ = ["adamw_step_", "adamw_state_values", "AdamW"]
+
+STATE_BLOCK = 256  # entries of 8-bit moments that share a scale
+
+
+@torch.no_grad()
+def adamw_step_(params: list[Tensor], grads: list[Tensor], exp_avgs: list[Tensor], exp_avg_sqs: list[Tensor], steps: list[Tensor], *,
+                lr: float | Tensor = 1e-3, betas: tuple[float, float] = (0.9, 0.999), eps: float = 1e-8, weight_decay: float = 0.01,
+                max_grad_norm: float | None = None, exp_avg_scales: list[Tensor] | None = None,
+                exp_avg_sq_scales: list[Tensor] | None = None, seed: int = 0) -> Tensor | None:
+    """One AdamW step on `params` in place, each in fp32, bf16 or fp16 with a gradient of its type.  The arithmetic is
+    `torch.optim.AdamW`'s, in fp32; parameters are rounded once to their type.  `steps` (fp32, one number each, on the GPU) count
+    up first.  `lr` may be an fp32 number on the GPU.
+
+    With `max_grad_norm` the gradients count as multiplied by `min(1, max_grad_norm / (norm + 1e-6))`, `norm` the 2-norm of all of
+    them, as `torch.nn.utils.clip_grad_norm_` does (which writes them; they stay as they are here), and the norm is returned (fp32,
+    on the GPU).  0 returns the norm and clips nothing.
+
+    `exp_avgs` and `exp_avg_sqs` are fp32, or float8_e4m3fn and uint8 codes with fp32 scales, one for each 256 entries (`AdamW`
+    makes them; all zeros is a valid start).  Codes round up or down by bits that are a hash of `seed`, the step, the parameter's
+    place in the list and the entry: the same call gives the same state."""
+    on_gpu = isinstance(lr, Tensor) and lr.is_cuda
+    norm = ops.adamw_step_(params, grads, exp_avgs, exp_avg_sqs, steps, exp_avg_scales or [], exp_avg_sq_scales or [], [],
+                           [0.0 if on_gpu else float(lr), float(betas[0]), float(betas[1]), float(eps), float(weight_decay)],
+                           [lr] if on_gpu else [], -1.0 if max_grad_norm is None else _clip(max_grad_norm), seed & 0xFFFFFFFF)
+    return None if max_grad_norm is None else norm
+
+
+def _clip(max_grad_norm: float) -> float:
+    if not max_grad_norm >= 0:
+        raise ValueError(f"max_grad_norm must not be negative, got {max_grad_norm}")
+    return float(max_grad_norm)
+
+
+def adamw_state_values(codes: Tensor, scales: Tensor) -> Tensor:
+    """The values of 8-bit moments, exact in bf16, in the shape of `codes`."""
+    return ops.adamw_state_values(codes, scales)
+
+
+class AdamW(torch.optim.Optimizer):
+    """AdamW whose step is one call for all parameter groups (`adamw_step_`), for GPU parameters in fp32, bf16 or fp16.
+
+    `state_bits=8` holds both moments of every parameter of `min_8bit_size` entries or more in 8 bits, 2.03 bytes per entry instead
+    of 8.  With `max_grad_norm` the step clips the norm over all groups, without a pass that writes the gradients, and leaves it in
+    `grad_norm` (fp32, on the GPU); `transformers.Trainer` then runs with `max_grad_norm=0`.  Step counters live on the GPU and a
+    group's `lr` may: a step can be captured into a graph.  Parameters without a gradient are left alone."""
+
+    def __init__(self, params, lr: float | Tensor = 1e-3, betas: tuple[float, float] = (0.9, 0.999), eps: float = 1e-8,
+                 weight_decay: float = 0.01, *, state_bits: int = 32, min_8bit_size: int = 4096, max_grad_norm: float | None = None,
+                 seed: int = 0):
+        if state_bits not in (8, 32):
+            raise ValueError(f"state_bits must be 8 or 32, got {state_bits}")
+        if not 0.0 <= float(lr) or not 0.0 <= eps or not 0.0 <= weight_decay:
+            raise ValueError(f"lr, eps and weight_decay must not be negative, got {lr}, {eps}, {weight_decay}")
+        if not 0.0 <= betas[0] < 1.0 or not 0.0 <= betas[1] < 1.0:
+            raise ValueError(f"betas must be in [0, 1), got {betas}")
+        self.max_grad_norm = None if max_grad_norm is None else _clip(max_grad_norm)
+        self.seed, self.grad_norm = int(seed), None
+        super().__init__(params, dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay, state_bits=state_bits,
+                                      min_8bit_size=min_8bit_size))
+
+    def _state_of(self, p: Tensor, group: dict) -> dict:
+        state = self.state[p]
+        if not state:
+            state["step"] = torch.zeros((), dtype=torch.float32, device=p.device)
+            if group["state_bits"] == 8 and p.numel() >= group["min_8bit_size"]:
+                blocks = -(-p.numel() // STATE_BLOCK)
+                state["exp_avg"] = torch.zeros_like(p, dtype=torch.uint8, memory_format=torch.preserve_format).view(torch.float8_e4m3fn)
+                state["exp_avg_sq"] = torch.zeros_like(p, dtype=torch.uint8, memory_format=torch.preserve_format)
+                state["exp_avg_scale"] = torch.ones(blocks, dtype=torch.float32, device=p.device)
+                state["exp_avg_sq_scale"] = torch.ones(blocks, dtype=torch.float32, device=p.device)
+            else:
+                state["exp_avg"] = torch.zeros_like(p, dtype=torch.float32, memory_format=torch.preserve_format)
+                state["exp_avg_sq"] = torch.zeros_like(p, dtype=torch.float32, memory_format=torch.preserve_format)
+        return state
+
+    @torch.no_grad()
+    def step(self, closure=None):
+        loss = None
+        if closure is not None:
+            with torch.enable_grad():
+                loss = closure()
+        params, grads, states, group_of, hyper, lrs = [], [], [], [], [], []
+        for i, group in enumerate(self.param_groups):
+            lr = group["lr"]
+            on_gpu = isinstance(lr, Tensor) and lr.is_cuda
+            hyper += [0.0 if on_gpu else float(lr), *map(float, group["betas"]), float(group["eps"]), float(group["weight_decay"])]
+            lrs.append(lr if on_gpu else None)
+            for p in group["params"]:
+                if p.grad is None:
+                    continue
+                if p.grad.is_sparse:
+                    raise RuntimeError("AdamW does not take sparse gradients")
+                if not p.is_cuda:
+                    raise RuntimeError("AdamW steps GPU parameters only")
+                params.append(p)
+                grads.append(p.grad)
+                states.append(self._state_of(p, group))
+                group_of.append(i)
+        if not params:
+            return loss
+        none = params[0].new_empty(0, dtype=torch.float32)
+        scales = [[s.get(k, none) for s in states] for k in ("exp_avg_scale", "exp_avg_sq_scale")]
+        norm = ops.adamw_step_(params, grads, [s["exp_avg"] for s in states], [s["exp_avg_sq"] for s in states],
+                               [s["step"] for s in states], *scales, group_of, hyper,
+                               [none if lr is None else lr for lr in lrs] if any(lr is not None for lr in lrs) else [],
+                               -1.0 if self.max_grad_norm is None else self.max_grad_norm, self.seed & 0xFFFFFFFF)
+        self.grad_norm = None if self.max_grad_norm is None else norm
+        return loss
+
+    def load_state_dict(self, state_dict: dict) -> None:
+        """As the base class, except that the moments keep their own types (it would cast them to the parameters')."""
+        super().load_state_dict(state_dict)
+        ids = [i for g in state_dict["param_groups"] for i in g["params"]]
+        params = [p for g in self.param_groups for p in g["params"]]
+        for i, p in zip(ids, params):
+            if i in state_dict["state"]:
+                self.state[p] = {k: v.to(device=p.device, copy=True) if torch.is_tensor(v) else v for k, v in state_dict["state"][i].items()}
