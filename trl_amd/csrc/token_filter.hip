@@ -31,6 +31,7 @@ constexpr int kList = 2048;                  // blocks over the bound that are l
 constexpr int64_t kMaxVocab = int64_t(1) << 22;
 
 typedef unsigned long long u64;
+#define TRLK_INLINE __attribute__((always_inline))
 typedef u32x4 u32x4_u __attribute__((aligned(2)));  // a 16-byte vector at any element alignment
 
 // ---- weights ---------------------------------------------------------------------------------------------------------
@@ -147,12 +148,11 @@ struct ScanArgs {
     void* block_max;    // [rows, chunks * kBlocksPerChunk] in the logits' type, or null
 };
 
-// The VEC = kChunk / (64 * EPV) vectors of a lane: vector i holds the logits (i * 64 + lane) * EPV on of the chunk.  What lies behind
-// the row's end is -inf.
+// NV vectors of a lane: vector i holds the logits (i * 64 + lane) * EPV on of those at p.  What lies behind the n there are is -inf.
 template <int DT, int NV>
-__device__ __forceinline__ void load_chunk(const typename Elem<DT>::type* p, int n, int lane, float (&x)[NV * Elem<DT>::EPV]) {
+__device__ __forceinline__ void load_vectors(const typename Elem<DT>::type* p, int64_t n, int lane, float (&x)[NV * Elem<DT>::EPV]) {
     constexpr int EPV = Elem<DT>::EPV;
-    if (n == kChunk) {
+    if (n >= NV * kWave * EPV) {
         u32x4 q[NV];
 #pragma unroll
         for (int i = 0; i < NV; ++i) q[i] = *reinterpret_cast<const u32x4_u*>(p + (i * kWave + lane) * EPV);
@@ -184,9 +184,8 @@ __global__ __launch_bounds__(kScanThreads) void filter_scan_kernel(ScanArgs a) {
     const int chunk = int(unit - row * a.chunks);
     if (a.row_mask && a.row_mask[row] == 0) return;
     const T* p = a.x.row<DT>(row) + int64_t(chunk) * kChunk;
-    const int64_t left = a.x.vocab - int64_t(chunk) * kChunk;
     float x[NV * EPV];
-    load_chunk<DT, NV>(p, left < kChunk ? int(left) : kChunk, lane, x);
+    load_vectors<DT, NV>(p, a.x.vocab - int64_t(chunk) * kChunk, lane, x);
     float m = -INFINITY, mine = 0.f;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
@@ -225,7 +224,7 @@ struct SelectArgs {
     int32_t chunks, fix;
     Filters f;
     const uint8_t* row_mask;
-    const double* chunk_sum;
+    double* chunk_sum;  // (a row with very many candidates puts the kept weights of its chunks there)
     const float* chunk_max;
     const void* block_max;
     const void* uniform;  // sample: fp32 or fp64 [rows]
@@ -238,17 +237,21 @@ struct SelectArgs {
     int32_t* error_flag;
 };
 
+struct alignas(16) Candidate {
+    u64 order;  // key above, ~index below: larger is earlier
+    u64 weight;
+};
 struct SelectShared {
     u64 bins[kBins];
-    u64 weight[kCandidates];
-    uint32_t key[kCandidates], index[kCandidates];
+    Candidate cand[kCandidates];
     uint16_t list[kList];
     u64 scan[kSelWaves];
     double scan_f[kSelWaves];
     float wave_f[kSelWaves];
+    int hit[kSelWaves], tail[kSelWaves];
+    double prefix[kSelWaves];
     u64 before;
-    double prefix;
-    uint32_t bin, n_list, n_cand, min_key, lo, hi;
+    uint32_t bin, n_list, n_cand, min_key, low_key, border, border_index;
 };
 
 template <typename V>
@@ -260,11 +263,14 @@ __device__ __forceinline__ V wave_inclusive(V v, int lane) {
     }
     return v;
 }
-// Sum over the threads before this one; `total` over all.  Contains two barriers.
+// Sums over the threads before this one (returned) and up to it (`upto`), and over all.  What one thread's `upto` is, is the next
+// one's exclusive sum to the last bit.  Contains two barriers.
 template <typename V>
-__device__ __forceinline__ V block_exclusive(V v, V* scratch, V& total) {
+__device__ __forceinline__ V block_scan(V v, V* scratch, V& upto, V& total) {
     const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
     const V inc = wave_inclusive(v, lane);
+    V exc = __shfl_up(inc, 1);
+    if (lane == 0) exc = 0;
     __syncthreads();
     if (lane == kWave - 1) scratch[wave] = inc;
     __syncthreads();
@@ -275,7 +281,8 @@ __device__ __forceinline__ V block_exclusive(V v, V* scratch, V& total) {
         all += scratch[w];
     }
     total = all;
-    return base + (inc - v);
+    upto = base + inc;
+    return base + exc;
 }
 __device__ __forceinline__ u64 block_total(u64 v, u64* scratch) {
 #pragma unroll
@@ -289,41 +296,53 @@ __device__ __forceinline__ u64 block_total(u64 v, u64* scratch) {
     return r;
 }
 
+// The bin up to which the values of bins [0, n) and `before` reach `target` first, and in `before` what lies before it; false if
+// all of them do not.  The bins are complete and the barrier behind them passed; s.bin is ~0.  Contains three barriers.
+__device__ __forceinline__ bool crossing(SelectShared& s, int n, u64 target, uint32_t& bin, u64& before) {
+    u64 v[4], sum = 0, upto, total;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        const int i = 4 * threadIdx.x + j;
+        v[j] = i < n ? s.bins[i] : 0;
+        sum += v[j];
+    }
+    u64 at = before + block_scan(sum, s.scan, upto, total);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        if (at < target && at + v[j] >= target) {  // (one bin of one thread)
+            s.bin = 4 * threadIdx.x + j;
+            s.before = at;
+        }
+        at += v[j];
+    }
+    __syncthreads();
+    bin = s.bin;
+    if (bin == ~0u) return false;
+    before = s.before;
+    return true;
+}
+// all bins 0 and no crossing yet, behind a barrier
+__device__ __forceinline__ void clear_bins(SelectShared& s, int n) {
+    for (int i = threadIdx.x; i < n; i += kSelThreads) s.bins[i] = 0;
+    __syncthreads();
+    if (threadIdx.x == 0) s.bin = ~0u;  // (everyone has read the last one; the next is written two barriers from here)
+}
+
 // The smallest position in [lo, hi] up to which `before` and the values reach `target`, and in `before` what lies before it.
 // `each(f)` calls f(position, value) for this thread's share of the items.  False if all of them do not reach it.
 template <typename Each>
-__device__ bool descend(SelectShared& s, Each each, uint32_t lo, uint32_t hi, u64 target, uint32_t& position, u64& before) {
+__device__ __forceinline__ bool descend(SelectShared& s, Each each, uint32_t lo, uint32_t hi, u64 target, uint32_t& position, u64& before) {
     for (;;) {
         const uint32_t span = hi - lo;
         const int bits = span ? 32 - __builtin_clz(span) : 0, shift = bits > kBinBits ? bits - kBinBits : 0;
         const int n = int(span >> shift) + 1;
-        for (int i = threadIdx.x; i < n; i += kSelThreads) s.bins[i] = 0;
-        __syncthreads();
-        if (threadIdx.x == 0) s.bin = ~0u;  // (everyone has read the last step's; the next is written two barriers from here)
+        clear_bins(s, n);
         each([&](uint32_t at, u64 value) {
             if (at >= lo && at <= hi && value) atomicAdd(&s.bins[(at - lo) >> shift], value);
         });
         __syncthreads();
-        u64 v[4], sum = 0, total;
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const int i = 4 * threadIdx.x + j;
-            v[j] = i < n ? s.bins[i] : 0;
-            sum += v[j];
-        }
-        u64 at = before + block_exclusive(sum, s.scan, total);
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            if (at < target && at + v[j] >= target) {  // (one bin of one thread)
-                s.bin = 4 * threadIdx.x + j;
-                s.before = at;
-            }
-            at += v[j];
-        }
-        __syncthreads();
-        const uint32_t bin = s.bin;
-        if (bin == ~0u) return false;
-        before = s.before;
+        uint32_t bin;
+        if (!crossing(s, n, target, bin, before)) return false;
         lo += bin << shift;
         position = lo;
         if (shift == 0) return true;
@@ -332,325 +351,650 @@ __device__ bool descend(SelectShared& s, Each each, uint32_t lo, uint32_t hi, u6
     }
 }
 
+// Distance from the maximum in bins of 1/128 of itself: 0 for less than 2^-8, then 128 bins for each power of two.  Monotone, and it
+// depends neither on where a row's logits lie nor on the temperature.
+__device__ __forceinline__ int distance_bin(float m, float x) {
+    const int b = int(__float_as_uint(m - x) >> 16) - (119 << 7);
+    return b > 0 ? b : 0;
+}
+constexpr int kEveryBin = 1 << 30;
+
+// `owner` of the smallest thread number, and if there is none of the largest with `some`: its number, the same for all threads
+__device__ __forceinline__ int first_thread(SelectShared& s, bool owner, bool some) {
+    const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
+    const u64 a = __ballot(owner), b = __ballot(some);
+    if (lane == 0) {
+        s.hit[wave] = a ? wave * kWave + __builtin_ctzll(a) : -1;
+        s.tail[wave] = b ? wave * kWave + 63 - __builtin_clzll(b) : -1;
+    }
+    __syncthreads();
+    int r = -1;
+#pragma unroll
+    for (int w = kSelWaves - 1; w >= 0; --w)
+        if (s.hit[w] >= 0) r = s.hit[w];
+    if (r >= 0) return r;
+#pragma unroll
+    for (int w = 0; w < kSelWaves; ++w)
+        if (s.tail[w] >= 0) r = s.tail[w];
+    return r;
+}
+
 template <int DT, bool SCORE>
-__global__ __launch_bounds__(kSelThreads) void filter_select_kernel(SelectArgs a) {
+__global__ __launch_bounds__(kSelThreads, 4) void filter_select_kernel(SelectArgs a) {
     typedef typename Elem<DT>::type T;
     typedef Key<DT> K;
+    constexpr int EPV = Elem<DT>::EPV, PER = kChunk / kSelThreads;
+    constexpr int NV = kChunk / (kWave * EPV);
+    constexpr int kKeep = sizeof(T) == 4 ? 2 : 1;  // vectors of block maxima that a thread holds: 4096 blocks
     __shared__ SelectShared s;
     const int tid = threadIdx.x, lane = tid & (kWave - 1), wave = tid / kWave;
     const int64_t row = blockIdx.x, V = a.x.vocab;
-    if (a.row_mask && a.row_mask[row] == 0) {
-        if (tid == 0) {
-            if constexpr (SCORE) {
-                a.out_state[row * 4] = INFINITY;
-                a.out_state[row * 4 + 1] = a.out_state[row * 4 + 2] = a.out_state[row * 4 + 3] = 0.f;
-            } else {
-                a.out_ids[row] = a.fill_id;
-            }
-            a.out_logp[row] = 0.f;
+    // what a row without a token, or without a distribution, returns
+    const auto nothing = [&](int64_t id, float logp) TRLK_INLINE {
+        if (tid != 0) return;
+        if constexpr (SCORE) {
+            a.out_state[row * 4] = INFINITY;
+            a.out_state[row * 4 + 1] = a.out_state[row * 4 + 2] = a.out_state[row * 4 + 3] = 0.f;
+        } else {
+            a.out_ids[row] = id;
         }
-        return;
-    }
+        a.out_logp[row] = logp;
+    };
+    if (a.row_mask && a.row_mask[row] == 0) return nothing(a.fill_id, 0.f);
     const RowFilter f = row_filter(a.f, row, V);
+    const bool filtered = f.top_k || f.top_p > 0.0 || f.min_p > 0.0;
+    const bool with_sum = !filtered || (f.top_p > 0.0 && !f.top_k);
     const T* x = a.x.row<DT>(row);
     const float* cmax = a.chunk_max + row * a.chunks;
-    const double* csum = a.chunk_sum + row * a.chunks;
+    double* csum = a.chunk_sum + row * a.chunks;
+    const int n_blocks = a.chunks * kBlocksPerChunk, n_vec = n_blocks / EPV;  // (blocks behind the row's end are -inf)
+    const u32x4* bmax = reinterpret_cast<const u32x4*>(static_cast<const T*>(a.block_max) + row * n_blocks);
 
-    // the row's maximum
+    // block maxima (chunk maxima where there are no others) and the row's maximum
+    u32x4 held[kKeep];
     float m = -INFINITY;
-    for (int i = tid; i < a.chunks; i += kSelThreads) m = max_nan(m, cmax[i]);
-    m = wave_max_nan(m);
-    if (lane == 0) s.wave_f[wave] = m;
-    if (tid == 0) {
-        s.n_list = s.n_cand = 0;
-        s.min_key = ~0u;
-        s.lo = ~0u;
-        s.hi = 0;
-    }
-    __syncthreads();
-    m = s.wave_f[0];
+    if (filtered) {
 #pragma unroll
-    for (int w = 1; w < kSelWaves; ++w) m = max_nan(m, s.wave_f[w]);
+        for (int j = 0; j < kKeep; ++j) {
+            if (tid + j * kSelThreads < n_vec) {
+                held[j] = bmax[tid + j * kSelThreads];
+                float v[EPV];
+                Elem<DT>::unpack(held[j], v);
+#pragma unroll
+                for (int e = 0; e < EPV; ++e) m = max_nan(m, v[e]);
+            }
+        }
+        for (int i = tid + kKeep * kSelThreads; i < n_vec; i += kSelThreads) {
+            float v[EPV];
+            Elem<DT>::unpack(bmax[i], v);
+#pragma unroll
+            for (int e = 0; e < EPV; ++e) m = max_nan(m, v[e]);
+        }
+    } else {
+        for (int i = tid; i < a.chunks; i += kSelThreads) m = max_nan(m, cmax[i]);
+    }
+    const int per = (a.chunks + kSelThreads - 1) / kSelThreads, first = tid * per, last = first + per < a.chunks ? first + per : a.chunks;
+    double sum0 = 0.0, max0 = 0.0;  // this thread's first chunk, loaded beside the maxima
+    if (with_sum && first < last) {
+        sum0 = csum[first];
+        max0 = double(cmax[first]);
+    }
     int64_t token = 0;
     bool token_ok = true;
+    T token_raw = 0;
     if constexpr (SCORE) {
         token = a.index[row];
         token_ok = token >= 0 && token < V;
+        if (token_ok) token_raw = x[token];
         if (!token_ok && tid == 0 && a.error_flag) atomicOr(a.error_flag, TRLK_FLAG_INDEX_OUT_OF_RANGE);
-    }
-    if (!f.ok || !(m < INFINITY) || m == -INFINITY) {  // no distribution
-        if (tid == 0) {
-            if constexpr (SCORE) {
-                a.out_state[row * 4] = INFINITY;
-                a.out_state[row * 4 + 1] = a.out_state[row * 4 + 2] = a.out_state[row * 4 + 3] = 0.f;
-            } else {
-                a.out_ids[row] = -1;
-            }
-            a.out_logp[row] = NAN;
-            if (a.error_flag) atomicOr(a.error_flag, TRLK_FLAG_NO_DISTRIBUTION);
-        }
-        return;
     }
     double u = 0.0;
     if constexpr (!SCORE) {
         u = a.uniform_f64 ? static_cast<const double*>(a.uniform)[row] : double(static_cast<const float*>(a.uniform)[row]);
         u = u > 0.0 ? u : 0.0;  // (and NaN)
     }
+    if (filtered)
+        for (int i = tid; i < kBins; i += kSelThreads) s.bins[i] = 0;
+    m = wave_max_nan(m);
+    if (lane == 0) s.wave_f[wave] = m;
+    if (tid == 0) {
+        s.n_list = s.n_cand = 0;
+        s.min_key = s.low_key = s.bin = ~0u;
+    }
+    __syncthreads();
+    m = s.wave_f[0];
+#pragma unroll
+    for (int w = 1; w < kSelWaves; ++w) m = max_nan(m, s.wave_f[w]);
+    if (!f.ok || !(m < INFINITY) || m == -INFINITY) {
+        if (tid == 0 && a.error_flag) atomicOr(a.error_flag, TRLK_FLAG_NO_DISTRIBUTION);
+        return nothing(-1, NAN);
+    }
     const double c = f.c, ref = double(m), unit = __builtin_amdgcn_ldexp(1.0, a.fix);
-    const auto weight = [&](float v) { return exp2_f64((double(v) - ref) * c); };
-    const auto fixed = [&](double w) { return u64(int64_t(__builtin_rint(w * unit))); };
-
-    // the row's sum of weights, and this thread's chunks' place in it
-    const bool filtered = f.top_k || f.top_p > 0.0 || f.min_p > 0.0;
-    double S = 0.0, mine = 0.0, base = 0.0;
-    const int per = (a.chunks + kSelThreads - 1) / kSelThreads, first = tid * per,
-              last = first + per < a.chunks ? first + per : a.chunks;
-    if (!filtered || (f.top_p > 0.0 && !f.top_k)) {
-        for (int i = first; i < last; ++i) mine += csum[i] * weight(cmax[i]);
-        base = block_exclusive(mine, s.scan_f, S);
-    }
-
-    uint32_t border = 0, border_index = ~0u;  // everything
-    double log2_mass;
-    int64_t id = 0;
-    if (!filtered) {
-        log2_mass = log2(S);
-        if constexpr (!SCORE) {
-            const double target = u * S;
-            double at = base;
-            for (int i = first; i < last; ++i) {
-                const double v = csum[i] * weight(cmax[i]);
-                if (v > 0.0) atomicMax(&s.hi, uint32_t(i));
-                if (at + v > target) {
-                    atomicMin(&s.lo, uint32_t(i));
-                    break;
-                }
-                at += v;
-            }
-            __syncthreads();
-            const int chunk = s.lo != ~0u ? int(s.lo) : int(s.hi);  // (u * S rounded up to the whole sum: the last one)
-            if (chunk >= first && chunk < last) {
-                double before = base;
-                for (int i = first; i < chunk; ++i) before += csum[i] * weight(cmax[i]);
-                s.prefix = before;
-            }
-            __syncthreads();
-            const double prefix = s.prefix;
-            if (tid == 0) {
-                s.lo = ~0u;
-                s.hi = 0;
-            }
-            constexpr int PER = kChunk / kSelThreads;
-            double w[PER], sum = 0.0, all;
-            const int64_t e0 = int64_t(chunk) * kChunk + tid * PER;
-#pragma unroll
-            for (int j = 0; j < PER; ++j) {
-                w[j] = e0 + j < V ? weight(Elem<DT>::load1(x + e0 + j)) : 0.0;
-                sum += w[j];
-            }
-            double run = prefix + block_exclusive(sum, s.scan_f, all);
-#pragma unroll
-            for (int j = 0; j < PER; ++j) {
-                run += w[j];
-                if (w[j] > 0.0) {
-                    atomicMax(&s.hi, uint32_t(e0 + j));
-                    if (run > target) atomicMin(&s.lo, uint32_t(e0 + j));
-                }
-            }
-            __syncthreads();
-            id = s.lo != ~0u ? s.lo : s.hi;
-        }
-    } else {
-        const T* bmax = static_cast<const T*>(a.block_max) + row * a.chunks * kBlocksPerChunk;
-        const int n_blocks = int((V + kBlock - 1) / kBlock);
-        const uint32_t top = K::of_float(m), lowest = K::of_float(-INFINITY) + 1u;
-        // a bound under the border, as a key and as a value
-        uint32_t bound = lowest, at;
-        float x_bound = -INFINITY;
-        u64 before = 0;
-        const u64 mass_target = [&] {  // of top-p without top-k
-            const double t = __builtin_ceil(f.top_p * S * unit);
-            return t < 1.0 ? u64(1) : u64(int64_t(t));
-        }();
-        if (f.top_k) {
-            if (f.top_k <= uint32_t(n_blocks) &&
-                descend(s, [&](auto put) {
-                    for (int i = tid; i < n_blocks; i += kSelThreads) {
-                        const uint32_t k = K::of(bmax[i]);
-                        if (k >= lowest) put(top - k, 1);
-                    }
-                }, 0, top - lowest, f.top_k, at, before))
-                bound = top - at;
-        } else if (f.top_p > 0.0) {
-            // (the sum of rounded weights may be half a unit for each block too large)
-            if (descend(s, [&](auto put) {
-                    for (int i = tid; i < n_blocks; i += kSelThreads) {
-                        const uint32_t k = K::of(bmax[i]);
-                        if (k >= lowest) put(top - k, fixed(weight(K::to_float(k))));
-                    }
-                }, 0, top - lowest, mass_target + n_blocks, at, before)) {
-                bound = top - at;
-            } else {  // all tokens of less than (1 - top_p) / V of the mass together have less than 1 - top_p
-                const double e = (1.0 - f.top_p) * S / double(V) * (1.0 - 1e-9);
-                x_bound = float(ref + log2(e) / c);
-                x_bound -= 1e-6f * fabsf(x_bound) + 1e-30f;
-            }
-        }
-        if (f.min_p > 0.0 && !(f.top_k && f.top_p > 0.0)) {  // (top-p of top-k counts what min-p takes away)
-            float b = float(ref + log2(f.min_p) / c);
-            b -= 1e-6f * fabsf(b) + 1e-30f;
-            x_bound = fmaxf(x_bound, b);
-        }
-        // blocks over the bound
-        const auto block_in = [&](int i) {
-            const uint32_t k = K::of(bmax[i]);
-            return k >= bound && K::to_float(k) >= x_bound;
-        };
-        __syncthreads();
-        for (int i = tid; i < n_blocks; i += kSelThreads) {
-            if (block_in(i)) {
-                const uint32_t to = atomicAdd(&s.n_list, 1u);
-                if (to < kList) s.list[to] = uint16_t(i);
-            }
-        }
-        __syncthreads();
-        const bool listed = s.n_list <= kList;
-        const int n_visit = listed ? int(s.n_list) : n_blocks;
-        // all logits over the bound, a wave to a block: g(valid, key, index), with all lanes of the wave in it
-        const auto stream = [&](auto g) {
-            for (int j = wave; j < n_visit; j += kSelWaves) {
-                const int blk = listed ? int(s.list[j]) : j;
-                if (!listed && !block_in(blk)) continue;
-                const int64_t e = int64_t(blk) * kBlock + lane;
-                const uint32_t k = e < V ? K::of(x[e]) : 0u;
-                g(e < V && k >= bound && K::to_float(k) >= x_bound, k, uint32_t(e));
-            }
-        };
-        uint32_t min_key = ~0u;
-        stream([&](bool in, uint32_t k, uint32_t e) {
-            const u64 vote = __ballot(in);
-            uint32_t to = 0;
-            if (lane == 0 && vote) to = atomicAdd(&s.n_cand, uint32_t(__popcll(vote)));
-            to = __shfl(to, 0) + __popcll(vote & ((u64(1) << lane) - 1));
-            if (in) {
-                const double w = weight(K::to_float(k));
-                if (w >= f.min_p && k < min_key) min_key = k;
-                if (to < kCandidates) {
-                    s.key[to] = k;
-                    s.index[to] = e;
-                    s.weight[to] = fixed(w);
-                }
-            }
-        });
-        if (f.min_p > 0.0 && min_key != ~0u) atomicMin(&s.min_key, min_key);
-        __syncthreads();
-        const int n_cand = int(s.n_cand);
-        const uint32_t kept_from = f.min_p > 0.0 ? s.min_key : 0u;
-        const bool in_lds = n_cand <= kCandidates;
-        // g(key, index, weight) for this thread's candidates
-        const auto each = [&](auto g) {
-            if (in_lds) {
-                for (int i = tid; i < n_cand; i += kSelThreads) g(s.key[i], s.index[i], [&] { return s.weight[i]; });
-            } else {
-                stream([&](bool in, uint32_t k, uint32_t e) {
-                    if (in) g(k, e, [&] { return fixed(weight(K::to_float(k))); });
-                });
-            }
-        };
-        const uint32_t span = top - lowest;
-        u64 ties = ~u64(0);  // how many tokens of the border's value are kept
-        if (f.top_k) {
-            before = 0;
-            if (descend(s, [&](auto put) { each([&](uint32_t k, uint32_t, auto) { put(top - k, 1); }); }, 0, span, f.top_k, at, before)) {
-                border = top - at;
-                ties = f.top_k - before;
-            }
-        }
-        if (f.top_p > 0.0) {
-            u64 target = mass_target;
-            if (f.top_k) {
-                u64 mass = 0;
-                each([&](uint32_t k, uint32_t, auto w) {
-                    if (k > border) mass += w();
-                });
-                mass = block_total(mass, s.scan);
-                if (border) mass += ties * fixed(weight(K::to_float(border)));
-                const double t = __builtin_ceil(f.top_p * double(mass));
-                target = t < 1.0 ? u64(1) : u64(int64_t(t));
-            }
-            before = 0;
-            const uint32_t from = border;
-            if (descend(s, [&](auto put) {
-                    each([&](uint32_t k, uint32_t, auto w) {
-                        if (k >= from) put(top - k, w());
-                    });
-                }, 0, span, target, at, before)) {
-                const uint32_t b = top - at;
-                const u64 w = fixed(weight(K::to_float(b))), n = (target - before + w - 1) / w;
-                ties = b == border && n > ties ? ties : n;
-                border = b;
-            }
-        }
-        if (border) {
-            u64 count = 0;
-            each([&](uint32_t k, uint32_t, auto) { count += k == border; });
-            if (ties < block_total(count, s.scan)) {
-                const uint32_t b = border;
-                before = 0;
-                descend(s, [&](auto put) { each([&](uint32_t k, uint32_t e, auto) { put(e, k == b); }); }, 0, uint32_t(V - 1), ties,
-                        border_index, before);
-            }
-        }
-        if (kept_from > border) {
-            border = kept_from;
-            border_index = ~0u;
-        }
-        if (border < lowest) border = lowest;
-        const auto kept = [&](uint32_t k, uint32_t e) { return k > border || (k == border && e <= border_index); };
-        u64 W = 0;
-        each([&](uint32_t k, uint32_t e, auto w) {
-            if (kept(k, e)) W += w();
-        });
-        W = block_total(W, s.scan);
-        log2_mass = log2(double(W)) - a.fix;
-        if constexpr (!SCORE) {
-            double t = u * double(W);
-            u64 target = t < double(W) ? u64(int64_t(t)) : W - 1;
-            target = target < W ? target : W - 1;
-            before = 0;
-            uint32_t e_at = 0;
-            // (a target of 0 is reached by the first kept token, also by one whose weight is less than a unit)
-            descend(s, [&](auto put) {
-                each([&](uint32_t k, uint32_t e, auto w) {
-                    if (kept(k, e)) put(e, target ? w() : u64(1));
-                });
-            }, 0, uint32_t(V - 1), target ? target + 1 : 1, e_at, before);
-            id = e_at;
-        }
-    }
-
-    if (tid != 0) return;
-    if constexpr (SCORE) {
-        const float bx = filtered ? K::to_float(border) : -INFINITY;
+    const auto weight_at = [&](double v) TRLK_INLINE { return exp2_f64((v - ref) * c); };
+    const auto weight = [&](float v) TRLK_INLINE { return weight_at(double(v)); };
+    const auto fixed = [&](double w) TRLK_INLINE { return u64(int64_t(__builtin_rint(w * unit))); };
+    const auto drawn = [&](int64_t id, float v, double log2_mass) TRLK_INLINE {  // one thread
+        a.out_ids[row] = id;
+        a.out_logp[row] = float(((double(v) - ref) * c - log2_mass) * 0.69314718055994530942);
+    };
+    const auto scored = [&](uint32_t border, uint32_t border_index, double log2_mass) TRLK_INLINE {  // all threads
+        if (tid != 0) return;
         float logp = NAN;
         bool inside = false;
         if (token_ok) {
-            const T raw = x[token];
-            const float v = Elem<DT>::to_float(raw);
-            const uint32_t k = K::of(raw);
+            const float v = Elem<DT>::to_float(token_raw);
+            const uint32_t k = K::of(token_raw);
             inside = v > -INFINITY && (!filtered || k > border || (k == border && uint32_t(token) <= border_index));
             logp = inside ? float(((double(v) - ref) * c - log2_mass) * 0.69314718055994530942) : -INFINITY;
         }
         float* st = a.out_state + row * 4;
-        st[0] = inside ? bx : INFINITY;  // (no gradient reaches a row whose token lies outside)
+        st[0] = !inside ? INFINITY : filtered ? K::to_float(border) : -INFINITY;  // (no gradient reaches a row whose token lies outside)
         st[1] = __uint_as_float(border_index);
         st[2] = m;
         st[3] = float(log2_mass);
         a.out_logp[row] = logp;
+    };
+
+    // the row's sum of weights, and this thread's chunks' place in it
+    double S = 0.0, mine = 0.0, base = 0.0, upto = 0.0;
+    if (with_sum) {
+        if (first < last) mine = sum0 * weight_at(max0);
+        for (int i = first + 1; i < last; ++i) mine += csum[i] * weight(cmax[i]);
+        base = block_scan(mine, s.scan_f, upto, S);
+    }
+    // ---- no filter: the chunk, then the token in it
+    if (!filtered) {
+        if constexpr (SCORE) {
+            return scored(0, ~0u, log2(S));
+        } else {
+            // (u * S can round up to the whole sum, and the last bits of a scan are not monotone: the first thread whose sum passes it,
+            // and that has something, or the last one that has)
+            const double target = u * S;
+            const int owner = first_thread(s, mine > 0.0 && upto > target, mine > 0.0);
+            if (tid == owner) {
+                double at = base, v = sum0 * weight_at(max0);
+                int chunk = first, some = v > 0.0 ? first : -1;
+                double some_at = at;
+                for (;;) {
+                    if (v > 0.0) {
+                        some = chunk;
+                        some_at = at;
+                        if (at + v > target) break;
+                    }
+                    at += v;
+                    if (++chunk >= last) break;
+                    v = csum[chunk] * weight(cmax[chunk]);
+                }
+                s.border = uint32_t(some);
+                s.prefix[0] = some_at;
+            }
+            __syncthreads();
+            const int chunk = int(s.border);
+            const double prefix = s.prefix[0];
+            double w[PER], sum = 0.0, up, all;
+            float v[PER];
+            const int64_t e0 = int64_t(chunk) * kChunk + tid * PER;
+#pragma unroll
+            for (int j = 0; j < PER; ++j) v[j] = e0 + j < V ? Elem<DT>::load1(x + e0 + j) : -INFINITY;
+#pragma unroll
+            for (int j = 0; j < PER; ++j) {
+                w[j] = weight(v[j]);
+                sum += w[j];
+            }
+            double run = prefix + block_scan(sum, s.scan_f, up, all);
+            const int at = first_thread(s, sum > 0.0 && prefix + up > target, sum > 0.0);
+            if (tid == at) {
+                int some = 0;
+                float vs = v[0];
+                bool past = false;
+#pragma unroll
+                for (int j = 0; j < PER; ++j) {
+                    run += w[j];
+                    if (w[j] > 0.0 && !past) {
+                        some = j;
+                        vs = v[j];
+                        past = run > target;
+                    }
+                }
+                drawn(e0 + some, vs, log2(S));
+            }
+            return;
+        }
+    }
+
+    // ---- a bound under the border, in bins of the distance from the maximum
+    const auto each_max = [&](auto g) TRLK_INLINE {  // g(block, value)
+        const auto vec = [&](int i, u32x4 q) TRLK_INLINE {
+            float v[EPV];
+            Elem<DT>::unpack(q, v);
+#pragma unroll
+            for (int e = 0; e < EPV; ++e) g(i * EPV + e, v[e]);
+        };
+#pragma unroll
+        for (int j = 0; j < kKeep; ++j)
+            if (tid + j * kSelThreads < n_vec) vec(tid + j * kSelThreads, held[j]);
+        for (int i = tid + kKeep * kSelThreads; i < n_vec; i += kSelThreads) vec(i, bmax[i]);
+    };
+    const u64 mass_target = [&]() TRLK_INLINE {  // of top-p without top-k
+        const double t = __builtin_ceil(f.top_p * S * unit);
+        return t < 1.0 ? u64(1) : u64(int64_t(t));
+    }();
+    int bound = kEveryBin;
+    float x_low = -INFINITY;  // no candidate lies under it
+    {
+        const bool by_count = f.top_k != 0, by_mass = !by_count && f.top_p > 0.0;
+        if (by_count || by_mass) {
+            each_max([&](int, float v) TRLK_INLINE {
+                const int d = distance_bin(m, v);
+                if (d < kBins) atomicAdd(&s.bins[d], by_count ? u64(1) : fixed(weight(v)));
+            });
+            __syncthreads();
+            uint32_t bin;
+            u64 before = 0;
+            // (the sum of rounded weights may be half a unit for each block too large)
+            if (crossing(s, kBins, by_count ? u64(f.top_k) : mass_target + n_blocks, bin, before)) bound = int(bin);
+        }
+        if (by_mass) {  // all tokens of less than (1 - top_p) / V of the mass together have less than 1 - top_p of it
+            x_low = float(ref + log2((1.0 - f.top_p) * S / double(V) * (1.0 - 1e-9)) / c);
+            x_low -= 1e-6f * fabsf(x_low) + 1e-30f;
+        }
+        if (f.min_p > 0.0 && !(f.top_k && f.top_p > 0.0)) {  // (top-p of top-k counts what min-p takes away)
+            float b = float(ref + log2(f.min_p) / c);
+            b -= 1e-6f * fabsf(b) + 1e-30f;
+            x_low = fmaxf(x_low, b);
+        }
+        if (x_low > -INFINITY) {
+            const int d = distance_bin(m, x_low);
+            bound = d < bound ? d : bound;
+        }
+    }
+    const auto in_bound = [&](float v) TRLK_INLINE { return v > -INFINITY && distance_bin(m, v) <= bound; };
+
+    // ---- blocks that reach the bound, and the candidates in them
+    each_max([&](int i, float v) TRLK_INLINE {
+        if (in_bound(v)) {
+            const uint32_t to = atomicAdd(&s.n_list, 1u);
+            if (to < kList) s.list[to] = uint16_t(i);
+        }
+    });
+    __syncthreads();
+    const bool listed = s.n_list <= kList;
+    const int n_visit = listed ? int(s.n_list) : n_blocks;
+    // all logits over the bound, a wave to a block, four blocks in flight: g(in, value, key, index), with all lanes of the wave in it
+    const auto stream = [&](auto g) TRLK_INLINE {
+        constexpr int U = 4;
+        for (int j0 = wave; j0 < n_visit; j0 += U * kSelWaves) {
+            T raw[U];
+            int64_t e[U];
+#pragma unroll
+            for (int q = 0; q < U; ++q) {
+                const int j = j0 + q * kSelWaves;
+                e[q] = j < n_visit ? int64_t(listed ? int(s.list[j]) : j) * kBlock + lane : V;
+                raw[q] = e[q] < V ? x[e[q]] : T(0);
+            }
+#pragma unroll
+            for (int q = 0; q < U; ++q) {
+                const float v = Elem<DT>::to_float(raw[q]);
+                g(e[q] < V && in_bound(v), v, K::of(raw[q]), uint32_t(e[q]));
+            }
+        }
+    };
+    const bool too_many = !listed && !f.top_k;  // (kList blocks have as many candidates at least)
+    if (!too_many) {
+        uint32_t min_key = ~0u, low_key = ~0u;
+        stream([&](bool in, float v, uint32_t k, uint32_t e) TRLK_INLINE {
+            const u64 vote = __ballot(in);
+            if (!vote) return;
+            uint32_t to = 0;
+            if (lane == 0) to = atomicAdd(&s.n_cand, uint32_t(__popcll(vote)));
+            to = __shfl(to, 0) + __popcll(vote & ((u64(1) << lane) - 1));
+            if (in) {
+                const double w = weight(v);
+                if (w >= f.min_p && k < min_key) min_key = k;
+                if (k < low_key) low_key = k;
+                if (to < kCandidates) s.cand[to] = Candidate{u64(k) << 32 | (~e & 0xffffffffu), fixed(w)};
+            }
+        });
+#pragma unroll
+        for (int o = kWave / 2; o > 0; o >>= 1) {
+            const uint32_t p = __shfl_xor(min_key, o), q = __shfl_xor(low_key, o);
+            min_key = p < min_key ? p : min_key;
+            low_key = q < low_key ? q : low_key;
+        }
+        if (lane == 0) {
+            atomicMin(&s.min_key, min_key);
+            atomicMin(&s.low_key, low_key);
+        }
+        __syncthreads();
+    }
+    const int n_cand = too_many ? kCandidates + 1 : int(s.n_cand);
+    uint32_t kept_from = f.min_p > 0.0 ? s.min_key : 0u;  // the smallest key that min-p keeps
+
+    // the integer that a cumulative weight has to pass, and whether it is none (the first kept token passes it then, also one whose
+    // weight is less than a unit)
+    const auto draw_target = [&](u64 W) TRLK_INLINE {
+        const double t = u * double(W);
+        const u64 target = t < double(W) ? u64(int64_t(t)) : W - 1;
+        return target < W ? target : W - 1;
+    };
+
+    // ---- up to 256 candidates: every pair is compared, which gives each one its rank and the mass before it
+    constexpr int kPairs = 256;
+    if (n_cand <= kPairs) {
+        const int np = n_cand <= 64 ? 64 : n_cand <= 128 ? 128 : 256, parts = kSelThreads / np, len = np / parts;
+        const int i = tid & (np - 1), part = tid / np;
+        if (tid >= n_cand && tid < np) s.cand[tid] = Candidate{0, 0};
+        __syncthreads();
+        const Candidate me = s.cand[i];
+        const bool real = tid < n_cand;  // (the first np threads go on with a candidate each)
+        u64* sums = s.bins;
+        uint32_t* ranks = reinterpret_cast<uint32_t*>(s.bins + kSelThreads);
+        u64 before = 0;
+        uint32_t rank = 0;
+        for (int j = 0; j < len; ++j) {
+            const Candidate o = s.cand[part * len + j];
+            const bool earlier = o.order > me.order;
+            before += earlier ? o.weight : 0;
+            rank += earlier ? 1u : 0u;
+        }
+        sums[tid] = before;
+        ranks[tid] = rank;
+        __syncthreads();
+        for (int q = 1; q < parts; ++q) {
+            before += sums[(tid + q * np) & (kSelThreads - 1)];
+            rank += ranks[(tid + q * np) & (kSelThreads - 1)];
+        }
+        bool kept = real && (f.top_k == 0 || rank < f.top_k);
+        if (f.top_p > 0.0) {
+            u64 target = mass_target;
+            if (f.top_k) {
+                const u64 W1 = block_total(kept ? me.weight : 0, s.scan);
+                const double t = __builtin_ceil(f.top_p * double(W1));
+                target = t < 1.0 ? u64(1) : u64(int64_t(t));
+            }
+            kept = kept && before < target;
+        }
+        kept = kept && uint32_t(me.order >> 32) >= kept_from;
+        const u64 W = block_total(kept ? me.weight : 0, s.scan);
+        const double log2_mass = log2(double(W)) - a.fix;
+        if constexpr (SCORE) {
+            const int n_kept = __syncthreads_count(kept);  // (a prefix of the order)
+            if (real && int(rank) == n_kept - 1) {
+                s.border = uint32_t(me.order >> 32);
+                s.border_index = ~uint32_t(me.order);
+            }
+            __syncthreads();
+            scored(s.border, s.border_index, log2_mass);
+        } else {
+            const u64 target = draw_target(W);
+            const u64 mine_w = kept ? (target ? me.weight : 1) : 0;
+            if (tid < np) s.cand[tid].weight = mine_w;  // (everyone has read its own)
+            __syncthreads();
+            const uint32_t my_index = ~uint32_t(me.order);
+            u64 cum = 0;
+            for (int j = 0; j < len; ++j) {
+                const Candidate o = s.cand[part * len + j];
+                cum += ~uint32_t(o.order) <= my_index ? o.weight : 0;
+            }
+            sums[tid] = cum;
+            __syncthreads();
+            for (int q = 1; q < parts; ++q) cum += sums[(tid + q * np) & (kSelThreads - 1)];
+            if (kept && cum > target && cum - mine_w <= target) drawn(my_index, K::to_float(uint32_t(me.order >> 32)), log2_mass);
+        }
+        return;
+    }
+
+    const uint32_t top = K::of_float(m), lowest = K::of_float(-INFINITY) + 1u;
+    uint32_t border = 0, border_index = ~0u, at;
+    u64 before = 0;
+    // ---- very many candidates, without top-k: two passes over the row.  The first adds the weights up in bins linear in the logit; the
+    // second sums, chunk by chunk, what lies before the border's bin, and lists that bin, where the border is then found.
+    if (n_cand > kCandidates && !f.top_k && x_low > -INFINITY) {
+        const float scale = float(kBins - 1) / fmaxf(m - x_low, 1e-30f);
+        const auto bin_of = [&](float v) TRLK_INLINE {
+            const float t = (m - v) * scale;
+            return t < float(kBins) ? int(t) : kBins;
+        };
+        // g(value, index) for every logit, end(chunk) after a wave's chunk: a vector at a time, the next one in flight (rows of other kinds
+        // want the registers)
+        const auto row_pass = [&](auto g, auto end) TRLK_INLINE {
+            for (int ch = wave; ch < a.chunks; ch += kSelWaves) {
+                const int64_t e0 = int64_t(ch) * kChunk;
+                const auto load = [&](int i) TRLK_INLINE -> u32x4 {
+                    const int64_t at = e0 + (i * kWave + lane) * EPV;
+                    if (at + EPV <= V) return *reinterpret_cast<const u32x4_u*>(x + at);
+                    float v[EPV];
+#pragma unroll
+                    for (int e = 0; e < EPV; ++e) v[e] = at + e < V ? Elem<DT>::load1(x + at + e) : -INFINITY;
+                    return Elem<DT>::pack(v);
+                };
+                u32x4 next = load(0);
+#pragma unroll 1
+                for (int i = 0; i < NV; ++i) {
+                    float v[EPV];
+                    Elem<DT>::unpack(next, v);
+                    if (i + 1 < NV) next = load(i + 1);
+#pragma unroll
+                    for (int e = 0; e < EPV; ++e) {
+                        g(v[e], uint32_t(e0) + (i * kWave + lane) * EPV + e);
+                        __builtin_amdgcn_sched_barrier(0);
+                    }
+                }
+                end(ch);
+            }
+        };
+        int border_bin = kBins;
+        bool found = true;
+        if (f.top_p > 0.0) {
+            clear_bins(s, kBins);
+            row_pass(
+                [&](float v, uint32_t) TRLK_INLINE {
+                    if (v >= x_low) atomicAdd(&s.bins[bin_of(v)], fixed(weight(v)));
+                },
+                [](int) TRLK_INLINE {});
+            __syncthreads();
+            uint32_t bin;
+            found = crossing(s, kBins, mass_target, bin, before);
+            border_bin = int(bin);
+        }
+        __syncthreads();
+        if (tid == 0) {
+            s.n_cand = 0;
+            s.min_key = ~0u;
+        }
+        __syncthreads();
+        u64* cmass = reinterpret_cast<u64*>(csum);
+        if (found) {
+            u64 mass = 0;
+            uint32_t min_key = ~0u;
+            row_pass(
+                [&](float v, uint32_t e) TRLK_INLINE {
+                    const int b = v >= x_low ? bin_of(v) : kBins + 1;
+                    if (b > border_bin) return;
+                    const double w = weight(v);
+                    const uint32_t k = K::of_float(v);
+                    if (w >= f.min_p) {
+                        if (b < border_bin) mass += fixed(w);
+                        if (k < min_key) min_key = k;
+                    }
+                    if (b == border_bin) {
+                        const uint32_t to = atomicAdd(&s.n_cand, 1u);
+                        if (to < kCandidates) s.cand[to] = Candidate{u64(k) << 32 | (~e & 0xffffffffu), fixed(w)};
+                    }
+                },
+                [&](int ch) TRLK_INLINE {
+#pragma unroll
+                    for (int o = kWave / 2; o > 0; o >>= 1) mass += __shfl_xor(mass, o);
+                    if (lane == 0) cmass[ch] = mass;
+                    mass = 0;
+                });
+#pragma unroll
+            for (int o = kWave / 2; o > 0; o >>= 1) {
+                const uint32_t p = __shfl_xor(min_key, o);
+                min_key = p < min_key ? p : min_key;
+            }
+            if (lane == 0) atomicMin(&s.min_key, min_key);
+        }
+        __syncthreads();
+        const int n_bin = int(s.n_cand);
+        if (found && n_bin <= kCandidates) {
+            kept_from = f.min_p > 0.0 ? s.min_key : 0u;
+            const auto each = [&](auto g) TRLK_INLINE {
+                for (int i = tid; i < n_bin; i += kSelThreads) g(uint32_t(s.cand[i].order >> 32), ~uint32_t(s.cand[i].order), s.cand[i].weight);
+            };
+            if (f.top_p > 0.0) {
+                descend(s, [&](auto put) TRLK_INLINE { each([&](uint32_t k, uint32_t, u64 w) TRLK_INLINE { put(top - k, w); }); }, 0, top - lowest, mass_target, at, before);
+                border = top - at;
+                const u64 w = fixed(weight(K::to_float(border))), ties = (mass_target - before + w - 1) / w;
+                u64 count = 0;
+                each([&](uint32_t k, uint32_t, u64) TRLK_INLINE { count += k == border; });
+                if (ties < block_total(count, s.scan)) {
+                    before = 0;
+                    descend(s, [&](auto put) TRLK_INLINE { each([&](uint32_t k, uint32_t e, u64) TRLK_INLINE { put(e, k == border); }); }, 0, uint32_t(V - 1), ties,
+                            border_index, before);
+                }
+            }
+            if (kept_from > border) {
+                border = kept_from;
+                border_index = ~0u;
+            }
+            const auto kept = [&](uint32_t k, uint32_t e) TRLK_INLINE { return k > border || (k == border && e <= border_index); };
+            // the border's bin joins its chunks
+            clear_bins(s, a.chunks);
+            each([&](uint32_t k, uint32_t e, u64 w) TRLK_INLINE {
+                if (kept(k, e)) atomicAdd(&s.bins[e / kChunk], w);
+            });
+            __syncthreads();
+            const auto chunk_mass = [&](int i) TRLK_INLINE { return cmass[i] + s.bins[i]; };
+            u64 sum = 0, up, W;
+            for (int i = first; i < last; ++i) sum += chunk_mass(i);
+            const u64 exc = block_scan(sum, s.scan, up, W);
+            const double log2_mass = log2(double(W)) - a.fix;
+            if constexpr (SCORE) {
+                scored(border, border_index, log2_mass);
+            } else {
+                const u64 target = draw_target(W);
+                if (exc <= target && up > target) {  // (one thread)
+                    u64 run = exc;
+                    int ch = first;
+                    for (; ch + 1 < last && run + chunk_mass(ch) <= target; ++ch) run += chunk_mass(ch);
+                    s.n_list = uint32_t(ch);
+                    s.before = run;
+                }
+                __syncthreads();
+                const int64_t e0 = int64_t(s.n_list) * kChunk + tid * PER;
+                u64 run = s.before, w[PER], part = 0, all;
+                float v[PER];
+#pragma unroll
+                for (int j = 0; j < PER; ++j) {
+                    v[j] = e0 + j < V ? Elem<DT>::load1(x + e0 + j) : -INFINITY;
+                    w[j] = v[j] > -INFINITY && kept(K::of_float(v[j]), uint32_t(e0 + j)) ? fixed(weight(v[j])) : 0;
+                    part += w[j];
+                }
+                run += block_scan(part, s.scan, up, all);
+#pragma unroll
+                for (int j = 0; j < PER; ++j) {
+                    if (w[j] && run <= target && run + w[j] > target) drawn(e0 + j, v[j], log2_mass);
+                    run += w[j];
+                }
+            }
+            return;
+        }
+        if (tid == 0) s.n_cand = kCandidates + 1;
+        __syncthreads();
+    }
+
+    // ---- the rest: radix descents over the candidates, in LDS or (more of them) read again in each step
+    const bool in_lds = n_cand <= kCandidates;
+    if (!in_lds && f.min_p > 0.0) {  // (a row that came past the gathering has not seen its smallest kept key)
+        if (tid == 0) s.min_key = ~0u;
+        __syncthreads();
+        uint32_t min_key = ~0u;
+        stream([&](bool in, float v, uint32_t k, uint32_t) TRLK_INLINE {
+            if (in && weight(v) >= f.min_p && k < min_key) min_key = k;
+        });
+        if (min_key != ~0u) atomicMin(&s.min_key, min_key);
+        __syncthreads();
+        kept_from = s.min_key;
+    }
+    // g(key, index, weight()) for this thread's candidates
+    const auto each = [&](auto g) TRLK_INLINE {
+        if (in_lds) {
+            for (int i = tid; i < n_cand; i += kSelThreads) g(uint32_t(s.cand[i].order >> 32), ~uint32_t(s.cand[i].order), [&]() TRLK_INLINE { return s.cand[i].weight; });
+        } else {
+            stream([&](bool in, float v, uint32_t k, uint32_t e) TRLK_INLINE {
+                if (in) g(k, e, [&]() TRLK_INLINE { return fixed(weight(v)); });
+            });
+        }
+    };
+    const uint32_t span = top - (in_lds ? s.low_key : lowest);
+    u64 ties = ~u64(0);  // how many tokens of the border's value are kept
+    before = 0;
+    if (f.top_k) {
+        if (descend(s, [&](auto put) TRLK_INLINE { each([&](uint32_t k, uint32_t, auto) TRLK_INLINE { put(top - k, 1); }); }, 0, span, f.top_k, at, before)) {
+            border = top - at;
+            ties = f.top_k - before;
+        }
+    }
+    if (f.top_p > 0.0) {
+        u64 target = mass_target;
+        if (f.top_k) {
+            u64 mass = 0;
+            each([&](uint32_t k, uint32_t, auto w) TRLK_INLINE {
+                if (k > border) mass += w();
+            });
+            mass = block_total(mass, s.scan);
+            if (border) mass += ties * fixed(weight(K::to_float(border)));
+            const double t = __builtin_ceil(f.top_p * double(mass));
+            target = t < 1.0 ? u64(1) : u64(int64_t(t));
+        }
+        before = 0;
+        const uint32_t from = border;
+        if (descend(s, [&](auto put) TRLK_INLINE {
+                each([&](uint32_t k, uint32_t, auto w) TRLK_INLINE {
+                    if (k >= from) put(top - k, w());
+                });
+            }, 0, span, target, at, before)) {
+            const uint32_t b = top - at;
+            const u64 w = fixed(weight(K::to_float(b))), n = (target - before + w - 1) / w;
+            ties = b == border && n > ties ? ties : n;
+            border = b;
+        }
+    }
+    if (border) {
+        u64 count = 0;
+        each([&](uint32_t k, uint32_t, auto) TRLK_INLINE { count += k == border; });
+        if (ties < block_total(count, s.scan)) {
+            const uint32_t b = border;
+            before = 0;
+            descend(s, [&](auto put) TRLK_INLINE { each([&](uint32_t k, uint32_t e, auto) TRLK_INLINE { put(e, k == b); }); }, 0, uint32_t(V - 1), ties,
+                    border_index, before);
+        }
+    }
+    if (kept_from > border) {
+        border = kept_from;
+        border_index = ~0u;
+    }
+    if (border < lowest) border = lowest;
+    const auto kept = [&](uint32_t k, uint32_t e) TRLK_INLINE { return k > border || (k == border && e <= border_index); };
+    u64 W = 0;
+    each([&](uint32_t k, uint32_t e, auto w) TRLK_INLINE {
+        if (kept(k, e)) W += w();
+    });
+    W = block_total(W, s.scan);
+    const double log2_mass = log2(double(W)) - a.fix;
+    if constexpr (SCORE) {
+        scored(border, border_index, log2_mass);
     } else {
-        a.out_ids[row] = id;
-        const float v = Elem<DT>::load1(x + id);
-        a.out_logp[row] = float(((double(v) - ref) * c - log2_mass) * 0.69314718055994530942);
+        const u64 target = draw_target(W);
+        before = 0;
+        uint32_t id = 0;
+        descend(s, [&](auto put) TRLK_INLINE {
+            each([&](uint32_t k, uint32_t e, auto w) TRLK_INLINE {
+                if (kept(k, e)) put(e, target ? w() : u64(1));
+            });
+        }, 0, uint32_t(V - 1), target ? target + 1 : 1, id, before);
+        if (tid == 0) drawn(id, Elem<DT>::load1(x + id), log2_mass);
     }
 }
 
