@@ -53,6 +53,25 @@ __device__ __forceinline__ double exp2_f64(double t) {
     return __builtin_amdgcn_ldexp(y, int(n));
 }
 
+// The same for sums, where what underflows may count 2^-1000: n comes from the low bits of t + 1.5 * 2^52 and goes into the exponent
+// with one integer addition (rounding, conversion and ldexp of 64-bit numbers run at a quarter of the rate of the products).
+__device__ __forceinline__ double exp2_sum(double t) {
+    t = __builtin_fmax(t, -1000.0);
+    const double big = t + 0x1.8p52, f = t - (big - 0x1.8p52);
+    double y = 1.0205905413765595e-07;
+    y = __builtin_fma(y, f, 1.325964524488711e-06);
+    y = __builtin_fma(y, f, 1.5252672924850737e-05);
+    y = __builtin_fma(y, f, 0.0001540343375125101);
+    y = __builtin_fma(y, f, 0.0013333558200794592);
+    y = __builtin_fma(y, f, 0.009618129193934313);
+    y = __builtin_fma(y, f, 0.05550410866465167);
+    y = __builtin_fma(y, f, 0.2402265069564034);
+    y = __builtin_fma(y, f, 0.6931471805599462);
+    y = __builtin_fma(y, f, 1.0);
+    const uint32_t n = uint32_t(__builtin_bit_cast(uint64_t, big));
+    return __builtin_bit_cast(double, __builtin_bit_cast(uint64_t, y) + (uint64_t(n) << 52));
+}
+
 // maximum that lets a NaN through
 __device__ __forceinline__ float max_nan(float a, float b) { return __builtin_elementwise_maximum(a, b); }
 __device__ __forceinline__ float wave_max_nan(float v) {
@@ -209,7 +228,7 @@ __global__ __launch_bounds__(kScanThreads) void filter_scan_kernel(ScanArgs a) {
         const double c = row_filter(a.f, row, a.x.vocab).c, ref = m > -INFINITY && m < INFINITY ? double(m) : 0.0;
         double s = 0.0;
 #pragma unroll
-        for (int j = 0; j < NV * EPV; ++j) s += exp2_f64((double(x[j]) - ref) * c);
+        for (int j = 0; j < NV * EPV; ++j) s += exp2_sum((double(x[j]) - ref) * c);
 #pragma unroll
         for (int o = kWave / 2; o > 0; o >>= 1) s += __shfl_xor(s, o);
         if (lane == 0) a.chunk_sum[unit] = s;
@@ -237,6 +256,35 @@ struct SelectArgs {
     int32_t* error_flag;
 };
 
+// A 64-bit value from the lane that the data-parallel primitive names, 0 where there is none.
+template <int CTRL, int ROWS, typename V>
+__device__ __forceinline__ V moved(V v) {
+    const uint64_t b = __builtin_bit_cast(uint64_t, v);
+    const uint32_t lo = uint32_t(__builtin_amdgcn_update_dpp(0, int(uint32_t(b)), CTRL, ROWS, 0xf, false));
+    const uint32_t hi = uint32_t(__builtin_amdgcn_update_dpp(0, int(uint32_t(b >> 32)), CTRL, ROWS, 0xf, false));
+    return __builtin_bit_cast(V, uint64_t(hi) << 32 | lo);
+}
+// Sums over the lanes up to each one: shifts within rows of 16 lanes, then the last lane of row 0 (2) to row 1 (3), that of row 1 to
+// rows 2 and 3.  A fifth of the time that six shuffles through LDS take.
+template <typename V>
+__device__ __forceinline__ V wave_inclusive(V v) {
+    v += moved<0x111, 0xf>(v);
+    v += moved<0x112, 0xf>(v);
+    v += moved<0x114, 0xf>(v);
+    v += moved<0x118, 0xf>(v);
+    v += moved<0x142, 0xa>(v);
+    v += moved<0x143, 0xc>(v);
+    return v;
+}
+// A place for one number of each wave.  Two neighbouring block-wide sums take different ones, so that a barrier lies between a
+// place's readers and its next writers.
+union WaveSlots {
+    u64 u[kSelWaves];
+    double f[kSelWaves];
+};
+__device__ __forceinline__ u64& slot_of(WaveSlots& s, int i, u64) { return s.u[i]; }
+__device__ __forceinline__ double& slot_of(WaveSlots& s, int i, double) { return s.f[i]; }
+
 struct alignas(16) Candidate {
     u64 order;  // key above, ~index below: larger is earlier
     u64 weight;
@@ -245,59 +293,46 @@ struct SelectShared {
     u64 bins[kBins];
     Candidate cand[kCandidates];
     uint16_t list[kList];
-    u64 scan[kSelWaves];
-    double scan_f[kSelWaves];
+    WaveSlots slots[4];
     float wave_f[kSelWaves];
-    int hit[kSelWaves], tail[kSelWaves];
+    int hit[2][kSelWaves], tail[2][kSelWaves];
     double prefix[kSelWaves];
     u64 before;
     uint32_t bin, n_list, n_cand, min_key, low_key, border, border_index;
 };
 
-template <typename V>
-__device__ __forceinline__ V wave_inclusive(V v, int lane) {
-#pragma unroll
-    for (int o = 1; o < kWave; o <<= 1) {
-        const V u = __shfl_up(v, o);
-        if (lane >= o) v += u;
-    }
-    return v;
-}
 // Sums over the threads before this one (returned) and up to it (`upto`), and over all.  What one thread's `upto` is, is the next
-// one's exclusive sum to the last bit.  Contains two barriers.
+// one's exclusive sum to the last bit.  Contains one barrier.
 template <typename V>
-__device__ __forceinline__ V block_scan(V v, V* scratch, V& upto, V& total) {
+__device__ __forceinline__ V block_scan(V v, WaveSlots& slots, V& upto, V& total) {
     const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
-    const V inc = wave_inclusive(v, lane);
+    const V inc = wave_inclusive(v);
     V exc = __shfl_up(inc, 1);
     if (lane == 0) exc = 0;
-    __syncthreads();
-    if (lane == kWave - 1) scratch[wave] = inc;
+    if (lane == kWave - 1) slot_of(slots, wave, v) = inc;
     __syncthreads();
     V base = 0, all = 0;
 #pragma unroll
     for (int w = 0; w < kSelWaves; ++w) {
         if (w == wave) base = all;
-        all += scratch[w];
+        all += slot_of(slots, w, v);
     }
     total = all;
     upto = base + inc;
     return base + exc;
 }
-__device__ __forceinline__ u64 block_total(u64 v, u64* scratch) {
-#pragma unroll
-    for (int o = kWave / 2; o > 0; o >>= 1) v += __shfl_xor(v, o);
-    __syncthreads();
-    if ((threadIdx.x & (kWave - 1)) == 0) scratch[threadIdx.x / kWave] = v;
+__device__ __forceinline__ u64 block_total(u64 v, WaveSlots& slots) {
+    const u64 inc = wave_inclusive(v);
+    if ((threadIdx.x & (kWave - 1)) == kWave - 1) slots.u[threadIdx.x / kWave] = inc;
     __syncthreads();
     u64 r = 0;
 #pragma unroll
-    for (int w = 0; w < kSelWaves; ++w) r += scratch[w];
+    for (int w = 0; w < kSelWaves; ++w) r += slots.u[w];
     return r;
 }
 
 // The bin up to which the values of bins [0, n) and `before` reach `target` first, and in `before` what lies before it; false if
-// all of them do not.  The bins are complete and the barrier behind them passed; s.bin is ~0.  Contains three barriers.
+// all of them do not.  The bins are complete and the barrier behind them passed; s.bin is ~0.  Contains two barriers.
 __device__ __forceinline__ bool crossing(SelectShared& s, int n, u64 target, uint32_t& bin, u64& before) {
     u64 v[4], sum = 0, upto, total;
 #pragma unroll
@@ -306,7 +341,7 @@ __device__ __forceinline__ bool crossing(SelectShared& s, int n, u64 target, uin
         v[j] = i < n ? s.bins[i] : 0;
         sum += v[j];
     }
-    u64 at = before + block_scan(sum, s.scan, upto, total);
+    u64 at = before + block_scan(sum, s.slots[0], upto, total);
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
         if (at < target && at + v[j] >= target) {  // (one bin of one thread)
@@ -325,7 +360,7 @@ __device__ __forceinline__ bool crossing(SelectShared& s, int n, u64 target, uin
 __device__ __forceinline__ void clear_bins(SelectShared& s, int n) {
     for (int i = threadIdx.x; i < n; i += kSelThreads) s.bins[i] = 0;
     __syncthreads();
-    if (threadIdx.x == 0) s.bin = ~0u;  // (everyone has read the last one; the next is written two barriers from here)
+    if (threadIdx.x == 0) s.bin = ~0u;  // (everyone has read the last one, and two barriers lie before the next is written)
 }
 
 // The smallest position in [lo, hi] up to which `before` and the values reach `target`, and in `before` what lies before it.
@@ -360,22 +395,22 @@ __device__ __forceinline__ int distance_bin(float m, float x) {
 constexpr int kEveryBin = 1 << 30;
 
 // `owner` of the smallest thread number, and if there is none of the largest with `some`: its number, the same for all threads
-__device__ __forceinline__ int first_thread(SelectShared& s, bool owner, bool some) {
+__device__ __forceinline__ int first_thread(SelectShared& s, int which, bool owner, bool some) {
     const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
     const u64 a = __ballot(owner), b = __ballot(some);
     if (lane == 0) {
-        s.hit[wave] = a ? wave * kWave + __builtin_ctzll(a) : -1;
-        s.tail[wave] = b ? wave * kWave + 63 - __builtin_clzll(b) : -1;
+        s.hit[which][wave] = a ? wave * kWave + __builtin_ctzll(a) : -1;
+        s.tail[which][wave] = b ? wave * kWave + 63 - __builtin_clzll(b) : -1;
     }
     __syncthreads();
     int r = -1;
 #pragma unroll
     for (int w = kSelWaves - 1; w >= 0; --w)
-        if (s.hit[w] >= 0) r = s.hit[w];
+        if (s.hit[which][w] >= 0) r = s.hit[which][w];
     if (r >= 0) return r;
 #pragma unroll
     for (int w = 0; w < kSelWaves; ++w)
-        if (s.tail[w] >= 0) r = s.tail[w];
+        if (s.tail[which][w] >= 0) r = s.tail[which][w];
     return r;
 }
 
@@ -500,7 +535,7 @@ __global__ __launch_bounds__(kSelThreads, 4) void filter_select_kernel(SelectArg
     if (with_sum) {
         if (first < last) mine = sum0 * weight_at(max0);
         for (int i = first + 1; i < last; ++i) mine += csum[i] * weight(cmax[i]);
-        base = block_scan(mine, s.scan_f, upto, S);
+        base = block_scan(mine, s.slots[1], upto, S);
     }
     // ---- no filter: the chunk, then the token in it
     if (!filtered) {
@@ -510,7 +545,7 @@ __global__ __launch_bounds__(kSelThreads, 4) void filter_select_kernel(SelectArg
             // (u * S can round up to the whole sum, and the last bits of a scan are not monotone: the first thread whose sum passes it,
             // and that has something, or the last one that has)
             const double target = u * S;
-            const int owner = first_thread(s, mine > 0.0 && upto > target, mine > 0.0);
+            const int owner = first_thread(s, 0, mine > 0.0 && upto > target, mine > 0.0);
             if (tid == owner) {
                 double at = base, v = sum0 * weight_at(max0);
                 int chunk = first, some = v > 0.0 ? first : -1;
@@ -541,8 +576,8 @@ __global__ __launch_bounds__(kSelThreads, 4) void filter_select_kernel(SelectArg
                 w[j] = weight(v[j]);
                 sum += w[j];
             }
-            double run = prefix + block_scan(sum, s.scan_f, up, all);
-            const int at = first_thread(s, sum > 0.0 && prefix + up > target, sum > 0.0);
+            double run = prefix + block_scan(sum, s.slots[2], up, all);
+            const int at = first_thread(s, 1, sum > 0.0 && prefix + up > target, sum > 0.0);
             if (tid == at) {
                 int some = 0;
                 float vs = v[0];
@@ -612,17 +647,20 @@ __global__ __launch_bounds__(kSelThreads, 4) void filter_select_kernel(SelectArg
 
     // ---- blocks that reach the bound, and the candidates in them
     each_max([&](int i, float v) TRLK_INLINE {
-        if (in_bound(v)) {
-            const uint32_t to = atomicAdd(&s.n_list, 1u);
-            if (to < kList) s.list[to] = uint16_t(i);
-        }
+        const bool in = in_bound(v);
+        const u64 vote = __ballot(in);
+        if (!vote) return;
+        uint32_t to = 0;
+        if (lane == __builtin_ctzll(vote)) to = atomicAdd(&s.n_list, uint32_t(__popcll(vote)));
+        to = __shfl(to, __builtin_ctzll(vote)) + __popcll(vote & ((u64(1) << lane) - 1));
+        if (in && to < kList) s.list[to] = uint16_t(i);
     });
     __syncthreads();
     const bool listed = s.n_list <= kList;
     const int n_visit = listed ? int(s.n_list) : n_blocks;
-    // all logits over the bound, a wave to a block, four blocks in flight: g(in, value, key, index), with all lanes of the wave in it
+    // all logits over the bound, a wave to a block, eight blocks in flight: g(in, value, key, index), with all lanes of the wave in it
     const auto stream = [&](auto g) TRLK_INLINE {
-        constexpr int U = 4;
+        constexpr int U = 8;
         for (int j0 = wave; j0 < n_visit; j0 += U * kSelWaves) {
             T raw[U];
             int64_t e[U];
@@ -681,41 +719,40 @@ __global__ __launch_bounds__(kSelThreads, 4) void filter_select_kernel(SelectArg
     // ---- up to 256 candidates: every pair is compared, which gives each one its rank and the mass before it
     constexpr int kPairs = 256;
     if (n_cand <= kPairs) {
-        const int np = n_cand <= 64 ? 64 : n_cand <= 128 ? 128 : 256, parts = kSelThreads / np, len = np / parts;
-        const int i = tid & (np - 1), part = tid / np;
+        // (`parts` neighbouring lanes have a candidate together, and each compares it with its part of all; the sums stay in the wave)
+        const int lp = n_cand <= 64 ? 3 : n_cand <= 128 ? 2 : 1, parts = 1 << lp, np = kSelThreads >> lp, len = np >> lp;
+        const int i = tid >> lp, part = tid & (parts - 1);
         if (tid >= n_cand && tid < np) s.cand[tid] = Candidate{0, 0};
         __syncthreads();
         const Candidate me = s.cand[i];
-        const bool real = tid < n_cand;  // (the first np threads go on with a candidate each)
-        u64* sums = s.bins;
-        uint32_t* ranks = reinterpret_cast<uint32_t*>(s.bins + kSelThreads);
-        u64 before = 0;
-        uint32_t rank = 0;
+        const bool real = i < n_cand && part == 0;
+        const auto over_parts = [&](u64 v) TRLK_INLINE {
+            v += moved<0xb1, 0xf>(v);                 // the neighbour
+            if (parts > 2) v += moved<0x4e, 0xf>(v);  // the other pair of four
+            if (parts > 4) v += moved<0x141, 0xf>(v); // the mirrored lane of eight
+            return v;
+        };
+        u64 before = 0, rank = 0;
         for (int j = 0; j < len; ++j) {
-            const Candidate o = s.cand[part * len + j];
+            const Candidate o = s.cand[j * parts + part];
             const bool earlier = o.order > me.order;
             before += earlier ? o.weight : 0;
-            rank += earlier ? 1u : 0u;
+            rank += earlier ? 1 : 0;
         }
-        sums[tid] = before;
-        ranks[tid] = rank;
-        __syncthreads();
-        for (int q = 1; q < parts; ++q) {
-            before += sums[(tid + q * np) & (kSelThreads - 1)];
-            rank += ranks[(tid + q * np) & (kSelThreads - 1)];
-        }
+        before = over_parts(before);
+        rank = over_parts(rank);
         bool kept = real && (f.top_k == 0 || rank < f.top_k);
         if (f.top_p > 0.0) {
             u64 target = mass_target;
             if (f.top_k) {
-                const u64 W1 = block_total(kept ? me.weight : 0, s.scan);
+                const u64 W1 = block_total(kept ? me.weight : 0, s.slots[1]);
                 const double t = __builtin_ceil(f.top_p * double(W1));
                 target = t < 1.0 ? u64(1) : u64(int64_t(t));
             }
             kept = kept && before < target;
         }
         kept = kept && uint32_t(me.order >> 32) >= kept_from;
-        const u64 W = block_total(kept ? me.weight : 0, s.scan);
+        const u64 W = block_total(kept ? me.weight : 0, s.slots[2]);
         const double log2_mass = log2(double(W)) - a.fix;
         if constexpr (SCORE) {
             const int n_kept = __syncthreads_count(kept);  // (a prefix of the order)
@@ -728,17 +765,15 @@ __global__ __launch_bounds__(kSelThreads, 4) void filter_select_kernel(SelectArg
         } else {
             const u64 target = draw_target(W);
             const u64 mine_w = kept ? (target ? me.weight : 1) : 0;
-            if (tid < np) s.cand[tid].weight = mine_w;  // (everyone has read its own)
+            if (part == 0) s.cand[i].weight = mine_w;  // (everyone has read its own)
             __syncthreads();
             const uint32_t my_index = ~uint32_t(me.order);
             u64 cum = 0;
             for (int j = 0; j < len; ++j) {
-                const Candidate o = s.cand[part * len + j];
+                const Candidate o = s.cand[j * parts + part];
                 cum += ~uint32_t(o.order) <= my_index ? o.weight : 0;
             }
-            sums[tid] = cum;
-            __syncthreads();
-            for (int q = 1; q < parts; ++q) cum += sums[(tid + q * np) & (kSelThreads - 1)];
+            cum = over_parts(cum);
             if (kept && cum > target && cum - mine_w <= target) drawn(my_index, K::to_float(uint32_t(me.order >> 32)), log2_mass);
         }
         return;
@@ -848,7 +883,7 @@ __global__ __launch_bounds__(kSelThreads, 4) void filter_select_kernel(SelectArg
                 const u64 w = fixed(weight(K::to_float(border))), ties = (mass_target - before + w - 1) / w;
                 u64 count = 0;
                 each([&](uint32_t k, uint32_t, u64) TRLK_INLINE { count += k == border; });
-                if (ties < block_total(count, s.scan)) {
+                if (ties < block_total(count, s.slots[3])) {
                     before = 0;
                     descend(s, [&](auto put) TRLK_INLINE { each([&](uint32_t k, uint32_t e, u64) TRLK_INLINE { put(e, k == border); }); }, 0, uint32_t(V - 1), ties,
                             border_index, before);
@@ -868,7 +903,7 @@ __global__ __launch_bounds__(kSelThreads, 4) void filter_select_kernel(SelectArg
             const auto chunk_mass = [&](int i) TRLK_INLINE { return cmass[i] + s.bins[i]; };
             u64 sum = 0, up, W;
             for (int i = first; i < last; ++i) sum += chunk_mass(i);
-            const u64 exc = block_scan(sum, s.scan, up, W);
+            const u64 exc = block_scan(sum, s.slots[2], up, W);
             const double log2_mass = log2(double(W)) - a.fix;
             if constexpr (SCORE) {
                 scored(border, border_index, log2_mass);
@@ -891,7 +926,7 @@ __global__ __launch_bounds__(kSelThreads, 4) void filter_select_kernel(SelectArg
                     w[j] = v[j] > -INFINITY && kept(K::of_float(v[j]), uint32_t(e0 + j)) ? fixed(weight(v[j])) : 0;
                     part += w[j];
                 }
-                run += block_scan(part, s.scan, up, all);
+                run += block_scan(part, s.slots[3], up, all);
 #pragma unroll
                 for (int j = 0; j < PER; ++j) {
                     if (w[j] && run <= target && run + w[j] > target) drawn(e0 + j, v[j], log2_mass);
@@ -943,7 +978,7 @@ __global__ __launch_bounds__(kSelThreads, 4) void filter_select_kernel(SelectArg
             each([&](uint32_t k, uint32_t, auto w) TRLK_INLINE {
                 if (k > border) mass += w();
             });
-            mass = block_total(mass, s.scan);
+            mass = block_total(mass, s.slots[1]);
             if (border) mass += ties * fixed(weight(K::to_float(border)));
             const double t = __builtin_ceil(f.top_p * double(mass));
             target = t < 1.0 ? u64(1) : u64(int64_t(t));
@@ -964,7 +999,7 @@ __global__ __launch_bounds__(kSelThreads, 4) void filter_select_kernel(SelectArg
     if (border) {
         u64 count = 0;
         each([&](uint32_t k, uint32_t, auto) TRLK_INLINE { count += k == border; });
-        if (ties < block_total(count, s.scan)) {
+        if (ties < block_total(count, s.slots[3])) {
             const uint32_t b = border;
             before = 0;
             descend(s, [&](auto put) TRLK_INLINE { each([&](uint32_t k, uint32_t e, auto) TRLK_INLINE { put(e, k == b); }); }, 0, uint32_t(V - 1), ties,
@@ -981,7 +1016,7 @@ __global__ __launch_bounds__(kSelThreads, 4) void filter_select_kernel(SelectArg
     each([&](uint32_t k, uint32_t e, auto w) TRLK_INLINE {
         if (kept(k, e)) W += w();
     });
-    W = block_total(W, s.scan);
+    W = block_total(W, s.slots[2]);
     const double log2_mass = log2(double(W)) - a.fix;
     if constexpr (SCORE) {
         scored(border, border_index, log2_mass);

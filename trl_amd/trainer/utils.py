@@ -106,6 +106,8 @@ def entropy_from_logits(logits: Tensor, chunk_size: int = 128, out_dtype: torch.
 # ----------------------------------------------------------------------------------------------
 def _settings(shape: torch.Size, temperature, top_k, top_p, min_p) -> tuple:
     """The four settings as the operators take them: numbers, and tensors (or None) with a value for each row."""
+    if type(temperature) is float and type(top_k) is int and type(top_p) is float and type(min_p) is float:
+        return temperature, top_k, top_p, min_p, None, None, None, None
     numbers, tensors = [], []
     for name, value, off in (("temperature", temperature, 1.0), ("top_k", top_k, 0), ("top_p", top_p, 1.0), ("min_p", min_p, 0.0)):
         if isinstance(value, Tensor) and (value.dim() or value.is_cuda):
