@@ -26,8 +26,9 @@ constexpr int kSelThreads = 512;
 constexpr int kSelWaves = kSelThreads / kWave;
 constexpr int kBins = 4 * kSelThreads;       // of a step of the descent
 constexpr int kBinBits = 11;
-constexpr int kCandidates = 2048;            // that are kept in LDS; rows with more read their blocks again in every step
-constexpr int kList = 2048;                  // blocks over the bound that are listed; with more every block is looked at
+constexpr int kCandidates = 4096;            // that are kept in LDS; rows with more read their blocks again in every step
+constexpr int kList = 4096;                  // blocks over the bound that are listed; with more every block is looked at
+constexpr int kPairs = 256;                  // candidates of which every pair is compared
 constexpr int64_t kMaxVocab = int64_t(1) << 22;
 
 typedef unsigned long long u64;
@@ -53,11 +54,31 @@ __device__ __forceinline__ double exp2_f64(double t) {
     return __builtin_amdgcn_ldexp(y, int(n));
 }
 
-// The same for sums, where what underflows may count 2^-1000: n comes from the low bits of t + 1.5 * 2^52 and goes into the exponent
-// with one integer addition (rounding, conversion and ldexp of 64-bit numbers run at a quarter of the rate of the products).
-__device__ __forceinline__ double exp2_sum(double t) {
-    t = __builtin_fmax(t, -1000.0);
-    const double big = t + 0x1.8p52, f = t - (big - 0x1.8p52);
+// What a chunk's sum of weights is measured in.  Ordinarily 2^exponent, a whole number of at least max * c: x * c - exponent then needs one
+// rounding, n comes from the low bits of x * c - exponent + 1.5 * 2^52 and goes into the result with one integer addition.  Where
+// max * c is too large for that, or neighbouring logits are so far apart that the clamp against underflow would not hold, the
+// chunk's maximum itself, by subtraction.
+struct ChunkUnit {
+    double exponent;
+    float x_min;  // logits under it count as it (2^-1000 at most)
+    bool whole;
+};
+__device__ __forceinline__ ChunkUnit chunk_unit(float m, double c) {
+    ChunkUnit u;
+    u.exponent = m > -INFINITY ? __builtin_ceil(double(m) * c) : 0.0;
+    u.x_min = float((u.exponent - 1000.0) / c);
+    const double t = __builtin_fma(double(u.x_min), c, -u.exponent);
+    u.whole = u.exponent > -0x1p40 && u.exponent < 0x1p40 && t < -900.0 && t > -1020.0;
+    return u;
+}
+// log2 of the unit of a chunk with maximum m, relative to a row's maximum
+__device__ __forceinline__ double chunk_scale(float m, double c, double ref) {
+    const ChunkUnit u = chunk_unit(m, c);
+    return m == -INFINITY ? -INFINITY : u.whole ? -__builtin_fma(ref, c, -u.exponent) : (double(m) - ref) * c;
+}
+// 2^(x * c - unit's exponent), 0.7 at the lowest x_min's 2^-1000: 16 operations of 64 bits, all of the full rate
+__device__ __forceinline__ double exp2_whole(float x, double c, double magic) {
+    const double v = double(x), big = __builtin_fma(v, c, magic), f = __builtin_fma(v, c, magic - big);
     double y = 1.0205905413765595e-07;
     y = __builtin_fma(y, f, 1.325964524488711e-06);
     y = __builtin_fma(y, f, 1.5252672924850737e-05);
@@ -68,8 +89,9 @@ __device__ __forceinline__ double exp2_sum(double t) {
     y = __builtin_fma(y, f, 0.2402265069564034);
     y = __builtin_fma(y, f, 0.6931471805599462);
     y = __builtin_fma(y, f, 1.0);
-    const uint32_t n = uint32_t(__builtin_bit_cast(uint64_t, big));
-    return __builtin_bit_cast(double, __builtin_bit_cast(uint64_t, y) + (uint64_t(n) << 52));
+    const uint64_t bits = __builtin_bit_cast(uint64_t, y);
+    const uint32_t hi = uint32_t(bits >> 32) + (uint32_t(__builtin_bit_cast(uint64_t, big)) << 20);
+    return __builtin_bit_cast(double, uint64_t(hi) << 32 | uint32_t(bits));
 }
 
 // maximum that lets a NaN through
@@ -225,10 +247,17 @@ __global__ __launch_bounds__(kScanThreads) void filter_scan_kernel(ScanArgs a) {
     }
     m = wave_max_nan(m);
     if constexpr (SUMS) {
-        const double c = row_filter(a.f, row, a.x.vocab).c, ref = m > -INFINITY && m < INFINITY ? double(m) : 0.0;
+        const double c = row_filter(a.f, row, a.x.vocab).c;
+        const ChunkUnit in = chunk_unit(m, c);
         double s = 0.0;
+        if (in.whole) {
+            const double magic = 0x1.8p52 - in.exponent;
 #pragma unroll
-        for (int j = 0; j < NV * EPV; ++j) s += exp2_sum((double(x[j]) - ref) * c);
+            for (int j = 0; j < NV * EPV; ++j) s += exp2_whole(fmaxf(x[j], in.x_min), c, magic);
+        } else {
+#pragma unroll
+            for (int j = 0; j < NV * EPV; ++j) s += exp2_f64((double(x[j]) - double(m)) * c);
+        }
 #pragma unroll
         for (int o = kWave / 2; o > 0; o >>= 1) s += __shfl_xor(s, o);
         if (lane == 0) a.chunk_sum[unit] = s;
@@ -285,13 +314,10 @@ union WaveSlots {
 __device__ __forceinline__ u64& slot_of(WaveSlots& s, int i, u64) { return s.u[i]; }
 __device__ __forceinline__ double& slot_of(WaveSlots& s, int i, double) { return s.f[i]; }
 
-struct alignas(16) Candidate {
-    u64 order;  // key above, ~index below: larger is earlier
-    u64 weight;
-};
 struct SelectShared {
     u64 bins[kBins];
-    Candidate cand[kCandidates];
+    u64 order[kCandidates];  // of the candidates: key above, ~index below, larger is earlier
+    u64 weight[kPairs];
     uint16_t list[kList];
     WaveSlots slots[4];
     float wave_f[kSelWaves];
@@ -469,10 +495,11 @@ __global__ __launch_bounds__(kSelThreads, 4) void filter_select_kernel(SelectArg
         for (int i = tid; i < a.chunks; i += kSelThreads) m = max_nan(m, cmax[i]);
     }
     const int per = (a.chunks + kSelThreads - 1) / kSelThreads, first = tid * per, last = first + per < a.chunks ? first + per : a.chunks;
-    double sum0 = 0.0, max0 = 0.0;  // this thread's first chunk, loaded beside the maxima
+    double sum0 = 0.0;  // this thread's first chunk, loaded beside the maxima
+    float max0 = -INFINITY;
     if (with_sum && first < last) {
         sum0 = csum[first];
-        max0 = double(cmax[first]);
+        max0 = cmax[first];
     }
     int64_t token = 0;
     bool token_ok = true;
@@ -505,8 +532,8 @@ __global__ __launch_bounds__(kSelThreads, 4) void filter_select_kernel(SelectArg
         return nothing(-1, NAN);
     }
     const double c = f.c, ref = double(m), unit = __builtin_amdgcn_ldexp(1.0, a.fix);
-    const auto weight_at = [&](double v) TRLK_INLINE { return exp2_f64((v - ref) * c); };
-    const auto weight = [&](float v) TRLK_INLINE { return weight_at(double(v)); };
+    const auto weight = [&](float v) TRLK_INLINE { return exp2_f64((double(v) - ref) * c); };
+    const auto chunk_weight = [&](double sum, float chunk_m) TRLK_INLINE { return sum * exp2_f64(chunk_scale(chunk_m, c, ref)); };
     const auto fixed = [&](double w) TRLK_INLINE { return u64(int64_t(__builtin_rint(w * unit))); };
     const auto drawn = [&](int64_t id, float v, double log2_mass) TRLK_INLINE {  // one thread
         a.out_ids[row] = id;
@@ -533,8 +560,8 @@ __global__ __launch_bounds__(kSelThreads, 4) void filter_select_kernel(SelectArg
     // the row's sum of weights, and this thread's chunks' place in it
     double S = 0.0, mine = 0.0, base = 0.0, upto = 0.0;
     if (with_sum) {
-        if (first < last) mine = sum0 * weight_at(max0);
-        for (int i = first + 1; i < last; ++i) mine += csum[i] * weight(cmax[i]);
+        if (first < last) mine = chunk_weight(sum0, max0);
+        for (int i = first + 1; i < last; ++i) mine += chunk_weight(csum[i], cmax[i]);
         base = block_scan(mine, s.slots[1], upto, S);
     }
     // ---- no filter: the chunk, then the token in it
@@ -547,7 +574,7 @@ __global__ __launch_bounds__(kSelThreads, 4) void filter_select_kernel(SelectArg
             const double target = u * S;
             const int owner = first_thread(s, 0, mine > 0.0 && upto > target, mine > 0.0);
             if (tid == owner) {
-                double at = base, v = sum0 * weight_at(max0);
+                double at = base, v = chunk_weight(sum0, max0);
                 int chunk = first, some = v > 0.0 ? first : -1;
                 double some_at = at;
                 for (;;) {
@@ -558,7 +585,7 @@ __global__ __launch_bounds__(kSelThreads, 4) void filter_select_kernel(SelectArg
                     }
                     at += v;
                     if (++chunk >= last) break;
-                    v = csum[chunk] * weight(cmax[chunk]);
+                    v = chunk_weight(csum[chunk], cmax[chunk]);
                 }
                 s.border = uint32_t(some);
                 s.prefix[0] = some_at;
@@ -658,55 +685,70 @@ __global__ __launch_bounds__(kSelThreads, 4) void filter_select_kernel(SelectArg
     __syncthreads();
     const bool listed = s.n_list <= kList;
     const int n_visit = listed ? int(s.n_list) : n_blocks;
-    // all logits over the bound, a wave to a block, eight blocks in flight: g(in, value, key, index), with all lanes of the wave in it
+    // all logits over the bound, EPV blocks to a load of a wave: g(in, value, key, index), with all lanes of the wave in it
     const auto stream = [&](auto g) TRLK_INLINE {
-        constexpr int U = 8;
-        for (int j0 = wave; j0 < n_visit; j0 += U * kSelWaves) {
-            T raw[U];
+        constexpr int LPB = kBlock / EPV, U = 2;
+        for (int j0 = wave * EPV; j0 < n_visit; j0 += U * kSelWaves * EPV) {
+            u32x4 raw[U];
             int64_t e[U];
 #pragma unroll
             for (int q = 0; q < U; ++q) {
-                const int j = j0 + q * kSelWaves;
-                e[q] = j < n_visit ? int64_t(listed ? int(s.list[j]) : j) * kBlock + lane : V;
-                raw[q] = e[q] < V ? x[e[q]] : T(0);
+                const int j = j0 + q * kSelWaves * EPV + lane / LPB;
+                e[q] = j < n_visit ? int64_t(listed ? int(s.list[j]) : j) * kBlock + (lane & (LPB - 1)) * EPV : V;
+                if (e[q] + EPV <= V) {
+                    raw[q] = *reinterpret_cast<const u32x4_u*>(x + e[q]);
+                } else {
+                    float v[EPV];
+#pragma unroll
+                    for (int k = 0; k < EPV; ++k) v[k] = e[q] + k < V ? Elem<DT>::load1(x + e[q] + k) : -INFINITY;
+                    raw[q] = Elem<DT>::pack(v);
+                }
             }
 #pragma unroll
             for (int q = 0; q < U; ++q) {
-                const float v = Elem<DT>::to_float(raw[q]);
-                g(e[q] < V && in_bound(v), v, K::of(raw[q]), uint32_t(e[q]));
+                float v[EPV];
+                Elem<DT>::unpack(raw[q], v);
+#pragma unroll
+                for (int k = 0; k < EPV; ++k) g(in_bound(v[k]), v[k], uint32_t(e[q]) + k);
             }
         }
     };
     const bool too_many = !listed && !f.top_k;  // (kList blocks have as many candidates at least)
     if (!too_many) {
-        uint32_t min_key = ~0u, low_key = ~0u;
-        stream([&](bool in, float v, uint32_t k, uint32_t e) TRLK_INLINE {
+        stream([&](bool in, float v, uint32_t e) TRLK_INLINE {
             const u64 vote = __ballot(in);
             if (!vote) return;
             uint32_t to = 0;
             if (lane == 0) to = atomicAdd(&s.n_cand, uint32_t(__popcll(vote)));
             to = __shfl(to, 0) + __popcll(vote & ((u64(1) << lane) - 1));
-            if (in) {
-                const double w = weight(v);
-                if (w >= f.min_p && k < min_key) min_key = k;
-                if (k < low_key) low_key = k;
-                if (to < kCandidates) s.cand[to] = Candidate{u64(k) << 32 | (~e & 0xffffffffu), fixed(w)};
-            }
+            if (in && to < kCandidates) s.order[to] = u64(K::of_float(v)) << 32 | uint32_t(~e);
         });
-#pragma unroll
-        for (int o = kWave / 2; o > 0; o >>= 1) {
-            const uint32_t p = __shfl_xor(min_key, o), q = __shfl_xor(low_key, o);
-            min_key = p < min_key ? p : min_key;
-            low_key = q < low_key ? q : low_key;
-        }
-        if (lane == 0) {
-            atomicMin(&s.min_key, min_key);
-            atomicMin(&s.low_key, low_key);
-        }
         __syncthreads();
     }
     const int n_cand = too_many ? kCandidates + 1 : int(s.n_cand);
-    uint32_t kept_from = f.min_p > 0.0 ? s.min_key : 0u;  // the smallest key that min-p keeps
+    const auto key_of = [&](u64 order) TRLK_INLINE { return uint32_t(order >> 32); };
+    const auto index_of = [&](u64 order) TRLK_INLINE { return ~uint32_t(order); };
+    const auto key_weight = [&](uint32_t k) TRLK_INLINE { return weight(K::to_float(k)); };
+    // the smallest of the threads' keys, in a word that was ~0
+    const auto smallest = [&](uint32_t& word, uint32_t k) TRLK_INLINE {
+#pragma unroll
+        for (int o = kWave / 2; o > 0; o >>= 1) {
+            const uint32_t p = __shfl_xor(k, o);
+            k = p < k ? p : k;
+        }
+        if (lane == 0) atomicMin(&word, k);
+        __syncthreads();
+        return word;
+    };
+    uint32_t kept_from = 0;  // the smallest key that min-p keeps
+    if (f.min_p > 0.0 && n_cand <= kCandidates) {
+        uint32_t k = ~0u;
+        for (int i = tid; i < n_cand; i += kSelThreads) {
+            const uint32_t q = key_of(s.order[i]);
+            if (q < k && key_weight(q) >= f.min_p) k = q;
+        }
+        kept_from = smallest(s.min_key, k);
+    }
 
     // the integer that a cumulative weight has to pass, and whether it is none (the first kept token passes it then, also one whose
     // weight is less than a unit)
@@ -717,14 +759,16 @@ __global__ __launch_bounds__(kSelThreads, 4) void filter_select_kernel(SelectArg
     };
 
     // ---- up to 256 candidates: every pair is compared, which gives each one its rank and the mass before it
-    constexpr int kPairs = 256;
     if (n_cand <= kPairs) {
         // (`parts` neighbouring lanes have a candidate together, and each compares it with its part of all; the sums stay in the wave)
         const int lp = n_cand <= 64 ? 3 : n_cand <= 128 ? 2 : 1, parts = 1 << lp, np = kSelThreads >> lp, len = np >> lp;
         const int i = tid >> lp, part = tid & (parts - 1);
-        if (tid >= n_cand && tid < np) s.cand[tid] = Candidate{0, 0};
+        if (tid < np) {
+            if (tid >= n_cand) s.order[tid] = 0;
+            s.weight[tid] = tid < n_cand ? fixed(key_weight(key_of(s.order[tid]))) : 0;
+        }
         __syncthreads();
-        const Candidate me = s.cand[i];
+        const u64 me = s.order[i], my_weight = s.weight[i];
         const bool real = i < n_cand && part == 0;
         const auto over_parts = [&](u64 v) TRLK_INLINE {
             v += moved<0xb1, 0xf>(v);                 // the neighbour
@@ -734,9 +778,8 @@ __global__ __launch_bounds__(kSelThreads, 4) void filter_select_kernel(SelectArg
         };
         u64 before = 0, rank = 0;
         for (int j = 0; j < len; ++j) {
-            const Candidate o = s.cand[j * parts + part];
-            const bool earlier = o.order > me.order;
-            before += earlier ? o.weight : 0;
+            const bool earlier = s.order[j * parts + part] > me;
+            before += earlier ? s.weight[j * parts + part] : 0;
             rank += earlier ? 1 : 0;
         }
         before = over_parts(before);
@@ -745,36 +788,35 @@ __global__ __launch_bounds__(kSelThreads, 4) void filter_select_kernel(SelectArg
         if (f.top_p > 0.0) {
             u64 target = mass_target;
             if (f.top_k) {
-                const u64 W1 = block_total(kept ? me.weight : 0, s.slots[1]);
+                const u64 W1 = block_total(kept ? my_weight : 0, s.slots[1]);
                 const double t = __builtin_ceil(f.top_p * double(W1));
                 target = t < 1.0 ? u64(1) : u64(int64_t(t));
             }
             kept = kept && before < target;
         }
-        kept = kept && uint32_t(me.order >> 32) >= kept_from;
-        const u64 W = block_total(kept ? me.weight : 0, s.slots[2]);
+        kept = kept && key_of(me) >= kept_from;
+        const u64 W = block_total(kept ? my_weight : 0, s.slots[2]);
         const double log2_mass = log2(double(W)) - a.fix;
         if constexpr (SCORE) {
             const int n_kept = __syncthreads_count(kept);  // (a prefix of the order)
             if (real && int(rank) == n_kept - 1) {
-                s.border = uint32_t(me.order >> 32);
-                s.border_index = ~uint32_t(me.order);
+                s.border = key_of(me);
+                s.border_index = index_of(me);
             }
             __syncthreads();
             scored(s.border, s.border_index, log2_mass);
         } else {
             const u64 target = draw_target(W);
-            const u64 mine_w = kept ? (target ? me.weight : 1) : 0;
-            if (part == 0) s.cand[i].weight = mine_w;  // (everyone has read its own)
+            const u64 mine_w = kept ? (target ? my_weight : 1) : 0;
+            if (part == 0) s.weight[i] = mine_w;  // (everyone has read its own)
             __syncthreads();
-            const uint32_t my_index = ~uint32_t(me.order);
+            const uint32_t my_index = index_of(me);
             u64 cum = 0;
             for (int j = 0; j < len; ++j) {
-                const Candidate o = s.cand[j * parts + part];
-                cum += ~uint32_t(o.order) <= my_index ? o.weight : 0;
+                cum += index_of(s.order[j * parts + part]) <= my_index ? s.weight[j * parts + part] : 0;
             }
             cum = over_parts(cum);
-            if (kept && cum > target && cum - mine_w <= target) drawn(my_index, K::to_float(uint32_t(me.order >> 32)), log2_mass);
+            if (kept && cum > target && cum - mine_w <= target) drawn(my_index, K::to_float(key_of(me)), log2_mass);
         }
         return;
     }
@@ -782,8 +824,9 @@ __global__ __launch_bounds__(kSelThreads, 4) void filter_select_kernel(SelectArg
     const uint32_t top = K::of_float(m), lowest = K::of_float(-INFINITY) + 1u;
     uint32_t border = 0, border_index = ~0u, at;
     u64 before = 0;
-    // ---- very many candidates, without top-k: two passes over the row.  The first adds the weights up in bins linear in the logit; the
-    // second sums, chunk by chunk, what lies before the border's bin, and lists that bin, where the border is then found.
+    // ---- very many candidates, without top-k: two passes over the row.  The first adds the weights up, in fp32 and rounded to 2^-31 of
+    // the sum, in bins linear in the logit: that tells the border's bin give or take one.  The second sums in 64 bits, chunk by chunk,
+    // what lies before those three bins, and lists what lies in them, where the border is then found.
     if (n_cand > kCandidates && !f.top_k && x_low > -INFINITY) {
         const float scale = float(kBins - 1) / fmaxf(m - x_low, 1e-30f);
         const auto bin_of = [&](float v) TRLK_INLINE {
@@ -818,19 +861,23 @@ __global__ __launch_bounds__(kSelThreads, 4) void filter_select_kernel(SelectArg
                 end(ch);
             }
         };
-        int border_bin = kBins;
+        int zone = kBins, zone_end = kBins;  // [zone, zone_end) has the border
         bool found = true;
         if (f.top_p > 0.0) {
             clear_bins(s, kBins);
+            const float cf = float(c), l2 = float(31.0 - log2(S));
             row_pass(
                 [&](float v, uint32_t) TRLK_INLINE {
-                    if (v >= x_low) atomicAdd(&s.bins[bin_of(v)], fixed(weight(v)));
+                    const uint32_t w = uint32_t(fast_exp2(fmaf(v - m, cf, l2)) + 0.5f);
+                    if (v >= x_low) atomicAdd(reinterpret_cast<uint32_t*>(&s.bins[bin_of(v)]), w);  // (all of them are less than 2^32)
                 },
                 [](int) TRLK_INLINE {});
             __syncthreads();
             uint32_t bin;
-            found = crossing(s, kBins, mass_target, bin, before);
-            border_bin = int(bin);
+            before = 0;
+            found = crossing(s, kBins, u64(f.top_p * 0x1p31) + 1, bin, before);
+            zone = int(bin) - 1;
+            zone_end = int(bin) + 2;
         }
         __syncthreads();
         if (tid == 0) {
@@ -839,54 +886,56 @@ __global__ __launch_bounds__(kSelThreads, 4) void filter_select_kernel(SelectArg
         }
         __syncthreads();
         u64* cmass = reinterpret_cast<u64*>(csum);
+        u64 all_mass = 0;
+        uint32_t min_key = ~0u;
         if (found) {
             u64 mass = 0;
-            uint32_t min_key = ~0u;
             row_pass(
                 [&](float v, uint32_t e) TRLK_INLINE {
                     const int b = v >= x_low ? bin_of(v) : kBins + 1;
-                    if (b > border_bin) return;
-                    const double w = weight(v);
+                    if (b >= zone_end) return;
+                    const double wd = weight(v);
+                    const u64 w = b < zone ? fixed(wd) : 0;
                     const uint32_t k = K::of_float(v);
-                    if (w >= f.min_p) {
-                        if (b < border_bin) mass += fixed(w);
+                    all_mass += w;
+                    if (wd >= f.min_p) {
+                        mass += w;
                         if (k < min_key) min_key = k;
                     }
-                    if (b == border_bin) {
+                    if (b >= zone) {
                         const uint32_t to = atomicAdd(&s.n_cand, 1u);
-                        if (to < kCandidates) s.cand[to] = Candidate{u64(k) << 32 | (~e & 0xffffffffu), fixed(w)};
+                        if (to < kCandidates) s.order[to] = u64(k) << 32 | uint32_t(~e);
                     }
                 },
                 [&](int ch) TRLK_INLINE {
-#pragma unroll
-                    for (int o = kWave / 2; o > 0; o >>= 1) mass += __shfl_xor(mass, o);
-                    if (lane == 0) cmass[ch] = mass;
+                    mass = wave_inclusive(mass);
+                    if (lane == kWave - 1) cmass[ch] = mass;
                     mass = 0;
                 });
-#pragma unroll
-            for (int o = kWave / 2; o > 0; o >>= 1) {
-                const uint32_t p = __shfl_xor(min_key, o);
-                min_key = p < min_key ? p : min_key;
-            }
-            if (lane == 0) atomicMin(&s.min_key, min_key);
         }
-        __syncthreads();
+        min_key = smallest(s.min_key, min_key);
+        all_mass = block_total(all_mass, s.slots[1]);
         const int n_bin = int(s.n_cand);
+        const auto each = [&](auto g) TRLK_INLINE {
+            for (int i = tid; i < n_bin; i += kSelThreads) g(key_of(s.order[i]), index_of(s.order[i]));
+        };
+        if (found && n_bin <= kCandidates && f.top_p > 0.0) {
+            before = all_mass;
+            found = before < mass_target &&
+                    descend(s, [&](auto put) TRLK_INLINE { each([&](uint32_t k, uint32_t) TRLK_INLINE { put(top - k, fixed(key_weight(k))); }); }, 0,
+                            top - lowest, mass_target, at, before);
+        }
         if (found && n_bin <= kCandidates) {
-            kept_from = f.min_p > 0.0 ? s.min_key : 0u;
-            const auto each = [&](auto g) TRLK_INLINE {
-                for (int i = tid; i < n_bin; i += kSelThreads) g(uint32_t(s.cand[i].order >> 32), ~uint32_t(s.cand[i].order), s.cand[i].weight);
-            };
+            kept_from = f.min_p > 0.0 ? min_key : 0u;
             if (f.top_p > 0.0) {
-                descend(s, [&](auto put) TRLK_INLINE { each([&](uint32_t k, uint32_t, u64 w) TRLK_INLINE { put(top - k, w); }); }, 0, top - lowest, mass_target, at, before);
                 border = top - at;
-                const u64 w = fixed(weight(K::to_float(border))), ties = (mass_target - before + w - 1) / w;
+                const u64 w = fixed(key_weight(border)), ties = (mass_target - before + w - 1) / w;
                 u64 count = 0;
-                each([&](uint32_t k, uint32_t, u64) TRLK_INLINE { count += k == border; });
+                each([&](uint32_t k, uint32_t) TRLK_INLINE { count += k == border; });
                 if (ties < block_total(count, s.slots[3])) {
                     before = 0;
-                    descend(s, [&](auto put) TRLK_INLINE { each([&](uint32_t k, uint32_t e, u64) TRLK_INLINE { put(e, k == border); }); }, 0, uint32_t(V - 1), ties,
-                            border_index, before);
+                    descend(s, [&](auto put) TRLK_INLINE { each([&](uint32_t k, uint32_t e) TRLK_INLINE { put(e, k == border); }); }, 0, uint32_t(V - 1),
+                            ties, border_index, before);
                 }
             }
             if (kept_from > border) {
@@ -894,10 +943,10 @@ __global__ __launch_bounds__(kSelThreads, 4) void filter_select_kernel(SelectArg
                 border_index = ~0u;
             }
             const auto kept = [&](uint32_t k, uint32_t e) TRLK_INLINE { return k > border || (k == border && e <= border_index); };
-            // the border's bin joins its chunks
+            // the kept ones of the zone join their chunks
             clear_bins(s, a.chunks);
-            each([&](uint32_t k, uint32_t e, u64 w) TRLK_INLINE {
-                if (kept(k, e)) atomicAdd(&s.bins[e / kChunk], w);
+            each([&](uint32_t k, uint32_t e) TRLK_INLINE {
+                if (kept(k, e)) atomicAdd(&s.bins[e / kChunk], fixed(key_weight(k)));
             });
             __syncthreads();
             const auto chunk_mass = [&](int i) TRLK_INLINE { return cmass[i] + s.bins[i]; };
@@ -935,34 +984,36 @@ __global__ __launch_bounds__(kSelThreads, 4) void filter_select_kernel(SelectArg
             }
             return;
         }
-        if (tid == 0) s.n_cand = kCandidates + 1;
-        __syncthreads();
     }
 
     // ---- the rest: radix descents over the candidates, in LDS or (more of them) read again in each step
     const bool in_lds = n_cand <= kCandidates;
-    if (!in_lds && f.min_p > 0.0) {  // (a row that came past the gathering has not seen its smallest kept key)
-        if (tid == 0) s.min_key = ~0u;
-        __syncthreads();
-        uint32_t min_key = ~0u;
-        stream([&](bool in, float v, uint32_t k, uint32_t) TRLK_INLINE {
-            if (in && weight(v) >= f.min_p && k < min_key) min_key = k;
+    uint32_t low_key = lowest;
+    if (in_lds) {
+        uint32_t k = ~0u;
+        for (int i = tid; i < n_cand; i += kSelThreads) k = key_of(s.order[i]) < k ? key_of(s.order[i]) : k;
+        low_key = smallest(s.low_key, k);
+    } else if (f.min_p > 0.0) {
+        uint32_t k = ~0u;
+        stream([&](bool in, float v, uint32_t) TRLK_INLINE {
+            if (in && weight(v) >= f.min_p && K::of_float(v) < k) k = K::of_float(v);
         });
-        if (min_key != ~0u) atomicMin(&s.min_key, min_key);
-        __syncthreads();
-        kept_from = s.min_key;
+        kept_from = smallest(s.low_key, k);
     }
     // g(key, index, weight()) for this thread's candidates
     const auto each = [&](auto g) TRLK_INLINE {
         if (in_lds) {
-            for (int i = tid; i < n_cand; i += kSelThreads) g(uint32_t(s.cand[i].order >> 32), ~uint32_t(s.cand[i].order), [&]() TRLK_INLINE { return s.cand[i].weight; });
+            for (int i = tid; i < n_cand; i += kSelThreads) {
+                const u64 o = s.order[i];
+                g(key_of(o), index_of(o), [&]() TRLK_INLINE { return fixed(key_weight(key_of(o))); });
+            }
         } else {
-            stream([&](bool in, float v, uint32_t k, uint32_t e) TRLK_INLINE {
-                if (in) g(k, e, [&]() TRLK_INLINE { return fixed(weight(v)); });
+            stream([&](bool in, float v, uint32_t e) TRLK_INLINE {
+                if (in) g(K::of_float(v), e, [&]() TRLK_INLINE { return fixed(weight(v)); });
             });
         }
     };
-    const uint32_t span = top - (in_lds ? s.low_key : lowest);
+    const uint32_t span = top - low_key;
     u64 ties = ~u64(0);  // how many tokens of the border's value are kept
     before = 0;
     if (f.top_k) {
@@ -979,7 +1030,7 @@ __global__ __launch_bounds__(kSelThreads, 4) void filter_select_kernel(SelectArg
                 if (k > border) mass += w();
             });
             mass = block_total(mass, s.slots[1]);
-            if (border) mass += ties * fixed(weight(K::to_float(border)));
+            if (border) mass += ties * fixed(key_weight(border));
             const double t = __builtin_ceil(f.top_p * double(mass));
             target = t < 1.0 ? u64(1) : u64(int64_t(t));
         }
@@ -991,7 +1042,7 @@ __global__ __launch_bounds__(kSelThreads, 4) void filter_select_kernel(SelectArg
                 });
             }, 0, span, target, at, before)) {
             const uint32_t b = top - at;
-            const u64 w = fixed(weight(K::to_float(b))), n = (target - before + w - 1) / w;
+            const u64 w = fixed(key_weight(b)), n = (target - before + w - 1) / w;
             ties = b == border && n > ties ? ties : n;
             border = b;
         }
