@@ -96,9 +96,44 @@ __device__ __forceinline__ double exp2_whole(float x, double c, double magic) {
 
 // maximum that lets a NaN through
 __device__ __forceinline__ float max_nan(float a, float b) { return __builtin_elementwise_maximum(a, b); }
+// v of the lane that differs in one bit of its number (1, 2), or that mirrors it in 8 or 16
+template <int CTRL>
+__device__ __forceinline__ float moved_f32(float v) {
+    return __uint_as_float(uint32_t(__builtin_amdgcn_mov_dpp(int(__float_as_uint(v)), CTRL, 0xf, 0xf, true)));
+}
+// maximum over groups of LANES neighbouring lanes (8 or 16)
+template <int LANES>
+__device__ __forceinline__ float group_max_nan(float v) {
+    v = max_nan(v, moved_f32<0xb1>(v));
+    v = max_nan(v, moved_f32<0x4e>(v));
+    v = max_nan(v, moved_f32<0x141>(v));
+    if constexpr (LANES == 16) v = max_nan(v, moved_f32<0x140>(v));
+    return v;
+}
 __device__ __forceinline__ float wave_max_nan(float v) {
-#pragma unroll
-    for (int o = kWave / 2; o > 0; o >>= 1) v = max_nan(v, __shfl_xor(v, o));
+    v = group_max_nan<16>(v);
+    v = max_nan(v, __shfl_xor(v, 16));
+    return max_nan(v, __shfl_xor(v, 32));
+}
+
+// A 64-bit value from the lane that the data-parallel primitive names, 0 where there is none.
+template <int CTRL, int ROWS, typename V>
+__device__ __forceinline__ V moved(V v) {
+    const uint64_t b = __builtin_bit_cast(uint64_t, v);
+    const uint32_t lo = uint32_t(__builtin_amdgcn_update_dpp(0, int(uint32_t(b)), CTRL, ROWS, 0xf, false));
+    const uint32_t hi = uint32_t(__builtin_amdgcn_update_dpp(0, int(uint32_t(b >> 32)), CTRL, ROWS, 0xf, false));
+    return __builtin_bit_cast(V, uint64_t(hi) << 32 | lo);
+}
+// Sums over the lanes up to each one: shifts within rows of 16 lanes, then the last lane of row 0 (2) to row 1 (3), that of row 1 to
+// rows 2 and 3.  A fifth of the time that six shuffles through LDS take.
+template <typename V>
+__device__ __forceinline__ V wave_inclusive(V v) {
+    v += moved<0x111, 0xf>(v);
+    v += moved<0x112, 0xf>(v);
+    v += moved<0x114, 0xf>(v);
+    v += moved<0x118, 0xf>(v);
+    v += moved<0x142, 0xa>(v);
+    v += moved<0x143, 0xc>(v);
     return v;
 }
 
@@ -171,9 +206,9 @@ struct RowView {
     const void* logits;
     int64_t rows_per_seq, vocab, seq_stride, row_stride;
     template <int DT>
-    __device__ __forceinline__ const typename Elem<DT>::type* row(int64_t r) const {
-        const int64_t b = r / rows_per_seq, t = r - b * rows_per_seq;
-        return static_cast<const typename Elem<DT>::type*>(logits) + b * seq_stride + t * row_stride;
+    __device__ __forceinline__ const typename Elem<DT>::type* row(uint32_t r) const {  // (rows are fewer than 2^31)
+        const uint32_t b = r / uint32_t(rows_per_seq), t = r - b * uint32_t(rows_per_seq);
+        return static_cast<const typename Elem<DT>::type*>(logits) + int64_t(b) * seq_stride + int64_t(t) * row_stride;
     }
 };
 
@@ -219,12 +254,13 @@ __global__ __launch_bounds__(kScanThreads) void filter_scan_kernel(ScanArgs a) {
     typedef typename Elem<DT>::type T;
     constexpr int EPV = Elem<DT>::EPV, NV = kChunk / (kWave * EPV), LPB = kBlock / EPV;  // LPB: lanes of a block
     const int lane = threadIdx.x & (kWave - 1);
-    const int64_t unit = __builtin_amdgcn_readfirstlane(int(blockIdx.x * (kScanThreads / kWave) + threadIdx.x / kWave));
-    const int64_t row = unit / a.chunks;
+    const uint32_t at_unit = __builtin_amdgcn_readfirstlane(int(blockIdx.x * (kScanThreads / kWave) + threadIdx.x / kWave));
+    const uint32_t at_row = at_unit / uint32_t(a.chunks);  // (units are fewer than 2^31)
+    const int64_t unit = at_unit, row = at_row;
     if (row >= a.rows) return;
-    const int chunk = int(unit - row * a.chunks);
+    const int chunk = int(at_unit - at_row * uint32_t(a.chunks));
     if (a.row_mask && a.row_mask[row] == 0) return;
-    const T* p = a.x.row<DT>(row) + int64_t(chunk) * kChunk;
+    const T* p = a.x.row<DT>(uint32_t(row)) + int64_t(chunk) * kChunk;
     float x[NV * EPV];
     load_vectors<DT, NV>(p, a.x.vocab - int64_t(chunk) * kChunk, lane, x);
     float m = -INFINITY, mine = 0.f;
@@ -234,8 +270,7 @@ __global__ __launch_bounds__(kScanThreads) void filter_scan_kernel(ScanArgs a) {
 #pragma unroll
         for (int e = 1; e < EPV; ++e) v = max_nan(v, x[i * EPV + e]);
         if constexpr (BLOCKS) {
-#pragma unroll
-            for (int o = 1; o < LPB; o <<= 1) v = max_nan(v, __shfl_xor(v, o));
+            v = group_max_nan<LPB>(v);
             if ((lane & (LPB - 1)) == i) mine = v;
         }
         m = max_nan(m, v);
@@ -258,9 +293,8 @@ __global__ __launch_bounds__(kScanThreads) void filter_scan_kernel(ScanArgs a) {
 #pragma unroll
             for (int j = 0; j < NV * EPV; ++j) s += exp2_f64((double(x[j]) - double(m)) * c);
         }
-#pragma unroll
-        for (int o = kWave / 2; o > 0; o >>= 1) s += __shfl_xor(s, o);
-        if (lane == 0) a.chunk_sum[unit] = s;
+        s = wave_inclusive(s);
+        if (lane == kWave - 1) a.chunk_sum[unit] = s;
     }
     if (lane == 0) a.chunk_max[unit] = m;
 }
@@ -285,26 +319,6 @@ struct SelectArgs {
     int32_t* error_flag;
 };
 
-// A 64-bit value from the lane that the data-parallel primitive names, 0 where there is none.
-template <int CTRL, int ROWS, typename V>
-__device__ __forceinline__ V moved(V v) {
-    const uint64_t b = __builtin_bit_cast(uint64_t, v);
-    const uint32_t lo = uint32_t(__builtin_amdgcn_update_dpp(0, int(uint32_t(b)), CTRL, ROWS, 0xf, false));
-    const uint32_t hi = uint32_t(__builtin_amdgcn_update_dpp(0, int(uint32_t(b >> 32)), CTRL, ROWS, 0xf, false));
-    return __builtin_bit_cast(V, uint64_t(hi) << 32 | lo);
-}
-// Sums over the lanes up to each one: shifts within rows of 16 lanes, then the last lane of row 0 (2) to row 1 (3), that of row 1 to
-// rows 2 and 3.  A fifth of the time that six shuffles through LDS take.
-template <typename V>
-__device__ __forceinline__ V wave_inclusive(V v) {
-    v += moved<0x111, 0xf>(v);
-    v += moved<0x112, 0xf>(v);
-    v += moved<0x114, 0xf>(v);
-    v += moved<0x118, 0xf>(v);
-    v += moved<0x142, 0xa>(v);
-    v += moved<0x143, 0xc>(v);
-    return v;
-}
 // A place for one number of each wave.  Two neighbouring block-wide sums take different ones, so that a barrier lies between a
 // place's readers and its next writers.
 union WaveSlots {
@@ -465,7 +479,7 @@ __global__ __launch_bounds__(kSelThreads, 4) void filter_select_kernel(SelectArg
     const RowFilter f = row_filter(a.f, row, V);
     const bool filtered = f.top_k || f.top_p > 0.0 || f.min_p > 0.0;
     const bool with_sum = !filtered || (f.top_p > 0.0 && !f.top_k);
-    const T* x = a.x.row<DT>(row);
+    const T* x = a.x.row<DT>(uint32_t(row));
     const float* cmax = a.chunk_max + row * a.chunks;
     double* csum = a.chunk_sum + row * a.chunks;
     const int n_blocks = a.chunks * kBlocksPerChunk, n_vec = n_blocks / EPV;  // (blocks behind the row's end are -inf)
@@ -833,29 +847,42 @@ __global__ __launch_bounds__(kSelThreads, 4) void filter_select_kernel(SelectArg
             const float t = (m - v) * scale;
             return t < float(kBins) ? int(t) : kBins;
         };
-        // g(value, index) for every logit, end(chunk) after a wave's chunk: a vector at a time, the next one in flight (rows of other kinds
-        // want the registers)
+        // g(value, index) for every logit, end(chunk) after a wave's chunk: 16 logits of a lane at a time, the next ones in flight
+        constexpr int G = 16 / EPV;
         const auto row_pass = [&](auto g, auto end) TRLK_INLINE {
-            for (int ch = wave; ch < a.chunks; ch += kSelWaves) {
-                const int64_t e0 = int64_t(ch) * kChunk;
-                const auto load = [&](int i) TRLK_INLINE -> u32x4 {
+            const auto load = [&](int64_t e0, u32x4(&q)[G]) TRLK_INLINE {
+#pragma unroll
+                for (int i = 0; i < G; ++i) {
                     const int64_t at = e0 + (i * kWave + lane) * EPV;
-                    if (at + EPV <= V) return *reinterpret_cast<const u32x4_u*>(x + at);
-                    float v[EPV];
+                    if (at + EPV <= V) {
+                        q[i] = *reinterpret_cast<const u32x4_u*>(x + at);
+                    } else {
+                        float v[EPV];
 #pragma unroll
-                    for (int e = 0; e < EPV; ++e) v[e] = at + e < V ? Elem<DT>::load1(x + at + e) : -INFINITY;
-                    return Elem<DT>::pack(v);
-                };
-                u32x4 next = load(0);
+                        for (int e = 0; e < EPV; ++e) v[e] = at + e < V ? Elem<DT>::load1(x + at + e) : -INFINITY;
+                        q[i] = Elem<DT>::pack(v);
+                    }
+                }
+            };
+            u32x4 next[G];
+            load(int64_t(wave) * kChunk, next);
+            for (int ch = wave; ch < a.chunks; ch += kSelWaves) {
 #pragma unroll 1
-                for (int i = 0; i < NV; ++i) {
-                    float v[EPV];
-                    Elem<DT>::unpack(next, v);
-                    if (i + 1 < NV) next = load(i + 1);
+                for (int h = 0; h < NV / G; ++h) {
+                    const uint32_t e0 = uint32_t(ch) * kChunk + h * 16 * kWave;
+                    u32x4 now[G];
 #pragma unroll
-                    for (int e = 0; e < EPV; ++e) {
-                        g(v[e], uint32_t(e0) + (i * kWave + lane) * EPV + e);
-                        __builtin_amdgcn_sched_barrier(0);
+                    for (int i = 0; i < G; ++i) now[i] = next[i];
+                    load(h + 1 < NV / G ? int64_t(e0) + 16 * kWave : int64_t(ch + kSelWaves) * kChunk, next);
+#pragma unroll
+                    for (int i = 0; i < G; ++i) {
+                        float v[EPV];
+                        Elem<DT>::unpack(now[i], v);
+#pragma unroll
+                        for (int e = 0; e < EPV; ++e) {
+                            g(v[e], e0 + (i * kWave + lane) * EPV + e);
+                            __builtin_amdgcn_sched_barrier(0);
+                        }
                     }
                 }
                 end(ch);
@@ -1105,10 +1132,11 @@ __global__ __launch_bounds__(kScanThreads) void filter_bwd_kernel(FilterBwdArgs 
     typedef typename Elem<DT>::type T;
     constexpr int EPV = Elem<DT>::EPV, NV = kChunk / (kWave * EPV), LPB = kBlock / EPV;
     const int lane = threadIdx.x & (kWave - 1);
-    const int64_t unit = __builtin_amdgcn_readfirstlane(int(blockIdx.x * (kScanThreads / kWave) + threadIdx.x / kWave));
-    const int64_t row = unit / a.chunks;
+    const uint32_t at_unit = __builtin_amdgcn_readfirstlane(int(blockIdx.x * (kScanThreads / kWave) + threadIdx.x / kWave));
+    const uint32_t at_row = at_unit / uint32_t(a.chunks);  // (units are fewer than 2^31)
+    const int64_t unit = at_unit, row = at_row;
     if (row >= a.rows) return;
-    const int chunk = int(unit - row * a.chunks);
+    const int chunk = int(at_unit - at_row * uint32_t(a.chunks));
     const int64_t V = a.x.vocab, e0 = int64_t(chunk) * kChunk;
     const int n = V - e0 < kChunk ? int(V - e0) : kChunk;
     const float g0 = a.g_logp[row];
@@ -1119,7 +1147,7 @@ __global__ __launch_bounds__(kScanThreads) void filter_bwd_kernel(FilterBwdArgs 
     const float g = float(double(g0) / temp), c = float(1.4426950408889634074 / temp);
     const bool active = bx < INFINITY && g0 != 0.f;
     const int token = active ? int(a.index[row] - e0) : -1;  // (within the row: the forward has looked)
-    const T* x = a.x.row<DT>(row) + e0;
+    const T* x = a.x.row<DT>(uint32_t(row)) + e0;
     T* out = static_cast<T*>(a.dlogits) + row * V + e0;
     const T* bmax = a.block_max ? static_cast<const T*>(a.block_max) + unit * kBlocksPerChunk : nullptr;
 #pragma unroll
