@@ -28,7 +28,7 @@ constexpr int kBins = 4 * kSelThreads;       // of a step of the descent
 constexpr int kBinBits = 11;
 constexpr int kCandidates = 4096;            // that are kept in LDS; rows with more read their blocks again in every step
 constexpr int kList = 4096;                  // blocks over the bound that are listed; with more every block is looked at
-constexpr int kPairs = 256;                  // candidates of which every pair is compared
+constexpr int kPairs = 128;                  // candidates of which every pair is compared
 constexpr int64_t kMaxVocab = int64_t(1) << 22;
 
 typedef unsigned long long u64;
@@ -135,6 +135,25 @@ __device__ __forceinline__ V wave_inclusive(V v) {
     v += moved<0x142, 0xa>(v);
     v += moved<0x143, 0xc>(v);
     return v;
+}
+
+__device__ __forceinline__ uint32_t wave_inclusive(uint32_t v) {
+    const auto add = [&](auto moved_of) TRLK_INLINE { v += uint32_t(moved_of(int(v))); };
+    add([](int x) TRLK_INLINE { return __builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, false); });
+    add([](int x) TRLK_INLINE { return __builtin_amdgcn_update_dpp(0, x, 0x112, 0xf, 0xf, false); });
+    add([](int x) TRLK_INLINE { return __builtin_amdgcn_update_dpp(0, x, 0x114, 0xf, 0xf, false); });
+    add([](int x) TRLK_INLINE { return __builtin_amdgcn_update_dpp(0, x, 0x118, 0xf, 0xf, false); });
+    add([](int x) TRLK_INLINE { return __builtin_amdgcn_update_dpp(0, x, 0x142, 0xa, 0xf, false); });
+    add([](int x) TRLK_INLINE { return __builtin_amdgcn_update_dpp(0, x, 0x143, 0xc, 0xf, false); });
+    return v;
+}
+// A place for each of a wave's items in a list in LDS: `count` of this lane, all lanes in it.
+__device__ __forceinline__ uint32_t reserve(uint32_t* size, uint32_t count) {
+    const uint32_t inc = wave_inclusive(count), total = uint32_t(__builtin_amdgcn_readlane(int(inc), kWave - 1));
+    if (total == 0) return 0;
+    uint32_t base = 0;
+    if ((threadIdx.x & (kWave - 1)) == kWave - 1) base = atomicAdd(size, total);
+    return uint32_t(__builtin_amdgcn_readlane(int(base), kWave - 1)) + inc - count;
 }
 
 // Unsigned numbers in the order of the values (16 bits for 16-bit types).  -0 comes right before +0: they are different keys of
@@ -331,14 +350,14 @@ __device__ __forceinline__ double& slot_of(WaveSlots& s, int i, double) { return
 struct SelectShared {
     u64 bins[kBins];
     u64 order[kCandidates];  // of the candidates: key above, ~index below, larger is earlier
-    u64 weight[kPairs];
+    u64 weight[kPairs], zone[kPairs];
     uint16_t list[kList];
     WaveSlots slots[4];
     float wave_f[kSelWaves];
     int hit[2][kSelWaves], tail[2][kSelWaves];
     double prefix[kSelWaves];
     u64 before;
-    uint32_t bin, n_list, n_cand, min_key, low_key, border, border_index;
+    uint32_t bin, n_list, n_cand, n_zone, min_key, low_key, border, border_index;
 };
 
 // Sums over the threads before this one (returned) and up to it (`upto`), and over all.  What one thread's `upto` is, is the next
@@ -371,9 +390,11 @@ __device__ __forceinline__ u64 block_total(u64 v, WaveSlots& slots) {
     return r;
 }
 
-// The bin up to which the values of bins [0, n) and `before` reach `target` first, and in `before` what lies before it; false if
-// all of them do not.  The bins are complete and the barrier behind them passed; s.bin is ~0.  Contains two barriers.
-__device__ __forceinline__ bool crossing(SelectShared& s, int n, u64 target, uint32_t& bin, u64& before) {
+// The bin up to which the values of bins [0, n) and `before` reach a target first, and in `before` what lies before it; false if
+// all of them do not.  The target comes from the sum of all bins.  The bins are complete and the barrier behind them passed; s.bin
+// is ~0.  Contains two barriers.
+template <typename Target>
+__device__ __forceinline__ bool crossing_of(SelectShared& s, int n, Target target_of, uint32_t& bin, u64& before) {
     u64 v[4], sum = 0, upto, total;
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
@@ -382,6 +403,7 @@ __device__ __forceinline__ bool crossing(SelectShared& s, int n, u64 target, uin
         sum += v[j];
     }
     u64 at = before + block_scan(sum, s.slots[0], upto, total);
+    const u64 target = target_of(total);
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
         if (at < target && at + v[j] >= target) {  // (one bin of one thread)
@@ -396,12 +418,61 @@ __device__ __forceinline__ bool crossing(SelectShared& s, int n, u64 target, uin
     before = s.before;
     return true;
 }
+__device__ __forceinline__ bool crossing(SelectShared& s, int n, u64 target, uint32_t& bin, u64& before) {
+    return crossing_of(s, n, [&](u64) TRLK_INLINE { return target; }, bin, before);
+}
 // all bins 0 and no crossing yet, behind a barrier
 __device__ __forceinline__ void clear_bins(SelectShared& s, int n) {
     for (int i = threadIdx.x; i < n; i += kSelThreads) s.bins[i] = 0;
     __syncthreads();
     if (threadIdx.x == 0) s.bin = ~0u;  // (everyone has read the last one, and two barriers lie before the next is written)
 }
+
+// The first n <= kPairs entries of an order and their weights in LDS, each compared with every other one: what comes before it in the
+// order (of its bits under `mask`; larger is earlier), how many and of which weight.  `parts` neighbouring lanes have an entry
+// together and a part of the others each; the first of them goes on with it.  Up to np entries behind the n are overwritten;
+// contains one barrier, after which both arrays may be read.
+struct Ranked {
+    u64 order, weight, before;
+    uint32_t rank;
+    bool real;
+};
+__device__ __forceinline__ Ranked rank_pairs(u64* order, u64* weight, int n, u64 mask) {
+    const int tid = threadIdx.x, lp = n <= 64 ? 3 : 2, parts = 1 << lp, np = kSelThreads >> lp, len = np >> lp;
+    const int i = tid >> lp, part = tid & (parts - 1);
+    if (tid >= n && tid < np) order[tid] = weight[tid] = 0;
+    __syncthreads();
+    Ranked r;
+    r.order = order[i];
+    r.weight = weight[i];
+    r.real = i < n && part == 0;
+    const u64 me = r.order & mask;
+    u64 before = 0, rank = 0;
+    for (int j0 = 0; j0 < len; j0 += 8) {
+        u64 o[8], w[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            o[j] = order[(j0 + j) * parts + part];
+            w[j] = weight[(j0 + j) * parts + part];
+        }
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const bool earlier = (o[j] & mask) > me;
+            before += earlier ? w[j] : 0;
+            rank += earlier ? 1 : 0;
+        }
+    }
+    const auto over_parts = [&](u64 v) TRLK_INLINE {
+        v += moved<0xb1, 0xf>(v);                  // the neighbour
+        v += moved<0x4e, 0xf>(v);                  // the other pair of four
+        if (parts > 4) v += moved<0x141, 0xf>(v);  // the mirrored lane of eight
+        return v;
+    };
+    r.before = over_parts(before);
+    r.rank = uint32_t(over_parts(rank));
+    return r;
+}
+constexpr u64 kByOrder = ~u64(0), kByIndex = 0xffffffffu;
 
 // The smallest position in [lo, hi] up to which `before` and the values reach `target`, and in `before` what lies before it.
 // `each(f)` calls f(position, value) for this thread's share of the items.  False if all of them do not reach it.
@@ -486,7 +557,7 @@ __global__ __launch_bounds__(kSelThreads, 4) void filter_select_kernel(SelectArg
     const u32x4* bmax = reinterpret_cast<const u32x4*>(static_cast<const T*>(a.block_max) + row * n_blocks);
 
     // block maxima (chunk maxima where there are no others) and the row's maximum
-    u32x4 held[kKeep];
+    u32x4 held[kKeep] = {};
     float m = -INFINITY;
     if (filtered) {
 #pragma unroll
@@ -534,7 +605,7 @@ __global__ __launch_bounds__(kSelThreads, 4) void filter_select_kernel(SelectArg
     m = wave_max_nan(m);
     if (lane == 0) s.wave_f[wave] = m;
     if (tid == 0) {
-        s.n_list = s.n_cand = 0;
+        s.n_list = s.n_cand = s.n_zone = 0;
         s.min_key = s.low_key = s.bin = ~0u;
     }
     __syncthreads();
@@ -549,12 +620,14 @@ __global__ __launch_bounds__(kSelThreads, 4) void filter_select_kernel(SelectArg
     const auto weight = [&](float v) TRLK_INLINE { return exp2_f64((double(v) - ref) * c); };
     const auto chunk_weight = [&](double sum, float chunk_m) TRLK_INLINE { return sum * exp2_f64(chunk_scale(chunk_m, c, ref)); };
     const auto fixed = [&](double w) TRLK_INLINE { return u64(int64_t(__builtin_rint(w * unit))); };
+    const auto log2_of = [&](u64 W) TRLK_INLINE { return log2(double(W)) - a.fix; };
     const auto drawn = [&](int64_t id, float v, double log2_mass) TRLK_INLINE {  // one thread
         a.out_ids[row] = id;
         a.out_logp[row] = float(((double(v) - ref) * c - log2_mass) * 0.69314718055994530942);
     };
-    const auto scored = [&](uint32_t border, uint32_t border_index, double log2_mass) TRLK_INLINE {  // all threads
+    const auto scored = [&](uint32_t border, uint32_t border_index, auto mass) TRLK_INLINE {  // all threads
         if (tid != 0) return;
+        const double log2_mass = mass();
         float logp = NAN;
         bool inside = false;
         if (token_ok) {
@@ -581,7 +654,7 @@ __global__ __launch_bounds__(kSelThreads, 4) void filter_select_kernel(SelectArg
     // ---- no filter: the chunk, then the token in it
     if (!filtered) {
         if constexpr (SCORE) {
-            return scored(0, ~0u, log2(S));
+            return scored(0, ~0u, [&]() TRLK_INLINE { return log2(S); });
         } else {
             // (u * S can round up to the whole sum, and the last bits of a scan are not monotone: the first thread whose sum passes it,
             // and that has something, or the last one that has)
@@ -639,18 +712,26 @@ __global__ __launch_bounds__(kSelThreads, 4) void filter_select_kernel(SelectArg
     }
 
     // ---- a bound under the border, in bins of the distance from the maximum
-    const auto each_max = [&](auto g) TRLK_INLINE {  // g(block, value)
+    const auto key_of = [&](u64 order) TRLK_INLINE { return uint32_t(order >> 32); };
+    const auto index_of = [&](u64 order) TRLK_INLINE { return ~uint32_t(order); };
+    const auto order_of = [&](float v, uint32_t e) TRLK_INLINE { return u64(K::of_float(v)) << 32 | uint32_t(~e); };
+    const auto key_weight = [&](uint32_t k) TRLK_INLINE { return weight(K::to_float(k)); };
+    const auto each_max = [&](auto g) TRLK_INLINE {  // g(vector, its values), all lanes of a wave together; there may be none (-inf)
         const auto vec = [&](int i, u32x4 q) TRLK_INLINE {
             float v[EPV];
             Elem<DT>::unpack(q, v);
 #pragma unroll
-            for (int e = 0; e < EPV; ++e) g(i * EPV + e, v[e]);
+            for (int e = 0; e < EPV; ++e) v[e] = i < n_vec ? v[e] : -INFINITY;
+            g(i, v);
         };
 #pragma unroll
-        for (int j = 0; j < kKeep; ++j)
-            if (tid + j * kSelThreads < n_vec) vec(tid + j * kSelThreads, held[j]);
-        for (int i = tid + kKeep * kSelThreads; i < n_vec; i += kSelThreads) vec(i, bmax[i]);
+        for (int j = 0; j < kKeep; ++j) vec(tid + j * kSelThreads, held[j]);
+        for (int i = kKeep * kSelThreads; i < n_vec; i += kSelThreads) vec(i + tid, i + tid < n_vec ? bmax[i + tid] : u32x4{0, 0, 0, 0});
     };
+    // weights in fp32, in units of 2^-31 of the row's sum (off by 1e-5 at most, and half a unit): they narrow down, nothing is decided by them
+    const float cf = float(c), l2 = 31.f - __builtin_amdgcn_logf(float(S));
+    const auto about = [&](float v) TRLK_INLINE { return uint32_t(fast_exp2(fmaf(v - m, cf, l2)) + 0.5f); };
+    const auto add_low = [&](int bin, uint32_t v) TRLK_INLINE { atomicAdd(reinterpret_cast<uint32_t*>(&s.bins[bin]), v); };  // (sums under 2^32)
     const u64 mass_target = [&]() TRLK_INLINE {  // of top-p without top-k
         const double t = __builtin_ceil(f.top_p * S * unit);
         return t < 1.0 ? u64(1) : u64(int64_t(t));
@@ -660,15 +741,17 @@ __global__ __launch_bounds__(kSelThreads, 4) void filter_select_kernel(SelectArg
     {
         const bool by_count = f.top_k != 0, by_mass = !by_count && f.top_p > 0.0;
         if (by_count || by_mass) {
-            each_max([&](int, float v) TRLK_INLINE {
-                const int d = distance_bin(m, v);
-                if (d < kBins) atomicAdd(&s.bins[d], by_count ? u64(1) : fixed(weight(v)));
+            each_max([&](int, const float(&v)[EPV]) TRLK_INLINE {
+#pragma unroll
+                for (int e = 0; e < EPV; ++e) {
+                    const int d = distance_bin(m, v[e]);
+                    if (d < kBins) add_low(d, by_count ? 1u : about(v[e]));
+                }
             });
             __syncthreads();
             uint32_t bin;
             u64 before = 0;
-            // (the sum of rounded weights may be half a unit for each block too large)
-            if (crossing(s, kBins, by_count ? u64(f.top_k) : mass_target + n_blocks, bin, before)) bound = int(bin);
+            if (crossing(s, kBins, by_count ? u64(f.top_k) : u64(f.top_p * 0x1p31 * (1.0 + 1e-5)) + n_blocks, bin, before)) bound = int(bin);
         }
         if (by_mass) {  // all tokens of less than (1 - top_p) / V of the mass together have less than 1 - top_p of it
             x_low = float(ref + log2((1.0 - f.top_p) * S / double(V) * (1.0 - 1e-9)) / c);
@@ -687,20 +770,24 @@ __global__ __launch_bounds__(kSelThreads, 4) void filter_select_kernel(SelectArg
     const auto in_bound = [&](float v) TRLK_INLINE { return v > -INFINITY && distance_bin(m, v) <= bound; };
 
     // ---- blocks that reach the bound, and the candidates in them
-    each_max([&](int i, float v) TRLK_INLINE {
-        const bool in = in_bound(v);
-        const u64 vote = __ballot(in);
-        if (!vote) return;
-        uint32_t to = 0;
-        if (lane == __builtin_ctzll(vote)) to = atomicAdd(&s.n_list, uint32_t(__popcll(vote)));
-        to = __shfl(to, __builtin_ctzll(vote)) + __popcll(vote & ((u64(1) << lane) - 1));
-        if (in && to < kList) s.list[to] = uint16_t(i);
+    each_max([&](int i, const float(&v)[EPV]) TRLK_INLINE {
+        uint32_t in = 0;
+#pragma unroll
+        for (int e = 0; e < EPV; ++e) in |= in_bound(v[e]) ? 1u << e : 0u;
+        uint32_t to = reserve(&s.n_list, __popc(in));
+#pragma unroll
+        for (int e = 0; e < EPV; ++e) {
+            if (in >> e & 1u) {
+                if (to < kList) s.list[to] = uint16_t(i * EPV + e);
+                ++to;
+            }
+        }
     });
     __syncthreads();
     const bool listed = s.n_list <= kList;
     const int n_visit = listed ? int(s.n_list) : n_blocks;
-    // all logits over the bound, EPV blocks to a load of a wave: g(in, value, key, index), with all lanes of the wave in it
-    const auto stream = [&](auto g) TRLK_INLINE {
+    // the logits of those blocks, EPV blocks to a load of a wave: h(values, index of the first)
+    const auto blocks_pass = [&](auto h) TRLK_INLINE {
         constexpr int LPB = kBlock / EPV, U = 2;
         for (int j0 = wave * EPV; j0 < n_visit; j0 += U * kSelWaves * EPV) {
             u32x4 raw[U];
@@ -722,27 +809,29 @@ __global__ __launch_bounds__(kSelThreads, 4) void filter_select_kernel(SelectArg
             for (int q = 0; q < U; ++q) {
                 float v[EPV];
                 Elem<DT>::unpack(raw[q], v);
-#pragma unroll
-                for (int k = 0; k < EPV; ++k) g(in_bound(v[k]), v[k], uint32_t(e[q]) + k);
+                h(v, uint32_t(e[q]));
             }
         }
     };
-    const bool too_many = !listed && !f.top_k;  // (kList blocks have as many candidates at least)
+    // (where most blocks reach the bound there are thousands of candidates: such a row is passed over as a whole)
+    const bool too_many = !f.top_k && n_visit > 256 && 2 * n_visit > n_blocks;
     if (!too_many) {
-        stream([&](bool in, float v, uint32_t e) TRLK_INLINE {
-            const u64 vote = __ballot(in);
-            if (!vote) return;
-            uint32_t to = 0;
-            if (lane == 0) to = atomicAdd(&s.n_cand, uint32_t(__popcll(vote)));
-            to = __shfl(to, 0) + __popcll(vote & ((u64(1) << lane) - 1));
-            if (in && to < kCandidates) s.order[to] = u64(K::of_float(v)) << 32 | uint32_t(~e);
+        blocks_pass([&](const float(&v)[EPV], uint32_t e0) TRLK_INLINE {
+            uint32_t in = 0;
+#pragma unroll
+            for (int e = 0; e < EPV; ++e) in |= in_bound(v[e]) ? 1u << e : 0u;
+            uint32_t to = reserve(&s.n_cand, __popc(in));
+#pragma unroll
+            for (int e = 0; e < EPV; ++e) {
+                if (in >> e & 1u) {
+                    if (to < kCandidates) s.order[to] = order_of(v[e], e0 + e);
+                    ++to;
+                }
+            }
         });
         __syncthreads();
     }
     const int n_cand = too_many ? kCandidates + 1 : int(s.n_cand);
-    const auto key_of = [&](u64 order) TRLK_INLINE { return uint32_t(order >> 32); };
-    const auto index_of = [&](u64 order) TRLK_INLINE { return ~uint32_t(order); };
-    const auto key_weight = [&](uint32_t k) TRLK_INLINE { return weight(K::to_float(k)); };
     // the smallest of the threads' keys, in a word that was ~0
     const auto smallest = [&](uint32_t& word, uint32_t k) TRLK_INLINE {
 #pragma unroll
@@ -771,66 +860,45 @@ __global__ __launch_bounds__(kSelThreads, 4) void filter_select_kernel(SelectArg
         const u64 target = t < double(W) ? u64(int64_t(t)) : W - 1;
         return target < W ? target : W - 1;
     };
+    // among n <= kPairs kept tokens in s.zone, with their weights, that follow `before`: the one whose cumulative weight in index
+    // order passes the target
+    const auto draw_from_zone = [&](int n, u64 before, u64 target, u64 W) TRLK_INLINE {
+        const Ranked r = rank_pairs(s.zone, s.weight, n, kByIndex);
+        const u64 at = before + r.before;
+        if (r.real && at <= target && at + r.weight > target) drawn(index_of(r.order), K::to_float(key_of(r.order)), log2_of(W));
+    };
 
-    // ---- up to 256 candidates: every pair is compared, which gives each one its rank and the mass before it
+    // ---- few candidates: every pair is compared, which gives each one its rank and the mass before it
     if (n_cand <= kPairs) {
-        // (`parts` neighbouring lanes have a candidate together, and each compares it with its part of all; the sums stay in the wave)
-        const int lp = n_cand <= 64 ? 3 : n_cand <= 128 ? 2 : 1, parts = 1 << lp, np = kSelThreads >> lp, len = np >> lp;
-        const int i = tid >> lp, part = tid & (parts - 1);
-        if (tid < np) {
-            if (tid >= n_cand) s.order[tid] = 0;
-            s.weight[tid] = tid < n_cand ? fixed(key_weight(key_of(s.order[tid]))) : 0;
-        }
-        __syncthreads();
-        const u64 me = s.order[i], my_weight = s.weight[i];
-        const bool real = i < n_cand && part == 0;
-        const auto over_parts = [&](u64 v) TRLK_INLINE {
-            v += moved<0xb1, 0xf>(v);                 // the neighbour
-            if (parts > 2) v += moved<0x4e, 0xf>(v);  // the other pair of four
-            if (parts > 4) v += moved<0x141, 0xf>(v); // the mirrored lane of eight
-            return v;
-        };
-        u64 before = 0, rank = 0;
-        for (int j = 0; j < len; ++j) {
-            const bool earlier = s.order[j * parts + part] > me;
-            before += earlier ? s.weight[j * parts + part] : 0;
-            rank += earlier ? 1 : 0;
-        }
-        before = over_parts(before);
-        rank = over_parts(rank);
-        bool kept = real && (f.top_k == 0 || rank < f.top_k);
+        if (tid < n_cand) s.weight[tid] = fixed(key_weight(key_of(s.order[tid])));
+        const Ranked r = rank_pairs(s.order, s.weight, n_cand, kByOrder);
+        bool kept = r.real && (f.top_k == 0 || r.rank < f.top_k);
         if (f.top_p > 0.0) {
             u64 target = mass_target;
             if (f.top_k) {
-                const u64 W1 = block_total(kept ? my_weight : 0, s.slots[1]);
+                const u64 W1 = block_total(kept ? r.weight : 0, s.slots[1]);
                 const double t = __builtin_ceil(f.top_p * double(W1));
                 target = t < 1.0 ? u64(1) : u64(int64_t(t));
             }
-            kept = kept && before < target;
+            kept = kept && r.before < target;
         }
-        kept = kept && key_of(me) >= kept_from;
-        const u64 W = block_total(kept ? my_weight : 0, s.slots[2]);
-        const double log2_mass = log2(double(W)) - a.fix;
+        kept = kept && key_of(r.order) >= kept_from;
+        const u64 W = block_total(kept ? r.weight : 0, s.slots[2]);
         if constexpr (SCORE) {
             const int n_kept = __syncthreads_count(kept);  // (a prefix of the order)
-            if (real && int(rank) == n_kept - 1) {
-                s.border = key_of(me);
-                s.border_index = index_of(me);
+            if (r.real && int(r.rank) == n_kept - 1) {
+                s.border = key_of(r.order);
+                s.border_index = index_of(r.order);
             }
             __syncthreads();
-            scored(s.border, s.border_index, log2_mass);
+            scored(s.border, s.border_index, [&]() TRLK_INLINE { return log2_of(W); });
         } else {
             const u64 target = draw_target(W);
-            const u64 mine_w = kept ? (target ? my_weight : 1) : 0;
-            if (part == 0) s.weight[i] = mine_w;  // (everyone has read its own)
-            __syncthreads();
-            const uint32_t my_index = index_of(me);
-            u64 cum = 0;
-            for (int j = 0; j < len; ++j) {
-                cum += index_of(s.order[j * parts + part]) <= my_index ? s.weight[j * parts + part] : 0;
+            if (r.real) {  // (in the order of the ranks, without those that are not kept: their weight is 0)
+                s.zone[r.rank] = r.order;
+                s.weight[r.rank] = kept ? (target ? r.weight : 1) : 0;
             }
-            cum = over_parts(cum);
-            if (kept && cum > target && cum - mine_w <= target) drawn(my_index, K::to_float(key_of(me)), log2_mass);
+            draw_from_zone(n_cand, 0, target, W);
         }
         return;
     }
@@ -838,8 +906,97 @@ __global__ __launch_bounds__(kSelThreads, 4) void filter_select_kernel(SelectArg
     const uint32_t top = K::of_float(m), lowest = K::of_float(-INFINITY) + 1u;
     uint32_t border = 0, border_index = ~0u, at;
     u64 before = 0;
-    // ---- very many candidates, without top-k: two passes over the row.  The first adds the weights up, in fp32 and rounded to 2^-31 of
-    // the sum, in bins linear in the logit: that tells the border's bin give or take one.  The second sums in 64 bits, chunk by chunk,
+    // ---- some thousands in LDS, one of top-k and top-p (or min-p alone): the border's bin of distances, then the pairs in it; the token's
+    // chunk of the row, then the pairs in it
+    if (n_cand <= kCandidates && !(f.top_k && f.top_p > 0.0) && bound < kBins) {
+        const auto each = [&](auto g) TRLK_INLINE {
+            for (int i0 = 0; i0 < n_cand; i0 += kSelThreads) g(i0 + tid < n_cand, i0 + tid < n_cand ? s.order[i0 + tid] : 0);
+        };
+        const auto bin_of = [&](u64 o) TRLK_INLINE { return distance_bin(m, K::to_float(key_of(o))); };
+        bool found = true;
+        if (f.top_k || f.top_p > 0.0) {
+            clear_bins(s, bound + 1);
+            each([&](bool in, u64 o) TRLK_INLINE {
+                if (in) atomicAdd(&s.bins[bin_of(o)], f.top_k ? u64(1) : fixed(key_weight(key_of(o))));
+            });
+            __syncthreads();
+            uint32_t bin = 0;
+            found = crossing(s, bound + 1, f.top_k ? u64(f.top_k) : mass_target, bin, before);
+            if (found) {
+                each([&](bool in, u64 o) TRLK_INLINE {
+                    in = in && bin_of(o) == int(bin);
+                    const uint32_t to = reserve(&s.n_zone, in ? 1 : 0);
+                    if (in && to < kPairs) {
+                        s.zone[to] = o;
+                        s.weight[to] = f.top_k ? u64(1) : fixed(key_weight(key_of(o)));
+                    }
+                });
+                __syncthreads();
+                const int n = int(s.n_zone);
+                found = n <= kPairs;
+                if (found) {
+                    const Ranked r = rank_pairs(s.zone, s.weight, n, kByOrder);
+                    const bool kept = r.real && before + r.before < (f.top_k ? u64(f.top_k) : mass_target);
+                    const int n_kept = __syncthreads_count(kept);
+                    if (r.real && int(r.rank) == n_kept - 1) {
+                        s.border = key_of(r.order);
+                        s.border_index = index_of(r.order);
+                    }
+                    if (tid == 0) s.n_zone = 0;
+                    __syncthreads();
+                    border = s.border;
+                    border_index = s.border_index;
+                }
+            }
+        }
+        if (found) {
+            if (kept_from > border) {
+                border = kept_from;
+                border_index = ~0u;
+            }
+            const auto kept = [&](u64 o) TRLK_INLINE { return key_of(o) > border || (key_of(o) == border && index_of(o) <= border_index); };
+            if constexpr (SCORE) {
+                u64 W = 0;
+                each([&](bool in, u64 o) TRLK_INLINE {
+                    if (in && kept(o)) W += fixed(key_weight(key_of(o)));
+                });
+                W = block_total(W, s.slots[2]);
+                return scored(border, border_index, [&]() TRLK_INLINE { return log2_of(W); });
+            } else {
+                clear_bins(s, a.chunks);
+                each([&](bool in, u64 o) TRLK_INLINE {
+                    if (in && kept(o)) atomicAdd(&s.bins[index_of(o) / kChunk], fixed(key_weight(key_of(o))));
+                });
+                __syncthreads();
+                u64 W = 0, target = 0;
+                uint32_t bin = 0;
+                before = 0;
+                crossing_of(s, a.chunks, [&](u64 total) TRLK_INLINE {
+                    W = total;
+                    target = draw_target(W);
+                    return target + 1;
+                }, bin, before);
+                if (target) {
+                    each([&](bool in, u64 o) TRLK_INLINE {
+                        in = in && kept(o) && index_of(o) / kChunk == bin;
+                        const uint32_t to = reserve(&s.n_zone, in ? 1 : 0);
+                        if (in && to < kPairs) {
+                            s.zone[to] = o;
+                            s.weight[to] = fixed(key_weight(key_of(o)));
+                        }
+                    });
+                    __syncthreads();
+                    const int n = int(s.n_zone);
+                    if (n <= kPairs) return draw_from_zone(n, before, target, W);
+                }
+            }
+        }
+        border = 0;
+        border_index = ~0u;
+        before = 0;
+    }
+    // ---- very many candidates, without top-k: two passes over the row.  The first adds the weights up, in fp32, in bins linear in the
+    // logit: that tells the border's bin give or take one.  The second sums in 64 bits, chunk by chunk,
     // what lies before those three bins, and lists what lies in them, where the border is then found.
     if (n_cand > kCandidates && !f.top_k && x_low > -INFINITY) {
         const float scale = float(kBins - 1) / fmaxf(m - x_low, 1e-30f);
@@ -892,11 +1049,10 @@ __global__ __launch_bounds__(kSelThreads, 4) void filter_select_kernel(SelectArg
         bool found = true;
         if (f.top_p > 0.0) {
             clear_bins(s, kBins);
-            const float cf = float(c), l2 = float(31.0 - log2(S));
             row_pass(
                 [&](float v, uint32_t) TRLK_INLINE {
-                    const uint32_t w = uint32_t(fast_exp2(fmaf(v - m, cf, l2)) + 0.5f);
-                    if (v >= x_low) atomicAdd(reinterpret_cast<uint32_t*>(&s.bins[bin_of(v)]), w);  // (all of them are less than 2^32)
+                    const uint32_t w = about(v);
+                    if (v >= x_low) add_low(bin_of(v), w);
                 },
                 [](int) TRLK_INLINE {});
             __syncthreads();
@@ -946,7 +1102,26 @@ __global__ __launch_bounds__(kSelThreads, 4) void filter_select_kernel(SelectArg
         const auto each = [&](auto g) TRLK_INLINE {
             for (int i = tid; i < n_bin; i += kSelThreads) g(key_of(s.order[i]), index_of(s.order[i]));
         };
-        if (found && n_bin <= kCandidates && f.top_p > 0.0) {
+        bool paired = false;
+        if (found && n_bin <= kPairs && f.top_p > 0.0 && all_mass < mass_target) {
+            if (tid < n_bin) s.weight[tid] = fixed(key_weight(key_of(s.order[tid])));
+            const Ranked r = rank_pairs(s.order, s.weight, n_bin, kByOrder);
+            const bool kept = r.real && all_mass + r.before < mass_target;
+            const int n_kept = __syncthreads_count(kept);
+            if (r.real && int(r.rank) == n_kept - 1) {
+                s.border = key_of(r.order);
+                s.border_index = index_of(r.order);
+                s.before = all_mass + r.before + r.weight;
+            }
+            __syncthreads();
+            paired = n_kept > 0 && s.before >= mass_target;
+            if (paired) {
+                border = s.border;
+                border_index = s.border_index;
+            }
+            __syncthreads();
+        }
+        if (found && n_bin <= kCandidates && f.top_p > 0.0 && !paired) {
             before = all_mass;
             found = before < mass_target &&
                     descend(s, [&](auto put) TRLK_INLINE { each([&](uint32_t k, uint32_t) TRLK_INLINE { put(top - k, fixed(key_weight(k))); }); }, 0,
@@ -954,7 +1129,7 @@ __global__ __launch_bounds__(kSelThreads, 4) void filter_select_kernel(SelectArg
         }
         if (found && n_bin <= kCandidates) {
             kept_from = f.min_p > 0.0 ? min_key : 0u;
-            if (f.top_p > 0.0) {
+            if (f.top_p > 0.0 && !paired) {
                 border = top - at;
                 const u64 w = fixed(key_weight(border)), ties = (mass_target - before + w - 1) / w;
                 u64 count = 0;
@@ -980,9 +1155,8 @@ __global__ __launch_bounds__(kSelThreads, 4) void filter_select_kernel(SelectArg
             u64 sum = 0, up, W;
             for (int i = first; i < last; ++i) sum += chunk_mass(i);
             const u64 exc = block_scan(sum, s.slots[2], up, W);
-            const double log2_mass = log2(double(W)) - a.fix;
             if constexpr (SCORE) {
-                scored(border, border_index, log2_mass);
+                scored(border, border_index, [&]() TRLK_INLINE { return log2_of(W); });
             } else {
                 const u64 target = draw_target(W);
                 if (exc <= target && up > target) {  // (one thread)
@@ -1005,7 +1179,7 @@ __global__ __launch_bounds__(kSelThreads, 4) void filter_select_kernel(SelectArg
                 run += block_scan(part, s.slots[3], up, all);
 #pragma unroll
                 for (int j = 0; j < PER; ++j) {
-                    if (w[j] && run <= target && run + w[j] > target) drawn(e0 + j, v[j], log2_mass);
+                    if (w[j] && run <= target && run + w[j] > target) drawn(e0 + j, v[j], log2_of(W));
                     run += w[j];
                 }
             }
@@ -1022,8 +1196,9 @@ __global__ __launch_bounds__(kSelThreads, 4) void filter_select_kernel(SelectArg
         low_key = smallest(s.low_key, k);
     } else if (f.min_p > 0.0) {
         uint32_t k = ~0u;
-        stream([&](bool in, float v, uint32_t) TRLK_INLINE {
-            if (in && weight(v) >= f.min_p && K::of_float(v) < k) k = K::of_float(v);
+        blocks_pass([&](const float(&v)[EPV], uint32_t) TRLK_INLINE {
+            for (int e = 0; e < EPV; ++e)
+                if (in_bound(v[e]) && weight(v[e]) >= f.min_p && K::of_float(v[e]) < k) k = K::of_float(v[e]);
         });
         kept_from = smallest(s.low_key, k);
     }
@@ -1035,8 +1210,10 @@ __global__ __launch_bounds__(kSelThreads, 4) void filter_select_kernel(SelectArg
                 g(key_of(o), index_of(o), [&]() TRLK_INLINE { return fixed(key_weight(key_of(o))); });
             }
         } else {
-            stream([&](bool in, float v, uint32_t e) TRLK_INLINE {
-                if (in) g(K::of_float(v), e, [&]() TRLK_INLINE { return fixed(weight(v)); });
+            blocks_pass([&](const float(&v)[EPV], uint32_t e0) TRLK_INLINE {
+#pragma unroll
+                for (int e = 0; e < EPV; ++e)
+                    if (in_bound(v[e])) g(K::of_float(v[e]), e0 + e, [&]() TRLK_INLINE { return fixed(weight(v[e])); });
             });
         }
     };
@@ -1095,9 +1272,8 @@ __global__ __launch_bounds__(kSelThreads, 4) void filter_select_kernel(SelectArg
         if (kept(k, e)) W += w();
     });
     W = block_total(W, s.slots[2]);
-    const double log2_mass = log2(double(W)) - a.fix;
     if constexpr (SCORE) {
-        scored(border, border_index, log2_mass);
+        scored(border, border_index, [&]() TRLK_INLINE { return log2_of(W); });
     } else {
         const u64 target = draw_target(W);
         before = 0;
@@ -1107,7 +1283,7 @@ __global__ __launch_bounds__(kSelThreads, 4) void filter_select_kernel(SelectArg
                 if (kept(k, e)) put(e, target ? w() : u64(1));
             });
         }, 0, uint32_t(V - 1), target ? target + 1 : 1, id, before);
-        if (tid == 0) drawn(id, Elem<DT>::load1(x + id), log2_mass);
+        if (tid == 0) drawn(id, Elem<DT>::load1(x + id), log2_of(W));
     }
 }
 
