@@ -29,6 +29,7 @@ constexpr int kBinBits = 11;
 constexpr int kCandidates = 4096;            // that are kept in LDS; rows with more read their blocks again in every step
 constexpr int kList = 4096;                  // blocks over the bound that are listed; with more every block is looked at
 constexpr int kPairs = 128;                  // candidates of which every pair is compared
+constexpr int kLine = 128;                   // bytes of a cache line
 constexpr int64_t kMaxVocab = int64_t(1) << 22;
 
 typedef unsigned long long u64;
@@ -63,17 +64,17 @@ struct ChunkUnit {
     float x_min;  // logits under it count as it (2^-1000 at most)
     bool whole;
 };
-__device__ __forceinline__ ChunkUnit chunk_unit(float m, double c) {
+__device__ __forceinline__ ChunkUnit chunk_unit(float m, double c, double inv_c) {
     ChunkUnit u;
     u.exponent = m > -INFINITY ? __builtin_ceil(double(m) * c) : 0.0;
-    u.x_min = float((u.exponent - 1000.0) / c);
+    u.x_min = float((u.exponent - 1000.0) * inv_c);
     const double t = __builtin_fma(double(u.x_min), c, -u.exponent);
     u.whole = u.exponent > -0x1p40 && u.exponent < 0x1p40 && t < -900.0 && t > -1020.0;
     return u;
 }
 // log2 of the unit of a chunk with maximum m, relative to a row's maximum
-__device__ __forceinline__ double chunk_scale(float m, double c, double ref) {
-    const ChunkUnit u = chunk_unit(m, c);
+__device__ __forceinline__ double chunk_scale(float m, double c, double inv_c, double ref) {
+    const ChunkUnit u = chunk_unit(m, c, inv_c);
     return m == -INFINITY ? -INFINITY : u.whole ? -__builtin_fma(ref, c, -u.exponent) : (double(m) - ref) * c;
 }
 // 2^(x * c - unit's exponent), 0.7 at the lowest x_min's 2^-1000: 16 operations of 64 bits, all of the full rate
@@ -194,9 +195,10 @@ struct Filters {
     int64_t top_k;
     const float *d_temperature, *d_top_p, *d_min_p;  // a value for each row, or null: the number above
     const int32_t* d_top_k;
+    double c, inv_c;  // log2(e) / temperature and its inverse (a division of 64 bits costs a wave as much as two of its logits)
 };
 struct RowFilter {
-    double c;         // log2(e) / T
+    double c, inv_c;  // log2(e) / T and T / log2(e)
     double top_p;     // 0: not in force
     double min_p;     // 0: not in force
     uint32_t top_k;   // 0: not in force
@@ -213,7 +215,8 @@ __device__ __forceinline__ RowFilter row_filter(const Filters& f, int64_t row, i
         T = 1.0;
         k = 1;
     }
-    r.c = 1.4426950408889634074 / T;
+    r.c = f.d_temperature ? 1.4426950408889634074 / T : f.c;
+    r.inv_c = f.d_temperature ? 0.69314718055994530942 * T : f.inv_c;
     r.ok = r.ok && r.c < INFINITY;
     r.top_k = k > 0 && k < vocab ? uint32_t(k) : 0u;
     r.top_p = p >= 1.0 ? 0.0 : __builtin_fmax(p, 1e-300);  // (0 or less keeps the first token, as the smallest positive number does)
@@ -269,7 +272,7 @@ __device__ __forceinline__ void load_vectors(const typename Elem<DT>::type* p, i
 }
 
 template <int DT, bool SUMS, bool BLOCKS>
-__global__ __launch_bounds__(kScanThreads) void filter_scan_kernel(ScanArgs a) {
+__global__ __launch_bounds__(kScanThreads, 8) void filter_scan_kernel(ScanArgs a) {
     typedef typename Elem<DT>::type T;
     constexpr int EPV = Elem<DT>::EPV, NV = kChunk / (kWave * EPV), LPB = kBlock / EPV;  // LPB: lanes of a block
     const int lane = threadIdx.x & (kWave - 1);
@@ -301,8 +304,9 @@ __global__ __launch_bounds__(kScanThreads) void filter_scan_kernel(ScanArgs a) {
     }
     m = wave_max_nan(m);
     if constexpr (SUMS) {
-        const double c = row_filter(a.f, row, a.x.vocab).c;
-        const ChunkUnit in = chunk_unit(m, c);
+        const RowFilter f = row_filter(a.f, row, a.x.vocab);
+        const double c = f.c;
+        const ChunkUnit in = chunk_unit(m, c, f.inv_c);
         double s = 0.0;
         if (in.whole) {
             const double magic = 0x1.8p52 - in.exponent;
@@ -618,7 +622,7 @@ __global__ __launch_bounds__(kSelThreads, 4) void filter_select_kernel(SelectArg
     }
     const double c = f.c, ref = double(m), unit = __builtin_amdgcn_ldexp(1.0, a.fix);
     const auto weight = [&](float v) TRLK_INLINE { return exp2_f64((double(v) - ref) * c); };
-    const auto chunk_weight = [&](double sum, float chunk_m) TRLK_INLINE { return sum * exp2_f64(chunk_scale(chunk_m, c, ref)); };
+    const auto chunk_weight = [&](double sum, float chunk_m) TRLK_INLINE { return sum * exp2_f64(chunk_scale(chunk_m, c, f.inv_c, ref)); };
     const auto fixed = [&](double w) TRLK_INLINE { return u64(int64_t(__builtin_rint(w * unit))); };
     const auto log2_of = [&](u64 W) TRLK_INLINE { return log2(double(W)) - a.fix; };
     const auto drawn = [&](int64_t id, float v, double log2_mass) TRLK_INLINE {  // one thread
@@ -1291,7 +1295,7 @@ __global__ __launch_bounds__(kSelThreads, 4) void filter_select_kernel(SelectArg
 struct FilterBwdArgs {
     RowView x;
     int64_t rows;
-    int32_t chunks;
+    int32_t chunks, units_per_row;  // chunks of the forward; waves that a row of the gradient takes
     const int64_t* index;
     double temperature;
     const float* d_temperature;
@@ -1302,63 +1306,78 @@ struct FilterBwdArgs {
 };
 
 // d logits = g / T * (1[v = token] - kept_v * 2^((x_v - max) * c - log2 W)): the gradient is written once, and only the blocks
-// whose maximum reaches the border are read.
-template <int DT>
+// whose maximum reaches the border are read.  A wave's vectors lie at whole cache lines of the gradient, wherever its rows start.  STREAM
+// writes past the caches: for a gradient that they cannot hold.  What is left of it in them would be written back under the next
+// scan (4096 rows of 151936 in bf16: scan 181 us after cached stores, 130 after these; the gradient itself 202 and 221 us).
+template <int DT, bool STREAM>
 __global__ __launch_bounds__(kScanThreads) void filter_bwd_kernel(FilterBwdArgs a) {
     typedef typename Elem<DT>::type T;
-    constexpr int EPV = Elem<DT>::EPV, NV = kChunk / (kWave * EPV), LPB = kBlock / EPV;
+    constexpr int EPV = Elem<DT>::EPV, NV = kChunk / (kWave * EPV);
     const int lane = threadIdx.x & (kWave - 1);
-    const uint32_t at_unit = __builtin_amdgcn_readfirstlane(int(blockIdx.x * (kScanThreads / kWave) + threadIdx.x / kWave));
-    const uint32_t at_row = at_unit / uint32_t(a.chunks);  // (units are fewer than 2^31)
-    const int64_t unit = at_unit, row = at_row;
+    const uint32_t unit = __builtin_amdgcn_readfirstlane(int(blockIdx.x * (kScanThreads / kWave) + threadIdx.x / kWave));
+    const uint32_t row = unit / uint32_t(a.units_per_row);
     if (row >= a.rows) return;
-    const int chunk = int(at_unit - at_row * uint32_t(a.chunks));
-    const int64_t V = a.x.vocab, e0 = int64_t(chunk) * kChunk;
-    const int n = V - e0 < kChunk ? int(V - e0) : kChunk;
+    const int64_t V = a.x.vocab;
+    T* out = static_cast<T*>(a.dlogits) + int64_t(row) * V;
+    const int shift = int(reinterpret_cast<uintptr_t>(out) % kLine / sizeof(T));  // entries of the first line that are another row's
+    const int64_t first = int64_t(unit - row * uint32_t(a.units_per_row)) * kChunk - shift;
     const float g0 = a.g_logp[row];
-    const float bx = a.state[row * 4], m = a.state[row * 4 + 2], l2 = a.state[row * 4 + 3];
-    const uint32_t bi = __float_as_uint(a.state[row * 4 + 1]);
+    const float bx = a.state[row * int64_t(4)], m = a.state[row * int64_t(4) + 2], l2 = a.state[row * int64_t(4) + 3];
+    const uint32_t bi = __float_as_uint(a.state[row * int64_t(4) + 1]);
     double temp = a.d_temperature ? double(a.d_temperature[row]) : a.temperature;
     temp = temp == 0.0 ? 1.0 : temp;
     const float g = float(double(g0) / temp), c = float(1.4426950408889634074 / temp);
     const bool active = bx < INFINITY && g0 != 0.f;
-    const int token = active ? int(a.index[row] - e0) : -1;  // (within the row: the forward has looked)
-    const T* x = a.x.row<DT>(uint32_t(row)) + e0;
-    T* out = static_cast<T*>(a.dlogits) + row * V + e0;
-    const T* bmax = a.block_max ? static_cast<const T*>(a.block_max) + unit * kBlocksPerChunk : nullptr;
+    const int token = active ? int(a.index[row]) : -1;  // (within the row: the forward has looked)
+    const T* x = a.x.row<DT>(row);
+    const T* bmax = a.block_max ? static_cast<const T*>(a.block_max) + int64_t(row) * a.chunks * kBlocksPerChunk : nullptr;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-        const int at = (i * kWave + lane) * EPV;
+        const int64_t at = first + (i * kWave + lane) * EPV;
+        if (at >= V || at + EPV <= 0) continue;
+        const bool whole = at >= 0 && at + EPV <= V;
         float y[EPV];
 #pragma unroll
         for (int e = 0; e < EPV; ++e) y[e] = 0.f;
-        if (active && at < n && (!bmax || Elem<DT>::load1(bmax + i * (kWave / LPB) + lane / LPB) >= bx)) {
+        bool read = active;
+        if (active && bmax) {  // (a vector may lie in two blocks)
+            const int64_t lo = at < 0 ? 0 : at, hi = at + EPV <= V ? at + EPV - 1 : V - 1;
+            read = fmaxf(Elem<DT>::load1(bmax + lo / kBlock), Elem<DT>::load1(bmax + hi / kBlock)) >= bx;
+        }
+        if (read) {
             float v[EPV];
-            if (at + EPV <= n) {
+            if (whole) {
                 const u32x4 q = *reinterpret_cast<const u32x4_u*>(x + at);
                 Elem<DT>::unpack(q, v);
             } else {
 #pragma unroll
-                for (int e = 0; e < EPV; ++e) v[e] = at + e < n ? Elem<DT>::load1(x + at + e) : -INFINITY;
+                for (int e = 0; e < EPV; ++e) v[e] = at + e >= 0 && at + e < V ? Elem<DT>::load1(x + at + e) : -INFINITY;
             }
 #pragma unroll
             for (int e = 0; e < EPV; ++e) {
-                const bool kept = v[e] > bx || (v[e] == bx && uint32_t(e0 + at + e) <= bi);
+                const int j = int(at) + e;
+                const bool kept = v[e] > bx || (v[e] == bx && uint32_t(j) <= bi);
                 const float p = kept ? fast_exp2(fmaf(v[e] - m, c, -l2)) : 0.f;
-                y[e] = g * ((at + e == token ? 1.f : 0.f) - p);
+                y[e] = g * ((j == token ? 1.f : 0.f) - p);
             }
         }
-        if (at + EPV <= n) {
-            *reinterpret_cast<u32x4_u*>(out + at) = Elem<DT>::pack(y);
+        if (whole) {
+            u32x4* to = reinterpret_cast<u32x4*>(out + at);
+            if constexpr (STREAM)
+                __builtin_nontemporal_store(Elem<DT>::pack(y), to);
+            else
+                *to = Elem<DT>::pack(y);
         } else {
 #pragma unroll
             for (int e = 0; e < EPV; ++e)
-                if (at + e < n) Elem<DT>::store1(out + at + e, y[e]);
+                if (at + e >= 0 && at + e < V) Elem<DT>::store1(out + at + e, y[e]);
         }
     }
 }
 
 // ---- host ------------------------------------------------------------------------------------------------------------
+constexpr double ln2 = 0.69314718055994530942;
+double log2e_over(double temperature) { return 1.4426950408889634074 / (temperature == 0.0 ? 1.0 : temperature); }
 int64_t chunks_of(int64_t vocab) { return (vocab + kChunk - 1) / kChunk; }
 size_t up16(size_t n) { return (n + 15) / 16 * 16; }
 
@@ -1382,7 +1401,7 @@ int check_view(const RowView& x, int dtype, int64_t n_seq, const char* what) {
                  (long long)x.row_stride, (long long)x.vocab);
     TRLK_REQUIRE(n_seq == 1 || x.seq_stride >= 0, TRLK_ERR_BAD_STRIDE, "%s: negative seq_stride", what);
     TRLK_REQUIRE(n_seq < (int64_t(1) << 31) && x.rows_per_seq < (int64_t(1) << 31) &&
-                     n_seq * x.rows_per_seq < (int64_t(1) << 31) / chunks_of(x.vocab) - 8,
+                     n_seq * x.rows_per_seq < (int64_t(1) << 31) / (chunks_of(x.vocab) + 1) - 8,
                  TRLK_ERR_BAD_SHAPE, "%s: too many rows", what);
     TRLK_REQUIRE(x.logits, TRLK_ERR_NULL_POINTER, "%s: null logits", what);
     TRLK_REQUIRE(reinterpret_cast<uintptr_t>(x.logits) % elem_size(dtype) == 0, TRLK_ERR_BAD_STRIDE, "%s: misaligned logits", what);
@@ -1410,6 +1429,15 @@ void launch_scan(const ScanArgs& a, bool sums, bool blocks, hipStream_t stream) 
         filter_scan_kernel<DT, true, false><<<grid, kScanThreads, 0, stream>>>(a);
     else
         filter_scan_kernel<DT, false, true><<<grid, kScanThreads, 0, stream>>>(a);
+}
+
+constexpr size_t kCacheBytes = size_t(256) << 20;  // the last level
+template <int DT>
+void launch_bwd(const FilterBwdArgs& a, bool past_caches, dim3 grid, hipStream_t stream) {
+    if (past_caches)
+        filter_bwd_kernel<DT, true><<<grid, kScanThreads, 0, stream>>>(a);
+    else
+        filter_bwd_kernel<DT, false><<<grid, kScanThreads, 0, stream>>>(a);
 }
 
 int run(SelectArgs& a, int dtype, void* workspace, size_t workspace_bytes, void* block_max, bool score, hipStream_t stream, const char* what) {
@@ -1472,7 +1500,7 @@ extern "C" int trlk_sample_tokens(const void* d_logits, int dtype, int64_t n_seq
                                   int64_t* d_out_ids, float* d_out_logp, int32_t* d_error_flag, void* d_workspace,
                                   size_t workspace_bytes, trlk_stream_t stream) {
     clear_error();
-    const Filters f{temperature, top_p, min_p, top_k, d_temperature, d_top_p, d_min_p, d_top_k};
+    const Filters f{temperature, top_p, min_p, top_k, d_temperature, d_top_p, d_min_p, d_top_k, log2e_over(temperature), ln2 * (temperature == 0.0 ? 1.0 : temperature)};
     SelectArgs a{};
     a.x = RowView{d_logits, rows_per_seq, vocab, seq_stride, row_stride};
     a.f = f;
@@ -1499,7 +1527,7 @@ extern "C" int trlk_filtered_logps_fwd(const void* d_logits, int dtype, int64_t 
                                        float* d_out_logp, float* d_out_state, void* d_out_block_max, int32_t* d_error_flag,
                                        void* d_workspace, size_t workspace_bytes, trlk_stream_t stream) {
     clear_error();
-    const Filters f{temperature, top_p, min_p, top_k, d_temperature, d_top_p, d_min_p, d_top_k};
+    const Filters f{temperature, top_p, min_p, top_k, d_temperature, d_top_p, d_min_p, d_top_k, log2e_over(temperature), ln2 * (temperature == 0.0 ? 1.0 : temperature)};
     SelectArgs a{};
     a.x = RowView{d_logits, rows_per_seq, vocab, seq_stride, row_stride};
     a.f = f;
@@ -1520,7 +1548,7 @@ extern "C" int trlk_filtered_logps_fwd(const void* d_logits, int dtype, int64_t 
 
 extern "C" int trlk_token_filter_has_blocks(double temperature, const float* d_temperature, int64_t top_k, const int32_t* d_top_k,
                                             double top_p, const float* d_top_p, double min_p, const float* d_min_p) {
-    return needs_blocks(Filters{temperature, top_p, min_p, top_k, d_temperature, d_top_p, d_min_p, d_top_k}) ? 1 : 0;
+    return needs_blocks(Filters{temperature, top_p, min_p, top_k, d_temperature, d_top_p, d_min_p, d_top_k, 0.0, 0.0}) ? 1 : 0;
 }
 
 extern "C" int trlk_filtered_logps_bwd(const void* d_logits, int dtype, int64_t n_seq, int64_t rows_per_seq, int64_t vocab,
@@ -1546,13 +1574,17 @@ extern "C" int trlk_filtered_logps_bwd(const void* d_logits, int dtype, int64_t 
     a.block_max = d_block_max;
     a.g_logp = d_g_logp;
     a.dlogits = d_dlogits;
-    const dim3 grid(unsigned((a.rows * a.chunks + kScanThreads / kWave - 1) / (kScanThreads / kWave)));
+    const size_t row_bytes = size_t(vocab) * elem_size(dtype);
+    const bool lines = row_bytes % kLine == 0 && reinterpret_cast<uintptr_t>(d_dlogits) % kLine == 0;
+    a.units_per_row = lines ? a.chunks : int32_t((vocab + kLine / int64_t(elem_size(dtype)) - 1 + kChunk - 1) / kChunk);
+    const bool past_caches = row_bytes * size_t(a.rows) > kCacheBytes;
+    const dim3 grid(unsigned((a.rows * a.units_per_row + kScanThreads / kWave - 1) / (kScanThreads / kWave)));
     const hipStream_t st = static_cast<hipStream_t>(stream);
     if (dtype == TRLK_F32)
-        filter_bwd_kernel<TRLK_F32><<<grid, kScanThreads, 0, st>>>(a);
+        launch_bwd<TRLK_F32>(a, past_caches, grid, st);
     else if (dtype == TRLK_BF16)
-        filter_bwd_kernel<TRLK_BF16><<<grid, kScanThreads, 0, st>>>(a);
+        launch_bwd<TRLK_BF16>(a, past_caches, grid, st);
     else
-        filter_bwd_kernel<TRLK_F16><<<grid, kScanThreads, 0, st>>>(a);
+        launch_bwd<TRLK_F16>(a, past_caches, grid, st);
     return launch_status("filtered_logps backward");
 }
