@@ -211,6 +211,10 @@ def _load_torch_ops() -> None:
 
 _load_torch_ops()
 
+# the AdamW step for lists of plain tensors, past the dispatcher; called with the GIL held, raises Python exceptions
+py_adamw_step = ctypes.PyDLL(TORCH_LIB_PATH).trlk_py_adamw_step
+py_adamw_step.restype, py_adamw_step.argtypes = ctypes.py_object, [ctypes.py_object]
+
 
 def last_error() -> str:
     return lib.trlk_last_error().decode()

@@ -21,11 +21,13 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kStateBlock = 256;         // entries that share a scale
-constexpr int kNormChunk = 16384;        // entries of a workgroup of the norm
-constexpr int kChunk = 8192;             // entries of a workgroup of the update
-constexpr int kTable = 56;               // tensors of an update launch   (3.6 KB of arguments)
-constexpr int kNormTable = 160;          // of a norm launch              (3.9 KB)
-constexpr int kStepTable = 240;          // of a launch of the step counters
+constexpr int kNormChunk = 8192;         // entries of a workgroup of the norm
+constexpr int kChunk = 4096;             // entries of a workgroup of the update: adapters of 40000 entries fill the chip, too
+constexpr int kTable32 = 83;             // tensors of an update launch with fp32 moments  (4 KB of arguments)
+constexpr int kTable8 = 62;              // with 8-bit moments                             (4 KB)
+constexpr int kNormTable = 250;          // pieces of tensors of a norm launch             (4 KB)
+constexpr int64_t kNormPiece = int64_t(1) << 31;
+constexpr int kStepTable = 240;          // tensors of a launch of the step counters
 
 // ---- scalars that the update reads: one record per tensor -------------------------------------------------------------
 struct alignas(16) Scalars {
@@ -48,8 +50,8 @@ __device__ __forceinline__ uint32_t mix(uint32_t x) {
 // ---- norm ------------------------------------------------------------------------------------------------------------
 struct NormEntry {
     const void* grad;
-    int64_t numel;
-    uint32_t first, aligned;  // first workgroup of the launch; whether the data is 16-byte aligned
+    uint32_t numel;
+    uint32_t first : 31, aligned : 1;  // first workgroup of the launch; whether the data is 16-byte aligned
 };
 struct NormTable {
     NormEntry e[kNormTable];
@@ -81,11 +83,21 @@ __global__ __launch_bounds__(kThreads) void norm_kernel(NormTable t) {
     int64_t e = begin;
     if (t.e[i].aligned) {
         const int64_t whole = begin + (end - begin) / EPV * EPV;
-        for (int64_t at = begin + threadIdx.x * EPV; at < whole; at += kThreads * EPV) {
-            float x[EPV];
-            Elem<DT>::unpack(*reinterpret_cast<const u32x4*>(g + at), x);
+        constexpr int U = 4;  // loads in flight
+        for (int64_t at = begin + threadIdx.x * EPV; at < whole; at += U * kThreads * EPV) {
+            u32x4 q[U];
 #pragma unroll
-            for (int k = 0; k < EPV; ++k) s = __builtin_fma(double(x[k]), double(x[k]), s);
+            for (int j = 0; j < U; ++j) {
+                const int64_t to = at + j * kThreads * EPV;
+                q[j] = to < whole ? *reinterpret_cast<const u32x4*>(g + to) : u32x4{0, 0, 0, 0};
+            }
+#pragma unroll
+            for (int j = 0; j < U; ++j) {
+                float x[EPV];
+                Elem<DT>::unpack(q[j], x);
+#pragma unroll
+                for (int k = 0; k < EPV; ++k) s = __builtin_fma(double(x[k]), double(x[k]), s);
+            }
         }
         e = whole;
     }
@@ -160,17 +172,23 @@ __global__ __launch_bounds__(1024) void step_kernel(StepTable t) {
 }
 
 // ---- update ----------------------------------------------------------------------------------------------------------
+template <int BITS>
 struct UpdateEntry {
     void* param;
     const void* grad;
     void *exp_avg, *exp_avg_sq;
-    float *exp_avg_scale, *exp_avg_sq_scale;
     int64_t numel;
     uint32_t first;
     uint32_t index : 31, aligned : 1;
 };
+template <>
+struct UpdateEntry<8> : UpdateEntry<32> {
+    float *exp_avg_scale, *exp_avg_sq_scale;
+};
+template <int BITS>
 struct UpdateTable {
-    UpdateEntry e[kTable];
+    static constexpr int kSize = BITS == 32 ? kTable32 : kTable8;
+    UpdateEntry<BITS> e[kSize];
     int32_t n;
     const Scalars* scalars;
     const Header* header;  // null: no clipping
@@ -263,10 +281,10 @@ __device__ __forceinline__ float half_wave_max(float v) {
 }
 
 template <int DT, int BITS>
-__global__ __launch_bounds__(kThreads) void update_kernel(UpdateTable t) {
+__global__ __launch_bounds__(kThreads) void update_kernel(UpdateTable<BITS> t) {
     typedef typename Elem<DT>::type T;
     const int i = entry_of(t.e, t.n, blockIdx.x);
-    const UpdateEntry& en = t.e[i];
+    const UpdateEntry<BITS>& en = t.e[i];
     const Scalars s = t.scalars[en.index];
     const float clip = t.header ? t.header->clip : 1.f;
     const int64_t n = en.numel, begin = int64_t(blockIdx.x - en.first) * kChunk;
@@ -388,24 +406,39 @@ int64_t norm_groups(const trlk_adamw_tensor* t, int32_t n) {
     for (int32_t i = 0; i < n; ++i) sum += chunks(t[i].numel, kNormChunk);
     return sum;
 }
-template <int DT>
-void launch_norm(const NormTable& t, unsigned grid, hipStream_t stream) {
-    norm_kernel<DT><<<grid, kThreads, 0, stream>>>(t);
-}
 void launch_norm(int dtype, const NormTable& t, unsigned grid, hipStream_t stream) {
-    if (dtype == TRLK_F32) launch_norm<TRLK_F32>(t, grid, stream);
-    else if (dtype == TRLK_BF16) launch_norm<TRLK_BF16>(t, grid, stream);
-    else launch_norm<TRLK_F16>(t, grid, stream);
+    if (dtype == TRLK_F32) norm_kernel<TRLK_F32><<<grid, kThreads, 0, stream>>>(t);
+    else if (dtype == TRLK_BF16) norm_kernel<TRLK_BF16><<<grid, kThreads, 0, stream>>>(t);
+    else norm_kernel<TRLK_F16><<<grid, kThreads, 0, stream>>>(t);
 }
-template <int DT>
-void launch_update(int bits, const UpdateTable& t, unsigned grid, hipStream_t stream) {
-    if (bits == 32) update_kernel<DT, 32><<<grid, kThreads, 0, stream>>>(t);
-    else update_kernel<DT, 8><<<grid, kThreads, 0, stream>>>(t);
-}
-void launch_update(int dtype, int bits, const UpdateTable& t, unsigned grid, hipStream_t stream) {
-    if (dtype == TRLK_F32) launch_update<TRLK_F32>(bits, t, grid, stream);
-    else if (dtype == TRLK_BF16) launch_update<TRLK_BF16>(bits, t, grid, stream);
-    else launch_update<TRLK_F16>(bits, t, grid, stream);
+// the update of the tensors of one type with moments of one kind
+template <int DT, int BITS>
+void update(const trlk_adamw_tensor* tensors, int32_t n_tensors, const Scalars* scalars, const Header* header, hipStream_t stream) {
+    UpdateTable<BITS> t;
+    t.n = 0;
+    t.scalars = scalars;
+    t.header = header;
+    int64_t grid = 0;
+    const auto flush = [&] {
+        if (t.n) update_kernel<DT, BITS><<<unsigned(grid), kThreads, 0, stream>>>(t);
+        t.n = 0;
+        grid = 0;
+    };
+    for (int32_t i = 0; i < n_tensors; ++i) {
+        const trlk_adamw_tensor& x = tensors[i];
+        if (x.dtype != DT || x.state_bits != BITS || x.numel == 0) continue;
+        const int64_t need = chunks(x.numel, kChunk);
+        if (t.n == UpdateTable<BITS>::kSize || grid + need > (int64_t(1) << 31) - 1) flush();
+        const size_t state_align = BITS == 32 ? 16 : 8, value_align = BITS == 32 && DT != TRLK_F32 ? 8 : 16;
+        UpdateEntry<BITS>& e = t.e[t.n++];
+        e.param = x.d_param, e.grad = x.d_grad, e.exp_avg = x.d_exp_avg, e.exp_avg_sq = x.d_exp_avg_sq;
+        if constexpr (BITS == 8) e.exp_avg_scale = x.d_exp_avg_scale, e.exp_avg_sq_scale = x.d_exp_avg_sq_scale;
+        e.numel = x.numel, e.first = uint32_t(grid), e.index = uint32_t(i);
+        e.aligned = aligned_to(x.d_param, value_align) && aligned_to(x.d_grad, value_align) && aligned_to(x.d_exp_avg, state_align) &&
+                    aligned_to(x.d_exp_avg_sq, state_align);
+        grid += need;
+    }
+    flush();
 }
 
 int check_adamw(const trlk_adamw_tensor* t, int32_t n, const trlk_adamw_group* g, int32_t n_groups) {
@@ -417,7 +450,7 @@ int check_adamw(const trlk_adamw_tensor* t, int32_t n, const trlk_adamw_group* g
                      "adamw: lr, eps and weight_decay must not be negative");
     }
     for (int32_t i = 0; i < n; ++i) {
-        TRLK_REQUIRE(t[i].numel >= 0 && t[i].numel < (int64_t(1) << 43), TRLK_ERR_BAD_SHAPE, "adamw: tensor %d has %lld entries", i, (long long)t[i].numel);
+        TRLK_REQUIRE(t[i].numel >= 0 && t[i].numel < (int64_t(1) << 42), TRLK_ERR_BAD_SHAPE, "adamw: tensor %d has %lld entries", i, (long long)t[i].numel);
         TRLK_REQUIRE(t[i].dtype == TRLK_F32 || t[i].dtype == TRLK_BF16 || t[i].dtype == TRLK_F16, TRLK_ERR_BAD_DTYPE, "adamw: tensor %d: unsupported dtype %d", i, t[i].dtype);
         TRLK_REQUIRE(t[i].state_bits == 32 || t[i].state_bits == 8, TRLK_ERR_BAD_VALUE, "adamw: tensor %d: state_bits must be 8 or 32", i);
         TRLK_REQUIRE(t[i].group >= 0 && t[i].group < n_groups, TRLK_ERR_BAD_VALUE, "adamw: tensor %d is in no group", i);
@@ -472,11 +505,15 @@ extern "C" int trlk_adamw_step(const trlk_adamw_tensor* tensors, int32_t n_tenso
                 grid = 0;
             };
             for (int32_t i = 0; i < n_tensors; ++i) {
-                if (tensors[i].dtype != dtype || tensors[i].numel == 0) continue;
-                const int64_t need = chunks(tensors[i].numel, kNormChunk);
-                if (t.n == kNormTable || grid + need > (int64_t(1) << 30)) flush();
-                t.e[t.n++] = NormEntry{tensors[i].d_grad, tensors[i].numel, uint32_t(grid), aligned_to(tensors[i].d_grad, 16) ? 1u : 0u};
-                grid += need;
+                if (tensors[i].dtype != dtype) continue;
+                for (int64_t at = 0; at < tensors[i].numel; at += kNormPiece) {
+                    const int64_t n = tensors[i].numel - at < kNormPiece ? tensors[i].numel - at : kNormPiece, need = chunks(n, kNormChunk);
+                    const char* g = static_cast<const char*>(tensors[i].d_grad) + at * int64_t(elem_size(dtype));
+                    if (t.n == kNormTable || grid + need > (int64_t(1) << 30)) flush();
+                    NormEntry& e = t.e[t.n++];
+                    e.grad = g, e.numel = uint32_t(n), e.first = uint32_t(grid), e.aligned = aligned_to(g, 16);
+                    grid += need;
+                }
             }
             flush();
         }
@@ -508,36 +545,13 @@ extern "C" int trlk_adamw_step(const trlk_adamw_tensor* tensors, int32_t n_tenso
         }
         flush();
     }
-    // the update
-    for (int dtype : {int(TRLK_F32), int(TRLK_BF16), int(TRLK_F16)}) {
-        for (int bits : {32, 8}) {
-            UpdateTable t;
-            t.n = 0;
-            t.scalars = scalars;
-            t.header = with_norm ? header : nullptr;
-            int64_t grid = 0;
-            const auto flush = [&] {
-                if (t.n) launch_update(dtype, bits, t, unsigned(grid), stream);
-                t.n = 0;
-                grid = 0;
-            };
-            for (int32_t i = 0; i < n_tensors; ++i) {
-                const trlk_adamw_tensor& x = tensors[i];
-                if (x.dtype != dtype || x.state_bits != bits || x.numel == 0) continue;
-                const int64_t need = chunks(x.numel, kChunk);
-                if (t.n == kTable || grid + need > (int64_t(1) << 30)) flush();
-                const size_t state_align = bits == 32 ? 16 : 8, value_align = bits == 32 && dtype != TRLK_F32 ? 8 : 16;
-                const bool al = aligned_to(x.d_param, value_align) && aligned_to(x.d_grad, value_align) && aligned_to(x.d_exp_avg, state_align) &&
-                                aligned_to(x.d_exp_avg_sq, state_align);
-                UpdateEntry& e = t.e[t.n++];
-                e.param = x.d_param, e.grad = x.d_grad, e.exp_avg = x.d_exp_avg, e.exp_avg_sq = x.d_exp_avg_sq;
-                e.exp_avg_scale = x.d_exp_avg_scale, e.exp_avg_sq_scale = x.d_exp_avg_sq_scale;
-                e.numel = x.numel, e.first = uint32_t(grid), e.index = uint32_t(i), e.aligned = al ? 1u : 0u;
-                grid += need;
-            }
-            flush();
-        }
-    }
+    const Header* clip = with_norm ? header : nullptr;
+    update<TRLK_F32, 32>(tensors, n_tensors, scalars, clip, stream);
+    update<TRLK_BF16, 32>(tensors, n_tensors, scalars, clip, stream);
+    update<TRLK_F16, 32>(tensors, n_tensors, scalars, clip, stream);
+    update<TRLK_F32, 8>(tensors, n_tensors, scalars, clip, stream);
+    update<TRLK_BF16, 8>(tensors, n_tensors, scalars, clip, stream);
+    update<TRLK_F16, 8>(tensors, n_tensors, scalars, clip, stream);
     return launch_status("adamw");
 }
 

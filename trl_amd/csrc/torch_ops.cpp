@@ -15,6 +15,8 @@
 #include <torch/csrc/autograd/autograd_not_implemented_fallback.h>
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/Exceptions.h>
+#include <torch/csrc/autograd/python_variable.h>
 #include <torch/library.h>
 #include <torch/python.h>
 
@@ -712,6 +714,8 @@ Tensor adamw_step_(at::TensorList params, at::TensorList grads_, at::TensorList 
                       "adamw_step_: five numbers and one learning rate for each group are expected");
     TORCH_CHECK_VALUE(n > 0, "adamw_step_: no parameters");
     const at::Device device = params[0].device();
+    TORCH_CHECK(device.is_cuda(), "adamw_step_: the parameters are on ", device, ", not on a GPU");
+    const at::NoGradGuard no_grad;
     const c10::DeviceGuard guard(device);
     std::vector<trlk_adamw_tensor> table(n);
     std::vector<trlk_adamw_group> groups(n_groups);
@@ -787,6 +791,19 @@ Tensor adamw_step_(at::TensorList params, at::TensorList grads_, at::TensorList 
     return norm;
 }
 
+// The tensors of a list or tuple of plain tensors and parameters; false if something else is among them.
+bool plain_tensors(PyObject* object, std::vector<Tensor>& out) {
+    if (!PyList_Check(object) && !PyTuple_Check(object)) return false;
+    const Py_ssize_t n = PySequence_Fast_GET_SIZE(object);
+    PyObject** items = PySequence_Fast_ITEMS(object);
+    out.reserve(n);
+    for (Py_ssize_t i = 0; i < n; ++i) {
+        if (!THPVariable_CheckExact(items[i])) return false;
+        out.push_back(THPVariable_Unpack(items[i]));
+    }
+    return true;
+}
+
 Tensor adamw_state_values(const Tensor& codes, const Tensor& scales) {
     const bool has_sign = codes.scalar_type() == at::kFloat8_e4m3fn;
     TORCH_CHECK_TYPE(has_sign || codes.scalar_type() == at::kByte, "adamw_state_values: codes are float8_e4m3fn (exp_avg) or uint8 (exp_avg_sq)");
@@ -801,6 +818,32 @@ Tensor adamw_state_values(const Tensor& codes, const Tensor& scales) {
     return values;
 }
 }  // namespace
+
+// The AdamW step for lists of plain tensors, called with the arguments of the operator in one tuple and the GIL held.  The
+// dispatcher takes 80 ns for each entry of a list that comes from Python, 90 us for the five lists of 224 tensors: this takes a fifth.
+// Returns None where the operator has to be called (a subclass of tensor, another kind of list), null with a Python error set.
+extern "C" __attribute__((visibility("default"))) PyObject* trlk_py_adamw_step(PyObject* args) {
+    HANDLE_TH_ERRORS
+    PyObject* lists[7];
+    PyObject *groups, *hyper, *lrs;
+    double max_grad_norm;
+    long long seed;
+    if (!PyArg_ParseTuple(args, "OOOOOOOOOOdL", &lists[0], &lists[1], &lists[2], &lists[3], &lists[4], &lists[5], &lists[6], &groups, &hyper,
+                          &lrs, &max_grad_norm, &seed))
+        return nullptr;
+    std::vector<Tensor> tensors[8];
+    for (int i = 0; i < 7; ++i)
+        if (!plain_tensors(lists[i], tensors[i])) Py_RETURN_NONE;
+    if (!plain_tensors(lrs, tensors[7]) || !PyList_Check(groups) || !PyList_Check(hyper)) Py_RETURN_NONE;
+    std::vector<int64_t> group_of;
+    std::vector<double> numbers;
+    for (Py_ssize_t i = 0; i < PyList_GET_SIZE(groups); ++i) group_of.push_back(PyLong_AsLongLong(PyList_GET_ITEM(groups, i)));
+    for (Py_ssize_t i = 0; i < PyList_GET_SIZE(hyper); ++i) numbers.push_back(PyFloat_AsDouble(PyList_GET_ITEM(hyper, i)));
+    if (PyErr_Occurred()) return nullptr;
+    return THPVariable_Wrap(adamw_step_(tensors[0], tensors[1], tensors[2], tensors[3], tensors[4], tensors[5], tensors[6], group_of, numbers,
+                                        tensors[7], max_grad_norm, seed));
+    END_HANDLE_TH_ERRORS
+}
 
 TORCH_LIBRARY_FRAGMENT(trl_amd, m) {
     m.def("error_flag(int device_index) -> Tensor", error_flag);

@@ -70,6 +70,15 @@ def raise_for_error_bits(bits: float, device: torch.device) -> None:
         _raise_for(bits)
 
 
+def _observed() -> bool:
+    """Whether a tracer, a dispatch mode or a function transform is at work.  A torch that does not answer counts as one where it is."""
+    if torch.compiler.is_compiling() or torch.jit.is_tracing():
+        return True
+    modes = getattr(torch._C, "_len_torch_dispatch_stack", None)
+    transforms = getattr(torch._C, "_are_functorch_transforms_active", None)
+    return modes is None or transforms is None or modes() > 0 or transforms()
+
+
 _library = torch.library.Library("trl_amd", "FRAGMENT")
 
 
@@ -270,9 +279,20 @@ filtered_logps_bwd = _native_op(
 # Lists with an entry for each parameter (the scales' may be empty; an empty tensor stands for none); `hyper` has lr, beta1,
 # beta2, eps and weight_decay of each group, `lrs` (may be empty) a learning rate on the GPU for each, `group_of` (may be empty) the
 # parameters' groups.  max_grad_norm > 0 clips, 0 only returns the norm (fp32 0-d), less than 0 does neither (an empty tensor).
-adamw_step_ = _native_op(
+_adamw_step_op = _native_op(
     "adamw_step_", lambda params, grads, exp_avgs, exp_avg_sqs, steps, exp_avg_scales, exp_avg_sq_scales, group_of, hyper, lrs,
     max_grad_norm, seed: torch.empty((0,) if max_grad_norm < 0 else (), dtype=torch.float32, device=params[0].device))
+
+
+
+def adamw_step_(*args):
+    """The operator with these arguments; its kernels' entry point at once where nothing looks on that would want the operator."""
+    if not _observed():
+        norm = _lib.py_adamw_step(args)
+        if norm is not None:
+            return norm
+    return _adamw_step_op(*args)
+
 
 # The bf16 values of 8-bit moments, in the codes' shape.
 adamw_state_values = _native_op(

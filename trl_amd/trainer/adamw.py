@@ -12,7 +12,6 @@ __all__ = ["adamw_step_", "adamw_state_values", "AdamW"]
 STATE_BLOCK = 256  # entries of 8-bit moments that share a scale
 
 
-@torch.no_grad()
 def adamw_step_(params: list[Tensor], grads: list[Tensor], exp_avgs: list[Tensor], exp_avg_sqs: list[Tensor], steps: list[Tensor], *,
                 lr: float | Tensor = 1e-3, betas: tuple[float, float] = (0.9, 0.999), eps: float = 1e-8, weight_decay: float = 0.01,
                 max_grad_norm: float | None = None, exp_avg_scales: list[Tensor] | None = None,
@@ -83,7 +82,6 @@ class AdamW(torch.optim.Optimizer):
                 state["exp_avg_sq"] = torch.zeros_like(p, dtype=torch.float32, memory_format=torch.preserve_format)
         return state
 
-    @torch.no_grad()
     def step(self, closure=None):
         loss = None
         if closure is not None:
