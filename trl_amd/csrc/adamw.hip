@@ -39,6 +39,18 @@ struct alignas(16) Header {
     float clip, norm, pad[2];
 };
 
+// Loads and stores of what a step touches once, past the caches: 355M fp32 entries with fp32 moments 2.02 ms instead of 2.16, 117M in bf16
+// 529 us instead of 554 (the norm's loads are plain: the update reads the gradients again).
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+template <typename V>
+__device__ __forceinline__ V once(const void* p) {
+    return __builtin_nontemporal_load(static_cast<const V*>(p));
+}
+template <typename V>
+__device__ __forceinline__ void once(void* p, V v) {
+    __builtin_nontemporal_store(v, static_cast<V*>(p));
+}
+
 // A 32-bit hash: xor with the upper half, multiply, twice (the multipliers: best of 400 random odd pairs in how evenly one
 // flipped bit flips the others).
 __device__ __forceinline__ uint32_t mix(uint32_t x) {
@@ -215,9 +227,9 @@ __device__ __forceinline__ void load_n(const typename Elem<DT>::type* p, int64_t
     if (whole) {
         if constexpr (N >= EPV) {
 #pragma unroll
-            for (int i = 0; i < N / EPV; ++i) Elem<DT>::unpack(*reinterpret_cast<const u32x4*>(p + at + i * EPV), x + i * EPV);
+            for (int i = 0; i < N / EPV; ++i) Elem<DT>::unpack(once<u32x4>(p + at + i * EPV), x + i * EPV);
         } else {  // 4 entries of a 16-bit type
-            const uint2 q = *reinterpret_cast<const uint2*>(p + at);
+            const u32x2 q = once<u32x2>(p + at);
             Elem<DT>::unpack2(q.x, x);
             Elem<DT>::unpack2(q.y, x + 2);
         }
@@ -232,9 +244,9 @@ __device__ __forceinline__ void store_n(typename Elem<DT>::type* p, int64_t at, 
     if (whole) {
         if constexpr (N >= EPV) {
 #pragma unroll
-            for (int i = 0; i < N / EPV; ++i) *reinterpret_cast<u32x4*>(p + at + i * EPV) = Elem<DT>::pack(x + i * EPV);
+            for (int i = 0; i < N / EPV; ++i) once(p + at + i * EPV, Elem<DT>::pack(x + i * EPV));
         } else {
-            *reinterpret_cast<uint2*>(p + at) = make_uint2(Elem<DT>::pack2(x[0], x[1]), Elem<DT>::pack2(x[2], x[3]));
+            once(p + at, u32x2{Elem<DT>::pack2(x[0], x[1]), Elem<DT>::pack2(x[2], x[3])});
         }
     } else {
 #pragma unroll
@@ -319,7 +331,7 @@ __global__ __launch_bounds__(kThreads) void update_kernel(UpdateTable<BITS> t) {
             const float sm = en.exp_avg_scale[block], sv = en.exp_avg_sq_scale[block];
             uint32_t cm[2] = {0, 0}, cv[2] = {0, 0};
             if (whole) {
-                const uint2 a = *reinterpret_cast<const uint2*>(pm + at), b = *reinterpret_cast<const uint2*>(pv + at);
+                const u32x2 a = once<u32x2>(pm + at), b = once<u32x2>(pv + at);
                 cm[0] = a.x, cm[1] = a.y, cv[0] = b.x, cv[1] = b.y;
             } else {
 #pragma unroll
@@ -360,8 +372,8 @@ __global__ __launch_bounds__(kThreads) void update_kernel(UpdateTable<BITS> t) {
                 cv[k / 4] |= ev << (8 * (k % 4));
             }
             if (whole) {
-                *reinterpret_cast<uint2*>(pm + at) = make_uint2(cm[0], cm[1]);
-                *reinterpret_cast<uint2*>(pv + at) = make_uint2(cv[0], cv[1]);
+                once(pm + at, u32x2{cm[0], cm[1]});
+                once(pv + at, u32x2{cv[0], cv[1]});
             } else {
 #pragma unroll
                 for (int k = 0; k < N; ++k) {
@@ -386,11 +398,11 @@ __global__ __launch_bounds__(kThreads) void state_values_kernel(const uint8_t* c
     if (at >= n) return;
     const float s = scales[at / kStateBlock];
     if (aligned && at + 8 <= n) {
-        const uint2 c = *reinterpret_cast<const uint2*>(codes + at);
+        const u32x2 c = once<u32x2>(codes + at);
         float x[8];
 #pragma unroll
         for (int k = 0; k < 8; ++k) x[k] = decode8<MANT>((k < 4 ? c.x : c.y) >> (8 * (k % 4)) & 0xffu) * s;
-        *reinterpret_cast<u32x4*>(out + at) = Elem<TRLK_BF16>::pack(x);
+        once(out + at, Elem<TRLK_BF16>::pack(x));
     } else {
         for (int k = 0; k < 8 && at + k < n; ++k) Elem<TRLK_BF16>::store1(out + at + k, decode8<MANT>(codes[at + k]) * s);
     }
