@@ -14,6 +14,8 @@
 // are 3 to 6 % apart: rounding to the nearest would leave v where it is for good.  So the rounding is stochastic, up with the
 // probability that keeps the mean; its 16 random bits per moment are a hash of seed, step, tensor and entry, and the same call
 // gives the same bits.  The arithmetic of the moments is that of separate fp32 products and sums, in a fixed order.
+#include <math.h>
+
 #include "common.hpp"
 
 namespace trlk {
@@ -22,7 +24,7 @@ namespace {
 constexpr int kThreads = 256;
 constexpr int kStateBlock = 256;         // entries that share a scale
 constexpr int kNormChunk = 8192;         // entries of a workgroup of the norm
-constexpr int kChunk = 4096;             // entries of a workgroup of the update: adapters of 40000 entries fill the chip, too
+constexpr int kChunk = 2048;             // entries of a workgroup of the update: adapters of 40000 entries fill the chip, too
 constexpr int kTable32 = 83;             // tensors of an update launch with fp32 moments  (4 KB of arguments)
 constexpr int kTable8 = 62;              // with 8-bit moments                             (4 KB)
 constexpr int kNormTable = 250;          // pieces of tensors of a norm launch             (4 KB)
@@ -139,6 +141,7 @@ struct StepTable {
     int32_t n;
     uint32_t seed;
     double lr, beta1, beta2, eps, weight_decay;
+    double log2_beta1, log2_beta2;
     const float* d_lr;
     Scalars* scalars;
     const double* partial;  // null: this launch does not add up the norm
@@ -159,8 +162,8 @@ __global__ __launch_bounds__(1024) void step_kernel(StepTable t) {
         s.one_minus_beta1 = float(1.0 - t.beta1);
         s.beta2 = float(t.beta2);
         s.one_minus_beta2 = float(1.0 - t.beta2);
-        s.size = float(lr / (1.0 - pow(t.beta1, double(now))));
-        s.inv_sqrt_bc2 = float(1.0 / sqrt(1.0 - pow(t.beta2, double(now))));
+        s.size = float(lr / (1.0 - exp2(t.log2_beta1 * double(now))));
+        s.inv_sqrt_bc2 = float(1.0 / sqrt(1.0 - exp2(t.log2_beta2 * double(now))));
         s.eps = float(t.eps);
         s.decay = float(1.0 - lr * t.weight_decay);
         s.salt = mix(mix(uint32_t(int64_t(now)) ^ t.seed) + 0x9E3779B9u * (t.e[i].index + 1u));
@@ -265,6 +268,17 @@ __device__ __forceinline__ float decode8(uint32_t c) {
     else
         return __uint_as_float(c << 19) * 0x1p120f;
 }
+// the four e4m3 codes of a word: the hardware knows the format
+__device__ __forceinline__ void decode_e4m3(uint32_t w, float* x) {
+    typedef float f32x2_t __attribute__((ext_vector_type(2)));
+    const f32x2_t a = __builtin_amdgcn_cvt_pk_f32_fp8(int(w), false), b = __builtin_amdgcn_cvt_pk_f32_fp8(int(w), true);
+    x[0] = a.x, x[1] = a.y, x[2] = b.x, x[3] = b.y;
+}
+// the lowest bytes of four words
+__device__ __forceinline__ uint32_t pack_bytes(const uint32_t* c) {
+    const uint32_t lo = __builtin_amdgcn_perm(c[1], c[0], 0x0c0c0400u), hi = __builtin_amdgcn_perm(c[3], c[2], 0x0c0c0400u);
+    return __builtin_amdgcn_perm(hi, lo, 0x05040100u);
+}
 // code of y >= 0, 448 at most, rounded up where the dropped part and 16 random bits exceed one step
 template <int MANT>
 __device__ __forceinline__ uint32_t encode8(float y, uint32_t r16) {
@@ -342,10 +356,12 @@ __global__ __launch_bounds__(kThreads) void update_kernel(UpdateTable<BITS> t) {
                     }
                 }
             }
+            decode_e4m3(cm[0], m);
+            decode_e4m3(cm[1], m + 4);
             float am = 0.f, av = 0.f;
 #pragma unroll
             for (int k = 0; k < N; ++k) {
-                m[k] = decode8<3>(cm[k / 4] >> (8 * (k % 4)) & 0xffu) * sm;
+                m[k] *= sm;
                 v[k] = decode8<4>(cv[k / 4] >> (8 * (k % 4)) & 0xffu) * sv;
                 moments(s, clip, y[k], m[k], v[k]);
                 x[k] = updated(s, x[k], m[k], v[k]);
@@ -360,17 +376,16 @@ __global__ __launch_bounds__(kThreads) void update_kernel(UpdateTable<BITS> t) {
             float nm, nv, im, iv;
             block_scale(am, nm, im);
             block_scale(av, nv, iv);
-            cm[0] = cm[1] = cv[0] = cv[1] = 0;
+            uint32_t em[N], ev[N];  // (of a block that is not finite any bytes: its scale is NaN)
 #pragma unroll
             for (int k = 0; k < N; ++k) {
                 const uint32_t r = mix(s.salt + uint32_t(at + k) * 0x9E3779B1u);
-                const float ym = fminf(fabsf(m[k]) * im, 448.f), yv = fminf(v[k] * iv, 448.f);  // (what is not finite, too)
-                const uint32_t em = encode8<3>(ym, r & 0xffffu) | (m[k] < 0.f ? 0x80u : 0u);
-                uint32_t ev = encode8<4>(yv, r >> 16);
-                ev = yv > 0.f && ev == 0 ? 1u : ev;
-                cm[k / 4] |= em << (8 * (k % 4));
-                cv[k / 4] |= ev << (8 * (k % 4));
+                const float yv = v[k] * iv;
+                em[k] = encode8<3>(fabsf(m[k]) * im, r & 0xffffu) | (m[k] < 0.f ? 0x80u : 0u);
+                ev[k] = encode8<4>(yv, r >> 16);
+                ev[k] = yv > 0.f && ev[k] == 0 ? 1u : ev[k];
             }
+            cm[0] = pack_bytes(em), cm[1] = pack_bytes(em + 4), cv[0] = pack_bytes(ev), cv[1] = pack_bytes(ev + 4);
             if (whole) {
                 once(pm + at, u32x2{cm[0], cm[1]});
                 once(pv + at, u32x2{cv[0], cv[1]});
@@ -539,6 +554,7 @@ extern "C" int trlk_adamw_step(const trlk_adamw_tensor* tensors, int32_t n_tenso
         const trlk_adamw_group none{0.0, 0.0, 0.0, 0.0, 0.0, nullptr};
         const trlk_adamw_group& gr = g < n_groups ? groups[g] : none;
         t.lr = gr.lr, t.beta1 = gr.beta1, t.beta2 = gr.beta2, t.eps = gr.eps, t.weight_decay = gr.weight_decay, t.d_lr = gr.d_lr;
+        t.log2_beta1 = log2(gr.beta1), t.log2_beta2 = log2(gr.beta2);  // (0: -inf, and its power 0)
         t.scalars = scalars;
         t.partial = partial;
         t.n_partial = n_partial;
