@@ -177,6 +177,64 @@ def test_large_vocabulary():
         check_draw(logits, u, s)
 
 
+@pytest.mark.parametrize("dtype", list(DTYPES))
+@pytest.mark.parametrize("slope", [0.7, 1.0, 1.3, 2.0])
+def test_every_number_of_candidates(slope, dtype):
+    """Nuclei and top-k of a few tokens to most of the vocabulary: rows whose candidates are compared in pairs, binned in LDS, or found
+    by passes over the row, drawn from and scored."""
+    import trl_amd
+
+    logits, u = make_logits(4, 60013, dtype, int(10 * slope), slope)
+    logits[3, ::3] = -math.inf
+    for s in (settings(1.0, 127), settings(1.0, 128), settings(1.0, 129), settings(0.9, 700), settings(1.0, 3000), settings(1.0, 5000),
+              settings(1.0, 400, 0.9), settings(1.0, 0, 0.3), settings(1.0, 0, 0.7), settings(1.0, 0, 0.9), settings(1.0, 0, 0.99),
+              settings(1.0, 0, 0.9999), settings(1.0, 0, 1.0, 1e-3), settings(1.0, 0, 1.0, 1e-5), settings(1.0, 0, 0.99, 1e-4),
+              settings(1.0, 2000, 1.0, 1e-3), settings(3.0, 0, 0.9), settings(3.0, 900)):
+        check_draw(logits, u, s)
+        ids, lp = trl_amd.sample_tokens(logits.to(DEV), u.to(DEV), **s)
+        assert torch.equal(trl_amd.filtered_logps(logits.to(DEV), ids, **s), lp)
+
+
+@pytest.mark.parametrize("dtype", list(DTYPES))
+def test_long_nuclei_and_their_gradient(dtype):
+    g = torch.Generator().manual_seed(17)
+    logits, _ = make_logits(4, 30011, dtype, 18, 1.05)
+    for s in (settings(1.0, 0, 0.9), settings(1.0, 0, 0.99, 1e-4), settings(1.0, 1500), settings(1.0, 0, 1.0, 1e-4), settings(1.0, 300, 0.95)):
+        ids = torch.stack([row_support(x.double(), 1.0, s["top_k"], s["top_p"], s["min_p"])[0][-1] for x in logits])
+        ids[0] = int(logits[0].argmin())
+        check_score(logits, ids, s, torch.randn(4, generator=g))
+
+
+def test_offsets_past_32_bits():
+    """Rows that start behind 2^31 and 2^32 entries of their tensor, and a gradient of more than 2^32."""
+    import trl_amd
+
+    V, rows = 262144, 16400  # 4.3e9 entries
+    if torch.cuda.mem_get_info()[0] < 24 * 2**30:
+        pytest.skip("needs 24 GiB of GPU memory")
+    logits = torch.zeros((rows, V), dtype=torch.bfloat16, device=DEV)
+    mask = torch.zeros(rows, dtype=torch.bool, device=DEV)
+    at = torch.tensor([0, 8191, 8192, 8193, 16383, 16384, 16399])
+    few, u = make_logits(len(at), V, "bf16", 19)
+    logits[at.to(DEV)] = few.to(DEV)
+    mask[at.to(DEV)] = True
+    uniforms = torch.zeros(rows, device=DEV)
+    uniforms[at.to(DEV)] = u.to(DEV)
+    s = settings(1.0, 30, 0.9)
+    ids, lp = trl_amd.sample_tokens(logits, uniforms, **s, row_mask=mask)
+    want_ids, want = expected(few, s, uniforms=u)
+    assert torch.equal(ids.cpu()[at], want_ids)
+    close(lp.cpu()[at], want, V)
+    x = logits.requires_grad_(True)
+    scored = trl_amd.filtered_logps(x, ids, **s, row_mask=mask)
+    assert torch.equal(scored.detach()[at.to(DEV)], lp[at.to(DEV)])
+    (grad,) = torch.autograd.grad(scored, x, torch.ones_like(scored))
+    y = few.to(DEV).requires_grad_(True)
+    (small,) = torch.autograd.grad(trl_amd.filtered_logps(y, want_ids.to(DEV), **s).sum(), y)
+    assert torch.equal(grad[at.to(DEV)], small)
+    assert int(grad.any(-1).sum()) == int(small.any(-1).sum())  # (a row that keeps one token has the gradient 1 - 1)
+
+
 @pytest.mark.parametrize("temperature", [1e-4, 0.05, 30.0, 1e4])
 def test_temperatures(temperature):
     logits, u = make_logits(6, 3001, "fp32", 31)

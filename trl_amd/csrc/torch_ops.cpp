@@ -575,34 +575,51 @@ Settings settings(const char* op, int64_t rows, double temperature, int64_t top_
     return {temperature, top_p, min_p, top_k, f32c(temperatures),
             top_ks ? optional<Tensor>(top_ks->contiguous().to(at::kInt)) : std::nullopt, f32c(top_ps), f32c(min_ps)};
 }
-const uint8_t* mask_ptr(const char* op, const optional<Tensor>& mask, int64_t rows) {
-    if (!mask) return nullptr;
-    TORCH_CHECK_VALUE(mask->numel() == rows && mask->element_size() == 1 && mask->is_contiguous(), op,
-                      ": the row mask must be one contiguous byte for each of ", rows, " rows");
-    return static_cast<const uint8_t*>(operand(*mask));
+// Logits [..., V] as rows [n_seq, rows_per_seq] with strides: where they lie if the strides say so, else a copy.
+struct Rows {
+    Tensor x;  // as in memory, or the copy
+    int64_t n_seq = 1, length = 1, vocab, seq_stride = 0, row_stride = 0, count;
+    int dtype;
+    explicit Rows(const Tensor& logits) : x(logits) {
+        TORCH_CHECK_VALUE(x.dim() > 0, "logits must have at least one dimension");
+        (void)operand(x);
+        dtype = dtype_code(x);
+        vocab = x.size(-1);
+        if (x.dim() > 3) x = x.reshape({-1, x.size(-2), vocab});
+        if ((vocab > 1 && x.stride(-1) != 1) || (x.dim() > 1 && x.size(-2) > 1 && x.stride(-2) < vocab)) x = x.contiguous();
+        if (x.dim() > 1) length = x.size(-2), row_stride = x.stride(-2);
+        if (x.dim() > 2) n_seq = x.size(0), seq_stride = x.stride(0);
+        count = n_seq * length;
+    }
+    const void* data() const { return x.const_data_ptr(); }
+};
+// one byte for each row
+optional<Tensor> byte_mask(const char* op, const optional<Tensor>& mask, int64_t rows) {
+    if (!mask) return std::nullopt;
+    TORCH_CHECK_VALUE(mask->numel() == rows, op, ": the row mask has ", mask->numel(), " entries for ", rows, " rows");
+    return mask->scalar_type() == at::kBool ? mask->contiguous() : mask->ne(0).contiguous();
 }
+const uint8_t* mask_ptr(const optional<Tensor>& mask) { return mask ? static_cast<const uint8_t*>(operand(*mask)) : nullptr; }
 Tensor bytes(const Tensor& like, size_t n) { return at::empty({int64_t(n)}, like.options().dtype(at::kByte)); }
 
 std::tuple<Tensor, Tensor> sample_tokens(const Tensor& logits, const Tensor& uniforms_, double temperature, int64_t top_k, double top_p,
                                          double min_p, const optional<Tensor>& temperatures, const optional<Tensor>& top_ks,
                                          const optional<Tensor>& top_ps, const optional<Tensor>& min_ps,
                                          const optional<Tensor>& row_mask, int64_t fill_id) {
-    check_logits3d(logits);
-    const int64_t n_seq = logits.size(0), length = logits.size(1), vocab = logits.size(2), rows = n_seq * length;
     const c10::DeviceGuard guard(logits.device());
-    const int dtype = dtype_code(logits);
-    TORCH_CHECK_VALUE(uniforms_.numel() == rows, "sample_tokens: ", uniforms_.numel(), " uniform numbers for ", rows, " rows");
-    const Tensor ids = at::empty({rows}, logits.options().dtype(at::kLong)), logp = f32(logits, {rows});
-    const Settings s = settings("sample_tokens", rows, temperature, top_k, top_p, min_p, temperatures, top_ks, top_ps, min_ps);
-    const uint8_t* mask = mask_ptr("sample_tokens", row_mask, rows);
+    const Rows r(logits);
+    TORCH_CHECK_VALUE(uniforms_.numel() == r.count, "sample_tokens: ", uniforms_.numel(), " uniform numbers for ", r.count, " rows");
+    const Tensor ids = at::empty(uniforms_.sizes(), logits.options().dtype(at::kLong)), logp = f32(logits, uniforms_.sizes());
+    const Settings s = settings("sample_tokens", r.count, temperature, top_k, top_p, min_p, temperatures, top_ks, top_ps, min_ps);
+    const optional<Tensor> mask = byte_mask("sample_tokens", row_mask, r.count);
     const bool f64 = uniforms_.scalar_type() == at::kDouble;
     const Tensor uniforms = f64 ? uniforms_.contiguous() : f32c(uniforms_);
-    const size_t ws_bytes = trlk_token_filter_workspace_bytes(rows, vocab, dtype);
+    const size_t ws_bytes = trlk_token_filter_workspace_bytes(r.count, r.vocab, r.dtype);
     const Tensor ws = bytes(logits, ws_bytes);
-    check(trlk_sample_tokens(logits.const_data_ptr(), dtype, n_seq, length, vocab, logits.stride(0), logits.stride(1),
-                             operand(uniforms), f64 ? 1 : 0, s.temperature, s.t(), s.top_k, s.k(), s.top_p, s.p(), s.min_p, s.m(),
-                             mask, fill_id, static_cast<int64_t*>(ids.mutable_data_ptr()), out(logp), error_word(logits),
-                             ws.mutable_data_ptr(), ws_bytes, stream_of(logits)));
+    check(trlk_sample_tokens(r.data(), r.dtype, r.n_seq, r.length, r.vocab, r.seq_stride, r.row_stride, operand(uniforms), f64 ? 1 : 0,
+                             s.temperature, s.t(), s.top_k, s.k(), s.top_p, s.p(), s.min_p, s.m(), mask_ptr(mask), fill_id,
+                             static_cast<int64_t*>(ids.mutable_data_ptr()), out(logp), error_word(logits), ws.mutable_data_ptr(), ws_bytes,
+                             stream_of(logits)));
     check_ids();
     return {ids, logp};
 }
@@ -610,22 +627,20 @@ std::tuple<Tensor, Tensor> sample_tokens(const Tensor& logits, const Tensor& uni
 Tensor3 filtered_logps_fwd(const Tensor& logits, const Tensor& index_, double temperature, int64_t top_k, double top_p, double min_p,
                            const optional<Tensor>& temperatures, const optional<Tensor>& top_ks, const optional<Tensor>& top_ps,
                            const optional<Tensor>& min_ps, const optional<Tensor>& row_mask) {
-    check_logits3d(logits);
-    const int64_t n_seq = logits.size(0), length = logits.size(1), vocab = logits.size(2), rows = n_seq * length;
     const c10::DeviceGuard guard(logits.device());
-    const int dtype = dtype_code(logits);
-    TORCH_CHECK_VALUE(index_.numel() == rows && index_.scalar_type() == at::kLong, "filtered_logps: ", index_.numel(), " ", index_.scalar_type(),
-                      " token ids for ", rows, " rows of int64");
-    const Settings s = settings("filtered_logps", rows, temperature, top_k, top_p, min_p, temperatures, top_ks, top_ps, min_ps);
-    const uint8_t* mask = mask_ptr("filtered_logps", row_mask, rows);
+    const Rows r(logits);
+    TORCH_CHECK_VALUE(index_.numel() == r.count && index_.scalar_type() == at::kLong, "filtered_logps: ", index_.numel(), " ",
+                      index_.scalar_type(), " token ids for ", r.count, " rows of int64");
+    const Settings s = settings("filtered_logps", r.count, temperature, top_k, top_p, min_p, temperatures, top_ks, top_ps, min_ps);
+    const optional<Tensor> mask = byte_mask("filtered_logps", row_mask, r.count);
     const bool blocks = trlk_token_filter_has_blocks(s.temperature, s.t(), s.top_k, s.k(), s.top_p, s.p(), s.min_p, s.m()) != 0;
-    const Tensor logp = f32(logits, {rows}), state = f32(logits, {rows, 4});
-    const Tensor block_max = at::empty({blocks ? rows : 0, trlk_token_filter_blocks(vocab)}, logits.options());
+    const Tensor logp = f32(logits, index_.sizes()), state = f32(logits, {r.count, 4});
+    const Tensor block_max = at::empty({blocks ? r.count : 0, trlk_token_filter_blocks(r.vocab)}, logits.options());
     const Tensor index = index_.contiguous();
-    const size_t ws_bytes = trlk_token_filter_workspace_bytes(rows, vocab, dtype);
+    const size_t ws_bytes = trlk_token_filter_workspace_bytes(r.count, r.vocab, r.dtype);
     const Tensor ws = bytes(logits, ws_bytes);
-    check(trlk_filtered_logps_fwd(logits.const_data_ptr(), dtype, n_seq, length, vocab, logits.stride(0), logits.stride(1), iptr(index),
-                                  s.temperature, s.t(), s.top_k, s.k(), s.top_p, s.p(), s.min_p, s.m(), mask, out(logp), out(state),
+    check(trlk_filtered_logps_fwd(r.data(), r.dtype, r.n_seq, r.length, r.vocab, r.seq_stride, r.row_stride, iptr(index), s.temperature,
+                                  s.t(), s.top_k, s.k(), s.top_p, s.p(), s.min_p, s.m(), mask_ptr(mask), out(logp), out(state),
                                   blocks ? block_max.mutable_data_ptr() : nullptr, error_word(logits), ws.mutable_data_ptr(), ws_bytes,
                                   stream_of(logits)));
     check_ids();
@@ -634,21 +649,19 @@ Tensor3 filtered_logps_fwd(const Tensor& logits, const Tensor& index_, double te
 
 Tensor filtered_logps_bwd(const Tensor& logits, const Tensor& index_, double temperature, const optional<Tensor>& temperatures_,
                           const Tensor& state, const Tensor& block_max, const Tensor& g_logp_) {
-    check_logits3d(logits);
-    const int64_t n_seq = logits.size(0), length = logits.size(1), vocab = logits.size(2), rows = n_seq * length;
     const c10::DeviceGuard guard(logits.device());
-    const Tensor dlogits = at::empty({n_seq, length, vocab}, logits.options());
+    const Tensor dlogits = at::empty(logits.sizes(), logits.options());
     if (dlogits.numel() == 0) return dlogits;
-    TORCH_CHECK_VALUE(index_.numel() == rows && g_logp_.numel() == rows && state.numel() == 4 * rows && state.is_contiguous() &&
-                          (!temperatures_ || temperatures_->numel() == rows) &&
-                          (block_max.numel() == 0 || block_max.numel() == rows * trlk_token_filter_blocks(vocab)),
+    const Rows r(logits);
+    TORCH_CHECK_VALUE(index_.numel() == r.count && g_logp_.numel() == r.count && state.numel() == 4 * r.count && state.is_contiguous() &&
+                          (!temperatures_ || temperatures_->numel() == r.count) &&
+                          (block_max.numel() == 0 || block_max.numel() == r.count * trlk_token_filter_blocks(r.vocab)),
                       "filtered_logps: the backward's operands do not match");
     const Tensor index = index_.contiguous(), g_logp = f32c(g_logp_);
     const optional<Tensor> temperatures = f32c(temperatures_);
-    check(trlk_filtered_logps_bwd(logits.const_data_ptr(), dtype_code(logits), n_seq, length, vocab, logits.stride(0), logits.stride(1),
-                                  iptr(index), temperature, fptr(temperatures), fptr(state),
-                                  block_max.numel() ? operand(block_max) : nullptr, fptr(g_logp), dlogits.mutable_data_ptr(),
-                                  stream_of(logits)));
+    check(trlk_filtered_logps_bwd(r.data(), r.dtype, r.n_seq, r.length, r.vocab, r.seq_stride, r.row_stride, iptr(index), temperature,
+                                  fptr(temperatures), fptr(state), block_max.numel() ? operand(block_max) : nullptr, fptr(g_logp),
+                                  dlogits.mutable_data_ptr(), stream_of(logits)));
     return dlogits;
 }
 
@@ -702,9 +715,11 @@ bool twice(std::vector<const void*> p) {
     return std::adjacent_find(p.begin(), p.end()) != p.end();
 }
 
-Tensor adamw_step_(at::TensorList params, at::TensorList grads_, at::TensorList exp_avgs, at::TensorList exp_avg_sqs,
-                   at::TensorList steps, at::TensorList exp_avg_scales, at::TensorList exp_avg_sq_scales, at::IntArrayRef group_of,
-                   at::ArrayRef<double> hyper, at::TensorList lrs, double max_grad_norm, int64_t seed) {
+// (List: at::TensorList, or the tensors of a Python list where they are)
+template <typename List>
+Tensor adamw_step(const List& params, const List& grads_, const List& exp_avgs, const List& exp_avg_sqs, const List& steps,
+                  const List& exp_avg_scales, const List& exp_avg_sq_scales, at::IntArrayRef group_of, at::ArrayRef<double> hyper,
+                  const List& lrs, double max_grad_norm, int64_t seed) {
     const size_t n = params.size(), n_groups = hyper.size() / 5;
     TORCH_CHECK_VALUE(grads_.size() == n && exp_avgs.size() == n && exp_avg_sqs.size() == n && steps.size() == n &&
                           (group_of.empty() || group_of.size() == n) && (exp_avg_scales.empty() || exp_avg_scales.size() == n) &&
@@ -785,24 +800,32 @@ Tensor adamw_step_(at::TensorList params, at::TensorList grads_, at::TensorList 
     const Tensor ws = bytes(params[0], ws_bytes);
     check(trlk_adamw_step(table.data(), int32_t(n), groups.data(), int32_t(n_groups), max_grad_norm, uint32_t(seed),
                           max_grad_norm < 0 ? nullptr : out(norm), ws.mutable_data_ptr(), ws_bytes, stream_of(params[0])));
-    for (at::TensorList list : {params, exp_avgs, exp_avg_sqs, steps, exp_avg_scales, exp_avg_sq_scales})
-        for (const Tensor& t : list)
-            if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();  // (graphs that saved one of them learn that it has changed)
+    for (const List* list : {&params, &exp_avgs, &exp_avg_sqs, &steps, &exp_avg_scales, &exp_avg_sq_scales})
+        for (size_t i = 0; i < list->size(); ++i)
+            if (!(*list)[i].is_inference()) (*list)[i].unsafeGetTensorImpl()->bump_version();  // (graphs that saved it learn that it has changed)
     return norm;
 }
-
-// The tensors of a list or tuple of plain tensors and parameters; false if something else is among them.
-bool plain_tensors(PyObject* object, std::vector<Tensor>& out) {
-    if (!PyList_Check(object) && !PyTuple_Check(object)) return false;
-    const Py_ssize_t n = PySequence_Fast_GET_SIZE(object);
-    PyObject** items = PySequence_Fast_ITEMS(object);
-    out.reserve(n);
-    for (Py_ssize_t i = 0; i < n; ++i) {
-        if (!THPVariable_CheckExact(items[i])) return false;
-        out.push_back(THPVariable_Unpack(items[i]));
-    }
-    return true;
+Tensor adamw_step_(at::TensorList params, at::TensorList grads, at::TensorList exp_avgs, at::TensorList exp_avg_sqs, at::TensorList steps,
+                   at::TensorList exp_avg_scales, at::TensorList exp_avg_sq_scales, at::IntArrayRef group_of, at::ArrayRef<double> hyper,
+                   at::TensorList lrs, double max_grad_norm, int64_t seed) {
+    return adamw_step(params, grads, exp_avgs, exp_avg_sqs, steps, exp_avg_scales, exp_avg_sq_scales, group_of, hyper, lrs, max_grad_norm, seed);
 }
+
+// The tensors of a Python list or tuple, held by it.
+struct PyTensors {
+    PyObject** items = nullptr;
+    size_t n = 0;
+    size_t size() const { return n; }
+    bool empty() const { return n == 0; }
+    const Tensor& operator[](size_t i) const { return THPVariable_Unpack(items[i]); }
+    // false if something else than plain tensors and parameters is in it
+    bool take(PyObject* object) {
+        if (!PyList_Check(object) && !PyTuple_Check(object)) return false;
+        n = size_t(PySequence_Fast_GET_SIZE(object));
+        items = PySequence_Fast_ITEMS(object);
+        return std::all_of(items, items + n, [](PyObject* o) { return THPVariable_CheckExact(o); });
+    }
+};
 
 Tensor adamw_state_values(const Tensor& codes, const Tensor& scales) {
     const bool has_sign = codes.scalar_type() == at::kFloat8_e4m3fn;
@@ -831,17 +854,17 @@ extern "C" __attribute__((visibility("default"))) PyObject* trlk_py_adamw_step(P
     if (!PyArg_ParseTuple(args, "OOOOOOOOOOdL", &lists[0], &lists[1], &lists[2], &lists[3], &lists[4], &lists[5], &lists[6], &groups, &hyper,
                           &lrs, &max_grad_norm, &seed))
         return nullptr;
-    std::vector<Tensor> tensors[8];
+    PyTensors tensors[8];
     for (int i = 0; i < 7; ++i)
-        if (!plain_tensors(lists[i], tensors[i])) Py_RETURN_NONE;
-    if (!plain_tensors(lrs, tensors[7]) || !PyList_Check(groups) || !PyList_Check(hyper)) Py_RETURN_NONE;
+        if (!tensors[i].take(lists[i])) Py_RETURN_NONE;
+    if (!tensors[7].take(lrs) || !PyList_Check(groups) || !PyList_Check(hyper)) Py_RETURN_NONE;
     std::vector<int64_t> group_of;
     std::vector<double> numbers;
     for (Py_ssize_t i = 0; i < PyList_GET_SIZE(groups); ++i) group_of.push_back(PyLong_AsLongLong(PyList_GET_ITEM(groups, i)));
     for (Py_ssize_t i = 0; i < PyList_GET_SIZE(hyper); ++i) numbers.push_back(PyFloat_AsDouble(PyList_GET_ITEM(hyper, i)));
     if (PyErr_Occurred()) return nullptr;
-    return THPVariable_Wrap(adamw_step_(tensors[0], tensors[1], tensors[2], tensors[3], tensors[4], tensors[5], tensors[6], group_of, numbers,
-                                        tensors[7], max_grad_norm, seed));
+    return THPVariable_Wrap(adamw_step(tensors[0], tensors[1], tensors[2], tensors[3], tensors[4], tensors[5], tensors[6], group_of, numbers,
+                                       tensors[7], max_grad_norm, seed));
     END_HANDLE_TH_ERRORS
 }
 

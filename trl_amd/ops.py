@@ -244,30 +244,26 @@ def logp_entropy_forward(logits: Tensor, index: Tensor, temperature: float, keep
 # --------------------------------------------------------------------------------------------
 # tokens drawn from, and scored under, a filtered distribution (K8)
 # --------------------------------------------------------------------------------------------
-def _rows_of(logits) -> int:
-    return logits.shape[0] * logits.shape[1]
-
-
-# logits [n_seq, L, V] (strided view, last axis contiguous), uniforms fp32 or fp64 with an entry for each row.  A setting is a
-# number, or (the tensors behind them) a value for each row.  Returns (ids int64 [rows], logps fp32 [rows]).
+# logits [..., V] (copied where the rows' strides are none), uniforms fp32 or fp64 with an entry for each row.  A setting is a
+# number, or (the tensors behind them) a value for each row.  Returns (ids int64, logps fp32) in the shape of the uniforms.
 sample_tokens = _native_op(
     "sample_tokens", lambda logits, uniforms, temperature, top_k, top_p, min_p, temperatures, top_ks, top_ps, min_ps, row_mask, fill_id:
-    (torch.empty((_rows_of(logits),), dtype=torch.int64, device=logits.device), _f32_like(logits, _rows_of(logits))))
+    (torch.empty(uniforms.shape, dtype=torch.int64, device=logits.device), _f32_like(logits, *uniforms.shape)))
 
 
-# As above for given tokens, index int64 [rows].  Returns (logps fp32 [rows], the backward's row state fp32 [rows, 4], block
-# maxima in the logits' type); the first carries the gradient.
+# As above for given tokens, index int64.  Returns (logps fp32 in the shape of the index, the backward's row state fp32 [rows, 4],
+# block maxima in the logits' type); the first carries the gradient.
 def _filtered_logps_fake(logits, index, temperature, top_k, top_p, min_p, temperatures, top_ks, top_ps, min_ps, row_mask):
-    rows, blocks = _rows_of(logits), -(-logits.shape[2] // 2048) * 32
+    rows, blocks = index.numel(), -(-logits.shape[-1] // 2048) * 32
     per_row = any(t is not None for t in (temperatures, top_ks, top_ps, min_ps))
     has = per_row or temperature == 0.0 or top_k > 0 or top_p < 1.0 or min_p > 0.0
-    return (_f32_like(logits, rows), _f32_like(logits, rows, 4),
+    return (_f32_like(logits, *index.shape), _f32_like(logits, rows, 4),
             torch.empty((rows if has else 0, blocks), dtype=logits.dtype, device=logits.device))
 
 
 filtered_logps_fwd = _native_op("filtered_logps_fwd", _filtered_logps_fake)
 
-# d(loss)/d(logits), contiguous [n_seq, L, V] in the logits' type.
+# d(loss)/d(logits), contiguous in the logits' shape and type.
 filtered_logps_bwd = _native_op(
     "filtered_logps_bwd", lambda logits, index, temperature, temperatures, state, block_max, g_logp:
     torch.empty(logits.shape, dtype=logits.dtype, device=logits.device))

@@ -123,14 +123,9 @@ def _settings(shape: torch.Size, temperature, top_k, top_p, min_p) -> tuple:
     return (*numbers, *tensors)
 
 
-def _byte_mask(row_mask: Tensor | None, shape: torch.Size) -> Tensor | None:
-    if row_mask is None:
-        return None
-    if row_mask.shape != shape:
+def _check_rows(shape: torch.Size, row_mask: Tensor | None) -> None:
+    if row_mask is not None and row_mask.shape != shape:
         raise ValueError(f"row_mask of shape {tuple(row_mask.shape)} for rows of shape {tuple(shape)}")
-    if row_mask.dtype != torch.bool:
-        row_mask = row_mask != 0
-    return row_mask.contiguous().view(torch.uint8)
 
 
 def sample_tokens(logits: Tensor, uniforms: Tensor, temperature: float | Tensor = 1.0, top_k: int | Tensor | None = 0,
@@ -154,9 +149,8 @@ def sample_tokens(logits: Tensor, uniforms: Tensor, temperature: float | Tensor 
     shape = logits.shape[:-1]
     if uniforms.shape != shape:
         raise ValueError(f"uniforms of shape {tuple(uniforms.shape)} for logits of shape {tuple(logits.shape)}")
-    ids, logps = ops.sample_tokens(_as_3d(logits), uniforms, *_settings(shape, temperature, top_k, top_p, min_p),
-                                   _byte_mask(row_mask, shape), pad_token_id)
-    return ids.view(shape), logps.view(shape)
+    _check_rows(shape, row_mask)
+    return ops.sample_tokens(logits, uniforms, *_settings(shape, temperature, top_k, top_p, min_p), row_mask, pad_token_id)
 
 
 def filtered_logps(logits: Tensor, index: Tensor, temperature: float | Tensor = 1.0, top_k: int | Tensor | None = 0,
@@ -174,9 +168,8 @@ def filtered_logps(logits: Tensor, index: Tensor, temperature: float | Tensor = 
         raise ValueError(f"index of shape {tuple(index.shape)} for logits of shape {tuple(logits.shape)}")
     if index.dtype != torch.int64:
         index = index.long()
-    logps, _, _ = ops.filtered_logps_fwd(_as_3d(logits), index, *_settings(shape, temperature, top_k, top_p, min_p),
-                                         _byte_mask(row_mask, shape))
-    return logps.view(shape)
+    _check_rows(shape, row_mask)
+    return ops.filtered_logps_fwd(logits, index, *_settings(shape, temperature, top_k, top_p, min_p), row_mask)[0]
 
 
 # ----------------------------------------------------------------------------------------------
