@@ -26,7 +26,7 @@ constexpr int kSelThreads = 512;
 constexpr int kSelWaves = kSelThreads / kWave;
 constexpr int kBins = 4 * kSelThreads;       // of a step of the descent
 constexpr int kBinBits = 11;
-constexpr int kCandidates = 4096;            // that are kept in LDS; rows with more read their blocks again in every step
+constexpr int kMaxCandidates = 4096;         // that are kept in LDS; rows with more read their blocks again in every step
 constexpr int kList = 4096;                  // blocks over the bound that are listed; with more every block is looked at
 constexpr int kPairs = 128;                  // candidates of which every pair is compared
 constexpr int kLine = 128;                   // bytes of a cache line
@@ -351,9 +351,10 @@ union WaveSlots {
 __device__ __forceinline__ u64& slot_of(WaveSlots& s, int i, u64) { return s.u[i]; }
 __device__ __forceinline__ double& slot_of(WaveSlots& s, int i, double) { return s.f[i]; }
 
+template <int CANDIDATES>
 struct SelectShared {
     u64 bins[kBins];
-    u64 order[kCandidates];  // of the candidates: key above, ~index below, larger is earlier
+    u64 order[CANDIDATES];  // of the candidates: key above, ~index below, larger is earlier
     u64 weight[kPairs], zone[kPairs];
     uint16_t list[kList];
     WaveSlots slots[4];
@@ -397,8 +398,8 @@ __device__ __forceinline__ u64 block_total(u64 v, WaveSlots& slots) {
 // The bin up to which the values of bins [0, n) and `before` reach a target first, and in `before` what lies before it; false if
 // all of them do not.  The target comes from the sum of all bins.  The bins are complete and the barrier behind them passed; s.bin
 // is ~0.  Contains two barriers.
-template <typename Target>
-__device__ __forceinline__ bool crossing_of(SelectShared& s, int n, Target target_of, uint32_t& bin, u64& before) {
+template <typename Shared, typename Target>
+__device__ __forceinline__ bool crossing_of(Shared& s, int n, Target target_of, uint32_t& bin, u64& before) {
     u64 v[4], sum = 0, upto, total;
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
@@ -422,11 +423,13 @@ __device__ __forceinline__ bool crossing_of(SelectShared& s, int n, Target targe
     before = s.before;
     return true;
 }
-__device__ __forceinline__ bool crossing(SelectShared& s, int n, u64 target, uint32_t& bin, u64& before) {
+template <typename Shared>
+__device__ __forceinline__ bool crossing(Shared& s, int n, u64 target, uint32_t& bin, u64& before) {
     return crossing_of(s, n, [&](u64) TRLK_INLINE { return target; }, bin, before);
 }
 // all bins 0 and no crossing yet, behind a barrier
-__device__ __forceinline__ void clear_bins(SelectShared& s, int n) {
+template <typename Shared>
+__device__ __forceinline__ void clear_bins(Shared& s, int n) {
     for (int i = threadIdx.x; i < n; i += kSelThreads) s.bins[i] = 0;
     __syncthreads();
     if (threadIdx.x == 0) s.bin = ~0u;  // (everyone has read the last one, and two barriers lie before the next is written)
@@ -480,8 +483,8 @@ constexpr u64 kByOrder = ~u64(0), kByIndex = 0xffffffffu;
 
 // The smallest position in [lo, hi] up to which `before` and the values reach `target`, and in `before` what lies before it.
 // `each(f)` calls f(position, value) for this thread's share of the items.  False if all of them do not reach it.
-template <typename Each>
-__device__ __forceinline__ bool descend(SelectShared& s, Each each, uint32_t lo, uint32_t hi, u64 target, uint32_t& position, u64& before) {
+template <typename Shared, typename Each>
+__device__ __forceinline__ bool descend(Shared& s, Each each, uint32_t lo, uint32_t hi, u64 target, uint32_t& position, u64& before) {
     for (;;) {
         const uint32_t span = hi - lo;
         const int bits = span ? 32 - __builtin_clz(span) : 0, shift = bits > kBinBits ? bits - kBinBits : 0;
@@ -510,7 +513,8 @@ __device__ __forceinline__ int distance_bin(float m, float x) {
 constexpr int kEveryBin = 1 << 30;
 
 // `owner` of the smallest thread number, and if there is none of the largest with `some`: its number, the same for all threads
-__device__ __forceinline__ int first_thread(SelectShared& s, int which, bool owner, bool some) {
+template <typename Shared>
+__device__ __forceinline__ int first_thread(Shared& s, int which, bool owner, bool some) {
     const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
     const u64 a = __ballot(owner), b = __ballot(some);
     if (lane == 0) {
@@ -529,14 +533,16 @@ __device__ __forceinline__ int first_thread(SelectShared& s, int which, bool own
     return r;
 }
 
-template <int DT, bool SCORE>
-__global__ __launch_bounds__(kSelThreads, 4) void filter_select_kernel(SelectArgs a) {
+// LONG: rows may have no top-k, and so any number of tokens, or no filter at all.  Without, three workgroups fit into a CU instead of two.
+template <int DT, bool SCORE, bool LONG>
+__global__ __launch_bounds__(kSelThreads, LONG ? 4 : 6) void filter_select_kernel(SelectArgs a) {
     typedef typename Elem<DT>::type T;
     typedef Key<DT> K;
     constexpr int EPV = Elem<DT>::EPV, PER = kChunk / kSelThreads;
     constexpr int NV = kChunk / (kWave * EPV);
     constexpr int kKeep = sizeof(T) == 4 ? 2 : 1;  // vectors of block maxima that a thread holds: 4096 blocks
-    __shared__ SelectShared s;
+    constexpr int kCandidates = LONG ? kMaxCandidates : kMaxCandidates / 2;
+    __shared__ SelectShared<kCandidates> s;
     const int tid = threadIdx.x, lane = tid & (kWave - 1), wave = tid / kWave;
     const int64_t row = blockIdx.x, V = a.x.vocab;
     // what a row without a token, or without a distribution, returns
@@ -552,8 +558,8 @@ __global__ __launch_bounds__(kSelThreads, 4) void filter_select_kernel(SelectArg
     };
     if (a.row_mask && a.row_mask[row] == 0) return nothing(a.fill_id, 0.f);
     const RowFilter f = row_filter(a.f, row, V);
-    const bool filtered = f.top_k || f.top_p > 0.0 || f.min_p > 0.0;
-    const bool with_sum = !filtered || (f.top_p > 0.0 && !f.top_k);
+    const bool filtered = !LONG || f.top_k || f.top_p > 0.0 || f.min_p > 0.0;
+    const bool with_sum = LONG && (!filtered || (f.top_p > 0.0 && !f.top_k));
     const T* x = a.x.row<DT>(uint32_t(row));
     const float* cmax = a.chunk_max + row * a.chunks;
     double* csum = a.chunk_sum + row * a.chunks;
@@ -623,7 +629,8 @@ __global__ __launch_bounds__(kSelThreads, 4) void filter_select_kernel(SelectArg
     const double c = f.c, ref = double(m), unit = __builtin_amdgcn_ldexp(1.0, a.fix);
     const auto weight = [&](float v) TRLK_INLINE { return exp2_f64((double(v) - ref) * c); };
     const auto chunk_weight = [&](double sum, float chunk_m) TRLK_INLINE { return sum * exp2_f64(chunk_scale(chunk_m, c, f.inv_c, ref)); };
-    const auto fixed = [&](double w) TRLK_INLINE { return u64(int64_t(__builtin_rint(w * unit))); };
+    // w <= 1 in units of 2^-fix, rounded to the nearest: the low bits of a sum with 1.5 * 2^52 (fix is at most 50)
+    const auto fixed = [&](double w) TRLK_INLINE { return __builtin_bit_cast(u64, __builtin_fma(w, unit, 0x1.8p52)) - __builtin_bit_cast(u64, 0x1.8p52); };
     const auto log2_of = [&](u64 W) TRLK_INLINE { return log2(double(W)) - a.fix; };
     const auto drawn = [&](int64_t id, float v, double log2_mass) TRLK_INLINE {  // one thread
         a.out_ids[row] = id;
@@ -656,7 +663,7 @@ __global__ __launch_bounds__(kSelThreads, 4) void filter_select_kernel(SelectArg
         base = block_scan(mine, s.slots[1], upto, S);
     }
     // ---- no filter: the chunk, then the token in it
-    if (!filtered) {
+    if (LONG && !filtered) {
         if constexpr (SCORE) {
             return scored(0, ~0u, [&]() TRLK_INLINE { return log2(S); });
         } else {
@@ -1002,13 +1009,13 @@ __global__ __launch_bounds__(kSelThreads, 4) void filter_select_kernel(SelectArg
     // ---- very many candidates, without top-k: two passes over the row.  The first adds the weights up, in fp32, in bins linear in the
     // logit: that tells the border's bin give or take one.  The second sums in 64 bits, chunk by chunk,
     // what lies before those three bins, and lists what lies in them, where the border is then found.
-    if (n_cand > kCandidates && !f.top_k && x_low > -INFINITY) {
+    if (LONG && n_cand > kCandidates && !f.top_k && x_low > -INFINITY) {
         const float scale = float(kBins - 1) / fmaxf(m - x_low, 1e-30f);
         const auto bin_of = [&](float v) TRLK_INLINE {
             const float t = (m - v) * scale;
             return t < float(kBins) ? int(t) : kBins;
         };
-        // g(value, index) for every logit, end(chunk) after a wave's chunk: 16 logits of a lane at a time, the next ones in flight
+        // g(values, index of the first) for every vector, end(chunk) after a wave's chunk: 16 logits of a lane at a time, the next in flight
         constexpr int G = 16 / EPV;
         const auto row_pass = [&](auto g, auto end) TRLK_INLINE {
             const auto load = [&](int64_t e0, u32x4(&q)[G]) TRLK_INLINE {
@@ -1039,11 +1046,8 @@ __global__ __launch_bounds__(kSelThreads, 4) void filter_select_kernel(SelectArg
                     for (int i = 0; i < G; ++i) {
                         float v[EPV];
                         Elem<DT>::unpack(now[i], v);
-#pragma unroll
-                        for (int e = 0; e < EPV; ++e) {
-                            g(v[e], e0 + (i * kWave + lane) * EPV + e);
-                            __builtin_amdgcn_sched_barrier(0);
-                        }
+                        g(v, e0 + (i * kWave + lane) * EPV);
+                        __builtin_amdgcn_sched_barrier(0);
                     }
                 }
                 end(ch);
@@ -1054,9 +1058,17 @@ __global__ __launch_bounds__(kSelThreads, 4) void filter_select_kernel(SelectArg
         if (f.top_p > 0.0) {
             clear_bins(s, kBins);
             row_pass(
-                [&](float v, uint32_t) TRLK_INLINE {
-                    const uint32_t w = about(v);
-                    if (v >= x_low) add_low(bin_of(v), w);
+                [&](const float(&v)[EPV], uint32_t) TRLK_INLINE {
+                    uint32_t w[EPV];
+                    int b[EPV];
+#pragma unroll
+                    for (int e = 0; e < EPV; ++e) {
+                        w[e] = about(v[e]);
+                        b[e] = bin_of(v[e]);
+                    }
+#pragma unroll
+                    for (int e = 0; e < EPV; ++e)
+                        if (v[e] >= x_low) add_low(b[e], w[e]);
                 },
                 [](int) TRLK_INLINE {});
             __syncthreads();
@@ -1078,20 +1090,30 @@ __global__ __launch_bounds__(kSelThreads, 4) void filter_select_kernel(SelectArg
         if (found) {
             u64 mass = 0;
             row_pass(
-                [&](float v, uint32_t e) TRLK_INLINE {
-                    const int b = v >= x_low ? bin_of(v) : kBins + 1;
-                    if (b >= zone_end) return;
-                    const double wd = weight(v);
-                    const u64 w = b < zone ? fixed(wd) : 0;
-                    const uint32_t k = K::of_float(v);
-                    all_mass += w;
-                    if (wd >= f.min_p) {
-                        mass += w;
-                        if (k < min_key) min_key = k;
+                [&](const float(&v)[EPV], uint32_t e0) TRLK_INLINE {
+                    int b[EPV];
+                    bool some = false;
+#pragma unroll
+                    for (int e = 0; e < EPV; ++e) {
+                        b[e] = v[e] >= x_low ? bin_of(v[e]) : kBins + 1;
+                        some |= b[e] < zone_end;
                     }
-                    if (b >= zone) {
-                        const uint32_t to = atomicAdd(&s.n_cand, 1u);
-                        if (to < kCandidates) s.order[to] = u64(k) << 32 | uint32_t(~e);
+                    if (!__ballot(some)) return;
+                    double wd[EPV];
+#pragma unroll
+                    for (int e = 0; e < EPV; ++e) wd[e] = weight(v[e]);
+#pragma unroll
+                    for (int e = 0; e < EPV; ++e) {
+                        const u64 w = b[e] < zone ? fixed(wd[e]) : 0;
+                        const bool enough = wd[e] >= f.min_p;
+                        all_mass += w;
+                        mass += enough ? w : 0;
+                        const uint32_t k = K::of_float(v[e]);
+                        if (enough && b[e] < zone_end && k < min_key) min_key = k;
+                        if (b[e] >= zone && b[e] < zone_end) {
+                            const uint32_t to = atomicAdd(&s.n_cand, 1u);
+                            if (to < kCandidates) s.order[to] = order_of(v[e], e0 + e);
+                        }
                     }
                 },
                 [&](int ch) TRLK_INLINE {
@@ -1413,10 +1435,12 @@ int check_view(const RowView& x, int dtype, int64_t n_seq, const char* what) {
 bool needs_blocks(const Filters& f) {
     return f.d_temperature || f.d_top_k || f.d_top_p || f.d_min_p || f.temperature == 0.0 || f.top_k > 0 || f.top_p < 1.0 || f.min_p > 0.0;
 }
+bool every_top_k(const Filters& f, int64_t vocab) {
+    return vocab > 1 && ((!f.d_top_k && f.top_k > 0 && f.top_k < vocab) || (!f.d_temperature && f.temperature == 0.0));
+}
 bool needs_sums(const Filters& f, int64_t vocab) {
-    const bool every_k = vocab > 1 && ((!f.d_top_k && f.top_k > 0 && f.top_k < vocab) || (!f.d_temperature && f.temperature == 0.0));
     const bool min_p_alone = !f.d_min_p && f.min_p > 0.0 && !f.d_top_p && f.top_p >= 1.0;
-    return !every_k && !min_p_alone;
+    return !every_top_k(f, vocab) && !min_p_alone;
 }
 
 template <int DT>
@@ -1431,6 +1455,18 @@ void launch_scan(const ScanArgs& a, bool sums, bool blocks, hipStream_t stream) 
         filter_scan_kernel<DT, false, true><<<grid, kScanThreads, 0, stream>>>(a);
 }
 
+template <int DT>
+void launch_select(const SelectArgs& a, bool score, bool any_length, hipStream_t stream) {
+    const dim3 grid{unsigned(a.rows)};
+    if (score && any_length)
+        filter_select_kernel<DT, true, true><<<grid, kSelThreads, 0, stream>>>(a);
+    else if (score)
+        filter_select_kernel<DT, true, false><<<grid, kSelThreads, 0, stream>>>(a);
+    else if (any_length)
+        filter_select_kernel<DT, false, true><<<grid, kSelThreads, 0, stream>>>(a);
+    else
+        filter_select_kernel<DT, false, false><<<grid, kSelThreads, 0, stream>>>(a);
+}
 constexpr size_t kCacheBytes = size_t(256) << 20;  // the last level
 template <int DT>
 void launch_bwd(const FilterBwdArgs& a, bool past_caches, dim3 grid, hipStream_t stream) {
@@ -1442,7 +1478,7 @@ void launch_bwd(const FilterBwdArgs& a, bool past_caches, dim3 grid, hipStream_t
 
 int run(SelectArgs& a, int dtype, void* workspace, size_t workspace_bytes, void* block_max, bool score, hipStream_t stream, const char* what) {
     const int64_t units = a.rows * a.chunks;
-    const bool blocks = needs_blocks(a.f), sums = needs_sums(a.f, a.x.vocab);
+    const bool blocks = needs_blocks(a.f), sums = needs_sums(a.f, a.x.vocab), any_length = !every_top_k(a.f, a.x.vocab);
     const size_t sum_bytes = up16(size_t(units) * 8), max_bytes = up16(size_t(units) * 4);
     const size_t need = trlk_token_filter_workspace_bytes(a.rows, a.x.vocab, dtype);
     TRLK_REQUIRE(workspace && workspace_bytes >= need, TRLK_ERR_WORKSPACE, "%s: workspace of %zu bytes, %zu needed", what, workspace_bytes, need);
@@ -1454,24 +1490,20 @@ int run(SelectArgs& a, int dtype, void* workspace, size_t workspace_bytes, void*
     a.block_max = block_max;
     int bits = 0;
     while ((a.x.vocab >> bits) != 0) ++bits;
-    a.fix = 62 - bits;  // a sum of `vocab` weights of at most 1 stays under 2^62
+    a.fix = 62 - bits < 50 ? 62 - bits : 50;  // a sum of `vocab` weights of at most 1 stays under 2^62
     const ScanArgs sc{a.x, a.rows, a.chunks, a.f, a.row_mask, reinterpret_cast<double*>(ws), reinterpret_cast<float*>(ws + sum_bytes), block_max};
-    const dim3 grid{unsigned(a.rows)};
     switch (dtype) {
         case TRLK_F32:
             launch_scan<TRLK_F32>(sc, sums, blocks, stream);
-            score ? filter_select_kernel<TRLK_F32, true><<<grid, kSelThreads, 0, stream>>>(a)
-                  : filter_select_kernel<TRLK_F32, false><<<grid, kSelThreads, 0, stream>>>(a);
+            launch_select<TRLK_F32>(a, score, any_length, stream);
             break;
         case TRLK_BF16:
             launch_scan<TRLK_BF16>(sc, sums, blocks, stream);
-            score ? filter_select_kernel<TRLK_BF16, true><<<grid, kSelThreads, 0, stream>>>(a)
-                  : filter_select_kernel<TRLK_BF16, false><<<grid, kSelThreads, 0, stream>>>(a);
+            launch_select<TRLK_BF16>(a, score, any_length, stream);
             break;
         default:
             launch_scan<TRLK_F16>(sc, sums, blocks, stream);
-            score ? filter_select_kernel<TRLK_F16, true><<<grid, kSelThreads, 0, stream>>>(a)
-                  : filter_select_kernel<TRLK_F16, false><<<grid, kSelThreads, 0, stream>>>(a);
+            launch_select<TRLK_F16>(a, score, any_length, stream);
             break;
     }
     return launch_status(what);
