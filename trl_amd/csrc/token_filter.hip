@@ -13,6 +13,8 @@
 //
 // Whole numbers come out, and the same ones whatever the launch: sums of weights are 64-bit floats in a fixed order over a row's
 // chunks, or 64-bit integers (weights in units of 2^-fix, whose sums do not depend on the order in which threads add them).
+#include <type_traits>
+
 #include "common.hpp"
 
 namespace trlk {
@@ -332,6 +334,7 @@ struct SelectArgs {
     double* chunk_sum;  // (a row with very many candidates puts the kept weights of its chunks there)
     const float* chunk_max;
     const void* block_max;
+    int32_t has_blocks, has_sums;  // what the scan has left
     const void* uniform;  // sample: fp32 or fp64 [rows]
     int32_t uniform_f64;
     int64_t fill_id;
@@ -557,25 +560,37 @@ __global__ __launch_bounds__(kSelThreads, LONG ? 4 : 6) void filter_select_kerne
         a.out_logp[row] = logp;
     };
     if (a.row_mask && a.row_mask[row] == 0) return nothing(a.fill_id, 0.f);
-    const RowFilter f = row_filter(a.f, row, V);
-    const bool filtered = !LONG || f.top_k || f.top_p > 0.0 || f.min_p > 0.0;
-    const bool with_sum = LONG && (!filtered || (f.top_p > 0.0 && !f.top_k));
-    const T* x = a.x.row<DT>(uint32_t(row));
+    // (what every row needs is on its way before the row's settings are known)
     const float* cmax = a.chunk_max + row * a.chunks;
     double* csum = a.chunk_sum + row * a.chunks;
     const int n_blocks = a.chunks * kBlocksPerChunk, n_vec = n_blocks / EPV;  // (blocks behind the row's end are -inf)
     const u32x4* bmax = reinterpret_cast<const u32x4*>(static_cast<const T*>(a.block_max) + row * n_blocks);
-
-    // block maxima (chunk maxima where there are no others) and the row's maximum
     u32x4 held[kKeep] = {};
+    if (a.has_blocks) {
+#pragma unroll
+        for (int j = 0; j < kKeep; ++j)
+            if (tid + j * kSelThreads < n_vec) held[j] = bmax[tid + j * kSelThreads];
+    }
+    const int per = (a.chunks + kSelThreads - 1) / kSelThreads, first = tid * per, last = first + per < a.chunks ? first + per : a.chunks;
+    double sum0 = 0.0;  // this thread's first chunk
+    float max0 = -INFINITY;
+    if (LONG && a.has_sums && first < last) {
+        sum0 = csum[first];
+        max0 = cmax[first];
+    }
+    const RowFilter f = row_filter(a.f, row, V);
+    const bool filtered = !LONG || f.top_k || f.top_p > 0.0 || f.min_p > 0.0;
+    const bool with_sum = LONG && (!filtered || (f.top_p > 0.0 && !f.top_k));
+    const T* x = a.x.row<DT>(uint32_t(row));
+
+    // the row's maximum: of its blocks, or of its chunks where there are no blocks
     float m = -INFINITY;
     if (filtered) {
 #pragma unroll
         for (int j = 0; j < kKeep; ++j) {
+            float v[EPV];
+            Elem<DT>::unpack(held[j], v);
             if (tid + j * kSelThreads < n_vec) {
-                held[j] = bmax[tid + j * kSelThreads];
-                float v[EPV];
-                Elem<DT>::unpack(held[j], v);
 #pragma unroll
                 for (int e = 0; e < EPV; ++e) m = max_nan(m, v[e]);
             }
@@ -588,13 +603,6 @@ __global__ __launch_bounds__(kSelThreads, LONG ? 4 : 6) void filter_select_kerne
         }
     } else {
         for (int i = tid; i < a.chunks; i += kSelThreads) m = max_nan(m, cmax[i]);
-    }
-    const int per = (a.chunks + kSelThreads - 1) / kSelThreads, first = tid * per, last = first + per < a.chunks ? first + per : a.chunks;
-    double sum0 = 0.0;  // this thread's first chunk, loaded beside the maxima
-    float max0 = -INFINITY;
-    if (with_sum && first < last) {
-        sum0 = csum[first];
-        max0 = cmax[first];
     }
     int64_t token = 0;
     bool token_ok = true;
@@ -1015,8 +1023,10 @@ __global__ __launch_bounds__(kSelThreads, LONG ? 4 : 6) void filter_select_kerne
             const float t = (m - v) * scale;
             return t < float(kBins) ? int(t) : kBins;
         };
-        // g(values, index of the first) for every vector, end(chunk) after a wave's chunk: 16 logits of a lane at a time, the next in flight
-        constexpr int G = 16 / EPV;
+        // g(values, index of the first) for every vector, end(chunk) after a wave's half of a chunk (waves get as many halves each): 16 logits
+        // of a lane at a time, the next in flight
+        constexpr int G = 16 / EPV, kHalf = 16 * kWave;
+        static_assert(2 * kHalf == kChunk && NV == 2 * G, "a half is one set of vectors");
         const auto row_pass = [&](auto g, auto end) TRLK_INLINE {
             const auto load = [&](int64_t e0, u32x4(&q)[G]) TRLK_INLINE {
 #pragma unroll
@@ -1033,24 +1043,21 @@ __global__ __launch_bounds__(kSelThreads, LONG ? 4 : 6) void filter_select_kerne
                 }
             };
             u32x4 next[G];
-            load(int64_t(wave) * kChunk, next);
-            for (int ch = wave; ch < a.chunks; ch += kSelWaves) {
-#pragma unroll 1
-                for (int h = 0; h < NV / G; ++h) {
-                    const uint32_t e0 = uint32_t(ch) * kChunk + h * 16 * kWave;
-                    u32x4 now[G];
+            load(int64_t(wave) * kHalf, next);
+            for (int half = wave; half < 2 * a.chunks; half += kSelWaves) {
+                const uint32_t e0 = uint32_t(half) * kHalf;
+                u32x4 now[G];
 #pragma unroll
-                    for (int i = 0; i < G; ++i) now[i] = next[i];
-                    load(h + 1 < NV / G ? int64_t(e0) + 16 * kWave : int64_t(ch + kSelWaves) * kChunk, next);
+                for (int i = 0; i < G; ++i) now[i] = next[i];
+                load(int64_t(half + kSelWaves) * kHalf, next);
 #pragma unroll
-                    for (int i = 0; i < G; ++i) {
-                        float v[EPV];
-                        Elem<DT>::unpack(now[i], v);
-                        g(v, e0 + (i * kWave + lane) * EPV);
-                        __builtin_amdgcn_sched_barrier(0);
-                    }
+                for (int i = 0; i < G; ++i) {
+                    float v[EPV];
+                    Elem<DT>::unpack(now[i], v);
+                    g(v, e0 + (i * kWave + lane) * EPV);
+                    __builtin_amdgcn_sched_barrier(0);
                 }
-                end(ch);
+                end(half / 2);
             }
         };
         int zone = kBins, zone_end = kBins;  // [zone, zone_end) has the border
@@ -1088,39 +1095,56 @@ __global__ __launch_bounds__(kSelThreads, LONG ? 4 : 6) void filter_select_kerne
         u64 all_mass = 0;
         uint32_t min_key = ~0u;
         if (found) {
-            u64 mass = 0;
-            row_pass(
-                [&](const float(&v)[EPV], uint32_t e0) TRLK_INLINE {
-                    int b[EPV];
-                    bool some = false;
+            clear_bins(s, a.chunks);  // (of chunks here)
+            const float before_zone = float(zone), behind_zone = float(zone_end);
+            // (min-p takes away some of what top-p counts)
+            const auto second_pass = [&](auto with_min_p) TRLK_INLINE {
+                u64 mass = 0;
+                row_pass(
+                    [&](const float(&v)[EPV], uint32_t e0) TRLK_INLINE {
+                        float t[EPV];
+                        bool some = false;
 #pragma unroll
-                    for (int e = 0; e < EPV; ++e) {
-                        b[e] = v[e] >= x_low ? bin_of(v[e]) : kBins + 1;
-                        some |= b[e] < zone_end;
-                    }
-                    if (!__ballot(some)) return;
-                    double wd[EPV];
-#pragma unroll
-                    for (int e = 0; e < EPV; ++e) wd[e] = weight(v[e]);
-#pragma unroll
-                    for (int e = 0; e < EPV; ++e) {
-                        const u64 w = b[e] < zone ? fixed(wd[e]) : 0;
-                        const bool enough = wd[e] >= f.min_p;
-                        all_mass += w;
-                        mass += enough ? w : 0;
-                        const uint32_t k = K::of_float(v[e]);
-                        if (enough && b[e] < zone_end && k < min_key) min_key = k;
-                        if (b[e] >= zone && b[e] < zone_end) {
-                            const uint32_t to = atomicAdd(&s.n_cand, 1u);
-                            if (to < kCandidates) s.order[to] = order_of(v[e], e0 + e);
+                        for (int e = 0; e < EPV; ++e) {
+                            t[e] = v[e] >= x_low ? (m - v[e]) * scale : INFINITY;
+                            some |= t[e] < behind_zone;
                         }
-                    }
-                },
-                [&](int ch) TRLK_INLINE {
-                    mass = wave_inclusive(mass);
-                    if (lane == kWave - 1) cmass[ch] = mass;
-                    mass = 0;
-                });
+                        if (!__ballot(some)) return;
+                        double wd[EPV];
+#pragma unroll
+                        for (int e = 0; e < EPV; ++e) wd[e] = weight(t[e] < before_zone || with_min_p.value ? v[e] : -INFINITY);
+#pragma unroll
+                        for (int e = 0; e < EPV; ++e) {
+                            u64 w = fixed(wd[e]);
+                            if constexpr (with_min_p.value) {
+                                w = t[e] < before_zone ? w : 0;
+                                all_mass += w;
+                                const bool enough = wd[e] >= f.min_p;
+                                w = enough ? w : 0;
+                                const uint32_t k = K::of_float(v[e]);
+                                if (enough && t[e] < behind_zone && k < min_key) min_key = k;
+                            }
+                            mass += w;
+                        }
+#pragma unroll
+                        for (int e = 0; e < EPV; ++e) {
+                            if (t[e] >= before_zone && t[e] < behind_zone) {
+                                const uint32_t to = atomicAdd(&s.n_cand, 1u);
+                                if (to < kCandidates) s.order[to] = order_of(v[e], e0 + e);
+                            }
+                        }
+                    },
+                    [&](int ch) TRLK_INLINE {
+                        if constexpr (!with_min_p.value) all_mass += mass;
+                        mass = wave_inclusive(mass);
+                        if (lane == kWave - 1) atomicAdd(&s.bins[ch], mass);
+                        mass = 0;
+                    });
+            };
+            if (f.min_p > 0.0) second_pass(std::true_type{});
+            else second_pass(std::false_type{});
+            __syncthreads();
+            for (int i = first; i < last; ++i) cmass[i] = s.bins[i];
         }
         min_key = smallest(s.min_key, min_key);
         all_mass = block_total(all_mass, s.slots[1]);
@@ -1488,6 +1512,8 @@ int run(SelectArgs& a, int dtype, void* workspace, size_t workspace_bytes, void*
     a.chunk_max = reinterpret_cast<float*>(ws + sum_bytes);
     if (!block_max) block_max = ws + sum_bytes + max_bytes;
     a.block_max = block_max;
+    a.has_blocks = blocks;
+    a.has_sums = sums;
     int bits = 0;
     while ((a.x.vocab >> bits) != 0) ++bits;
     a.fix = 62 - bits < 50 ? 62 - bits : 50;  // a sum of `vocab` weights of at most 1 stays under 2^62
