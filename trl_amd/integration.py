@@ -11,13 +11,17 @@ every trainer module, and the loss is a trainer method.  `patch_trl()` therefore
   * the fused-linear loss operators behind `use_liger_kernel` (optional, `liger=True`): the names
     `LigerFusedLinearGRPOLoss` / `LigerFusedLinearDPOLoss` and `is_liger_kernel_available` in
     `trl.trainer.grpo_trainer` / `trl.trainer.dpo_trainer` (trl/trainer/grpo_trainer.py:1020-1044,
-    trl/trainer/dpo_trainer.py:834), so that `compute_liger_loss` / `_compute_loss_liger` call the fused head.
+    trl/trainer/dpo_trainer.py:834), so that `compute_liger_loss` / `_compute_loss_liger` call the fused head;
+  * the trainers' `get_optimizer_cls_and_kwargs` (optional, `adamw=True`): `optim="adamw_torch"`, `"adamw_torch_fused"`, `"adamw_8bit"`
+    and `"adamw_bnb_8bit"` then make `trl_amd.AdamW`.
 `unpatch_trl()` restores the originals.
 """
 from __future__ import annotations
 
+import importlib
 import sys
 
+from .trainer import adamw as _adamw
 from .trainer import grpo_trainer as _grpo
 from .trainer import utils as _utils
 
@@ -33,7 +37,16 @@ def _set(mod, name, value) -> None:
     setattr(mod, name, value)
 
 
-def patch_trl(grpo: bool = True, liger: bool = False, dpo: bool = False, rloo: bool = False, kto: bool = False) -> int:
+def _with_adamw(original):
+    """A `get_optimizer_cls_and_kwargs` that asks `trl_amd` first."""
+    def get_optimizer_cls_and_kwargs(args, model=None):
+        return _adamw.optimizer_cls_and_kwargs(args) or original(args, model)
+
+    return staticmethod(get_optimizer_cls_and_kwargs)
+
+
+def patch_trl(grpo: bool = True, liger: bool = False, dpo: bool = False, rloo: bool = False, kto: bool = False,
+              adamw: bool = False) -> int:
     """Returns the number of names rebound.  Needs `trl` to be importable."""
     import trl.trainer.utils as ref_utils
 
@@ -120,6 +133,15 @@ def patch_trl(grpo: bool = True, liger: bool = False, dpo: bool = False, rloo: b
             pass
         _set(ref_dpo, "is_liger_kernel_available", lambda *a, **k: True)
         count += 4
+    if adamw:
+        for kind, name in (("grpo", "GRPOTrainer"), ("dpo", "DPOTrainer"), ("rloo", "RLOOTrainer"), ("kto", "KTOTrainer"), ("sft", "SFTTrainer")):
+            try:
+                cls = getattr(importlib.import_module(f"trl.trainer.{kind}_trainer"), name)
+            except (ImportError, AttributeError):
+                continue
+            _saved.append((cls, "get_optimizer_cls_and_kwargs", cls.__dict__.get("get_optimizer_cls_and_kwargs", _MISSING)))
+            cls.get_optimizer_cls_and_kwargs = _with_adamw(cls.get_optimizer_cls_and_kwargs)
+            count += 1
     return count
 
 

@@ -7,7 +7,7 @@ from torch import Tensor
 
 from .. import ops
 
-__all__ = ["adamw_step_", "adamw_state_values", "AdamW"]
+__all__ = ["adamw_step_", "adamw_state_values", "AdamW", "optimizer_cls_and_kwargs"]
 
 STATE_BLOCK = 256  # entries of 8-bit moments that share a scale
 
@@ -104,6 +104,7 @@ class AdamW(torch.optim.Optimizer):
                 grads.append(p.grad)
                 states.append(self._state_of(p, group))
                 group_of.append(i)
+        self.grad_norm = None
         if not params:
             return loss
         none = params[0].new_empty(0, dtype=torch.float32)
@@ -116,10 +117,31 @@ class AdamW(torch.optim.Optimizer):
         return loss
 
     def load_state_dict(self, state_dict: dict) -> None:
-        """As the base class, except that the moments keep their own types (it would cast them to the parameters')."""
+        """As the base class, except that the moments keep their own types (it would cast them to the parameters').  The state of a
+        `torch.optim.AdamW` is taken too: its moments become fp32 and its step counters move to the parameters' device."""
         super().load_state_dict(state_dict)
+        for group in self.param_groups:
+            for k, v in self.defaults.items():
+                group.setdefault(k, v)
         ids = [i for g in state_dict["param_groups"] for i in g["params"]]
         params = [p for g in self.param_groups for p in g["params"]]
         for i, p in zip(ids, params):
             if i in state_dict["state"]:
-                self.state[p] = {k: v.to(device=p.device, copy=True) if torch.is_tensor(v) else v for k, v in state_dict["state"][i].items()}
+                saved = state_dict["state"][i]
+                names = ("step", "exp_avg", "exp_avg_sq", "exp_avg_scale", "exp_avg_sq_scale")
+                self.state[p] = {k: torch.as_tensor(saved[k]).to(device=p.device, copy=True) for k in names if k in saved}
+                for k, v in self.state[p].items():
+                    if "exp_avg_scale" not in saved:
+                        self.state[p][k] = v.float()
+
+
+_STATE_BITS = {"adamw_torch": 32, "adamw_torch_fused": 32, "adamw_8bit": 8, "adamw_bnb_8bit": 8}  # names of `TrainingArguments.optim`
+
+
+def optimizer_cls_and_kwargs(args) -> tuple[type, dict] | None:
+    """`AdamW` and its arguments for training arguments whose `optim` is an AdamW, plain or with 8-bit states; `None` for others.  What
+    `transformers.Trainer.get_optimizer_cls_and_kwargs` returns, and its trainers take as `optimizer_cls_and_kwargs`."""
+    bits = _STATE_BITS.get(getattr(args.optim, "value", args.optim))
+    if bits is None:
+        return None
+    return AdamW, dict(lr=args.learning_rate, betas=(args.adam_beta1, args.adam_beta2), eps=args.adam_epsilon, state_bits=bits)
