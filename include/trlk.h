@@ -449,7 +449,8 @@ int trlk_scale_unless_one(void* d_data, int dtype, int64_t n_elems, const float*
  * > 1: 1).  A row without a distribution (a NaN or +inf, nothing but -inf, or a temperature that is negative, infinite or NaN, a
  * NaN top_p or min_p) gets the token -1 and a NaN log-prob, and sets TRLK_FLAG_NO_DISTRIBUTION in *d_error_flag (may be NULL).
  * d_row_mask (optional, uint8 [rows]): rows whose mask is 0 are not read, and get the token fill_id and the log-prob 0.
- * d_uniform: numbers in [0, 1), fp64 if uniform_f64 is non-zero, else fp32.  vocab <= trlk_token_filter_max_vocab().
+ * d_uniform: numbers in [0, 1), fp64 if uniform_f64 is non-zero, else fp32.  vocab <= trlk_token_filter_max_vocab().  Fewer than 2^23
+ * rows, and than 2^26 / (ceil(vocab / 2048) + 1).
  * d_workspace: trlk_token_filter_workspace_bytes(rows, vocab, dtype) bytes, 16-byte aligned.
  */
 int64_t trlk_token_filter_max_vocab(void);
@@ -490,7 +491,7 @@ int trlk_filtered_logps_bwd(const void* d_logits, int dtype, int64_t n_seq, int6
  *   t += 1;  m = beta1 m + (1 - beta1) clip g;  v = beta2 v + (1 - beta2) (clip g)^2
  *   p = p (1 - lr weight_decay) - lr / (1 - beta1^t) * m / (sqrt(v) / sqrt(1 - beta2^t) + eps)
  * in fp32, p rounded once to its type.  The tables are HOST memory, read before the call returns.  All operands of a tensor have
- * `numel` entries in the same order; no two tensors share one.  d_step (fp32, device) counts the tensor's steps.
+ * `numel` (2^34 at most) entries in the same order; no two tensors share one.  d_step (fp32, device) counts the tensor's steps.
  *   state_bits 32: d_exp_avg, d_exp_avg_sq fp32
  *   state_bits 8:  codes of one byte in blocks of 256 entries, with fp32 scales (powers of two), one per block
  *                  exp_avg: sign, 4 bits of exponent (bias 7), 3 of mantissa (e4m3);  exp_avg_sq: 4 bits of exponent (bias 7), 4

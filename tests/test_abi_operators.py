@@ -146,3 +146,27 @@ def test_host_code_is_clean_under_asan_and_ubsan():
     assert run.returncode == 0, report
     assert "AddressSanitizer" not in report and "runtime error:" not in report, report
     assert " passed" in run.stdout
+
+
+def test_launches_that_would_have_too_many_threads_are_refused():
+    from trl_amd import _lib
+
+    def sample(n_seq, rows, vocab):
+        return _lib.lib.trlk_sample_tokens(FAKE, _lib.BF16, n_seq, rows, vocab, rows * vocab, vocab, FAKE, 0, 1.0, None, 0, None, 1.0, None, 0.0, None,
+                                           None, 0, FAKE, FAKE, None, FAKE, 1 << 10, None)
+
+    def grad(n_seq, rows, vocab):
+        return _lib.lib.trlk_filtered_logps_bwd(FAKE, _lib.F32, n_seq, rows, vocab, rows * vocab, vocab, FAKE, 1.0, None, FAKE, None, FAKE, FAKE, None)
+
+    for call in (sample, grad):
+        for shape in ((1, 1 << 23, 8), (1 << 12, 1 << 11, 8), (1 << 62, 4, 8), (1, (1 << 26) // 76 + 1, 151936)):
+            assert call(*shape) == -2 and "rows" in _lib.last_error()
+    assert sample(1, (1 << 23) - 1, 8) == -6  # (rows that fit: the workspace does not)
+    assert sample(1, (1 << 26) // 76 - 8, 151936) == -6
+    t = Tensor(FAKE, FAKE, FAKE, FAKE, FAKE, FAKE, FAKE, (1 << 34) + 1, _lib.BF16, 32, 0, 0)
+    g = Group(1e-3, 0.9, 0.999, 1e-8, 0.0, None)
+    step = lambda: _lib.lib.trlk_adamw_step(ctypes.addressof(t), 1, ctypes.addressof(g), 1, 1.0, 0, FAKE, FAKE, 16, None)  # noqa: E731
+    assert step() == -2
+    t.numel = 1 << 34
+    assert step() == -6
+    assert _lib.lib.trlk_adamw_state_values(FAKE, FAKE, (1 << 34) + 1, 1, FAKE, None) == -2

@@ -29,6 +29,9 @@ constexpr int kTable32 = 83;             // tensors of an update launch with fp3
 constexpr int kTable8 = 62;              // with 8-bit moments                             (4 KB)
 constexpr int kNormTable = 250;          // pieces of tensors of a norm launch             (4 KB)
 constexpr int64_t kNormPiece = int64_t(1) << 31;
+constexpr int64_t kMaxGroups = (int64_t(1) << 32) / kThreads - 1;  // of a launch: it has fewer than 2^32 threads
+constexpr int64_t kMaxNumel = int64_t(1) << 34;
+static_assert(kMaxNumel / kChunk <= kMaxGroups && kNormPiece / kNormChunk <= kMaxGroups, "a tensor, or a piece of one, fits into a launch");
 constexpr int kStepTable = 240;          // tensors of a launch of the step counters
 
 // ---- scalars that the update reads: one record per tensor -------------------------------------------------------------
@@ -455,7 +458,7 @@ void update(const trlk_adamw_tensor* tensors, int32_t n_tensors, const Scalars* 
         const trlk_adamw_tensor& x = tensors[i];
         if (x.dtype != DT || x.state_bits != BITS || x.numel == 0) continue;
         const int64_t need = chunks(x.numel, kChunk);
-        if (t.n == UpdateTable<BITS>::kSize || grid + need > (int64_t(1) << 31) - 1) flush();
+        if (t.n == UpdateTable<BITS>::kSize || grid + need > kMaxGroups) flush();
         const size_t state_align = BITS == 32 ? 16 : 8, value_align = BITS == 32 && DT != TRLK_F32 ? 8 : 16;
         UpdateEntry<BITS>& e = t.e[t.n++];
         e.param = x.d_param, e.grad = x.d_grad, e.exp_avg = x.d_exp_avg, e.exp_avg_sq = x.d_exp_avg_sq;
@@ -477,7 +480,7 @@ int check_adamw(const trlk_adamw_tensor* t, int32_t n, const trlk_adamw_group* g
                      "adamw: lr, eps and weight_decay must not be negative");
     }
     for (int32_t i = 0; i < n; ++i) {
-        TRLK_REQUIRE(t[i].numel >= 0 && t[i].numel < (int64_t(1) << 42), TRLK_ERR_BAD_SHAPE, "adamw: tensor %d has %lld entries", i, (long long)t[i].numel);
+        TRLK_REQUIRE(t[i].numel >= 0 && t[i].numel <= kMaxNumel, TRLK_ERR_BAD_SHAPE, "adamw: tensor %d has %lld entries", i, (long long)t[i].numel);
         TRLK_REQUIRE(t[i].dtype == TRLK_F32 || t[i].dtype == TRLK_BF16 || t[i].dtype == TRLK_F16, TRLK_ERR_BAD_DTYPE, "adamw: tensor %d: unsupported dtype %d", i, t[i].dtype);
         TRLK_REQUIRE(t[i].state_bits == 32 || t[i].state_bits == 8, TRLK_ERR_BAD_VALUE, "adamw: tensor %d: state_bits must be 8 or 32", i);
         TRLK_REQUIRE(t[i].group >= 0 && t[i].group < n_groups, TRLK_ERR_BAD_VALUE, "adamw: tensor %d is in no group", i);
@@ -536,7 +539,7 @@ extern "C" int trlk_adamw_step(const trlk_adamw_tensor* tensors, int32_t n_tenso
                 for (int64_t at = 0; at < tensors[i].numel; at += kNormPiece) {
                     const int64_t n = tensors[i].numel - at < kNormPiece ? tensors[i].numel - at : kNormPiece, need = chunks(n, kNormChunk);
                     const char* g = static_cast<const char*>(tensors[i].d_grad) + at * int64_t(elem_size(dtype));
-                    if (t.n == kNormTable || grid + need > (int64_t(1) << 30)) flush();
+                    if (t.n == kNormTable || grid + need > kMaxGroups) flush();
                     NormEntry& e = t.e[t.n++];
                     e.grad = g, e.numel = uint32_t(n), e.first = uint32_t(grid), e.aligned = aligned_to(g, 16);
                     grid += need;
@@ -585,7 +588,7 @@ extern "C" int trlk_adamw_step(const trlk_adamw_tensor* tensors, int32_t n_tenso
 
 extern "C" int trlk_adamw_state_values(const uint8_t* d_codes, const float* d_scales, int64_t n, int32_t has_sign, void* d_out_bf16, trlk_stream_t stream) {
     clear_error();
-    TRLK_REQUIRE(n >= 0 && n < (int64_t(1) << 41), TRLK_ERR_BAD_SHAPE, "adamw_state_values: bad size %lld", (long long)n);
+    TRLK_REQUIRE(n >= 0 && n <= kMaxNumel, TRLK_ERR_BAD_SHAPE, "adamw_state_values: bad size %lld", (long long)n);
     if (n == 0) return TRLK_OK;
     TRLK_REQUIRE(d_codes && d_scales && d_out_bf16, TRLK_ERR_NULL_POINTER, "adamw_state_values: null operand");
     TRLK_REQUIRE(aligned_to(d_out_bf16, 2), TRLK_ERR_BAD_STRIDE, "adamw_state_values: misaligned output");

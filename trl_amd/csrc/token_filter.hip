@@ -33,6 +33,7 @@ constexpr int kList = 4096;                  // blocks over the bound that are l
 constexpr int kPairs = 128;                  // candidates of which every pair is compared
 constexpr int kLine = 128;                   // bytes of a cache line
 constexpr int64_t kMaxVocab = int64_t(1) << 22;
+constexpr int64_t kMaxRows = (int64_t(1) << 32) / kSelThreads, kMaxUnits = (int64_t(1) << 32) / kWave - 8;
 
 typedef unsigned long long u64;
 #define TRLK_INLINE __attribute__((always_inline))
@@ -230,7 +231,7 @@ struct RowView {
     const void* logits;
     int64_t rows_per_seq, vocab, seq_stride, row_stride;
     template <int DT>
-    __device__ __forceinline__ const typename Elem<DT>::type* row(uint32_t r) const {  // (rows are fewer than 2^31)
+    __device__ __forceinline__ const typename Elem<DT>::type* row(uint32_t r) const {  // (rows are fewer than 2^23)
         const uint32_t b = r / uint32_t(rows_per_seq), t = r - b * uint32_t(rows_per_seq);
         return static_cast<const typename Elem<DT>::type*>(logits) + int64_t(b) * seq_stride + int64_t(t) * row_stride;
     }
@@ -279,7 +280,7 @@ __global__ __launch_bounds__(kScanThreads, 8) void filter_scan_kernel(ScanArgs a
     constexpr int EPV = Elem<DT>::EPV, NV = kChunk / (kWave * EPV), LPB = kBlock / EPV;  // LPB: lanes of a block
     const int lane = threadIdx.x & (kWave - 1);
     const uint32_t at_unit = __builtin_amdgcn_readfirstlane(int(blockIdx.x * (kScanThreads / kWave) + threadIdx.x / kWave));
-    const uint32_t at_row = at_unit / uint32_t(a.chunks);  // (units are fewer than 2^31)
+    const uint32_t at_row = at_unit / uint32_t(a.chunks);  // (units are fewer than 2^26)
     const int64_t unit = at_unit, row = at_row;
     if (row >= a.rows) return;
     const int chunk = int(at_unit - at_row * uint32_t(a.chunks));
@@ -1446,8 +1447,9 @@ int check_view(const RowView& x, int dtype, int64_t n_seq, const char* what) {
     TRLK_REQUIRE(x.rows_per_seq == 1 || x.row_stride >= x.vocab, TRLK_ERR_BAD_STRIDE, "%s: row_stride %lld is less than vocab %lld", what,
                  (long long)x.row_stride, (long long)x.vocab);
     TRLK_REQUIRE(n_seq == 1 || x.seq_stride >= 0, TRLK_ERR_BAD_STRIDE, "%s: negative seq_stride", what);
-    TRLK_REQUIRE(n_seq < (int64_t(1) << 31) && x.rows_per_seq < (int64_t(1) << 31) &&
-                     n_seq * x.rows_per_seq < (int64_t(1) << 31) / (chunks_of(x.vocab) + 1) - 8,
+    // (a launch has fewer than 2^32 threads: 512 for a row, 64 for a chunk of one)
+    TRLK_REQUIRE(n_seq < kMaxRows && x.rows_per_seq < kMaxRows && n_seq * x.rows_per_seq < kMaxRows &&
+                     n_seq * x.rows_per_seq * (chunks_of(x.vocab) + 1) < kMaxUnits,
                  TRLK_ERR_BAD_SHAPE, "%s: too many rows", what);
     TRLK_REQUIRE(x.logits, TRLK_ERR_NULL_POINTER, "%s: null logits", what);
     TRLK_REQUIRE(reinterpret_cast<uintptr_t>(x.logits) % elem_size(dtype) == 0, TRLK_ERR_BAD_STRIDE, "%s: misaligned logits", what);
