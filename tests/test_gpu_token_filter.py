@@ -548,3 +548,51 @@ def test_traced_calls_have_the_shapes():
         ids, lp = trl_amd.sample_tokens(x, torch.empty(2, 3, device=DEV), top_k=5)
         assert ids.shape == lp.shape == (2, 3) and ids.dtype == torch.int64 and lp.dtype == torch.float32
         assert trl_amd.filtered_logps(x, ids, top_p=0.9).shape == (2, 3)
+
+
+def test_top_k_beyond_32_bits():
+    """Values for each row as int64: those over any vocabulary keep all tokens, those under 0 switch the filter off."""
+    import trl_amd
+
+    logits, u = make_logits(6, 3001, "bf16", 231)
+    x, v = logits.to(DEV), u.to(DEV)
+    ks = torch.tensor([2**32 + 1, 2**40, 2**63 - 1, -(2**32) + 1, -(2**63), 7], device=DEV)
+    ids, lp = trl_amd.sample_tokens(x, v, top_k=ks)
+    scored = trl_amd.filtered_logps(x, ids, top_k=ks)
+    for i, k in enumerate((0, 0, 0, 0, 0, 7)):
+        want_id, want = trl_amd.sample_tokens(x[i], v[i], top_k=k)
+        assert ids[i] == want_id and lp[i] == want and scored[i] == want
+    trl_amd.check_device_errors()
+    with pytest.raises(RuntimeError):
+        trl_amd.sample_tokens(x, v, top_k=ks.cpu())
+    with pytest.raises(RuntimeError):
+        trl_amd.filtered_logps(x, ids, row_mask=torch.ones(6, dtype=torch.bool))
+
+
+def test_two_graphs_replayed_at_once():
+    """Two captured calls of different sizes on two streams, replayed side by side: neither touches what the other works with."""
+    import trl_amd
+
+    made, streams = [], [torch.cuda.Stream(), torch.cuda.Stream()]
+    for seed, (rows, V, dtype, s) in ((241, (90, 50257, "bf16", settings(1.0, 0, 0.95))), (242, (40, 32000, "fp32", settings(0.8, 40, 0.9)))):
+        logits, u = make_logits(rows, V, dtype, seed)
+        x, v = logits.to(DEV), u.to(DEV)
+        want = trl_amd.sample_tokens(x, v, **s)
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            ids, lp = trl_amd.sample_tokens(x, v, **s)
+        made.append((graph, ids, lp, want, x, v))
+    for _ in range(5):
+        for _, ids, lp, *_ in made:
+            ids.fill_(-7)
+            lp.fill_(-7.0)
+        for stream, (graph, *_) in zip(streams, made):
+            stream.wait_stream(torch.cuda.current_stream())
+            with torch.cuda.stream(stream):
+                graph.replay()
+        for stream in streams:
+            torch.cuda.current_stream().wait_stream(stream)
+        for _, ids, lp, want, *_ in made:
+            assert torch.equal(ids, want[0]) and torch.equal(lp, want[1])
+    trl_amd.check_device_errors()

@@ -89,3 +89,6 @@ def test_state_of_torch_adamw_is_taken():
     again.load_state_dict(ours.state_dict())
     assert all(torch.equal(again.state[b][k], ours.state[a][k])
                for a, b in zip(group["params"], again.param_groups[0]["params"]) for k in ("step", "exp_avg", "exp_avg_sq"))
+    for kw in (dict(amsgrad=True), dict(maximize=True)):
+        with pytest.raises(ValueError, match=next(iter(kw))):
+            again.load_state_dict(torch.optim.AdamW(theirs, **kw).state_dict())

@@ -21,6 +21,7 @@
 #include <torch/python.h>
 
 #include <algorithm>
+#include <limits>
 #include <cstdlib>
 #include <map>
 #include <mutex>
@@ -557,6 +558,10 @@ Tensor dpo_log_values(const Tensor& entropy_, const Tensor& row_stats_, const Te
 }
 
 // ---- tokens drawn from, and scored under, a filtered distribution ------------------------------------------------------
+// an operand is where the logits are
+void beside(const char* op, const Tensor& logits, const Tensor& t) {
+    TORCH_CHECK(t.device() == logits.device(), op, ": an operand is on ", t.device(), ", the logits are on ", logits.device());
+}
 // The sampling settings: a number for all rows, or a tensor with a value for each.
 struct Settings {
     double temperature, top_p, min_p;
@@ -567,13 +572,21 @@ struct Settings {
     const float* m() const { return fptr(min_ps); }
     const int32_t* k() const { return top_ks ? static_cast<const int32_t*>(operand(*top_ks)) : nullptr; }
 };
-Settings settings(const char* op, int64_t rows, double temperature, int64_t top_k, double top_p, double min_p,
+// int32, and what lies beyond it (all tokens, or no filter) at its ends
+Tensor int32_values(const Tensor& t) {
+    constexpr int64_t most = std::numeric_limits<int32_t>::max();
+    return t.scalar_type() == at::kInt ? t.contiguous() : t.to(at::kLong).clamp(-most, most).to(at::kInt).contiguous();
+}
+Settings settings(const char* op, const Tensor& logits, int64_t rows, double temperature, int64_t top_k, double top_p, double min_p,
                   const optional<Tensor>& temperatures, const optional<Tensor>& top_ks, const optional<Tensor>& top_ps,
                   const optional<Tensor>& min_ps) {
-    for (const optional<Tensor>* t : {&temperatures, &top_ks, &top_ps, &min_ps})
-        TORCH_CHECK_VALUE(!*t || (*t)->numel() == rows, op, ": a setting has ", *t ? (*t)->numel() : 0, " values for ", rows, " rows");
-    return {temperature, top_p, min_p, top_k, f32c(temperatures),
-            top_ks ? optional<Tensor>(top_ks->contiguous().to(at::kInt)) : std::nullopt, f32c(top_ps), f32c(min_ps)};
+    for (const optional<Tensor>* t : {&temperatures, &top_ks, &top_ps, &min_ps}) {
+        if (!*t) continue;
+        TORCH_CHECK_VALUE((*t)->numel() == rows, op, ": a setting has ", (*t)->numel(), " values for ", rows, " rows");
+        beside(op, logits, **t);
+    }
+    return {temperature, top_p, min_p, top_k, f32c(temperatures), top_ks ? optional<Tensor>(int32_values(*top_ks)) : std::nullopt, f32c(top_ps),
+            f32c(min_ps)};
 }
 // Logits [..., V] as rows [n_seq, rows_per_seq] with strides: where they lie if the strides say so, else a copy.
 struct Rows {
@@ -594,8 +607,9 @@ struct Rows {
     const void* data() const { return x.const_data_ptr(); }
 };
 // one byte for each row
-optional<Tensor> byte_mask(const char* op, const optional<Tensor>& mask, int64_t rows) {
+optional<Tensor> byte_mask(const char* op, const Tensor& logits, const optional<Tensor>& mask, int64_t rows) {
     if (!mask) return std::nullopt;
+    beside(op, logits, *mask);
     TORCH_CHECK_VALUE(mask->numel() == rows, op, ": the row mask has ", mask->numel(), " entries for ", rows, " rows");
     return mask->scalar_type() == at::kBool ? mask->contiguous() : mask->ne(0).contiguous();
 }
@@ -609,9 +623,10 @@ std::tuple<Tensor, Tensor> sample_tokens(const Tensor& logits, const Tensor& uni
     const c10::DeviceGuard guard(logits.device());
     const Rows r(logits);
     TORCH_CHECK_VALUE(uniforms_.numel() == r.count, "sample_tokens: ", uniforms_.numel(), " uniform numbers for ", r.count, " rows");
+    beside("sample_tokens", logits, uniforms_);
     const Tensor ids = at::empty(uniforms_.sizes(), logits.options().dtype(at::kLong)), logp = f32(logits, uniforms_.sizes());
-    const Settings s = settings("sample_tokens", r.count, temperature, top_k, top_p, min_p, temperatures, top_ks, top_ps, min_ps);
-    const optional<Tensor> mask = byte_mask("sample_tokens", row_mask, r.count);
+    const Settings s = settings("sample_tokens", logits, r.count, temperature, top_k, top_p, min_p, temperatures, top_ks, top_ps, min_ps);
+    const optional<Tensor> mask = byte_mask("sample_tokens", logits, row_mask, r.count);
     const bool f64 = uniforms_.scalar_type() == at::kDouble;
     const Tensor uniforms = f64 ? uniforms_.contiguous() : f32c(uniforms_);
     const size_t ws_bytes = trlk_token_filter_workspace_bytes(r.count, r.vocab, r.dtype);
@@ -631,8 +646,9 @@ Tensor3 filtered_logps_fwd(const Tensor& logits, const Tensor& index_, double te
     const Rows r(logits);
     TORCH_CHECK_VALUE(index_.numel() == r.count && index_.scalar_type() == at::kLong, "filtered_logps: ", index_.numel(), " ",
                       index_.scalar_type(), " token ids for ", r.count, " rows of int64");
-    const Settings s = settings("filtered_logps", r.count, temperature, top_k, top_p, min_p, temperatures, top_ks, top_ps, min_ps);
-    const optional<Tensor> mask = byte_mask("filtered_logps", row_mask, r.count);
+    beside("filtered_logps", logits, index_);
+    const Settings s = settings("filtered_logps", logits, r.count, temperature, top_k, top_p, min_p, temperatures, top_ks, top_ps, min_ps);
+    const optional<Tensor> mask = byte_mask("filtered_logps", logits, row_mask, r.count);
     const bool blocks = trlk_token_filter_has_blocks(s.temperature, s.t(), s.top_k, s.k(), s.top_p, s.p(), s.min_p, s.m()) != 0;
     const Tensor logp = f32(logits, index_.sizes()), state = f32(logits, {r.count, 4});
     const Tensor block_max = at::empty({blocks ? r.count : 0, trlk_token_filter_blocks(r.vocab)}, logits.options());

@@ -119,6 +119,9 @@ class AdamW(torch.optim.Optimizer):
     def load_state_dict(self, state_dict: dict) -> None:
         """As the base class, except that the moments keep their own types (it would cast them to the parameters').  The state of a
         `torch.optim.AdamW` is taken too: its moments become fp32 and its step counters move to the parameters' device."""
+        for k in ("amsgrad", "maximize"):
+            if any(g.get(k) for g in state_dict["param_groups"]):
+                raise ValueError(f"AdamW has no {k}")
         super().load_state_dict(state_dict)
         for group in self.param_groups:
             for k, v in self.defaults.items():
