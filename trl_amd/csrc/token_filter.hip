@@ -1029,10 +1029,6 @@ __global__ __launch_bounds__(kSelThreads, LONG ? 4 : 6) void filter_select_kerne
     // what lies before those three bins, and lists what lies in them, where the border is then found.
     if (LONG && n_cand > kCandidates && !f.top_k && x_low > -INFINITY) {
         const float scale = float(kBins - 1) / fmaxf(m - x_low, 1e-30f);
-        const auto bin_of = [&](float v) TRLK_INLINE {
-            const float t = (m - v) * scale;
-            return t < float(kBins) ? int(t) : kBins;
-        };
         // g(values, index of the first) for every vector, end(chunk) after a wave's half of a chunk (waves get as many halves each): 16 logits
         // of a lane at a time, the next in flight
         constexpr int G = 16 / EPV, kHalf = 16 * kWave;
@@ -1076,18 +1072,20 @@ __global__ __launch_bounds__(kSelThreads, LONG ? 4 : 6) void filter_select_kerne
             clear_bins(s, kBins);
             row_pass(
                 [&](const float(&v)[EPV], uint32_t) TRLK_INLINE {
-                    uint32_t w[EPV];
-                    int b[EPV];
 #pragma unroll
                     for (int e = 0; e < EPV; ++e) {
-                        w[e] = about(v[e]);
-                        b[e] = bin_of(v[e]);
+                        const uint32_t t = uint32_t((m - v[e]) * (256.f * scale));  // (infinity is the largest number)
+                        if (t < 256u * kBins) atomicAdd(&s.bins[t / 256u], u64(1) << 32 | t % 256u);
                     }
-#pragma unroll
-                    for (int e = 0; e < EPV; ++e)
-                        if (v[e] >= x_low) add_low(b[e], w[e]);
                 },
                 [](int) TRLK_INLINE {});
+            __syncthreads();
+            // how many tokens a bin has, times the weight at their mean (a bin is a hundredth of a power of two wide)
+            for (int i = tid; i < kBins; i += kSelThreads) {
+                const u64 all = s.bins[i];
+                const float n = float(uint32_t(all >> 32)), mean = (float(uint32_t(all)) / fmaxf(n, 1.f) + 0.5f) * (1.f / 256.f);
+                s.bins[i] = u64(n * fast_exp2(fmaf(-(float(i) + mean) / scale, cf, l2)) + 0.5f);
+            }
             __syncthreads();
             uint32_t bin;
             before = 0;
