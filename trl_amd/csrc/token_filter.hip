@@ -796,7 +796,9 @@ __global__ __launch_bounds__(kSelThreads, LONG ? 4 : 6) void filter_select_kerne
             bound = d < bound ? d : bound;
         }
     }
-    const auto in_bound = [&](float v) TRLK_INLINE { return v > -INFINITY && distance_bin(m, v) <= bound; };
+    // (the same bin or a nearer one: a distance of at most the largest number of that bin)
+    const float reach = bound < kEveryBin ? __uint_as_float((uint32_t(bound + (119 << 7) + 1) << 16) - 1u) : INFINITY;
+    const auto in_bound = [&](float v) TRLK_INLINE { return v > -INFINITY && m - v <= reach; };
 
     // ---- blocks that reach the bound, and the candidates in them
     each_max([&](int i, const float(&v)[EPV]) TRLK_INLINE {
@@ -815,45 +817,67 @@ __global__ __launch_bounds__(kSelThreads, LONG ? 4 : 6) void filter_select_kerne
     __syncthreads();
     const bool listed = s.n_list <= kList;
     const int n_visit = listed ? int(s.n_list) : n_blocks;
-    // the logits of those blocks, EPV blocks to a load of a wave: h(values, index of the first)
-    const auto blocks_pass = [&](auto h) TRLK_INLINE {
-        constexpr int LPB = kBlock / EPV, U = 2;
+    // the logits of those blocks, EPV blocks to a load of a wave and U loads together: g(vectors, indices of their first logits)
+    constexpr int U = LONG ? 4 : 2;
+    const auto blocks_raw = [&](auto g) TRLK_INLINE {
+        constexpr int LPB = kBlock / EPV;
         for (int j0 = wave * EPV; j0 < n_visit; j0 += U * kSelWaves * EPV) {
             u32x4 raw[U];
-            int64_t e[U];
+            int e[U];
 #pragma unroll
             for (int q = 0; q < U; ++q) {
                 const int j = j0 + q * kSelWaves * EPV + lane / LPB;
-                e[q] = j < n_visit ? int64_t(listed ? int(s.list[j]) : j) * kBlock + (lane & (LPB - 1)) * EPV : V;
-                if (e[q] + EPV <= V) {
+                e[q] = j < n_visit ? (listed ? int(s.list[j]) : j) * kBlock + (lane & (LPB - 1)) * EPV : int(V);
+                if (e[q] + EPV <= int(V)) {
                     raw[q] = *reinterpret_cast<const u32x4_u*>(x + e[q]);
                 } else {
                     float v[EPV];
 #pragma unroll
-                    for (int k = 0; k < EPV; ++k) v[k] = e[q] + k < V ? Elem<DT>::load1(x + e[q] + k) : -INFINITY;
+                    for (int k = 0; k < EPV; ++k) v[k] = e[q] + k < int(V) ? Elem<DT>::load1(x + e[q] + k) : -INFINITY;
                     raw[q] = Elem<DT>::pack(v);
                 }
             }
+            g(raw, e);
+        }
+    };
+    const auto blocks_pass = [&](auto h) TRLK_INLINE {  // h(values, index of the first)
+        blocks_raw([&](const u32x4(&raw)[U], const int(&e)[U]) TRLK_INLINE {
 #pragma unroll
             for (int q = 0; q < U; ++q) {
                 float v[EPV];
                 Elem<DT>::unpack(raw[q], v);
                 h(v, uint32_t(e[q]));
             }
-        }
+        });
     };
     // (where most blocks reach the bound there are thousands of candidates: such a row is passed over as a whole)
     const bool too_many = !f.top_k && n_visit > 256 && 2 * n_visit > n_blocks;
     if (!too_many) {
-        blocks_pass([&](const float(&v)[EPV], uint32_t e0) TRLK_INLINE {
-            uint32_t in = 0;
+        blocks_raw([&](const u32x4(&raw)[U], const int(&e0)[U]) TRLK_INLINE {
+            uint32_t in[U], count = 0;
 #pragma unroll
-            for (int e = 0; e < EPV; ++e) in |= in_bound(v[e]) ? 1u << e : 0u;
-            uint32_t to = reserve(&s.n_cand, __popc(in));
+            for (int q = 0; q < U; ++q) {
+                float v[EPV];
+                Elem<DT>::unpack(raw[q], v);
+                in[q] = 0;
 #pragma unroll
-            for (int e = 0; e < EPV; ++e) {
-                if (in >> e & 1u) {
-                    if (to < kCandidates) s.order[to] = order_of(v[e], e0 + e);
+                for (int e = 0; e < EPV; ++e) in[q] |= in_bound(v[e]) ? 1u << e : 0u;
+                count += __popc(in[q]);
+            }
+            uint32_t to = reserve(&s.n_cand, count);
+            // (a lane has one of a vector's logits, two at times: a turn for each, not a branch for each place)
+#pragma unroll
+            for (int q = 0; q < U; ++q) {
+                for (; in[q]; in[q] &= in[q] - 1) {
+                    const int e = __builtin_ctz(in[q]);
+                    uint32_t key;
+                    if constexpr (K::k16) {
+                        const uint32_t word = e & 4 ? (e & 2 ? raw[q].w : raw[q].z) : (e & 2 ? raw[q].y : raw[q].x);
+                        key = K::of(T(word >> (16 * (e & 1))));
+                    } else {
+                        key = K::of(__uint_as_float(e & 2 ? (e & 1 ? raw[q].w : raw[q].z) : (e & 1 ? raw[q].y : raw[q].x)));
+                    }
+                    if (to < kCandidates) s.order[to] = u64(key) << 32 | uint32_t(~(e0[q] + e));
                     ++to;
                 }
             }
