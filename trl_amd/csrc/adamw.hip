@@ -174,7 +174,14 @@ __global__ __launch_bounds__(1024) void step_kernel(StepTable t) {
     }
     if (!t.header) return;
     double sum = 0.0;
-    for (int64_t i = threadIdx.x; i < t.n_partial; i += 1024) sum += t.partial[i];
+    constexpr int U = 8;  // loads in flight
+    for (int64_t i = threadIdx.x; i < t.n_partial; i += U * 1024) {
+        double x[U];
+#pragma unroll
+        for (int j = 0; j < U; ++j) x[j] = i + j * 1024 < t.n_partial ? t.partial[i + j * 1024] : 0.0;
+#pragma unroll
+        for (int j = 0; j < U; ++j) sum += x[j];
+    }
 #pragma unroll
     for (int o = kWave / 2; o > 0; o >>= 1) sum += __shfl_xor(sum, o);
     if ((threadIdx.x & (kWave - 1)) == 0) scratch[threadIdx.x / kWave] = sum;
