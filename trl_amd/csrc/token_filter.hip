@@ -5,11 +5,20 @@
 // so what a row keeps is one border: a value, and among the tokens of exactly that value the last index.  With
 // w_v = exp((x_v - max) / T) for the kept tokens, a token is drawn as the first index whose cumulative weight exceeds u * W.
 //
-// Two launches.  filter_scan_kernel reads the logits once, a wave per chunk of 2048, and leaves the chunk's maximum, its sum of
-// weights in 64 bits and the maximum of every block of 64 logits.  filter_select_kernel has one workgroup per row: the block
-// maxima bound the border from below (the k-th largest of them is at most the k-th largest logit; blocks whose maxima hold
+// Two launches, three with the gradient.  filter_scan_kernel reads the logits once, a wave per chunk of 2048, and leaves the chunk's
+// maximum, its sum of weights in 64 bits and the maximum of every block of 64 logits.  filter_select_kernel has one workgroup per row:
+// the block maxima bound the border from below (the k-th largest of them is at most the k-th largest logit; blocks whose maxima hold
 // top_p of the mass hold the tokens of top-p), so that only blocks with a maximum over that bound are read again -- a few dozen of
-// some thousand -- and the border, the kept mass and the token come from those candidates.
+// some thousand.  What comes after goes by the number of candidates in them: up to 128 are compared pair by pair; of up to 4096 the border
+// is found in bins of distances from the maximum and then among the pairs of its bin, the token in its chunk; with more, without top-k,
+// the row is passed over twice more (a count in bins; exact sums, chunk by chunk, before the border's bin); the rest goes by a
+// radix descent.  filter_bwd_kernel writes the gradient once and reads only the blocks that reach the border.
+//
+// What bounds it, and what it takes (us, kernels alone): the scan the memory where there are no sums (4096 rows of 151936 in bf16, half
+// of them masked away: 129, 5.7 TB/s) or fp32 logits (384 rows of 151936: 46, 5.1 TB/s), the issue of its 10 operations of 64 bits per
+// logit with sums of 16-bit ones (256 rows of 128257: 24, 2.7 TB/s); the selection a workgroup's chain of barriers (8 to 10 for a short
+// nucleus, 20 for a long one) and in rows of very many candidates, which one CU passes over alone, LDS atomics and arithmetic (36 for
+// 50257 logits, 78 for 151936); the gradient the memory (4096 rows of 151936: 222, 5.6 TB/s).
 //
 // Whole numbers come out, and the same ones whatever the launch: sums of weights are 64-bit floats in a fixed order over a row's
 // chunks, or 64-bit integers (weights in units of 2^-fix, whose sums do not depend on the order in which threads add them).
@@ -546,7 +555,8 @@ __device__ __forceinline__ int first_thread(Shared& s, int which, bool owner, bo
     return r;
 }
 
-// LONG: rows may have no top-k, and so any number of tokens, or no filter at all.  Without, three workgroups fit into a CU instead of two.
+// LONG: rows may have no top-k, and so any number of tokens, or no filter at all.  Without, three workgroups fit into a CU instead of two:
+// 4096 rows of 151936 with top-k and top-p 39 us instead of 50.
 template <int DT, bool SCORE, bool LONG>
 __global__ __launch_bounds__(kSelThreads, LONG ? 4 : 6) void filter_select_kernel(SelectArgs a) {
     typedef typename Elem<DT>::type T;
@@ -850,7 +860,8 @@ __global__ __launch_bounds__(kSelThreads, LONG ? 4 : 6) void filter_select_kerne
             }
         });
     };
-    // (where most blocks reach the bound there are thousands of candidates: such a row is passed over as a whole)
+    // (where most blocks reach the bound there are thousands of candidates: such a row is passed over as a whole.  384 rows of 151936 in fp32
+    // 78 us instead of 110 with the attempt to list them first)
     const bool too_many = !f.top_k && n_visit > 256 && 2 * n_visit > n_blocks;
     if (!too_many) {
         blocks_raw([&](const u32x4(&raw)[U], const int(&e0)[U]) TRLK_INLINE {
