@@ -8,8 +8,8 @@
 // moves every tensor's step counter on (so that a captured step counts when it is replayed), the update.  Tensors come as tables
 // in the kernels' arguments: nothing is copied to the device, and a captured graph holds its own.  Measured on 355M entries: norm 229 us in
 // fp32 (6.2 TB/s), 119 in bf16 (6.0); update 1720 us in fp32 with fp32 moments (5.8 TB/s), 405 for 117M in bf16 (6.3), 660 to 750 in bf16
-// with 8-bit moments (4.8 to 5.4: the hash and the rounding take as long as the memory).  With adapters, 224 tensors of 40000 entries, the
-// three or four launches' beginnings and ends are a third of the 61 us.
+// with 8-bit moments (4.8 to 5.4: the hash and the rounding take as long as the memory).  With adapters, 224 tensors of 8192 to 81920
+// entries in fp32, the five launches' beginnings and ends are a third of the 66 us.
 //
 // 8-bit moments: blocks of 256 entries with a power-of-two scale that takes the block's largest entry to at most 448.  m has a
 // sign, 4 bits of exponent and 3 of mantissa (the OCP e4m3 format); v, which is not negative, 4 and 4 and keeps a code over 0
