@@ -596,3 +596,48 @@ def test_two_graphs_replayed_at_once():
         for _, ids, lp, want, *_ in made:
             assert torch.equal(ids, want[0]) and torch.equal(lp, want[1])
     trl_amd.check_device_errors()
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
+@pytest.mark.parametrize("rows", [1, 20, 63, 530])
+def test_rows_of_very_many_candidates_side_by_side(rows, dtype):
+    """Nuclei of thousands of tokens: as many as all CUs pass over together, more, and so many rows that none is; with short nuclei between
+    them, a border among equal logits, and min-p beside top-p."""
+    import trl_amd
+
+    V = 9001 if rows > 1 else 50257
+    logits, u = make_logits(rows, V, dtype, 250 + rows, slope=0.5)
+    logits[::5] *= 6.0  # short nuclei
+    if rows > 3:
+        logits[3] = 1.5  # equal logits
+        logits[2, : V // 2] = 2.0
+    for s in (settings(0.9, 0, 0.9), settings(1.0, 0, 0.97, 0.02), settings(1.2, 0, 1.0, 1e-3)):
+        check_draw(logits, u, s)
+        x = logits.to(DEV)
+        ids, lp = trl_amd.sample_tokens(x, u.to(DEV), **s)
+        for _ in range(3):
+            again = trl_amd.sample_tokens(x, u.to(DEV), **s)
+            assert torch.equal(again[0], ids) and torch.equal(again[1], lp)
+        assert torch.equal(trl_amd.filtered_logps(x, ids, **s), lp)
+        one = trl_amd.sample_tokens(x[rows - 1], u[rows - 1].to(DEV), **s)
+        assert one[0] == ids[rows - 1] and one[1] == lp[rows - 1]
+
+
+def test_a_border_between_two_distant_tokens():
+    """The nucleus ends where the next token lies far below the last one, and its mass is within 1e-5 of top_p on one side or the other:
+    thousands of tokens of little mass follow."""
+    import trl_amd
+
+    V, heads = 20000, 12
+    g = torch.Generator().manual_seed(271)
+    x = torch.full((40, V), -3.0) + 0.5 * torch.rand(40, V, generator=g)
+    for i in range(40):
+        x[i, torch.randperm(V, generator=g)[:heads]] = torch.linspace(7.0, 1.0, heads) + 0.3 * torch.rand(heads, generator=g)
+    u = torch.rand(40, generator=g)
+    order = x.double().sort(-1, descending=True).values
+    mass = order.softmax(-1).cumsum(-1)
+    for at, off in ((heads - 1, 1e-6), (heads - 1, -1e-6), (heads - 2, 1e-5), (heads - 2, -1e-5), (5, 3e-5), (5000, 0.0)):
+        p = (mass[:, at] + off).float()
+        check_draw(x, u, settings(1.0, 0, p))
+        ids, lp = trl_amd.sample_tokens(x.to(DEV), u.to(DEV), top_p=p.to(DEV))
+        assert torch.equal(trl_amd.filtered_logps(x.to(DEV), ids, top_p=p.to(DEV)), lp)

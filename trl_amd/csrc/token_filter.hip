@@ -5,20 +5,21 @@
 // so what a row keeps is one border: a value, and among the tokens of exactly that value the last index.  With
 // w_v = exp((x_v - max) / T) for the kept tokens, a token is drawn as the first index whose cumulative weight exceeds u * W.
 //
-// Two launches, three with the gradient.  filter_scan_kernel reads the logits once, a wave per chunk of 2048, and leaves the chunk's
+// Two launches or four, and one for the gradient.  filter_scan_kernel reads the logits once, a wave per chunk of 2048, and leaves the chunk's
 // maximum, its sum of weights in 64 bits and the maximum of every block of 64 logits.  filter_select_kernel has one workgroup per row:
 // the block maxima bound the border from below (the k-th largest of them is at most the k-th largest logit; blocks whose maxima hold
 // top_p of the mass hold the tokens of top-p), so that only blocks with a maximum over that bound are read again -- a few dozen of
 // some thousand.  What comes after goes by the number of candidates in them: up to 128 are compared pair by pair; of up to 4096 the border
 // is found in bins of distances from the maximum and then among the pairs of its bin, the token in its chunk; with more, without top-k,
-// the row is passed over twice more (a count in bins; exact sums, chunk by chunk, before the border's bin); the rest goes by a
+// the row is passed over twice more (a count in bins; exact sums, chunk by chunk, before the border's bin), by its workgroup or, of up to
+// 512 rows, by all CUs in two more launches (filter_count_kernel, filter_select_kernel<.., true>); the rest goes by a
 // radix descent.  filter_bwd_kernel writes the gradient once and reads only the blocks that reach the border.
 //
 // What bounds it, and what it takes (us, kernels alone): the scan the memory where there are no sums (4096 rows of 151936 in bf16, half
 // of them masked away: 129, 5.7 TB/s) or fp32 logits (384 rows of 151936: 46, 5.1 TB/s), the issue of its 10 operations of 64 bits per
 // logit with sums of 16-bit ones (256 rows of 128257: 24, 2.7 TB/s); the selection a workgroup's chain of barriers (8 to 10 for a short
-// nucleus, 20 for a long one) and in rows of very many candidates, which one CU passes over alone, LDS atomics and arithmetic (36 for
-// 50257 logits, 78 for 151936); the gradient the memory (4096 rows of 151936: 222, 5.6 TB/s).
+// nucleus, 20 for a long one), and where one CU passes over a row of very many candidates alone, its LDS atomics and arithmetic (36 for
+// 50257 logits, 78 for 151936; 25 in parts, 8 for their launches where there is no such row); the gradient the memory (4096 rows of 151936: 222, 5.6 TB/s).
 //
 // Whole numbers come out, and the same ones whatever the launch: sums of weights are 64-bit floats in a fixed order over a row's
 // chunks, or 64-bit integers (weights in units of 2^-fix, whose sums do not depend on the order in which threads add them).
@@ -41,6 +42,8 @@ constexpr int kMaxCandidates = 4096;         // that are kept in LDS; rows with 
 constexpr int kList = 4096;                  // blocks over the bound that are listed; with more every block is looked at
 constexpr int kPairs = 128;                  // candidates of which every pair is compared
 constexpr int kLine = 128;                   // bytes of a cache line
+constexpr int kLongRows = 32;                // rows with very many candidates whose passes all CUs share
+constexpr int kHalf = kChunk / 2;            // logits of a wave's step in these passes
 constexpr int64_t kMaxVocab = int64_t(1) << 22;
 constexpr int64_t kMaxRows = (int64_t(1) << 32) / kSelThreads, kMaxUnits = (int64_t(1) << 32) / kWave - 8;
 
@@ -250,6 +253,26 @@ struct RowView {
     }
 };
 
+// ---- rows with very many candidates ------------------------------------------------------------------------------------
+// What the selection leaves of such a row for the two launches behind it, which pass over it in parts.
+struct alignas(64) LongRow {
+    double sum;      // of the row's weights
+    u64 mass;        // before the bins that have the border
+    float m, x_low;  // the row's maximum, and what no candidate lies under
+    uint32_t row, n_zone, min_key, done;
+    __device__ u64* bins() { return reinterpret_cast<u64*>(this + 1); }
+    __device__ u64* zone() { return bins() + kBins; }
+};
+constexpr size_t kLongRowBytes = sizeof(LongRow) + sizeof(u64) * (kBins + kMaxCandidates);
+struct LongRows {
+    uint32_t* count;  // null: no row can be one.  More rows than there are slots are passed over by their own workgroups
+    char* slots;
+    uint32_t n_slots;
+    int32_t parts;    // workgroups that share a row's pass, one half chunk to a wave
+    __device__ LongRow* at(uint32_t i) const { return reinterpret_cast<LongRow*>(slots + i * kLongRowBytes); }
+    __device__ bool has(uint32_t i) const { return i < *count; }
+};
+
 // ---- scan ------------------------------------------------------------------------------------------------------------
 struct ScanArgs {
     RowView x;
@@ -260,6 +283,7 @@ struct ScanArgs {
     double* chunk_sum;  // [rows, chunks] or null
     float* chunk_max;   // [rows, chunks]
     void* block_max;    // [rows, chunks * kBlocksPerChunk] in the logits' type, or null
+    uint32_t* long_count;  // set to 0, or null
 };
 
 // NV vectors of a lane: vector i holds the logits (i * 64 + lane) * EPV on of those at p.  What lies behind the n there are is -inf.
@@ -287,11 +311,29 @@ __device__ __forceinline__ void load_vectors(const typename Elem<DT>::type* p, i
     }
 }
 
+template <int DT, int NV>
+__device__ __forceinline__ void load_raw(const typename Elem<DT>::type* p, int64_t n, int lane, u32x4 (&q)[NV]) {
+    constexpr int EPV = Elem<DT>::EPV;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+        const int at = (i * kWave + lane) * EPV;
+        if (at + EPV <= n) {
+            q[i] = *reinterpret_cast<const u32x4_u*>(p + at);
+        } else {
+            float x[EPV];
+#pragma unroll
+            for (int e = 0; e < EPV; ++e) x[e] = at + e < n ? Elem<DT>::load1(p + at + e) : -INFINITY;
+            q[i] = Elem<DT>::pack(x);
+        }
+    }
+}
+
 template <int DT, bool SUMS, bool BLOCKS>
 __global__ __launch_bounds__(kScanThreads, 8) void filter_scan_kernel(ScanArgs a) {
     typedef typename Elem<DT>::type T;
     constexpr int EPV = Elem<DT>::EPV, NV = kChunk / (kWave * EPV), LPB = kBlock / EPV;  // LPB: lanes of a block
     __shared__ double roots[SUMS ? kRoots : 1];
+    if (blockIdx.x == 0 && threadIdx.x == 0 && a.long_count) *a.long_count = 0;
     if constexpr (SUMS) {
         if (threadIdx.x < kRoots) roots[threadIdx.x] = stored_root(int(threadIdx.x));
         __syncthreads();
@@ -362,6 +404,7 @@ struct SelectArgs {
     float* out_state;      // score: [rows, 4]: border value, border index (bits), maximum, log2 of the kept mass in units of its weight
     float* out_logp;
     int32_t* error_flag;
+    LongRows longs;
 };
 
 // A place for one number of each wave.  Two neighbouring block-wide sums take different ones, so that a barrier lies between a
@@ -534,6 +577,17 @@ __device__ __forceinline__ int distance_bin(float m, float x) {
 }
 constexpr int kEveryBin = 1 << 30;
 
+// Bins of a row with very many candidates: the logits down to x_low, and of each bin the count and the sum of the places in it, in 256ths.
+__device__ __forceinline__ float bins_per_logit(float m, float x_low) { return float(kBins - 1) / fmaxf(m - x_low, 1e-30f); }
+template <int N>
+__device__ __forceinline__ void count_in_bins(const float (&v)[N], float m, float scale, u64* bins) {
+#pragma unroll
+    for (int e = 0; e < N; ++e) {
+        const uint32_t t = uint32_t((m - v[e]) * (256.f * scale));  // (infinity is the largest number)
+        if (t < 256u * kBins) atomicAdd(&bins[t / 256u], u64(1) << 32 | t % 256u);
+    }
+}
+
 // `owner` of the smallest thread number, and if there is none of the largest with `some`: its number, the same for all threads
 template <typename Shared>
 __device__ __forceinline__ int first_thread(Shared& s, int which, bool owner, bool some) {
@@ -557,7 +611,8 @@ __device__ __forceinline__ int first_thread(Shared& s, int which, bool owner, bo
 
 // LONG: rows may have no top-k, and so any number of tokens, or no filter at all.  Without, three workgroups fit into a CU instead of two:
 // 4096 rows of 151936 with top-k and top-p 39 us instead of 50.
-template <int DT, bool SCORE, bool LONG>
+// SECOND: a part of the second pass over one of the rows that the selection has left; the workgroup that is through last goes on alone.
+template <int DT, bool SCORE, bool LONG, bool SECOND = false>
 __global__ __launch_bounds__(kSelThreads, LONG ? 4 : 6) void filter_select_kernel(SelectArgs a) {
     typedef typename Elem<DT>::type T;
     typedef Key<DT> K;
@@ -567,7 +622,9 @@ __global__ __launch_bounds__(kSelThreads, LONG ? 4 : 6) void filter_select_kerne
     constexpr int kCandidates = LONG ? kMaxCandidates : kMaxCandidates / 2;
     __shared__ SelectShared<kCandidates> s;
     const int tid = threadIdx.x, lane = tid & (kWave - 1), wave = tid / kWave;
-    const int64_t row = blockIdx.x, V = a.x.vocab;
+    LongRow* const left = SECOND ? a.longs.at(blockIdx.y) : nullptr;
+    if (SECOND && !a.longs.has(blockIdx.y)) return;
+    const int64_t row = SECOND ? left->row : blockIdx.x, V = a.x.vocab;
     // what a row without a token, or without a distribution, returns
     const auto nothing = [&](int64_t id, float logp) TRLK_INLINE {
         if (tid != 0) return;
@@ -579,14 +636,14 @@ __global__ __launch_bounds__(kSelThreads, LONG ? 4 : 6) void filter_select_kerne
         }
         a.out_logp[row] = logp;
     };
-    if (a.row_mask && a.row_mask[row] == 0) return nothing(a.fill_id, 0.f);
+    if (!SECOND && a.row_mask && a.row_mask[row] == 0) return nothing(a.fill_id, 0.f);
     // (what every row needs is on its way before the row's settings are known)
     const float* cmax = a.chunk_max + row * a.chunks;
     double* csum = a.chunk_sum + row * a.chunks;
     const int n_blocks = a.chunks * kBlocksPerChunk, n_vec = n_blocks / EPV;  // (blocks behind the row's end are -inf)
     const u32x4* bmax = reinterpret_cast<const u32x4*>(static_cast<const T*>(a.block_max) + row * n_blocks);
     u32x4 held[kKeep] = {};
-    if (a.has_blocks) {
+    if (!SECOND && a.has_blocks) {
 #pragma unroll
         for (int j = 0; j < kKeep; ++j)
             if (tid + j * kSelThreads < n_vec) held[j] = bmax[tid + j * kSelThreads];
@@ -594,18 +651,20 @@ __global__ __launch_bounds__(kSelThreads, LONG ? 4 : 6) void filter_select_kerne
     const int per = (a.chunks + kSelThreads - 1) / kSelThreads, first = tid * per, last = first + per < a.chunks ? first + per : a.chunks;
     double sum0 = 0.0;  // this thread's first chunk
     float max0 = -INFINITY;
-    if (LONG && a.has_sums && first < last) {
+    if (LONG && !SECOND && a.has_sums && first < last) {
         sum0 = csum[first];
         max0 = cmax[first];
     }
     const RowFilter f = row_filter(a.f, row, V);
-    const bool filtered = !LONG || f.top_k || f.top_p > 0.0 || f.min_p > 0.0;
+    const bool filtered = !LONG || SECOND || f.top_k || f.top_p > 0.0 || f.min_p > 0.0;
     const bool with_sum = LONG && (!filtered || (f.top_p > 0.0 && !f.top_k));
     const T* x = a.x.row<DT>(uint32_t(row));
 
     // the row's maximum: of its blocks, or of its chunks where there are no blocks
     float m = -INFINITY;
-    if (filtered) {
+    if (SECOND) {
+        m = left->m;
+    } else if (filtered) {
 #pragma unroll
         for (int j = 0; j < kKeep; ++j) {
             float v[EPV];
@@ -685,7 +744,9 @@ __global__ __launch_bounds__(kSelThreads, LONG ? 4 : 6) void filter_select_kerne
 
     // the row's sum of weights, and this thread's chunks' place in it
     double S = 0.0, mine = 0.0, base = 0.0, upto = 0.0;
-    if (with_sum) {
+    if (SECOND) {
+        S = left->sum;
+    } else if (with_sum) {
         if (first < last) mine = chunk_weight(sum0, max0);
         for (int i = first + 1; i < last; ++i) mine += chunk_weight(csum[i], cmax[i]);
         base = block_scan(mine, s.slots[1], upto, S);
@@ -777,7 +838,9 @@ __global__ __launch_bounds__(kSelThreads, LONG ? 4 : 6) void filter_select_kerne
     }();
     int bound = kEveryBin;
     float x_low = -INFINITY;  // no candidate lies under it
-    {
+    if (SECOND) {
+        x_low = left->x_low;
+    } else {
         const bool by_count = f.top_k != 0, by_mass = !by_count && f.top_p > 0.0;
         if (by_count || by_mass) {
             each_max([&](int, const float(&v)[EPV]) TRLK_INLINE {
@@ -811,7 +874,7 @@ __global__ __launch_bounds__(kSelThreads, LONG ? 4 : 6) void filter_select_kerne
     const auto in_bound = [&](float v) TRLK_INLINE { return v > -INFINITY && m - v <= reach; };
 
     // ---- blocks that reach the bound, and the candidates in them
-    each_max([&](int i, const float(&v)[EPV]) TRLK_INLINE {
+    if (!SECOND) each_max([&](int i, const float(&v)[EPV]) TRLK_INLINE {
         uint32_t in = 0;
 #pragma unroll
         for (int e = 0; e < EPV; ++e) in |= in_bound(v[e]) ? 1u << e : 0u;
@@ -825,7 +888,7 @@ __global__ __launch_bounds__(kSelThreads, LONG ? 4 : 6) void filter_select_kerne
         }
     });
     __syncthreads();
-    const bool listed = s.n_list <= kList;
+    const bool listed = !SECOND && s.n_list <= kList;
     const int n_visit = listed ? int(s.n_list) : n_blocks;
     // the logits of those blocks, EPV blocks to a load of a wave and U loads together: g(vectors, indices of their first logits)
     constexpr int U = LONG ? 4 : 2;
@@ -860,9 +923,9 @@ __global__ __launch_bounds__(kSelThreads, LONG ? 4 : 6) void filter_select_kerne
             }
         });
     };
-    // (where most blocks reach the bound there are thousands of candidates: such a row is passed over as a whole.  384 rows of 151936 in fp32
-    // 78 us instead of 110 with the attempt to list them first)
-    const bool too_many = !f.top_k && n_visit > 256 && 2 * n_visit > n_blocks;
+    // (where most blocks reach the bound there are thousands of candidates: such a row is passed over as a whole.  1000 rows of 50257 in fp32
+    // 44 us instead of 58 with the attempt to list them first)
+    const bool too_many = SECOND || (!f.top_k && n_visit > 256 && 2 * n_visit > n_blocks);
     if (!too_many) {
         blocks_raw([&](const u32x4(&raw)[U], const int(&e0)[U]) TRLK_INLINE {
             uint32_t in[U], count = 0;
@@ -1059,33 +1122,50 @@ __global__ __launch_bounds__(kSelThreads, LONG ? 4 : 6) void filter_select_kerne
         border_index = ~0u;
         before = 0;
     }
-    // ---- very many candidates, without top-k: two passes over the row.  The first adds the weights up, in fp32, in bins linear in the
-    // logit: that tells the border's bin give or take one.  The second sums in 64 bits, chunk by chunk,
-    // what lies before those three bins, and lists what lies in them, where the border is then found.
+    // ---- very many candidates, without top-k: two passes over the row.  The first counts the logits in bins linear in them, with their
+    // mean in each: that tells the border's bin, or the few where it may be.  The second sums in 64 bits, chunk by chunk,
+    // what lies before those bins, and lists what lies in them, where the border is then found.
     if (LONG && n_cand > kCandidates && !f.top_k && x_low > -INFINITY) {
-        const float scale = float(kBins - 1) / fmaxf(m - x_low, 1e-30f);
+        if (!SECOND && a.longs.count) {  // left to launches of all CUs, if there is a slot
+            if (tid == 0) s.bin = atomicAdd(a.longs.count, 1u);
+            __syncthreads();
+            const uint32_t slot = s.bin;
+            if (slot < a.longs.n_slots) {
+                LongRow* to = a.longs.at(slot);
+                for (int i = tid; i < kBins; i += kSelThreads) to->bins()[i] = 0;
+                if (tid == 0) {
+                    to->sum = S, to->mass = 0, to->m = m, to->x_low = x_low;
+                    to->row = uint32_t(row), to->n_zone = to->done = 0, to->min_key = ~0u;
+                }
+                return;
+            }
+        }
+        const float scale = bins_per_logit(m, x_low);
+        // this workgroup's halves of chunks
+        const int half0 = SECOND ? int(blockIdx.x) * kSelWaves : 0, half1 = SECOND && half0 + kSelWaves < 2 * a.chunks ? half0 + kSelWaves : 2 * a.chunks;
+        const int64_t v_end = int64_t(half1) * kHalf < V ? int64_t(half1) * kHalf : V;
         // g(values, index of the first) for every vector, end(chunk) after a wave's half of a chunk (waves get as many halves each): 16 logits
         // of a lane at a time, the next in flight
-        constexpr int G = 16 / EPV, kHalf = 16 * kWave;
-        static_assert(2 * kHalf == kChunk && NV == 2 * G, "a half is one set of vectors");
+        constexpr int G = 16 / EPV;
+        static_assert(kHalf == 16 * kWave && NV == 2 * G, "a half is one set of vectors");
         const auto row_pass = [&](auto g, auto end) TRLK_INLINE {
             const auto load = [&](int64_t e0, u32x4(&q)[G]) TRLK_INLINE {
 #pragma unroll
                 for (int i = 0; i < G; ++i) {
                     const int64_t at = e0 + (i * kWave + lane) * EPV;
-                    if (at + EPV <= V) {
+                    if (at + EPV <= v_end) {
                         q[i] = *reinterpret_cast<const u32x4_u*>(x + at);
                     } else {
                         float v[EPV];
 #pragma unroll
-                        for (int e = 0; e < EPV; ++e) v[e] = at + e < V ? Elem<DT>::load1(x + at + e) : -INFINITY;
+                        for (int e = 0; e < EPV; ++e) v[e] = at + e < v_end ? Elem<DT>::load1(x + at + e) : -INFINITY;
                         q[i] = Elem<DT>::pack(v);
                     }
                 }
             };
             u32x4 next[G];
-            load(int64_t(wave) * kHalf, next);
-            for (int half = wave; half < 2 * a.chunks; half += kSelWaves) {
+            load(int64_t(half0 + wave) * kHalf, next);
+            for (int half = half0 + wave; half < half1; half += kSelWaves) {
                 const uint32_t e0 = uint32_t(half) * kHalf;
                 u32x4 now[G];
 #pragma unroll
@@ -1104,29 +1184,31 @@ __global__ __launch_bounds__(kSelThreads, LONG ? 4 : 6) void filter_select_kerne
         int zone = kBins, zone_end = kBins;  // [zone, zone_end) has the border
         bool found = true;
         if (f.top_p > 0.0) {
-            clear_bins(s, kBins);
-            row_pass(
-                [&](const float(&v)[EPV], uint32_t) TRLK_INLINE {
-#pragma unroll
-                    for (int e = 0; e < EPV; ++e) {
-                        const uint32_t t = uint32_t((m - v[e]) * (256.f * scale));  // (infinity is the largest number)
-                        if (t < 256u * kBins) atomicAdd(&s.bins[t / 256u], u64(1) << 32 | t % 256u);
-                    }
-                },
-                [](int) TRLK_INLINE {});
+            if constexpr (SECOND) {  // (the launch before this one has counted)
+                for (int i = tid; i < kBins; i += kSelThreads) s.bins[i] = left->bins()[i];
+            } else {
+                clear_bins(s, kBins);
+                row_pass([&](const float(&v)[EPV], uint32_t) TRLK_INLINE { count_in_bins(v, m, scale, s.bins); }, [](int) TRLK_INLINE {});
+            }
             __syncthreads();
-            // how many tokens a bin has, times the weight at their mean (a bin is a hundredth of a power of two wide)
+            // how many logits a bin has, times the weight at their mean
             for (int i = tid; i < kBins; i += kSelThreads) {
                 const u64 all = s.bins[i];
                 const float n = float(uint32_t(all >> 32)), mean = (float(uint32_t(all)) / fmaxf(n, 1.f) + 0.5f) * (1.f / 256.f);
                 s.bins[i] = u64(n * fast_exp2(fmaf(-(float(i) + mean) / scale, cf, l2)) + 0.5f);
             }
             __syncthreads();
+            // A bin is a hundredth of a power of two wide: a mean stands for its logits to 1e-5 at most, the sums are that good too, and
+            // the border lies where they are within 1e-4 of top_p.
             uint32_t bin;
-            before = 0;
-            found = crossing(s, kBins, u64(f.top_p * 0x1p31) + 1, bin, before);
-            zone = int(bin) - 1;
-            zone_end = int(bin) + 2;
+            u64 unused = 0;
+            const double p = f.top_p * 0x1p31;
+            found = crossing(s, kBins, p > 0x1p31 * 1e-4 ? u64(p - 0x1p31 * 1e-4) + 1 : 1, bin, unused);
+            zone = int(bin);
+            __syncthreads();
+            if (tid == 0) s.bin = ~0u;
+            unused = 0;
+            zone_end = crossing(s, kBins, u64(p + 0x1p31 * 1e-4) + 1, bin, unused) ? int(bin) + 1 : kBins;
         }
         __syncthreads();
         if (tid == 0) {
@@ -1187,11 +1269,37 @@ __global__ __launch_bounds__(kSelThreads, LONG ? 4 : 6) void filter_select_kerne
             if (f.min_p > 0.0) second_pass(std::true_type{});
             else second_pass(std::false_type{});
             __syncthreads();
-            for (int i = first; i < last; ++i) cmass[i] = s.bins[i];
+            if (SECOND) {
+                for (int i = half0 / 2 + tid; i < (half1 + 1) / 2; i += kSelThreads) cmass[i] = s.bins[i];
+            } else {
+                for (int i = first; i < last; ++i) cmass[i] = s.bins[i];
+            }
         }
         min_key = smallest(s.min_key, min_key);
         all_mass = block_total(all_mass, s.slots[1]);
-        const int n_bin = int(s.n_cand);
+        int n_bin = int(s.n_cand);
+        if constexpr (SECOND) {
+            if (tid == 0) {
+                s.bin = n_bin ? atomicAdd(&left->n_zone, uint32_t(n_bin)) : 0;
+                atomicAdd(&left->mass, all_mass);
+                atomicMin(&left->min_key, min_key);
+            }
+            __syncthreads();
+            const uint32_t to = s.bin;  // (with more than kCandidates in all, or in one part, nothing of the list is used)
+            for (int i = tid; i < n_bin && i < kCandidates; i += kSelThreads)
+                if (to + i < kCandidates) left->zone()[to + i] = s.order[i];
+            __threadfence();
+            __syncthreads();
+            if (tid == 0) s.bin = atomicAdd(&left->done, 1u);
+            __syncthreads();
+            if (s.bin + 1 != uint32_t(a.longs.parts)) return;
+            __threadfence();
+            all_mass = __hip_atomic_load(&left->mass, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            min_key = __hip_atomic_load(&left->min_key, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            n_bin = int(__hip_atomic_load(&left->n_zone, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT));
+            for (int i = tid; i < n_bin && i < kCandidates; i += kSelThreads) s.order[i] = left->zone()[i];
+            __syncthreads();
+        }
         const auto each = [&](auto g) TRLK_INLINE {
             for (int i = tid; i < n_bin; i += kSelThreads) g(key_of(s.order[i]), index_of(s.order[i]));
         };
@@ -1380,6 +1488,37 @@ __global__ __launch_bounds__(kSelThreads, LONG ? 4 : 6) void filter_select_kerne
     }
 }
 
+// The first pass over the rows that the selection has left, in parts.
+template <int DT>
+__global__ __launch_bounds__(kSelThreads) void filter_count_kernel(SelectArgs a) {
+    typedef typename Elem<DT>::type T;
+    constexpr int EPV = Elem<DT>::EPV, G = 16 / EPV;
+    __shared__ u64 bins[kBins];
+    if (!a.longs.has(blockIdx.y)) return;
+    LongRow* const left = a.longs.at(blockIdx.y);
+    const RowFilter f = row_filter(a.f, left->row, a.x.vocab);
+    if (!(f.top_p > 0.0)) return;
+    const float m = left->m, scale = bins_per_logit(m, left->x_low);
+    const int lane = threadIdx.x & (kWave - 1);
+    const int64_t e0 = (int64_t(blockIdx.x) * kSelWaves + threadIdx.x / kWave) * kHalf, V = a.x.vocab;
+    const T* x = a.x.row<DT>(left->row);
+    u32x4 q[G];
+    if (e0 < V) load_raw<DT, G>(x + e0, V - e0, lane, q);
+    for (int i = threadIdx.x; i < kBins; i += kSelThreads) bins[i] = 0;
+    __syncthreads();
+    if (e0 < V) {
+#pragma unroll
+        for (int i = 0; i < G; ++i) {
+            float v[EPV];
+            Elem<DT>::unpack(q[i], v);
+            count_in_bins(v, m, scale, bins);
+        }
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < kBins; i += kSelThreads)
+        if (bins[i]) atomicAdd(&left->bins()[i], bins[i]);
+}
+
 // ---- backward --------------------------------------------------------------------------------------------------------
 struct FilterBwdArgs {
     RowView x;
@@ -1506,6 +1645,14 @@ bool needs_blocks(const Filters& f) {
 bool every_top_k(const Filters& f, int64_t vocab) {
     return vocab > 1 && ((!f.d_top_k && f.top_k > 0 && f.top_k < vocab) || (!f.d_temperature && f.temperature == 0.0));
 }
+// How many rows with more candidates than are held (without top-k, where top-p or min-p bounds them) may be left to the launches of all CUs.
+// None where there are more rows than workgroups at a time: so many rows have such ones in every round, and what a round waits for they do
+// beside each other.  Mean of 20 draws of logits, with these launches and without: 256 rows of 128257 in bf16 59 and 63 us, 384 of 151936
+// in fp32 82 and 95, 1000 of 50257 104 and 71.
+int64_t long_rows(int64_t rows, int64_t vocab) { return vocab <= kMaxCandidates || rows > 512 ? 0 : rows < kLongRows ? rows : kLongRows; }
+bool may_be_long(const Filters& f, int64_t rows, int64_t vocab) {
+    return long_rows(rows, vocab) > 0 && !every_top_k(f, vocab) && (f.d_top_p || f.top_p < 1.0 || f.d_min_p || f.min_p > 0.0);
+}
 bool needs_sums(const Filters& f, int64_t vocab) {
     const bool min_p_alone = !f.d_min_p && f.min_p > 0.0 && !f.d_top_p && f.top_p >= 1.0;
     return !every_top_k(f, vocab) && !min_p_alone;
@@ -1534,6 +1681,13 @@ void launch_select(const SelectArgs& a, bool score, bool any_length, hipStream_t
         filter_select_kernel<DT, false, true><<<grid, kSelThreads, 0, stream>>>(a);
     else
         filter_select_kernel<DT, false, false><<<grid, kSelThreads, 0, stream>>>(a);
+    if (!a.longs.count) return;
+    const dim3 parts(unsigned(a.longs.parts), a.longs.n_slots);
+    filter_count_kernel<DT><<<parts, kSelThreads, 0, stream>>>(a);
+    if (score)
+        filter_select_kernel<DT, true, true, true><<<parts, kSelThreads, 0, stream>>>(a);
+    else
+        filter_select_kernel<DT, false, true, true><<<parts, kSelThreads, 0, stream>>>(a);
 }
 constexpr size_t kCacheBytes = size_t(256) << 20;  // the last level
 template <int DT>
@@ -1554,6 +1708,11 @@ int run(SelectArgs& a, int dtype, void* workspace, size_t workspace_bytes, void*
     char* ws = static_cast<char*>(workspace);
     a.chunk_sum = reinterpret_cast<double*>(ws);
     a.chunk_max = reinterpret_cast<float*>(ws + sum_bytes);
+    if (may_be_long(a.f, a.rows, a.x.vocab)) {
+        char* at = ws + sum_bytes + max_bytes + up16(size_t(units) * kBlocksPerChunk * elem_size(dtype));
+        at += (64 - reinterpret_cast<uintptr_t>(at) % 64) % 64;
+        a.longs = LongRows{reinterpret_cast<uint32_t*>(at), at + 64, uint32_t(long_rows(a.rows, a.x.vocab)), (2 * a.chunks + kSelWaves - 1) / kSelWaves};
+    }
     if (!block_max) block_max = ws + sum_bytes + max_bytes;
     a.block_max = block_max;
     a.has_blocks = blocks;
@@ -1561,7 +1720,7 @@ int run(SelectArgs& a, int dtype, void* workspace, size_t workspace_bytes, void*
     int bits = 0;
     while ((a.x.vocab >> bits) != 0) ++bits;
     a.fix = 62 - bits < 50 ? 62 - bits : 50;  // a sum of `vocab` weights of at most 1 stays under 2^62
-    const ScanArgs sc{a.x, a.rows, a.chunks, a.f, a.row_mask, reinterpret_cast<double*>(ws), reinterpret_cast<float*>(ws + sum_bytes), block_max};
+    const ScanArgs sc{a.x, a.rows, a.chunks, a.f, a.row_mask, reinterpret_cast<double*>(ws), reinterpret_cast<float*>(ws + sum_bytes), block_max, a.longs.count};
     switch (dtype) {
         case TRLK_F32:
             launch_scan<TRLK_F32>(sc, sums, blocks, stream);
@@ -1592,7 +1751,8 @@ extern "C" int64_t trlk_token_filter_max_vocab(void) { return kMaxVocab; }
 extern "C" size_t trlk_token_filter_workspace_bytes(int64_t rows, int64_t vocab, int dtype) {
     if (rows <= 0 || vocab <= 0 || vocab > kMaxVocab) return 0;
     const size_t units = size_t(rows) * size_t(chunks_of(vocab));
-    return up16(units * 8) + up16(units * 4) + up16(units * kBlocksPerChunk * elem_size(dtype));
+    const size_t n_long = size_t(long_rows(rows, vocab));
+    return up16(units * 8) + up16(units * 4) + up16(units * kBlocksPerChunk * elem_size(dtype)) + (n_long ? 128 + n_long * kLongRowBytes : 0);
 }
 
 extern "C" int trlk_sample_tokens(const void* d_logits, int dtype, int64_t n_seq, int64_t rows_per_seq, int64_t vocab,
