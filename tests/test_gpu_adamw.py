@@ -507,3 +507,42 @@ def test_one_on_policy_step_end_to_end():
         zero = torch.zeros(p.shape)
         want_p, _, _, update = definition(x, p.grad, zero, zero, 1, min(1.0, 0.1 / (norm + 1e-6)), lr=1e-2, wd=0.1)
         check_param(p.detach(), x, want_p, update, torch.float32, lr=1e-2)
+
+
+def test_traced_calls_have_the_shapes():
+    from torch._subclasses.fake_tensor import FakeTensorMode
+
+    import trl_amd
+
+    with FakeTensorMode():
+        x = [torch.empty(300, device=DEV, dtype=torch.bfloat16), torch.empty(7, 5, device=DEV, dtype=torch.bfloat16)]
+        m = [torch.empty(t.shape, device=DEV) for t in x]
+        steps = [torch.empty((), device=DEV) for _ in x]
+        norm = trl_amd.adamw_step_(x, [t.clone() for t in x], m, [t.clone() for t in m], steps, max_grad_norm=1.0)
+        assert norm.shape == () and norm.dtype == torch.float32 and norm.device.type == "cuda"
+        assert trl_amd.adamw_step_(x, [t.clone() for t in x], m, [t.clone() for t in m], steps) is None
+        values = trl_amd.adamw_state_values(torch.empty(600, device=DEV, dtype=torch.uint8), torch.empty(3, device=DEV))
+        assert values.shape == (600,) and values.dtype == torch.bfloat16
+
+
+def test_one_learning_rate_for_each_group_and_empty_tensors():
+    """Groups with rates on the host and on the GPU, tensors of no and of one entry, and one without a gradient, against torch's AdamW."""
+    import trl_amd
+
+    g = torch.Generator().manual_seed(71)
+    shapes = ((0,), (1,), (4097,), (3, 0, 2), (70, 71), (5,))
+    mine, theirs = ([torch.nn.Parameter(torch.randn(s, generator=torch.Generator().manual_seed(i)).to(DEV)) for i, s in enumerate(shapes)]
+                    for _ in range(2))
+    groups = lambda w, lr: [dict(params=w[:2], lr=1e-2), dict(params=w[2:5], lr=lr, weight_decay=0.1), dict(params=w[5:], eps=1e-3)]  # noqa: E731
+    a = trl_amd.AdamW(groups(mine, torch.tensor(3e-3, device=DEV)), lr=1e-3)
+    b = torch.optim.AdamW(groups(theirs, 3e-3), lr=1e-3, foreach=False)
+    for _ in range(4):
+        for p, q in zip(mine[:5], theirs[:5]):
+            p.grad = torch.randn(p.shape, generator=g).to(DEV)
+            q.grad = p.grad.clone()
+        a.step()
+        b.step()
+    for p, q in zip(mine, theirs):
+        # four steps, each a few roundings of a step of 1e-2 at most and one of the value
+        assert torch.allclose(p, q, rtol=4 * 2.0**-23, atol=4 * 1e-2 * 8 * 2.0**-24)
+    assert mine[5].grad is None and not a.state.get(mine[5])

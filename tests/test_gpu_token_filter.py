@@ -641,3 +641,36 @@ def test_a_border_between_two_distant_tokens():
         check_draw(x, u, settings(1.0, 0, p))
         ids, lp = trl_amd.sample_tokens(x.to(DEV), u.to(DEV), top_p=p.to(DEV))
         assert torch.equal(trl_amd.filtered_logps(x.to(DEV), ids, top_p=p.to(DEV)), lp)
+
+
+@pytest.mark.parametrize("rows", [3, 515])
+def test_nuclei_of_almost_everything(rows):
+    """top_p so near 1 that the border lies among the last tokens, in rows of very many, with and without min-p and masked rows; ids outside
+    the vocabulary are reported by such rows as well."""
+    import trl_amd
+
+    V = 6007
+    logits, u = make_logits(rows, V, "fp32", 280, slope=0.4)
+    for s in (settings(1.0, 0, 0.99995), settings(0.8, 0, 1.0 - 2.0**-24), settings(1.0, 0, 0.99999, 1e-3), settings(5.0, 0, 0.5), settings(40.0, 0, 0.999)):
+        check_draw(logits, u, s)
+    x, ids = logits.to(DEV), torch.randint(0, V, (rows,), generator=torch.Generator().manual_seed(281)).to(DEV)
+    mask = torch.ones(rows, dtype=torch.bool, device=DEV)
+    mask[1] = False
+    s = settings(1.0, 0, 0.99)
+    whole = trl_amd.filtered_logps(x, ids, **s)
+    part = trl_amd.filtered_logps(x, ids, row_mask=mask, **s)
+    assert part[1] == 0 and torch.equal(part[mask], whole[mask])
+    trl_amd.check_device_errors()
+    ids[2] = V
+    assert torch.isnan(trl_amd.filtered_logps(x, ids, **s)[2])
+    with pytest.raises(IndexError):
+        trl_amd.check_device_errors()
+
+
+def test_very_many_candidates_of_a_large_vocabulary():
+    import trl_amd
+
+    V = trl_amd._lib.lib.trlk_token_filter_max_vocab()
+    logits, u = make_logits(2, V, "bf16", 291, slope=0.3)
+    check_draw(logits, u, settings(1.0, 0, 0.9))
+    check_draw(logits, u, settings(1.0, 0, 1.0, 0.05))
