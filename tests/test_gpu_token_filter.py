@@ -674,3 +674,12 @@ def test_very_many_candidates_of_a_large_vocabulary():
     logits, u = make_logits(2, V, "bf16", 291, slope=0.3)
     check_draw(logits, u, settings(1.0, 0, 0.9))
     check_draw(logits, u, settings(1.0, 0, 1.0, 0.05))
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
+def test_a_top_k_of_a_thousand_and_more(dtype):
+    logits, u = make_logits(5, 20011, dtype, 301)
+    logits[4] = logits[4].sign()  # three values
+    for k in (900, 1024, 1025, 1500, 2500, 4095, 4097, 19999):
+        for s in (settings(1.0, k), settings(0.7, k, 0.9), settings(3.0, k, 0.999, 1e-3)):
+            check_draw(logits, u, s)

@@ -40,7 +40,7 @@ constexpr int kBins = 4 * kSelThreads;       // of a step of the descent
 constexpr int kBinBits = 11;
 constexpr int kMaxCandidates = 4096;         // that are kept in LDS; rows with more read their blocks again in every step
 constexpr int kList = 4096;                  // blocks over the bound that are listed; with more every block is looked at
-constexpr int kPairs = 128;                  // candidates of which every pair is compared
+constexpr int kPairs = 128;                  // candidates of which every pair is compared (256 rows with 100 of them 10.8 us, 13.1 by bins)
 constexpr int kLine = 128;                   // bytes of a cache line
 constexpr int kLongRows = 32;                // rows with very many candidates whose passes all CUs share
 constexpr int kHalf = kChunk / 2;            // logits of a wave's step in these passes
@@ -1653,6 +1653,9 @@ int64_t long_rows(int64_t rows, int64_t vocab) { return vocab <= kMaxCandidates 
 bool may_be_long(const Filters& f, int64_t rows, int64_t vocab) {
     return long_rows(rows, vocab) > 0 && !every_top_k(f, vocab) && (f.d_top_p || f.top_p < 1.0 || f.d_min_p || f.min_p > 0.0);
 }
+// a top-k whose candidates fit into the variant without LONG only at times (256 rows of 128257 in bf16 with k = 1500: 256 us there, 39 with LONG;
+// k = 1000: 26 both)
+bool many_top_k(const Filters& f) { return f.top_k > kMaxCandidates / 4 && f.temperature != 0.0; }
 bool needs_sums(const Filters& f, int64_t vocab) {
     const bool min_p_alone = !f.d_min_p && f.min_p > 0.0 && !f.d_top_p && f.top_p >= 1.0;
     return !every_top_k(f, vocab) && !min_p_alone;
@@ -1700,7 +1703,7 @@ void launch_bwd(const FilterBwdArgs& a, bool past_caches, dim3 grid, hipStream_t
 
 int run(SelectArgs& a, int dtype, void* workspace, size_t workspace_bytes, void* block_max, bool score, hipStream_t stream, const char* what) {
     const int64_t units = a.rows * a.chunks;
-    const bool blocks = needs_blocks(a.f), sums = needs_sums(a.f, a.x.vocab), any_length = !every_top_k(a.f, a.x.vocab);
+    const bool blocks = needs_blocks(a.f), sums = needs_sums(a.f, a.x.vocab), any_length = !every_top_k(a.f, a.x.vocab) || many_top_k(a.f);
     const size_t sum_bytes = up16(size_t(units) * 8), max_bytes = up16(size_t(units) * 4);
     const size_t need = trlk_token_filter_workspace_bytes(a.rows, a.x.vocab, dtype);
     TRLK_REQUIRE(workspace && workspace_bytes >= need, TRLK_ERR_WORKSPACE, "%s: workspace of %zu bytes, %zu needed", what, workspace_bytes, need);
