@@ -10,6 +10,7 @@
 #include <ATen/ops/empty.h>
 #include <ATen/ops/empty_strided.h>
 #include <ATen/ops/zeros.h>
+#include <c10/core/AutogradState.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/core/InferenceMode.h>
 #include <torch/csrc/autograd/autograd_not_implemented_fallback.h>
@@ -189,10 +190,12 @@ template <typename Signature>
 c10::TypedOperatorHandle<Signature> handle(const char* name) {
     return c10::Dispatcher::singleton().findSchemaOrThrow(name, "").typed<Signature>();
 }
+// Whether a derivative of the call is wanted.  A tangent (forward mode, which needs neither grad mode nor a tensor that requires a gradient)
+// counts: the autograd functions have no formula for it and raise, where the plain call would return outputs without one.
 bool needs_grad(std::initializer_list<const Tensor*> tensors) {
-    if (!c10::GradMode::is_enabled()) return false;
+    const bool forward_mode = c10::AutogradState::get_tls_state().get_fw_grad_mode();
     for (const Tensor* t : tensors)
-        if (t->defined() && t->requires_grad()) return true;
+        if (t->defined() && ((c10::GradMode::is_enabled() && t->requires_grad()) || (forward_mode && t->_fw_grad(0).defined()))) return true;
     return false;
 }
 bool needs_grad(const optional<Tensor>& t) { return t && needs_grad({&*t}); }

@@ -19,6 +19,7 @@ from typing import Optional
 
 import torch
 from torch import Tensor
+from torch.autograd import forward_ad
 
 from . import _lib
 from ._lib import check, current_stream, dtype_code, lib, on_device, ptr
@@ -77,6 +78,13 @@ def _observed() -> bool:
     modes = getattr(torch._C, "_len_torch_dispatch_stack", None)
     transforms = getattr(torch._C, "_are_functorch_transforms_active", None)
     return modes is None or transforms is None or modes() > 0 or transforms()
+
+
+def refuse_tangents(name: str, *tensors: Tensor) -> None:
+    """Raises if one of the tensors has a tangent (forward mode).  For operators whose autograd layer is `custom_op`'s: it looks at
+    `requires_grad` alone, and what such a tensor goes through would come out without its tangent."""
+    if getattr(forward_ad, "_current_level", 0) >= 0 and any(forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise NotImplementedError(f"{name} has no derivative in forward mode")
 
 
 _library = torch.library.Library("trl_amd", "FRAGMENT")
@@ -237,7 +245,10 @@ logp_entropy_fwd_f64.register_autograd(_lpe64_backward, setup_context=_lpe64_set
 def logp_entropy_forward(logits: Tensor, index: Tensor, temperature: float, keep_start: int, keep_len: int,
                          row_mask: Optional[Tensor]) -> tuple[Tensor, Tensor, Tensor]:
     """The forward op for these logits: the double-precision pair for float64, the streaming kernels otherwise."""
-    op = logp_entropy_fwd_f64 if logits.dtype == torch.float64 else logp_entropy_fwd
+    op = logp_entropy_fwd
+    if logits.dtype == torch.float64:
+        op = logp_entropy_fwd_f64
+        refuse_tangents("the log-prob of float64 logits", logits)
     return op(logits, index, temperature, keep_start, keep_len, row_mask)
 
 

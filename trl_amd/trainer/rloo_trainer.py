@@ -17,6 +17,7 @@ RLOO_METRIC_NAMES = ("clip_ratio/low_mean", "clip_ratio/low_min", "clip_ratio/hi
 def rloo_loss(per_token_logps: Tensor, completion_mask: Tensor, old_logps: Tensor, advantages: Tensor,
               epsilon_low: float, epsilon_high: float):
     """Returns `(loss, sequence_logps [B], metrics [8])`; metric order = `RLOO_METRIC_NAMES`."""
+    ops.refuse_tangents("rloo_loss", per_token_logps, completion_mask, old_logps, advantages)
     loss, seq, metrics, _ = ops.rloo_loss_op(per_token_logps, completion_mask, old_logps, advantages,
                                              float(epsilon_low), float(epsilon_high))
     return loss, seq, metrics
