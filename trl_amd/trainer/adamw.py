@@ -117,12 +117,31 @@ class AdamW(torch.optim.Optimizer):
         return loss
 
     def load_state_dict(self, state_dict: dict) -> None:
-        """As the base class, except that the moments keep their own types (it would cast them to the parameters').  The state of a
-        `torch.optim.AdamW` is taken too: its moments become fp32 and its step counters move to the parameters' device."""
+        """As the base class, hooks included, except that the moments keep their own types (it would cast them to the parameters').  The
+        state of a `torch.optim.AdamW` is taken too: its moments become fp32 and its step counters move to the parameters' device."""
+        taken = {}
+
+        def take(_, given):
+            self._check_state_dict(given)
+            taken.update(given)
+
+        # (behind the caller's hooks of the one kind and before those of the other: what a pre-hook returns is what is loaded, and a post-hook
+        # finds the state as it will be)
+        hooks = [self.register_load_state_dict_pre_hook(take),
+                 self.register_load_state_dict_post_hook(lambda _: self._take_state(taken), prepend=True)]
+        try:
+            super().load_state_dict(state_dict)
+        finally:
+            for hook in hooks:
+                hook.remove()
+
+    def _check_state_dict(self, state_dict: dict) -> None:
         for k in ("amsgrad", "maximize"):
             if any(g.get(k) for g in state_dict["param_groups"]):
                 raise ValueError(f"AdamW has no {k}")
-        super().load_state_dict(state_dict)
+
+    def _take_state(self, state_dict: dict) -> None:
+        """The moments and step counters of `state_dict`, which the base class has loaded, in their own types."""
         for group in self.param_groups:
             for k, v in self.defaults.items():
                 group.setdefault(k, v)
