@@ -52,3 +52,72 @@ def test_what_a_post_hook_writes_stays():
         assert not opt.state[p]["exp_avg_sq"].any() and opt.state[p]["mine"] == 1 and opt.state[p]["exp_avg"].any()
     opt.load_state_dict(torch_state())  # (again: no hook of the first call is left)
     assert seen == [torch.float32] * 4 and len(opt._optimizer_load_state_dict_pre_hooks) == 0 and len(opt._optimizer_load_state_dict_post_hooks) == 1
+
+
+def bad_states():
+    good = torch_state()
+    one = lambda entry: {**good, "state": {**good["state"], 1: entry}}  # noqa: E731
+    moments = good["state"][1]
+    codes = {"step": torch.tensor(1.0), "exp_avg": torch.zeros(5000, dtype=torch.uint8).view(torch.float8_e4m3fn),
+             "exp_avg_sq": torch.zeros(5000, dtype=torch.uint8)}
+    return {
+        "another optimiser's moments": one({"step": 7, "state1": torch.zeros(5000), "state2": torch.zeros(5000)}),
+        "momentum": one({"momentum_buffer": torch.zeros(5000)}),
+        "no step": one({k: v for k, v in moments.items() if k != "step"}),
+        "no second moment": one({k: v for k, v in moments.items() if k != "exp_avg_sq"}),
+        "one scale": one({**codes, "exp_avg_scale": torch.ones(20)}),
+        "codes without scales": one(codes),
+        "scales of fp32 moments": one({**moments, "exp_avg_scale": torch.ones(20), "exp_avg_sq_scale": torch.ones(20)}),
+        "another shape": one({**moments, "exp_avg": torch.zeros(4999)}),
+        "scales of another size": one({**codes, "exp_avg_scale": torch.ones(19), "exp_avg_sq_scale": torch.ones(20)}),
+    }
+
+
+@pytest.mark.parametrize("what", list(bad_states()))
+def test_states_that_are_none_of_its_own_are_refused(what):
+    w, opt = optimiser()
+    opt.load_state_dict(torch_state())
+    before = {p: {k: v.clone() for k, v in opt.state[p].items()} for p in w}
+    with pytest.raises(ValueError, match="parameter 1"):
+        opt.load_state_dict(bad_states()[what])
+    for p in w:  # (and what was there stays)
+        assert set(opt.state[p]) == set(before[p]) and all(torch.equal(opt.state[p][k], v) for k, v in before[p].items())
+
+
+def test_coupled_decay_is_refused():
+    w, opt = optimiser()
+    saved = torch_state()
+    saved["param_groups"][0]["decoupled_weight_decay"] = False
+    with pytest.raises(ValueError, match="decoupled"):
+        opt.load_state_dict(saved)
+    saved["param_groups"][0]["weight_decay"] = 0.0  # (no decay: the two are the same)
+    opt.load_state_dict(saved)
+    assert opt.state[w[1]]["step"].item() == 2.0
+
+
+def test_a_hook_may_convert_a_state():
+    """What is refused is what the hooks leave."""
+    w, opt = optimiser()
+    saved = bad_states()["another optimiser's moments"]
+
+    def convert(_, given):
+        names = {"state1": "exp_avg", "state2": "exp_avg_sq"}
+        return {**given, "state": {i: {names.get(k, k): v for k, v in s.items()} for i, s in given["state"].items()}}
+
+    opt.register_load_state_dict_pre_hook(convert)
+    opt.load_state_dict(saved)
+    assert opt.state[w[1]]["step"].item() == 7.0 and opt.state[w[1]]["exp_avg"].shape == (5000,)
+
+
+def test_8bit_state_round_trip_and_empty_entries():
+    w, opt = optimiser(8)
+    for p in w:
+        opt._state_of(p, opt.param_groups[0])
+    opt.state[w[1]]["exp_avg_sq"].fill_(7)
+    other, again = optimiser(8)
+    again.load_state_dict(opt.state_dict())
+    assert again.state[other[1]]["exp_avg"].dtype == torch.float8_e4m3fn and bool((again.state[other[1]]["exp_avg_sq"] == 7).all())
+    saved = opt.state_dict()
+    saved["state"][0] = {}  # (a parameter that has made no step)
+    again.load_state_dict(saved)
+    assert not again.state[other[0]] and again.state[other[1]]["exp_avg"].dtype == torch.float8_e4m3fn

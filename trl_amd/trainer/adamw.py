@@ -136,9 +136,29 @@ class AdamW(torch.optim.Optimizer):
                 hook.remove()
 
     def _check_state_dict(self, state_dict: dict) -> None:
-        for k in ("amsgrad", "maximize"):
-            if any(g.get(k) for g in state_dict["param_groups"]):
-                raise ValueError(f"AdamW has no {k}")
+        """Refuses what would not go on as it was: another optimiser's state, or another kind of step."""
+        for group in state_dict["param_groups"]:
+            for k in ("amsgrad", "maximize"):
+                if group.get(k):
+                    raise ValueError(f"AdamW has no {k}")
+            if group.get("decoupled_weight_decay") is False and group.get("weight_decay"):
+                raise ValueError("AdamW's weight decay is decoupled, the state's is not")
+        ids = [i for g in state_dict["param_groups"] for i in g["params"]]
+        params = [p for g in self.param_groups for p in g["params"]]
+        for place, (i, p) in enumerate(zip(ids, params)):
+            saved = state_dict["state"].get(i)
+            if not saved:
+                continue
+            missing = [k for k in ("step", "exp_avg", "exp_avg_sq") if k not in saved]
+            if missing:
+                raise ValueError(f"the state of parameter {place} is not AdamW's: it has {sorted(saved)}, but no {', '.join(missing)}")
+            scales = [saved[k] for k in ("exp_avg_scale", "exp_avg_sq_scale") if k in saved]
+            kinds = saved["exp_avg"].dtype, saved["exp_avg_sq"].dtype
+            coded = kinds == (torch.float8_e4m3fn, torch.uint8)
+            if len(scales) != 2 * coded or not coded and any(k.itemsize == 1 for k in kinds):
+                raise ValueError(f"the state of parameter {place} has moments in {kinds[0]} and {kinds[1]} and {len(scales)} scales")
+            if any(saved[k].shape != p.shape for k in ("exp_avg", "exp_avg_sq")) or any(t.numel() != -(-p.numel() // STATE_BLOCK) for t in scales):
+                raise ValueError(f"the state of parameter {place} is that of another shape than {tuple(p.shape)}")
 
     def _take_state(self, state_dict: dict) -> None:
         """The moments and step counters of `state_dict`, which the base class has loaded, in their own types."""
