@@ -121,3 +121,16 @@ def test_8bit_state_round_trip_and_empty_entries():
     saved["state"][0] = {}  # (a parameter that has made no step)
     again.load_state_dict(saved)
     assert not again.state[other[0]] and again.state[other[1]]["exp_avg"].dtype == torch.float8_e4m3fn
+
+
+def test_copies_and_pickles_are_whole():
+    import copy
+    import pickle
+
+    w, opt = optimiser(max_grad_norm=0.5, seed=9)
+    opt.load_state_dict(torch_state())
+    for other in (copy.deepcopy(opt), pickle.loads(pickle.dumps(opt))):
+        assert (other.max_grad_norm, other.seed, other.grad_norm) == (0.5, 9, None)
+        (a, b) = other.param_groups[0]["params"]
+        assert torch.equal(a, w[0]) and torch.equal(other.state[b]["exp_avg"], opt.state[w[1]]["exp_avg"])
+        assert other.step() is None  # (no gradients: nothing to do)

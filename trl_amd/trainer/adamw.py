@@ -67,6 +67,9 @@ class AdamW(torch.optim.Optimizer):
         super().__init__(params, dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay, state_bits=state_bits,
                                       min_8bit_size=min_8bit_size))
 
+    def __getstate__(self) -> dict:
+        return {**super().__getstate__(), "max_grad_norm": self.max_grad_norm, "seed": self.seed, "grad_norm": self.grad_norm}
+
     def _state_of(self, p: Tensor, group: dict) -> dict:
         state = self.state[p]
         if not state:
