@@ -13,7 +13,7 @@ every trainer module, and the loss is a trainer method.  `patch_trl()` therefore
     `trl.trainer.grpo_trainer` / `trl.trainer.dpo_trainer` (trl/trainer/grpo_trainer.py:1020-1044,
     trl/trainer/dpo_trainer.py:834), so that `compute_liger_loss` / `_compute_loss_liger` call the fused head;
   * the trainers' `get_optimizer_cls_and_kwargs` (optional, `adamw=True`): `optim="adamw_torch"`, `"adamw_torch_fused"`, `"adamw_8bit"`
-    and `"adamw_bnb_8bit"` then make `trl_amd.AdamW`.
+    and `"adamw_bnb_8bit"` then make `trl_amd.AdamW`, for models that it can step (trainable parameters on one GPU, not sharded).
 `unpatch_trl()` restores the originals.
 """
 from __future__ import annotations
@@ -40,7 +40,7 @@ def _set(mod, name, value) -> None:
 def _with_adamw(original):
     """A `get_optimizer_cls_and_kwargs` that asks `trl_amd` first."""
     def get_optimizer_cls_and_kwargs(args, model=None):
-        return _adamw.optimizer_cls_and_kwargs(args) or original(args, model)
+        return _adamw.optimizer_cls_and_kwargs(args, model) or original(args, model)
 
     return staticmethod(get_optimizer_cls_and_kwargs)
 

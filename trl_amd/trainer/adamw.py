@@ -4,6 +4,7 @@ from __future__ import annotations
 
 import torch
 from torch import Tensor
+from torch.utils._python_dispatch import is_traceable_wrapper_subclass
 
 from .. import ops
 
@@ -183,10 +184,18 @@ class AdamW(torch.optim.Optimizer):
 _STATE_BITS = {"adamw_torch": 32, "adamw_torch_fused": 32, "adamw_8bit": 8, "adamw_bnb_8bit": 8}  # names of `TrainingArguments.optim`
 
 
-def optimizer_cls_and_kwargs(args) -> tuple[type, dict] | None:
-    """`AdamW` and its arguments for training arguments whose `optim` is an AdamW, plain or with 8-bit states; `None` for others.  What
+def _steps_all_of(model: torch.nn.Module) -> bool:
+    """Whether one call can step the model's trainable parameters: plain tensors of its types on one GPU (sharded ones are none)."""
+    params = [p for p in model.parameters() if p.requires_grad]
+    return (len({p.device for p in params}) == 1 and params[0].is_cuda and not any(map(is_traceable_wrapper_subclass, params))
+            and all(p.dtype in (torch.float32, torch.bfloat16, torch.float16) for p in params))
+
+
+def optimizer_cls_and_kwargs(args, model: torch.nn.Module | None = None) -> tuple[type, dict] | None:
+    """`AdamW` and its arguments for training arguments whose `optim` is an AdamW, plain or with 8-bit states; `None` for others, and for
+    a model that it cannot step (on the CPU, on several GPUs, with sharded parameters or in another type).  What
     `transformers.Trainer.get_optimizer_cls_and_kwargs` returns, and its trainers take as `optimizer_cls_and_kwargs`."""
     bits = _STATE_BITS.get(getattr(args.optim, "value", args.optim))
-    if bits is None:
+    if bits is None or model is not None and not _steps_all_of(model):
         return None
     return AdamW, dict(lr=args.learning_rate, betas=(args.adam_beta1, args.adam_beta2), eps=args.adam_epsilon, state_bits=bits)
