@@ -57,3 +57,26 @@ def test_sharded_parameters_keep_their_optimiser(patched):
         w = sharded[1].weight.detach()
         sharded[1].weight = torch.nn.Parameter(TwoTensor(w, w.clone()))
     assert cls.get_optimizer_cls_and_kwargs(args(), sharded)[0] is torch.optim.AdamW
+
+
+def test_embeddings_keep_fp32_moments(patched):
+    """The 8-bit optimisers behind these names hold embeddings' moments in 32 bits."""
+    import copy
+
+    import trl_amd
+
+    cls, args = patched
+    with FakeTensorMode():
+        m = model("cuda:0")
+        m[1].weight = torch.nn.Parameter(torch.empty(100, 64, device="cuda:0"))
+        for optim in ("adamw_8bit", "adamw_bnb_8bit"):
+            found, kwargs = cls.get_optimizer_cls_and_kwargs(args(optim), m)
+            assert found is trl_amd.AdamW and kwargs["state_bits"] == 8
+            opt = found(m.parameters(), **kwargs)
+            kinds = {n: opt._state_of(p, opt.param_groups[0])["exp_avg"].dtype for n, p in m.named_parameters()}
+            assert kinds == {"0.weight": torch.float32, "1.weight": torch.float8_e4m3fn, "1.bias": torch.float32}
+        assert "keep_32bit" not in cls.get_optimizer_cls_and_kwargs(args(), m)[1]
+    w = [torch.nn.Parameter(torch.zeros(5000)) for _ in range(2)]
+    opt = copy.deepcopy(trl_amd.AdamW(w, state_bits=8, keep_32bit=w[:1]))
+    kinds = [opt._state_of(p, opt.param_groups[0])["exp_avg"].dtype for p in opt.param_groups[0]["params"]]
+    assert kinds == [torch.float32, torch.float8_e4m3fn]

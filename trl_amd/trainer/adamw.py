@@ -2,6 +2,8 @@
 `max_grad_norm`): one call for all tensors of a model."""
 from __future__ import annotations
 
+from collections.abc import Iterable
+
 import torch
 from torch import Tensor
 from torch.utils._python_dispatch import is_traceable_wrapper_subclass
@@ -50,13 +52,13 @@ class AdamW(torch.optim.Optimizer):
     """AdamW whose step is one call for all parameter groups (`adamw_step_`), for GPU parameters in fp32, bf16 or fp16.
 
     `state_bits=8` holds both moments of every parameter of `min_8bit_size` entries or more in 8 bits, 2.03 bytes per entry instead
-    of 8.  With `max_grad_norm` the step clips the norm over all groups, without a pass that writes the gradients, and leaves it in
+    of 8, but for those in `keep_32bit`.  With `max_grad_norm` the step clips the norm over all groups, without a pass that writes the gradients, and leaves it in
     `grad_norm` (fp32, on the GPU); `transformers.Trainer` then runs with `max_grad_norm=0`.  Step counters live on the GPU and a
     group's `lr` may: a step can be captured into a graph.  Parameters without a gradient are left alone."""
 
     def __init__(self, params, lr: float | Tensor = 1e-3, betas: tuple[float, float] = (0.9, 0.999), eps: float = 1e-8,
                  weight_decay: float = 0.01, *, state_bits: int = 32, min_8bit_size: int = 4096, max_grad_norm: float | None = None,
-                 seed: int = 0):
+                 seed: int = 0, keep_32bit: Iterable[Tensor] = ()):
         if state_bits not in (8, 32):
             raise ValueError(f"state_bits must be 8 or 32, got {state_bits}")
         if not 0.0 <= float(lr) or not 0.0 <= eps or not 0.0 <= weight_decay:
@@ -64,18 +66,19 @@ class AdamW(torch.optim.Optimizer):
         if not 0.0 <= betas[0] < 1.0 or not 0.0 <= betas[1] < 1.0:
             raise ValueError(f"betas must be in [0, 1), got {betas}")
         self.max_grad_norm = None if max_grad_norm is None else _clip(max_grad_norm)
-        self.seed, self.grad_norm = int(seed), None
+        self.seed, self.grad_norm, self.keep_32bit = int(seed), None, set(keep_32bit)
         super().__init__(params, dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay, state_bits=state_bits,
                                       min_8bit_size=min_8bit_size))
 
     def __getstate__(self) -> dict:
-        return {**super().__getstate__(), "max_grad_norm": self.max_grad_norm, "seed": self.seed, "grad_norm": self.grad_norm}
+        return {**super().__getstate__(), "max_grad_norm": self.max_grad_norm, "seed": self.seed, "grad_norm": self.grad_norm,
+                "keep_32bit": self.keep_32bit}
 
     def _state_of(self, p: Tensor, group: dict) -> dict:
         state = self.state[p]
         if not state:
             state["step"] = torch.zeros((), dtype=torch.float32, device=p.device)
-            if group["state_bits"] == 8 and p.numel() >= group["min_8bit_size"]:
+            if group["state_bits"] == 8 and p.numel() >= group["min_8bit_size"] and p not in self.keep_32bit:
                 blocks = -(-p.numel() // STATE_BLOCK)
                 state["exp_avg"] = torch.zeros_like(p, dtype=torch.uint8, memory_format=torch.preserve_format).view(torch.float8_e4m3fn)
                 state["exp_avg_sq"] = torch.zeros_like(p, dtype=torch.uint8, memory_format=torch.preserve_format)
@@ -198,4 +201,7 @@ def optimizer_cls_and_kwargs(args, model: torch.nn.Module | None = None) -> tupl
     bits = _STATE_BITS.get(getattr(args.optim, "value", args.optim))
     if bits is None or model is not None and not _steps_all_of(model):
         return None
-    return AdamW, dict(lr=args.learning_rate, betas=(args.adam_beta1, args.adam_beta2), eps=args.adam_epsilon, state_bits=bits)
+    kwargs = dict(lr=args.learning_rate, betas=(args.adam_beta1, args.adam_beta2), eps=args.adam_epsilon, state_bits=bits)
+    if bits == 8 and model is not None:  # (as the trainers have it of the optimiser that they know by these names)
+        kwargs["keep_32bit"] = [m.weight for m in model.modules() if isinstance(m, torch.nn.Embedding)]
+    return AdamW, kwargs
