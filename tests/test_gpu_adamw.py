@@ -546,3 +546,49 @@ def test_one_learning_rate_for_each_group_and_empty_tensors():
         # four steps, each a few roundings of a step of 1e-2 at most and one of the value
         assert torch.allclose(p, q, rtol=4 * 2.0**-23, atol=4 * 1e-2 * 8 * 2.0**-24)
     assert mine[5].grad is None and not a.state.get(mine[5])
+
+
+# ---- tiny second moments ----------------------------------------------------------------------------------------------
+TINY = [0.0, 1e-24, 2e-23, 1.5e-22, 1e-21, 3e-20, 1e-19, 2e-18, 1e-15, 1e-8, 1.0]  # (g^2 (1 - b2) is 0, subnormal up to 3e-18, normal)
+
+
+def tiny_step(bits, eps, t, seed=0):
+    """One step from zero moments on gradients of these sizes: parameters, moments (in 64 bits, from their fp32 arithmetic), results."""
+    import trl_amd
+
+    g = torch.tensor(TINY, dtype=torch.float64).float().repeat_interleave(256) * torch.tensor([1.0, -1.0]).repeat(len(TINY) * 128)
+    p = torch.randn(g.numel(), generator=torch.Generator().manual_seed(seed))
+    w, grad = p.to(DEV, t), g.to(DEV, t)
+    g, p = grad.cpu().float(), w.cpu()
+    if bits == 32:
+        m, v = [torch.zeros(g.numel(), device=DEV)], [torch.zeros(g.numel(), device=DEV)]
+        kw = {}
+    else:
+        m, v, ms, vs = eight_bit_state([(g.numel(),)])
+        kw = dict(exp_avg_scales=ms, exp_avg_sq_scales=vs)
+    trl_amd.adamw_step_([w], [grad], m, v, step_counters(1), lr=LR, betas=(B1, B2), eps=eps, weight_decay=WD, **kw)
+    one_minus_b1, one_minus_b2 = torch.tensor(1 - B1).float(), torch.tensor(1 - B2).float()
+    return w, p, (g * one_minus_b1).double(), (g * g * one_minus_b2).double(), m, v
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("eps", [0.0, 2.0**-130, 1e-30, 1e-21, 1e-12, 1e-8])
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+def test_tiny_second_moments(bits, eps, dtype):
+    """Second moments that are subnormal, and an eps that does not hide them: the update is the formula's.  Its root and reciprocal are off by
+    a unit of 2^-23 each, scaling by powers of two is exact, so the bounds are those of `check_param`; eps and a sum with it are normal
+    numbers, or exact."""
+    t = DTYPES[dtype]
+    w, p, m, v, got_m, got_v = tiny_step(bits, eps, t)
+    if bits == 32:
+        assert torch.equal(got_m[0].cpu().double(), m) and torch.equal(got_v[0].cpu().double(), v)
+        assert int(((v > 0) & (v < 2.0**-126)).sum()) >= 4 * 256 and int((v == 0).sum()) >= 2 * 256
+    eps32 = float(torch.tensor(eps).float())
+    update = (m / (1 - B1)) / ((v / (1 - B2)).sqrt() + eps32)
+    want = p.double() * (1 - LR * WD) - LR * update
+    finite = want.abs() < torch.finfo(t).max / 2
+    check_param(w.cpu()[finite], p[finite], want[finite], update[finite], t)
+    rest = w.cpu()[~finite].double()
+    # (0 / 0 is a NaN, anything else over 0 infinite, as in `torch.optim.AdamW`; what is too large for the type is infinite, too)
+    assert torch.equal(rest.isnan(), want[~finite].isnan()) and bool((rest.isnan() | (rest.abs() >= torch.finfo(t).max / 4)).all())
+    assert bool(finite.all()) == (eps > 0)

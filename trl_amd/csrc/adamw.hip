@@ -231,9 +231,29 @@ __device__ __forceinline__ void moments(const Scalars& s, float clip, float g, f
     const float c = v * s.beta2, d = g * g, e = d * s.one_minus_beta2;
     v = c + e;
 }
+// The hardware's root and reciprocal, each good to a unit of the last place, save that the root of a subnormal number is 0 and the reciprocal of
+// one infinite.  TINY scales both away from there, by powers of two; it is for an eps that does not hide the root of a subnormal number:
+// that is under 2^-63, and with eps >= 2^-38 / sqrt(1 - b2^t) it changes the divisor by less than 2^-25 of itself.
+template <bool TINY>
 __device__ __forceinline__ float updated(const Scalars& s, float p, float m, float v) {
+    if constexpr (TINY) {
+        const bool low = v < 0x1p-96f;
+        const float root = __builtin_amdgcn_sqrtf(low ? v * 0x1p64f : v) * (low ? 0x1p-32f : 1.f);
+        const float d = fmaf(root, s.inv_sqrt_bc2, s.eps), up = d < 0x1p-64f ? 0x1p64f : 1.f;
+        return fmaf(-s.size, (m * up) * __builtin_amdgcn_rcpf(d * up), p * s.decay);
+    }
     const float d = fmaf(__builtin_amdgcn_sqrtf(v), s.inv_sqrt_bc2, s.eps);
     return fmaf(-s.size, m * __builtin_amdgcn_rcpf(d), p * s.decay);
+}
+template <int N>
+__device__ __forceinline__ void update_n(const Scalars& s, const float (&m)[N], const float (&v)[N], float (&x)[N]) {
+    if (s.eps < s.inv_sqrt_bc2 * 0x1p-38f) {  // (the same for a whole tensor)
+#pragma unroll
+        for (int k = 0; k < N; ++k) x[k] = updated<true>(s, x[k], m[k], v[k]);
+    } else {
+#pragma unroll
+        for (int k = 0; k < N; ++k) x[k] = updated<false>(s, x[k], m[k], v[k]);
+    }
 }
 
 // N entries at `at`, all of them or those before `n`
@@ -345,10 +365,8 @@ __global__ __launch_bounds__(kThreads) void update_kernel(UpdateTable<BITS> t) {
             load_n<TRLK_F32, N>(pm, at, n, whole, m);
             load_n<TRLK_F32, N>(pv, at, n, whole, v);
 #pragma unroll
-            for (int k = 0; k < N; ++k) {
-                moments(s, clip, y[k], m[k], v[k]);
-                x[k] = updated(s, x[k], m[k], v[k]);
-            }
+            for (int k = 0; k < N; ++k) moments(s, clip, y[k], m[k], v[k]);
+            update_n(s, m, v, x);
             store_n<DT, N>(p, at, n, whole, x);
             store_n<TRLK_F32, N>(pm, at, n, whole, m);
             store_n<TRLK_F32, N>(pv, at, n, whole, v);
@@ -377,12 +395,12 @@ __global__ __launch_bounds__(kThreads) void update_kernel(UpdateTable<BITS> t) {
                 m[k] *= sm;
                 v[k] = decode8<4>(cv[k / 4] >> (8 * (k % 4)) & 0xffu) * sv;
                 moments(s, clip, y[k], m[k], v[k]);
-                x[k] = updated(s, x[k], m[k], v[k]);
                 if (whole || at + k < n) {
                     am = __builtin_elementwise_maximum(am, fabsf(m[k]));
                     av = __builtin_elementwise_maximum(av, v[k]);
                 }
             }
+            update_n(s, m, v, x);
             store_n<DT, N>(p, at, n, whole, x);
             am = half_wave_max(am);
             av = half_wave_max(av);
