@@ -134,3 +134,29 @@ def test_copies_and_pickles_are_whole():
         (a, b) = other.param_groups[0]["params"]
         assert torch.equal(a, w[0]) and torch.equal(other.state[b]["exp_avg"], opt.state[w[1]]["exp_avg"])
         assert other.step() is None  # (no gradients: nothing to do)
+
+
+def test_what_looks_on_sees_the_operator(monkeypatch):
+    """The way past the dispatcher is for calls that nobody watches: under a function mode or a profiler the operator itself is called."""
+    import torch.overrides
+
+    from trl_amd import _lib, ops
+
+    taken = []
+    monkeypatch.setattr(_lib, "py_adamw_step", lambda args: taken.append("entry point") or torch.zeros(()))
+    monkeypatch.setattr(ops, "_adamw_step_op", lambda *args: taken.append("operator") or torch.zeros(()))
+
+    class Mode(torch.overrides.TorchFunctionMode):
+        def __torch_function__(self, func, types, args=(), kwargs=None):
+            return func(*args, **(kwargs or {}))
+
+    ops.adamw_step_()
+    with Mode():
+        ops.adamw_step_()
+    with torch.profiler.profile(activities=[torch.profiler.ProfilerActivity.CPU]):
+        ops.adamw_step_()
+    ops.adamw_step_()
+    assert taken == ["entry point", "operator", "operator", "entry point"]
+    monkeypatch.delattr(torch._C, "_len_torch_function_stack")  # (a torch that does not answer)
+    ops.adamw_step_()
+    assert taken[4:] == ["operator"]

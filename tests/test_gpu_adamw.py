@@ -592,3 +592,13 @@ def test_tiny_second_moments(bits, eps, dtype):
     # (0 / 0 is a NaN, anything else over 0 infinite, as in `torch.optim.AdamW`; what is too large for the type is infinite, too)
     assert torch.equal(rest.isnan(), want[~finite].isnan()) and bool((rest.isnan() | (rest.abs() >= torch.finfo(t).max / 4)).all())
     assert bool(finite.all()) == (eps > 0)
+
+
+def test_a_profiler_sees_the_operator():
+    import trl_amd
+
+    p, grads, put = make([(300,)], torch.float32, 3)
+    m, v = zeros32([(300,)], put)
+    with torch.profiler.profile(activities=[torch.profiler.ProfilerActivity.CPU]) as prof:
+        trl_amd.adamw_step_(p, grads, m, v, step_counters(1))
+    assert "trl_amd::adamw_step_" in {e.key for e in prof.key_averages()}

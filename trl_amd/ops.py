@@ -72,12 +72,17 @@ def raise_for_error_bits(bits: float, device: torch.device) -> None:
 
 
 def _observed() -> bool:
-    """Whether a tracer, a dispatch mode or a function transform is at work.  A torch that does not answer counts as one where it is."""
+    """Whether a tracer, a dispatch or function mode, a function transform or a profiler is at work.  A torch that does not answer counts as one
+    where it is."""
     if torch.compiler.is_compiling() or torch.jit.is_tracing():
         return True
     modes = getattr(torch._C, "_len_torch_dispatch_stack", None)
+    function_modes = getattr(torch._C, "_len_torch_function_stack", None)
     transforms = getattr(torch._C, "_are_functorch_transforms_active", None)
-    return modes is None or transforms is None or modes() > 0 or transforms()
+    profiled = getattr(torch.autograd, "_profiler_enabled", None)
+    if modes is None or function_modes is None or transforms is None or profiled is None:
+        return True
+    return modes() > 0 or function_modes() > 0 or transforms() or profiled()
 
 
 def refuse_tangents(name: str, *tensors: Tensor) -> None:
