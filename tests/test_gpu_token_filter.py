@@ -683,3 +683,23 @@ def test_a_top_k_of_a_thousand_and_more(dtype):
     for k in (900, 1024, 1025, 1500, 2500, 4095, 4097, 19999):
         for s in (settings(1.0, k), settings(0.7, k, 0.9), settings(3.0, k, 0.999, 1e-3)):
             check_draw(logits, u, s)
+
+
+@pytest.mark.parametrize("shape", [(0,), (3, 0), (0, 4), (2, 3, 0), (2, 0, 3), (0, 2, 3), (2, 0, 3, 4), (2, 3, 4, 0), (2, 1, 3, 2)])
+def test_ranks_and_no_rows(shape):
+    """Leading dimensions of any number and size, zero among them."""
+    import trl_amd
+
+    g = torch.Generator().manual_seed(5)
+    x = torch.randn(*shape, 70, generator=g).to(DEV).requires_grad_()
+    u = torch.rand(shape, generator=g).to(DEV)
+    s = settings(0.8, 9, 0.9)
+    ids, logps = trl_amd.sample_tokens(x, u, **s)
+    assert ids.shape == logps.shape == shape and ids.dtype == torch.int64
+    scored = trl_amd.filtered_logps(x, ids, **s)
+    assert scored.shape == shape and torch.equal(scored.detach(), logps)
+    scored.sum().backward()
+    assert x.grad.shape == x.shape
+    if x.numel():
+        want, _ = expected(x, s, u)
+        assert torch.equal(ids.cpu().reshape(-1), want)

@@ -601,7 +601,11 @@ struct Rows {
         (void)operand(x);
         dtype = dtype_code(x);
         vocab = x.size(-1);
-        if (x.dim() > 3) x = x.reshape({-1, x.size(-2), vocab});
+        if (x.dim() > 3) {  // (the product by itself: without rows in the last but one dimension a reshape could not tell it)
+            int64_t leading = 1;
+            for (int64_t i = 0; i < x.dim() - 2; ++i) leading *= x.size(i);
+            x = x.reshape({leading, x.size(-2), vocab});
+        }
         if ((vocab > 1 && x.stride(-1) != 1) || (x.dim() > 1 && x.size(-2) > 1 && x.stride(-2) < vocab)) x = x.contiguous();
         if (x.dim() > 1) length = x.size(-2), row_stride = x.stride(-2);
         if (x.dim() > 2) n_seq = x.size(0), seq_stride = x.stride(0);
