@@ -465,7 +465,7 @@ int trlk_sample_tokens(const void* d_logits, int dtype, int64_t n_seq, int64_t r
 /* trlk_filtered_logps_fwd: log(w_token / C_last) of given tokens (d_index int64 [rows]) under the same distribution; -inf for a
  * token that the filters take away, NaN (and the flag TRLK_FLAG_INDEX_OUT_OF_RANGE) for one outside [0, vocab), 0 for a row
  * whose mask is 0.  d_out_state fp32 [rows, 4] and d_out_block_max (in the logits' type, [rows, trlk_token_filter_blocks(vocab)];
- * may be NULL) are what the backward needs; block maxima exist where trlk_token_filter_has_blocks(...) is 1.
+ * 16-byte aligned, may be NULL) are what the backward needs; block maxima exist where trlk_token_filter_has_blocks(...) is 1.
  * trlk_filtered_logps_bwd: the whole gradient of the logits, d_dlogits dense [rows, vocab],
  *   dlogits[r, v] = g_logp[r] / T * (1[v == index[r]] - w_v / C_last)
  * (the kept tokens are taken as given), 0 in rows whose token lies outside the support, whose mask is 0 or whose g_logp is 0.

@@ -170,3 +170,17 @@ def test_launches_that_would_have_too_many_threads_are_refused():
     t.numel = 1 << 34
     assert step() == -6
     assert _lib.lib.trlk_adamw_state_values(FAKE, FAKE, (1 << 34) + 1, 1, FAKE, None) == -2
+
+
+def test_block_maxima_are_read_by_vectors():
+    """The caller's buffer of block maxima has the alignment that 16-byte loads of it need."""
+    from trl_amd import _lib
+
+    def fwd(dtype, block_max):
+        return _lib.lib.trlk_filtered_logps_fwd(FAKE, dtype, 1, 3, 100, 300, 100, FAKE, 1.0, None, 5, None, 1.0, None, 0.0, None, None, FAKE, FAKE,
+                                                block_max, None, FAKE, 8, None)
+
+    for dtype in (_lib.F32, _lib.BF16, _lib.F16):
+        for off in (2, 4, 8, 12):
+            assert fwd(dtype, FAKE + off) == -4 and "block maxima" in _lib.last_error()
+        assert fwd(dtype, FAKE) == -6 and fwd(dtype, FAKE + 16) == -6  # (aligned: the workspace is too small)

@@ -1801,7 +1801,8 @@ extern "C" int trlk_filtered_logps_fwd(const void* d_logits, int dtype, int64_t 
     a.rows = n_seq * rows_per_seq;
     if (a.rows == 0) return TRLK_OK;
     TRLK_REQUIRE(d_index && d_out_logp && d_out_state, TRLK_ERR_NULL_POINTER, "filtered_logps: null operand");
-    TRLK_REQUIRE(reinterpret_cast<uintptr_t>(d_out_block_max) % elem_size(dtype) == 0, TRLK_ERR_BAD_STRIDE, "filtered_logps: misaligned block maxima");
+    // (the selection reads them by vectors: a row has a multiple of 32 of them)
+    TRLK_REQUIRE(reinterpret_cast<uintptr_t>(d_out_block_max) % 16 == 0, TRLK_ERR_BAD_STRIDE, "filtered_logps: misaligned block maxima");
     a.chunks = int32_t(chunks_of(vocab));
     a.row_mask = d_row_mask;
     a.index = d_index;
