@@ -491,7 +491,8 @@ int trlk_filtered_logps_bwd(const void* d_logits, int dtype, int64_t n_seq, int6
  *   t += 1;  m = beta1 m + (1 - beta1) clip g;  v = beta2 v + (1 - beta2) (clip g)^2
  *   p = p (1 - lr weight_decay) - lr / (1 - beta1^t) * m / (sqrt(v) / sqrt(1 - beta2^t) + eps)
  * in fp32, p rounded once to its type.  The tables are HOST memory, read before the call returns.  All operands of a tensor have
- * `numel` (2^34 at most) entries in the same order; no two tensors share one.  d_step (fp32, device) counts the tensor's steps.
+ * `numel` (2^34 at most) entries in the same order; no two of those that are written (parameters, moments, scales, steps) share memory,
+ * nor does a gradient with one of them.  d_step (fp32, device) counts the tensor's steps.
  *   state_bits 32: d_exp_avg, d_exp_avg_sq fp32
  *   state_bits 8:  codes of one byte in blocks of 256 entries, with fp32 scales (powers of two), one per block
  *                  exp_avg: sign, 4 bits of exponent (bias 7), 3 of mantissa (e4m3);  exp_avg_sq: 4 bits of exponent (bias 7), 4

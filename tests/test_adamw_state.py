@@ -160,3 +160,40 @@ def test_what_looks_on_sees_the_operator(monkeypatch):
     monkeypatch.delattr(torch._C, "_len_torch_function_stack")  # (a torch that does not answer)
     ops.adamw_step_()
     assert taken[4:] == ["operator"]
+
+
+def test_operands_that_share_memory_are_refused():
+    """Two workgroups would write the same entries.  (On the host: the check comes before that of the device.)"""
+    import trl_amd
+
+    def call(p=None, g=None, m=None, v=None, s=None, **kw):
+        new = lambda: [torch.zeros(600) for _ in range(2)]  # noqa: E731
+        trl_amd.adamw_step_(p or new(), g or new(), m or new(), v or new(), s or [torch.zeros(()) for _ in range(2)], **kw)
+
+    x, y = torch.zeros(600), torch.zeros(600)
+    flat = torch.zeros(1801)
+    apart, over = [flat[:600], flat[600:1200]], [flat[:600], flat[599:1199]]
+    for ok in (dict(), dict(p=apart), dict(m=apart), dict(p=[flat[1201:], flat[:600]], v=[flat[600:1200], y]), dict(g=[x, x]), dict(g=over),
+               dict(g=[flat[:600], x], p=[flat[600:1200], y])):
+        with pytest.raises(RuntimeError, match="not on a GPU"):
+            call(**ok)
+    step = torch.zeros(())
+    for bad in (dict(p=[x, x]), dict(p=over), dict(m=[x, x]), dict(v=over), dict(s=[step, step]), dict(m=[x, y], v=[y, x]), dict(p=[x, y], m=[y, flat[:600]]),
+                dict(p=[x, y], g=[y, x]), dict(p=apart, g=[flat[300:900], x]), dict(p=[flat[1:601], y], s=[flat[0], flat[600]])):
+        with pytest.raises(ValueError, match="twice|share"):
+            call(**bad)
+    codes = [torch.zeros(600, dtype=torch.uint8) for _ in range(4)]
+    eight = dict(m=[c.view(torch.float8_e4m3fn) for c in codes[:2]], v=codes[2:])
+    scales = [torch.ones(3) for _ in range(4)]
+    with pytest.raises(RuntimeError, match="not on a GPU"):
+        call(**eight, exp_avg_scales=scales[:2], exp_avg_sq_scales=scales[2:])
+    with pytest.raises(ValueError, match="twice|share"):
+        call(**eight, exp_avg_scales=scales[:2], exp_avg_sq_scales=[scales[2], scales[0]])
+    with pytest.raises(ValueError, match="twice|share"):
+        call(m=eight["m"], v=[codes[0], codes[2]], exp_avg_scales=scales[:2], exp_avg_sq_scales=scales[2:])
+    none = torch.zeros(0)
+    with pytest.raises(RuntimeError, match="not on a GPU"):  # (an empty tensor shares nothing, and stands for no scale)
+        call([none, none], [none, none], [none, none], [none, none], exp_avg_scales=[none, none], exp_avg_sq_scales=[none, none])
+    one = torch.ones(1)
+    with pytest.raises(RuntimeError, match="not on a GPU"):  # (scales of fp32 moments are not looked at)
+        call(exp_avg_scales=[one, one], exp_avg_sq_scales=[one, one])

@@ -21,7 +21,7 @@ def adamw_step_(params: list[Tensor], grads: list[Tensor], exp_avgs: list[Tensor
                 exp_avg_sq_scales: list[Tensor] | None = None, seed: int = 0) -> Tensor | None:
     """One AdamW step on `params` in place, each in fp32, bf16 or fp16 with a gradient of its type.  The arithmetic is
     `torch.optim.AdamW`'s, in fp32; parameters are rounded once to their type.  `steps` (fp32, one number each, on the GPU) count
-    up first.  `lr` may be an fp32 number on the GPU.
+    up first.  `lr` may be an fp32 number on the GPU.  Tensors that are written share no memory, with each other or with a gradient.
 
     With `max_grad_norm` the gradients count as multiplied by `min(1, max_grad_norm / (norm + 1e-6))`, `norm` the 2-norm of all of
     them, as `torch.nn.utils.clip_grad_norm_` does (which writes them; they stay as they are here), and the norm is returned (fp32,
