@@ -444,9 +444,9 @@ int trlk_scale_unless_one(void* d_data, int dtype, int64_t n_elems, const float*
  * 0 for the others, and C_v = w_0 + ... + w_v:
  *   token = min { v : C_v > u C_last },  logp = log(w_token / C_last)
  * Weights and their sums are held in 64 bits, so that a row's token is the same one whatever the number of rows.
- * Each setting is one number for all rows (0 <= temperature < inf, top_k <= 0: none, 0 < top_p <= 1, 0 <= min_p <= 1) or, where
+ * Each setting is one number for all rows (0 <= temperature <= 2^100, top_k <= 0: none, 0 < top_p <= 1, 0 <= min_p <= 1) or, where
  * d_temperature / d_top_k / d_top_p / d_min_p is not NULL, one for each row (top_p <= 0: the first token, > 1: 1, min_p < 0: 0,
- * > 1: 1).  A row without a distribution (a NaN or +inf, nothing but -inf, or a temperature that is negative, infinite or NaN, a
+ * > 1: 1).  A row without a distribution (a NaN or +inf, nothing but -inf, or a temperature that is negative, over 2^100 or NaN, a
  * NaN top_p or min_p) gets the token -1 and a NaN log-prob, and sets TRLK_FLAG_NO_DISTRIBUTION in *d_error_flag (may be NULL).
  * d_row_mask (optional, uint8 [rows]): rows whose mask is 0 are not read, and get the token fill_id and the log-prob 0.
  * d_uniform: numbers in [0, 1), fp64 if uniform_f64 is non-zero, else fp32.  vocab <= trlk_token_filter_max_vocab().  Fewer than 2^23

@@ -184,3 +184,22 @@ def test_block_maxima_are_read_by_vectors():
         for off in (2, 4, 8, 12):
             assert fwd(dtype, FAKE + off) == -4 and "block maxima" in _lib.last_error()
         assert fwd(dtype, FAKE) == -6 and fwd(dtype, FAKE + 16) == -6  # (aligned: the workspace is too small)
+
+
+def test_temperatures_beyond_what_distances_in_fp32_bear():
+    """Over 2^100 logits that are further apart than the largest fp32 number would both count."""
+    from trl_amd import _lib
+
+    def call(t, entry):
+        if entry == "sample":
+            return _lib.lib.trlk_sample_tokens(FAKE, _lib.F32, 1, 3, 100, 300, 100, FAKE, 0, t, None, 0, None, 0.9, None, 0.0, None, None, 0, FAKE, FAKE,
+                                               None, FAKE, 8, None)
+        if entry == "score":
+            return _lib.lib.trlk_filtered_logps_fwd(FAKE, _lib.F32, 1, 3, 100, 300, 100, FAKE, t, None, 0, None, 0.9, None, 0.0, None, None, FAKE, FAKE,
+                                                    None, None, FAKE, 8, None)
+        return _lib.lib.trlk_filtered_logps_bwd(FAKE, _lib.F32, 1, 3, 100, 300, 100, FAKE, t, None, None, None, FAKE, FAKE, None)
+
+    for entry, fine in (("sample", -6), ("score", -6), ("gradient", -1)):  # (the workspace is too small, an operand is missing)
+        for t in (2.0**100 * (1 + 2.0**-52), 1.7e38, 1e300):
+            assert call(t, entry) == -5 and "2^100" in _lib.last_error()
+        assert call(2.0**100, entry) == fine and call(0.0, entry) == fine

@@ -703,3 +703,26 @@ def test_ranks_and_no_rows(shape):
     if x.numel():
         want, _ = expected(x, s, u)
         assert torch.equal(ids.cpu().reshape(-1), want)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
+def test_the_largest_temperatures_and_logits(dtype):
+    """Logits of up to 3e38 and a temperature of up to 2^100: distances beyond fp32's range have no weight.  Larger temperatures of a row's own
+    have no distribution."""
+    import trl_amd
+
+    g = torch.Generator().manual_seed(31)
+    for V in (300, 6000):
+        near = (torch.rand(6, V, generator=g) * 2.0**101 - 2.0**100).to(DTYPES[dtype])
+        far = ((torch.rand(6, V, generator=g) * 2 - 1) * 3e38).to(DTYPES[dtype])
+        far[::2, : V // 2] = 3e38
+        u = torch.rand(6, generator=g)
+        for logits in (near, far):
+            for s in (settings(2.0**100), settings(2.0**100, 0, 0.9), settings(2.0**99, 0, 1.0, 0.3), settings(2.0**100, 0, 0.95, 0.2),
+                      settings(2.0**100, 20, 0.9)):
+                check_draw(logits, u, s)
+        t = torch.tensor([2.0**100, 2.0**101, 3e38, 1.0, math.inf, 0.0], device=DEV)
+        ids, lp = trl_amd.sample_tokens(near.to(DEV), u.to(DEV), t, 0, 0.9)
+        with pytest.raises(ValueError, match="no distribution"):
+            trl_amd.check_device_errors()
+        assert (ids < 0).tolist() == [False, True, True, False, True, False] and torch.equal(lp.isnan(), ids < 0)

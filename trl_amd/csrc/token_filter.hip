@@ -45,6 +45,9 @@ constexpr int kLine = 128;                   // bytes of a cache line
 constexpr int kLongRows = 32;                // rows with very many candidates whose passes all CUs share
 constexpr int kHalf = kChunk / 2;            // logits of a wave's step in these passes
 constexpr int64_t kMaxVocab = int64_t(1) << 22;
+// Temperatures up to it: over 2^100 logits further apart than the largest fp32 number could both count, and their distance is not one.  (Under it
+// whatever is over 2^127 away from the maximum has no weight, and a bound that the filters set lies less than 2^111 under it.)
+constexpr double kMaxTemperature = 0x1p100;
 constexpr int64_t kMaxRows = (int64_t(1) << 32) / kSelThreads, kMaxUnits = (int64_t(1) << 32) / kWave - 8;
 
 typedef unsigned long long u64;
@@ -229,7 +232,7 @@ __device__ __forceinline__ RowFilter row_filter(const Filters& f, int64_t row, i
     const double q = f.d_min_p ? double(f.d_min_p[row]) : f.min_p;
     int64_t k = f.d_top_k ? int64_t(f.d_top_k[row]) : f.top_k;
     RowFilter r;
-    r.ok = T >= 0.0 && T < INFINITY && p == p && q == q;
+    r.ok = T >= 0.0 && T <= kMaxTemperature && p == p && q == q;
     if (T == 0.0) {
         T = 1.0;
         k = 1;
@@ -1610,8 +1613,8 @@ int64_t chunks_of(int64_t vocab) { return (vocab + kChunk - 1) / kChunk; }
 size_t up16(size_t n) { return (n + 15) / 16 * 16; }
 
 int check_filters(const Filters& f, const char* what) {
-    TRLK_REQUIRE(f.d_temperature || (f.temperature >= 0.0 && f.temperature < INFINITY), TRLK_ERR_BAD_VALUE,
-                 "%s: temperature must be >= 0 and finite", what);
+    TRLK_REQUIRE(f.d_temperature || (f.temperature >= 0.0 && f.temperature <= kMaxTemperature), TRLK_ERR_BAD_VALUE,
+                 "%s: temperature must be from 0 to 2^100", what);
     TRLK_REQUIRE(f.d_temperature || f.temperature == 0.0 || 1.4426950408889634074 / f.temperature < INFINITY, TRLK_ERR_BAD_VALUE,
                  "%s: temperature is too small", what);
     TRLK_REQUIRE(f.d_top_p || (f.top_p > 0.0 && f.top_p <= 1.0), TRLK_ERR_BAD_VALUE, "%s: top_p must be in (0, 1]", what);
@@ -1825,8 +1828,8 @@ extern "C" int trlk_filtered_logps_bwd(const void* d_logits, int dtype, int64_t 
     FilterBwdArgs a{};
     a.x = RowView{d_logits, rows_per_seq, vocab, seq_stride, row_stride};
     if (const int rc = check_view(a.x, dtype, n_seq, "filtered_logps backward")) return rc;
-    TRLK_REQUIRE(d_temperature || (temperature >= 0.0 && temperature < INFINITY), TRLK_ERR_BAD_VALUE,
-                 "filtered_logps backward: temperature must be >= 0 and finite");
+    TRLK_REQUIRE(d_temperature || (temperature >= 0.0 && temperature <= kMaxTemperature), TRLK_ERR_BAD_VALUE,
+                 "filtered_logps backward: temperature must be from 0 to 2^100");
     a.rows = n_seq * rows_per_seq;
     if (a.rows == 0) return TRLK_OK;
     TRLK_REQUIRE(d_index && d_state && d_g_logp && d_dlogits, TRLK_ERR_NULL_POINTER, "filtered_logps backward: null operand");

@@ -138,7 +138,7 @@ def sample_tokens(logits: Tensor, uniforms: Tensor, temperature: float | Tensor 
 
     A row's tokens are ordered by logit, ties by index.  `top_k` > 0 keeps the first k of them, `top_p` < 1 those before which
     less than `top_p` of the mass lies that top-k kept (one at least), `min_p` > 0 those of at least `min_p` times the largest
-    probability; `None`, and a `top_k` of 0 or less, switches a filter off.  A temperature of 0 takes the first token (log-prob 0).
+    probability; `None`, and a `top_k` of 0 or less, switches a filter off.  A temperature (2^100 at most) of 0 takes the first token (log-prob 0).
     The token is the first one in index order whose cumulative probability exceeds the uniform number.  All sums are held in 64
     bits: a row's token depends on its logits, settings and number alone, not on the batch.  Each setting is a number, or a
     tensor `[...]` with a value for each row.
