@@ -726,3 +726,23 @@ def test_the_largest_temperatures_and_logits(dtype):
         with pytest.raises(ValueError, match="no distribution"):
             trl_amd.check_device_errors()
         assert (ids < 0).tolist() == [False, True, True, False, True, False] and torch.equal(lp.isnan(), ids < 0)
+
+
+@pytest.mark.parametrize("V", [5, 3000])
+def test_the_gradient_at_the_smallest_temperatures(V):
+    """1 / T beyond fp32: where one token has all of the mass the gradient is 0, where two equal ones share it it is infinite, elsewhere 0."""
+    import trl_amd
+
+    for T in (1e-38, 1e-39, 1e-60, 1e-300):
+        x = torch.linspace(-1, 1, V).repeat(3, 1)
+        x[1, V - 2] = 1.0
+        x = x.to(DEV).requires_grad_()
+        for s in (settings(T), settings(T, 0, 0.9), settings(T, 3)):
+            ids = torch.full((3,), V - 1, device=DEV)
+            lp = trl_amd.filtered_logps(x, ids, **s)
+            want = torch.tensor([0.0, -math.log(2.0), 0.0])
+            assert bool(((lp.detach().cpu() - want).abs() <= 1e-6).all())
+            (grad,) = torch.autograd.grad(lp, x, torch.tensor([100.0, 100.0, 0.0], device=DEV))
+            grad = grad.cpu()
+            assert not grad[0].any() and not grad[2].any() and not grad[1, :-2].any()
+            assert grad[1, -1] == math.inf and grad[1, -2] == -math.inf

@@ -23,6 +23,7 @@
 //
 // Whole numbers come out, and the same ones whatever the launch: sums of weights are 64-bit floats in a fixed order over a row's
 // chunks, or 64-bit integers (weights in units of 2^-fix, whose sums do not depend on the order in which threads add them).
+#include <cfloat>
 #include <type_traits>
 
 #include "common.hpp"
@@ -1557,7 +1558,8 @@ __global__ __launch_bounds__(kScanThreads) void filter_bwd_kernel(FilterBwdArgs 
     const uint32_t bi = __float_as_uint(a.state[row * int64_t(4) + 1]);
     double temp = a.d_temperature ? double(a.d_temperature[row]) : a.temperature;
     temp = temp == 0.0 ? 1.0 : temp;
-    const float g = float(double(g0) / temp), c = float(1.4426950408889634074 / temp);
+    const float g = float(double(g0) / temp), c = fminf(float(1.4426950408889634074 / temp), FLT_MAX);  // (distances of 0 stay 0)
+    const bool too_large = fabsf(g) == INFINITY && fabsf(g0) < INFINITY;  // for fp32, but 0 times it is 0: a temperature of next to nothing
     const bool active = bx < INFINITY && g0 != 0.f;
     const int token = active ? int(a.index[row]) : -1;  // (within the row: the forward has looked)
     const T* x = a.x.row<DT>(row);
@@ -1590,6 +1592,10 @@ __global__ __launch_bounds__(kScanThreads) void filter_bwd_kernel(FilterBwdArgs 
                 const bool kept = v[e] > bx || (v[e] == bx && uint32_t(j) <= bi);
                 const float p = kept ? fast_exp2(fmaf(v[e] - m, c, -l2)) : 0.f;
                 y[e] = g * ((j == token ? 1.f : 0.f) - p);
+            }
+            if (too_large) {
+#pragma unroll
+                for (int e = 0; e < EPV; ++e) y[e] = y[e] == y[e] ? y[e] : 0.f;
             }
         }
         if (whole) {
