@@ -58,3 +58,23 @@ def test_operands_without_a_tangent_are_taken_at_a_dual_level(name):
     with FakeTensorMode(), fad.dual_level():
         call, x = calls(torch.bfloat16)[name]
         assert call(x).shape == call(x.requires_grad_()).shape and call(x).requires_grad
+
+
+def test_settings_have_no_derivative():
+    """A setting with a value for each row that wants a gradient, or has a tangent, is refused: it would get none, without an error."""
+    import trl_amd
+
+    with FakeTensorMode():
+        logits, ids = torch.empty(B, V, device="cuda", requires_grad=True), torch.zeros(B, dtype=torch.long, device="cuda")
+        for name in ("temperature", "top_p", "min_p"):
+            t = torch.full((B,), 0.5, device="cuda")
+            assert trl_amd.filtered_logps(logits, ids, **{name: t}).requires_grad
+            with fad.dual_level(), pytest.raises(RuntimeError, match="detach"):
+                trl_amd.filtered_logps(logits.detach(), ids, **{name: fad.make_dual(t, t)})
+            t.requires_grad_()
+            for x in (logits, logits.detach()):
+                with pytest.raises(RuntimeError, match="detach"):
+                    trl_amd.filtered_logps(x, ids, **{name: t})
+            assert trl_amd.filtered_logps(logits, ids, **{name: t.detach()}).requires_grad
+            with torch.no_grad():
+                trl_amd.filtered_logps(logits, ids, **{name: t})

@@ -720,6 +720,8 @@ class FilteredLogps : public torch::autograd::Function<FilteredLogps> {
 Tensor3 filtered_logps_fwd_autograd(const Tensor& logits, const Tensor& index, double temperature, int64_t top_k, double top_p,
                                     double min_p, const optional<Tensor>& temperatures, const optional<Tensor>& top_ks,
                                     const optional<Tensor>& top_ps, const optional<Tensor>& min_ps, const optional<Tensor>& row_mask) {
+    TORCH_CHECK(!needs_grad(temperatures) && !needs_grad(top_ps) && !needs_grad(min_ps),
+                "filtered_logps is differentiable with respect to the logits alone: detach the settings");
     if (needs_grad({&logits})) {
         const auto r = FilteredLogps::apply(logits, index, temperature, top_k, top_p, min_p, temperatures, top_ks, top_ps, min_ps, row_mask);
         return {r[0], r[1], r[2]};

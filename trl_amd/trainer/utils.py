@@ -157,7 +157,7 @@ def filtered_logps(logits: Tensor, index: Tensor, temperature: float | Tensor = 
                    top_p: float | Tensor | None = 1.0, min_p: float | Tensor | None = 0.0,
                    row_mask: Tensor | None = None) -> Tensor:
     """fp32 log-probs `[...]` of the tokens `index` (`[...]`, int64) under the distribution that `sample_tokens` draws from with
-    the same settings, differentiable w.r.t. `logits` (`[..., V]`).  `selective_log_softmax` scores under the whole
+    the same settings, differentiable w.r.t. `logits` (`[..., V]`) alone: a setting that requires a gradient raises.  `selective_log_softmax` scores under the whole
     vocabulary: with top-k, top-p or min-p in generation, the ratio of the two would compare distributions of different support.
 
     A token that the filters take away has log-prob -inf and its row no gradient.  The gradient takes the kept set as given:
