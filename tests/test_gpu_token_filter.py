@@ -746,3 +746,21 @@ def test_the_gradient_at_the_smallest_temperatures(V):
             grad = grad.cpu()
             assert not grad[0].any() and not grad[2].any() and not grad[1, :-2].any()
             assert grad[1, -1] == math.inf and grad[1, -2] == -math.inf
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
+@pytest.mark.parametrize("rows", [3, 515])
+def test_min_p_ends_a_long_row_before_top_p(rows, dtype):
+    """Thousands of tokens over min-p's border that hold less than top_p of the mass: the border is min-p's, and top-p's is not looked at."""
+    import trl_amd
+
+    V = 20000
+    g = torch.Generator().manual_seed(rows)
+    w = torch.where(torch.rand(rows, V, generator=g) < 0.3, 0.2 + 0.8 * torch.rand(rows, V, generator=g), 0.1 * (1 - 0.2 * torch.rand(rows, V, generator=g)))
+    logits, u = w.log().to(DTYPES[dtype]), torch.rand(rows, generator=g)
+    s = settings(1.0, 0, 0.95, 0.15)
+    tokens, weights = row_support(logits[0].double(), 1.0, 0, 0.95, 0.15)
+    assert len(tokens) > 4096 and float(weights.sum() / (logits[0].double() - logits[0].double().max()).exp().sum()) < 0.8
+    check_draw(logits, u, s)
+    ids, lp = trl_amd.sample_tokens(logits.to(DEV), u.to(DEV), **s)
+    assert torch.equal(trl_amd.filtered_logps(logits.to(DEV), ids, **s), lp)
