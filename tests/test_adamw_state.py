@@ -197,3 +197,17 @@ def test_operands_that_share_memory_are_refused():
     one = torch.ones(1)
     with pytest.raises(RuntimeError, match="not on a GPU"):  # (scales of fp32 moments are not looked at)
         call(exp_avg_scales=[one, one], exp_avg_sq_scales=[one, one])
+
+
+def test_groups_of_their_own_settings():
+    import trl_amd
+
+    w = [torch.nn.Parameter(torch.zeros(5000)) for _ in range(2)]
+    opt = trl_amd.AdamW([dict(params=w[:1], state_bits=8), dict(params=w[1:])])
+    kinds = [opt._state_of(p, g)["exp_avg"].dtype for g in opt.param_groups for p in g["params"]]
+    assert kinds == [torch.float8_e4m3fn, torch.float32]
+    for bad in (dict(state_bits=16), dict(state_bits="8"), dict(lr=-1.0), dict(eps=-1.0), dict(weight_decay=-1.0), dict(betas=(0.9, 1.0))):
+        with pytest.raises(ValueError):
+            trl_amd.AdamW([dict(params=w, **bad)])
+        with pytest.raises(ValueError):
+            trl_amd.AdamW(w[:1]).add_param_group(dict(params=w[1:], **bad))

@@ -48,6 +48,15 @@ def adamw_state_values(codes: Tensor, scales: Tensor) -> Tensor:
     return ops.adamw_state_values(codes, scales)
 
 
+def _check_settings(lr, betas, eps, weight_decay, state_bits) -> None:
+    if state_bits not in (8, 32):
+        raise ValueError(f"state_bits must be 8 or 32, got {state_bits}")
+    if not 0.0 <= float(lr) or not 0.0 <= eps or not 0.0 <= weight_decay:
+        raise ValueError(f"lr, eps and weight_decay must not be negative, got {lr}, {eps}, {weight_decay}")
+    if not 0.0 <= betas[0] < 1.0 or not 0.0 <= betas[1] < 1.0:
+        raise ValueError(f"betas must be in [0, 1), got {betas}")
+
+
 class AdamW(torch.optim.Optimizer):
     """AdamW whose step is one call for all parameter groups (`adamw_step_`), for GPU parameters in fp32, bf16 or fp16.
 
@@ -59,16 +68,15 @@ class AdamW(torch.optim.Optimizer):
     def __init__(self, params, lr: float | Tensor = 1e-3, betas: tuple[float, float] = (0.9, 0.999), eps: float = 1e-8,
                  weight_decay: float = 0.01, *, state_bits: int = 32, min_8bit_size: int = 4096, max_grad_norm: float | None = None,
                  seed: int = 0, keep_32bit: Iterable[Tensor] = ()):
-        if state_bits not in (8, 32):
-            raise ValueError(f"state_bits must be 8 or 32, got {state_bits}")
-        if not 0.0 <= float(lr) or not 0.0 <= eps or not 0.0 <= weight_decay:
-            raise ValueError(f"lr, eps and weight_decay must not be negative, got {lr}, {eps}, {weight_decay}")
-        if not 0.0 <= betas[0] < 1.0 or not 0.0 <= betas[1] < 1.0:
-            raise ValueError(f"betas must be in [0, 1), got {betas}")
+        _check_settings(lr, betas, eps, weight_decay, state_bits)
         self.max_grad_norm = None if max_grad_norm is None else _clip(max_grad_norm)
         self.seed, self.grad_norm, self.keep_32bit = int(seed), None, set(keep_32bit)
         super().__init__(params, dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay, state_bits=state_bits,
                                       min_8bit_size=min_8bit_size))
+
+    def add_param_group(self, param_group: dict) -> None:
+        _check_settings(**{k: param_group.get(k, self.defaults[k]) for k in ("lr", "betas", "eps", "weight_decay", "state_bits")})
+        super().add_param_group(param_group)
 
     def __getstate__(self) -> dict:
         return {**super().__getstate__(), "max_grad_norm": self.max_grad_norm, "seed": self.seed, "grad_norm": self.grad_norm,
