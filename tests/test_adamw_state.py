@@ -211,3 +211,13 @@ def test_groups_of_their_own_settings():
             trl_amd.AdamW([dict(params=w, **bad)])
         with pytest.raises(ValueError):
             trl_amd.AdamW(w[:1]).add_param_group(dict(params=w[1:], **bad))
+
+
+def test_other_entries_of_a_state_are_loaded_as_by_the_base_class():
+    w, opt = optimiser()
+    saved = torch_state()
+    saved["state"][1]["seen"] = 17
+    saved["state"][0]["step"] = 2  # (a number instead of a tensor)
+    opt.load_state_dict(saved)
+    assert opt.state[w[1]]["seen"] == 17 and opt.state_dict()["state"][1]["seen"] == 17
+    assert opt.state[w[0]]["step"].dtype == torch.float32 and opt.state[w[0]]["step"].item() == 2.0

@@ -61,9 +61,10 @@ class AdamW(torch.optim.Optimizer):
     """AdamW whose step is one call for all parameter groups (`adamw_step_`), for GPU parameters in fp32, bf16 or fp16.
 
     `state_bits=8` holds both moments of every parameter of `min_8bit_size` entries or more in 8 bits, 2.03 bytes per entry instead
-    of 8, but for those in `keep_32bit`.  With `max_grad_norm` the step clips the norm over all groups, without a pass that writes the gradients, and leaves it in
-    `grad_norm` (fp32, on the GPU); `transformers.Trainer` then runs with `max_grad_norm=0`.  Step counters live on the GPU and a
-    group's `lr` may: a step can be captured into a graph.  Parameters without a gradient are left alone."""
+    of 8, but for those in `keep_32bit`.  With `max_grad_norm` the step clips the norm over all groups (of this process's tensors), without a
+    pass that writes the gradients, and leaves it in `grad_norm` (fp32, on the GPU); `transformers.Trainer` then runs with `max_grad_norm=0`.
+    Step counters live on the GPU and a group's `lr` may: a step can be captured into a graph.  Parameters without a gradient are left alone; the
+    others lie on one GPU.  Moments are fp32 (or in 8 bits) whatever the parameters' type."""
 
     def __init__(self, params, lr: float | Tensor = 1e-3, betas: tuple[float, float] = (0.9, 0.999), eps: float = 1e-8,
                  weight_decay: float = 0.01, *, state_bits: int = 32, min_8bit_size: int = 4096, max_grad_norm: float | None = None,
@@ -183,13 +184,11 @@ class AdamW(torch.optim.Optimizer):
         ids = [i for g in state_dict["param_groups"] for i in g["params"]]
         params = [p for g in self.param_groups for p in g["params"]]
         for i, p in zip(ids, params):
-            if i in state_dict["state"]:
-                saved = state_dict["state"][i]
-                names = ("step", "exp_avg", "exp_avg_sq", "exp_avg_scale", "exp_avg_sq_scale")
-                self.state[p] = {k: torch.as_tensor(saved[k]).to(device=p.device, copy=True) for k in names if k in saved}
-                for k, v in self.state[p].items():
-                    if "exp_avg_scale" not in saved:
-                        self.state[p][k] = v.float()
+            saved = state_dict["state"].get(i, {})
+            for k in ("step", "exp_avg", "exp_avg_sq", "exp_avg_scale", "exp_avg_sq_scale"):
+                if k in saved:
+                    t = torch.as_tensor(saved[k]).to(device=p.device, copy=True)
+                    self.state[p][k] = t if "exp_avg_scale" in saved else t.float()
 
 
 _STATE_BITS = {"adamw_torch": 32, "adamw_torch_fused": 32, "adamw_8bit": 8, "adamw_bnb_8bit": 8}  # names of `TrainingArguments.optim`
