@@ -7,8 +7,9 @@
 // which has to be known first.  Three kinds of launches: partial sums of squares (64 bits), one workgroup that adds them and
 // moves every tensor's step counter on (so that a captured step counts when it is replayed), the update.  Tensors come as tables
 // in the kernels' arguments: nothing is copied to the device, and a captured graph holds its own.  Measured on 355M entries: norm 229 us in
-// fp32 (6.2 TB/s), 119 in bf16 (6.0); update 1720 us in fp32 with fp32 moments (5.8 TB/s), 405 for 117M in bf16 (6.3), 660 to 750 in bf16
-// with 8-bit moments (4.8 to 5.4: the hash and the rounding take as long as the memory).  With adapters, 224 tensors of 8192 to 81920
+// fp32 (6.2 TB/s), 118 in bf16 (6.0); update 1560 to 1720 us in fp32 with fp32 moments (5.8 to 6.4 TB/s, from box to box), 395 to 405 for 117M in
+// bf16 (6.3 to 6.5), 660 to 770 in bf16
+// with 8-bit moments (4.6 to 5.4: the hash and the rounding take as long as the memory).  With adapters, 224 tensors of 8192 to 81920
 // entries in fp32, the five launches' beginnings and ends are a third of the 66 us.
 //
 // 8-bit moments: blocks of 256 entries with a power-of-two scale that takes the block's largest entry to at most 448.  m has a
@@ -47,8 +48,8 @@ struct alignas(16) Header {
     float clip, norm, pad[2];
 };
 
-// Loads and stores of what a step touches once, past the caches: 355M fp32 entries with fp32 moments 2.02 ms instead of 2.16, 117M in bf16
-// 529 us instead of 554 (the norm's loads are plain: the update reads the gradients again).
+// Loads and stores of what a step touches once, past the caches: a step of 355M fp32 entries with fp32 moments 1.98 ms instead of 2.14, of 117M in
+// bf16 481 us instead of 544, both sides in turn (the norm's loads are plain: the update reads the gradients again).
 typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 template <typename V>
 __device__ __forceinline__ V once(const void* p) {

@@ -1538,9 +1538,12 @@ struct FilterBwdArgs {
 };
 
 // d logits = g / T * (1[v = token] - kept_v * 2^((x_v - max) * c - log2 W)): the gradient is written once, and only the blocks
-// whose maximum reaches the border are read.  A wave's vectors lie at whole cache lines of the gradient, wherever its rows start.  STREAM
-// writes past the caches: for a gradient that they cannot hold.  What is left of it in them would be written back under the next
-// scan (4096 rows of 151936 in bf16: scan 181 us after cached stores, 130 after these; the gradient itself 202 and 221 us).
+// whose maximum reaches the border are read.  Probabilities p = 2^t are in fp32: t is one rounded product and sum, log2 W comes rounded to fp32 from
+// the row state, and the power is the hardware's, so p is off by about |t| 2^-23 of itself (9e-7 of a value seen with fp32 logits; far under half a
+// step of a 16-bit gradient).  In 64 bits a logit would take 10 operations more of a kernel that the memory bounds.
+// A wave's vectors lie at whole cache lines of the gradient, wherever its rows start.  STREAM writes past the caches: for a gradient that they
+// cannot hold.  What is left of it in them would be written back under the next scan (4096 rows of 151936 in bf16: scan 181 us after cached
+// stores, 130 after these; the gradient itself 202 and 221 us).
 template <int DT, bool STREAM>
 __global__ __launch_bounds__(kScanThreads) void filter_bwd_kernel(FilterBwdArgs a) {
     typedef typename Elem<DT>::type T;
