@@ -443,7 +443,8 @@ int trlk_scale_unless_one(void* d_data, int dtype, int64_t n_elems, const float*
  * temperature 0 keeps the first token alone; -inf logits are never kept.  With w_v = exp((x_v - max) / T) for the kept tokens,
  * 0 for the others, and C_v = w_0 + ... + w_v:
  *   token = min { v : C_v > u C_last },  logp = log(w_token / C_last)
- * Weights and their sums are held in 64 bits, so that a row's token is the same one whatever the number of rows.
+ * Weights and their sums are held in 64 bits, so that a row's token is the same one whatever the number of rows; a mass that comes to 1.2e-14
+ * of itself near top_p counts as top_p.
  * Each setting is one number for all rows (0 <= temperature <= 2^100, top_k <= 0: none, 0 < top_p <= 1, 0 <= min_p <= 1) or, where
  * d_temperature / d_top_k / d_top_p / d_min_p is not NULL, one for each row (top_p <= 0: the first token, > 1: 1, min_p < 0: 0,
  * > 1: 1).  A row without a distribution (a NaN or +inf, nothing but -inf, or a temperature that is negative, over 2^100 or NaN, a

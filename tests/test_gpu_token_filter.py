@@ -764,3 +764,30 @@ def test_min_p_ends_a_long_row_before_top_p(rows, dtype):
     check_draw(logits, u, s)
     ids, lp = trl_amd.sample_tokens(logits.to(DEV), u.to(DEV), **s)
     assert torch.equal(trl_amd.filtered_logps(logits.to(DEV), ids, **s), lp)
+
+
+@pytest.mark.parametrize("dtype", list(DTYPES))
+def test_top_p_of_equal_logits_at_a_border(dtype):
+    """n equal logits, top_p a whole number of n-ths: exactly so many are kept, wherever the logits lie and whatever the temperature and the number
+    of rows (a sum that is off in its last bits must not add one)."""
+    import trl_amd
+
+    for n, V in ((2, 2), (2, 500), (4, 7000), (8, 8), (64, 64), (256, 3000), (4096, 4096), (8192, 8192)):
+        for rows in (1, 40, 520 if V < 1000 else 3):
+            g = torch.Generator().manual_seed(n + rows)
+            top = (torch.randn(rows, 1, generator=g) * 8).to(DTYPES[dtype])
+            x = torch.full((rows, V), -math.inf, dtype=DTYPES[dtype])
+            x[:, V - n :] = top
+            t = 10.0 ** (4 * torch.rand(rows, generator=g) - 2)
+            for part in (0.5, 0.25, 0.75):
+                kept = max(1, int(part * n)) if part * n == int(part * n) else None
+                if kept is None:
+                    continue
+                for u, place in ((0.0, 0), (1 - 2.0**-24, kept - 1)):
+                    s = dict(temperature=t.to(DEV), top_p=part)
+                    ids, lp = trl_amd.sample_tokens(x.to(DEV), torch.full((rows,), u, device=DEV), **s)
+                    assert bool((ids == V - n + place).all()), (n, V, rows, part, u, ids.unique())
+                    assert bool(((lp.double().cpu() + math.log(kept)).abs() <= 2.0**-24 * math.log(kept) + 1e-11).all())
+                    assert torch.equal(trl_amd.filtered_logps(x.to(DEV), ids, **s), lp)
+                out = torch.full((rows,), V - n + kept, device=DEV)
+                assert bool((trl_amd.filtered_logps(x.to(DEV), out, **s) == -math.inf).all())

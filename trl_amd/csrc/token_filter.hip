@@ -57,7 +57,7 @@ typedef u32x4 u32x4_u __attribute__((aligned(2)));  // a 16-byte vector at any e
 
 // ---- weights ---------------------------------------------------------------------------------------------------------
 // 2^t for t <= 0 in 64 bits: 2^(t - n) on [-1/2, 1/2] by a polynomial of degree 9 that interpolates it at the Chebyshev points
-// (relative error 3e-14), times 2^n.  -inf and everything under -1100 give 0.
+// (relative error 4e-14), times 2^n.  -inf and everything under -1100 give 0.
 __device__ __forceinline__ double exp2_f64(double t) {
     t = __builtin_fmax(t, -1100.0);
     const double n = __builtin_rint(t), f = t - n;
@@ -71,6 +71,25 @@ __device__ __forceinline__ double exp2_f64(double t) {
     y = __builtin_fma(y, f, 0.2402265069564034);
     y = __builtin_fma(y, f, 0.6931471805599462);
     y = __builtin_fma(y, f, 1.0);  // (2^0 is 1 to the last bit: equal logits at the top have whole weights)
+    return __builtin_amdgcn_ldexp(y, int(n));
+}
+
+// As above, of degree 11 (2e-17): for what a chunk's whole sum is multiplied by.
+__device__ __forceinline__ double exp2_f64_exact(double t) {
+    t = __builtin_fmax(t, -1100.0);
+    const double n = __builtin_rint(t), f = t - n;
+    double y = 4.4549605981865186e-10;
+    y = __builtin_fma(y, f, 7.072585949269223e-09);
+    y = __builtin_fma(y, f, 1.0178062445845774e-07);
+    y = __builtin_fma(y, f, 1.321544258792169e-06);
+    y = __builtin_fma(y, f, 1.525273382983612e-05);
+    y = __builtin_fma(y, f, 0.0001540353044173605);
+    y = __builtin_fma(y, f, 0.0013333558146416936);
+    y = __builtin_fma(y, f, 0.009618129107606888);
+    y = __builtin_fma(y, f, 0.0555041086648216);
+    y = __builtin_fma(y, f, 0.24022650695910097);
+    y = __builtin_fma(y, f, 0.6931471805599453);
+    y = __builtin_fma(y, f, 1.0);
     return __builtin_amdgcn_ldexp(y, int(n));
 }
 
@@ -719,7 +738,7 @@ __global__ __launch_bounds__(kSelThreads, LONG ? 4 : 6) void filter_select_kerne
     }
     const double c = f.c, ref = double(m), unit = __builtin_amdgcn_ldexp(1.0, a.fix);
     const auto weight = [&](float v) TRLK_INLINE { return exp2_f64((double(v) - ref) * c); };
-    const auto chunk_weight = [&](double sum, float chunk_m) TRLK_INLINE { return sum * exp2_f64(chunk_scale(chunk_m, c, f.inv_c, ref)); };
+    const auto chunk_weight = [&](double sum, float chunk_m) TRLK_INLINE { return sum * exp2_f64_exact(chunk_scale(chunk_m, c, f.inv_c, ref)); };
     // w <= 1 in units of 2^-fix, rounded to the nearest: the low bits of a sum with 1.5 * 2^52 (fix is at most 50)
     const auto fixed = [&](double w) TRLK_INLINE { return __builtin_bit_cast(u64, __builtin_fma(w, unit, 0x1.8p52)) - __builtin_bit_cast(u64, 0x1.8p52); };
     const auto log2_of = [&](u64 W) TRLK_INLINE { return log2(double(W)) - a.fix; };
@@ -837,7 +856,9 @@ __global__ __launch_bounds__(kSelThreads, LONG ? 4 : 6) void filter_select_kerne
     const auto about = [&](float v) TRLK_INLINE { return uint32_t(fast_exp2(fmaf(v - m, cf, l2)) + 0.5f); };
     const auto add_low = [&](int bin, uint32_t v) TRLK_INLINE { atomicAdd(reinterpret_cast<uint32_t*>(&s.bins[bin]), v); };  // (sums under 2^32)
     const u64 mass_target = [&]() TRLK_INLINE {  // of top-p without top-k
-        const double t = __builtin_ceil(f.top_p * S * unit);
+        // (S is off by up to 1.1e-14 of itself: 5e-15 in the powers, the rest in the sums.  A border that lies closer counts as reached: of 8 equal
+        // logits top_p = 0.5 keeps 4, also where S is 8 and a few last bits)
+        const double t = __builtin_ceil(f.top_p * S * (1.0 - 1.2e-14) * unit);
         return t < 1.0 ? u64(1) : u64(int64_t(t));
     }();
     int bound = kEveryBin;
