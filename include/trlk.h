@@ -527,6 +527,23 @@ int trlk_adamw_step(const trlk_adamw_tensor* tensors, int32_t n_tensors, const t
 int trlk_adamw_state_values(const uint8_t* d_codes, const float* d_scales, int64_t n, int32_t has_sign, void* d_out_bf16,
                             trlk_stream_t stream);
 
+/* ---------------------------------------------------------------------------------------
+ * K10  rows of the embedding table times a scale, and the table's gradient (the reference leaves both to the model):
+ *   out[t, :] = scale * weight[ids[t], :], rounded once to the table's type
+ * d_ids: whole numbers of id_bits (32 or 64), n of them.  weight [vocab, cols] with row_stride entries between rows, out dense [n, cols].  An id
+ * outside the table gives a row of NaN and sets TRLK_FLAG_INDEX_OUT_OF_RANGE in *d_error_flag (may be NULL).
+ *   dweight[v, :] = scale * sum over the t with ids[t] = v of grad[t, :]
+ * in fp32, in an order that depends on nothing but the ids; rounded once.  Tokens padding_idx (-1: none) count for nothing, and ids outside the
+ * table neither (they set the flag).  accumulate 0: the whole table is written, dense; else the sums are added to what is there, and
+ * rows of ids that do not occur are not touched.  The gradients' type, or fp32, is dweight's.
+ * d_workspace: trlk_embedding_bwd_workspace_bytes(n, vocab, cols) bytes, 16-byte aligned.  n < 2^31, vocab < 2^31 - 1, cols <= 2^20. */
+int trlk_embedding_fwd(const void* d_weight, int dtype, int64_t vocab, int64_t cols, int64_t row_stride, const void* d_ids,
+                       int32_t id_bits, int64_t n, float scale, void* d_out, int32_t* d_error_flag, trlk_stream_t stream);
+size_t trlk_embedding_bwd_workspace_bytes(int64_t n, int64_t vocab, int64_t cols);
+int trlk_embedding_bwd(const void* d_grad, int dtype, int64_t n, int64_t cols, int64_t grad_stride, const void* d_ids, int32_t id_bits,
+                       int64_t vocab, float scale, int64_t padding_idx, int32_t accumulate, void* d_dweight, int out_dtype,
+                       int64_t out_stride, int32_t* d_error_flag, void* d_workspace, size_t workspace_bytes, trlk_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

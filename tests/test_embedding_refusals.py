@@ -1,0 +1,81 @@
+"""CPU-only checks of the embedding's entry points: what they refuse is refused on the host, before anything is launched."""
+import pytest
+import torch
+
+FAKE = 0x1000  # never dereferenced: every call below fails validation first
+
+
+def test_library_refuses():
+    from trl_amd import _lib
+
+    def fwd(weight=FAKE, dtype=_lib.BF16, vocab=100, cols=64, stride=64, ids=FAKE, bits=64, n=10, out=FAKE):
+        return _lib.lib.trlk_embedding_fwd(weight, dtype, vocab, cols, stride, ids, bits, n, 1.0, out, None, None)
+
+    assert fwd(dtype=9) == -3 and fwd(bits=16) == -5 and fwd(n=-1) == -2 and fwd(vocab=-1) == -2 and fwd(cols=-1) == -2
+    assert fwd(cols=(1 << 20) + 1, stride=1 << 21) == -2 and fwd(n=1 << 31) == -2 and fwd(vocab=(1 << 31) - 1) == -2
+    assert fwd(stride=63) == -4 and fwd(weight=None) == -1 and fwd(ids=None) == -1 and fwd(out=None) == -1
+    assert fwd(weight=FAKE + 1) == -4 and fwd(out=FAKE + 1) == -4 and fwd(ids=FAKE + 4) == -4
+    assert fwd(n=0, weight=None) == 0 and fwd(cols=0, stride=0) == 0 and _lib.last_error() == ""
+
+    def bwd(grad=FAKE, dtype=_lib.BF16, n=10, cols=64, stride=64, ids=FAKE, bits=64, vocab=100, add=1, dw=FAKE, out=_lib.BF16, out_stride=64,
+            ws=FAKE, ws_bytes=1 << 20):
+        return _lib.lib.trlk_embedding_bwd(grad, dtype, n, cols, stride, ids, bits, vocab, 1.0, -1, add, dw, out, out_stride, None, ws, ws_bytes, None)
+
+    assert bwd(dtype=9) == -3 and bwd(out=_lib.F16) == -3 and bwd(dtype=_lib.F32) == -3 and bwd(bits=8) == -5
+    assert bwd(n=-1) == -2 and bwd(n=1 << 31) == -2 and bwd(cols=(1 << 20) + 1, stride=1 << 21, out_stride=1 << 21) == -2
+    assert bwd(stride=63) == -4 and bwd(out_stride=63) == -4 and bwd(out_stride=72, add=0) == -4
+    assert bwd(grad=None) == -1 and bwd(ids=None) == -1 and bwd(dw=None) == -1
+    assert bwd(grad=FAKE + 1) == -4 and bwd(dw=FAKE + 1) == -4 and bwd(ids=FAKE + 4) == -4
+    need = _lib.lib.trlk_embedding_bwd_workspace_bytes(10, 100, 64)
+    assert need > 0 and bwd(ws_bytes=need - 1) == -6 and bwd(ws=None) == -6 and bwd(ws=FAKE + 8) == -6
+    assert _lib.lib.trlk_embedding_bwd_workspace_bytes(0, 100, 64) == 0 and _lib.lib.trlk_embedding_bwd_workspace_bytes(1 << 31, 100, 64) == 0
+    assert bwd(n=0, grad=None, ids=None) == 0 and bwd(vocab=0, dw=None) == 0 and _lib.last_error() == ""
+
+
+def test_host_tensors_and_bad_arguments_raise():
+    import trl_amd
+
+    ids, weight = torch.zeros((2, 3), dtype=torch.int64), torch.zeros((5, 4))
+    with pytest.raises(NotImplementedError):
+        trl_amd.embedding(ids, weight)
+    with pytest.raises(NotImplementedError):
+        trl_amd.embedding_grad_(weight, torch.zeros((2, 3, 4)), ids)
+    for bad in (5, -6):
+        with pytest.raises(ValueError, match="padding_idx"):
+            trl_amd.embedding(ids, weight, padding_idx=bad)
+
+
+class Model(torch.nn.Module):
+    def __init__(self, embed):
+        super().__init__()
+        self.embed = embed
+
+    def get_input_embeddings(self):
+        return self.embed
+
+
+class Other(torch.nn.Embedding):
+    def forward(self, input):
+        return super().forward(input) + 1
+
+
+def test_patch_embedding_refuses():
+    import trl_amd
+
+    for module in (torch.nn.Linear(3, 4), torch.nn.Embedding(5, 4, max_norm=1.0), torch.nn.Embedding(5, 4, sparse=True),
+                   torch.nn.Embedding(5, 4, scale_grad_by_freq=True), Other(5, 4)):
+        with pytest.raises(ValueError):
+            trl_amd.patch_embedding(Model(module))
+
+
+def test_shapes_for_tracers():
+    from torch._subclasses.fake_tensor import FakeTensorMode
+
+    import trl_amd
+
+    with FakeTensorMode():
+        weight = torch.empty((50, 8), dtype=torch.bfloat16, device="cuda")
+        ids = torch.empty((2, 3), dtype=torch.int64, device="cuda")
+        rows = trl_amd.embedding(ids, weight)
+        assert rows.shape == (2, 3, 8) and rows.dtype == torch.bfloat16
+        assert trl_amd.ops.embedding_bwd(rows, ids, 50, 1.0, -1).shape == (50, 8)

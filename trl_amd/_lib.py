@@ -161,6 +161,16 @@ SIGNATURES = {
         [c_void_p, c_int32, c_int64, c_int64, c_int64, c_int64, c_int64, c_void_p, c_double, c_void_p, c_void_p, c_void_p,
          c_void_p, c_void_p, c_void_p],
     ),
+    "trlk_embedding_fwd": (
+        c_int32,
+        [c_void_p, c_int32, c_int64, c_int64, c_int64, c_void_p, c_int32, c_int64, c_float, c_void_p, c_void_p, c_void_p],
+    ),
+    "trlk_embedding_bwd_workspace_bytes": (c_size_t, [c_int64, c_int64, c_int64]),
+    "trlk_embedding_bwd": (
+        c_int32,
+        [c_void_p, c_int32, c_int64, c_int64, c_int64, c_void_p, c_int32, c_int64, c_float, c_int64, c_int32, c_void_p, c_int32,
+         c_int64, c_void_p, c_void_p, c_size_t, c_void_p],
+    ),
     "trlk_rloo_loss": (
         c_int32,
         [c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_int64, c_float, c_float, c_void_p, c_void_p, c_void_p,

@@ -7,6 +7,7 @@
 // Each operator checks its shapes, allocates its outputs and hands raw device pointers, sizes, strides and the
 // current stream of the tensors' device to the library.  GPU tensors only: other devices have no kernel registered.
 #include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
+#include <ATen/MemoryOverlap.h>
 #include <ATen/ops/empty.h>
 #include <ATen/ops/empty_strided.h>
 #include <ATen/ops/zeros.h>
@@ -731,6 +732,97 @@ Tensor3 filtered_logps_fwd_autograd(const Tensor& logits, const Tensor& index, d
     return op.call(logits, index, temperature, top_k, top_p, min_p, temperatures, top_ks, top_ps, min_ps, row_mask);
 }
 
+// ---- embeddings -------------------------------------------------------------------------------------------------------
+// Ids of 32 or 64 bits, contiguous.
+Tensor token_ids(const char* op, const Tensor& ids) {
+    TORCH_CHECK_TYPE(ids.scalar_type() == at::kLong || ids.scalar_type() == at::kInt, op, ": ids are int64 or int32, not ", ids.scalar_type());
+    return ids.contiguous();
+}
+int id_bits(const Tensor& ids) { return ids.scalar_type() == at::kLong ? 64 : 32; }
+// Matrices whose rows are apart but whose entries are not.
+Tensor with_rows(const Tensor& t) { return (t.size(1) <= 1 || t.stride(1) == 1) && (t.size(0) <= 1 || t.stride(0) >= t.size(1)) ? t : t.contiguous(); }
+
+Tensor embedding_fwd(const Tensor& ids_, const Tensor& weight_, double scale) {
+    TORCH_CHECK_VALUE(weight_.dim() == 2, "embedding: the table is [tokens, width], got shape ", weight_.sizes());
+    TORCH_CHECK(ids_.device() == weight_.device(), "embedding: ids are on ", ids_.device(), ", the table on ", weight_.device());
+    const c10::DeviceGuard guard(weight_.device());
+    const Tensor ids = token_ids("embedding", ids_), weight = with_rows(weight_);
+    std::vector<int64_t> sizes = ids.sizes().vec();
+    sizes.push_back(weight.size(1));
+    const Tensor rows = at::empty(sizes, weight.options());
+    check(trlk_embedding_fwd(weight.const_data_ptr(), dtype_code(weight), weight.size(0), weight.size(1), weight.stride(0), ids.const_data_ptr(),
+                             id_bits(ids), ids.numel(), float(scale), rows.mutable_data_ptr(), error_word(weight), stream_of(weight)));
+    if (rows.numel()) check_ids();
+    return rows;
+}
+
+void embedding_into(const Tensor& into, const Tensor& grad_, const Tensor& ids_, double scale, int64_t padding_idx, bool accumulate) {
+    TORCH_CHECK_VALUE(grad_.dim() == ids_.dim() + 1 && grad_.sizes().slice(0, ids_.dim()) == ids_.sizes() && grad_.size(-1) == into.size(1),
+                      "embedding's gradient: ids of shape ", ids_.sizes(), ", gradients of shape ", grad_.sizes(), ", table of shape ", into.sizes());
+    TORCH_CHECK(grad_.device() == into.device() && ids_.device() == into.device(), "embedding's gradient: the table is on ", into.device(),
+                ", gradients on ", grad_.device(), ", ids on ", ids_.device());
+    const Tensor ids = token_ids("embedding's gradient", ids_);
+    const Tensor grad = with_rows(grad_.reshape({ids.numel(), into.size(1)}));
+    const size_t ws_bytes = trlk_embedding_bwd_workspace_bytes(ids.numel(), into.size(0), into.size(1));
+    const Tensor ws = bytes(into, ws_bytes);
+    check(trlk_embedding_bwd(grad.const_data_ptr(), dtype_code(grad), ids.numel(), into.size(1), grad.stride(0), ids.const_data_ptr(), id_bits(ids),
+                             into.size(0), float(scale), padding_idx, accumulate ? 1 : 0, into.mutable_data_ptr(), dtype_code(into), into.stride(0),
+                             error_word(into), ws.mutable_data_ptr(), ws_bytes, stream_of(into)));
+}
+
+Tensor embedding_bwd(const Tensor& grad, const Tensor& ids, int64_t vocab, double scale, int64_t padding_idx) {
+    const c10::DeviceGuard guard(grad.device());
+    TORCH_CHECK_VALUE(grad.dim() > 0, "embedding_bwd: gradients have a width");
+    const Tensor dweight = at::empty({vocab, grad.size(-1)}, grad.options());
+    embedding_into(dweight, grad, ids, scale, padding_idx, false);
+    return dweight;
+}
+
+void embedding_grad_(const Tensor& grad_weight, const Tensor& grad, const Tensor& ids, double scale, int64_t padding_idx) {
+    TORCH_CHECK_VALUE(grad_weight.dim() == 2, "embedding_grad_: the table's gradient is [tokens, width], got shape ", grad_weight.sizes());
+    TORCH_CHECK_TYPE(grad_weight.scalar_type() == grad.scalar_type() || grad_weight.scalar_type() == at::kFloat, "embedding_grad_: gradients in ",
+                     grad.scalar_type(), " add to a table's gradient of that type or fp32, not ", grad_weight.scalar_type());
+    const c10::DeviceGuard guard(grad_weight.device());
+    TORCH_CHECK_VALUE((grad_weight.size(1) <= 1 || grad_weight.stride(1) == 1) && (grad_weight.size(0) <= 1 || grad_weight.stride(0) >= grad_weight.size(1)),
+                      "embedding_grad_: the table's gradient has gaps between the entries of a row, or rows that overlap");
+    at::assert_no_partial_overlap(grad_weight, grad);
+    TORCH_CHECK_VALUE(grad.numel() == 0 || !grad_weight.is_alias_of(grad) || at::get_overlap_status(grad_weight, grad) == at::MemOverlapStatus::No,
+                      "embedding_grad_: the table's gradient shares memory with the tokens' gradients");
+    embedding_into(grad_weight, grad, ids, scale, padding_idx, true);
+    if (!grad_weight.is_inference()) grad_weight.unsafeGetTensorImpl()->bump_version();
+    if (grad.numel()) check_ids();
+}
+
+class Embedding : public torch::autograd::Function<Embedding> {
+  public:
+    static Tensor forward(AutogradContext* ctx, const Tensor& ids, const Tensor& weight, double scale, int64_t padding_idx) {
+        ctx->save_for_backward({ids});
+        ctx->saved_data["scale"] = scale;
+        ctx->saved_data["padding_idx"] = padding_idx;
+        ctx->saved_data["vocab"] = weight.sym_size(0);
+        at::AutoDispatchBelowADInplaceOrView below;
+        static const auto op = handle<Tensor(const Tensor&, const Tensor&, double, int64_t)>("trl_amd::embedding");
+        return op.call(ids, weight, scale, padding_idx);
+    }
+    static variable_list backward(AutogradContext* ctx, const variable_list& grads) {
+        variable_list result(4);
+        if (!grads[0].defined()) return result;
+        const auto saved = ctx->get_saved_variables();
+        static const auto op = handle<Tensor(const Tensor&, const Tensor&, c10::SymInt, double, int64_t)>("trl_amd::embedding_bwd");
+        result[1] = op.call(grads[0], saved[0], ctx->saved_data["vocab"].toSymInt(), ctx->saved_data["scale"].toDouble(),
+                            ctx->saved_data["padding_idx"].toInt());
+        return result;
+    }
+};
+// (padding_idx is the backward's alone)
+Tensor embedding(const Tensor& ids, const Tensor& weight, double scale, int64_t) { return embedding_fwd(ids, weight, scale); }
+Tensor embedding_autograd(const Tensor& ids, const Tensor& weight, double scale, int64_t padding_idx) {
+    if (needs_grad({&weight})) return Embedding::apply(ids, weight, scale, padding_idx);
+    at::AutoDispatchBelowADInplaceOrView below;
+    static const auto op = handle<Tensor(const Tensor&, const Tensor&, double, int64_t)>("trl_amd::embedding");
+    return op.call(ids, weight, scale, padding_idx);
+}
+
 // ---- AdamW ------------------------------------------------------------------------------------------------------------
 constexpr int64_t kStateBlock = 256;  // entries of 8-bit moments that share a scale
 
@@ -984,6 +1076,9 @@ TORCH_LIBRARY_FRAGMENT(trl_amd, m) {
           "Tensor(e!)[] exp_avg_scales, Tensor(f!)[] exp_avg_sq_scales, int[] group_of, float[] hyper, Tensor[] lrs, "
           "float max_grad_norm, int seed) -> Tensor");
     m.def("adamw_state_values(Tensor codes, Tensor scales) -> Tensor");
+    m.def("embedding(Tensor ids, Tensor weight, float scale, int padding_idx) -> Tensor");
+    m.def("embedding_bwd(Tensor grad, Tensor ids, SymInt vocab, float scale, int padding_idx) -> Tensor");
+    m.def("embedding_grad_(Tensor(a!) grad_weight, Tensor grad, Tensor ids, float scale, int padding_idx) -> ()");
 }
 TORCH_LIBRARY_IMPL(trl_amd, CUDA, m) {
     m.impl("logp_entropy_fwd", logp_entropy_fwd);
@@ -1001,6 +1096,9 @@ TORCH_LIBRARY_IMPL(trl_amd, CUDA, m) {
     m.impl("filtered_logps_bwd", filtered_logps_bwd);
     m.impl("adamw_step_", adamw_step_);
     m.impl("adamw_state_values", adamw_state_values);
+    m.impl("embedding", embedding);
+    m.impl("embedding_bwd", embedding_bwd);
+    m.impl("embedding_grad_", embedding_grad_);
 }
 TORCH_LIBRARY_IMPL(trl_amd, Autograd, m) {
     m.impl("logp_entropy_fwd", logp_entropy_fwd_autograd);
@@ -1008,8 +1106,10 @@ TORCH_LIBRARY_IMPL(trl_amd, Autograd, m) {
     m.impl("grpo_loss", grpo_loss_autograd);
     m.impl("dpo_loss", dpo_loss_autograd);
     m.impl("filtered_logps_fwd", filtered_logps_fwd_autograd);
-    for (const char* name : {"logp_entropy_bwd", "grpo_row_scale", "dpo_log_values", "filtered_logps_bwd"})
+    m.impl("embedding", embedding_autograd);
+    for (const char* name : {"logp_entropy_bwd", "grpo_row_scale", "dpo_log_values", "filtered_logps_bwd", "embedding_bwd"})
         m.impl(name, torch::autograd::autogradNotImplementedFallback());
     // (these hand out a gradient, scale one in place, draw or step: their results belong to no graph, whatever the operands require)
-    for (const char* name : {"grpo_fused", "scale_unless_one_", "sample_tokens", "adamw_step_", "adamw_state_values"}) m.impl(name, torch::CppFunction::makeFallthrough());
+    for (const char* name : {"grpo_fused", "scale_unless_one_", "sample_tokens", "adamw_step_", "adamw_state_values", "embedding_grad_"})
+        m.impl(name, torch::CppFunction::makeFallthrough());
 }

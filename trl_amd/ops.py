@@ -312,6 +312,22 @@ adamw_state_values = _native_op(
 
 
 # --------------------------------------------------------------------------------------------
+# embeddings (K10)
+# --------------------------------------------------------------------------------------------
+# ids int64 or int32 [...], weight [V, H]; padding_idx (-1: none) is the backward's alone.  The rows times `scale`, [..., H].
+embedding = _native_op(
+    "embedding", lambda ids, weight, scale, padding_idx: torch.empty((*ids.shape, weight.shape[1]), dtype=weight.dtype, device=weight.device))
+
+# The table's whole gradient, in the type of `grad` ([..., H]).
+embedding_bwd = _native_op(
+    "embedding_bwd", lambda grad, ids, vocab, scale, padding_idx:
+    torch.empty((vocab, grad.shape[-1]), dtype=grad.dtype, device=grad.device))
+
+# The same, added to what is there: rows of tokens that do not occur are not touched.
+embedding_grad_ = _native_op("embedding_grad_", lambda grad_weight, grad, ids, scale, padding_idx: None)
+
+
+# --------------------------------------------------------------------------------------------
 # group advantages (K2a)
 # --------------------------------------------------------------------------------------------
 _SCALE_MODES = {"group": _lib.SCALE_GROUP, "batch": _lib.SCALE_BATCH, "none": _lib.SCALE_NONE}

@@ -1,0 +1,67 @@
+"""The other end of the table that the fused head reads: the embedding of the tokens, times a scale, and its gradient from sorted tokens."""
+from __future__ import annotations
+
+import types
+
+import torch
+from torch import Tensor
+
+from .. import ops
+
+__all__ = ["embedding", "embedding_grad_", "patch_embedding"]
+
+
+def _padding(padding_idx: int | None, vocab: int) -> int:
+    """As `torch.nn.functional.embedding` takes it: negative ones count from the end.  -1: none."""
+    if padding_idx is None:
+        return -1
+    if not -vocab <= padding_idx < vocab:
+        raise ValueError(f"padding_idx {padding_idx} is outside a table of {vocab} tokens")
+    return padding_idx % vocab
+
+
+def embedding(input_ids: Tensor, weight: Tensor, *, scale: float = 1.0, padding_idx: int | None = None) -> Tensor:
+    """`scale * weight[input_ids]`, rounded once: `[..., H]` in the type of `weight` (`[V, H]`, fp32, bf16 or fp16, rows at any
+    stride) for int64 or int32 ids `[...]`.  Differentiable w.r.t. `weight`: the gradient, dense, sums a token's rows in fp32 in
+    an order that depends on the ids alone (the same call gives the same bits) and is rounded once; tokens `padding_idx` have none.
+
+    Ids outside [0, V) give NaN, have no gradient and are reported by `check_device_errors()`."""
+    return ops.embedding(input_ids, weight, float(scale), _padding(padding_idx, weight.shape[0]))
+
+
+def embedding_grad_(grad_weight: Tensor, grad_output: Tensor, input_ids: Tensor, *, scale: float = 1.0,
+                    padding_idx: int | None = None) -> Tensor:
+    """Adds the gradient that `embedding` has with the upstream gradient `grad_output` (`[..., H]`) to `grad_weight` (`[V, H]`, of that
+    type or fp32, rows at any stride) in place, and returns it.  Only the rows of tokens that occur are read and written, each
+    entry rounded once: for gradients that are kept by the caller, of a tied head's table or over several micro-batches, where
+    a dense gradient would be written, read and added for all V tokens."""
+    ops.embedding_grad_(grad_weight, grad_output, input_ids, float(scale), _padding(padding_idx, grad_weight.shape[0]))
+    return grad_weight
+
+
+def _scale_of(module: torch.nn.Embedding) -> float:
+    """The factor that the module's forward multiplies its rows by."""
+    if type(module).forward is torch.nn.Embedding.forward:
+        return 1.0
+    if not type(module).__name__.endswith("ScaledWordEmbedding") or not hasattr(module, "embed_scale"):
+        raise ValueError(f"{type(module).__name__} is not a lookup, or a scaled one, that patch_embedding knows")
+    scale = module.embed_scale
+    # (as a tensor it is rounded to the table's type before it is multiplied with, as a number it is not)
+    return float(scale.to(module.weight.dtype)) if isinstance(scale, Tensor) else float(scale)
+
+
+def patch_embedding(model: torch.nn.Module) -> None:
+    """Replaces the forward of `model.get_input_embeddings()` by `embedding`, with the module's own scale and padding index.  Takes
+    `torch.nn.Embedding` and the scaled embeddings of transformers' models; others, and embeddings with `max_norm`, `sparse` or
+    `scale_grad_by_freq`, raise ValueError."""
+    module = model.get_input_embeddings()
+    if not isinstance(module, torch.nn.Embedding):
+        raise ValueError(f"the model's input embeddings are a {type(module).__name__}, not a torch.nn.Embedding")
+    if module.max_norm is not None or module.sparse or module.scale_grad_by_freq:
+        raise ValueError("patch_embedding takes no max_norm, sparse or scale_grad_by_freq")
+    scale = _scale_of(module)
+
+    def forward(self, input: Tensor) -> Tensor:
+        return embedding(input, self.weight, scale=scale, padding_idx=self.padding_idx)
+
+    module.forward = types.MethodType(forward, module)
