@@ -544,6 +544,40 @@ int trlk_embedding_bwd(const void* d_grad, int dtype, int64_t n, int64_t cols, i
                        int64_t vocab, float scale, int64_t padding_idx, int32_t accumulate, void* d_dweight, int out_dtype,
                        int64_t out_stride, int32_t* d_error_flag, void* d_workspace, size_t workspace_bytes, trlk_stream_t stream);
 
+/* ---------------------------------------------------------------------------------------
+ * K11  Newton-Schulz orthogonalisation of many matrices, and the optimiser's step around it:
+ *   m = momentum m + (1 - momentum) g;  u = m, or with nesterov momentum m + (1 - momentum) g
+ *   X = u / max(|u|, eps) (Frobenius norm; transposed if u has more rows than columns)
+ *   `steps` times:  A = X X^T;  X = a X + (b A + c A A) X
+ *   p = p (1 - lr weight_decay) - lr stretch X;   stretch = sqrt(max(1, rows / cols)), or 0.2 sqrt(max(rows, cols)) (MATCH_ADAMW)
+ * Elementwise arithmetic and sums are fp32 (norms in 64 bits), p is rounded once to its type.  Matrices of 16 bits: the products' operands are
+ * rounded to 11 bits, the result is off by 2e-3 of its norm at most; of fp32: 22 bits, 1e-6 or so times how much the iteration stretches small
+ * singular values.  The tables are HOST memory, read before the call returns.  d_param, d_grad and d_momentum (fp32) are dense [rows, cols];
+ * what is written shares no memory with anything else that is listed.  trlk_orthogonalize: d_param takes X, turned back, of d_grad (they may be
+ * the same), d_momentum is NULL.  The smaller side is 32768 at most, the larger one 2^22, both 2^34 entries.  A matrix with a NaN or an infinity comes out as NaN.
+ * Coefficients with which singular values of at most 1 grow past 2.5 on the way are refused.  eps in (0, 1].
+ * d_workspace: trlk_muon_workspace_bytes(...) bytes, 256-byte aligned. */
+enum trlk_muon_adjust { TRLK_MUON_ORIGINAL = 0, TRLK_MUON_MATCH_ADAMW = 1 };
+typedef struct {
+    void* d_param;
+    const void* d_grad;
+    float* d_momentum;
+    int64_t rows, cols;
+    int32_t dtype; /* trlk_dtype of param and grad */
+    int32_t group;
+} trlk_muon_matrix;
+typedef struct {
+    double lr, momentum, weight_decay;
+    const float* d_lr; /* fp32, device; read in place of lr if not NULL */
+    int32_t nesterov;
+    int32_t adjust; /* trlk_muon_adjust */
+} trlk_muon_group;
+size_t trlk_muon_workspace_bytes(const trlk_muon_matrix* matrices, int32_t n_matrices);
+int trlk_orthogonalize(const trlk_muon_matrix* matrices, int32_t n_matrices, int32_t steps, double a, double b, double c, double eps,
+                       void* d_workspace, size_t workspace_bytes, trlk_stream_t stream);
+int trlk_muon_step(const trlk_muon_matrix* matrices, int32_t n_matrices, const trlk_muon_group* groups, int32_t n_groups, int32_t steps,
+                   double a, double b, double c, double eps, void* d_workspace, size_t workspace_bytes, trlk_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,166 @@
+"""CPU-only checks of the orthogonalised updates' entry points: what they refuse is refused on the host, before anything is launched."""
+import copy
+import ctypes
+import math
+
+import pytest
+import torch
+
+FAKE = 0x1000  # never dereferenced: every call below fails validation first
+
+
+class Matrix(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_void_p) for n in ("param", "grad", "momentum")] + [
+        ("rows", ctypes.c_int64), ("cols", ctypes.c_int64), ("dtype", ctypes.c_int32), ("group", ctypes.c_int32)]
+
+
+class Group(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_double) for n in ("lr", "momentum", "weight_decay")] + [
+        ("d_lr", ctypes.c_void_p), ("nesterov", ctypes.c_int32), ("adjust", ctypes.c_int32)]
+
+
+def test_library_refuses():
+    from trl_amd import _lib
+
+    lib = _lib.lib
+
+    def table(**changed):
+        x = dict(param=FAKE, grad=FAKE, momentum=FAKE, rows=70, cols=130, dtype=_lib.BF16, group=0, **{})
+        return (Matrix * 1)(Matrix(**{**x, **changed}))
+
+    def step(x=None, n=1, groups=1, lr=0.1, momentum=0.9, decay=0.1, d_lr=None, adjust=0, steps=5, c=(3.4445, -4.775, 2.0315), eps=1e-7, ws=FAKE,
+             ws_bytes=1 << 30):
+        g = (Group * 1)(Group(lr, momentum, decay, d_lr, 1, adjust))
+        return lib.trlk_muon_step(x if x is not None else table(), n, g, groups, steps, *c, eps, ws, ws_bytes, None)
+
+    assert step(n=-1) == -1 and lib.trlk_muon_step(None, 1, None, 0, 5, 1.0, 0.0, 0.0, 1e-7, FAKE, 1 << 30, None) == -1
+    for bad in (-0.1, 1.0, math.nan):
+        assert step(momentum=bad) == -5 and "momentum" in _lib.last_error()
+    assert step(lr=-1.0) == -5 and step(lr=math.nan) == -5 and step(decay=-1.0) == -5 and step(adjust=2) == -5
+    assert step(table(group=1)) == -5 and step(table(group=-1)) == -5 and step(table(dtype=7)) == -3
+    assert step(table(rows=-1)) == -2 and step(table(rows=32769, cols=32769)) == -2 and step(table(cols=(1 << 22) + 1)) == -2
+    assert step(table(rows=32768, cols=1 << 20)) == -2
+    for name in ("param", "grad", "momentum"):
+        assert step(table(**{name: None})) == -1 and step(table(**{name: FAKE + 1})) == -4
+    for bad in (0, -1, 101):
+        assert step(steps=bad) == -5
+    for bad in (0.0, -1.0, 2.0, math.nan):
+        assert step(eps=bad) == -5
+    for bad in ((math.inf, 0.0, 0.0), (9.0, 0.0, 0.0), (3.4445, 4.775, 2.0315), (1.0, 0.0, -8.0)):
+        assert step(c=bad) == -5, bad
+    need = lib.trlk_muon_workspace_bytes(table(), 1)
+    assert need > 0 and step(ws_bytes=need - 1) == -6 and step(ws=None) == -6 and step(ws=FAKE + 16) == -6
+    assert lib.trlk_muon_workspace_bytes(None, 1) == 0 and lib.trlk_muon_workspace_bytes(table(rows=-1), 1) == 0
+    assert lib.trlk_muon_workspace_bytes(table(rows=0), 1) == 0
+    assert step(table(rows=0, param=None, grad=None, momentum=None), ws=None, ws_bytes=0) == 0 and step(n=0, ws=None, ws_bytes=0) == 0
+    assert lib.trlk_orthogonalize(table(), 1, 5, 3.4445, -4.775, 2.0315, 1e-7, FAKE, 1 << 30, None) == -5  # a momentum
+    assert lib.trlk_orthogonalize(table(momentum=None), 1, 5, 3.4445, -4.775, 2.0315, 1e-7, FAKE, need - 1, None) == -6
+
+
+def test_host_tensors_raise():
+    import trl_amd
+
+    x = [torch.zeros((4, 5))]
+    with pytest.raises(NotImplementedError):
+        trl_amd.muon_step_(x, x, x)
+    with pytest.raises(NotImplementedError):
+        trl_amd.orthogonalize(x[0])
+    p = torch.nn.Parameter(torch.zeros((4, 5)))
+    p.grad = torch.zeros((4, 5))
+    with pytest.raises(RuntimeError, match="GPU"):
+        trl_amd.Muon([p]).step()
+
+
+def params():
+    return [torch.nn.Parameter(torch.zeros(s)) for s in ((4, 5), (6, 3), (5,))]
+
+
+def test_settings():
+    import trl_amd
+
+    p = params()
+    for bad in (dict(lr=-1.0), dict(weight_decay=-1.0), dict(momentum=1.0), dict(momentum=-0.1), dict(eps=0.0), dict(ns_steps=0), dict(ns_steps=101),
+                dict(ns_coefficients=(1.0,)), dict(adjust_lr_fn="x")):
+        with pytest.raises(ValueError):
+            trl_amd.Muon(p[:2], **bad)
+        with pytest.raises(ValueError):
+            trl_amd.Muon([dict(params=p[:2], **bad)])
+    with pytest.raises(ValueError, match="adamw"):
+        trl_amd.Muon(p)
+    for bad in (dict(betas=(1.0, 0.9)), dict(adamw_eps=-1.0)):
+        with pytest.raises(ValueError):
+            trl_amd.Muon([dict(params=p, adamw=True, **bad)])
+    opt = trl_amd.Muon(p[:2])
+    with pytest.raises(ValueError):
+        opt.add_param_group(dict(params=p[2:]))
+    assert len(opt.param_groups) == 1
+    opt.add_param_group(dict(params=p[2:], adamw=True))
+    again = copy.deepcopy(opt)
+    assert again.param_groups[1]["adamw"] and again.param_groups[0]["momentum"] == 0.95
+
+
+def test_foreign_states_are_refused():
+    import trl_amd
+
+    def optimizer(adamw):
+        p = params()
+        return trl_amd.Muon([dict(params=p[:2]), dict(params=p[2:], adamw=adamw)] if adamw else p[:2])
+
+    whole = optimizer(True)
+    state = whole.state_dict()
+    theirs = torch.optim.AdamW(params()[:2])
+    for q in theirs.param_groups[0]["params"]:
+        q.grad = torch.ones_like(q)
+    theirs.step()
+    with pytest.raises(ValueError, match="momentum_buffer"):
+        optimizer(False).load_state_dict(theirs.state_dict())
+    changed = copy.deepcopy(state)
+    changed["param_groups"][1]["adamw"] = False
+    with pytest.raises(ValueError, match="AdamW"):
+        whole.load_state_dict(changed)
+    muon = torch.optim.Muon(params()[:2])
+    for q in muon.param_groups[0]["params"]:
+        q.grad = torch.ones_like(q)
+    muon.step()
+    wrong = copy.deepcopy(muon.state_dict())
+    wrong["state"][0]["momentum_buffer"] = torch.zeros((5, 4))
+    with pytest.raises(ValueError, match="momentum_buffer"):
+        optimizer(False).load_state_dict(wrong)
+    mine = optimizer(False)
+    mine.load_state_dict(muon.state_dict())
+    q = mine.param_groups[0]["params"][0]
+    assert mine.state[q]["momentum_buffer"].dtype == torch.float32 and mine.param_groups[0]["adamw"] is False
+
+
+class Small(torch.nn.Module):
+    def __init__(self, tied):
+        super().__init__()
+        self.embed = torch.nn.Embedding(11, 6)
+        self.a, self.norm, self.lm_head = torch.nn.Linear(6, 6), torch.nn.LayerNorm(6), torch.nn.Linear(6, 11, bias=False)
+        self.frozen = torch.nn.Linear(6, 6).requires_grad_(False)
+        if tied:
+            self.lm_head.weight = self.embed.weight
+
+    def get_output_embeddings(self):
+        return self.lm_head
+
+
+def test_param_groups():
+    import trl_amd
+
+    for tied in (False, True):
+        model = Small(tied)
+        matrices, rest = trl_amd.muon_param_groups(model)
+        assert [id(p) for p in matrices["params"]] == [id(model.a.weight)] and rest["adamw"]
+        assert {id(p) for p in rest["params"]} == {id(p) for p in (model.embed.weight, model.a.bias, model.norm.weight, model.norm.bias, model.lm_head.weight)}
+        trl_amd.Muon([matrices, rest], adjust_lr_fn="match_rms_adamw")
+
+
+def test_shapes_for_tracers():
+    from torch._subclasses.fake_tensor import FakeTensorMode
+
+    import trl_amd
+
+    with FakeTensorMode():
+        x = torch.empty((3, 50, 8), dtype=torch.bfloat16, device="cuda")
+        assert trl_amd.orthogonalize(x).shape == x.shape and trl_amd.orthogonalize([x, x[0]])[1].shape == (50, 8)

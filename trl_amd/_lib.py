@@ -171,6 +171,12 @@ SIGNATURES = {
         [c_void_p, c_int32, c_int64, c_int64, c_int64, c_void_p, c_int32, c_int64, c_float, c_int64, c_int32, c_void_p, c_int32,
          c_int64, c_void_p, c_void_p, c_size_t, c_void_p],
     ),
+    "trlk_muon_workspace_bytes": (c_size_t, [c_void_p, c_int32]),
+    "trlk_orthogonalize": (c_int32, [c_void_p, c_int32, c_int32, c_double, c_double, c_double, c_double, c_void_p, c_size_t, c_void_p]),
+    "trlk_muon_step": (
+        c_int32,
+        [c_void_p, c_int32, c_void_p, c_int32, c_int32, c_double, c_double, c_double, c_double, c_void_p, c_size_t, c_void_p],
+    ),
     "trlk_rloo_loss": (
         c_int32,
         [c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_int64, c_float, c_float, c_void_p, c_void_p, c_void_p,

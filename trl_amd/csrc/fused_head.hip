@@ -1008,7 +1008,7 @@ __device__ __forceinline__ void gemm_nt_body(const GemmArgs& a, int block, char*
         typedef LeftKm<kConvert> Left;
         Left left(B, c0, b_krows, scale, smem);
         if (idle)
-            move_tiles_only<true, false, Left&>(DirectLoader<true, false>(B, c0, A, r0, smem), K, false, left);
+            move_tiles_only<true, false, OneRun, Left&>(DirectLoader<true, false>(B, c0, A, r0, smem), K, false, left);
         else
             gemm_tile_nt<DT, true>(B, c0, A, r0, K, acc, smem, left);
         if (kConvert && __any(left.top > kF16Max) && lane == 0)

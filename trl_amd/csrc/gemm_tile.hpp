@@ -89,6 +89,22 @@ struct Operand {
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
 
+// The contraction's k as it lies in the operands: one run (the k of the loop is the operands' own), or, for operands that are each the sum
+// of two pieces, x = hi + lo, one plane behind the other, three runs of `k` (a multiple of the k step): lo * hi, hi * lo and hi * hi.
+// lo * lo is below the rounding of fp32 where a piece has 11 bits.  Bytes to add for the planes, and the k inside of them.
+struct OneRun {
+    __device__ __forceinline__ int64_t left_plane(int) const { return 0; }
+    __device__ __forceinline__ int64_t right_plane(int) const { return 0; }
+    __device__ __forceinline__ int inside(int k0) const { return k0; }
+};
+struct PieceRuns {
+    int k;
+    int64_t left_lo, right_lo;  // bytes from the hi plane to the lo plane
+    __device__ __forceinline__ int64_t left_plane(int k0) const { return k0 < k ? left_lo : 0; }
+    __device__ __forceinline__ int64_t right_plane(int k0) const { return k0 >= k && k0 < 2 * k ? right_lo : 0; }
+    __device__ __forceinline__ int inside(int k0) const { return k0 < k ? k0 : k0 < 2 * k ? k0 - k : k0 - 2 * k; }
+};
+
 // Direct-to-LDS variant of the tile loop (K % BK == 0): `global_load_lds_dwordx4` moves 16 bytes per
 // lane from memory straight into LDS, 1 KiB contiguous per wave instruction = 8 tile rows of 64 k, with no register
 // staging and no ds_write.  Rows are dense (no padding is possible inside a wave's 1 KiB), so bank conflicts are avoided
@@ -108,7 +124,7 @@ __device__ __forceinline__ int tile_swizzle(int r) { return (r & 7) ^ ((r >> 3) 
 // k rows; the 16-byte unit at physical position pu of k row r holds logical unit pu ^ ((r & 3) << 1) ^ (r & 8), which
 // spreads the eight k rows that two neighbouring groups of 16 lanes read with a transpose load over all banks.
 // LEFT: the left operand travels this way too (otherwise LeftKm moves it).
-template <bool BKM = false, bool LEFT = true>
+template <bool BKM = false, bool LEFT = true, typename Runs = OneRun>
 struct DirectLoader {
     static constexpr int kWaves = kHeadThreads / 64, kRowsPerBlk = 1024 / kRowBytes;
     static constexpr int kBlkA = LEFT ? BM / kRowsPerBlk / kWaves : 0, kBlkB = BN / kRowsPerBlk / kWaves;  // per wave and stage
@@ -119,8 +135,9 @@ struct DirectLoader {
     int wave;
     int64_t bkstep;  // bytes between two k of the right operand
     uint32_t ao[LEFT ? kBlkA : 1], bo[kBlkB];
+    Runs runs;
 
-    __device__ __forceinline__ DirectLoader(const Operand A, int m0, const Operand B, int n0, char* lds) : smem(lds) {
+    __device__ __forceinline__ DirectLoader(const Operand A, int m0, const Operand B, int n0, char* lds, Runs runs_ = {}) : smem(lds), runs(runs_) {
         const int lane = fresh(threadIdx.x & 63);
         wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);  // uniform: LDS targets stay scalar
         const int rr = lane / kCpr, pc = lane % kCpr;  // row inside a block, chunk position
@@ -170,9 +187,9 @@ struct DirectLoader {
     // transfer j of a stage (A blocks first, then B blocks)
     __device__ __forceinline__ void issue_one(int buf, int k0, int j) const {
         if (j < kBlkA)
-            transfer(abase + int64_t(k0) * 2, ao[j], lds_base(buf) + (wave + kWaves * j) * 1024);
+            transfer(abase + runs.left_plane(k0) + int64_t(runs.inside(k0)) * 2, ao[j], lds_base(buf) + (wave + kWaves * j) * 1024);
         else
-            transfer(bbase + int64_t(k0) * bkstep, bo[j - kBlkA], lds_base(buf) + kDenseA + (wave + kWaves * (j - kBlkA)) * 1024);
+            transfer(bbase + runs.right_plane(k0) + int64_t(runs.inside(k0)) * bkstep, bo[j - kBlkA], lds_base(buf) + kDenseA + (wave + kWaves * (j - kBlkA)) * 1024);
     }
     __device__ __forceinline__ void issue(int buf, int k0) const {
 #pragma unroll
@@ -200,7 +217,7 @@ struct DirectLoader {
 // The conversion is what this costs beside the plain loop: 1392 tokens, H = 2048, V = 128256, backward of a bf16 problem 1562 us,
 // of an fp16 problem (nothing to convert) 1555; behind every MFMA of the refill instead of behind two of three 1577.
 // An entry whose scaled value fp16 does not hold counts as fp16's largest (see direct_scale).
-template <bool CONVERT>
+template <bool CONVERT, typename Runs = OneRun>
 struct LeftKm {
     static constexpr int kVecs = 4;
     const char* base;
@@ -208,8 +225,9 @@ struct LeftKm {
     uint32_t row_bytes, col;  // (a tile spans less than 4 GiB)
     int row0, krows;
     float scale, top;  // top: the largest magnitude converted so far, times the scale
-    __device__ __forceinline__ LeftKm(const Operand A, int m0, int krows_, float scale_, char* smem)
-        : krows(krows_), scale(scale_), top(0.f) {
+    Runs runs;
+    __device__ __forceinline__ LeftKm(const Operand A, int m0, int krows_, float scale_, char* smem, Runs runs_ = {})
+        : krows(krows_), scale(scale_), top(0.f), runs(runs_) {
         // FP16_OVFL: what overflows fp16 becomes its largest value (infinities stay), for the rest of the wave's life.  A bit of
         // the mode register, where a clamp would be two instructions more per pair of columns in the tile loop.
         if constexpr (CONVERT) asm volatile("s_setreg_imm32_b32 hwreg(HW_REG_MODE, 23, 1), 1" ::: "memory");
@@ -222,8 +240,8 @@ struct LeftKm {
         lds = smem + wave * 1024 + lane * 16;
     }
     __device__ __forceinline__ void load(int k0, int j, u32x4& w) const {
-        const int row = min(row0 + 16 * j, krows - 1 - k0);
-        w = *reinterpret_cast<const u32x4*>(base + int64_t(k0) * row_bytes + (uint32_t(row) * row_bytes + col));
+        const int row = min(row0 + 16 * j, krows - 1 - runs.inside(k0));
+        w = *reinterpret_cast<const u32x4*>(base + runs.left_plane(k0) + int64_t(runs.inside(k0)) * row_bytes + (uint32_t(row) * row_bytes + col));
     }
     // two neighbouring columns; exact wherever fp16 holds the scaled value (below its range one rounding to nearest)
     __device__ __forceinline__ void convert(uint32_t& w) {
@@ -263,8 +281,8 @@ struct NoLeftKm {};
 
 // What a wave whose rows or columns all lie beyond the operands does in place of the tile loop: it moves its share of the
 // tiles (exactly the transfers, waits and barriers of the loop) and spends nothing on matrix work.
-template <bool BKM, bool LEFT, typename Left = NoLeftKm>
-__device__ __forceinline__ void move_tiles_only(const DirectLoader<BKM, LEFT>& loader, int K, bool prefetched, Left left = {}) {
+template <bool BKM, bool LEFT, typename Runs, typename Left = NoLeftKm>
+__device__ __forceinline__ void move_tiles_only(const DirectLoader<BKM, LEFT, Runs>& loader, int K, bool prefetched, Left left = {}) {
     const int nk = K / BK;
     u32x4 w[4];
     if (!prefetched) loader.prologue(K);
@@ -301,12 +319,12 @@ __device__ __forceinline__ void move_tiles_only(const DirectLoader<BKM, LEFT>& l
 }
 
 // `left`: a LeftKm, where the left operand is k-major.
-template <int DT, bool BKM = false, typename Left = NoLeftKm>
+template <int DT, bool BKM = false, typename Left = NoLeftKm, typename Runs = OneRun>
 __device__ __forceinline__ void gemm_tile_nt_direct(const Operand A, int m0, const Operand B, int n0, int K,
-                                                    f32x4 (&acc)[MI][NI], char* smem, Left&& left = {}) {
+                                                    f32x4 (&acc)[MI][NI], char* smem, Left&& left = {}, Runs runs = {}) {
     constexpr bool AKM = !std::is_same_v<std::decay_t<Left>, NoLeftKm>;
-    const DirectLoader<BKM, !AKM> loader(A, m0, B, n0, smem);
-    constexpr int kStageLoads = DirectLoader<BKM, !AKM>::kStageLoads;
+    const DirectLoader<BKM, !AKM, Runs> loader(A, m0, B, n0, smem, runs);
+    constexpr int kStageLoads = DirectLoader<BKM, !AKM, Runs>::kStageLoads;
     const int lane = threadIdx.x & 63, wave = loader.wave;
     const int wm = wave_m(wave), wn = wave_n(wave);
 

@@ -1,0 +1,689 @@
+// K11: updates brought near the nearest matrix with orthonormal rows (or columns) by Newton-Schulz products, for many matrices in one
+// call, alone or inside of an optimiser's step.
+//
+//   u = m' = momentum m + (1 - momentum) g,   with nesterov  u = momentum m' + (1 - momentum) g
+//   X = u / max(|u|, eps)   (Frobenius norm; X is u or its transpose, m x n with m <= n)
+//   `steps` times:  A = X X^T,  B = b A + c A A,  X = a X + B X
+//   p = p (1 - lr decay) - lr stretch X
+//
+// Bound by the matrix cores: m^2 n + m^3 + 2 m^2 n operations a step (X X^T and A A are symmetric, half of their tiles are computed and
+// written twice).  The products run on fp16 operands with fp32 sums.  X is held as two fp16 pieces, x = hi + lo, 22 bits, in units of 2^-14 (its
+// singular values stay under 1.3, so do its entries; the units keep what is 2^-28 of the largest out of fp16's subnormals), A and B in
+// units of 2^-13.  Parameters in 16 bits: the products take X's hi piece and A and B of one piece, and the term a X, which carries the small
+// singular values (they grow by a in each step), all 22 bits.  Against the exact iteration that is off by 1.7e-3 of the result for
+// matrices of independent entries and less where singular values differ by much; with one piece everywhere those cases lose up to 4e-2,
+// with bf16 operands 30 times the fp16 error.  Parameters in fp32: A and B have two pieces, too, and every product is three, lo hi + hi lo +
+// hi hi, which is fp32's precision at a third of the rate.
+#include <math.h>
+
+#include <algorithm>
+#include <exception>
+#include <mutex>
+#include <vector>
+
+#include "common.hpp"
+#include "gemm_tile.hpp"
+
+namespace trlk {
+namespace {
+
+typedef u32x4 u32x4_u __attribute__((aligned(2)));  // vectors at any element alignment
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+typedef u32x2 u32x2_u __attribute__((aligned(2)));
+
+constexpr int kThreads = 256;
+constexpr int kChunk = 8192;       // entries of a workgroup of the momentum's pass
+constexpr int kTurn = 64;          // rows and columns of a tile of the pass that makes X
+constexpr int kLdsBytes = 2 * kDenseStage;
+constexpr float kUnitX = 16384.f, kUnitA = 8192.f;  // X and A, B are held times these
+constexpr int64_t kMostRows = 32768, kMostCols = int64_t(1) << 22, kMostEntries = int64_t(1) << 34;
+constexpr size_t kGroupBytes = size_t(1) << 31;  // of workspace, unless one matrix needs more
+
+// One matrix of a launch: X is m x n, m <= n, rows of npad entries, mpad of them (multiples of the k step; what lies between is zero).
+struct Mat {
+    uint16_t* x;     // [2 buffers][hi, lo][mpad][npad], then A and B, [pieces][mpad][mpad] each
+    void* p;         // parameter, or the output
+    const void* g;   // gradient, or the input
+    float* momentum;  // null: no step, the output is X
+    const float* d_lr;
+    int32_t m, n, mpad, npad;
+    float lr, stretch, weight_decay, beta, rest;  // rest: 1 - beta
+    int32_t nesterov, tall, pieces;               // tall: p is n x m
+    uint32_t first_chunk, first_turn, first_half, first_tile;  // workgroups of the four kinds of launches
+    __device__ __forceinline__ int64_t plane() const { return int64_t(mpad) * npad; }
+    __device__ __forceinline__ int64_t square() const { return int64_t(mpad) * mpad; }
+    __device__ __forceinline__ uint16_t* buffer(int i) const { return x + 2 * i * plane(); }
+    __device__ __forceinline__ uint16_t* a() const { return x + 4 * plane(); }
+    __device__ __forceinline__ uint16_t* b() const { return x + 4 * plane() + pieces * square(); }
+};
+
+constexpr int kTable = 34;
+struct MatTable {
+    Mat e[kTable];
+    Mat* to;
+    int32_t n;
+};
+static_assert(sizeof(MatTable) <= 4096, "a launch's arguments");
+
+__global__ __launch_bounds__(64) void table_kernel(MatTable t) {
+    for (int i = threadIdx.x; i < t.n; i += 64) t.to[i] = t.e[i];
+}
+
+// the matrix of workgroup w
+template <uint32_t Mat::*FIRST>
+__device__ __forceinline__ int mat_of(const Mat* e, int n, uint32_t w) {
+    int lo = 0, hi = n;
+    while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (e[mid].*FIRST <= w) lo = mid;
+        else hi = mid;
+    }
+    return lo;
+}
+
+// ---- momentum, norms, X ------------------------------------------------------------------------------------------------
+__device__ __forceinline__ float moved(float was, float g, const Mat& e) { return fmaf(e.beta, was, e.rest * g); }
+__device__ __forceinline__ float update_of(float now, float g, const Mat& e) { return e.nesterov ? fmaf(e.beta, now, e.rest * g) : now; }
+
+__device__ __forceinline__ void load8f(const float* p, float (&x)[8]) {
+    Elem<TRLK_F32>::unpack(*reinterpret_cast<const u32x4_u*>(p), x);
+    Elem<TRLK_F32>::unpack(*reinterpret_cast<const u32x4_u*>(p + 4), x + 4);
+}
+template <int DT>
+__device__ __forceinline__ void load8(const typename Elem<DT>::type* p, float (&x)[8]) {
+#pragma unroll
+    for (int k = 0; k < 8; k += Elem<DT>::EPV) Elem<DT>::unpack(*reinterpret_cast<const u32x4_u*>(p + k), x + k);
+}
+
+// The momentum moves on; partial sums of u's squares, in 64 bits.
+template <int DT>
+__global__ __launch_bounds__(kThreads) void momentum_kernel(const Mat* mats, int n_mats, double* partial) {
+    __shared__ double scratch[kThreads / kWave];
+    const Mat e = mats[mat_of<&Mat::first_chunk>(mats, n_mats, blockIdx.x)];
+    const int64_t numel = int64_t(e.m) * e.n, begin = int64_t(blockIdx.x - e.first_chunk) * kChunk;
+    const auto* g = static_cast<const typename Elem<DT>::type*>(e.g);
+    double s = 0.0;
+    for (int64_t at = begin + threadIdx.x * 8; at < begin + kChunk && at < numel; at += kThreads * 8) {
+        float x[8], w[8];
+        if (at + 8 <= numel) {
+            load8<DT>(g + at, x);
+            if (e.momentum) {
+                load8f(e.momentum + at, w);
+#pragma unroll
+                for (int k = 0; k < 8; ++k) {
+                    w[k] = moved(w[k], x[k], e);
+                    x[k] = update_of(w[k], x[k], e);
+                }
+                *reinterpret_cast<u32x4_u*>(e.momentum + at) = Elem<TRLK_F32>::pack(w);
+                *reinterpret_cast<u32x4_u*>(e.momentum + at + 4) = Elem<TRLK_F32>::pack(w + 4);
+            }
+#pragma unroll
+            for (int k = 0; k < 8; ++k) s = __builtin_fma(double(x[k]), double(x[k]), s);
+        } else {
+            for (int64_t k = at; k < numel; ++k) {
+                float u = Elem<DT>::load1(g + k);
+                if (e.momentum) {
+                    const float now = moved(e.momentum[k], u, e);
+                    e.momentum[k] = now;
+                    u = update_of(now, u, e);
+                }
+                s = __builtin_fma(double(u), double(u), s);
+            }
+        }
+    }
+#pragma unroll
+    for (int o = kWave / 2; o > 0; o >>= 1) s += __shfl_xor(s, o);
+    if ((threadIdx.x & (kWave - 1)) == 0) scratch[threadIdx.x / kWave] = s;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        double r = 0.0;
+#pragma unroll
+        for (int w = 0; w < kThreads / kWave; ++w) r += scratch[w];
+        partial[blockIdx.x] = r;
+    }
+}
+
+// kUnitX / max(|u|, eps) of each matrix (NaN where the norm is)
+__global__ __launch_bounds__(kThreads) void norm_kernel(const Mat* mats, const double* partial, float* factor, double eps) {
+    __shared__ double scratch[kThreads / kWave];
+    const Mat& e = mats[blockIdx.x];
+    const int64_t n = (int64_t(e.m) * e.n + kChunk - 1) / kChunk;
+    double s = 0.0;
+    for (int64_t i = threadIdx.x; i < n; i += kThreads) s += partial[e.first_chunk + i];
+#pragma unroll
+    for (int o = kWave / 2; o > 0; o >>= 1) s += __shfl_xor(s, o);
+    if ((threadIdx.x & (kWave - 1)) == 0) scratch[threadIdx.x / kWave] = s;
+    __syncthreads();
+    if (threadIdx.x != 0) return;
+    double r = 0.0;
+#pragma unroll
+    for (int w = 0; w < kThreads / kWave; ++w) r += scratch[w];
+    const double norm = sqrt(r);
+    factor[blockIdx.x] = float(double(kUnitX) / (norm < eps ? eps : norm));
+}
+
+// The value as it stands in a register.  Without this the compiler rounds the same expression to fp16 in two ways, once from its fp32 value and
+// once, in one instruction, from its exact one; now and then they differ by a step, and hi and lo did not belong together (fp32 matrices came
+// out 10 to 100 times less exact).
+__device__ __forceinline__ float settled(float x) {
+    asm("" : "+v"(x));
+    return x;
+}
+// x = hi + lo, the rounding of hi made good by lo
+__device__ __forceinline__ void split(float x, float& hi, float& lo) {
+    x = settled(x);
+    hi = float(_Float16(x));
+    lo = x - hi;
+}
+__device__ __forceinline__ void store_pieces8(uint16_t* hi, int64_t lo_plane, const float (&x)[8]) {
+    float h[8], l[8];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) split(x[k], h[k], l[k]);
+    *reinterpret_cast<u32x4*>(hi) = Elem<TRLK_F16>::pack(h);
+    *reinterpret_cast<u32x4*>(hi + lo_plane) = Elem<TRLK_F16>::pack(l);
+}
+
+// X in two pieces, a tile of 64 x 64 a workgroup, turned over where the parameter is tall; the zeros around X, A and B.
+template <int DT>
+__global__ __launch_bounds__(kThreads) void make_x_kernel(const Mat* mats, int n_mats, const float* factor) {
+    __shared__ float tile[kTurn][kTurn + 1];
+    const int i = mat_of<&Mat::first_turn>(mats, n_mats, blockIdx.x);
+    const Mat e = mats[i];
+    const float f = factor[i];
+    const auto* g = static_cast<const typename Elem<DT>::type*>(e.g);
+    const uint32_t t = blockIdx.x - e.first_turn, across = uint32_t(e.npad / kTurn);
+    const int r0 = int(t / across) * kTurn, c0 = int(t % across) * kTurn;
+    const auto value = [&](int64_t at) {
+        const float x = Elem<DT>::load1(g + at);
+        return (e.momentum ? update_of(e.momentum[at], x, e) : x) * f;
+    };
+    if (e.tall) {  // u is n x m: its rows are X's columns
+        const int r = threadIdx.x & 63;
+        for (int c = threadIdx.x >> 6; c < kTurn; c += kThreads / 64)
+            tile[r][c] = r0 + r < e.m && c0 + c < e.n ? value(int64_t(c0 + c) * e.m + r0 + r) : 0.f;
+        __syncthreads();
+    }
+    for (int v = threadIdx.x; v < kTurn * kTurn / 8; v += kThreads) {
+        const int r = v / (kTurn / 8), c = v % (kTurn / 8) * 8;
+        const bool inside = r0 + r < e.m && c0 + c + 8 <= e.n;
+        float x[8];
+        if (e.tall) {
+#pragma unroll
+            for (int k = 0; k < 8; ++k) x[k] = tile[r][c + k];
+        } else if (inside) {
+            const int64_t at = int64_t(r0 + r) * e.n + c0 + c;
+            load8<DT>(g + at, x);
+            if (e.momentum) {
+                float w[8];
+                load8f(e.momentum + at, w);
+#pragma unroll
+                for (int k = 0; k < 8; ++k) x[k] = update_of(w[k], x[k], e);
+            }
+#pragma unroll
+            for (int k = 0; k < 8; ++k) x[k] *= f;
+        } else {
+#pragma unroll
+            for (int k = 0; k < 8; ++k) x[k] = r0 + r < e.m && c0 + c + k < e.n ? value(int64_t(r0 + r) * e.n + c0 + c + k) : 0.f;
+        }
+        const int64_t to = int64_t(r0 + r) * e.npad + c0 + c;
+        store_pieces8(e.buffer(0) + to, e.plane(), x);
+        if (!inside) {  // (the entries of X among them are written later)
+            const float zero[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+            store_pieces8(e.buffer(1) + to, e.plane(), zero);
+        }
+    }
+    if (c0 == 0 && e.m < e.mpad) {
+        const int gap = e.mpad - e.m;
+        for (int v = threadIdx.x; v < kTurn * gap; v += kThreads) {
+            const int64_t to = int64_t(r0 + v / gap) * e.mpad + e.m + v % gap;
+            for (int q = 0; q < e.pieces; ++q) e.a()[q * e.square() + to] = e.b()[q * e.square() + to] = 0;
+        }
+    }
+}
+
+// ---- products --------------------------------------------------------------------------------------------------------
+enum Stage { kStageA, kStageB, kStageX, kStageLast };
+
+struct ProductArgs {
+    const Mat* mats;
+    int32_t n, from;  // from: the buffer that holds X
+    float a, b, c;
+};
+
+__device__ __forceinline__ float half_at(const uint16_t* p) { return Elem<TRLK_F16>::load1(p); }
+// four neighbouring entries
+__device__ __forceinline__ f32x4 halves4(const uint16_t* p) {
+    const u32x2 q = *reinterpret_cast<const u32x2*>(p);
+    float x[4];
+    Elem<TRLK_F16>::unpack2(q.x, x);
+    Elem<TRLK_F16>::unpack2(q.y, x + 2);
+    return f32x4{x[0], x[1], x[2], x[3]};
+}
+__device__ __forceinline__ void store_halves4(uint16_t* p, f32x4 x) {
+    *reinterpret_cast<u32x2*>(p) = u32x2{Elem<TRLK_F16>::pack2(x[0], x[1]), Elem<TRLK_F16>::pack2(x[2], x[3])};
+}
+__device__ __forceinline__ void split4(f32x4 x, f32x4& hi, f32x4& lo) {
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+        float h, l;
+        split(x[k], h, l);
+        hi[k] = h;
+        lo[k] = l;
+    }
+}
+
+// Four neighbouring entries of a parameter (or the output), `left` of them inside: p = p decay - size x, or p = x.
+template <int DT>
+__device__ __forceinline__ void finish4(const Mat& e, int64_t at, int left, f32x4 x, float decay, float size) {
+    auto* p = static_cast<typename Elem<DT>::type*>(e.p) + at;
+    if (left >= 4) {
+        float w[4] = {x[0], x[1], x[2], x[3]};
+        if constexpr (DT == TRLK_F32) {
+            if (e.momentum) {
+                float was[4];
+                Elem<DT>::unpack(*reinterpret_cast<const u32x4_u*>(p), was);
+#pragma unroll
+                for (int k = 0; k < 4; ++k) w[k] = fmaf(was[k], decay, -size * x[k]);
+            }
+            *reinterpret_cast<u32x4_u*>(p) = Elem<DT>::pack(w);
+        } else {
+            if (e.momentum) {
+                const u32x2 q = *reinterpret_cast<const u32x2_u*>(p);
+                float was[4];
+                Elem<DT>::unpack2(q.x, was);
+                Elem<DT>::unpack2(q.y, was + 2);
+#pragma unroll
+                for (int k = 0; k < 4; ++k) w[k] = fmaf(was[k], decay, -size * x[k]);
+            }
+            *reinterpret_cast<u32x2_u*>(p) = u32x2{Elem<DT>::pack2(w[0], w[1]), Elem<DT>::pack2(w[2], w[3])};
+        }
+    } else {
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+            if (k < left) Elem<DT>::store1(p + k, e.momentum ? fmaf(Elem<DT>::load1(p + k), decay, -size * x[k]) : x[k]);
+    }
+}
+
+// One tile of A, B, the next X or, DT, the parameter.  PIECES: two pieces to every operand (fp32).
+template <bool PIECES, int STAGE, int DT>
+TRLK_HEAD_KERNEL void product_kernel(ProductArgs args) {
+    extern __shared__ __attribute__((aligned(16))) char smem[];
+    typedef std::conditional_t<PIECES, PieceRuns, OneRun> Runs;
+    constexpr bool kSquare = STAGE == kStageA || STAGE == kStageB;
+    const Mat e = args.mats[kSquare ? mat_of<&Mat::first_half>(args.mats, args.n, blockIdx.x) : mat_of<&Mat::first_tile>(args.mats, args.n, blockIdx.x)];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int wm = wave_m(wave), wn = wave_n(wave);
+    const uint16_t* x = e.buffer(args.from);
+    const int64_t plane = e.plane(), square = e.square();
+    f32x4 acc[MI][NI];
+    const auto runs = [&](int k, int64_t left, int64_t right) {
+        if constexpr (PIECES) return PieceRuns{k, left * 2, right * 2};
+        else return OneRun{};
+    };
+    constexpr int kRuns = PIECES ? 3 : 1;
+    if constexpr (kSquare) {
+        // tiles on and below the diagonal; an entry has the row of the left operand, i, and the right one's, j
+        const int t = int(blockIdx.x - e.first_half);
+        int ti = int((sqrtf(8.f * float(t) + 1.f) - 1.f) * 0.5f);
+        while ((ti + 1) * (ti + 2) / 2 <= t) ++ti;
+        while (ti * (ti + 1) / 2 > t) --ti;
+        const int tj = t - ti * (ti + 1) / 2;
+        const int i0 = ti * BM, j0 = tj * BN;
+        const uint16_t* from = STAGE == kStageA ? x : e.a();
+        const int k = STAGE == kStageA ? e.npad : e.mpad;
+        const Operand q{from, k, e.m};
+        const int64_t lo = STAGE == kStageA ? plane : square;
+        gemm_tile_nt_direct<TRLK_F16, false, NoLeftKm, Runs>(q, i0, q, j0, kRuns * k, acc, smem, NoLeftKm{}, runs(k, lo, lo));
+        uint16_t* out = STAGE == kStageA ? e.a() : e.b();
+#pragma unroll
+        for (int jj = 0; jj < NI; ++jj) {
+            const int j = j0 + acc_col(wn, jj, lane);
+            if (j >= e.m) continue;
+#pragma unroll
+            for (int ii = 0; ii < MI; ++ii) {
+                const int i = i0 + acc_row(wm, ii, 0, lane);
+                if (i >= e.m) continue;
+                const int64_t at = int64_t(j) * e.mpad + i;
+                f32x4 v;
+                if constexpr (STAGE == kStageA) {
+                    v = acc[ii][jj] * (kUnitA / (kUnitX * kUnitX));
+                } else {
+                    f32x4 w = halves4(e.a() + at);
+                    if constexpr (PIECES) w += halves4(e.a() + square + at);
+                    v = w * args.b + acc[ii][jj] * (args.c / kUnitA);
+                }
+#pragma unroll
+                for (int r = 0; r < 4; ++r)
+                    if (i + r >= e.m) v[r] = 0.f;
+                f32x4 h, l;
+                split4(v, h, l);
+                store_halves4(out + at, h);
+                if constexpr (PIECES) store_halves4(out + square + at, l);
+                if (ti != tj) {
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) {
+                        if (i + r >= e.m) continue;
+                        const int64_t across = int64_t(i + r) * e.mpad + j;
+                        Elem<TRLK_F16>::store1(out + across, h[r]);
+                        if constexpr (PIECES) Elem<TRLK_F16>::store1(out + square + across, l[r]);
+                    }
+                }
+            }
+        }
+    } else {
+        const int t = int(blockIdx.x - e.first_tile), down = (e.m + BN - 1) / BN;
+        const int r0 = t % down * BN, c0 = t / down * BM;
+        const Operand xs{x, e.npad, e.npad}, bs{e.b(), e.mpad, e.m};
+        const float scale = 1.f / kUnitA;
+        float decay = 1.f, size = 0.f;
+        if constexpr (STAGE == kStageLast) {
+            if (e.momentum) {
+                const float lr = e.d_lr ? *e.d_lr : e.lr;
+                decay = float(1.0 - double(lr) * double(e.weight_decay));
+                size = lr * e.stretch;
+            }
+            if (e.tall) {  // entries have a row of the left operand, B, and a column of X: neighbours in the parameter's row
+                gemm_tile_nt_direct<TRLK_F16, true, NoLeftKm, Runs>(bs, r0, xs, c0, kRuns * e.mpad, acc, smem, NoLeftKm{}, runs(e.mpad, square, plane));
+#pragma unroll
+                for (int jj = 0; jj < NI; ++jj) {
+                    const int c = c0 + acc_col(wn, jj, lane);
+                    if (c >= e.n) continue;
+#pragma unroll
+                    for (int ii = 0; ii < MI; ++ii) {
+                        const int r = r0 + acc_row(wm, ii, 0, lane);
+                        if (r >= e.m) continue;
+                        f32x4 v;
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) {  // (rows of X's padding are there)
+                            const uint16_t* p = x + int64_t(r + k) * e.npad + c;
+                            v[k] = half_at(p) + half_at(p + plane);
+                        }
+                        finish4<DT>(e, int64_t(c) * e.m + r, e.m - r, (v * args.a + acc[ii][jj] * scale) * (1.f / kUnitX), decay, size);
+                    }
+                }
+                return;
+            }
+        }
+        // entries have a column of the left operand, X, and a row of B: neighbours in a row of the result
+        LeftKm<false, Runs> left(xs, c0, e.mpad, 1.f, smem, runs(e.mpad, plane, square));
+        gemm_tile_nt_direct<TRLK_F16, false, LeftKm<false, Runs>&, Runs>(xs, c0, bs, r0, kRuns * e.mpad, acc, smem, left, runs(e.mpad, plane, square));
+        uint16_t* out = e.buffer(args.from ^ 1);
+#pragma unroll
+        for (int jj = 0; jj < NI; ++jj) {
+            const int r = r0 + acc_col(wn, jj, lane);
+            if (r >= e.m) continue;
+#pragma unroll
+            for (int ii = 0; ii < MI; ++ii) {
+                const int c = c0 + acc_row(wm, ii, 0, lane);
+                if (c >= e.n) continue;
+                const int64_t at = int64_t(r) * e.npad + c;
+                f32x4 v = (halves4(x + at) + halves4(x + plane + at)) * args.a + acc[ii][jj] * scale;
+                if constexpr (STAGE == kStageLast) {
+                    finish4<DT>(e, int64_t(r) * e.n + c, e.n - c, v * (1.f / kUnitX), decay, size);
+                } else {
+#pragma unroll
+                    for (int k = 0; k < 4; ++k)
+                        if (c + k >= e.n) v[k] = 0.f;
+                    f32x4 h, l;
+                    split4(v, h, l);
+                    store_halves4(out + at, h);
+                    store_halves4(out + plane + at, l);
+                }
+            }
+        }
+    }
+}
+
+// ---- host ------------------------------------------------------------------------------------------------------------
+bool aligned_to(const void* p, size_t a) { return reinterpret_cast<uintptr_t>(p) % a == 0; }
+int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
+int64_t up_to(int64_t n, int64_t unit) { return ceil_div(n, unit) * unit; }
+size_t up256(size_t n) { return (n + 255) / 256 * 256; }
+
+int pieces_of(int dtype) { return dtype == TRLK_F32 ? 2 : 1; }
+size_t matrix_bytes(const trlk_muon_matrix& x) {
+    const int64_t m = up_to(std::min(x.rows, x.cols), BK), n = up_to(std::max(x.rows, x.cols), BK);
+    return up256(size_t(4 * m * n + 2 * pieces_of(x.dtype) * m * m) * 2);
+}
+
+// Matrices that go through the launches together: of one type, as many as the workspace's share holds.
+struct Group {
+    std::vector<int32_t> each;
+    int64_t chunks = 0;
+    size_t bytes = 0;
+    size_t total() const { return up256(each.size() * sizeof(Mat)) + up256(each.size() * sizeof(float)) + up256(size_t(chunks) * sizeof(double)) + bytes; }
+};
+std::vector<Group> groups_of(const trlk_muon_matrix* x, int32_t n) {
+    std::vector<Group> groups;
+    for (int dtype : {int(TRLK_F32), int(TRLK_BF16), int(TRLK_F16)}) {
+        bool fresh = true;
+        for (int32_t i = 0; i < n; ++i) {
+            if (x[i].dtype != dtype || x[i].rows == 0 || x[i].cols == 0) continue;
+            const size_t need = matrix_bytes(x[i]);
+            if (fresh || groups.back().bytes + need > kGroupBytes) groups.emplace_back();
+            fresh = false;
+            groups.back().each.push_back(i);
+            groups.back().chunks += ceil_div(x[i].rows * x[i].cols, kChunk);
+            groups.back().bytes += need;
+        }
+    }
+    return groups;
+}
+
+size_t most_bytes(const trlk_muon_matrix* x, int32_t n) {
+    size_t most = 0;
+    for (const Group& g : groups_of(x, n)) most = std::max(most, g.total());
+    return most;
+}
+
+int reserve_lds(const void* kernel, const char* what) {
+    struct Done {
+        const void* kernel;
+        int device;
+    };
+    static std::mutex guard;
+    static std::vector<Done>& done = *new std::vector<Done>;  // (never destroyed)
+    int device = 0;
+    if (hipGetDevice(&device) != hipSuccess) device = 0;
+    std::lock_guard<std::mutex> lock(guard);
+    for (const Done& d : done)
+        if (d.kernel == kernel && d.device == device) return TRLK_OK;
+    const hipError_t e = hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, kLdsBytes);
+    if (e != hipSuccess) return fail(int(e), "%s: cannot reserve %d bytes of LDS: %s", what, kLdsBytes, hipGetErrorString(e));
+    done.push_back(Done{kernel, device});
+    return TRLK_OK;
+}
+
+template <bool PIECES, int STAGE, int DT = TRLK_F32>
+int launch_product(const ProductArgs& a, int64_t grid, hipStream_t stream, const char* what) {
+    const auto kernel = product_kernel<PIECES, STAGE, DT>;
+    if (const int rc = reserve_lds(reinterpret_cast<const void*>(kernel), what)) return rc;
+    kernel<<<unsigned(grid), kHeadThreads, kLdsBytes, stream>>>(a);
+    return TRLK_OK;
+}
+
+struct Numbers {
+    int32_t steps;
+    double a, b, c, eps;
+};
+
+template <int DT>
+int run_group(const Group& group, const trlk_muon_matrix* x, const trlk_muon_group* groups, const Numbers& num, char* ws, hipStream_t stream, const char* what) {
+    constexpr bool PIECES = DT == TRLK_F32;
+    const int n = int(group.each.size());
+    Mat* mats = reinterpret_cast<Mat*>(ws);
+    float* factor = reinterpret_cast<float*>(ws + up256(n * sizeof(Mat)));
+    double* partial = reinterpret_cast<double*>(reinterpret_cast<char*>(factor) + up256(n * sizeof(float)));
+    char* at = reinterpret_cast<char*>(partial) + up256(size_t(group.chunks) * sizeof(double));
+    int64_t chunks = 0, turns = 0, halves = 0, tiles = 0;
+    MatTable t;
+    t.n = 0;
+    t.to = mats;
+    for (int i = 0; i < n; ++i) {
+        const trlk_muon_matrix& y = x[group.each[i]];
+        Mat& e = t.e[t.n++];
+        e = {};
+        e.x = reinterpret_cast<uint16_t*>(at);
+        at += matrix_bytes(y);
+        e.p = y.d_param, e.g = y.d_grad, e.momentum = y.d_momentum;
+        e.tall = y.rows > y.cols;
+        e.m = int32_t(std::min(y.rows, y.cols)), e.n = int32_t(std::max(y.rows, y.cols));
+        e.mpad = int32_t(up_to(e.m, BK)), e.npad = int32_t(up_to(e.n, BK));
+        e.pieces = pieces_of(DT);
+        if (groups) {
+            const trlk_muon_group& g = groups[y.group];
+            e.lr = float(g.lr), e.d_lr = g.d_lr, e.weight_decay = float(g.weight_decay);
+            e.beta = float(g.momentum), e.rest = float(1.0 - g.momentum), e.nesterov = g.nesterov;
+            const double ratio = double(y.rows) / double(y.cols);
+            e.stretch = float(g.adjust == TRLK_MUON_MATCH_ADAMW ? 0.2 * sqrt(double(e.n)) : sqrt(ratio > 1.0 ? ratio : 1.0));
+        }
+        const int64_t down = ceil_div(e.m, BN);
+        e.first_chunk = uint32_t(chunks), e.first_turn = uint32_t(turns), e.first_half = uint32_t(halves), e.first_tile = uint32_t(tiles);
+        chunks += ceil_div(int64_t(e.m) * e.n, kChunk);
+        turns += int64_t(e.mpad / kTurn) * (e.npad / kTurn);
+        halves += down * (down + 1) / 2;
+        tiles += down * ceil_div(e.n, BM);
+        if (t.n == kTable || i + 1 == n) {
+            table_kernel<<<1, 64, 0, stream>>>(t);
+            t.to += t.n;
+            t.n = 0;
+        }
+    }
+    momentum_kernel<DT><<<unsigned(chunks), kThreads, 0, stream>>>(mats, n, partial);
+    norm_kernel<<<unsigned(n), kThreads, 0, stream>>>(mats, partial, factor, num.eps);
+    make_x_kernel<DT><<<unsigned(turns), kThreads, 0, stream>>>(mats, n, factor);
+    ProductArgs a{mats, n, 0, float(num.a), float(num.b), float(num.c)};
+    for (int s = 0; s < num.steps; ++s) {
+        if (const int rc = launch_product<PIECES, kStageA>(a, halves, stream, what)) return rc;
+        if (const int rc = launch_product<PIECES, kStageB>(a, halves, stream, what)) return rc;
+        const int rc = s + 1 < num.steps ? launch_product<PIECES, kStageX>(a, tiles, stream, what)
+                                         : launch_product<PIECES, kStageLast, DT>(a, tiles, stream, what);
+        if (rc) return rc;
+        a.from ^= 1;
+    }
+    return TRLK_OK;
+}
+
+// The largest |a s + b s^3 + c s^5| for s in [0, top].
+double largest_image(double top, double a, double b, double c) {
+    const auto p = [&](double s) { return fabs(s * (a + s * s * (b + c * s * s))); };
+    double most = p(top);
+    // a + 3 b t + 5 c t^2 = 0, t = s^2
+    double roots[2];
+    int n = 0;
+    if (c != 0.0) {
+        const double d = 9.0 * b * b - 20.0 * a * c;
+        if (d >= 0.0)
+            for (double sign : {-1.0, 1.0}) roots[n++] = (-3.0 * b + sign * sqrt(d)) / (10.0 * c);
+    } else if (b != 0.0) {
+        roots[n++] = -a / (3.0 * b);
+    }
+    for (int i = 0; i < n; ++i)
+        if (roots[i] > 0.0 && roots[i] < top * top) most = std::max(most, p(sqrt(roots[i])));
+    return most;
+}
+
+int check_numbers(const Numbers& num, const char* what) {
+    TRLK_REQUIRE(num.steps >= 1 && num.steps <= 100, TRLK_ERR_BAD_VALUE, "%s: 1 to 100 steps, not %d", what, num.steps);
+    TRLK_REQUIRE(num.eps > 0.0 && num.eps <= 1.0, TRLK_ERR_BAD_VALUE, "%s: eps must be in (0, 1]", what);
+    TRLK_REQUIRE(isfinite(num.a) && isfinite(num.b) && isfinite(num.c), TRLK_ERR_BAD_VALUE, "%s: coefficients must be finite", what);
+    // the fp16 pieces hold singular values up to 65504 / kUnitX, and A and B up to 65504 / kUnitA
+    double top = 1.0;
+    for (int s = 0; s < num.steps; ++s) {
+        const double t = top * top, peak = num.c != 0.0 ? -num.b / (2.0 * num.c) : -1.0;
+        double b_most = fabs(num.b * t + num.c * t * t);
+        if (peak > 0.0 && peak < t) b_most = std::max(b_most, fabs(num.b * peak + num.c * peak * peak));
+        TRLK_REQUIRE(top <= 2.5 && b_most <= 7.0, TRLK_ERR_BAD_VALUE, "%s: with these coefficients singular values grow to %g in step %d", what, top, s);
+        top = largest_image(top, num.a, num.b, num.c);
+    }
+    TRLK_REQUIRE(top <= 1e6, TRLK_ERR_BAD_VALUE, "%s: with these coefficients singular values grow to %g", what, top);
+    return TRLK_OK;
+}
+
+bool size_ok(const trlk_muon_matrix& y) {
+    return y.rows >= 0 && y.cols >= 0 && std::min(y.rows, y.cols) <= kMostRows && std::max(y.rows, y.cols) <= kMostCols && y.rows * y.cols <= kMostEntries;
+}
+int check_matrices(const trlk_muon_matrix* x, int32_t n, const trlk_muon_group* g, int32_t n_groups, bool step, const char* what) {
+    TRLK_REQUIRE(n >= 0 && (n == 0 || x), TRLK_ERR_NULL_POINTER, "%s: null table", what);
+    TRLK_REQUIRE(!step || (n_groups >= 0 && (n == 0 || g)), TRLK_ERR_NULL_POINTER, "%s: null groups", what);
+    for (int32_t i = 0; step && i < n_groups; ++i) {
+        TRLK_REQUIRE(g[i].momentum >= 0.0 && g[i].momentum < 1.0, TRLK_ERR_BAD_VALUE, "%s: momentum must be in [0, 1)", what);
+        TRLK_REQUIRE(g[i].weight_decay >= 0.0 && (g[i].d_lr || g[i].lr >= 0.0), TRLK_ERR_BAD_VALUE, "%s: lr and weight_decay must not be negative", what);
+        TRLK_REQUIRE(g[i].adjust == TRLK_MUON_ORIGINAL || g[i].adjust == TRLK_MUON_MATCH_ADAMW, TRLK_ERR_BAD_VALUE, "%s: unknown adjustment %d", what, g[i].adjust);
+    }
+    for (int32_t i = 0; i < n; ++i) {
+        const trlk_muon_matrix& y = x[i];
+        TRLK_REQUIRE(size_ok(y), TRLK_ERR_BAD_SHAPE, "%s: matrix %d is %lld x %lld", what, i, (long long)y.rows, (long long)y.cols);
+        TRLK_REQUIRE(y.dtype == TRLK_F32 || y.dtype == TRLK_BF16 || y.dtype == TRLK_F16, TRLK_ERR_BAD_DTYPE, "%s: matrix %d: unsupported dtype %d", what, i, y.dtype);
+        TRLK_REQUIRE(!step || (y.group >= 0 && y.group < n_groups), TRLK_ERR_BAD_VALUE, "%s: matrix %d is in no group", what, i);
+        if (y.rows == 0 || y.cols == 0) continue;
+        TRLK_REQUIRE(y.d_param && y.d_grad && (y.d_momentum || !step), TRLK_ERR_NULL_POINTER, "%s: matrix %d: null operand", what, i);
+        TRLK_REQUIRE(step || !y.d_momentum, TRLK_ERR_BAD_VALUE, "%s: matrix %d has a momentum", what, i);
+        TRLK_REQUIRE(aligned_to(y.d_param, elem_size(y.dtype)) && aligned_to(y.d_grad, elem_size(y.dtype)) && aligned_to(y.d_momentum, 4), TRLK_ERR_BAD_STRIDE,
+                     "%s: matrix %d: misaligned operand", what, i);
+    }
+    return TRLK_OK;
+}
+
+int run(const trlk_muon_matrix* x, int32_t n, const trlk_muon_group* groups, int32_t n_groups, bool step, const Numbers& num, void* d_workspace,
+        size_t workspace_bytes, trlk_stream_t stream_, const char* what) {
+    if (const int rc = check_matrices(x, n, groups, n_groups, step, what)) return rc;
+    if (const int rc = check_numbers(num, what)) return rc;
+    const size_t need = n ? most_bytes(x, n) : 0;
+    if (need == 0) return TRLK_OK;
+    TRLK_REQUIRE(d_workspace && workspace_bytes >= need, TRLK_ERR_WORKSPACE, "%s: workspace too small", what);
+    TRLK_REQUIRE(aligned_to(d_workspace, 256), TRLK_ERR_WORKSPACE, "%s: misaligned workspace", what);
+    const hipStream_t stream = static_cast<hipStream_t>(stream_);
+    char* ws = static_cast<char*>(d_workspace);
+    for (const Group& g : groups_of(x, n)) {
+        const int dtype = x[g.each[0]].dtype;
+        const trlk_muon_group* hyper = step ? groups : nullptr;
+        const int rc = dtype == TRLK_F32    ? run_group<TRLK_F32>(g, x, hyper, num, ws, stream, what)
+                       : dtype == TRLK_BF16 ? run_group<TRLK_BF16>(g, x, hyper, num, ws, stream, what)
+                                            : run_group<TRLK_F16>(g, x, hyper, num, ws, stream, what);
+        if (rc) return rc;
+    }
+    return launch_status(what);
+}
+
+// (the tables are vectors: what they throw ends here)
+template <typename F>
+int guarded(const char* what, F f) {
+    clear_error();
+    try {
+        return f();
+    } catch (const std::exception& e) {
+        return fail(TRLK_ERR_BAD_VALUE, "%s: %s", what, e.what());
+    }
+}
+
+}  // namespace
+}  // namespace trlk
+
+using namespace trlk;
+
+extern "C" size_t trlk_muon_workspace_bytes(const trlk_muon_matrix* matrices, int32_t n_matrices) {
+    if (!matrices || n_matrices <= 0) return 0;
+    for (int32_t i = 0; i < n_matrices; ++i)
+        if (!size_ok(matrices[i])) return 0;
+    size_t most = 0;
+    guarded("muon", [&] {
+        most = most_bytes(matrices, n_matrices);
+        return TRLK_OK;
+    });
+    return most;
+}
+
+extern "C" int trlk_orthogonalize(const trlk_muon_matrix* matrices, int32_t n_matrices, int32_t steps, double a, double b, double c, double eps,
+                                  void* d_workspace, size_t workspace_bytes, trlk_stream_t stream) {
+    return guarded("orthogonalize", [&] {
+        return run(matrices, n_matrices, nullptr, 0, false, Numbers{steps, a, b, c, eps}, d_workspace, workspace_bytes, stream, "orthogonalize");
+    });
+}
+
+extern "C" int trlk_muon_step(const trlk_muon_matrix* matrices, int32_t n_matrices, const trlk_muon_group* groups, int32_t n_groups, int32_t steps,
+                              double a, double b, double c, double eps, void* d_workspace, size_t workspace_bytes, trlk_stream_t stream) {
+    return guarded("muon", [&] {
+        return run(matrices, n_matrices, groups, n_groups, true, Numbers{steps, a, b, c, eps}, d_workspace, workspace_bytes, stream, "muon");
+    });
+}

@@ -1009,6 +1009,115 @@ Tensor adamw_state_values(const Tensor& codes, const Tensor& scales) {
                                   values.mutable_data_ptr(), stream_of(codes)));
     return values;
 }
+// ---- Muon -------------------------------------------------------------------------------------------------------------
+// The matrices of tensors [..., m, n], one entry of the table each.  `momenta` null: no step, params are the outputs.
+template <typename List>
+class MatrixTable {
+  public:
+    std::vector<trlk_muon_matrix> table;
+    MatrixTable(const char* op, const at::Device& device) : op_(op), device_(device) {}
+    void add(size_t i, const Tensor& p, const Tensor& g, const Tensor* momentum, int32_t group) {
+        TORCH_CHECK(p.device() == device_ && g.device() == device_ && (momentum == nullptr || momentum->device() == device_), op_, ": matrix ", i,
+                    " or what belongs to it is not on ", device_, " as the first one");
+        TORCH_CHECK_VALUE(p.dim() >= 2, op_, ": matrices are expected, entry ", i, " has shape ", p.sizes());
+        const int64_t rows = p.size(-2), cols = p.size(-1), count = p.numel() == 0 ? 0 : p.numel() / (rows * cols);
+        for (int64_t k = 0; k < count; ++k) {
+            trlk_muon_matrix x{};
+            const int64_t at = k * rows * cols;
+            x.d_param = static_cast<char*>(p.mutable_data_ptr()) + at * p.element_size();
+            x.d_grad = static_cast<const char*>(g.const_data_ptr()) + at * g.element_size();
+            x.d_momentum = momentum ? out(*momentum) + at : nullptr;
+            x.rows = rows, x.cols = cols, x.dtype = dtype_code(p), x.group = group;
+            table.push_back(x);
+        }
+    }
+
+  private:
+    const char* op_;
+    at::Device device_;
+};
+void check_coefficients(const char* op, at::ArrayRef<double> c) { TORCH_CHECK_VALUE(c.size() == 3, op, ": three coefficients are expected, got ", c.size()); }
+
+template <typename List>
+void muon_step(const List& params, const List& grads_, const List& momenta, at::IntArrayRef group_of, at::ArrayRef<double> hyper, const List& lrs,
+               at::ArrayRef<double> coefficients, int64_t steps, double eps) {
+    const size_t n = params.size(), n_groups = hyper.size() / 5;
+    TORCH_CHECK_VALUE(grads_.size() == n && momenta.size() == n && (group_of.empty() || group_of.size() == n), "muon_step_: the lists differ in length");
+    TORCH_CHECK_VALUE(hyper.size() == 5 * n_groups && n_groups > 0 && (lrs.empty() || lrs.size() == n_groups),
+                      "muon_step_: five numbers and one learning rate for each group are expected");
+    TORCH_CHECK_VALUE(n > 0, "muon_step_: no parameters");
+    check_coefficients("muon_step_", coefficients);
+    const at::Device device = params[0].device();
+    const at::NoGradGuard no_grad;
+    const c10::DeviceGuard guard(device);
+    std::vector<trlk_muon_group> groups(n_groups);
+    for (size_t g = 0; g < n_groups; ++g) {
+        const double* h = hyper.data() + 5 * g;
+        groups[g] = {h[0], h[1], h[2], nullptr, h[3] != 0.0, int32_t(h[4])};
+        if (lrs.empty() || lrs[g].numel() == 0) continue;
+        TORCH_CHECK(lrs[g].device() == device, "muon_step_: learning rate ", g, " is on ", lrs[g].device(), ", the first parameter on ", device);
+        TORCH_CHECK_VALUE(lrs[g].numel() == 1 && lrs[g].scalar_type() == at::kFloat, "muon_step_: a learning rate on the GPU is one fp32 number");
+        groups[g].d_lr = static_cast<const float*>(lrs[g].const_data_ptr());
+    }
+    MatrixTable<List> matrices("muon_step_", device);
+    std::vector<Tensor> copies;  // of gradients that are not contiguous
+    Ranges ranges(4, n);
+    for (size_t i = 0; i < n; ++i) {
+        const Tensor &p = params[i], &m = momenta[i];
+        TORCH_CHECK_VALUE(grads_[i].sizes() == p.sizes() && m.sizes() == p.sizes(), "muon_step_: parameter ", i, " of shape ", p.sizes(),
+                          " and its gradient or momentum differ in shape");
+        TORCH_CHECK_TYPE(grads_[i].scalar_type() == p.scalar_type(), "muon_step_: parameter ", i, " is ", p.scalar_type(), ", its gradient ",
+                         grads_[i].scalar_type());
+        TORCH_CHECK_TYPE(m.scalar_type() == at::kFloat, "muon_step_: momentum is fp32, not ", m.scalar_type());
+        TORCH_CHECK_VALUE(p.is_contiguous() && m.is_contiguous(), "muon_step_: parameter ", i, " or its momentum is not contiguous");
+        Tensor g = grads_[i];
+        if (!g.is_contiguous()) copies.push_back(g = g.contiguous());
+        matrices.add(i, p, g, &m, group_of.empty() ? 0 : int32_t(group_of[i]));
+        if (p.numel() == 0) continue;
+        const size_t numel = size_t(p.numel());
+        ranges.add(0, true, p, p.const_data_ptr(), numel * p.element_size());
+        ranges.add(1, false, g, g.const_data_ptr(), numel * g.element_size());
+        ranges.add(2, true, m, m.const_data_ptr(), numel * sizeof(float));
+    }
+    for (size_t g = 0; g < lrs.size(); ++g) {
+        if (lrs[g].numel()) ranges.add(3, false, lrs[g], lrs[g].const_data_ptr(), sizeof(float));
+    }
+    TORCH_CHECK_VALUE(!ranges.shared(), "muon_step_: parameters or momenta are listed twice or share memory, with each other, a gradient or a learning rate");
+    TORCH_CHECK(device.is_cuda(), "muon_step_: the parameters are on ", device, ", not on a GPU");
+    const int32_t count = int32_t(matrices.table.size());
+    const size_t ws_bytes = trlk_muon_workspace_bytes(matrices.table.data(), count);
+    const Tensor ws = bytes(params[0], ws_bytes);
+    check(trlk_muon_step(matrices.table.data(), count, groups.data(), int32_t(n_groups), int32_t(steps), coefficients[0], coefficients[1],
+                         coefficients[2], eps, ws.mutable_data_ptr(), ws_bytes, stream_of(params[0])));
+    for (const List* list : {&params, &momenta})
+        for (size_t i = 0; i < list->size(); ++i)
+            if (!(*list)[i].is_inference()) (*list)[i].unsafeGetTensorImpl()->bump_version();  // (graphs that saved it learn that it has changed)
+}
+void muon_step_(at::TensorList params, at::TensorList grads, at::TensorList momenta, at::IntArrayRef group_of, at::ArrayRef<double> hyper,
+                at::TensorList lrs, at::ArrayRef<double> coefficients, int64_t steps, double eps) {
+    muon_step(params, grads, momenta, group_of, hyper, lrs, coefficients, steps, eps);
+}
+
+std::vector<Tensor> orthogonalize(at::TensorList matrices, at::ArrayRef<double> coefficients, int64_t steps, double eps) {
+    TORCH_CHECK_VALUE(!matrices.empty(), "orthogonalize: no matrices");
+    check_coefficients("orthogonalize", coefficients);
+    const at::Device device = matrices[0].device();
+    const c10::DeviceGuard guard(device);
+    MatrixTable<at::TensorList> list("orthogonalize", device);
+    std::vector<Tensor> inputs, results;
+    for (size_t i = 0; i < matrices.size(); ++i) {
+        inputs.push_back(matrices[i].contiguous());
+        results.push_back(at::empty(matrices[i].sizes(), matrices[i].options()));
+        list.add(i, results[i], inputs[i], nullptr, 0);
+    }
+    TORCH_CHECK(device.is_cuda(), "orthogonalize: the matrices are on ", device, ", not on a GPU");
+    const int32_t count = int32_t(list.table.size());
+    const size_t ws_bytes = trlk_muon_workspace_bytes(list.table.data(), count);
+    const Tensor ws = bytes(matrices[0], ws_bytes);
+    check(trlk_orthogonalize(list.table.data(), count, int32_t(steps), coefficients[0], coefficients[1], coefficients[2], eps, ws.mutable_data_ptr(),
+                             ws_bytes, stream_of(matrices[0])));
+    return results;
+}
 }  // namespace
 
 // The AdamW step for lists of plain tensors, called with the arguments of the operator in one tuple and the GIL held.  The
@@ -1076,6 +1185,9 @@ TORCH_LIBRARY_FRAGMENT(trl_amd, m) {
           "Tensor(e!)[] exp_avg_scales, Tensor(f!)[] exp_avg_sq_scales, int[] group_of, float[] hyper, Tensor[] lrs, "
           "float max_grad_norm, int seed) -> Tensor");
     m.def("adamw_state_values(Tensor codes, Tensor scales) -> Tensor");
+    m.def("muon_step_(Tensor(a!)[] params, Tensor[] grads, Tensor(b!)[] momentum_buffers, int[] group_of, float[] hyper, Tensor[] lrs, "
+          "float[] coefficients, int steps, float eps) -> ()");
+    m.def("orthogonalize(Tensor[] matrices, float[] coefficients, int steps, float eps) -> Tensor[]");
     m.def("embedding(Tensor ids, Tensor weight, float scale, int padding_idx) -> Tensor");
     m.def("embedding_bwd(Tensor grad, Tensor ids, SymInt vocab, float scale, int padding_idx) -> Tensor");
     m.def("embedding_grad_(Tensor(a!) grad_weight, Tensor grad, Tensor ids, float scale, int padding_idx) -> ()");
@@ -1096,6 +1208,8 @@ TORCH_LIBRARY_IMPL(trl_amd, CUDA, m) {
     m.impl("filtered_logps_bwd", filtered_logps_bwd);
     m.impl("adamw_step_", adamw_step_);
     m.impl("adamw_state_values", adamw_state_values);
+    m.impl("muon_step_", muon_step_);
+    m.impl("orthogonalize", orthogonalize);
     m.impl("embedding", embedding);
     m.impl("embedding_bwd", embedding_bwd);
     m.impl("embedding_grad_", embedding_grad_);
@@ -1107,9 +1221,9 @@ TORCH_LIBRARY_IMPL(trl_amd, Autograd, m) {
     m.impl("dpo_loss", dpo_loss_autograd);
     m.impl("filtered_logps_fwd", filtered_logps_fwd_autograd);
     m.impl("embedding", embedding_autograd);
-    for (const char* name : {"logp_entropy_bwd", "grpo_row_scale", "dpo_log_values", "filtered_logps_bwd", "embedding_bwd"})
+    for (const char* name : {"logp_entropy_bwd", "grpo_row_scale", "dpo_log_values", "filtered_logps_bwd", "embedding_bwd", "orthogonalize"})
         m.impl(name, torch::autograd::autogradNotImplementedFallback());
     // (these hand out a gradient, scale one in place, draw or step: their results belong to no graph, whatever the operands require)
-    for (const char* name : {"grpo_fused", "scale_unless_one_", "sample_tokens", "adamw_step_", "adamw_state_values", "embedding_grad_"})
+    for (const char* name : {"grpo_fused", "scale_unless_one_", "sample_tokens", "adamw_step_", "adamw_state_values", "muon_step_", "embedding_grad_"})
         m.impl(name, torch::CppFunction::makeFallthrough());
 }

@@ -6,6 +6,7 @@ from .grpo_trainer import (GRPOLossMixin, get_high_entropy_mask, get_off_policy_
                            grpo_loss_from_logits, grpo_single_pass_supported,
                            metrics_to_dict, per_token_logps_and_entropies, vllm_importance_sampling_ratio)
 from .kto_trainer import KTOLossMixin, kto_compute_loss, kto_sequence_logps
+from .muon import Muon, muon_param_groups, muon_step_, orthogonalize
 from .rloo_trainer import RLOOLossMixin, rloo_advantages, rloo_loss
 from .utils import (_ChunkedLogProbFunction, chunked_logprobs_from_hidden, entropy_from_logits, filtered_logps,
                     logps_and_entropies, nanmax, nanmin, nanstd, patch_chunked_lm_head, sample_tokens, selective_log_softmax)
