@@ -217,7 +217,7 @@ struct DirectLoader {
 // The conversion is what this costs beside the plain loop: 1392 tokens, H = 2048, V = 128256, backward of a bf16 problem 1562 us,
 // of an fp16 problem (nothing to convert) 1555; behind every MFMA of the refill instead of behind two of three 1577.
 // An entry whose scaled value fp16 does not hold counts as fp16's largest (see direct_scale).
-template <bool CONVERT, typename Runs = OneRun>
+template <bool CONVERT>
 struct LeftKm {
     static constexpr int kVecs = 4;
     const char* base;
@@ -225,9 +225,8 @@ struct LeftKm {
     uint32_t row_bytes, col;  // (a tile spans less than 4 GiB)
     int row0, krows;
     float scale, top;  // top: the largest magnitude converted so far, times the scale
-    Runs runs;
-    __device__ __forceinline__ LeftKm(const Operand A, int m0, int krows_, float scale_, char* smem, Runs runs_ = {})
-        : krows(krows_), scale(scale_), top(0.f), runs(runs_) {
+    __device__ __forceinline__ LeftKm(const Operand A, int m0, int krows_, float scale_, char* smem)
+        : krows(krows_), scale(scale_), top(0.f) {
         // FP16_OVFL: what overflows fp16 becomes its largest value (infinities stay), for the rest of the wave's life.  A bit of
         // the mode register, where a clamp would be two instructions more per pair of columns in the tile loop.
         if constexpr (CONVERT) asm volatile("s_setreg_imm32_b32 hwreg(HW_REG_MODE, 23, 1), 1" ::: "memory");
@@ -240,8 +239,8 @@ struct LeftKm {
         lds = smem + wave * 1024 + lane * 16;
     }
     __device__ __forceinline__ void load(int k0, int j, u32x4& w) const {
-        const int row = min(row0 + 16 * j, krows - 1 - runs.inside(k0));
-        w = *reinterpret_cast<const u32x4*>(base + runs.left_plane(k0) + int64_t(runs.inside(k0)) * row_bytes + (uint32_t(row) * row_bytes + col));
+        const int row = min(row0 + 16 * j, krows - 1 - k0);
+        w = *reinterpret_cast<const u32x4*>(base + int64_t(k0) * row_bytes + (uint32_t(row) * row_bytes + col));
     }
     // two neighbouring columns; exact wherever fp16 holds the scaled value (below its range one rounding to nearest)
     __device__ __forceinline__ void convert(uint32_t& w) {
@@ -318,8 +317,9 @@ __device__ __forceinline__ void move_tiles_only(const DirectLoader<BKM, LEFT, Ru
     }
 }
 
-// `left`: a LeftKm, where the left operand is k-major.
-template <int DT, bool BKM = false, typename Left = NoLeftKm, typename Runs = OneRun>
+// `left`: a LeftKm, where the left operand is k-major.  TURNED: an accumulator block holds four neighbouring rows of the right operand for one of
+// the left operand (acc_turned_...), not the other way round.
+template <int DT, bool BKM = false, typename Left = NoLeftKm, typename Runs = OneRun, bool TURNED = false>
 __device__ __forceinline__ void gemm_tile_nt_direct(const Operand A, int m0, const Operand B, int n0, int K,
                                                     f32x4 (&acc)[MI][NI], char* smem, Left&& left = {}, Runs runs = {}) {
     constexpr bool AKM = !std::is_same_v<std::decay_t<Left>, NoLeftKm>;
@@ -464,7 +464,10 @@ __device__ __forceinline__ void gemm_tile_nt_direct(const Operand A, int m0, con
 #pragma unroll
                     for (int jj = 0; jj < 2; ++jj) {
                         const int j = half * 2 + jj;
-                        acc[i][j] = mfma<DT>(a[i], b[j], acc[i][j]);
+                        if constexpr (TURNED)
+                            acc[i][j] = mfma<DT>(b[j], a[i], acc[i][j]);
+                        else
+                            acc[i][j] = mfma<DT>(a[i], b[j], acc[i][j]);
                         __builtin_amdgcn_sched_barrier(0);  // (a load moved above the MFMA would need registers of its own)
                         if (load) {
                             if (half == 1 && jj == 1) a[i] = read_a(na, i, ks ^ 1);
@@ -511,6 +514,9 @@ __device__ __forceinline__ void gemm_tile_nt_direct(const Operand A, int m0, con
 __device__ __forceinline__ int acc_row(int wm, int i, int r, int lane) { return wm * WM + i * 16 + (lane >> 4) * 4 + r; }
 // Column (N index) inside the workgroup tile of block j, for this lane.
 __device__ __forceinline__ int acc_col(int wn, int j, int lane) { return wn * WN + j * 16 + (lane & 15); }
+// The same with TURNED: the row of block i, and the column of element 0 of block j.
+__device__ __forceinline__ int acc_turned_row(int wm, int i, int lane) { return wm * WM + i * 16 + (lane & 15); }
+__device__ __forceinline__ int acc_turned_col(int wn, int j, int lane) { return wn * WN + j * 16 + (lane >> 4) * 4; }
 
 // Workgroup id -> (tile along axis `a`, tile along axis `b`) such that the workgroups that run
 // together on one XCD (ids congruent mod 8, dispatched round-robin) form patches of about 4 x 8 tiles: they share

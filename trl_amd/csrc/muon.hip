@@ -35,13 +35,14 @@ constexpr int kThreads = 256;
 constexpr int kChunk = 8192;       // entries of a workgroup of the momentum's pass
 constexpr int kTurn = 64;          // rows and columns of a tile of the pass that makes X
 constexpr int kLdsBytes = 2 * kDenseStage;
+constexpr int cmax_lds(int a, int b) { return a > b ? a : b; }
 constexpr float kUnitX = 16384.f, kUnitA = 8192.f;  // X and A, B are held times these
 constexpr int64_t kMostRows = 32768, kMostCols = int64_t(1) << 22, kMostEntries = int64_t(1) << 34;
-constexpr size_t kGroupBytes = size_t(1) << 31;  // of workspace, unless one matrix needs more
+constexpr size_t kGroupBytes = size_t(1) << 33;  // of workspace, unless one matrix needs more
 
 // One matrix of a launch: X is m x n, m <= n, rows of npad entries, mpad of them (multiples of the k step; what lies between is zero).
 struct Mat {
-    uint16_t* x;     // [2 buffers][hi, lo][mpad][npad], then A and B, [pieces][mpad][mpad] each
+    uint16_t* x;     // narrow ones: partial sums of G, then T.  Others: [2 buffers][hi, lo][mpad][npad], then A and B, [pieces][mpad][mpad] each
     void* p;         // parameter, or the output
     const void* g;   // gradient, or the input
     float* momentum;  // null: no step, the output is X
@@ -175,6 +176,15 @@ __device__ __forceinline__ void split(float x, float& hi, float& lo) {
     hi = float(_Float16(x));
     lo = x - hi;
 }
+__device__ __forceinline__ void split4(f32x4 x, f32x4& hi, f32x4& lo) {
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+        float h, l;
+        split(x[k], h, l);
+        hi[k] = h;
+        lo[k] = l;
+    }
+}
 __device__ __forceinline__ void store_pieces8(uint16_t* hi, int64_t lo_plane, const float (&x)[8]) {
     float h[8], l[8];
 #pragma unroll
@@ -247,61 +257,112 @@ enum Stage { kStageA, kStageB, kStageX, kStageLast };
 struct ProductArgs {
     const Mat* mats;
     int32_t n, from;  // from: the buffer that holds X
+    uint32_t tiles, run;
     float a, b, c;
 };
 
+// The tiles of all matrices of a launch are numbered one after the other, a matrix's so that 16 or 32 neighbours form a patch of 4 x 4 or 4 x 8, and
+// dealt out in runs of neighbours to the XCDs (xcd_piece): those that run on one XCD together share their slabs of the operands through its L2.
+// bands of 4 rows, column by column
+__device__ __forceinline__ void tile_at(int index, int down, int across, int& tr, int& tc) {
+    const int band = index / (4 * across), rest = index - band * 4 * across, rows = min(4, down - 4 * band);
+    tc = rest / rows;
+    tr = band * 4 + rest - tc * rows;
+}
+// the same for the tiles on and below the diagonal: band k has 16 k + 10 of them, the bands before it 8 k^2 + 2 k
+__device__ __forceinline__ void half_tile_at(int index, int down, int& tr, int& tc) {
+    int band = int((sqrtf(float(4 + 32 * index)) - 2.f) * (1.f / 16.f));
+    while (8 * (band + 1) * (band + 1) + 2 * (band + 1) <= index) ++band;
+    while (8 * band * band + 2 * band > index) --band;
+    const int rest = index - 8 * band * band - 2 * band, rows = min(4, down - 4 * band), square = rows * 4 * band;
+    if (rest < square) {
+        tc = rest / rows;
+        tr = 4 * band + rest - tc * rows;
+        return;
+    }
+    const int t = rest - square;  // (0, 0), (1, 0), (1, 1), (2, 0) ...
+    const int r = t >= 6 ? 3 : t >= 3 ? 2 : t >= 1 ? 1 : 0;
+    tr = 4 * band + r;
+    tc = 4 * band + t - r * (r + 1) / 2;
+}
+
+// Two neighbouring blocks of four fp16 a lane (the lane groups of 16 hold one after the other) as eight neighbours a lane: the groups 0 and 2
+// get the first block's, 1 and 3 the second's; and back.  Offset of a lane's eight in the 32.
+__device__ __forceinline__ int pair_offset(int lane) { return ((lane >> 4) & 1) * 16 + (lane >> 5) * 8; }
+__device__ __forceinline__ u32x4 pair_up(u32x2 a, u32x2 b) {
+    const auto lo = __builtin_amdgcn_permlane16_swap(a.x, b.x, false, false);
+    const auto hi = __builtin_amdgcn_permlane16_swap(a.y, b.y, false, false);
+    return u32x4{lo[0], hi[0], lo[1], hi[1]};
+}
+__device__ __forceinline__ void pair_apart(u32x4 q, u32x2& a, u32x2& b) {
+    const auto lo = __builtin_amdgcn_permlane16_swap(q.x, q.z, false, false);
+    const auto hi = __builtin_amdgcn_permlane16_swap(q.y, q.w, false, false);
+    a = u32x2{lo[0], hi[0]};
+    b = u32x2{lo[1], hi[1]};
+}
+
 __device__ __forceinline__ float half_at(const uint16_t* p) { return Elem<TRLK_F16>::load1(p); }
-// four neighbouring entries
-__device__ __forceinline__ f32x4 halves4(const uint16_t* p) {
-    const u32x2 q = *reinterpret_cast<const u32x2*>(p);
+template <int DT>
+__device__ __forceinline__ f32x4 unpack4(u32x2 q) {
     float x[4];
-    Elem<TRLK_F16>::unpack2(q.x, x);
-    Elem<TRLK_F16>::unpack2(q.y, x + 2);
+    Elem<DT>::unpack2(q.x, x);
+    Elem<DT>::unpack2(q.y, x + 2);
     return f32x4{x[0], x[1], x[2], x[3]};
 }
-__device__ __forceinline__ void store_halves4(uint16_t* p, f32x4 x) {
-    *reinterpret_cast<u32x2*>(p) = u32x2{Elem<TRLK_F16>::pack2(x[0], x[1]), Elem<TRLK_F16>::pack2(x[2], x[3])};
-}
-__device__ __forceinline__ void split4(f32x4 x, f32x4& hi, f32x4& lo) {
-#pragma unroll
-    for (int k = 0; k < 4; ++k) {
-        float h, l;
-        split(x[k], h, l);
-        hi[k] = h;
-        lo[k] = l;
-    }
-}
+template <int DT>
+__device__ __forceinline__ u32x2 pack4(f32x4 x) { return u32x2{Elem<DT>::pack2(x[0], x[1]), Elem<DT>::pack2(x[2], x[3])}; }
 
 // Four neighbouring entries of a parameter (or the output), `left` of them inside: p = p decay - size x, or p = x.
 template <int DT>
 __device__ __forceinline__ void finish4(const Mat& e, int64_t at, int left, f32x4 x, float decay, float size) {
     auto* p = static_cast<typename Elem<DT>::type*>(e.p) + at;
     if (left >= 4) {
-        float w[4] = {x[0], x[1], x[2], x[3]};
+        f32x4 was = {0.f, 0.f, 0.f, 0.f};
         if constexpr (DT == TRLK_F32) {
-            if (e.momentum) {
-                float was[4];
-                Elem<DT>::unpack(*reinterpret_cast<const u32x4_u*>(p), was);
-#pragma unroll
-                for (int k = 0; k < 4; ++k) w[k] = fmaf(was[k], decay, -size * x[k]);
-            }
-            *reinterpret_cast<u32x4_u*>(p) = Elem<DT>::pack(w);
+            if (e.momentum) was = __builtin_bit_cast(f32x4, *reinterpret_cast<const u32x4_u*>(p));
         } else {
-            if (e.momentum) {
-                const u32x2 q = *reinterpret_cast<const u32x2_u*>(p);
-                float was[4];
-                Elem<DT>::unpack2(q.x, was);
-                Elem<DT>::unpack2(q.y, was + 2);
-#pragma unroll
-                for (int k = 0; k < 4; ++k) w[k] = fmaf(was[k], decay, -size * x[k]);
-            }
-            *reinterpret_cast<u32x2_u*>(p) = u32x2{Elem<DT>::pack2(w[0], w[1]), Elem<DT>::pack2(w[2], w[3])};
+            if (e.momentum) was = unpack4<DT>(*reinterpret_cast<const u32x2_u*>(p));
         }
+        if (e.momentum) {
+#pragma unroll
+            for (int k = 0; k < 4; ++k) x[k] = fmaf(was[k], decay, -size * x[k]);
+        }
+        if constexpr (DT == TRLK_F32) *reinterpret_cast<u32x4_u*>(p) = __builtin_bit_cast(u32x4, x);
+        else *reinterpret_cast<u32x2_u*>(p) = pack4<DT>(x);
     } else {
 #pragma unroll
         for (int k = 0; k < 4; ++k)
             if (k < left) Elem<DT>::store1(p + k, e.momentum ? fmaf(Elem<DT>::load1(p + k), decay, -size * x[k]) : x[k]);
     }
+}
+
+// The transposed part of a symmetric result: a wave's 128 x 64 entries go through LDS of its own, 64 rows of 128 (and 8 of padding against bank
+// conflicts), and come back with eight neighbours of the other side a lane, by the transpose loads: lane t of a group of 16 points at the
+// 8 bytes with columns 4 (t % 4) .. + 3 of row t / 4 (of 4 rows) and receives column t of those rows.
+constexpr int kMirrorRow = (WM + 8) * 2, kMirrorWave = WN * kMirrorRow;
+constexpr int kProductLds = cmax_lds(kLdsBytes, WGM * WGN * kMirrorWave);
+__device__ __forceinline__ void mirror(char* mine, const u32x2 (&q)[MI][NI], uint16_t* out, int64_t ld, int i0, int j0, int most, int lane) {
+    const int l15 = lane & 15, g = lane >> 4;
+#pragma unroll
+    for (int jj = 0; jj < NI; ++jj)
+#pragma unroll
+        for (int ii = 0; ii < MI; ++ii)
+            *reinterpret_cast<u32x2*>(mine + (jj * 16 + l15) * kMirrorRow + (ii * 16 + g * 4) * 2) = q[ii][jj];
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    const uint32_t base = uint32_t(reinterpret_cast<uintptr_t>(mine)) + (l15 >> 2) * kMirrorRow + (l15 & 3) * 8;
+#pragma unroll
+    for (int jj = 0; jj < WN / 32; ++jj) {
+#pragma unroll
+        for (int ii = 0; ii < MI; ++ii) {
+            const uint32_t at = base + (jj * 32 + g * 8) * kMirrorRow + ii * 32;
+            const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16(reinterpret_cast<lds_s16x4*>(at));
+            const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16(reinterpret_cast<lds_s16x4*>(at + 4 * kMirrorRow));
+            const u32x2 a = __builtin_bit_cast(u32x2, lo), b = __builtin_bit_cast(u32x2, hi);
+            const int i = i0 + ii * 16 + l15, j = j0 + jj * 32 + g * 8;
+            if (i < most && j < most) *reinterpret_cast<u32x4*>(out + int64_t(i) * ld + j) = u32x4{a.x, a.y, b.x, b.y};
+        }
+    }
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
 }
 
 // One tile of A, B, the next X or, DT, the parameter.  PIECES: two pieces to every operand (fp32).
@@ -310,70 +371,99 @@ TRLK_HEAD_KERNEL void product_kernel(ProductArgs args) {
     extern __shared__ __attribute__((aligned(16))) char smem[];
     typedef std::conditional_t<PIECES, PieceRuns, OneRun> Runs;
     constexpr bool kSquare = STAGE == kStageA || STAGE == kStageB;
-    const Mat e = args.mats[kSquare ? mat_of<&Mat::first_half>(args.mats, args.n, blockIdx.x) : mat_of<&Mat::first_tile>(args.mats, args.n, blockIdx.x)];
+    constexpr uint32_t Mat::*kFirst = kSquare ? &Mat::first_half : &Mat::first_tile;
+    const int64_t piece = xcd_piece(blockIdx.x, args.run);
+    if (piece >= args.tiles) return;
+    const Mat e = args.mats[mat_of<kFirst>(args.mats, args.n, uint32_t(piece))];
+    const int index = int(uint32_t(piece) - e.*kFirst);
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int wm = wave_m(wave), wn = wave_n(wave);
     const uint16_t* x = e.buffer(args.from);
     const int64_t plane = e.plane(), square = e.square();
+    const int down = (e.m + BM - 1) / BM;
     f32x4 acc[MI][NI];
     const auto runs = [&](int k, int64_t left, int64_t right) {
         if constexpr (PIECES) return PieceRuns{k, left * 2, right * 2};
         else return OneRun{};
     };
     constexpr int kRuns = PIECES ? 3 : 1;
+    int tr, tc;
     if constexpr (kSquare) {
         // tiles on and below the diagonal; an entry has the row of the left operand, i, and the right one's, j
-        const int t = int(blockIdx.x - e.first_half);
-        int ti = int((sqrtf(8.f * float(t) + 1.f) - 1.f) * 0.5f);
-        while ((ti + 1) * (ti + 2) / 2 <= t) ++ti;
-        while (ti * (ti + 1) / 2 > t) --ti;
-        const int tj = t - ti * (ti + 1) / 2;
-        const int i0 = ti * BM, j0 = tj * BN;
+        half_tile_at(index, down, tr, tc);
+        const int i0 = tr * BM, j0 = tc * BN;
         const uint16_t* from = STAGE == kStageA ? x : e.a();
         const int k = STAGE == kStageA ? e.npad : e.mpad;
         const Operand q{from, k, e.m};
         const int64_t lo = STAGE == kStageA ? plane : square;
         gemm_tile_nt_direct<TRLK_F16, false, NoLeftKm, Runs>(q, i0, q, j0, kRuns * k, acc, smem, NoLeftKm{}, runs(k, lo, lo));
         uint16_t* out = STAGE == kStageA ? e.a() : e.b();
+        const int iw = i0 + wm * WM, jw = j0 + wn * WN;
+        if (iw >= e.m || jw >= e.m) return;  // (no barrier follows)
+        // (neighbours past m, up to mpad, are written as zeros: they are the contraction's padding in the next product)
+        u32x2 high[MI][NI], low[PIECES ? MI : 1][PIECES ? NI : 1];
+        u32x4 was[2][PIECES ? MI : MI / 2];  // A's entries, a column of blocks ahead
+        const auto fetch = [&](int jj) {
+            const uint16_t* p = e.a() + int64_t(min(j0 + acc_col(wn, jj, lane), e.m - 1)) * e.mpad;
+#pragma unroll
+            for (int ii = 0; ii < MI; ii += 2) {
+                const int at = min(iw + ii * 16 + pair_offset(lane), e.mpad - 8);
+                was[jj & 1][ii / 2] = *reinterpret_cast<const u32x4*>(p + at);
+                if constexpr (PIECES) was[jj & 1][MI / 2 + ii / 2] = *reinterpret_cast<const u32x4*>(p + square + at);
+            }
+        };
+        if constexpr (STAGE == kStageB) fetch(0);
 #pragma unroll
         for (int jj = 0; jj < NI; ++jj) {
             const int j = j0 + acc_col(wn, jj, lane);
-            if (j >= e.m) continue;
+            const bool live = j < e.m;
+            const int64_t row = int64_t(live ? j : 0) * e.mpad;
+            if (STAGE == kStageB && jj + 1 < NI) fetch(jj + 1);
 #pragma unroll
-            for (int ii = 0; ii < MI; ++ii) {
-                const int i = i0 + acc_row(wm, ii, 0, lane);
-                if (i >= e.m) continue;
-                const int64_t at = int64_t(j) * e.mpad + i;
-                f32x4 v;
-                if constexpr (STAGE == kStageA) {
-                    v = acc[ii][jj] * (kUnitA / (kUnitX * kUnitX));
-                } else {
-                    f32x4 w = halves4(e.a() + at);
-                    if constexpr (PIECES) w += halves4(e.a() + square + at);
-                    v = w * args.b + acc[ii][jj] * (args.c / kUnitA);
+            for (int ii = 0; ii < MI; ii += 2) {
+                const int at = iw + ii * 16 + pair_offset(lane);
+                const bool there = live && at < e.mpad;
+                u32x2 ah[2], al[2];
+                if constexpr (STAGE == kStageB) {
+                    pair_apart(was[jj & 1][ii / 2], ah[0], ah[1]);
+                    if constexpr (PIECES) pair_apart(was[jj & 1][MI / 2 + ii / 2], al[0], al[1]);
                 }
 #pragma unroll
-                for (int r = 0; r < 4; ++r)
-                    if (i + r >= e.m) v[r] = 0.f;
-                f32x4 h, l;
-                split4(v, h, l);
-                store_halves4(out + at, h);
-                if constexpr (PIECES) store_halves4(out + square + at, l);
-                if (ti != tj) {
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) {
-                        if (i + r >= e.m) continue;
-                        const int64_t across = int64_t(i + r) * e.mpad + j;
-                        Elem<TRLK_F16>::store1(out + across, h[r]);
-                        if constexpr (PIECES) Elem<TRLK_F16>::store1(out + square + across, l[r]);
+                for (int u = 0; u < 2; ++u) {
+                    const int i = i0 + acc_row(wm, ii + u, 0, lane);
+                    f32x4 v, h, l;
+                    if constexpr (STAGE == kStageA) {
+                        v = acc[ii + u][jj] * (kUnitA / (kUnitX * kUnitX));
+                    } else {
+                        f32x4 w = unpack4<TRLK_F16>(ah[u]);
+                        if constexpr (PIECES) w += unpack4<TRLK_F16>(al[u]);
+                        v = w * args.b + acc[ii + u][jj] * (args.c / kUnitA);
                     }
+#pragma unroll
+                    for (int r = 0; r < 4; ++r)
+                        if (i + r >= e.m || !live) v[r] = 0.f;
+                    split4(v, h, l);
+                    high[ii + u][jj] = pack4<TRLK_F16>(h);
+                    if constexpr (PIECES) low[ii + u][jj] = pack4<TRLK_F16>(l);
+                }
+                const u32x4 h8 = pair_up(high[ii][jj], high[ii + 1][jj]);
+                if (there) *reinterpret_cast<u32x4*>(out + row + at) = h8;
+                if constexpr (PIECES) {
+                    const u32x4 l8 = pair_up(low[ii][jj], low[ii + 1][jj]);
+                    if (there) *reinterpret_cast<u32x4*>(out + square + row + at) = l8;
                 }
             }
         }
+        if (tr != tc) {
+            char* mine = smem + wave * kMirrorWave;
+            mirror(mine, high, out, e.mpad, iw, jw, e.m, lane);
+            if constexpr (PIECES) mirror(mine, low, out + square, e.mpad, iw, jw, e.m, lane);
+        }
     } else {
-        const int t = int(blockIdx.x - e.first_tile), down = (e.m + BN - 1) / BN;
-        const int r0 = t % down * BN, c0 = t / down * BM;
-        const Operand xs{x, e.npad, e.npad}, bs{e.b(), e.mpad, e.m};
+        const int across = (e.n + BN - 1) / BN;
+        tile_at(index, down, across, tr, tc);
+        const int r0 = tr * BM, c0 = tc * BN;
+        const Operand bs{e.b(), e.mpad, e.m}, xs{x, e.npad, e.npad};
         const float scale = 1.f / kUnitA;
         float decay = 1.f, size = 0.f;
         if constexpr (STAGE == kStageLast) {
@@ -382,7 +472,7 @@ TRLK_HEAD_KERNEL void product_kernel(ProductArgs args) {
                 decay = float(1.0 - double(lr) * double(e.weight_decay));
                 size = lr * e.stretch;
             }
-            if (e.tall) {  // entries have a row of the left operand, B, and a column of X: neighbours in the parameter's row
+            if (e.tall) {  // neighbours are those of a column of X, which is the parameter's row
                 gemm_tile_nt_direct<TRLK_F16, true, NoLeftKm, Runs>(bs, r0, xs, c0, kRuns * e.mpad, acc, smem, NoLeftKm{}, runs(e.mpad, square, plane));
 #pragma unroll
                 for (int jj = 0; jj < NI; ++jj) {
@@ -404,31 +494,313 @@ TRLK_HEAD_KERNEL void product_kernel(ProductArgs args) {
                 return;
             }
         }
-        // entries have a column of the left operand, X, and a row of B: neighbours in a row of the result
-        LeftKm<false, Runs> left(xs, c0, e.mpad, 1.f, smem, runs(e.mpad, plane, square));
-        gemm_tile_nt_direct<TRLK_F16, false, LeftKm<false, Runs>&, Runs>(xs, c0, bs, r0, kRuns * e.mpad, acc, smem, left, runs(e.mpad, plane, square));
+        gemm_tile_nt_direct<TRLK_F16, true, NoLeftKm, Runs, true>(bs, r0, xs, c0, kRuns * e.mpad, acc, smem, NoLeftKm{}, runs(e.mpad, square, plane));
+        const int cw = c0 + wn * WN;
+        if (cw >= e.npad) return;  // (npad is a multiple of a wave's 64 columns: all of them are there or none)
         uint16_t* out = e.buffer(args.from ^ 1);
+        // X's own entries, loaded some rows of blocks ahead: a load cannot pass the stores before it, and each would wait for them
+        constexpr int kAhead = 4;
+        u32x4 own[kAhead][NI];  // of each pair of blocks, hi and lo
+        const auto row_of = [&](int ii) { return int64_t(min(r0 + acc_turned_row(wm, ii, lane), e.m - 1)) * e.npad + cw + pair_offset(lane); };
+        const auto fetch = [&](int ii) {
+            const uint16_t* p = x + row_of(ii);
 #pragma unroll
-        for (int jj = 0; jj < NI; ++jj) {
-            const int r = r0 + acc_col(wn, jj, lane);
-            if (r >= e.m) continue;
+            for (int jj = 0; jj < NI; jj += 2) {
+                own[ii % kAhead][jj] = *reinterpret_cast<const u32x4*>(p + jj * 16);
+                own[ii % kAhead][jj + 1] = *reinterpret_cast<const u32x4*>(p + plane + jj * 16);
+            }
+        };
 #pragma unroll
-            for (int ii = 0; ii < MI; ++ii) {
-                const int c = c0 + acc_row(wm, ii, 0, lane);
-                if (c >= e.n) continue;
-                const int64_t at = int64_t(r) * e.npad + c;
-                f32x4 v = (halves4(x + at) + halves4(x + plane + at)) * args.a + acc[ii][jj] * scale;
-                if constexpr (STAGE == kStageLast) {
-                    finish4<DT>(e, int64_t(r) * e.n + c, e.n - c, v * (1.f / kUnitX), decay, size);
-                } else {
+        for (int ii = 0; ii < kAhead; ++ii) fetch(ii);
 #pragma unroll
-                    for (int k = 0; k < 4; ++k)
-                        if (c + k >= e.n) v[k] = 0.f;
-                    f32x4 h, l;
-                    split4(v, h, l);
-                    store_halves4(out + at, h);
-                    store_halves4(out + plane + at, l);
+        for (int ii = 0; ii < MI; ++ii) {
+            const int r = r0 + acc_turned_row(wm, ii, lane);
+            const bool live = r < e.m;
+            f32x4 v[NI];
+#pragma unroll
+            for (int jj = 0; jj < NI; jj += 2) {
+                u32x2 xh[2], xl[2];
+                pair_apart(own[ii % kAhead][jj], xh[0], xh[1]);
+                pair_apart(own[ii % kAhead][jj + 1], xl[0], xl[1]);
+#pragma unroll
+                for (int u = 0; u < 2; ++u)
+                    v[jj + u] = (unpack4<TRLK_F16>(xh[u]) + unpack4<TRLK_F16>(xl[u])) * args.a + acc[ii][jj + u] * scale;
+            }
+            if (ii + kAhead < MI) fetch(ii + kAhead);
+            if constexpr (STAGE == kStageLast) {
+#pragma unroll
+                for (int jj = 0; jj < NI; ++jj) {
+                    const int c = c0 + acc_turned_col(wn, jj, lane);
+                    if (live && c < e.n) finish4<DT>(e, int64_t(r) * e.n + c, e.n - c, v[jj] * (1.f / kUnitX), decay, size);
                 }
+            } else {  // (X's padding is zero, and so is what is made of it)
+                const int64_t at = row_of(ii);
+#pragma unroll
+                for (int jj = 0; jj < NI; jj += 2) {
+                    u32x2 h2[2], l2[2];
+#pragma unroll
+                    for (int u = 0; u < 2; ++u) {
+                        f32x4 h, l;
+                        split4(v[jj + u], h, l);
+                        h2[u] = pack4<TRLK_F16>(h);
+                        l2[u] = pack4<TRLK_F16>(l);
+                    }
+                    const u32x4 h8 = pair_up(h2[0], h2[1]), l8 = pair_up(l2[0], l2[1]);
+                    if (live) {
+                        *reinterpret_cast<u32x4*>(out + at + jj * 16) = h8;
+                        *reinterpret_cast<u32x4*>(out + plane + at + jj * 16) = l8;
+                    }
+                }
+            }
+        }
+    }
+}
+
+// ---- narrow matrices: 64 rows or fewer ------------------------------------------------------------------------------------
+// With T = the product of the steps' factors, the result is T X, and both T and every step's X X^T are polynomials of the first one's, G = X X^T, which is
+// m x m: X is read once for G and once for T X, the steps are products of m x m matrices in one workgroup's LDS,
+//   P = a + b G + c G G,  T = P T,  G = P G P.
+// G squares the singular values: what X holds in 24 bits needs 48 in G, so all of this is in 64 bits (fp64 runs at full rate here, and there is
+// little of it: 224 adapters of rank 16 with 9M entries take 0.3 GFLOP).  Bound by the memory, and by launches: three and the tables instead of
+// the 18 of the larger matrices' way.
+constexpr int kNarrow = 64;          // rows at most
+constexpr int kCols = 128;           // columns of u at a time in LDS
+constexpr int kSpan = 4 * kCols;     // and of a workgroup
+constexpr int kLine = kCols + 1;
+
+// u of `cols` columns from c0 on as fp32, [row][column] (kLine apart), zero outside; MOVE: the momentum moves on (else it has).
+template <int DT, int MP, bool MOVE>
+__device__ __forceinline__ void load_u(const Mat& e, int c0, float* tile) {
+    const auto* g = static_cast<const typename Elem<DT>::type*>(e.g);
+    const auto value = [&](int64_t at) {
+        const float x = Elem<DT>::load1(g + at);
+        if (!e.momentum) return x;
+        float now = e.momentum[at];
+        if constexpr (MOVE) e.momentum[at] = now = moved(now, x, e);
+        return update_of(now, x, e);
+    };
+    const int cols = min(kCols, e.n - c0);
+    const auto four = [&](int64_t at, float (&u)[4]) {
+        float x[8], w[4];
+        if constexpr (DT == TRLK_F32) {
+            Elem<DT>::unpack(*reinterpret_cast<const u32x4_u*>(g + at), x);
+        } else {
+            const u32x2 q = *reinterpret_cast<const u32x2_u*>(g + at);
+            Elem<DT>::unpack2(q.x, x);
+            Elem<DT>::unpack2(q.y, x + 2);
+        }
+        if (e.momentum) {
+            Elem<TRLK_F32>::unpack(*reinterpret_cast<const u32x4_u*>(e.momentum + at), w);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                if constexpr (MOVE) w[k] = moved(w[k], x[k], e);
+                x[k] = update_of(w[k], x[k], e);
+            }
+            if constexpr (MOVE) *reinterpret_cast<u32x4_u*>(e.momentum + at) = Elem<TRLK_F32>::pack(w);
+        }
+#pragma unroll
+        for (int k = 0; k < 4; ++k) u[k] = x[k];
+    };
+    if (e.tall) {  // cols * m entries one behind the other
+        const int64_t from = int64_t(c0) * e.m;
+        const int count = cols * e.m;
+        for (int i = threadIdx.x * 4; i < count; i += kThreads * 4) {
+            float u[4] = {0.f, 0.f, 0.f, 0.f};
+            if (i + 4 <= count) four(from + i, u);
+            else
+                for (int k = 0; i + k < count; ++k) u[k] = value(from + i + k);
+            int c = i / e.m, r = i - c * e.m;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                if (i + k < count) tile[r * kLine + c] = u[k];
+                if (++r == e.m) r = 0, ++c;
+            }
+        }
+        for (int i = threadIdx.x; i < MP * kCols; i += kThreads) {
+            const int r = i / kCols, c = i % kCols;
+            if (r >= e.m || c >= cols) tile[r * kLine + c] = 0.f;
+        }
+    } else {
+        for (int i = threadIdx.x; i < MP * kCols / 4; i += kThreads) {
+            const int r = i / (kCols / 4), c = i % (kCols / 4) * 4;
+            const int64_t at = int64_t(r) * e.n + c0 + c;
+            float u[4] = {0.f, 0.f, 0.f, 0.f};
+            if (r < e.m) {
+                if (c + 4 <= cols) four(at, u);
+                else
+                    for (int k = 0; c + k < cols; ++k) u[k] = value(at + k);
+            }
+#pragma unroll
+            for (int k = 0; k < 4; ++k) tile[r * kLine + c + k] = u[k];
+        }
+    }
+}
+
+// The sum over a workgroup's columns of u u^T.  A lane has 4 x 4 entries of it; with fewer than 64 rows the lanes share the columns.
+template <int DT, int MP>
+__global__ __launch_bounds__(kThreads) void gram_kernel(const Mat* mats, int n_mats) {
+    constexpr int kBlocks = (MP / 4) * (MP / 4), kSlices = kThreads / kBlocks;
+    constexpr int kTileBytes = MP * kLine * 4, kSumBytes = kSlices > 1 ? kSlices * MP * MP * 8 : 0;
+    __shared__ __attribute__((aligned(16))) char smem[kTileBytes > kSumBytes ? kTileBytes : kSumBytes];
+    float* tile = reinterpret_cast<float*>(smem);
+    const Mat e = mats[mat_of<&Mat::first_chunk>(mats, n_mats, blockIdx.x)];
+    const int chunk = int(blockIdx.x - e.first_chunk), slice = threadIdx.x / kBlocks, block = threadIdx.x % kBlocks;
+    const int bi = block / (MP / 4) * 4, bj = block % (MP / 4) * 4;
+    double sum[4][4] = {};
+    for (int c0 = chunk * kSpan; c0 < (chunk + 1) * kSpan && c0 < e.n; c0 += kCols) {
+        __syncthreads();
+        load_u<DT, MP, true>(e, c0, tile);
+        __syncthreads();
+        for (int c = slice; c < kCols; c += kSlices) {
+            double x[4], y[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) x[k] = tile[(bi + k) * kLine + c], y[k] = tile[(bj + k) * kLine + c];
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) sum[i][j] = __builtin_fma(x[i], y[j], sum[i][j]);
+        }
+    }
+    double* out = reinterpret_cast<double*>(e.x) + int64_t(chunk) * MP * MP;
+    if constexpr (kSlices == 1) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) out[(bi + i) * MP + bj + j] = sum[i][j];
+    } else {
+        double* sums = reinterpret_cast<double*>(smem);
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) sums[slice * MP * MP + (bi + i) * MP + bj + j] = sum[i][j];
+        __syncthreads();
+        for (int k = threadIdx.x; k < MP * MP; k += kThreads) {
+            double s = 0.0;
+#pragma unroll
+            for (int q = 0; q < kSlices; ++q) s += sums[q * MP * MP + k];
+            out[k] = s;
+        }
+    }
+}
+
+// z = x y + d for symmetric x, y that commute, MP x MP in LDS, d on the diagonal; `x` and `z` may be the same.
+template <int MP, typename F>
+__device__ __forceinline__ void square_product(const double* x, const double* y, double* z, F f) {
+    constexpr int LD = MP + 1, kBlocks = (MP / 4) * (MP / 4);
+    const int block = threadIdx.x, bi = block / (MP / 4) * 4, bj = block % (MP / 4) * 4;
+    double sum[4][4] = {};
+    if (block < kBlocks) {
+        for (int k = 0; k < MP; ++k) {
+            double p[4], q[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) p[i] = x[(bi + i) * LD + k], q[i] = y[k * LD + bj + i];
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) sum[i][j] = __builtin_fma(p[i], q[j], sum[i][j]);
+        }
+    }
+    __syncthreads();
+    if (block < kBlocks) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) z[(bi + i) * LD + bj + j] = f(sum[i][j], bi + i, bj + j);
+    }
+    __syncthreads();
+}
+
+// T / max(|u|, eps) of a matrix, behind its partial sums.
+template <int MP>
+__global__ __launch_bounds__(kThreads) void narrow_steps_kernel(const Mat* mats, int steps, double a, double b, double c, double eps) {
+    constexpr int LD = MP + 1;
+    extern __shared__ double buffers[];
+    double *G = buffers, *P = G + MP * LD, *T = P + MP * LD, *W = T + MP * LD;
+    const Mat& e = mats[blockIdx.x];
+    const int chunks = (e.n + kSpan - 1) / kSpan;
+    double* parts = reinterpret_cast<double*>(e.x);
+    for (int k = threadIdx.x; k < MP * MP; k += kThreads) {
+        double s = 0.0;
+        for (int q = 0; q < chunks; ++q) s += parts[int64_t(q) * MP * MP + k];
+        G[k / MP * LD + k % MP] = s;
+    }
+    __syncthreads();
+    double trace = 0.0;
+    for (int k = 0; k < MP; ++k) trace += G[k * LD + k];
+    const double norm = sqrt(trace), f = 1.0 / (norm < eps ? eps : norm);
+    __syncthreads();
+    for (int k = threadIdx.x; k < MP * LD; k += kThreads) G[k] *= f * f;  // (the last column is nobody's)
+    __syncthreads();
+    for (int s = 0; s < steps; ++s) {
+        square_product<MP>(G, G, P, [&](double x, int i, int j) { return c * x + b * G[i * LD + j] + (i == j ? a : 0.0); });
+        if (s == 0) {
+            for (int k = threadIdx.x; k < MP * LD; k += kThreads) T[k] = P[k] * f;
+            __syncthreads();
+        } else {
+            square_product<MP>(T, P, T, [](double x, int, int) { return x; });
+        }
+        if (s + 1 == steps) break;
+        square_product<MP>(P, G, W, [](double x, int, int) { return x; });
+        square_product<MP>(W, P, G, [](double x, int, int) { return x; });
+    }
+    double* out = parts + int64_t(chunks) * MP * MP;
+    for (int k = threadIdx.x; k < MP * MP; k += kThreads) out[k] = T[k / MP * LD + k % MP];
+}
+
+// T u for a workgroup's columns, a lane half of a column's entries, and the parameter.
+template <int DT, int MP>
+__global__ __launch_bounds__(kThreads) void narrow_apply_kernel(const Mat* mats, int n_mats) {
+    static_assert(kThreads == 2 * kCols, "two lanes a column");
+    __shared__ float tile[MP * kLine];
+    const Mat e = mats[mat_of<&Mat::first_chunk>(mats, n_mats, blockIdx.x)];
+    const int chunk = int(blockIdx.x - e.first_chunk), c = threadIdx.x % kCols;
+    const int half = __builtin_amdgcn_readfirstlane(threadIdx.x / kCols);
+    const double* T = reinterpret_cast<const double*>(e.x) + int64_t((e.n + kSpan - 1) / kSpan) * MP * MP + half * (MP / 2) * MP;
+    float decay = 1.f, size = 0.f;
+    if (e.momentum) {
+        const float lr = e.d_lr ? *e.d_lr : e.lr;
+        decay = float(1.0 - double(lr) * double(e.weight_decay));
+        size = lr * e.stretch;
+    }
+    for (int c0 = chunk * kSpan; c0 < (chunk + 1) * kSpan && c0 < e.n; c0 += kCols) {
+        __syncthreads();
+        load_u<DT, MP, false>(e, c0, tile);
+        __syncthreads();
+        double u[MP];
+#pragma unroll
+        for (int k = 0; k < MP; ++k) u[k] = tile[k * kLine + c];
+        __syncthreads();
+#pragma unroll 2
+        for (int r = 0; r < MP / 2; ++r) {
+            double s = 0.0;
+#pragma unroll
+            for (int k = 0; k < MP; ++k) s = __builtin_fma(T[r * MP + k], u[k], s);
+            tile[(half * (MP / 2) + r) * kLine + c] = float(s);
+        }
+        __syncthreads();
+        const int cols = min(kCols, e.n - c0);
+        if (e.tall) {
+            const int64_t from = int64_t(c0) * e.m;
+            const int count = cols * e.m;
+            for (int i = threadIdx.x * 4; i < count; i += kThreads * 4) {
+                f32x4 x = {0.f, 0.f, 0.f, 0.f};
+                int q = i / e.m, r = i - q * e.m;
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    if (i + k < count) x[k] = tile[r * kLine + q];
+                    if (++r == e.m) r = 0, ++q;
+                }
+                finish4<DT>(e, from + i, count - i, x, decay, size);
+            }
+        } else {
+            for (int i = threadIdx.x; i < e.m * (kCols / 4); i += kThreads) {
+                const int r = i / (kCols / 4), q = i % (kCols / 4) * 4;
+                if (q >= cols) continue;
+                f32x4 x;
+#pragma unroll
+                for (int k = 0; k < 4; ++k) x[k] = tile[r * kLine + q + k];
+                finish4<DT>(e, int64_t(r) * e.n + c0 + q, cols - q, x, decay, size);
             }
         }
     }
@@ -441,32 +813,49 @@ int64_t up_to(int64_t n, int64_t unit) { return ceil_div(n, unit) * unit; }
 size_t up256(size_t n) { return (n + 255) / 256 * 256; }
 
 int pieces_of(int dtype) { return dtype == TRLK_F32 ? 2 : 1; }
+// Rows that a narrow matrix is padded to, 0 for the others.
+int narrow_rows(const trlk_muon_matrix& x) {
+    const int64_t m = std::min(x.rows, x.cols);
+    return m <= 16 ? 16 : m <= 32 ? 32 : m <= kNarrow ? 64 : 0;
+}
 size_t matrix_bytes(const trlk_muon_matrix& x) {
+    if (const int mp = narrow_rows(x)) return up256(size_t(ceil_div(std::max(x.rows, x.cols), kSpan) + 1) * mp * mp * sizeof(double));
     const int64_t m = up_to(std::min(x.rows, x.cols), BK), n = up_to(std::max(x.rows, x.cols), BK);
     return up256(size_t(4 * m * n + 2 * pieces_of(x.dtype) * m * m) * 2);
 }
 
-// Matrices that go through the launches together: of one type, as many as the workspace's share holds.
+// Matrices that go through the launches together: of one type, narrow ones of one kind, as many as the workspace's share holds.
 struct Group {
     std::vector<int32_t> each;
-    int64_t chunks = 0;
+    int32_t narrow = 0;
+    int64_t chunks = 0;  // partial sums of norms
     size_t bytes = 0;
     size_t total() const { return up256(each.size() * sizeof(Mat)) + up256(each.size() * sizeof(float)) + up256(size_t(chunks) * sizeof(double)) + bytes; }
 };
+// (the longest contractions first, so that a launch's last workgroups are short ones)
 std::vector<Group> groups_of(const trlk_muon_matrix* x, int32_t n) {
     std::vector<Group> groups;
-    for (int dtype : {int(TRLK_F32), int(TRLK_BF16), int(TRLK_F16)}) {
-        bool fresh = true;
-        for (int32_t i = 0; i < n; ++i) {
-            if (x[i].dtype != dtype || x[i].rows == 0 || x[i].cols == 0) continue;
-            const size_t need = matrix_bytes(x[i]);
-            if (fresh || groups.back().bytes + need > kGroupBytes) groups.emplace_back();
-            fresh = false;
-            groups.back().each.push_back(i);
-            groups.back().chunks += ceil_div(x[i].rows * x[i].cols, kChunk);
-            groups.back().bytes += need;
+    std::vector<int32_t> order;
+    for (int dtype : {int(TRLK_F32), int(TRLK_BF16), int(TRLK_F16)})
+        for (int narrow : {0, 16, 32, 64}) {
+            order.clear();
+            for (int32_t i = 0; i < n; ++i)
+                if (x[i].dtype == dtype && x[i].rows > 0 && x[i].cols > 0 && narrow_rows(x[i]) == narrow) order.push_back(i);
+            std::stable_sort(order.begin(), order.end(), [&](int32_t i, int32_t j) {
+                const int64_t mi = std::min(x[i].rows, x[i].cols), mj = std::min(x[j].rows, x[j].cols), ni = std::max(x[i].rows, x[i].cols), nj = std::max(x[j].rows, x[j].cols);
+                return ni != nj ? ni > nj : mi > mj;
+            });
+            bool fresh = true;
+            for (const int32_t i : order) {
+                const size_t need = matrix_bytes(x[i]);
+                if (fresh || groups.back().bytes + need > kGroupBytes) groups.emplace_back();
+                fresh = false;
+                groups.back().narrow = narrow;
+                groups.back().each.push_back(i);
+                groups.back().chunks += narrow ? 0 : ceil_div(x[i].rows * x[i].cols, kChunk);
+                groups.back().bytes += need;
+            }
         }
-    }
     return groups;
 }
 
@@ -476,7 +865,7 @@ size_t most_bytes(const trlk_muon_matrix* x, int32_t n) {
     return most;
 }
 
-int reserve_lds(const void* kernel, const char* what) {
+int reserve_lds(const void* kernel, int bytes, const char* what) {
     struct Done {
         const void* kernel;
         int device;
@@ -488,17 +877,22 @@ int reserve_lds(const void* kernel, const char* what) {
     std::lock_guard<std::mutex> lock(guard);
     for (const Done& d : done)
         if (d.kernel == kernel && d.device == device) return TRLK_OK;
-    const hipError_t e = hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, kLdsBytes);
-    if (e != hipSuccess) return fail(int(e), "%s: cannot reserve %d bytes of LDS: %s", what, kLdsBytes, hipGetErrorString(e));
+    const hipError_t e = hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (e != hipSuccess) return fail(int(e), "%s: cannot reserve %d bytes of LDS: %s", what, bytes, hipGetErrorString(e));
     done.push_back(Done{kernel, device});
     return TRLK_OK;
 }
 
 template <bool PIECES, int STAGE, int DT = TRLK_F32>
-int launch_product(const ProductArgs& a, int64_t grid, hipStream_t stream, const char* what) {
+int launch_product(ProductArgs a, int64_t tiles, hipStream_t stream, const char* what) {
+    // runs of 16 tiles, of fewer where an XCD would get under 8 of them, and the same number for all
+    const int64_t want = std::max<int64_t>(1, std::min<int64_t>(16, tiles / 64)), rounds = ceil_div(tiles, 8 * want);
+    a.tiles = uint32_t(tiles);
+    a.run = uint32_t(ceil_div(tiles, 8 * rounds));
+    const int64_t grid = xcd_grid(tiles, a.run);
     const auto kernel = product_kernel<PIECES, STAGE, DT>;
-    if (const int rc = reserve_lds(reinterpret_cast<const void*>(kernel), what)) return rc;
-    kernel<<<unsigned(grid), kHeadThreads, kLdsBytes, stream>>>(a);
+    if (const int rc = reserve_lds(reinterpret_cast<const void*>(kernel), kProductLds, what)) return rc;
+    kernel<<<unsigned(grid), kHeadThreads, kProductLds, stream>>>(a);
     return TRLK_OK;
 }
 
@@ -506,6 +900,16 @@ struct Numbers {
     int32_t steps;
     double a, b, c, eps;
 };
+
+template <int DT, int MP>
+int run_narrow(const Mat* mats, int n, int64_t chunks, const Numbers& num, hipStream_t stream, const char* what) {
+    constexpr int kBytes = 4 * MP * (MP + 1) * 8;
+    if (const int rc = reserve_lds(reinterpret_cast<const void*>(narrow_steps_kernel<MP>), kBytes, what)) return rc;
+    gram_kernel<DT, MP><<<unsigned(chunks), kThreads, 0, stream>>>(mats, n);
+    narrow_steps_kernel<MP><<<unsigned(n), kThreads, kBytes, stream>>>(mats, num.steps, num.a, num.b, num.c, num.eps);
+    narrow_apply_kernel<DT, MP><<<unsigned(chunks), kThreads, 0, stream>>>(mats, n);
+    return TRLK_OK;
+}
 
 template <int DT>
 int run_group(const Group& group, const trlk_muon_matrix* x, const trlk_muon_group* groups, const Numbers& num, char* ws, hipStream_t stream, const char* what) {
@@ -537,22 +941,25 @@ int run_group(const Group& group, const trlk_muon_matrix* x, const trlk_muon_gro
             const double ratio = double(y.rows) / double(y.cols);
             e.stretch = float(g.adjust == TRLK_MUON_MATCH_ADAMW ? 0.2 * sqrt(double(e.n)) : sqrt(ratio > 1.0 ? ratio : 1.0));
         }
-        const int64_t down = ceil_div(e.m, BN);
+        const int64_t down = ceil_div(e.m, BM);
         e.first_chunk = uint32_t(chunks), e.first_turn = uint32_t(turns), e.first_half = uint32_t(halves), e.first_tile = uint32_t(tiles);
-        chunks += ceil_div(int64_t(e.m) * e.n, kChunk);
+        chunks += group.narrow ? ceil_div(e.n, kSpan) : ceil_div(int64_t(e.m) * e.n, kChunk);
         turns += int64_t(e.mpad / kTurn) * (e.npad / kTurn);
         halves += down * (down + 1) / 2;
-        tiles += down * ceil_div(e.n, BM);
+        tiles += down * ceil_div(e.n, BN);
         if (t.n == kTable || i + 1 == n) {
             table_kernel<<<1, 64, 0, stream>>>(t);
             t.to += t.n;
             t.n = 0;
         }
     }
+    if (group.narrow == 16) return run_narrow<DT, 16>(mats, n, chunks, num, stream, what);
+    if (group.narrow == 32) return run_narrow<DT, 32>(mats, n, chunks, num, stream, what);
+    if (group.narrow == 64) return run_narrow<DT, 64>(mats, n, chunks, num, stream, what);
     momentum_kernel<DT><<<unsigned(chunks), kThreads, 0, stream>>>(mats, n, partial);
     norm_kernel<<<unsigned(n), kThreads, 0, stream>>>(mats, partial, factor, num.eps);
     make_x_kernel<DT><<<unsigned(turns), kThreads, 0, stream>>>(mats, n, factor);
-    ProductArgs a{mats, n, 0, float(num.a), float(num.b), float(num.c)};
+    ProductArgs a{mats, n, 0, 0, 1, float(num.a), float(num.b), float(num.c)};
     for (int s = 0; s < num.steps; ++s) {
         if (const int rc = launch_product<PIECES, kStageA>(a, halves, stream, what)) return rc;
         if (const int rc = launch_product<PIECES, kStageB>(a, halves, stream, what)) return rc;
