@@ -102,6 +102,25 @@ def test_gradient(dtype, tokens):
         assert torch.equal(grad, again)
 
 
+@pytest.mark.parametrize("tokens,vocab", [(1024, 300), (1025, 300), (8191, 1 << 20), (8193, (1 << 20) - 1), (32768, 1 << 18), (32768, (1 << 20) - 1),
+                                          (32769, 1000), (40000, 3), (70000, 1 << 21), (5000, 1 << 21)])
+def test_sorted_by_one_workgroup_or_many(tokens, vocab):
+    """Every way the tokens are brought into order, with ids all over the table, rare ones and very common ones."""
+    import trl_amd
+
+    gen = torch.Generator(device=DEV).manual_seed(vocab % 1000)
+    width = 11
+    ids = ((vocab - 1.0) ** torch.rand((tokens,), generator=gen, device=DEV, dtype=torch.float64)).long().clamp(0, vocab - 1)
+    ids[::3] = torch.randint(0, vocab, ids[::3].shape, generator=gen, device=DEV)
+    ids[-1], ids[1] = vocab - 1, 0
+    g = torch.randn((tokens, width), generator=gen, device=DEV)
+    grad = trl_amd.ops.embedding_bwd(g, ids, vocab, 0.5, 1)
+    check_gradient(grad, g, ids, 0.5, 1)
+    held = torch.randn((vocab, width), generator=gen, device=DEV)
+    was = held.clone()
+    check_gradient(trl_amd.embedding_grad_(held, g, ids.int(), scale=0.5), g, ids, 0.5, None, was)
+
+
 @pytest.mark.parametrize("dtype,into", [("bf16", "bf16"), ("bf16", "fp32"), ("fp16", "fp16"), ("fp16", "fp32"), ("fp32", "fp32")])
 @pytest.mark.parametrize("tokens", [1, 300, 3000, 9000])
 def test_added_gradient(dtype, into, tokens):

@@ -127,6 +127,19 @@ def test_many_matrices_in_one_call(dtype):
 
 
 @pytest.mark.parametrize("dtype", list(DTYPES))
+@pytest.mark.parametrize("shapes", [[(1703, 1801)] * 5 + [(1801, 1703)] * 4, [(1150, 700), (700, 1150), (2100, 90), (90, 2100), (900, 900)]])
+def test_larger_matrices(dtype, shapes):
+    """Launches of as many 256 x 256 tiles as there are CUs, and of few."""
+    import trl_amd
+
+    gen = torch.Generator(device=DEV).manual_seed(4)
+    each = [(torch.randn((s[0], 200), generator=gen, device=DEV) @ torch.randn((200, s[1]), generator=gen, device=DEV) * 0.3 + torch.randn(s, generator=gen, device=DEV)).to(DTYPES[dtype])
+            for s in shapes]
+    for u, x in zip(each, trl_amd.orthogonalize(each)):
+        check(x, u)
+
+
+@pytest.mark.parametrize("dtype", list(DTYPES))
 def test_other_numbers(dtype):
     import trl_amd
 

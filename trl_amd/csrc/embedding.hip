@@ -8,6 +8,10 @@
 // matter of chance, and in 16 bits round at every addition.  So the tokens are sorted by id (a stable radix sort of (id, position)
 // pairs, 9 bits a pass at most): the rows of one id are neighbours in the order of their positions, one workgroup adds them up in
 // registers and writes the table's row once.
+#include <algorithm>
+#include <mutex>
+#include <vector>
+
 #include "common.hpp"
 
 namespace trlk {
@@ -123,7 +127,7 @@ struct KeyArgs {
 };
 
 constexpr int kMaxDigit = 9, kBins = 1 << kMaxDigit;  // bits of a pass
-constexpr int kSortRows = 16;                         // tokens of a lane
+constexpr int kSortRows = 4;                          // tokens of a lane: a wave's ranks take 0.5 us a row
 constexpr int kSortWaves = kThreads / kWave;
 constexpr int kSortTile = kThreads * kSortRows;       // of a workgroup; a wave takes consecutive ones
 
@@ -137,14 +141,19 @@ struct SortArgs {
 };
 
 // Lanes of the wave with the same digit, as a mask.
+template <int MOST>
 __device__ __forceinline__ uint64_t peers(uint32_t digit, int bits) {
-    uint64_t mask = ~uint64_t(0);
-    for (int b = 0; b < bits; ++b) {
-        const bool one = (digit >> b) & 1u;
-        const uint64_t ones = __ballot(one);
-        mask &= one ? ones : ~ones;
+    uint32_t lo = ~0u, hi = ~0u;
+#pragma unroll
+    for (int b = 0; b < MOST; ++b) {
+        if (b < bits) {  // (uniform)
+            const uint32_t one = uint32_t(int32_t(digit << (31 - b)) >> 31);  // the bit in all places
+            const uint64_t ones = __ballot(one != 0u);
+            lo &= ~(uint32_t(ones) ^ one);
+            hi &= ~(uint32_t(ones >> 32) ^ one);
+        }
     }
-    return mask;
+    return uint64_t(hi) << 32 | lo;
 }
 
 // Ranks of a wave's tokens (kSortRows rows of 64, in order) among those of the wave with the same digit; `count` (LDS, the wave's
@@ -158,7 +167,7 @@ __device__ __forceinline__ void wave_ranks(const uint32_t (&key)[kSortRows], int
         if (uint32_t(r) < n_rows) {  // (uniform in the wave)
             const bool live = uint32_t(r * kWave + lane) < last;
             const uint32_t digit = (key[r] >> shift) & low;
-            const uint64_t same = peers(digit, bits) & __ballot(live);
+            const uint64_t same = peers<kMaxDigit>(digit, bits) & __ballot(live);
             const uint16_t before = count[digit];
             __builtin_amdgcn_wave_barrier();
             rank[r] = before + uint32_t(__popcll(same & ((uint64_t(1) << lane) - 1)));
@@ -267,20 +276,123 @@ __global__ __launch_bounds__(kThreads) void sort_place_kernel(SortArgs a) {
     }
 }
 
-// ---- the table's gradient ---------------------------------------------------------------------------------------------
-__global__ __launch_bounds__(kThreads) void zero_kernel(u32x4* p, int64_t vecs, uint8_t* tail, int bytes) {
-    const u32x4 z = {0, 0, 0, 0};
-    const int64_t base = int64_t(blockIdx.x) * kItems + threadIdx.x;
-    for (int64_t at = base; at < vecs; at += int64_t(gridDim.x) * kItems) {
+// ---- up to 8192 tokens: sorted by one workgroup, in its LDS -----------------------------------------------------------------
+// Two passes of up to 10 bits.  The first one's result is what the second needs, the upper digit and the position (13 bits), one word a token; the
+// ids themselves are looked up again at the end.  A wave takes consecutive tokens, 8 rows of 64 at most.  Bound by the ranks' instructions
+// on one CU: 8192 tokens, 18 bits 23 us, with six launches of the kernels above 28 and their gaps.
+constexpr int kOneThreads = 1024, kOneWaves = kOneThreads / kWave;
+constexpr int kOneRows = 8, kOneBits = 10;
+
+struct OneArgs {
+    KeyArgs source;
+    uint32_t *key, *at;
+    uint32_t n;
+    int32_t bits;  // of a pass
+};
+constexpr int one_lds_bytes(int bits) { return kOneRows * kOneThreads * 4 + (kOneWaves * 2 << bits); }
+
+__global__ __launch_bounds__(kOneThreads) void sort_one_kernel(OneArgs a) {
+    extern __shared__ __attribute__((aligned(16))) char smem[];
+    uint32_t* words = reinterpret_cast<uint32_t*>(smem);
+    uint16_t* counts = reinterpret_cast<uint16_t*>(smem + kOneRows * kOneThreads * 4);  // [wave][bin]
+    __shared__ uint32_t part[kOneWaves];
+    const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave, n_bins = 1 << a.bits;
+    const uint32_t rows = (a.n + kOneThreads - 1) / kOneThreads, begin = wave * rows * kWave;
+    const uint32_t left = begin < a.n ? a.n - begin : 0u, low = uint32_t(n_bins) - 1u;
+    uint32_t word[kOneRows], rank[kOneRows];
+    volatile uint16_t* mine = counts + wave * n_bins;
+#pragma unroll 1
+    for (int pass = 0; pass < 2; ++pass) {
+        for (int b = threadIdx.x; b < kOneWaves * n_bins / 2; b += kOneThreads) reinterpret_cast<uint32_t*>(counts)[b] = 0;
 #pragma unroll
-        for (int j = 0; j < kUnroll; ++j)
-            if (at + j * kThreads < vecs) __builtin_nontemporal_store(z, p + at + j * kThreads);
+        for (int r = 0; r < kOneRows; ++r) {
+            const uint32_t i = r * kWave + lane;
+            word[r] = 0;
+            if (uint32_t(r) < rows && i < left) word[r] = pass == 0 ? a.source.key(begin + i) : words[begin + i];
+        }
+        __syncthreads();
+#pragma unroll
+        for (int r = 0; r < kOneRows; ++r) {
+            if (uint32_t(r) < rows) {
+                const bool live = uint32_t(r * kWave + lane) < left;
+                const uint32_t digit = pass == 0 ? word[r] & low : word[r] >> 13;
+                const uint64_t same = peers<kOneBits>(digit, a.bits) & __ballot(live);
+                const uint16_t before = mine[digit];
+                __builtin_amdgcn_wave_barrier();
+                rank[r] = before + uint32_t(__popcll(same & ((uint64_t(1) << lane) - 1)));
+                if (live && (same >> lane) == 1) mine[digit] = uint16_t(before + __popcll(same));  // (the last of them)
+                __builtin_amdgcn_wave_barrier();
+            }
+        }
+        __syncthreads();
+        // exclusive sums, bin by bin and wave by wave (all under 32768)
+        uint32_t sum = 0;
+        if (int(threadIdx.x) < n_bins)
+#pragma unroll
+            for (int w = 0; w < kOneWaves; ++w) sum += counts[w * n_bins + threadIdx.x];
+        uint32_t upto = sum;
+#pragma unroll
+        for (int o = 1; o < kWave; o <<= 1) {
+            const uint32_t y = __shfl_up(upto, o);
+            if (lane >= o) upto += y;
+        }
+        if (lane == kWave - 1) part[wave] = upto;
+        __syncthreads();
+        uint32_t to = upto - sum;
+        for (int w = 0; w < wave; ++w) to += part[w];
+        if (int(threadIdx.x) < n_bins)
+#pragma unroll
+            for (int w = 0; w < kOneWaves; ++w) {
+                const uint32_t c = counts[w * n_bins + threadIdx.x];
+                counts[w * n_bins + threadIdx.x] = uint16_t(to);
+                to += c;
+            }
+        __syncthreads();
+        KeyArgs quiet = a.source;
+        quiet.flag = nullptr;  // (raised before)
+#pragma unroll
+        for (int r = 0; r < kOneRows; ++r) {
+            const uint32_t i = r * kWave + lane;
+            if (uint32_t(r) < rows && i < left) {
+                if (pass == 0) {
+                    words[mine[word[r] & low] + rank[r]] = word[r] >> a.bits << 13 | (begin + i);
+                } else {
+                    const uint32_t place = mine[word[r] >> 13] + rank[r], at = word[r] & 0x1fffu;
+                    a.key[place] = quiet.key(at);
+                    a.at[place] = at;
+                }
+            }
+        }
+        __syncthreads();
     }
-    if (blockIdx.x == 0 && int(threadIdx.x) < bytes) tail[threadIdx.x] = 0;
 }
 
+// ---- the table's zeros --------------------------------------------------------------------------------------------------
+// 1.24 GB 214 us (5.8 TB/s); in workgroups of 1024, beside the sort, 250.
+struct ZeroArgs {
+    u32x4* p;
+    int64_t vecs;
+    uint8_t *head, *tail;  // what lies before and behind the whole vectors
+    int32_t head_bytes, tail_bytes;
+};
+__global__ __launch_bounds__(kThreads) void zero_kernel(ZeroArgs z) {
+    const u32x4 zero = {0, 0, 0, 0};
+    for (int64_t at = int64_t(blockIdx.x) * kItems + threadIdx.x; at < z.vecs; at += int64_t(gridDim.x) * kItems) {
+#pragma unroll
+        for (int j = 0; j < kUnroll; ++j)
+            if (at + j * kThreads < z.vecs) __builtin_nontemporal_store(zero, z.p + at + j * kThreads);
+    }
+    if (blockIdx.x == 0) {
+        if (int(threadIdx.x) < z.head_bytes) z.head[threadIdx.x] = 0;
+        if (int(threadIdx.x) < z.tail_bytes) z.tail[threadIdx.x] = 0;
+    }
+}
+
+// ---- the table's gradient ---------------------------------------------------------------------------------------------
 struct GradArgs {
     const uint32_t *key, *at;  // sorted
+    float* part;               // of the chunks of kChunk places that one id has to itself: their sums [chunk][cols]
+    KeyArgs source;            // (unsorted: direct_kernel)
     const void* g;
     void* dw;
     int64_t ldg, ldw;
@@ -301,56 +413,192 @@ __device__ __forceinline__ void store8(typename Elem<DT>::type* p, const float (
     for (int k = 0; k < 8; k += Elem<DT>::EPV) *reinterpret_cast<u32x4_u*>(p + k) = Elem<DT>::pack(x + k);
 }
 
-// One workgroup for each sorted place where an id begins (the others return at once), and for 2048 columns.
-template <int GDT, int ODT, bool ADD>
-__global__ __launch_bounds__(kThreads) void grad_rows_kernel(GradArgs a) {
-    typedef typename Elem<GDT>::type TG;
-    typedef typename Elem<ODT>::type TO;
-    const int lane = threadIdx.x & (kWave - 1);
-    const int col = (blockIdx.y * kThreads + threadIdx.x) * 8;
-    for (uint32_t i = blockIdx.x; i < a.n; i += gridDim.x) {
-        const uint32_t key = a.key[i];
-        if (key >= a.vocab) return;  // (all further ones, too)
-        if (i > 0 && a.key[i - 1] == key) continue;
-        uint32_t end = i + 1;
-        while (true) {
-            const uint64_t other = __ballot(end + lane >= a.n || a.key[end + lane] != key);
-            if (other) {
-                end += uint32_t(__builtin_ctzll(other));
-                break;
-            }
-            end += kWave;
-        }
-        if (col >= a.cols) continue;
-        const TG* g = static_cast<const TG*>(a.g) + col;
-        TO* out = static_cast<TO*>(a.dw) + int64_t(key) * a.ldw + col;
-        float sum[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-        if (col + 8 <= a.cols) {
-#pragma unroll 4
-            for (uint32_t j = i; j < end; ++j) {
-                float x[8];
-                load8<GDT>(g + int64_t(a.at[j]) * a.ldg, x);
+constexpr int kChunk = 16;
+constexpr int kVecs = 4;  // vectors of a lane at most
+
+// A wave's columns: V vectors of 8 a lane, 512 apart.  The row's last vector, where it is cut, is read from 8 before the end and what the one before
+// it has, too, is not stored: no lane walks over its rows entry by entry.  (Rows of fewer than 8: NARROW.)
+template <int V>
+struct Columns {
+    int32_t from[V], skip[V];  // skip 8: nothing
+    __device__ __forceinline__ Columns(int cols, int first, int lane) {
 #pragma unroll
-                for (int k = 0; k < 8; ++k) sum[k] += x[k];
-            }
-            float was[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-            if constexpr (ADD) load8<ODT>(out, was);
-#pragma unroll
-            for (int k = 0; k < 8; ++k) sum[k] = ADD ? fmaf(sum[k], a.scale, was[k]) : sum[k] * a.scale;
-            store8<ODT>(out, sum);
-        } else {
-            const int left = a.cols - col;
-            for (uint32_t j = i; j < end; ++j) {
-                const TG* row = g + int64_t(a.at[j]) * a.ldg;
-#pragma unroll
-                for (int k = 0; k < 8; ++k)
-                    if (k < left) sum[k] += Elem<GDT>::load1(row + k);
-            }
-#pragma unroll
-            for (int k = 0; k < 8; ++k)
-                if (k < left) Elem<ODT>::store1(out + k, ADD ? fmaf(sum[k], a.scale, Elem<ODT>::load1(out + k)) : sum[k] * a.scale);
+        for (int v = 0; v < V; ++v) {
+            const int col = first + v * 512 + lane * 8;
+            from[v] = max(0, min(col, cols - 8));
+            skip[v] = min(8, max(0, col - max(0, cols - 8)));
         }
     }
+};
+// eight entries as they lie in memory
+template <int DT>
+struct Raw {
+    u32x4 q[8 / Elem<DT>::EPV];
+    template <bool NARROW>
+    __device__ __forceinline__ void load(const typename Elem<DT>::type* p, int cols) {
+        if constexpr (NARROW) {
+            float x[8];
+#pragma unroll
+            for (int k = 0; k < 8; ++k) x[k] = k < cols ? Elem<DT>::load1(p + k) : 0.f;
+#pragma unroll
+            for (int i = 0; i < 8 / Elem<DT>::EPV; ++i) q[i] = Elem<DT>::pack(x + i * Elem<DT>::EPV);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8 / Elem<DT>::EPV; ++i) q[i] = *reinterpret_cast<const u32x4_u*>(p + i * Elem<DT>::EPV);
+        }
+    }
+    __device__ __forceinline__ void add_to(float (&sum)[8]) const {
+        float x[8];
+#pragma unroll
+        for (int i = 0; i < 8 / Elem<DT>::EPV; ++i) Elem<DT>::unpack(q[i], x + i * Elem<DT>::EPV);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) sum[k] += x[k];
+    }
+};
+
+// sum += rows.  AT: row j is p + at[j] * ld, else p + j * ld.
+template <int DT, int V, bool NARROW, bool AT>
+__device__ __forceinline__ void add_rows(float (&sum)[V][8], uint32_t from, uint32_t to, const uint32_t* at, const void* base, int64_t ld, int cols,
+                                         const Columns<V>& c, int lane) {
+    constexpr int U = V * (DT == TRLK_F32 ? 2 : 1) >= 8 ? 2 : V * (DT == TRLK_F32 ? 2 : 1) >= 4 ? 4 : 8;  // rows in flight
+    const auto* p = static_cast<const typename Elem<DT>::type*>(base);
+    for (uint32_t begin = from; begin < to; begin += kWave) {
+        const uint32_t count = min(uint32_t(kWave), to - begin);
+        uint32_t mine = begin + lane;
+        if constexpr (AT) mine = at[min(mine, to - 1)];
+        for (uint32_t j = 0; j < count; j += U) {
+            Raw<DT> x[U][V];
+#pragma unroll
+            for (int u = 0; u < U; ++u)
+                if (j + u < count) {
+                    const auto* row = p + int64_t(uint32_t(__builtin_amdgcn_readlane(mine, j + u))) * ld;
+#pragma unroll
+                    for (int v = 0; v < V; ++v) x[u][v].template load<NARROW>(row + c.from[v], cols);
+                }
+#pragma unroll
+            for (int u = 0; u < U; ++u)
+                if (j + u < count)
+#pragma unroll
+                    for (int v = 0; v < V; ++v) x[u][v].add_to(sum[v]);
+        }
+    }
+}
+
+// scale * sum into a row of the table's gradient
+template <int ODT, bool ADD, bool NARROW>
+__device__ __forceinline__ void finish_row(typename Elem<ODT>::type* row, int from, int skip, int cols, float (&sum)[8], float scale) {
+    if (skip >= 8) return;
+    auto* out = row + from;
+    if (skip == 0 && !NARROW) {
+        float was[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+        if constexpr (ADD) load8<ODT>(out, was);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) sum[k] = ADD ? fmaf(sum[k], scale, was[k]) : sum[k] * scale;
+        store8<ODT>(out, sum);
+    } else {
+#pragma unroll
+        for (int k = 0; k < 8; ++k)
+            if (NARROW ? k < cols : k >= skip) Elem<ODT>::store1(out + k, ADD ? fmaf(sum[k], scale, Elem<ODT>::load1(out + k)) : sum[k] * scale);
+    }
+}
+
+// Sums of the whole chunks of ids that occur often, a wave each: a token in twenty is the commonest one, and one wave would add its rows one
+// after the other.
+template <int DT, int V, bool NARROW>
+__global__ __launch_bounds__(kThreads) void grad_chunks_kernel(GradArgs a) {
+    const int lane = threadIdx.x & (kWave - 1);
+    const uint32_t wave = __builtin_amdgcn_readfirstlane(blockIdx.x * (kThreads / kWave) + threadIdx.x / kWave), waves = gridDim.x * (kThreads / kWave);
+    const Columns<V> c(a.cols, blockIdx.y * (V * 512), lane);
+    for (uint32_t chunk = wave; chunk < a.n / kChunk; chunk += waves) {
+        const uint32_t from = chunk * kChunk, key = a.key[from];
+        if (key >= a.vocab || a.key[from + kChunk - 1] != key) continue;
+        float sum[V][8] = {};
+        add_rows<DT, V, NARROW, true>(sum, from, from + kChunk, a.at, a.g, a.ldg, a.cols, c, lane);
+#pragma unroll
+        for (int v = 0; v < V; ++v) finish_row<TRLK_F32, false, NARROW>(a.part + int64_t(chunk) * a.cols, c.from[v], c.skip[v], a.cols, sum[v], 1.f);
+    }
+}
+
+// One wave for each sorted place where an id begins (the others are done at once), all of the row's columns in flight: the rows up to the first
+// whole chunk, the chunks' sums, the rows behind the last one.
+template <int GDT, int ODT, bool ADD, int V, bool NARROW>
+__global__ __launch_bounds__(kThreads) void grad_rows_kernel(GradArgs a) {
+    const int lane = threadIdx.x & (kWave - 1);
+    const uint32_t wave = __builtin_amdgcn_readfirstlane(blockIdx.x * (kThreads / kWave) + threadIdx.x / kWave), waves = gridDim.x * (kThreads / kWave);
+    const Columns<V> c(a.cols, blockIdx.y * (V * 512), lane);
+    for (uint32_t i = wave; i < a.n; i += waves) {
+        // the place before (lane 0), its own and those behind
+        const uint32_t place = i + lane;
+        const uint32_t seen = place >= 1 && place - 1 < a.n ? a.key[place - 1] : ~0u;
+        const uint32_t key = __builtin_amdgcn_readlane(seen, 1);
+        if (key >= a.vocab) return;  // (all further ones, too)
+        if (uint32_t(__builtin_amdgcn_readlane(seen, 0)) == key) continue;
+        uint64_t other = __ballot(seen != key) >> 1;
+        uint32_t end = i + (other ? uint32_t(__builtin_ctzll(other)) : kWave - 1);
+        while (other == 0) {
+            other = __ballot(end + lane >= a.n || a.key[min(end + lane, a.n - 1)] != key);
+            end += other ? uint32_t(__builtin_ctzll(other)) : kWave;
+        }
+        const uint32_t first = (i + kChunk - 1) / kChunk, last = end / kChunk;  // whole chunks
+        const uint32_t head = first < last ? first * kChunk : end, tail = first < last ? last * kChunk : end;
+        float sum[V][8] = {};
+        add_rows<GDT, V, NARROW, true>(sum, i, head, a.at, a.g, a.ldg, a.cols, c, lane);
+        if (first < last) add_rows<TRLK_F32, V, NARROW, false>(sum, first, last, nullptr, a.part, a.cols, a.cols, c, lane);
+        add_rows<GDT, V, NARROW, true>(sum, tail, end, a.at, a.g, a.ldg, a.cols, c, lane);
+        auto* row = static_cast<typename Elem<ODT>::type*>(a.dw) + int64_t(key) * a.ldw;
+#pragma unroll
+        for (int v = 0; v < V; ++v) finish_row<ODT, ADD, NARROW>(row, c.from[v], c.skip[v], a.cols, sum[v], a.scale);
+    }
+}
+
+// Up to 1024 tokens need no order: a workgroup for each token looks at all ids, returns if its own occurs before, else lists where it
+// occurs and adds those rows up.  One launch: 256 tokens of 1024 columns 6 us, sorted first 23.
+constexpr int64_t kMostDirect = 1024;
+template <int GDT, int ODT, bool ADD, bool NARROW>
+__global__ __launch_bounds__(kThreads) void grad_direct_kernel(GradArgs a) {
+    __shared__ uint32_t list[kMostDirect];
+    __shared__ uint32_t counts[kThreads / kWave], before[kThreads / kWave];
+    const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
+    const uint32_t t = blockIdx.x;
+    KeyArgs source = a.source;
+    if (threadIdx.x != 0 || blockIdx.y != 0) source.flag = nullptr;
+    const uint32_t key = source.key(t);
+    if (key >= a.vocab) return;
+    source.flag = nullptr;
+    constexpr int R = kMostDirect / kThreads;
+    uint64_t same[R];
+    uint32_t count = 0;
+    bool earlier = false;
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+        const uint32_t i = (wave * R + r) * kWave + lane;
+        const bool is = i < a.n && source.key(i) == key;
+        same[r] = __ballot(is);
+        earlier |= __ballot(is && i < t) != 0;
+        count += uint32_t(__popcll(same[r]));
+    }
+    if (lane == 0) counts[wave] = count, before[wave] = earlier;
+    __syncthreads();
+    uint32_t at = 0, total = 0;
+#pragma unroll
+    for (int w = 0; w < kThreads / kWave; ++w) {
+        if (before[w]) return;  // (the same for all)
+        if (w < wave) at += counts[w];
+        total += counts[w];
+    }
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+        if (same[r] >> lane & 1) list[at + __popcll(same[r] & ((uint64_t(1) << lane) - 1))] = (wave * R + r) * kWave + lane;
+        at += uint32_t(__popcll(same[r]));
+    }
+    __syncthreads();
+    // (a wave's columns are consecutive ones)
+    const int from = (blockIdx.y * (kThreads / kWave) + wave) * 512;
+    if (from >= a.cols) return;
+    const Columns<1> c(a.cols, from, lane);
+    float sum[1][8] = {};
+    add_rows<GDT, 1, NARROW, true>(sum, 0, total, list, a.g, a.ldg, a.cols, c, lane);
+    finish_row<ODT, ADD, NARROW>(static_cast<typename Elem<ODT>::type*>(a.dw) + int64_t(key) * a.ldw, c.from[0], c.skip[0], a.cols, sum[0], a.scale);
 }
 
 // ---- host ------------------------------------------------------------------------------------------------------------
@@ -359,19 +607,66 @@ int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 size_t up16(size_t n) { return (n + 15) / 16 * 16; }
 bool known(int dtype) { return dtype == TRLK_F32 || dtype == TRLK_BF16 || dtype == TRLK_F16; }
 
-size_t sort_bytes(int64_t n) { return 4 * up16(size_t(n) * 4) + up16(size_t(ceil_div(n, kSortTile)) * kBins * 4); }
-
-// Sorted keys and positions, in the workspace.
-void sort_tokens(const KeyArgs& source, int64_t n, char* ws, hipStream_t stream, const uint32_t** keys, const uint32_t** places) {
-    const size_t each = up16(size_t(n) * 4);
-    uint32_t* buf[2][2];
-    for (int i = 0; i < 4; ++i) buf[i / 2][i % 2] = reinterpret_cast<uint32_t*>(ws + i * each);
+int key_bits(int64_t vocab) {
     int bits = 1;
-    while (bits < 32 && (uint64_t(source.vocab) >> bits) != 0) ++bits;  // (the keys go up to `vocab`)
-    const int passes = (bits + kMaxDigit - 1) / kMaxDigit, digit = (bits + passes - 1) / passes;
+    while (bits < 32 && (uint64_t(vocab) >> bits) != 0) ++bits;  // (the keys go up to `vocab`)
+    return bits;
+}
+bool by_one(int64_t n, int64_t vocab) { return n <= kOneRows * kOneThreads && key_bits(vocab) <= 2 * kOneBits; }
+
+// The workspace: sorted keys and positions, the many-workgroup sort's second pair and counts, the chunks' sums.
+struct Layout {
+    size_t each, counts, part, total;
+    Layout(int64_t n, int64_t vocab, int64_t cols) {
+        each = up16(size_t(n) * 4);
+        counts = by_one(n, vocab) ? 0 : 2 * each + up16(size_t(ceil_div(n, kSortTile)) * kBins * 4);
+        part = 2 * each + counts;
+        total = n <= kMostDirect ? 16 : part + up16(size_t(n / kChunk) * size_t(cols) * 4);
+    }
+};
+
+int reserve_lds(const void* kernel, int bytes) {
+    struct Done {
+        const void* kernel;
+        int device, bytes;
+    };
+    static std::mutex guard;
+    static std::vector<Done>& done = *new std::vector<Done>;  // (never destroyed)
+    int device = 0;
+    if (hipGetDevice(&device) != hipSuccess) device = 0;
+    std::lock_guard<std::mutex> lock(guard);
+    for (const Done& d : done)
+        if (d.kernel == kernel && d.device == device && d.bytes >= bytes) return TRLK_OK;
+    const hipError_t e = hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (e != hipSuccess) return fail(int(e), "embedding_bwd: cannot reserve %d bytes of LDS: %s", bytes, hipGetErrorString(e));
+    done.push_back(Done{kernel, device, bytes});
+    return TRLK_OK;
+}
+
+ZeroArgs zero_args(void* to, int64_t bytes) {
+    ZeroArgs z{};
+    char* p = static_cast<char*>(to);
+    const int64_t gap = (16 - int64_t(reinterpret_cast<uintptr_t>(p) & 15)) & 15, head = gap < bytes ? gap : bytes;
+    z.vecs = (bytes - head) / 16;
+    z.p = reinterpret_cast<u32x4*>(p + head);
+    z.head = reinterpret_cast<uint8_t*>(p), z.tail = reinterpret_cast<uint8_t*>(p + head + z.vecs * 16);
+    z.head_bytes = int32_t(head), z.tail_bytes = int32_t(bytes - head - z.vecs * 16);
+    return z;
+}
+int launch_one(const OneArgs& a, hipStream_t stream) {
+    if (const int rc = reserve_lds(reinterpret_cast<const void*>(sort_one_kernel), one_lds_bytes(kOneBits))) return rc;
+    sort_one_kernel<<<1, kOneThreads, one_lds_bytes(a.bits), stream>>>(a);
+    return TRLK_OK;
+}
+
+// Sorted keys and positions by many workgroups.
+void sort_tokens(const KeyArgs& source, int64_t n, char* ws, const Layout& layout, hipStream_t stream, const uint32_t** keys, const uint32_t** places) {
+    uint32_t* buf[2][2];
+    for (int i = 0; i < 4; ++i) buf[i / 2][i % 2] = reinterpret_cast<uint32_t*>(ws + i * layout.each);
+    const int bits = key_bits(source.vocab), passes = (bits + kMaxDigit - 1) / kMaxDigit, digit = (bits + passes - 1) / passes;
     SortArgs a{};
     a.source = source;
-    a.counts = reinterpret_cast<uint32_t*>(ws + 4 * each);
+    a.counts = reinterpret_cast<uint32_t*>(ws + 4 * layout.each);
     a.n = uint32_t(n);
     a.tiles = uint32_t(ceil_div(n, kSortTile));
     for (int p = 0; p < passes; ++p) {
@@ -390,13 +685,33 @@ void sort_tokens(const KeyArgs& source, int64_t n, char* ws, hipStream_t stream,
     *places = a.out_at;
 }
 
+template <int GDT, int ODT, bool ADD, int V, bool NARROW>
+void launch_sorted(const GradArgs& a, hipStream_t stream) {
+    const int64_t y = ceil_div(a.cols, V * 512), most = kMaxGroups / y, waves = kThreads / kWave;
+    const auto grid = [&](int64_t n) { return dim3(unsigned(std::min(ceil_div(n, waves), most)), unsigned(y)); };
+    grad_chunks_kernel<GDT, V, NARROW><<<grid(a.n / kChunk), kThreads, 0, stream>>>(a);
+    grad_rows_kernel<GDT, ODT, ADD, V, NARROW><<<grid(a.n), kThreads, 0, stream>>>(a);
+}
+template <int GDT, int ODT, bool ADD>
+void launch_rows(const GradArgs& a, bool direct, hipStream_t stream) {
+    if (direct) {
+        const dim3 grid(a.n, unsigned(ceil_div(a.cols, kThreads * 8)));
+        if (a.cols < 8) grad_direct_kernel<GDT, ODT, ADD, true><<<grid, kThreads, 0, stream>>>(a);
+        else grad_direct_kernel<GDT, ODT, ADD, false><<<grid, kThreads, 0, stream>>>(a);
+    } else if (a.cols < 8) {
+        launch_sorted<GDT, ODT, ADD, 1, true>(a, stream);
+    } else if (a.cols <= 512) {
+        launch_sorted<GDT, ODT, ADD, 1, false>(a, stream);
+    } else if (a.cols <= 1024) {
+        launch_sorted<GDT, ODT, ADD, 2, false>(a, stream);
+    } else {
+        launch_sorted<GDT, ODT, ADD, kVecs, false>(a, stream);
+    }
+}
 template <int GDT, int ODT>
-void launch_rows(const GradArgs& a, bool add, hipStream_t stream) {
-    const int64_t y = ceil_div(a.cols, kThreads * 8);
-    const int64_t most = kMaxGroups / y;
-    const dim3 grid(unsigned(a.n < most ? a.n : most), unsigned(y));
-    if (add) grad_rows_kernel<GDT, ODT, true><<<grid, kThreads, 0, stream>>>(a);
-    else grad_rows_kernel<GDT, ODT, false><<<grid, kThreads, 0, stream>>>(a);
+void launch_rows(const GradArgs& a, bool direct, bool add, hipStream_t stream) {
+    if (add) launch_rows<GDT, ODT, true>(a, direct, stream);
+    else launch_rows<GDT, ODT, false>(a, direct, stream);
 }
 
 }  // namespace
@@ -433,7 +748,7 @@ extern "C" int trlk_embedding_fwd(const void* d_weight, int dtype, int64_t vocab
 
 extern "C" size_t trlk_embedding_bwd_workspace_bytes(int64_t n, int64_t vocab, int64_t cols) {
     if (n <= 0 || n > kMaxTokens || vocab < 0 || vocab > kMaxVocab || cols < 0 || cols > kMaxCols) return 0;
-    return sort_bytes(n);
+    return Layout(n, vocab, cols).total;
 }
 
 extern "C" int trlk_embedding_bwd(const void* d_grad, int dtype, int64_t n, int64_t cols, int64_t grad_stride, const void* d_ids, int32_t id_bits,
@@ -454,27 +769,34 @@ extern "C" int trlk_embedding_bwd(const void* d_grad, int dtype, int64_t n, int6
     TRLK_REQUIRE(n == 0 || (d_workspace && workspace_bytes >= trlk_embedding_bwd_workspace_bytes(n, vocab, cols) && aligned_to(d_workspace, 16)),
                  TRLK_ERR_WORKSPACE, "embedding_bwd: workspace too small or misaligned");
     const hipStream_t stream = static_cast<hipStream_t>(stream_);
+    const bool direct = n <= kMostDirect, one = !direct && by_one(n, vocab);
+    const KeyArgs source{Ids{d_ids, id_bits == 64}, vocab, padding_idx, d_error_flag};
+    const Layout layout(n, vocab, cols);
+    char* ws = static_cast<char*>(d_workspace);
+    GradArgs a{};
     if (!accumulate) {
-        char* p = static_cast<char*>(d_dweight);
-        const int64_t bytes = vocab * cols * int64_t(elem_size(out_dtype));
-        // (whole vectors from the first aligned address on; what lies before and behind it goes with the last launch argument)
-        const int64_t head = (16 - int64_t(reinterpret_cast<uintptr_t>(p) & 15)) & 15;
-        const int64_t first = head < bytes ? head : bytes, vecs = (bytes - first) / 16, tail = bytes - first - vecs * 16;
-        if (first) zero_kernel<<<1, kThreads, 0, stream>>>(nullptr, 0, reinterpret_cast<uint8_t*>(p), int(first));
-        const int64_t need = ceil_div(vecs, kItems);
-        if (vecs || tail)
-            zero_kernel<<<unsigned(need < 1 ? 1 : need < kMaxGroups ? need : kMaxGroups), kThreads, 0, stream>>>(
-                reinterpret_cast<u32x4*>(p + first), vecs, reinterpret_cast<uint8_t*>(p + first + vecs * 16), int(tail));
+        const ZeroArgs z = zero_args(d_dweight, vocab * cols * int64_t(elem_size(out_dtype)));
+        const int64_t need = std::max<int64_t>(1, ceil_div(z.vecs, kItems));
+        zero_kernel<<<unsigned(std::min(need, kMaxGroups)), kThreads, 0, stream>>>(z);
     }
     if (n == 0) return launch_status("embedding_bwd");
-    GradArgs a{};
-    sort_tokens(KeyArgs{Ids{d_ids, id_bits == 64}, vocab, padding_idx, d_error_flag}, n, static_cast<char*>(d_workspace), stream, &a.key, &a.at);
+    if (one) {
+        const int digit = (key_bits(vocab) + 1) / 2;
+        const OneArgs o{source, reinterpret_cast<uint32_t*>(ws), reinterpret_cast<uint32_t*>(ws + layout.each), uint32_t(n), digit};
+        if (const int rc = launch_one(o, stream)) return rc;
+        a.key = o.key, a.at = o.at;
+    } else if (!direct) {
+        sort_tokens(source, n, ws, layout, stream, &a.key, &a.at);
+    }
+    a.source = source;
+    a.part = reinterpret_cast<float*>(ws + layout.part);
     a.g = d_grad, a.dw = d_dweight, a.ldg = grad_stride, a.ldw = out_stride;
     a.n = uint32_t(n), a.vocab = uint32_t(vocab), a.cols = int32_t(cols), a.scale = scale;
-    if (dtype == TRLK_F32) launch_rows<TRLK_F32, TRLK_F32>(a, accumulate != 0, stream);
-    else if (dtype == TRLK_BF16 && out_dtype == TRLK_BF16) launch_rows<TRLK_BF16, TRLK_BF16>(a, accumulate != 0, stream);
-    else if (dtype == TRLK_BF16) launch_rows<TRLK_BF16, TRLK_F32>(a, accumulate != 0, stream);
-    else if (out_dtype == TRLK_F16) launch_rows<TRLK_F16, TRLK_F16>(a, accumulate != 0, stream);
-    else launch_rows<TRLK_F16, TRLK_F32>(a, accumulate != 0, stream);
+    const bool add = accumulate != 0;
+    if (dtype == TRLK_F32) launch_rows<TRLK_F32, TRLK_F32>(a, direct, add, stream);
+    else if (dtype == TRLK_BF16 && out_dtype == TRLK_BF16) launch_rows<TRLK_BF16, TRLK_BF16>(a, direct, add, stream);
+    else if (dtype == TRLK_BF16) launch_rows<TRLK_BF16, TRLK_F32>(a, direct, add, stream);
+    else if (out_dtype == TRLK_F16) launch_rows<TRLK_F16, TRLK_F16>(a, direct, add, stream);
+    else launch_rows<TRLK_F16, TRLK_F32>(a, direct, add, stream);
     return launch_status("embedding_bwd");
 }

@@ -34,8 +34,6 @@ typedef u32x2 u32x2_u __attribute__((aligned(2)));
 constexpr int kThreads = 256;
 constexpr int kChunk = 8192;       // entries of a workgroup of the momentum's pass
 constexpr int kTurn = 64;          // rows and columns of a tile of the pass that makes X
-constexpr int kLdsBytes = 2 * kDenseStage;
-constexpr int cmax_lds(int a, int b) { return a > b ? a : b; }
 constexpr float kUnitX = 16384.f, kUnitA = 8192.f;  // X and A, B are held times these
 constexpr int64_t kMostRows = 32768, kMostCols = int64_t(1) << 22, kMostEntries = int64_t(1) << 34;
 constexpr size_t kGroupBytes = size_t(1) << 33;  // of workspace, unless one matrix needs more
@@ -50,7 +48,7 @@ struct Mat {
     int32_t m, n, mpad, npad;
     float lr, stretch, weight_decay, beta, rest;  // rest: 1 - beta
     int32_t nesterov, tall, pieces;               // tall: p is n x m
-    uint32_t first_chunk, first_turn, first_half, first_tile;  // workgroups of the four kinds of launches
+    uint32_t first_chunk, first_turn, first_half, first_tile, first_small_half, first_small;  // pieces of the kinds of launches
     __device__ __forceinline__ int64_t plane() const { return int64_t(mpad) * npad; }
     __device__ __forceinline__ int64_t square() const { return int64_t(mpad) * mpad; }
     __device__ __forceinline__ uint16_t* buffer(int i) const { return x + 2 * i * plane(); }
@@ -336,12 +334,140 @@ __device__ __forceinline__ void finish4(const Mat& e, int64_t at, int left, f32x
     }
 }
 
-// The transposed part of a symmetric result: a wave's 128 x 64 entries go through LDS of its own, 64 rows of 128 (and 8 of padding against bank
-// conflicts), and come back with eight neighbours of the other side a lane, by the transpose loads: lane t of a group of 16 points at the
+// A workgroup's tile of a product.  Big: 256 x 256 with the loop of the lm_head's products, 8 waves.
+struct BigTile {
+    static constexpr int kRows = BM, kCols = BN, kThreads = kHeadThreads, kWaveRows = WM, kWaveCols = WN, kI = MI, kJ = NI, kLds = 2 * kDenseStage;
+    static __device__ __forceinline__ int wave_row(int wave) { return wave_m(wave) * WM; }
+    static __device__ __forceinline__ int wave_col(int wave) { return wave_n(wave) * WN; }
+    template <bool BKM, bool TURNED, typename Runs>
+    static __device__ __forceinline__ void product(const Operand A, int m0, const Operand B, int n0, int K, f32x4 (&acc)[kI][kJ], char* smem, Runs runs) {
+        gemm_tile_nt_direct<TRLK_F16, BKM, NoLeftKm, Runs, TURNED>(A, m0, B, n0, K, acc, smem, NoLeftKm{}, runs);
+    }
+};
+// Small: 128 x 128, 4 waves of 64 x 64, for launches whose big tiles would leave CUs idle: four times the tiles, each with a quarter of the
+// work, two on a CU.  Bound by the LDS: a step of 64 k moves 96 KB in and out of it for 512 cycles of MFMAs, and takes 0.58 us with one tile on a CU
+// and 0.54 with two (165 and 180 GB/s a CU).  Four stages instead of two, which leave room for one tile only, and tiles that come
+// through registers two steps ahead were no faster (0.61 and 0.66 us).  Layouts are those of the big tile's loop; a k-major stage has
+// 64 k rows of 256 bytes.
+struct SmallTile {
+    static constexpr int kRows = 128, kCols = 128, kThreads = 256, kWaveRows = 64, kWaveCols = 64, kI = 4, kJ = 4;
+    static constexpr int kStages = 2, kHalf = kRows * kRowBytes, kStage = 2 * kHalf, kLds = kStages * kStage, kLoads = kHalf / 1024 / 4;
+    static __device__ __forceinline__ int wave_row(int wave) { return (wave >> 1) * 64; }
+    static __device__ __forceinline__ int wave_col(int wave) { return (wave & 1) * 64; }
+    template <bool BKM, bool TURNED, typename Runs>
+    static __device__ __forceinline__ void product(const Operand A, int m0, const Operand B, int n0, int K, f32x4 (&acc)[kI][kJ], char* smem, Runs runs) {
+        const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+        const char* abase = reinterpret_cast<const char*>(A.p + int64_t(m0) * A.ld);
+        const char* bbase = reinterpret_cast<const char*>(BKM ? B.p + n0 : B.p + int64_t(n0) * B.ld);
+        const uint32_t lda = uint32_t(A.ld * 2), ldb = uint32_t(B.ld * 2);
+        uint32_t ao[kLoads], bo[kLoads];
+#pragma unroll
+        for (int j = 0; j < kLoads; ++j) {
+            const int row = (wave + 4 * j) * 8 + lane / kCpr, kc = lane % kCpr ^ tile_swizzle(row);
+            ao[j] = uint32_t(min(row, A.rows - 1 - m0)) * lda + uint32_t(kc * 16);
+            bo[j] = uint32_t(min(row, B.rows - 1 - n0)) * ldb + uint32_t(kc * 16);
+            if constexpr (BKM) {
+                const int krow = (wave + 4 * j) * 4 + (lane >> 4), unit = (lane & 15) ^ ((krow & 3) << 1) ^ (krow & 8);
+                bo[j] = uint32_t(krow) * ldb + uint32_t(unit * 16);
+            }
+        }
+        const uint32_t lds0 = uint32_t(reinterpret_cast<uintptr_t>(smem));
+        const auto issue = [&](int kt) {
+            const int k0 = kt * BK;
+            const char* a = abase + runs.left_plane(k0) + int64_t(runs.inside(k0)) * 2;
+            const char* b = bbase + runs.right_plane(k0) + int64_t(runs.inside(k0)) * (BKM ? B.ld * 2 : 2);
+            const uint32_t to = lds0 + uint32_t(kt % kStages * kStage + wave * 1024);
+#pragma unroll
+            for (int j = 0; j < kLoads; ++j) {
+                DirectLoader<>::transfer(a, ao[j], to + j * 4096);
+                DirectLoader<>::transfer(b, bo[j], to + kHalf + j * 4096);
+            }
+        };
+        const int g = lane >> 4, l15 = lane & 15, wr = wave_row(wave), wc = wave_col(wave);
+        const int koff[2] = {(g ^ tile_swizzle(l15)) * 16, ((4 + g) ^ tile_swizzle(l15)) * 16};
+        int km[kJ];  // k-major: see the big loop
+        if constexpr (BKM) {
+#pragma unroll
+            for (int j = 0; j < kJ; ++j)
+                km[j] = (8 * g + (l15 >> 2)) * 256 + (((wc + j * 16) / 8 + ((l15 & 3) >> 1)) ^ ((l15 >> 2) << 1) ^ ((g & 1) << 3)) * 16 + (l15 & 1) * 8;
+        }
+#pragma unroll
+        for (int i = 0; i < kI; ++i)
+#pragma unroll
+            for (int j = 0; j < kJ; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+        const int nk = K / BK;
+        u32x4 a[2][kI], b[2][kJ];  // the fragments of both halves of a step
+        const auto read = [&](int kt, int ks) {
+            const char* sa = smem + kt % kStages * kStage;
+            const char* sb = sa + kHalf;
+#pragma unroll
+            for (int i = 0; i < kI; ++i) a[ks][i] = *reinterpret_cast<const u32x4*>(sa + (wr + i * 16 + l15) * kRowBytes + koff[ks]);
+#pragma unroll
+            for (int j = 0; j < kJ; ++j) {
+                if constexpr (BKM) {
+                    const uint32_t at = uint32_t(reinterpret_cast<uintptr_t>(sb)) + km[j] + ks * 32 * 256;
+                    const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16(reinterpret_cast<lds_s16x4*>(at));
+                    const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16(reinterpret_cast<lds_s16x4*>(at + 4 * 256));
+                    const u32x2 p = __builtin_bit_cast(u32x2, lo), q = __builtin_bit_cast(u32x2, hi);
+                    b[ks][j] = u32x4{p.x, p.y, q.x, q.y};
+                } else {
+                    b[ks][j] = *reinterpret_cast<const u32x4*>(sb + (wc + j * 16 + l15) * kRowBytes + koff[ks]);
+                }
+            }
+        };
+        const auto multiply = [&](int ks) {
+#pragma unroll
+            for (int i = 0; i < kI; ++i)
+#pragma unroll
+                for (int j = 0; j < kJ; ++j) acc[i][j] = TURNED ? mfma<TRLK_F16>(b[ks][j], a[ks][i], acc[i][j]) : mfma<TRLK_F16>(a[ks][i], b[ks][j], acc[i][j]);
+        };
+        // `later` stages may still be on their way; what this wave has asked the LDS for has arrived
+        const auto landed = [&](int later) {
+            static_assert(2 * kLoads == 8 && kStages == 2, "transfers of a stage");
+            if (later == 1) asm volatile("s_waitcnt vmcnt(8) lgkmcnt(0)" ::: "memory");
+            else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+            __builtin_amdgcn_sched_barrier(0);
+            __builtin_amdgcn_s_barrier();
+            __builtin_amdgcn_sched_barrier(0);
+            asm volatile("" ::: "memory");
+        };
+        for (int kt = 0; kt < kStages && kt < nk; ++kt) issue(kt);
+        landed(min(kStages, nk) - 1);
+        read(0, 0);
+        for (int kt = 0; kt < nk; ++kt) {
+            // (the fences keep the reads ahead of the MFMAs that run meanwhile: left to itself the compiler puts each beside its first use)
+            read(kt, 1);
+            __builtin_amdgcn_sched_barrier(0);
+            multiply(0);
+            __builtin_amdgcn_sched_barrier(0);
+            if (kt + 1 < nk) {
+                // the next stage is there, and everyone has read this one: it is filled again
+                landed(min(kt + kStages - 1, nk - 1) - (kt + 1));
+                if (kt + kStages < nk) issue(kt + kStages);
+                read(kt + 1, 0);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+            multiply(1);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        // (the caller reuses the LDS)
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        __syncthreads();
+    }
+};
+
+// The transposed part of a symmetric result: a wave's entries (128 or 64 x 64) go through LDS of its own, 64 rows of 128 or 64 (and 8 of padding against
+// bank conflicts), and come back with eight neighbours of the other side a lane, by the transpose loads: lane t of a group of 16 points at the
 // 8 bytes with columns 4 (t % 4) .. + 3 of row t / 4 (of 4 rows) and receives column t of those rows.
-constexpr int kMirrorRow = (WM + 8) * 2, kMirrorWave = WN * kMirrorRow;
-constexpr int kProductLds = cmax_lds(kLdsBytes, WGM * WGN * kMirrorWave);
-__device__ __forceinline__ void mirror(char* mine, const u32x2 (&q)[MI][NI], uint16_t* out, int64_t ld, int i0, int j0, int most, int lane) {
+template <typename Tile>
+constexpr int mirror_bytes() { return Tile::kWaveCols * (Tile::kWaveRows + 8) * 2; }
+template <typename Tile>
+constexpr int product_lds() {
+    return Tile::kLds > Tile::kThreads / 64 * mirror_bytes<Tile>() ? Tile::kLds : Tile::kThreads / 64 * mirror_bytes<Tile>();
+}
+template <typename Tile>
+__device__ __forceinline__ void mirror(char* mine, const u32x2 (&q)[Tile::kI][Tile::kJ], uint16_t* out, int64_t ld, int i0, int j0, int most, int lane) {
+    constexpr int MI = Tile::kI, NI = Tile::kJ, kMirrorRow = (Tile::kWaveRows + 8) * 2;
     const int l15 = lane & 15, g = lane >> 4;
 #pragma unroll
     for (int jj = 0; jj < NI; ++jj)
@@ -351,7 +477,7 @@ __device__ __forceinline__ void mirror(char* mine, const u32x2 (&q)[MI][NI], uin
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     const uint32_t base = uint32_t(reinterpret_cast<uintptr_t>(mine)) + (l15 >> 2) * kMirrorRow + (l15 & 3) * 8;
 #pragma unroll
-    for (int jj = 0; jj < WN / 32; ++jj) {
+    for (int jj = 0; jj < NI / 2; ++jj) {
 #pragma unroll
         for (int ii = 0; ii < MI; ++ii) {
             const uint32_t at = base + (jj * 32 + g * 8) * kMirrorRow + ii * 32;
@@ -366,18 +492,21 @@ __device__ __forceinline__ void mirror(char* mine, const u32x2 (&q)[MI][NI], uin
 }
 
 // One tile of A, B, the next X or, DT, the parameter.  PIECES: two pieces to every operand (fp32).
-template <bool PIECES, int STAGE, int DT>
-TRLK_HEAD_KERNEL void product_kernel(ProductArgs args) {
+template <typename Tile, bool PIECES, int STAGE, int DT>
+__global__ __launch_bounds__(Tile::kThreads) __attribute__((amdgpu_waves_per_eu(2, 2))) void product_kernel(
+    ProductArgs args) {
     extern __shared__ __attribute__((aligned(16))) char smem[];
+    constexpr int MI = Tile::kI, NI = Tile::kJ, BM = Tile::kRows, BN = Tile::kCols;
+    constexpr int kWhich = std::is_same_v<Tile, SmallTile> ? 1 : 0;
     typedef std::conditional_t<PIECES, PieceRuns, OneRun> Runs;
     constexpr bool kSquare = STAGE == kStageA || STAGE == kStageB;
-    constexpr uint32_t Mat::*kFirst = kSquare ? &Mat::first_half : &Mat::first_tile;
+    constexpr uint32_t Mat::*kFirst = kWhich ? (kSquare ? &Mat::first_small_half : &Mat::first_small) : kSquare ? &Mat::first_half : &Mat::first_tile;
     const int64_t piece = xcd_piece(blockIdx.x, args.run);
     if (piece >= args.tiles) return;
     const Mat e = args.mats[mat_of<kFirst>(args.mats, args.n, uint32_t(piece))];
     const int index = int(uint32_t(piece) - e.*kFirst);
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int wm = wave_m(wave), wn = wave_n(wave);
+    const int wr = Tile::wave_row(wave), wc = Tile::wave_col(wave);
     const uint16_t* x = e.buffer(args.from);
     const int64_t plane = e.plane(), square = e.square();
     const int down = (e.m + BM - 1) / BM;
@@ -396,15 +525,15 @@ TRLK_HEAD_KERNEL void product_kernel(ProductArgs args) {
         const int k = STAGE == kStageA ? e.npad : e.mpad;
         const Operand q{from, k, e.m};
         const int64_t lo = STAGE == kStageA ? plane : square;
-        gemm_tile_nt_direct<TRLK_F16, false, NoLeftKm, Runs>(q, i0, q, j0, kRuns * k, acc, smem, NoLeftKm{}, runs(k, lo, lo));
+        Tile::template product<false, false, Runs>(q, i0, q, j0, kRuns * k, acc, smem, runs(k, lo, lo));
         uint16_t* out = STAGE == kStageA ? e.a() : e.b();
-        const int iw = i0 + wm * WM, jw = j0 + wn * WN;
+        const int iw = i0 + wr, jw = j0 + wc;
         if (iw >= e.m || jw >= e.m) return;  // (no barrier follows)
         // (neighbours past m, up to mpad, are written as zeros: they are the contraction's padding in the next product)
         u32x2 high[MI][NI], low[PIECES ? MI : 1][PIECES ? NI : 1];
         u32x4 was[2][PIECES ? MI : MI / 2];  // A's entries, a column of blocks ahead
         const auto fetch = [&](int jj) {
-            const uint16_t* p = e.a() + int64_t(min(j0 + acc_col(wn, jj, lane), e.m - 1)) * e.mpad;
+            const uint16_t* p = e.a() + int64_t(min(jw + jj * 16 + (lane & 15), e.m - 1)) * e.mpad;
 #pragma unroll
             for (int ii = 0; ii < MI; ii += 2) {
                 const int at = min(iw + ii * 16 + pair_offset(lane), e.mpad - 8);
@@ -415,7 +544,7 @@ TRLK_HEAD_KERNEL void product_kernel(ProductArgs args) {
         if constexpr (STAGE == kStageB) fetch(0);
 #pragma unroll
         for (int jj = 0; jj < NI; ++jj) {
-            const int j = j0 + acc_col(wn, jj, lane);
+            const int j = jw + jj * 16 + (lane & 15);
             const bool live = j < e.m;
             const int64_t row = int64_t(live ? j : 0) * e.mpad;
             if (STAGE == kStageB && jj + 1 < NI) fetch(jj + 1);
@@ -430,7 +559,7 @@ TRLK_HEAD_KERNEL void product_kernel(ProductArgs args) {
                 }
 #pragma unroll
                 for (int u = 0; u < 2; ++u) {
-                    const int i = i0 + acc_row(wm, ii + u, 0, lane);
+                    const int i = iw + (ii + u) * 16 + (lane >> 4) * 4;
                     f32x4 v, h, l;
                     if constexpr (STAGE == kStageA) {
                         v = acc[ii + u][jj] * (kUnitA / (kUnitX * kUnitX));
@@ -455,9 +584,9 @@ TRLK_HEAD_KERNEL void product_kernel(ProductArgs args) {
             }
         }
         if (tr != tc) {
-            char* mine = smem + wave * kMirrorWave;
-            mirror(mine, high, out, e.mpad, iw, jw, e.m, lane);
-            if constexpr (PIECES) mirror(mine, low, out + square, e.mpad, iw, jw, e.m, lane);
+            char* mine = smem + wave * mirror_bytes<Tile>();
+            mirror<Tile>(mine, high, out, e.mpad, iw, jw, e.m, lane);
+            if constexpr (PIECES) mirror<Tile>(mine, low, out + square, e.mpad, iw, jw, e.m, lane);
         }
     } else {
         const int across = (e.n + BN - 1) / BN;
@@ -473,14 +602,14 @@ TRLK_HEAD_KERNEL void product_kernel(ProductArgs args) {
                 size = lr * e.stretch;
             }
             if (e.tall) {  // neighbours are those of a column of X, which is the parameter's row
-                gemm_tile_nt_direct<TRLK_F16, true, NoLeftKm, Runs>(bs, r0, xs, c0, kRuns * e.mpad, acc, smem, NoLeftKm{}, runs(e.mpad, square, plane));
+                Tile::template product<true, false, Runs>(bs, r0, xs, c0, kRuns * e.mpad, acc, smem, runs(e.mpad, square, plane));
 #pragma unroll
                 for (int jj = 0; jj < NI; ++jj) {
-                    const int c = c0 + acc_col(wn, jj, lane);
+                    const int c = c0 + wc + jj * 16 + (lane & 15);
                     if (c >= e.n) continue;
 #pragma unroll
                     for (int ii = 0; ii < MI; ++ii) {
-                        const int r = r0 + acc_row(wm, ii, 0, lane);
+                        const int r = r0 + wr + ii * 16 + (lane >> 4) * 4;
                         if (r >= e.m) continue;
                         f32x4 v;
 #pragma unroll
@@ -494,14 +623,14 @@ TRLK_HEAD_KERNEL void product_kernel(ProductArgs args) {
                 return;
             }
         }
-        gemm_tile_nt_direct<TRLK_F16, true, NoLeftKm, Runs, true>(bs, r0, xs, c0, kRuns * e.mpad, acc, smem, NoLeftKm{}, runs(e.mpad, square, plane));
-        const int cw = c0 + wn * WN;
+        Tile::template product<true, true, Runs>(bs, r0, xs, c0, kRuns * e.mpad, acc, smem, runs(e.mpad, square, plane));
+        const int cw = c0 + wc;
         if (cw >= e.npad) return;  // (npad is a multiple of a wave's 64 columns: all of them are there or none)
         uint16_t* out = e.buffer(args.from ^ 1);
         // X's own entries, loaded some rows of blocks ahead: a load cannot pass the stores before it, and each would wait for them
-        constexpr int kAhead = 4;
+        constexpr int kAhead = MI < 4 ? MI : 4;
         u32x4 own[kAhead][NI];  // of each pair of blocks, hi and lo
-        const auto row_of = [&](int ii) { return int64_t(min(r0 + acc_turned_row(wm, ii, lane), e.m - 1)) * e.npad + cw + pair_offset(lane); };
+        const auto row_of = [&](int ii) { return int64_t(min(r0 + wr + ii * 16 + (lane & 15), e.m - 1)) * e.npad + cw + pair_offset(lane); };
         const auto fetch = [&](int ii) {
             const uint16_t* p = x + row_of(ii);
 #pragma unroll
@@ -514,7 +643,7 @@ TRLK_HEAD_KERNEL void product_kernel(ProductArgs args) {
         for (int ii = 0; ii < kAhead; ++ii) fetch(ii);
 #pragma unroll
         for (int ii = 0; ii < MI; ++ii) {
-            const int r = r0 + acc_turned_row(wm, ii, lane);
+            const int r = r0 + wr + ii * 16 + (lane & 15);
             const bool live = r < e.m;
             f32x4 v[NI];
 #pragma unroll
@@ -530,7 +659,7 @@ TRLK_HEAD_KERNEL void product_kernel(ProductArgs args) {
             if constexpr (STAGE == kStageLast) {
 #pragma unroll
                 for (int jj = 0; jj < NI; ++jj) {
-                    const int c = c0 + acc_turned_col(wn, jj, lane);
+                    const int c = cw + jj * 16 + (lane >> 4) * 4;
                     if (live && c < e.n) finish4<DT>(e, int64_t(r) * e.n + c, e.n - c, v[jj] * (1.f / kUnitX), decay, size);
                 }
             } else {  // (X's padding is zero, and so is what is made of it)
@@ -883,17 +1012,28 @@ int reserve_lds(const void* kernel, int bytes, const char* what) {
     return TRLK_OK;
 }
 
-template <bool PIECES, int STAGE, int DT = TRLK_F32>
-int launch_product(ProductArgs a, int64_t tiles, hipStream_t stream, const char* what) {
+template <typename Tile, bool PIECES, int STAGE, int DT>
+int launch_tiles(ProductArgs a, int64_t tiles, hipStream_t stream, const char* what) {
+    const auto kernel = product_kernel<Tile, PIECES, STAGE, DT>;
+    constexpr int kBytes = product_lds<Tile>();
+    if (const int rc = reserve_lds(reinterpret_cast<const void*>(kernel), kBytes, what)) return rc;
     // runs of 16 tiles, of fewer where an XCD would get under 8 of them, and the same number for all
     const int64_t want = std::max<int64_t>(1, std::min<int64_t>(16, tiles / 64)), rounds = ceil_div(tiles, 8 * want);
     a.tiles = uint32_t(tiles);
     a.run = uint32_t(ceil_div(tiles, 8 * rounds));
-    const int64_t grid = xcd_grid(tiles, a.run);
-    const auto kernel = product_kernel<PIECES, STAGE, DT>;
-    if (const int rc = reserve_lds(reinterpret_cast<const void*>(kernel), kProductLds, what)) return rc;
-    kernel<<<unsigned(grid), kHeadThreads, kProductLds, stream>>>(a);
+    kernel<<<xcd_grid(tiles, a.run), Tile::kThreads, kBytes, stream>>>(a);
     return TRLK_OK;
+}
+// Big tiles or small ones, whichever are done sooner: a round is 256 big ones or, two on a CU, 512 small ones, which take 0.6 of a big one's time
+// (0.36 if a CU has but one).  bf16: one matrix of 1024 x 1024 478 us with big tiles, 252 with small ones; fp32, 24 matrices of 1150 x 2816: X X^T 468
+// and 431 us, A A 222 and 195, X's own product, 1320 big tiles, 660 and 697; bf16, 56 matrices of a model of width 1024: 126 and 140, 86 and
+// 83, 286 and 319.
+template <bool PIECES, int STAGE, int DT = TRLK_F32>
+int launch_product(const ProductArgs& a, const int64_t (&tiles)[2], hipStream_t stream, const char* what) {
+    const double small = tiles[1] <= 256 ? 0.36 : 0.6 * double(ceil_div(tiles[1], 512));
+    if (small < double(ceil_div(tiles[0], 256)))
+        return launch_tiles<SmallTile, PIECES, STAGE, DT>(a, tiles[1], stream, what);
+    return launch_tiles<BigTile, PIECES, STAGE, DT>(a, tiles[0], stream, what);
 }
 
 struct Numbers {
@@ -919,7 +1059,7 @@ int run_group(const Group& group, const trlk_muon_matrix* x, const trlk_muon_gro
     float* factor = reinterpret_cast<float*>(ws + up256(n * sizeof(Mat)));
     double* partial = reinterpret_cast<double*>(reinterpret_cast<char*>(factor) + up256(n * sizeof(float)));
     char* at = reinterpret_cast<char*>(partial) + up256(size_t(group.chunks) * sizeof(double));
-    int64_t chunks = 0, turns = 0, halves = 0, tiles = 0;
+    int64_t chunks = 0, turns = 0, halves[2] = {0, 0}, tiles[2] = {0, 0};
     MatTable t;
     t.n = 0;
     t.to = mats;
@@ -941,12 +1081,15 @@ int run_group(const Group& group, const trlk_muon_matrix* x, const trlk_muon_gro
             const double ratio = double(y.rows) / double(y.cols);
             e.stretch = float(g.adjust == TRLK_MUON_MATCH_ADAMW ? 0.2 * sqrt(double(e.n)) : sqrt(ratio > 1.0 ? ratio : 1.0));
         }
-        const int64_t down = ceil_div(e.m, BM);
-        e.first_chunk = uint32_t(chunks), e.first_turn = uint32_t(turns), e.first_half = uint32_t(halves), e.first_tile = uint32_t(tiles);
+        e.first_chunk = uint32_t(chunks), e.first_turn = uint32_t(turns), e.first_half = uint32_t(halves[0]), e.first_tile = uint32_t(tiles[0]);
+        e.first_small_half = uint32_t(halves[1]), e.first_small = uint32_t(tiles[1]);
         chunks += group.narrow ? ceil_div(e.n, kSpan) : ceil_div(int64_t(e.m) * e.n, kChunk);
         turns += int64_t(e.mpad / kTurn) * (e.npad / kTurn);
-        halves += down * (down + 1) / 2;
-        tiles += down * ceil_div(e.n, BN);
+        for (int k = 0; k < 2; ++k) {
+            const int64_t side = k ? SmallTile::kRows : BigTile::kRows, down = ceil_div(e.m, side);
+            halves[k] += down * (down + 1) / 2;
+            tiles[k] += down * ceil_div(e.n, side);
+        }
         if (t.n == kTable || i + 1 == n) {
             table_kernel<<<1, 64, 0, stream>>>(t);
             t.to += t.n;
