@@ -46,9 +46,9 @@ def rounded(u, steps=5, coefficients=(A, B, C), eps=1e-7):
     tall = x.shape[-2] > x.shape[-1]
     x = x.mT if tall else x
     x = x / max(float(torch.linalg.vector_norm(x)), eps)
-    for _ in range(steps):
+    for step in range(steps):
         hi = fp16(x, 16384.0)
-        x = hi + fp16(x - hi, 16384.0)
+        x = hi + fp16(x - hi, 16384.0) if step == 0 or step + 1 < steps else hi
         gram = fp16(hi @ hi.mT, 8192.0)
         x = a * x + fp16(b * gram + c * gram @ gram, 8192.0) @ hi
     return x.mT if tall else x

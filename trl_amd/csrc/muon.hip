@@ -10,9 +10,9 @@
 // written twice).  The products run on fp16 operands with fp32 sums.  X is held as two fp16 pieces, x = hi + lo, 22 bits, in units of 2^-14 (its
 // singular values stay under 1.3, so do its entries; the units keep what is 2^-28 of the largest out of fp16's subnormals), A and B in
 // units of 2^-13.  Parameters in 16 bits: the products take X's hi piece and A and B of one piece, and the term a X, which carries the small
-// singular values (they grow by a in each step), all 22 bits.  Against the exact iteration that is off by 1.7e-3 of the result for
-// matrices of independent entries and less where singular values differ by much; with one piece everywhere those cases lose up to 4e-2,
-// with bf16 operands 30 times the fp16 error.  Parameters in fp32: A and B have two pieces, too, and every product is three, lo hi + hi lo +
+// singular values (they grow by a in each step), all 22 bits but for the last step's.  Against the exact iteration that is off by 1.6e-3 of the
+// result for matrices of independent entries and less where singular values differ by much; with one piece everywhere those cases lose up
+// to 4e-2, with bf16 operands 3e-1.  Parameters in fp32: A and B have two pieces, too, and every product is three, lo hi + hi lo +
 // hi hi, which is fp32's precision at a third of the rate.
 #include <math.h>
 
@@ -48,7 +48,7 @@ struct Mat {
     int32_t m, n, mpad, npad;
     float lr, stretch, weight_decay, beta, rest;  // rest: 1 - beta
     int32_t nesterov, tall, pieces;               // tall: p is n x m
-    uint32_t first_chunk, first_turn, first_half, first_tile, first_small_half, first_small;  // pieces of the kinds of launches
+    uint32_t first_chunk, first_turn, first_half[3], first_tile[3];  // pieces of the kinds of launches
     __device__ __forceinline__ int64_t plane() const { return int64_t(mpad) * npad; }
     __device__ __forceinline__ int64_t square() const { return int64_t(mpad) * mpad; }
     __device__ __forceinline__ uint16_t* buffer(int i) const { return x + 2 * i * plane(); }
@@ -68,17 +68,23 @@ __global__ __launch_bounds__(64) void table_kernel(MatTable t) {
     for (int i = threadIdx.x; i < t.n; i += 64) t.to[i] = t.e[i];
 }
 
-// the matrix of workgroup w
-template <uint32_t Mat::*FIRST>
-__device__ __forceinline__ int mat_of(const Mat* e, int n, uint32_t w) {
+// the matrix of piece w
+template <typename F>
+__device__ __forceinline__ int mat_of(const Mat* e, int n, uint32_t w, F first) {
     int lo = 0, hi = n;
     while (hi - lo > 1) {
         const int mid = (lo + hi) >> 1;
-        if (e[mid].*FIRST <= w) lo = mid;
+        if (first(e[mid]) <= w) lo = mid;
         else hi = mid;
     }
     return lo;
 }
+struct FirstChunk {
+    __device__ __forceinline__ uint32_t operator()(const Mat& e) const { return e.first_chunk; }
+};
+struct FirstTurn {
+    __device__ __forceinline__ uint32_t operator()(const Mat& e) const { return e.first_turn; }
+};
 
 // ---- momentum, norms, X ------------------------------------------------------------------------------------------------
 __device__ __forceinline__ float moved(float was, float g, const Mat& e) { return fmaf(e.beta, was, e.rest * g); }
@@ -98,7 +104,7 @@ __device__ __forceinline__ void load8(const typename Elem<DT>::type* p, float (&
 template <int DT>
 __global__ __launch_bounds__(kThreads) void momentum_kernel(const Mat* mats, int n_mats, double* partial) {
     __shared__ double scratch[kThreads / kWave];
-    const Mat e = mats[mat_of<&Mat::first_chunk>(mats, n_mats, blockIdx.x)];
+    const Mat e = mats[mat_of(mats, n_mats, blockIdx.x, FirstChunk{})];
     const int64_t numel = int64_t(e.m) * e.n, begin = int64_t(blockIdx.x - e.first_chunk) * kChunk;
     const auto* g = static_cast<const typename Elem<DT>::type*>(e.g);
     double s = 0.0;
@@ -195,7 +201,7 @@ __device__ __forceinline__ void store_pieces8(uint16_t* hi, int64_t lo_plane, co
 template <int DT>
 __global__ __launch_bounds__(kThreads) void make_x_kernel(const Mat* mats, int n_mats, const float* factor) {
     __shared__ float tile[kTurn][kTurn + 1];
-    const int i = mat_of<&Mat::first_turn>(mats, n_mats, blockIdx.x);
+    const int i = mat_of(mats, n_mats, blockIdx.x, FirstTurn{});
     const Mat e = mats[i];
     const float f = factor[i];
     const auto* g = static_cast<const typename Elem<DT>::type*>(e.g);
@@ -256,6 +262,7 @@ struct ProductArgs {
     const Mat* mats;
     int32_t n, from;  // from: the buffer that holds X
     uint32_t tiles, run;
+    int32_t reads_lo, writes_lo;  // whether X, and the next X, have their lo piece (16 bits: the last one has not)
     float a, b, c;
 };
 
@@ -344,16 +351,21 @@ struct BigTile {
         gemm_tile_nt_direct<TRLK_F16, BKM, NoLeftKm, Runs, TURNED>(A, m0, B, n0, K, acc, smem, NoLeftKm{}, runs);
     }
 };
-// Small: 128 x 128, 4 waves of 64 x 64, for launches whose big tiles would leave CUs idle: four times the tiles, each with a quarter of the
-// work, two on a CU.  Bound by the LDS: a step of 64 k moves 96 KB in and out of it for 512 cycles of MFMAs, and takes 0.58 us with one tile on a CU
-// and 0.54 with two (165 and 180 GB/s a CU).  Four stages instead of two, which leave room for one tile only, and tiles that come
-// through registers two steps ahead were no faster (0.61 and 0.66 us).  Layouts are those of the big tile's loop; a k-major stage has
-// 64 k rows of 256 bytes.
-struct SmallTile {
-    static constexpr int kRows = 128, kCols = 128, kThreads = 256, kWaveRows = 64, kWaveCols = 64, kI = 4, kJ = 4;
+// Small: 128 x 128 or 64 x 64, 4 waves of a quarter each, for launches whose big tiles would leave CUs idle: four or sixteen times the tiles with as
+// much less work, two or four on a CU.  Bound by the LDS: of 128 x 128, a step of 64 k moves 96 KB in and out of it for 512 cycles of MFMAs,
+// and takes 0.58 us with one tile on a CU and 0.54 with two (165 and 180 GB/s a CU).  Four stages instead of two, which leave room for one
+// tile only, and tiles that come through registers two steps ahead were no faster (0.61 and 0.66 us).  Layouts are those of the big tile's
+// loop; a k-major stage has 64 k rows of 256 or 128 bytes.
+template <int SIDE>
+struct SmallTileOf {
+    static constexpr int kRows = SIDE, kCols = SIDE, kThreads = 256, kWaveRows = SIDE / 2, kWaveCols = SIDE / 2, kI = SIDE / 32, kJ = SIDE / 32;
     static constexpr int kStages = 2, kHalf = kRows * kRowBytes, kStage = 2 * kHalf, kLds = kStages * kStage, kLoads = kHalf / 1024 / 4;
-    static __device__ __forceinline__ int wave_row(int wave) { return (wave >> 1) * 64; }
-    static __device__ __forceinline__ int wave_col(int wave) { return (wave & 1) * 64; }
+    static constexpr int kKmRow = SIDE * 2, kKmUnits = SIDE / 8;  // of a k-major stage: bytes and 16-byte units of a k row
+    static __device__ __forceinline__ int wave_row(int wave) { return (wave >> 1) * (SIDE / 2); }
+    static __device__ __forceinline__ int wave_col(int wave) { return (wave & 1) * (SIDE / 2); }
+    // the unit at physical position u of k row r holds logical unit u ^ km_swizzle(r): the eight k rows that two neighbouring groups of 16 lanes
+    // read with a transpose load are spread over all banks (two k rows of 128 bytes lie in the 64 banks side by side)
+    static __device__ __forceinline__ int km_swizzle(int r) { return SIDE == 128 ? ((r & 3) << 1) ^ (r & 8) : (r & 2) ^ ((r & 8) >> 1); }
     template <bool BKM, bool TURNED, typename Runs>
     static __device__ __forceinline__ void product(const Operand A, int m0, const Operand B, int n0, int K, f32x4 (&acc)[kI][kJ], char* smem, Runs runs) {
         const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -367,7 +379,7 @@ struct SmallTile {
             ao[j] = uint32_t(min(row, A.rows - 1 - m0)) * lda + uint32_t(kc * 16);
             bo[j] = uint32_t(min(row, B.rows - 1 - n0)) * ldb + uint32_t(kc * 16);
             if constexpr (BKM) {
-                const int krow = (wave + 4 * j) * 4 + (lane >> 4), unit = (lane & 15) ^ ((krow & 3) << 1) ^ (krow & 8);
+                const int at = (wave + 4 * j) * 64 + lane, krow = at / kKmUnits, unit = at % kKmUnits ^ km_swizzle(krow);
                 bo[j] = uint32_t(krow) * ldb + uint32_t(unit * 16);
             }
         }
@@ -389,7 +401,7 @@ struct SmallTile {
         if constexpr (BKM) {
 #pragma unroll
             for (int j = 0; j < kJ; ++j)
-                km[j] = (8 * g + (l15 >> 2)) * 256 + (((wc + j * 16) / 8 + ((l15 & 3) >> 1)) ^ ((l15 >> 2) << 1) ^ ((g & 1) << 3)) * 16 + (l15 & 1) * 8;
+                km[j] = (8 * g + (l15 >> 2)) * kKmRow + (((wc + j * 16) / 8 + ((l15 & 3) >> 1)) ^ km_swizzle(8 * g + (l15 >> 2))) * 16 + (l15 & 1) * 8;
         }
 #pragma unroll
         for (int i = 0; i < kI; ++i)
@@ -405,9 +417,9 @@ struct SmallTile {
 #pragma unroll
             for (int j = 0; j < kJ; ++j) {
                 if constexpr (BKM) {
-                    const uint32_t at = uint32_t(reinterpret_cast<uintptr_t>(sb)) + km[j] + ks * 32 * 256;
+                    const uint32_t at = uint32_t(reinterpret_cast<uintptr_t>(sb)) + km[j] + ks * 32 * kKmRow;
                     const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16(reinterpret_cast<lds_s16x4*>(at));
-                    const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16(reinterpret_cast<lds_s16x4*>(at + 4 * 256));
+                    const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16(reinterpret_cast<lds_s16x4*>(at + 4 * kKmRow));
                     const u32x2 p = __builtin_bit_cast(u32x2, lo), q = __builtin_bit_cast(u32x2, hi);
                     b[ks][j] = u32x4{p.x, p.y, q.x, q.y};
                 } else {
@@ -423,8 +435,8 @@ struct SmallTile {
         };
         // `later` stages may still be on their way; what this wave has asked the LDS for has arrived
         const auto landed = [&](int later) {
-            static_assert(2 * kLoads == 8 && kStages == 2, "transfers of a stage");
-            if (later == 1) asm volatile("s_waitcnt vmcnt(8) lgkmcnt(0)" ::: "memory");
+            static_assert(kStages == 2, "one later stage");
+            if (later == 1) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(2 * kLoads) : "memory");
             else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
             __builtin_amdgcn_sched_barrier(0);
             __builtin_amdgcn_s_barrier();
@@ -456,7 +468,10 @@ struct SmallTile {
     }
 };
 
-// The transposed part of a symmetric result: a wave's entries (128 or 64 x 64) go through LDS of its own, 64 rows of 128 or 64 (and 8 of padding against
+typedef SmallTileOf<128> SmallTile;
+typedef SmallTileOf<64> TinyTile;
+
+// The transposed part of a symmetric result: a wave's entries (128 or 64 x 64, or 32 x 32) go through LDS of its own, rows of its columns (and 8 of padding against
 // bank conflicts), and come back with eight neighbours of the other side a lane, by the transpose loads: lane t of a group of 16 points at the
 // 8 bytes with columns 4 (t % 4) .. + 3 of row t / 4 (of 4 rows) and receives column t of those rows.
 template <typename Tile>
@@ -497,14 +512,14 @@ __global__ __launch_bounds__(Tile::kThreads) __attribute__((amdgpu_waves_per_eu(
     ProductArgs args) {
     extern __shared__ __attribute__((aligned(16))) char smem[];
     constexpr int MI = Tile::kI, NI = Tile::kJ, BM = Tile::kRows, BN = Tile::kCols;
-    constexpr int kWhich = std::is_same_v<Tile, SmallTile> ? 1 : 0;
+    constexpr int kWhich = std::is_same_v<Tile, TinyTile> ? 2 : std::is_same_v<Tile, SmallTile> ? 1 : 0;
     typedef std::conditional_t<PIECES, PieceRuns, OneRun> Runs;
     constexpr bool kSquare = STAGE == kStageA || STAGE == kStageB;
-    constexpr uint32_t Mat::*kFirst = kWhich ? (kSquare ? &Mat::first_small_half : &Mat::first_small) : kSquare ? &Mat::first_half : &Mat::first_tile;
-    const int64_t piece = xcd_piece(blockIdx.x, args.run);
+        const int64_t piece = xcd_piece(blockIdx.x, args.run);
     if (piece >= args.tiles) return;
-    const Mat e = args.mats[mat_of<kFirst>(args.mats, args.n, uint32_t(piece))];
-    const int index = int(uint32_t(piece) - e.*kFirst);
+    const auto first = [](const Mat& e) { return (kSquare ? e.first_half : e.first_tile)[kWhich]; };
+    const Mat e = args.mats[mat_of(args.mats, args.n, uint32_t(piece), first)];
+    const int index = int(uint32_t(piece) - first(e));
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int wr = Tile::wave_row(wave), wc = Tile::wave_col(wave);
     const uint16_t* x = e.buffer(args.from);
@@ -615,7 +630,7 @@ __global__ __launch_bounds__(Tile::kThreads) __attribute__((amdgpu_waves_per_eu(
 #pragma unroll
                         for (int k = 0; k < 4; ++k) {  // (rows of X's padding are there)
                             const uint16_t* p = x + int64_t(r + k) * e.npad + c;
-                            v[k] = half_at(p) + half_at(p + plane);
+                            v[k] = PIECES || args.reads_lo ? half_at(p) + half_at(p + plane) : half_at(p);
                         }
                         finish4<DT>(e, int64_t(c) * e.m + r, e.m - r, (v * args.a + acc[ii][jj] * scale) * (1.f / kUnitX), decay, size);
                     }
@@ -636,7 +651,7 @@ __global__ __launch_bounds__(Tile::kThreads) __attribute__((amdgpu_waves_per_eu(
 #pragma unroll
             for (int jj = 0; jj < NI; jj += 2) {
                 own[ii % kAhead][jj] = *reinterpret_cast<const u32x4*>(p + jj * 16);
-                own[ii % kAhead][jj + 1] = *reinterpret_cast<const u32x4*>(p + plane + jj * 16);
+                own[ii % kAhead][jj + 1] = PIECES || args.reads_lo ? *reinterpret_cast<const u32x4*>(p + plane + jj * 16) : u32x4{0u, 0u, 0u, 0u};
             }
         };
 #pragma unroll
@@ -677,7 +692,7 @@ __global__ __launch_bounds__(Tile::kThreads) __attribute__((amdgpu_waves_per_eu(
                     const u32x4 h8 = pair_up(h2[0], h2[1]), l8 = pair_up(l2[0], l2[1]);
                     if (live) {
                         *reinterpret_cast<u32x4*>(out + at + jj * 16) = h8;
-                        *reinterpret_cast<u32x4*>(out + plane + at + jj * 16) = l8;
+                        if (PIECES || args.writes_lo) *reinterpret_cast<u32x4*>(out + plane + at + jj * 16) = l8;
                     }
                 }
             }
@@ -693,8 +708,8 @@ __global__ __launch_bounds__(Tile::kThreads) __attribute__((amdgpu_waves_per_eu(
 // little of it: 224 adapters of rank 16 with 9M entries take 0.3 GFLOP).  Bound by the memory, and by launches: three and the tables instead of
 // the 18 of the larger matrices' way.
 constexpr int kNarrow = 64;          // rows at most
-constexpr int kCols = 128;           // columns of u at a time in LDS
-constexpr int kSpan = 4 * kCols;     // and of a workgroup
+constexpr int kCols = 128;           // columns of u at a time in LDS, and of a workgroup that applies T
+constexpr int kSpan = 2 * kCols;     // of one that sums for G
 constexpr int kLine = kCols + 1;
 
 // u of `cols` columns from c0 on as fp32, [row][column] (kLine apart), zero outside; MOVE: the momentum moves on (else it has).
@@ -772,7 +787,7 @@ __global__ __launch_bounds__(kThreads) void gram_kernel(const Mat* mats, int n_m
     constexpr int kTileBytes = MP * kLine * 4, kSumBytes = kSlices > 1 ? kSlices * MP * MP * 8 : 0;
     __shared__ __attribute__((aligned(16))) char smem[kTileBytes > kSumBytes ? kTileBytes : kSumBytes];
     float* tile = reinterpret_cast<float*>(smem);
-    const Mat e = mats[mat_of<&Mat::first_chunk>(mats, n_mats, blockIdx.x)];
+    const Mat e = mats[mat_of(mats, n_mats, blockIdx.x, FirstChunk{})];
     const int chunk = int(blockIdx.x - e.first_chunk), slice = threadIdx.x / kBlocks, block = threadIdx.x % kBlocks;
     const int bi = block / (MP / 4) * 4, bj = block % (MP / 4) * 4;
     double sum[4][4] = {};
@@ -813,30 +828,27 @@ __global__ __launch_bounds__(kThreads) void gram_kernel(const Mat* mats, int n_m
     }
 }
 
-// z = x y + d for symmetric x, y that commute, MP x MP in LDS, d on the diagonal; `x` and `z` may be the same.
+// z = f(x y) for symmetric x, y that commute, MP x MP in LDS; `x` and `z` may be the same.  A lane has a square of entries: 1, 2 x 2 or 4 x 4.
 template <int MP, typename F>
 __device__ __forceinline__ void square_product(const double* x, const double* y, double* z, F f) {
-    constexpr int LD = MP + 1, kBlocks = (MP / 4) * (MP / 4);
-    const int block = threadIdx.x, bi = block / (MP / 4) * 4, bj = block % (MP / 4) * 4;
-    double sum[4][4] = {};
-    if (block < kBlocks) {
-        for (int k = 0; k < MP; ++k) {
-            double p[4], q[4];
+    constexpr int LD = MP + 1, S = MP / 16;
+    const int bi = threadIdx.x / 16 * S, bj = threadIdx.x % 16 * S;
+    double sum[S][S] = {};
+#pragma unroll 8
+    for (int k = 0; k < MP; ++k) {
+        double p[S], q[S];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) p[i] = x[(bi + i) * LD + k], q[i] = y[k * LD + bj + i];
+        for (int i = 0; i < S; ++i) p[i] = x[(bi + i) * LD + k], q[i] = y[k * LD + bj + i];
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
+        for (int i = 0; i < S; ++i)
 #pragma unroll
-                for (int j = 0; j < 4; ++j) sum[i][j] = __builtin_fma(p[i], q[j], sum[i][j]);
-        }
+            for (int j = 0; j < S; ++j) sum[i][j] = __builtin_fma(p[i], q[j], sum[i][j]);
     }
     __syncthreads();
-    if (block < kBlocks) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
+    for (int i = 0; i < S; ++i)
 #pragma unroll
-            for (int j = 0; j < 4; ++j) z[(bi + i) * LD + bj + j] = f(sum[i][j], bi + i, bj + j);
-    }
+        for (int j = 0; j < S; ++j) z[(bi + i) * LD + bj + j] = f(sum[i][j], bi + i, bj + j);
     __syncthreads();
 }
 
@@ -851,7 +863,13 @@ __global__ __launch_bounds__(kThreads) void narrow_steps_kernel(const Mat* mats,
     double* parts = reinterpret_cast<double*>(e.x);
     for (int k = threadIdx.x; k < MP * MP; k += kThreads) {
         double s = 0.0;
-        for (int q = 0; q < chunks; ++q) s += parts[int64_t(q) * MP * MP + k];
+        for (int q = 0; q < chunks; q += 8) {  // (eight loads in flight, added in order)
+            double x[8];
+#pragma unroll
+            for (int u = 0; u < 8; ++u) x[u] = q + u < chunks ? parts[int64_t(q + u) * MP * MP + k] : 0.0;
+#pragma unroll
+            for (int u = 0; u < 8; ++u) s += x[u];
+        }
         G[k / MP * LD + k % MP] = s;
     }
     __syncthreads();
@@ -882,8 +900,8 @@ template <int DT, int MP>
 __global__ __launch_bounds__(kThreads) void narrow_apply_kernel(const Mat* mats, int n_mats) {
     static_assert(kThreads == 2 * kCols, "two lanes a column");
     __shared__ float tile[MP * kLine];
-    const Mat e = mats[mat_of<&Mat::first_chunk>(mats, n_mats, blockIdx.x)];
-    const int chunk = int(blockIdx.x - e.first_chunk), c = threadIdx.x % kCols;
+    const Mat e = mats[mat_of(mats, n_mats, blockIdx.x, FirstTurn{})];
+    const int c0 = int(blockIdx.x - e.first_turn) * kCols, c = threadIdx.x % kCols;
     const int half = __builtin_amdgcn_readfirstlane(threadIdx.x / kCols);
     const double* T = reinterpret_cast<const double*>(e.x) + int64_t((e.n + kSpan - 1) / kSpan) * MP * MP + half * (MP / 2) * MP;
     float decay = 1.f, size = 0.f;
@@ -892,45 +910,42 @@ __global__ __launch_bounds__(kThreads) void narrow_apply_kernel(const Mat* mats,
         decay = float(1.0 - double(lr) * double(e.weight_decay));
         size = lr * e.stretch;
     }
-    for (int c0 = chunk * kSpan; c0 < (chunk + 1) * kSpan && c0 < e.n; c0 += kCols) {
-        __syncthreads();
-        load_u<DT, MP, false>(e, c0, tile);
-        __syncthreads();
-        double u[MP];
+    load_u<DT, MP, false>(e, c0, tile);
+    __syncthreads();
+    double u[MP];
 #pragma unroll
-        for (int k = 0; k < MP; ++k) u[k] = tile[k * kLine + c];
-        __syncthreads();
+    for (int k = 0; k < MP; ++k) u[k] = tile[k * kLine + c];
+    __syncthreads();
 #pragma unroll 2
-        for (int r = 0; r < MP / 2; ++r) {
-            double s = 0.0;
+    for (int r = 0; r < MP / 2; ++r) {
+        double s = 0.0;
 #pragma unroll
-            for (int k = 0; k < MP; ++k) s = __builtin_fma(T[r * MP + k], u[k], s);
-            tile[(half * (MP / 2) + r) * kLine + c] = float(s);
+        for (int k = 0; k < MP; ++k) s = __builtin_fma(T[r * MP + k], u[k], s);
+        tile[(half * (MP / 2) + r) * kLine + c] = float(s);
+    }
+    __syncthreads();
+    const int cols = min(kCols, e.n - c0);
+    if (e.tall) {
+        const int64_t from = int64_t(c0) * e.m;
+        const int count = cols * e.m;
+        for (int i = threadIdx.x * 4; i < count; i += kThreads * 4) {
+            f32x4 x = {0.f, 0.f, 0.f, 0.f};
+            int q = i / e.m, r = i - q * e.m;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                if (i + k < count) x[k] = tile[r * kLine + q];
+                if (++r == e.m) r = 0, ++q;
+            }
+            finish4<DT>(e, from + i, count - i, x, decay, size);
         }
-        __syncthreads();
-        const int cols = min(kCols, e.n - c0);
-        if (e.tall) {
-            const int64_t from = int64_t(c0) * e.m;
-            const int count = cols * e.m;
-            for (int i = threadIdx.x * 4; i < count; i += kThreads * 4) {
-                f32x4 x = {0.f, 0.f, 0.f, 0.f};
-                int q = i / e.m, r = i - q * e.m;
+    } else {
+        for (int i = threadIdx.x; i < e.m * (kCols / 4); i += kThreads) {
+            const int r = i / (kCols / 4), q = i % (kCols / 4) * 4;
+            if (q >= cols) continue;
+            f32x4 x;
 #pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                    if (i + k < count) x[k] = tile[r * kLine + q];
-                    if (++r == e.m) r = 0, ++q;
-                }
-                finish4<DT>(e, from + i, count - i, x, decay, size);
-            }
-        } else {
-            for (int i = threadIdx.x; i < e.m * (kCols / 4); i += kThreads) {
-                const int r = i / (kCols / 4), q = i % (kCols / 4) * 4;
-                if (q >= cols) continue;
-                f32x4 x;
-#pragma unroll
-                for (int k = 0; k < 4; ++k) x[k] = tile[r * kLine + q + k];
-                finish4<DT>(e, int64_t(r) * e.n + c0 + q, cols - q, x, decay, size);
-            }
+            for (int k = 0; k < 4; ++k) x[k] = tile[r * kLine + q + k];
+            finish4<DT>(e, int64_t(r) * e.n + c0 + q, cols - q, x, decay, size);
         }
     }
 }
@@ -1029,9 +1044,11 @@ int launch_tiles(ProductArgs a, int64_t tiles, hipStream_t stream, const char* w
 // and 431 us, A A 222 and 195, X's own product, 1320 big tiles, 660 and 697; bf16, 56 matrices of a model of width 1024: 126 and 140, 86 and
 // 83, 286 and 319.
 template <bool PIECES, int STAGE, int DT = TRLK_F32>
-int launch_product(const ProductArgs& a, const int64_t (&tiles)[2], hipStream_t stream, const char* what) {
-    const double small = tiles[1] <= 256 ? 0.36 : 0.6 * double(ceil_div(tiles[1], 512));
-    if (small < double(ceil_div(tiles[0], 256)))
+int launch_product(const ProductArgs& a, const int64_t (&tiles)[3], hipStream_t stream, const char* what) {
+    const double big = double(ceil_div(tiles[0], 256)), small = tiles[1] <= 256 ? 0.36 : 0.6 * double(ceil_div(tiles[1], 512));
+    const double tiny = tiles[2] <= 256 ? 0.2 : 0.72 * double(ceil_div(tiles[2], 1024));
+    if (tiny < small && tiny < big) return launch_tiles<TinyTile, PIECES, STAGE, DT>(a, tiles[2], stream, what);
+    if (small < big)
         return launch_tiles<SmallTile, PIECES, STAGE, DT>(a, tiles[1], stream, what);
     return launch_tiles<BigTile, PIECES, STAGE, DT>(a, tiles[0], stream, what);
 }
@@ -1042,12 +1059,12 @@ struct Numbers {
 };
 
 template <int DT, int MP>
-int run_narrow(const Mat* mats, int n, int64_t chunks, const Numbers& num, hipStream_t stream, const char* what) {
+int run_narrow(const Mat* mats, int n, int64_t chunks, int64_t turns, const Numbers& num, hipStream_t stream, const char* what) {
     constexpr int kBytes = 4 * MP * (MP + 1) * 8;
     if (const int rc = reserve_lds(reinterpret_cast<const void*>(narrow_steps_kernel<MP>), kBytes, what)) return rc;
     gram_kernel<DT, MP><<<unsigned(chunks), kThreads, 0, stream>>>(mats, n);
     narrow_steps_kernel<MP><<<unsigned(n), kThreads, kBytes, stream>>>(mats, num.steps, num.a, num.b, num.c, num.eps);
-    narrow_apply_kernel<DT, MP><<<unsigned(chunks), kThreads, 0, stream>>>(mats, n);
+    narrow_apply_kernel<DT, MP><<<unsigned(turns), kThreads, 0, stream>>>(mats, n);
     return TRLK_OK;
 }
 
@@ -1059,7 +1076,7 @@ int run_group(const Group& group, const trlk_muon_matrix* x, const trlk_muon_gro
     float* factor = reinterpret_cast<float*>(ws + up256(n * sizeof(Mat)));
     double* partial = reinterpret_cast<double*>(reinterpret_cast<char*>(factor) + up256(n * sizeof(float)));
     char* at = reinterpret_cast<char*>(partial) + up256(size_t(group.chunks) * sizeof(double));
-    int64_t chunks = 0, turns = 0, halves[2] = {0, 0}, tiles[2] = {0, 0};
+    int64_t chunks = 0, turns = 0, halves[3] = {0, 0, 0}, tiles[3] = {0, 0, 0};
     MatTable t;
     t.n = 0;
     t.to = mats;
@@ -1081,12 +1098,12 @@ int run_group(const Group& group, const trlk_muon_matrix* x, const trlk_muon_gro
             const double ratio = double(y.rows) / double(y.cols);
             e.stretch = float(g.adjust == TRLK_MUON_MATCH_ADAMW ? 0.2 * sqrt(double(e.n)) : sqrt(ratio > 1.0 ? ratio : 1.0));
         }
-        e.first_chunk = uint32_t(chunks), e.first_turn = uint32_t(turns), e.first_half = uint32_t(halves[0]), e.first_tile = uint32_t(tiles[0]);
-        e.first_small_half = uint32_t(halves[1]), e.first_small = uint32_t(tiles[1]);
+        e.first_chunk = uint32_t(chunks), e.first_turn = uint32_t(turns);
         chunks += group.narrow ? ceil_div(e.n, kSpan) : ceil_div(int64_t(e.m) * e.n, kChunk);
-        turns += int64_t(e.mpad / kTurn) * (e.npad / kTurn);
-        for (int k = 0; k < 2; ++k) {
-            const int64_t side = k ? SmallTile::kRows : BigTile::kRows, down = ceil_div(e.m, side);
+        turns += group.narrow ? ceil_div(e.n, kCols) : int64_t(e.mpad / kTurn) * (e.npad / kTurn);
+        for (int k = 0; k < 3; ++k) {
+            const int64_t side = k == 2 ? TinyTile::kRows : k == 1 ? SmallTile::kRows : BigTile::kRows, down = ceil_div(e.m, side);
+            e.first_half[k] = uint32_t(halves[k]), e.first_tile[k] = uint32_t(tiles[k]);
             halves[k] += down * (down + 1) / 2;
             tiles[k] += down * ceil_div(e.n, side);
         }
@@ -1096,14 +1113,16 @@ int run_group(const Group& group, const trlk_muon_matrix* x, const trlk_muon_gro
             t.n = 0;
         }
     }
-    if (group.narrow == 16) return run_narrow<DT, 16>(mats, n, chunks, num, stream, what);
-    if (group.narrow == 32) return run_narrow<DT, 32>(mats, n, chunks, num, stream, what);
-    if (group.narrow == 64) return run_narrow<DT, 64>(mats, n, chunks, num, stream, what);
+    if (group.narrow == 16) return run_narrow<DT, 16>(mats, n, chunks, turns, num, stream, what);
+    if (group.narrow == 32) return run_narrow<DT, 32>(mats, n, chunks, turns, num, stream, what);
+    if (group.narrow == 64) return run_narrow<DT, 64>(mats, n, chunks, turns, num, stream, what);
     momentum_kernel<DT><<<unsigned(chunks), kThreads, 0, stream>>>(mats, n, partial);
     norm_kernel<<<unsigned(n), kThreads, 0, stream>>>(mats, partial, factor, num.eps);
     make_x_kernel<DT><<<unsigned(turns), kThreads, 0, stream>>>(mats, n, factor);
-    ProductArgs a{mats, n, 0, 0, 1, float(num.a), float(num.b), float(num.c)};
+    ProductArgs a{mats, n, 0, 0, 1, 1, 1, float(num.a), float(num.b), float(num.c)};
     for (int s = 0; s < num.steps; ++s) {
+        a.reads_lo = s == 0 || s + 1 < num.steps;
+        a.writes_lo = s + 2 < num.steps;
         if (const int rc = launch_product<PIECES, kStageA>(a, halves, stream, what)) return rc;
         if (const int rc = launch_product<PIECES, kStageB>(a, halves, stream, what)) return rc;
         const int rc = s + 1 < num.steps ? launch_product<PIECES, kStageX>(a, tiles, stream, what)
