@@ -279,6 +279,52 @@ def test_graph_capture(tokens):
         assert torch.equal(got, want)
 
 
+def test_what_has_no_derivative_raises():
+    import trl_amd
+
+    weight = torch.randn((20, 16), device=DEV, requires_grad=True)
+    ids = torch.arange(10, device=DEV)
+    with pytest.raises(RuntimeError):
+        torch.func.jvp(lambda w: trl_amd.embedding(ids, w), (weight.detach(),), (torch.ones_like(weight),))
+    (grad,) = torch.autograd.grad(trl_amd.embedding(ids, weight).square().sum(), weight, create_graph=True)
+    with pytest.raises(RuntimeError):
+        grad.sum().backward()
+
+
+def test_gradients_of_broadcast_and_summed_rows():
+    import trl_amd
+
+    gen = torch.Generator(device=DEV).manual_seed(2)
+    weight = table(60, 24, torch.float32, gen).requires_grad_(True)
+    ids = torch.randint(0, 60, (3, 7), generator=gen, device=DEV)
+    (grad,) = torch.autograd.grad(trl_amd.embedding(ids, weight, scale=0.5).sum(), weight)  # one number for all entries
+    assert torch.equal(grad, 0.5 * torch.bincount(ids.flatten(), minlength=60).float()[:, None].expand(60, 24))
+    u = torch.randn((7, 3, 24), generator=gen, device=DEV).transpose(0, 1)
+    (grad,) = torch.autograd.grad(trl_amd.embedding(ids, weight), weight, u)
+    check_gradient(grad, u, ids, 1.0, None)
+
+
+def test_refused_memory_and_types():
+    import trl_amd
+
+    held, ids = torch.zeros((30, 8), device=DEV), torch.arange(4, device=DEV)
+    for g, error in ((held[:4], ValueError), (torch.zeros((4, 7), device=DEV), ValueError), (torch.zeros((5, 8), device=DEV), ValueError),
+                     (torch.zeros((4, 8), device=DEV, dtype=torch.float64), TypeError), (torch.zeros((4, 8)), RuntimeError)):
+        with pytest.raises(error):
+            trl_amd.embedding_grad_(held, g, ids)
+    with pytest.raises(TypeError):
+        trl_amd.embedding_grad_(held.half(), torch.zeros((4, 8), device=DEV), ids)
+    with pytest.raises(ValueError):
+        trl_amd.embedding_grad_(held.t(), torch.zeros((4, 30), device=DEV), ids)
+    for bad, error in ((ids.float(), TypeError), (ids.short(), TypeError), (ids.cpu(), RuntimeError)):
+        with pytest.raises(error):
+            trl_amd.embedding(bad, held)
+    with pytest.raises(TypeError):
+        trl_amd.embedding(ids, held.double())
+    with pytest.raises(ValueError):
+        trl_amd.embedding(ids, held[0])
+
+
 class Tied(torch.nn.Module):
     def __init__(self, embed):
         super().__init__()

@@ -785,7 +785,6 @@ void embedding_grad_(const Tensor& grad_weight, const Tensor& grad, const Tensor
     const c10::DeviceGuard guard(grad_weight.device());
     TORCH_CHECK_VALUE((grad_weight.size(1) <= 1 || grad_weight.stride(1) == 1) && (grad_weight.size(0) <= 1 || grad_weight.stride(0) >= grad_weight.size(1)),
                       "embedding_grad_: the table's gradient has gaps between the entries of a row, or rows that overlap");
-    at::assert_no_partial_overlap(grad_weight, grad);
     TORCH_CHECK_VALUE(grad.numel() == 0 || !grad_weight.is_alias_of(grad) || at::get_overlap_status(grad_weight, grad) == at::MemOverlapStatus::No,
                       "embedding_grad_: the table's gradient shares memory with the tokens' gradients");
     embedding_into(grad_weight, grad, ids, scale, padding_idx, true);

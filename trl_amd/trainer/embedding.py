@@ -50,6 +50,10 @@ def _scale_of(module: torch.nn.Embedding) -> float:
     return float(scale.to(module.weight.dtype)) if isinstance(scale, Tensor) else float(scale)
 
 
+def _embedding_forward(self, input: Tensor) -> Tensor:
+    return embedding(input, self.weight, scale=self._trl_amd_scale, padding_idx=self.padding_idx)
+
+
 def patch_embedding(model: torch.nn.Module) -> None:
     """Replaces the forward of `model.get_input_embeddings()` by `embedding`, with the module's own scale and padding index.  Takes
     `torch.nn.Embedding` and the scaled embeddings of transformers' models; others, and embeddings with `max_norm`, `sparse` or
@@ -59,9 +63,5 @@ def patch_embedding(model: torch.nn.Module) -> None:
         raise ValueError(f"the model's input embeddings are a {type(module).__name__}, not a torch.nn.Embedding")
     if module.max_norm is not None or module.sparse or module.scale_grad_by_freq:
         raise ValueError("patch_embedding takes no max_norm, sparse or scale_grad_by_freq")
-    scale = _scale_of(module)
-
-    def forward(self, input: Tensor) -> Tensor:
-        return embedding(input, self.weight, scale=scale, padding_idx=self.padding_idx)
-
-    module.forward = types.MethodType(forward, module)
+    module._trl_amd_scale = _scale_of(module)
+    module.forward = types.MethodType(_embedding_forward, module)  # (a copy of the model gets one that is bound to its own table)
