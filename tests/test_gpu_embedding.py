@@ -178,6 +178,20 @@ def test_ids_outside_the_table():
     trl_amd.check_device_errors()
 
 
+@pytest.mark.parametrize("dtype", list(DTYPES))
+def test_large_outputs(dtype):
+    """Outputs that go past the caches, with cut rows."""
+    import trl_amd
+
+    gen = torch.Generator(device=DEV).manual_seed(8)
+    weight = table(5000, 2049, DTYPES[dtype], gen)
+    ids = torch.randint(0, 5000, (70000 if dtype != "fp32" else 35000,), generator=gen, device=DEV)
+    rows = trl_amd.embedding(ids, weight, scale=0.5)
+    for part in (slice(0, 100), slice(17000, 17100), slice(-100, None)):
+        check_rows(rows[part], weight, ids[part], 0.5)
+    assert torch.equal(rows, trl_amd.embedding(ids.flip(0), weight, scale=0.5).flip(0))
+
+
 def test_infinities_and_nan_stay_in_their_rows():
     import trl_amd
 
