@@ -211,10 +211,33 @@ __global__ __launch_bounds__(kThreads) void make_x_kernel(const Mat* mats, int n
         const float x = Elem<DT>::load1(g + at);
         return (e.momentum ? update_of(e.momentum[at], x, e) : x) * f;
     };
+    // eight neighbours of u, factor and all
+    const auto eight = [&](int64_t at, float (&x)[8]) {
+        load8<DT>(g + at, x);
+        if (e.momentum) {
+            float w[8];
+            load8f(e.momentum + at, w);
+#pragma unroll
+            for (int k = 0; k < 8; ++k) x[k] = update_of(w[k], x[k], e);
+        }
+#pragma unroll
+        for (int k = 0; k < 8; ++k) x[k] *= f;
+    };
     if (e.tall) {  // u is n x m: its rows are X's columns
-        const int r = threadIdx.x & 63;
-        for (int c = threadIdx.x >> 6; c < kTurn; c += kThreads / 64)
-            tile[r][c] = r0 + r < e.m && c0 + c < e.n ? value(int64_t(c0 + c) * e.m + r0 + r) : 0.f;
+#pragma unroll
+        for (int q = 0; q < kTurn * kTurn / 8 / kThreads; ++q) {
+            const int v = q * kThreads + threadIdx.x, c = v / (kTurn / 8), r = v % (kTurn / 8) * 8;
+            const int64_t at = int64_t(c0 + c) * e.m + r0 + r;
+            float x[8];
+            if (c0 + c < e.n && r0 + r + 8 <= e.m) {
+                eight(at, x);
+            } else {
+#pragma unroll
+                for (int k = 0; k < 8; ++k) x[k] = c0 + c < e.n && r0 + r + k < e.m ? value(at + k) : 0.f;
+            }
+#pragma unroll
+            for (int k = 0; k < 8; ++k) tile[r + k][c] = x[k];
+        }
         __syncthreads();
     }
     for (int v = threadIdx.x; v < kTurn * kTurn / 8; v += kThreads) {
@@ -225,16 +248,7 @@ __global__ __launch_bounds__(kThreads) void make_x_kernel(const Mat* mats, int n
 #pragma unroll
             for (int k = 0; k < 8; ++k) x[k] = tile[r][c + k];
         } else if (inside) {
-            const int64_t at = int64_t(r0 + r) * e.n + c0 + c;
-            load8<DT>(g + at, x);
-            if (e.momentum) {
-                float w[8];
-                load8f(e.momentum + at, w);
-#pragma unroll
-                for (int k = 0; k < 8; ++k) x[k] = update_of(w[k], x[k], e);
-            }
-#pragma unroll
-            for (int k = 0; k < 8; ++k) x[k] *= f;
+            eight(int64_t(r0 + r) * e.n + c0 + c, x);
         } else {
 #pragma unroll
             for (int k = 0; k < 8; ++k) x[k] = r0 + r < e.m && c0 + c + k < e.n ? value(int64_t(r0 + r) * e.n + c0 + c + k) : 0.f;
