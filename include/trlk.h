@@ -555,7 +555,7 @@ int trlk_embedding_bwd(const void* d_grad, int dtype, int64_t n, int64_t cols, i
  * singular values.  The tables are HOST memory, read before the call returns.  d_param, d_grad and d_momentum (fp32) are dense [rows, cols];
  * what is written shares no memory with anything else that is listed.  trlk_orthogonalize: d_param takes X, turned back, of d_grad (they may be
  * the same), d_momentum is NULL.  The smaller side is 32768 at most, the larger one 2^22, both 2^34 entries.  A matrix with a NaN or an infinity comes out as NaN.
- * Coefficients with which singular values of at most 1 grow past 2.5 on the way are refused.  eps in (0, 1].
+ * Coefficients with which singular values of at most 1 grow past 2.5 on the way are refused.  eps in [1e-30, 1].
  * d_workspace: trlk_muon_workspace_bytes(...) bytes, 256-byte aligned. */
 enum trlk_muon_adjust { TRLK_MUON_ORIGINAL = 0, TRLK_MUON_MATCH_ADAMW = 1 };
 typedef struct {

@@ -139,6 +139,35 @@ def test_larger_matrices(dtype, shapes):
         check(x, u)
 
 
+@pytest.mark.parametrize("shape", [(1100, 1 << 22), (1 << 22, 1100)])
+def test_offsets_past_32_bits(shape):
+    """With G = X X^T in 64 bits the result is T X, T the product of the steps' factors: columns from all over the matrix.  The bound: operands of 11
+    bits cost independent entries 1.7e-3 of the result at most (`rounded` on such matrices), and the rounding to bf16 half a step."""
+    import trl_amd
+
+    gen = torch.Generator(device=DEV).manual_seed(6)
+    u = torch.empty(shape, dtype=torch.bfloat16, device=DEV)
+    for part in u.view(-1).split(1 << 28):
+        part.normal_(generator=gen)
+    x = u if shape[0] < shape[1] else u.t()
+    rows, cols = x.shape
+    gram = torch.zeros((rows, rows), dtype=torch.float64, device=DEV)
+    for c in range(0, cols, 1 << 17):
+        part = x[:, c : c + (1 << 17)].double()
+        gram += part @ part.t().contiguous()
+    factor = 1 / gram.trace().sqrt()
+    gram *= factor**2
+    steps, eye = torch.eye(rows, dtype=torch.float64, device=DEV), torch.eye(rows, dtype=torch.float64, device=DEV)
+    for _ in range(5):
+        p = A * eye + B * gram + C * gram @ gram
+        steps, gram = p @ steps, p @ gram @ p
+    got = trl_amd.orthogonalize(u)
+    got = got if shape[0] < shape[1] else got.t()
+    for c in (0, cols // 2 - 777, cols - 4096):
+        want = steps @ (x[:, c : c + 4096].double() * factor)
+        assert distance(got[:, c : c + 4096], want) <= (1.5 * 1.7e-3 + 2.0**-8) * float(want.norm())
+
+
 @pytest.mark.parametrize("dtype", list(DTYPES))
 def test_other_numbers(dtype):
     import trl_amd

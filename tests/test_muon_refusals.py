@@ -44,7 +44,7 @@ def test_library_refuses():
         assert step(table(**{name: None})) == -1 and step(table(**{name: FAKE + 1})) == -4
     for bad in (0, -1, 101):
         assert step(steps=bad) == -5
-    for bad in (0.0, -1.0, 2.0, math.nan):
+    for bad in (0.0, -1.0, 2.0, 1e-31, math.nan):
         assert step(eps=bad) == -5
     for bad in ((math.inf, 0.0, 0.0), (9.0, 0.0, 0.0), (3.4445, 4.775, 2.0315), (1.0, 0.0, -8.0)):
         assert step(c=bad) == -5, bad
@@ -154,6 +154,14 @@ def test_param_groups():
         assert [id(p) for p in matrices["params"]] == [id(model.a.weight)] and rest["adamw"]
         assert {id(p) for p in rest["params"]} == {id(p) for p in (model.embed.weight, model.a.bias, model.norm.weight, model.norm.bias, model.lm_head.weight)}
         trl_amd.Muon([matrices, rest], adjust_lr_fn="match_rms_adamw")
+
+
+def test_convolutions_are_no_matrices():
+    import trl_amd
+
+    model = torch.nn.Sequential(torch.nn.Conv2d(3, 8, 4), torch.nn.Conv1d(8, 8, 4, groups=8), torch.nn.Linear(8, 8))
+    matrices, rest = trl_amd.muon_param_groups(model)
+    assert [id(p) for p in matrices["params"]] == [id(model[2].weight)] and len(rest["params"]) == 5
 
 
 def test_shapes_for_tracers():

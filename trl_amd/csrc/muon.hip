@@ -529,7 +529,7 @@ __global__ __launch_bounds__(Tile::kThreads) __attribute__((amdgpu_waves_per_eu(
     constexpr int kWhich = std::is_same_v<Tile, TinyTile> ? 2 : std::is_same_v<Tile, SmallTile> ? 1 : 0;
     typedef std::conditional_t<PIECES, PieceRuns, OneRun> Runs;
     constexpr bool kSquare = STAGE == kStageA || STAGE == kStageB;
-        const int64_t piece = xcd_piece(blockIdx.x, args.run);
+    const int64_t piece = xcd_piece(blockIdx.x, args.run);
     if (piece >= args.tiles) return;
     const auto first = [](const Mat& e) { return (kSquare ? e.first_half : e.first_tile)[kWhich]; };
     const Mat e = args.mats[mat_of(args.mats, args.n, uint32_t(piece), first)];
@@ -1168,7 +1168,7 @@ double largest_image(double top, double a, double b, double c) {
 
 int check_numbers(const Numbers& num, const char* what) {
     TRLK_REQUIRE(num.steps >= 1 && num.steps <= 100, TRLK_ERR_BAD_VALUE, "%s: 1 to 100 steps, not %d", what, num.steps);
-    TRLK_REQUIRE(num.eps > 0.0 && num.eps <= 1.0, TRLK_ERR_BAD_VALUE, "%s: eps must be in (0, 1]", what);
+    TRLK_REQUIRE(num.eps >= 1e-30 && num.eps <= 1.0, TRLK_ERR_BAD_VALUE, "%s: eps must be in [1e-30, 1]", what);
     TRLK_REQUIRE(isfinite(num.a) && isfinite(num.b) && isfinite(num.c), TRLK_ERR_BAD_VALUE, "%s: coefficients must be finite", what);
     // the fp16 pieces hold singular values up to 65504 / kUnitX, and A and B up to 65504 / kUnitA
     double top = 1.0;

@@ -71,8 +71,8 @@ def _check_settings(group: dict) -> None:
         return
     if not 0.0 <= group["momentum"] < 1.0:
         raise ValueError(f"momentum must be in [0, 1), got {group['momentum']}")
-    if not 0.0 < group["eps"] <= 1.0 or not 1 <= group["ns_steps"] <= 100:
-        raise ValueError(f"eps must be in (0, 1] and ns_steps 1 to 100, got {group['eps']}, {group['ns_steps']}")
+    if not 1e-30 <= group["eps"] <= 1.0 or not 1 <= group["ns_steps"] <= 100:
+        raise ValueError(f"eps must be in [1e-30, 1] and ns_steps 1 to 100, got {group['eps']}, {group['ns_steps']}")
     _numbers(group["ns_coefficients"], group["ns_steps"], group["eps"])
     _adjustment(group["adjust_lr_fn"])
     for p in group["params"]:
@@ -205,8 +205,9 @@ class Muon(torch.optim.Optimizer):
 
 def muon_param_groups(model: torch.nn.Module) -> list[dict]:
     """Two groups for `Muon`: the model's trainable matrices, and with `adamw=True` its embeddings, its output head and whatever is no
-    matrix."""
-    apart = {id(p) for m in model.modules() if isinstance(m, torch.nn.Embedding) for p in m.parameters(recurse=False)}
+    matrix (convolutions' weights neither)."""
+    kinds = (torch.nn.Embedding, torch.nn.modules.conv._ConvNd)
+    apart = {id(p) for m in model.modules() if isinstance(m, kinds) for p in m.parameters(recurse=False)}
     head = model.get_output_embeddings() if hasattr(model, "get_output_embeddings") else getattr(model, "lm_head", None)
     if isinstance(head, torch.nn.Module):
         apart |= {id(p) for p in head.parameters()}
