@@ -2,7 +2,7 @@
 
 Tolerances (2-norms of whole matrices).  16 bits: the iteration rounds the products' operands to fp16; `rounded` makes the same roundings at the
 same places in 64 bits, and how far that is from the exact iteration is what the formats cost for a given matrix.  Kernels sum in fp32 and round to
-other neighbours here and there: 1.5 times that, and half a step of the output's type.  fp32: the operands hold 22 bits and sums are
+other neighbours here and there: 1.5 times that, and half a step of the output's type.  fp32, and results in fp16: the operands hold 22 bits and sums are
 fp32, as in an iteration in plain fp32, whose own distance from the exact one on the same matrix is taken 4 times (a product of two pieces drops
 2^-22, four times fp32's rounding), and 1e-6.  Momentum: three roundings of 2^-24 of the summands.  Parameters: two roundings of fp32 and
 half a step of their type beside the update's error."""
@@ -50,7 +50,8 @@ def rounded(u, steps=5, coefficients=(A, B, C), eps=1e-7):
         hi = fp16(x, 16384.0)
         x = hi + fp16(x - hi, 16384.0) if step == 0 or step + 1 < steps else hi
         gram = fp16(hi @ hi.mT, 8192.0)
-        x = a * x + fp16(b * gram + c * gram @ gram, 8192.0) @ hi
+        factor = b * gram + c * gram @ gram
+        x = a * x + fp16(factor, 8192.0) @ hi + torch.diag(factor - fp16(factor, 8192.0))[:, None] * hi  # (B's diagonal loses nothing)
     return x.mT if tall else x
 
 
@@ -70,8 +71,8 @@ def distance(x, y):
     return float(torch.linalg.vector_norm(x.double() - y.double()))
 
 
-def allowed(u, dtype, want, **numbers):
-    if dtype == torch.float32:
+def allowed(u, dtype, want, step=False, **numbers):
+    if dtype == torch.float32 or (dtype == torch.float16 and not step):
         return 4 * distance(plain32(u, **numbers), want) + 1e-6 * float(want.norm())
     return 1.5 * distance(rounded(u, **numbers), want) + 1e-6 * float(want.norm())
 
@@ -221,7 +222,7 @@ def definition(p, g, m, lr, wd, beta, nesterov, adjust, **numbers):
     rows, cols = p.shape
     stretch = 0.2 * math.sqrt(max(rows, cols)) if adjust == "match_rms_adamw" else math.sqrt(max(1.0, rows / cols))
     x = exact(u, **numbers)
-    off = lr * stretch * allowed(u.float(), p.dtype, x, **numbers)
+    off = lr * stretch * allowed(u.float(), p.dtype, x, step=True, **numbers)
     return p.double() * (1 - lr * wd) - lr * stretch * x, now, off
 
 

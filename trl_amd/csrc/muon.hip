@@ -54,6 +54,7 @@ struct Mat {
     __device__ __forceinline__ uint16_t* buffer(int i) const { return x + 2 * i * plane(); }
     __device__ __forceinline__ uint16_t* a() const { return x + 4 * plane(); }
     __device__ __forceinline__ uint16_t* b() const { return x + 4 * plane() + pieces * square(); }
+    __device__ __forceinline__ float* rest_of_b() const { return reinterpret_cast<float*>(b() + square()); }  // (one piece)
 };
 
 constexpr int kTable = 34;
@@ -558,6 +559,7 @@ __global__ __launch_bounds__(Tile::kThreads) __attribute__((amdgpu_waves_per_eu(
         uint16_t* out = STAGE == kStageA ? e.a() : e.b();
         const int iw = i0 + wr, jw = j0 + wc;
         if (iw >= e.m || jw >= e.m) return;  // (no barrier follows)
+        const bool diagonal = !PIECES && STAGE == kStageB && tr == tc;
         // (neighbours past m, up to mpad, are written as zeros: they are the contraction's padding in the next product)
         u32x2 high[MI][NI], low[PIECES ? MI : 1][PIECES ? NI : 1];
         u32x4 was[2][PIECES ? MI : MI / 2];  // A's entries, a column of blocks ahead
@@ -601,6 +603,7 @@ __global__ __launch_bounds__(Tile::kThreads) __attribute__((amdgpu_waves_per_eu(
                     for (int r = 0; r < 4; ++r)
                         if (i + r >= e.m || !live) v[r] = 0.f;
                     split4(v, h, l);
+                    if (diagonal && i <= j && j < i + 4 && live) e.rest_of_b()[j] = j == i ? l[0] : j == i + 1 ? l[1] : j == i + 2 ? l[2] : l[3];
                     high[ii + u][jj] = pack4<TRLK_F16>(h);
                     if constexpr (PIECES) low[ii + u][jj] = pack4<TRLK_F16>(l);
                 }
@@ -644,9 +647,11 @@ __global__ __launch_bounds__(Tile::kThreads) __attribute__((amdgpu_waves_per_eu(
 #pragma unroll
                         for (int k = 0; k < 4; ++k) {  // (rows of X's padding are there)
                             const uint16_t* p = x + int64_t(r + k) * e.npad + c;
-                            v[k] = PIECES || args.reads_lo ? half_at(p) + half_at(p + plane) : half_at(p);
+                            const float high = half_at(p), low = PIECES || args.reads_lo ? half_at(p + plane) : 0.f;
+                            if constexpr (PIECES) v[k] = (high + low) * args.a;
+                            else v[k] = high * fmaf(e.rest_of_b()[r + k], scale, args.a) + low * args.a;
                         }
-                        finish4<DT>(e, int64_t(c) * e.m + r, e.m - r, (v * args.a + acc[ii][jj] * scale) * (1.f / kUnitX), decay, size);
+                        finish4<DT>(e, int64_t(c) * e.m + r, e.m - r, (v + acc[ii][jj] * scale) * (1.f / kUnitX), decay, size);
                     }
                 }
                 return;
@@ -659,9 +664,11 @@ __global__ __launch_bounds__(Tile::kThreads) __attribute__((amdgpu_waves_per_eu(
         // X's own entries, loaded some rows of blocks ahead: a load cannot pass the stores before it, and each would wait for them
         constexpr int kAhead = MI < 4 ? MI : 4;
         u32x4 own[kAhead][NI];  // of each pair of blocks, hi and lo
+        float rest[kAhead];
         const auto row_of = [&](int ii) { return int64_t(min(r0 + wr + ii * 16 + (lane & 15), e.m - 1)) * e.npad + cw + pair_offset(lane); };
         const auto fetch = [&](int ii) {
             const uint16_t* p = x + row_of(ii);
+            if constexpr (!PIECES) rest[ii % kAhead] = e.rest_of_b()[min(r0 + wr + ii * 16 + (lane & 15), e.m - 1)];
 #pragma unroll
             for (int jj = 0; jj < NI; jj += 2) {
                 own[ii % kAhead][jj] = *reinterpret_cast<const u32x4*>(p + jj * 16);
@@ -675,6 +682,7 @@ __global__ __launch_bounds__(Tile::kThreads) __attribute__((amdgpu_waves_per_eu(
             const int r = r0 + wr + ii * 16 + (lane & 15);
             const bool live = r < e.m;
             f32x4 v[NI];
+            const float a_hi = PIECES ? args.a : fmaf(rest[ii % kAhead], scale, args.a);
 #pragma unroll
             for (int jj = 0; jj < NI; jj += 2) {
                 u32x2 xh[2], xl[2];
@@ -682,7 +690,7 @@ __global__ __launch_bounds__(Tile::kThreads) __attribute__((amdgpu_waves_per_eu(
                 pair_apart(own[ii % kAhead][jj + 1], xl[0], xl[1]);
 #pragma unroll
                 for (int u = 0; u < 2; ++u)
-                    v[jj + u] = (unpack4<TRLK_F16>(xh[u]) + unpack4<TRLK_F16>(xl[u])) * args.a + acc[ii][jj + u] * scale;
+                    v[jj + u] = unpack4<TRLK_F16>(xh[u]) * a_hi + unpack4<TRLK_F16>(xl[u]) * args.a + acc[ii][jj + u] * scale;
             }
             if (ii + kAhead < MI) fetch(ii + kAhead);
             if constexpr (STAGE == kStageLast) {
@@ -970,7 +978,8 @@ int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 int64_t up_to(int64_t n, int64_t unit) { return ceil_div(n, unit) * unit; }
 size_t up256(size_t n) { return (n + 255) / 256 * 256; }
 
-int pieces_of(int dtype) { return dtype == TRLK_F32 ? 2 : 1; }
+// (an fp16 result shows what one piece loses, a step's parameter does not)
+int pieces_of(const trlk_muon_matrix& x) { return x.dtype == TRLK_F32 || (x.dtype == TRLK_F16 && !x.d_momentum) ? 2 : 1; }
 // Rows that a narrow matrix is padded to, 0 for the others.
 int narrow_rows(const trlk_muon_matrix& x) {
     const int64_t m = std::min(x.rows, x.cols);
@@ -979,7 +988,7 @@ int narrow_rows(const trlk_muon_matrix& x) {
 size_t matrix_bytes(const trlk_muon_matrix& x) {
     if (const int mp = narrow_rows(x)) return up256(size_t(ceil_div(std::max(x.rows, x.cols), kSpan) + 1) * mp * mp * sizeof(double));
     const int64_t m = up_to(std::min(x.rows, x.cols), BK), n = up_to(std::max(x.rows, x.cols), BK);
-    return up256(size_t(4 * m * n + 2 * pieces_of(x.dtype) * m * m) * 2);
+    return up256(size_t(4 * m * n + 2 * pieces_of(x) * m * m) * 2 + size_t(m) * sizeof(float));
 }
 
 // Matrices that go through the launches together: of one type, narrow ones of one kind, as many as the workspace's share holds.
@@ -1082,9 +1091,8 @@ int run_narrow(const Mat* mats, int n, int64_t chunks, int64_t turns, const Numb
     return TRLK_OK;
 }
 
-template <int DT>
+template <int DT, bool PIECES>
 int run_group(const Group& group, const trlk_muon_matrix* x, const trlk_muon_group* groups, const Numbers& num, char* ws, hipStream_t stream, const char* what) {
-    constexpr bool PIECES = DT == TRLK_F32;
     const int n = int(group.each.size());
     Mat* mats = reinterpret_cast<Mat*>(ws);
     float* factor = reinterpret_cast<float*>(ws + up256(n * sizeof(Mat)));
@@ -1104,7 +1112,7 @@ int run_group(const Group& group, const trlk_muon_matrix* x, const trlk_muon_gro
         e.tall = y.rows > y.cols;
         e.m = int32_t(std::min(y.rows, y.cols)), e.n = int32_t(std::max(y.rows, y.cols));
         e.mpad = int32_t(up_to(e.m, BK)), e.npad = int32_t(up_to(e.n, BK));
-        e.pieces = pieces_of(DT);
+        e.pieces = PIECES ? 2 : 1;
         if (groups) {
             const trlk_muon_group& g = groups[y.group];
             e.lr = float(g.lr), e.d_lr = g.d_lr, e.weight_decay = float(g.weight_decay);
@@ -1221,9 +1229,10 @@ int run(const trlk_muon_matrix* x, int32_t n, const trlk_muon_group* groups, int
     for (const Group& g : groups_of(x, n)) {
         const int dtype = x[g.each[0]].dtype;
         const trlk_muon_group* hyper = step ? groups : nullptr;
-        const int rc = dtype == TRLK_F32    ? run_group<TRLK_F32>(g, x, hyper, num, ws, stream, what)
-                       : dtype == TRLK_BF16 ? run_group<TRLK_BF16>(g, x, hyper, num, ws, stream, what)
-                                            : run_group<TRLK_F16>(g, x, hyper, num, ws, stream, what);
+        const int rc = dtype == TRLK_F32    ? run_group<TRLK_F32, true>(g, x, hyper, num, ws, stream, what)
+                       : dtype == TRLK_BF16 ? run_group<TRLK_BF16, false>(g, x, hyper, num, ws, stream, what)
+                       : step               ? run_group<TRLK_F16, false>(g, x, hyper, num, ws, stream, what)
+                                            : run_group<TRLK_F16, true>(g, x, hyper, num, ws, stream, what);
         if (rc) return rc;
     }
     return launch_status(what);
