@@ -367,14 +367,15 @@ struct BigTile {
     }
 };
 // Small: 128 x 128 or 64 x 64, 4 waves of a quarter each, for launches whose big tiles would leave CUs idle: four or sixteen times the tiles with as
-// much less work, two or four on a CU.  Bound by the LDS: of 128 x 128, a step of 64 k moves 96 KB in and out of it for 512 cycles of MFMAs,
+// much less work, two on a CU.  Of 128 x 128 the bound is the LDS: a step of 64 k moves 96 KB in and out of it for 512 cycles of MFMAs,
 // and takes 0.58 us with one tile on a CU and 0.54 with two (165 and 180 GB/s a CU).  Four stages instead of two, which leave room for one
-// tile only, and tiles that come through registers two steps ahead were no faster (0.61 and 0.66 us).  Layouts are those of the big tile's
-// loop; a k-major stage has 64 k rows of 256 or 128 bytes.
-template <int SIDE>
+// tile only, and tiles that come through registers two steps ahead were no faster (0.61 and 0.66 us).  Of 64 x 64 it is the transfers' latency: four stages
+// (one bf16 matrix of 1024 x 1024 151 us, with three 154, with two 174).  Layouts are those of the big tile's loop; a k-major stage has 64 k rows
+// of 256 or 128 bytes.
+template <int SIDE, int STAGES>
 struct SmallTileOf {
     static constexpr int kRows = SIDE, kCols = SIDE, kThreads = 256, kWaveRows = SIDE / 2, kWaveCols = SIDE / 2, kI = SIDE / 32, kJ = SIDE / 32;
-    static constexpr int kStages = 2, kHalf = kRows * kRowBytes, kStage = 2 * kHalf, kLds = kStages * kStage, kLoads = kHalf / 1024 / 4;
+    static constexpr int kStages = STAGES, kHalf = kRows * kRowBytes, kStage = 2 * kHalf, kLds = kStages * kStage, kLoads = kHalf / 1024 / 4;
     static constexpr int kKmRow = SIDE * 2, kKmUnits = SIDE / 8;  // of a k-major stage: bytes and 16-byte units of a k row
     static __device__ __forceinline__ int wave_row(int wave) { return (wave >> 1) * (SIDE / 2); }
     static __device__ __forceinline__ int wave_col(int wave) { return (wave & 1) * (SIDE / 2); }
@@ -450,8 +451,10 @@ struct SmallTileOf {
         };
         // `later` stages may still be on their way; what this wave has asked the LDS for has arrived
         const auto landed = [&](int later) {
-            static_assert(kStages == 2, "one later stage");
-            if (later == 1) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(2 * kLoads) : "memory");
+            static_assert(kStages >= 2 && kStages <= 4 && 6 * kLoads < 64, "up to three later stages, and what the counter holds");
+            if (kStages > 3 && later == 3) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(6 * kLoads) : "memory");
+            else if (kStages > 2 && later == 2) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(4 * kLoads) : "memory");
+            else if (later == 1) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(2 * kLoads) : "memory");
             else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
             __builtin_amdgcn_sched_barrier(0);
             __builtin_amdgcn_s_barrier();
@@ -483,8 +486,8 @@ struct SmallTileOf {
     }
 };
 
-typedef SmallTileOf<128> SmallTile;
-typedef SmallTileOf<64> TinyTile;
+typedef SmallTileOf<128, 2> SmallTile;
+typedef SmallTileOf<64, 4> TinyTile;
 
 // The transposed part of a symmetric result: a wave's entries (128 or 64 x 64, or 32 x 32) go through LDS of its own, rows of its columns (and 8 of padding against
 // bank conflicts), and come back with eight neighbours of the other side a lane, by the transpose loads: lane t of a group of 16 points at the
@@ -1062,14 +1065,15 @@ int launch_tiles(ProductArgs a, int64_t tiles, hipStream_t stream, const char* w
     kernel<<<xcd_grid(tiles, a.run), Tile::kThreads, kBytes, stream>>>(a);
     return TRLK_OK;
 }
-// Big tiles or small ones, whichever are done sooner: a round is 256 big ones or, two on a CU, 512 small ones, which take 0.6 of a big one's time
-// (0.36 if a CU has but one).  bf16: one matrix of 1024 x 1024 478 us with big tiles, 252 with small ones; fp32, 24 matrices of 1150 x 2816: X X^T 468
-// and 431 us, A A 222 and 195, X's own product, 1320 big tiles, 660 and 697; bf16, 56 matrices of a model of width 1024: 126 and 140, 86 and
-// 83, 286 and 319.
+// The size of tiles whose launch is done soonest, in units of a big tile's time.  A round is 256 big ones.  Of 128 x 128 two run on a CU, 512 take 0.6 of
+// that, 256 or fewer 0.36; of 64 x 64 two, too, 512 take 0.27, 256 or fewer 0.235.  Both sides in us: one bf16 matrix
+// of 1024 x 1024 478 with 256 alone, 252 with 128, 150 with 64; 1408 x 1408 314 with 128, 212 with 64; 2048 x 2048 420 and 455, 432 with 64 for
+// the symmetric products only, 528 tiles; 8 of 512 x 512 189 and 154; fp32, 24 of 1150 x 2816: X X^T 468 with 256, 431 with 128, A A 222 and 195, X's own
+// product, 1320 tiles of 256, 660 and 697.
 template <bool PIECES, int STAGE, int DT = TRLK_F32>
 int launch_product(const ProductArgs& a, const int64_t (&tiles)[3], hipStream_t stream, const char* what) {
     const double big = double(ceil_div(tiles[0], 256)), small = tiles[1] <= 256 ? 0.36 : 0.6 * double(ceil_div(tiles[1], 512));
-    const double tiny = tiles[2] <= 256 ? 0.2 : 0.72 * double(ceil_div(tiles[2], 1024));
+    const double tiny = tiles[2] <= 256 ? 0.235 : 0.27 * double(ceil_div(tiles[2], 512));
     if (tiny < small && tiny < big) return launch_tiles<TinyTile, PIECES, STAGE, DT>(a, tiles[2], stream, what);
     if (small < big)
         return launch_tiles<SmallTile, PIECES, STAGE, DT>(a, tiles[1], stream, what);
