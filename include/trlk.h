@@ -551,12 +551,12 @@ int trlk_embedding_bwd(const void* d_grad, int dtype, int64_t n, int64_t cols, i
  *   `steps` times:  A = X X^T;  X = a X + (b A + c A A) X
  *   p = p (1 - lr weight_decay) - lr stretch X;   stretch = sqrt(max(1, rows / cols)), or 0.2 sqrt(max(rows, cols)) (MATCH_ADAMW)
  * Elementwise arithmetic and sums are fp32 (norms in 64 bits), p is rounded once to its type.  Matrices of 16 bits: the products' operands are
- * rounded to 11 bits, the result is off by 2e-3 of its norm at most; of fp32: 22 bits, 1e-6 or so times how much the iteration stretches small
- * singular values.  The tables are HOST memory, read before the call returns.  d_param, d_grad and d_momentum (fp32) are dense [rows, cols];
+ * rounded to 11 bits, the result is off by 2e-3 of its norm at most before its own rounding; of fp32, and results in fp16: 22 bits, about what the
+ * iteration in plain fp32 is off by.  The tables are HOST memory, read before the call returns.  d_param, d_grad and d_momentum (fp32) are dense [rows, cols];
  * what is written shares no memory with anything else that is listed.  trlk_orthogonalize: d_param takes X, turned back, of d_grad (they may be
  * the same), d_momentum is NULL.  The smaller side is 32768 at most, the larger one 2^22, both 2^34 entries.  A matrix with a NaN or an infinity comes out as NaN.
  * Coefficients with which singular values of at most 1 grow past 2.5 on the way are refused.  eps in [1e-30, 1].
- * d_workspace: trlk_muon_workspace_bytes(...) bytes, 256-byte aligned. */
+ * d_workspace: trlk_muon_workspace_bytes(...) bytes, 256-byte aligned: 8 GiB at most, unless one matrix needs more (several take turns in it). */
 enum trlk_muon_adjust { TRLK_MUON_ORIGINAL = 0, TRLK_MUON_MATCH_ADAMW = 1 };
 typedef struct {
     void* d_param;

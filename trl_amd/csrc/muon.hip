@@ -10,10 +10,11 @@
 // written twice).  The products run on fp16 operands with fp32 sums.  X is held as two fp16 pieces, x = hi + lo, 22 bits, in units of 2^-14 (its
 // singular values stay under 1.3, so do its entries; the units keep what is 2^-28 of the largest out of fp16's subnormals), A and B in
 // units of 2^-13.  Parameters in 16 bits: the products take X's hi piece and A and B of one piece, and the term a X, which carries the small
-// singular values (they grow by a in each step), all 22 bits but for the last step's.  Against the exact iteration that is off by 1.6e-3 of the
-// result for matrices of independent entries and less where singular values differ by much; with one piece everywhere those cases lose up
-// to 4e-2, with bf16 operands 3e-1.  Parameters in fp32: A and B have two pieces, too, and every product is three, lo hi + hi lo +
-// hi hi, which is fp32's precision at a third of the rate.
+// singular values (they grow by a in each step), all 22 bits but for the last step's.  The largest entries of B are its diagonal's: what their rounding
+// leaves is kept in fp32 and multiplied with X's hi piece beside that term (66 rows: 1.96e-3 of the result -> 1.5e-3).  Against the exact
+// iteration that is off by 0.9 to 1.5e-3 of the result for matrices of independent entries and up to 1.8e-3 where few singular values are large; with one piece
+// everywhere those cases lose up to 4e-2, with bf16 operands 3e-1.  Parameters in fp32, and results in fp16, whose own rounding is 2e-4: A and B have two
+// pieces, too, and every product is three, lo hi + hi lo + hi hi, which is fp32's precision at a third of the rate.
 #include <math.h>
 
 #include <algorithm>
@@ -198,7 +199,8 @@ __device__ __forceinline__ void store_pieces8(uint16_t* hi, int64_t lo_plane, co
     *reinterpret_cast<u32x4*>(hi + lo_plane) = Elem<TRLK_F16>::pack(l);
 }
 
-// X in two pieces, a tile of 64 x 64 a workgroup, turned over where the parameter is tall; the zeros around X, A and B.
+// X in two pieces, a tile of 64 x 64 a workgroup, turned over where the parameter is tall; the zeros around X, A and B.  HBM bound: of a 4096-wide model's
+// four layers, 671 M entries of bf16, 1417 us, 4.7 TB/s; the momentum's pass before it 1219, 5.5 TB/s.
 template <int DT>
 __global__ __launch_bounds__(kThreads) void make_x_kernel(const Mat* mats, int n_mats, const float* factor) {
     __shared__ float tile[kTurn][kTurn + 1];
@@ -730,8 +732,8 @@ __global__ __launch_bounds__(Tile::kThreads) __attribute__((amdgpu_waves_per_eu(
 // m x m: X is read once for G and once for T X, the steps are products of m x m matrices in one workgroup's LDS,
 //   P = a + b G + c G G,  T = P T,  G = P G P.
 // G squares the singular values: what X holds in 24 bits needs 48 in G, so all of this is in 64 bits (fp64 runs at full rate here, and there is
-// little of it: 224 adapters of rank 16 with 9M entries take 0.3 GFLOP).  Bound by the memory, and by launches: three and the tables instead of
-// the 18 of the larger matrices' way.
+// little of it).  Bound by the memory and by launches, three and the tables instead of the 18 of the larger matrices' way: 224 adapters of rank 16 with
+// 9 M entries 121 us, 30 of them G's sums, 10 the steps, 49 T X and the parameters, 17 the tables.
 constexpr int kNarrow = 64;          // rows at most
 constexpr int kCols = 128;           // columns of u at a time in LDS, and of a workgroup that applies T
 constexpr int kSpan = 2 * kCols;     // of one that sums for G

@@ -27,9 +27,10 @@ def orthogonalize(matrices: Tensor | Sequence[Tensor], *, ns_coefficients: tuple
     `X = U / max(|U|, eps)` (Frobenius norm), `ns_steps` times `A = X X^T; X = a X + (b A + c A A) X`.  The singular vectors stay, each singular
     value s moves by `a s + b s^3 + c s^5`; the usual coefficients bring all but the smallest to between 0.7 and 1.2 in five steps.
 
-    `matrices` is one tensor `[..., m, n]` or a list of them (then a list is returned), in fp32, bf16 or fp16: all in one call.  In 16 bits the
-    products round their operands to 11 bits and the result is within 2e-3 of the exact iteration's (2-norm); in fp32 they hold 22 bits.  A matrix of zeros gives
-    zeros, one with a NaN or an infinity NaN.  Coefficients with which values of at most 1 would grow past 2.5 raise.  Not differentiable."""
+    `matrices` is one tensor `[..., m, n]` or a list of them (then a list is returned), in fp32, bf16 or fp16, all on one GPU: all in one call.  In bf16
+    the products round their operands to 11 bits and the result is within 2e-3 of the exact iteration's (2-norm) before it is rounded; in fp32 and fp16
+    they hold 22 bits.  A matrix of zeros gives zeros, one with a NaN or an infinity NaN.  Coefficients with which values of at most 1 would grow
+    past 2.5 raise.  Not differentiable."""
     numbers = _numbers(ns_coefficients, ns_steps, eps)
     if isinstance(matrices, Tensor):
         return ops.orthogonalize([matrices], *numbers)[0]
@@ -46,8 +47,8 @@ def muon_step_(params: list[Tensor], grads: list[Tensor], momentum_buffers: list
 
     `momentum_buffers` are fp32.  `stretch` is `sqrt(max(1, m / n))` (`adjust_lr_fn` None or "original") or `0.2 sqrt(max(m, n))`
     ("match_rms_adamw", with which learning rates are those of AdamW).  `lr` may be an fp32 number on the GPU.  Parameters are rounded once;
-    those in fp32 take their update from products of 22 bits, see `orthogonalize`.  Tensors that are written share no memory, with each other or with
-    a gradient."""
+    those in fp32 take their update from products of 22 bits, those in 16 bits from ones of 11, see `orthogonalize`.  Tensors that are written share
+    no memory, with each other or with a gradient."""
     if not len(params):
         raise ValueError("muon_step_: no parameters")
     on_gpu = isinstance(lr, Tensor) and lr.is_cuda
@@ -87,7 +88,8 @@ class Muon(torch.optim.Optimizer):
     Groups with `adamw=True` are stepped by `adamw_step_` in the same call of `step`, with `betas` and `adamw_eps`: embeddings, head, norms and
     biases, so that one optimiser (and one learning-rate schedule) serves a whole model; `muon_param_groups` makes such groups, and
     `adjust_lr_fn="match_rms_adamw"` lets both kinds share a learning rate.  A group's `lr` may be an fp32 number on the GPU, and step counters
-    live there: a step can be captured into a graph.  Parameters without a gradient are left alone.  Momentum and moments are fp32."""
+    live there: a step can be captured into a graph.  Parameters without a gradient are left alone.  Momentum and moments are fp32.  All of a call's
+    parameters are on one GPU; it takes up to 8 GiB of workspace, or what the largest matrix needs."""
 
     def __init__(self, params, lr: float | Tensor = 1e-3, weight_decay: float = 0.1, momentum: float = 0.95, nesterov: bool = True,
                  ns_coefficients: tuple[float, float, float] = NS_COEFFICIENTS, eps: float = 1e-7, ns_steps: int = 5,
