@@ -103,8 +103,9 @@ def test_gradient(dtype, tokens):
 
 
 @pytest.mark.parametrize("tokens,vocab", [(1024, 300), (1025, 300), (8191, 1 << 20), (8193, (1 << 20) - 1), (32768, 1 << 18), (32768, (1 << 20) - 1),
-                                          (32769, 1000), (40000, 3), (70000, 1 << 21), (5000, 1 << 21)])
-def test_sorted_by_one_workgroup_or_many(tokens, vocab):
+                                          (32769, 1000), (40000, 3), (70000, 1 << 21), (5000, 1 << 21), (16384, (1 << 18) - 1), (16384, 1 << 18),
+                                          (16385, 1000), (8192, (1 << 19) - 1), (8192, 1 << 19), (1055, 1)])
+def test_every_way_of_ordering(tokens, vocab):
     """Every way the tokens are brought into order, with ids all over the table, rare ones and very common ones."""
     import trl_amd
 

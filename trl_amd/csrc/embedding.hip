@@ -8,7 +8,7 @@
 // matter of chance, and in 16 bits round at every addition.  So the tokens are sorted by id (a stable radix sort of (id, position)
 // pairs, 9 bits a pass at most): the rows of one id are neighbours in the order of their positions, one wave adds them up in
 // registers and writes the table's row once.  1000 tokens into a table of 50257 x 1150 in fp16 30 us, 32768 into one of 151936 x 4096 in bf16 332 (213 of
-// them the table's zeros, at 5.8 TB/s); added, 8192 into one of 256000 x 2048 52.
+// them the table's zeros, at 5.8 TB/s); added, 8192 into one of 256000 x 2048 40.
 #include <algorithm>
 #include <atomic>
 
@@ -145,11 +145,10 @@ struct SortArgs {
 };
 
 // Lanes of the wave with the same digit, as a mask.
-template <int MOST>
 __device__ __forceinline__ uint64_t peers(uint32_t digit, int bits) {
     uint32_t lo = ~0u, hi = ~0u;
 #pragma unroll
-    for (int b = 0; b < MOST; ++b) {
+    for (int b = 0; b < kMaxDigit; ++b) {
         if (b < bits) {  // (uniform)
             const uint32_t one = uint32_t(int32_t(digit << (31 - b)) >> 31);  // the bit in all places
             const uint64_t ones = __ballot(one != 0u);
@@ -171,7 +170,7 @@ __device__ __forceinline__ void wave_ranks(const uint32_t (&key)[kSortRows], int
         if (uint32_t(r) < n_rows) {  // (uniform in the wave)
             const bool live = uint32_t(r * kWave + lane) < last;
             const uint32_t digit = (key[r] >> shift) & low;
-            const uint64_t same = peers<kMaxDigit>(digit, bits) & __ballot(live);
+            const uint64_t same = peers(digit, bits) & __ballot(live);
             const uint16_t before = count[digit];
             __builtin_amdgcn_wave_barrier();
             rank[r] = before + uint32_t(__popcll(same & ((uint64_t(1) << lane) - 1)));
@@ -280,95 +279,51 @@ __global__ __launch_bounds__(kThreads) void sort_place_kernel(SortArgs a) {
     }
 }
 
-// ---- up to 8192 tokens: sorted by one workgroup, in its LDS -----------------------------------------------------------------
-// Two passes of up to 10 bits.  The first one's result is what the second needs, the upper digit and the position (13 bits), one word a token; the
-// ids themselves are looked up again at the end.  A wave takes consecutive tokens, 8 rows of 64 at most.  Bound by the ranks' instructions
-// on one CU: 8192 tokens, 18 bits 23 us, with six launches of the kernels above 28 and their gaps.
-constexpr int kOneThreads = 1024, kOneWaves = kOneThreads / kWave;
-constexpr int kOneRows = 8, kOneBits = 10;
+// ---- up to 16384 tokens: every token's place is counted ----------------------------------------------------------------------
+// A token's place is the number of words (id, position), in 32 bits, that are smaller than its own.  A workgroup holds all words in LDS and counts
+// for 32 tokens, 32 lanes each; n^2 comparisons, two instructions, are few for 256 CUs: 8192 tokens 11 us, where one workgroup's radix sort takes 23 and the
+// six launches of the kernels above 28 and their gaps (an added gradient of 1024 bf16 columns, us a call, so and by those launches: 2048 tokens 18 and 34, 8192
+// 35 and 50, 12000 56 and 62, 16384 64 and 67).
+constexpr int kRankThreads = 1024, kRankTokens = 32, kRankSlices = kRankThreads / kRankTokens;
+constexpr int64_t kMostRanked = 16384;
 
-struct OneArgs {
+struct RankArgs {
     KeyArgs source;
     uint32_t *key, *at;
     uint32_t n;
-    int32_t bits;  // of a pass
+    int32_t bits;  // of a position
 };
-constexpr int one_lds_bytes(int bits) { return kOneRows * kOneThreads * 4 + (kOneWaves * 2 << bits); }
+constexpr int rank_words(int64_t n) { return int(n + kRankSlices * 4 - 1) / (kRankSlices * 4) * (kRankSlices * 4); }
 
-__global__ __launch_bounds__(kOneThreads) void sort_one_kernel(OneArgs a) {
-    extern __shared__ __attribute__((aligned(16))) char smem[];
-    uint32_t* words = reinterpret_cast<uint32_t*>(smem);
-    uint16_t* counts = reinterpret_cast<uint16_t*>(smem + kOneRows * kOneThreads * 4);  // [wave][bin]
-    __shared__ uint32_t part[kOneWaves];
-    const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave, n_bins = 1 << a.bits;
-    const uint32_t rows = (a.n + kOneThreads - 1) / kOneThreads, begin = wave * rows * kWave;
-    const uint32_t left = begin < a.n ? a.n - begin : 0u, low = uint32_t(n_bins) - 1u;
-    uint32_t word[kOneRows], rank[kOneRows];
-    volatile uint16_t* mine = counts + wave * n_bins;
-#pragma unroll 1
-    for (int pass = 0; pass < 2; ++pass) {
-        for (int b = threadIdx.x; b < kOneWaves * n_bins / 2; b += kOneThreads) reinterpret_cast<uint32_t*>(counts)[b] = 0;
-#pragma unroll
-        for (int r = 0; r < kOneRows; ++r) {
-            const uint32_t i = r * kWave + lane;
-            word[r] = 0;
-            if (uint32_t(r) < rows && i < left) word[r] = pass == 0 ? a.source.key(begin + i) : words[begin + i];
-        }
-        __syncthreads();
-#pragma unroll
-        for (int r = 0; r < kOneRows; ++r) {
-            if (uint32_t(r) < rows) {
-                const bool live = uint32_t(r * kWave + lane) < left;
-                const uint32_t digit = pass == 0 ? word[r] & low : word[r] >> 13;
-                const uint64_t same = peers<kOneBits>(digit, a.bits) & __ballot(live);
-                const uint16_t before = mine[digit];
-                __builtin_amdgcn_wave_barrier();
-                rank[r] = before + uint32_t(__popcll(same & ((uint64_t(1) << lane) - 1)));
-                if (live && (same >> lane) == 1) mine[digit] = uint16_t(before + __popcll(same));  // (the last of them)
-                __builtin_amdgcn_wave_barrier();
-            }
-        }
-        __syncthreads();
-        // exclusive sums, bin by bin and wave by wave (all under 32768)
-        uint32_t sum = 0;
-        if (int(threadIdx.x) < n_bins)
-#pragma unroll
-            for (int w = 0; w < kOneWaves; ++w) sum += counts[w * n_bins + threadIdx.x];
-        uint32_t upto = sum;
-#pragma unroll
-        for (int o = 1; o < kWave; o <<= 1) {
-            const uint32_t y = __shfl_up(upto, o);
-            if (lane >= o) upto += y;
-        }
-        if (lane == kWave - 1) part[wave] = upto;
-        __syncthreads();
-        uint32_t to = upto - sum;
-        for (int w = 0; w < wave; ++w) to += part[w];
-        if (int(threadIdx.x) < n_bins)
-#pragma unroll
-            for (int w = 0; w < kOneWaves; ++w) {
-                const uint32_t c = counts[w * n_bins + threadIdx.x];
-                counts[w * n_bins + threadIdx.x] = uint16_t(to);
-                to += c;
-            }
-        __syncthreads();
-        KeyArgs quiet = a.source;
-        quiet.flag = nullptr;  // (raised before)
-#pragma unroll
-        for (int r = 0; r < kOneRows; ++r) {
-            const uint32_t i = r * kWave + lane;
-            if (uint32_t(r) < rows && i < left) {
-                if (pass == 0) {
-                    words[mine[word[r] & low] + rank[r]] = word[r] >> a.bits << 13 | (begin + i);
-                } else {
-                    const uint32_t place = mine[word[r] >> 13] + rank[r], at = word[r] & 0x1fffu;
-                    a.key[place] = quiet.key(at);
-                    a.at[place] = at;
-                }
-            }
-        }
-        __syncthreads();
+__global__ __launch_bounds__(kRankThreads) void rank_kernel(RankArgs a) {
+    extern __shared__ __attribute__((aligned(16))) uint32_t words[];
+    __shared__ uint32_t counts[kRankThreads / kWave][kRankTokens];
+    KeyArgs source = a.source;
+    if (blockIdx.x != 0) source.flag = nullptr;
+    const uint32_t padded = uint32_t(rank_words(a.n));
+#pragma unroll 4
+    for (uint32_t i = threadIdx.x; i < padded; i += kRankThreads) words[i] = i < a.n ? source.key(i) << a.bits | i : ~0u;
+    __syncthreads();
+    const uint32_t slice = threadIdx.x / kRankTokens, token = blockIdx.x * kRankTokens + threadIdx.x % kRankTokens;
+    const uint32_t mine = token < a.n ? words[token] : 0u;
+    uint32_t count = 0;
+#pragma unroll 4
+    for (uint32_t at = slice * 4; at < padded; at += kRankSlices * 4) {
+        const u32x4 q = *reinterpret_cast<const u32x4*>(words + at);
+        count += q.x < mine;
+        count += q.y < mine;
+        count += q.z < mine;
+        count += q.w < mine;
     }
+    count += __shfl_xor(count, kRankTokens);
+    if ((threadIdx.x & kRankTokens) == 0) counts[threadIdx.x / kWave][threadIdx.x % kRankTokens] = count;
+    __syncthreads();
+    if (threadIdx.x >= kRankTokens || token >= a.n) return;
+    uint32_t place = 0;
+#pragma unroll
+    for (int w = 0; w < kRankThreads / kWave; ++w) place += counts[w][threadIdx.x];
+    a.key[place] = mine >> a.bits;
+    a.at[place] = token;
 }
 
 // ---- the table's zeros --------------------------------------------------------------------------------------------------
@@ -577,7 +532,8 @@ __global__ __launch_bounds__(kThreads) void grad_rows_kernel(GradArgs a) {
 }
 
 // Up to 1024 tokens need no order: a workgroup for each token looks at all ids, returns if its own occurs before, else lists where it
-// occurs and adds those rows up.  One launch: 256 tokens of 1024 columns 6 us, sorted first 23.
+// occurs and adds those rows up.  One launch: 256 tokens of 1024 columns 6.2 us, 1024 12.6;
+// with their places counted first 11.7 and 16.8.
 constexpr int64_t kMostDirect = 1024;
 template <int GDT, int ODT, bool ADD, bool NARROW>
 __global__ __launch_bounds__(kThreads) void grad_direct_kernel(GradArgs a) {
@@ -637,7 +593,7 @@ int key_bits(int64_t vocab) {
     while (bits < 32 && (uint64_t(vocab) >> bits) != 0) ++bits;  // (the keys go up to `vocab`)
     return bits;
 }
-bool by_one(int64_t n, int64_t vocab) { return n <= kOneRows * kOneThreads && key_bits(vocab) <= 2 * kOneBits; }
+bool ranked(int64_t n, int64_t vocab) { return n <= kMostRanked && key_bits(vocab) + key_bits(n - 1) <= 32; }
 
 // A further level from 512 chunks on: below, a wave adds them up itself (4096 rows of 4096, 60 % of one id, 98 us).
 int levels_of(int64_t n) {
@@ -656,7 +612,7 @@ struct Layout {
     size_t each, counts, part, total;
     Layout(int64_t n, int64_t vocab, int64_t cols) {
         each = up16(size_t(n) * 4);
-        counts = by_one(n, vocab) ? 0 : 2 * each + up16(size_t(ceil_div(n, kSortTile)) * kBins * 4);
+        counts = ranked(n, vocab) ? 0 : 2 * each + up16(size_t(ceil_div(n, kSortTile)) * kBins * 4);
         part = 2 * each + counts;
         total = n <= kMostDirect ? 16 : part + up16(size_t(chunks_of(n, levels_of(n))) * size_t(cols) * 4);
     }
@@ -672,18 +628,18 @@ ZeroArgs zero_args(void* to, int64_t bytes) {
     z.head_bytes = int32_t(head), z.tail_bytes = int32_t(bytes - head - z.vecs * 16);
     return z;
 }
-int launch_one(const OneArgs& a, hipStream_t stream) {
+int launch_rank(const RankArgs& a, hipStream_t stream) {
     static std::atomic<uint64_t> reserved{0};  // a bit for each device
     int device = 0;
     if (hipGetDevice(&device) != hipSuccess) device = 0;
     const uint64_t bit = device < 64 ? uint64_t(1) << device : 0;
     if (!(reserved.load() & bit)) {
-        const int most = one_lds_bytes(kOneBits);
-        const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(sort_one_kernel), hipFuncAttributeMaxDynamicSharedMemorySize, most);
-        if (e != hipSuccess) return fail(int(e), "embedding_bwd: cannot reserve %d bytes of LDS: %s", most, hipGetErrorString(e));
+        constexpr int kBytes = rank_words(kMostRanked) * 4;
+        const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(rank_kernel), hipFuncAttributeMaxDynamicSharedMemorySize, kBytes);
+        if (e != hipSuccess) return fail(int(e), "embedding_bwd: cannot reserve %d bytes of LDS: %s", kBytes, hipGetErrorString(e));
         reserved.fetch_or(bit);
     }
-    sort_one_kernel<<<1, kOneThreads, one_lds_bytes(a.bits), stream>>>(a);
+    rank_kernel<<<unsigned(ceil_div(a.n, kRankTokens)), kRankThreads, rank_words(a.n) * 4, stream>>>(a);
     return TRLK_OK;
 }
 
@@ -800,7 +756,7 @@ extern "C" int trlk_embedding_bwd(const void* d_grad, int dtype, int64_t n, int6
     TRLK_REQUIRE(n == 0 || (d_workspace && workspace_bytes >= trlk_embedding_bwd_workspace_bytes(n, vocab, cols) && aligned_to(d_workspace, 16)),
                  TRLK_ERR_WORKSPACE, "embedding_bwd: workspace too small or misaligned");
     const hipStream_t stream = static_cast<hipStream_t>(stream_);
-    const bool direct = n <= kMostDirect, one = !direct && by_one(n, vocab);
+    const bool direct = n <= kMostDirect, by_rank = !direct && ranked(n, vocab);
     const KeyArgs source{Ids{d_ids, id_bits == 64}, vocab, padding_idx, d_error_flag};
     const Layout layout(n, vocab, cols);
     char* ws = static_cast<char*>(d_workspace);
@@ -811,11 +767,10 @@ extern "C" int trlk_embedding_bwd(const void* d_grad, int dtype, int64_t n, int6
         zero_kernel<<<unsigned(std::min(need, kMaxGroups)), kThreads, 0, stream>>>(z);
     }
     if (n == 0) return launch_status("embedding_bwd");
-    if (one) {
-        const int digit = (key_bits(vocab) + 1) / 2;
-        const OneArgs o{source, reinterpret_cast<uint32_t*>(ws), reinterpret_cast<uint32_t*>(ws + layout.each), uint32_t(n), digit};
-        if (const int rc = launch_one(o, stream)) return rc;
-        a.key = o.key, a.at = o.at;
+    if (by_rank) {
+        const RankArgs r{source, reinterpret_cast<uint32_t*>(ws), reinterpret_cast<uint32_t*>(ws + layout.each), uint32_t(n), key_bits(n - 1)};
+        if (const int rc = launch_rank(r, stream)) return rc;
+        a.key = r.key, a.at = r.at;
     } else if (!direct) {
         sort_tokens(source, n, ws, layout, stream, &a.key, &a.at);
     }
