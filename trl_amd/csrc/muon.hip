@@ -58,6 +58,23 @@ struct Mat {
     __device__ __forceinline__ float* rest_of_b() const { return reinterpret_cast<float*>(b() + square()); }  // (one piece)
 };
 
+// A pointer into global memory.  One that comes from a table in memory may point anywhere, for all that the compiler knows: its loads would be flat ones, and
+// whoever uses one would wait for all loads in flight.
+template <typename T>
+__device__ __forceinline__ T* global(T* p) {
+    typedef __attribute__((address_space(1))) T* Global;
+    return (T*)(Global)reinterpret_cast<uint64_t>(p);
+}
+__device__ __forceinline__ Mat mat_at(const Mat* mats, int i) {
+    Mat e = mats[i];
+    e.x = global(e.x);
+    e.p = global(static_cast<char*>(e.p));
+    e.g = global(static_cast<const char*>(e.g));
+    e.momentum = e.momentum ? global(e.momentum) : nullptr;
+    e.d_lr = e.d_lr ? global(e.d_lr) : nullptr;
+    return e;
+}
+
 constexpr int kTable = 34;
 struct MatTable {
     Mat e[kTable];
@@ -106,7 +123,7 @@ __device__ __forceinline__ void load8(const typename Elem<DT>::type* p, float (&
 template <int DT>
 __global__ __launch_bounds__(kThreads) void momentum_kernel(const Mat* mats, int n_mats, double* partial) {
     __shared__ double scratch[kThreads / kWave];
-    const Mat e = mats[mat_of(mats, n_mats, blockIdx.x, FirstChunk{})];
+    const Mat e = mat_at(mats, mat_of(mats, n_mats, blockIdx.x, FirstChunk{}));
     const int64_t numel = int64_t(e.m) * e.n, begin = int64_t(blockIdx.x - e.first_chunk) * kChunk;
     const auto* g = static_cast<const typename Elem<DT>::type*>(e.g);
     double s = 0.0;
@@ -205,7 +222,7 @@ template <int DT>
 __global__ __launch_bounds__(kThreads) void make_x_kernel(const Mat* mats, int n_mats, const float* factor) {
     __shared__ float tile[kTurn][kTurn + 1];
     const int i = mat_of(mats, n_mats, blockIdx.x, FirstTurn{});
-    const Mat e = mats[i];
+    const Mat e = mat_at(mats, i);
     const float f = factor[i];
     const auto* g = static_cast<const typename Elem<DT>::type*>(e.g);
     const uint32_t t = blockIdx.x - e.first_turn, across = uint32_t(e.npad / kTurn);
@@ -538,7 +555,7 @@ __global__ __launch_bounds__(Tile::kThreads) __attribute__((amdgpu_waves_per_eu(
     const int64_t piece = xcd_piece(blockIdx.x, args.run);
     if (piece >= args.tiles) return;
     const auto first = [](const Mat& e) { return (kSquare ? e.first_half : e.first_tile)[kWhich]; };
-    const Mat e = args.mats[mat_of(args.mats, args.n, uint32_t(piece), first)];
+    const Mat e = mat_at(args.mats, mat_of(args.mats, args.n, uint32_t(piece), first));
     const int index = int(uint32_t(piece) - first(e));
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int wr = Tile::wave_row(wave), wc = Tile::wave_col(wave);
@@ -814,7 +831,7 @@ __global__ __launch_bounds__(kThreads) void gram_kernel(const Mat* mats, int n_m
     constexpr int kTileBytes = MP * kLine * 4, kSumBytes = kSlices > 1 ? kSlices * MP * MP * 8 : 0;
     __shared__ __attribute__((aligned(16))) char smem[kTileBytes > kSumBytes ? kTileBytes : kSumBytes];
     float* tile = reinterpret_cast<float*>(smem);
-    const Mat e = mats[mat_of(mats, n_mats, blockIdx.x, FirstChunk{})];
+    const Mat e = mat_at(mats, mat_of(mats, n_mats, blockIdx.x, FirstChunk{}));
     const int chunk = int(blockIdx.x - e.first_chunk), slice = threadIdx.x / kBlocks, block = threadIdx.x % kBlocks;
     const int bi = block / (MP / 4) * 4, bj = block % (MP / 4) * 4;
     double sum[4][4] = {};
@@ -885,7 +902,7 @@ __global__ __launch_bounds__(kThreads) void narrow_steps_kernel(const Mat* mats,
     constexpr int LD = MP + 1;
     extern __shared__ double buffers[];
     double *G = buffers, *P = G + MP * LD, *T = P + MP * LD, *W = T + MP * LD;
-    const Mat& e = mats[blockIdx.x];
+    const Mat e = mat_at(mats, blockIdx.x);
     const int chunks = (e.n + kSpan - 1) / kSpan;
     double* parts = reinterpret_cast<double*>(e.x);
     for (int k = threadIdx.x; k < MP * MP; k += kThreads) {
@@ -927,7 +944,7 @@ template <int DT, int MP>
 __global__ __launch_bounds__(kThreads) void narrow_apply_kernel(const Mat* mats, int n_mats) {
     static_assert(kThreads == 2 * kCols, "two lanes a column");
     __shared__ float tile[MP * kLine];
-    const Mat e = mats[mat_of(mats, n_mats, blockIdx.x, FirstTurn{})];
+    const Mat e = mat_at(mats, mat_of(mats, n_mats, blockIdx.x, FirstTurn{}));
     const int c0 = int(blockIdx.x - e.first_turn) * kCols, c = threadIdx.x % kCols;
     const int half = __builtin_amdgcn_readfirstlane(threadIdx.x / kCols);
     const double* T = reinterpret_cast<const double*>(e.x) + int64_t((e.n + kSpan - 1) / kSpan) * MP * MP + half * (MP / 2) * MP;
@@ -1004,36 +1021,45 @@ struct Group {
     size_t bytes = 0;
     size_t total() const { return up256(each.size() * sizeof(Mat)) + up256(each.size() * sizeof(float)) + up256(size_t(chunks) * sizeof(double)) + bytes; }
 };
-// (the longest contractions first, so that a launch's last workgroups are short ones)
 std::vector<Group> groups_of(const trlk_muon_matrix* x, int32_t n) {
+    constexpr int kTypes = 3, kKinds = 4;  // fp32, bf16, fp16; matrices of any size and the three narrow kinds
+    std::vector<int32_t> each[kTypes * kKinds];
+    for (int32_t i = 0; i < n; ++i) {
+        if (x[i].rows == 0 || x[i].cols == 0) continue;
+        const int type = x[i].dtype == TRLK_F32 ? 0 : x[i].dtype == TRLK_BF16 ? 1 : 2, rows = narrow_rows(x[i]);
+        each[type * kKinds + (rows == 0 ? 0 : rows == 16 ? 1 : rows == 32 ? 2 : 3)].push_back(i);
+    }
+    // (the longest contractions first, so that a launch's last workgroups are short ones)
+    for (int type = 0; type < kTypes; ++type) {
+        std::vector<int32_t>& order = each[type * kKinds];
+        std::stable_sort(order.begin(), order.end(), [&](int32_t i, int32_t j) {
+            const int64_t mi = std::min(x[i].rows, x[i].cols), mj = std::min(x[j].rows, x[j].cols), ni = std::max(x[i].rows, x[i].cols), nj = std::max(x[j].rows, x[j].cols);
+            return ni != nj ? ni > nj : mi > mj;
+        });
+    }
     std::vector<Group> groups;
-    std::vector<int32_t> order;
-    for (int dtype : {int(TRLK_F32), int(TRLK_BF16), int(TRLK_F16)})
-        for (int narrow : {0, 16, 32, 64}) {
-            order.clear();
-            for (int32_t i = 0; i < n; ++i)
-                if (x[i].dtype == dtype && x[i].rows > 0 && x[i].cols > 0 && narrow_rows(x[i]) == narrow) order.push_back(i);
-            std::stable_sort(order.begin(), order.end(), [&](int32_t i, int32_t j) {
-                const int64_t mi = std::min(x[i].rows, x[i].cols), mj = std::min(x[j].rows, x[j].cols), ni = std::max(x[i].rows, x[i].cols), nj = std::max(x[j].rows, x[j].cols);
-                return ni != nj ? ni > nj : mi > mj;
-            });
-            bool fresh = true;
-            for (const int32_t i : order) {
-                const size_t need = matrix_bytes(x[i]);
-                if (fresh || groups.back().bytes + need > kGroupBytes) groups.emplace_back();
-                fresh = false;
-                groups.back().narrow = narrow;
-                groups.back().each.push_back(i);
-                groups.back().chunks += narrow ? 0 : ceil_div(x[i].rows * x[i].cols, kChunk);
-                groups.back().bytes += need;
+    for (const std::vector<int32_t>& order : each) {
+        bool fresh = true;
+        for (const int32_t i : order) {
+            const size_t need = matrix_bytes(x[i]);
+            if (fresh || groups.back().bytes + need > kGroupBytes) {
+                groups.emplace_back();
+                groups.back().narrow = narrow_rows(x[i]);
+                groups.back().each.reserve(order.size());
             }
+            fresh = false;
+            Group& g = groups.back();
+            g.each.push_back(i);
+            g.chunks += g.narrow ? 0 : ceil_div(x[i].rows * x[i].cols, kChunk);
+            g.bytes += need;
         }
+    }
     return groups;
 }
 
-size_t most_bytes(const trlk_muon_matrix* x, int32_t n) {
+size_t most_bytes(const std::vector<Group>& groups) {
     size_t most = 0;
-    for (const Group& g : groups_of(x, n)) most = std::max(most, g.total());
+    for (const Group& g : groups) most = std::max(most, g.total());
     return most;
 }
 
@@ -1226,13 +1252,14 @@ int run(const trlk_muon_matrix* x, int32_t n, const trlk_muon_group* groups, int
         size_t workspace_bytes, trlk_stream_t stream_, const char* what) {
     if (const int rc = check_matrices(x, n, groups, n_groups, step, what)) return rc;
     if (const int rc = check_numbers(num, what)) return rc;
-    const size_t need = n ? most_bytes(x, n) : 0;
+    const std::vector<Group> all = groups_of(x, n);
+    const size_t need = most_bytes(all);
     if (need == 0) return TRLK_OK;
     TRLK_REQUIRE(d_workspace && workspace_bytes >= need, TRLK_ERR_WORKSPACE, "%s: workspace too small", what);
     TRLK_REQUIRE(aligned_to(d_workspace, 256), TRLK_ERR_WORKSPACE, "%s: misaligned workspace", what);
     const hipStream_t stream = static_cast<hipStream_t>(stream_);
     char* ws = static_cast<char*>(d_workspace);
-    for (const Group& g : groups_of(x, n)) {
+    for (const Group& g : all) {
         const int dtype = x[g.each[0]].dtype;
         const trlk_muon_group* hyper = step ? groups : nullptr;
         const int rc = dtype == TRLK_F32    ? run_group<TRLK_F32, true>(g, x, hyper, num, ws, stream, what)
@@ -1266,7 +1293,7 @@ extern "C" size_t trlk_muon_workspace_bytes(const trlk_muon_matrix* matrices, in
         if (!size_ok(matrices[i])) return 0;
     size_t most = 0;
     guarded("muon", [&] {
-        most = most_bytes(matrices, n_matrices);
+        most = most_bytes(groups_of(matrices, n_matrices));
         return TRLK_OK;
     });
     return most;
