@@ -369,6 +369,34 @@ def test_graph_capture(dtype):
         assert all(torch.equal(x, y) for x, y in zip(p + m, q + k))
 
 
+def test_through_the_operator_or_past_it():
+    """A dispatch mode sees the operator; tuples are no lists of plain tensors.  The results are the same to the last bit."""
+    from torch.utils._python_dispatch import TorchDispatchMode
+
+    import trl_amd
+
+    seen = []
+
+    class Watch(TorchDispatchMode):
+        def __torch_dispatch__(self, func, types, args=(), kwargs=None):
+            seen.append(str(func))
+            return func(*args, **(kwargs or {}))
+
+    lr = torch.tensor(0.1, device=DEV)
+    results = []
+    for way in ("past", "mode", "tuples"):
+        p, g, m = make([(20, 30), (90, 80), (0, 3)], torch.bfloat16, 4)
+        if way == "mode":
+            with Watch():
+                trl_amd.muon_step_(p, g, m, lr=lr)
+        else:
+            trl_amd.muon_step_(p if way == "past" else tuple(p), g, m, lr=lr)
+        results.append(p + m)
+    assert any("muon_step_" in name for name in seen)
+    for other in results[1:]:
+        assert all(torch.equal(x, y) for x, y in zip(results[0], other))
+
+
 def test_versions_and_inference_tensors():
     import trl_amd
 

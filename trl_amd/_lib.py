@@ -230,6 +230,9 @@ _load_torch_ops()
 # the AdamW step for lists of plain tensors, past the dispatcher; called with the GIL held, raises Python exceptions
 py_adamw_step = ctypes.PyDLL(TORCH_LIB_PATH).trlk_py_adamw_step
 py_adamw_step.restype, py_adamw_step.argtypes = ctypes.py_object, [ctypes.py_object]
+# the same of the orthogonalised updates
+py_muon_step = ctypes.PyDLL(TORCH_LIB_PATH).trlk_py_muon_step
+py_muon_step.restype, py_muon_step.argtypes = ctypes.py_object, [ctypes.py_object]
 
 
 def last_error() -> str:

@@ -7,8 +7,8 @@
 // to a gradient that is there, reads and writes the rows that occur.  Atomics would make the sums' order, and their last bits, a
 // matter of chance, and in 16 bits round at every addition.  So the tokens are sorted by id (a stable radix sort of (id, position)
 // pairs, 9 bits a pass at most): the rows of one id are neighbours in the order of their positions, one wave adds them up in
-// registers and writes the table's row once.  1000 tokens into a table of 50257 x 1150 in fp16 30 us, 32768 into one of 151936 x 4096 in bf16 332 (213 of
-// them the table's zeros, at 5.8 TB/s); added, 8192 into one of 256000 x 2048 40.
+// registers and writes the table's row once.  1000 tokens into a table of 50257 x 1150 in fp16 30 us, 32768 into one of 151936 x 4096 in bf16 316 (209 of
+// them the table's zeros, at 5.9 TB/s); added, 8192 into one of 256000 x 2048 40.
 #include <algorithm>
 #include <atomic>
 

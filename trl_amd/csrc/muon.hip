@@ -750,7 +750,7 @@ __global__ __launch_bounds__(Tile::kThreads) __attribute__((amdgpu_waves_per_eu(
 //   P = a + b G + c G G,  T = P T,  G = P G P.
 // G squares the singular values: what X holds in 24 bits needs 48 in G, so all of this is in 64 bits (fp64 runs at full rate here, and there is
 // little of it).  Bound by the memory and by launches, three and the tables instead of the 18 of the larger matrices' way: 224 adapters of rank 16 with
-// 9 M entries 121 us, 30 of them G's sums, 10 the steps, 49 T X and the parameters, 17 the tables.
+// 9 M entries 93 us, 30 of them G's sums, 10 the steps, 30 T X and the parameters, 17 the tables.
 constexpr int kNarrow = 64;          // rows at most
 constexpr int kCols = 128;           // columns of u at a time in LDS, and of a workgroup that applies T
 constexpr int kSpan = 2 * kCols;     // of one that sums for G

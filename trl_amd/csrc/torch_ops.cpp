@@ -1145,6 +1145,29 @@ extern "C" __attribute__((visibility("default"))) PyObject* trlk_py_adamw_step(P
     END_HANDLE_TH_ERRORS
 }
 
+// The same for the orthogonalised updates' step; True where it has been done.
+extern "C" __attribute__((visibility("default"))) PyObject* trlk_py_muon_step(PyObject* args) {
+    HANDLE_TH_ERRORS
+    PyObject *lists[4], *groups, *numbers[2];
+    long long steps;
+    double eps;
+    if (!PyArg_ParseTuple(args, "OOOOOOOLd", &lists[0], &lists[1], &lists[2], &groups, &numbers[0], &lists[3], &numbers[1], &steps, &eps)) return nullptr;
+    PyTensors tensors[4];
+    for (int i = 0; i < 4; ++i)
+        if (!tensors[i].take(lists[i])) Py_RETURN_NONE;
+    if (!PyList_Check(groups) || !PyList_Check(numbers[0]) || !PyList_Check(numbers[1])) Py_RETURN_NONE;
+    if (tensors[0].size() == 0 || !tensors[0][0].is_cuda()) Py_RETURN_NONE;
+    std::vector<int64_t> group_of;
+    std::vector<double> hyper, coefficients;
+    for (Py_ssize_t i = 0; i < PyList_GET_SIZE(groups); ++i) group_of.push_back(PyLong_AsLongLong(PyList_GET_ITEM(groups, i)));
+    for (Py_ssize_t i = 0; i < PyList_GET_SIZE(numbers[0]); ++i) hyper.push_back(PyFloat_AsDouble(PyList_GET_ITEM(numbers[0], i)));
+    for (Py_ssize_t i = 0; i < PyList_GET_SIZE(numbers[1]); ++i) coefficients.push_back(PyFloat_AsDouble(PyList_GET_ITEM(numbers[1], i)));
+    if (PyErr_Occurred()) return nullptr;
+    muon_step(tensors[0], tensors[1], tensors[2], group_of, hyper, tensors[3], coefficients, steps, eps);
+    Py_RETURN_TRUE;
+    END_HANDLE_TH_ERRORS
+}
+
 TORCH_LIBRARY_FRAGMENT(trl_amd, m) {
     m.def("error_flag(int device_index) -> Tensor", error_flag);
     m.def("error_flags() -> Tensor[]", all_error_flags);

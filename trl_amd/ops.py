@@ -317,7 +317,14 @@ adamw_state_values = _native_op(
 # Lists with an entry for each parameter; `hyper` has lr, momentum, weight_decay, nesterov (0 or 1) and the adjustment (0: original, 1: match
 # AdamW's) of each group, `lrs` (may be empty) a learning rate on the GPU for each (an empty tensor: none), `group_of` (may be empty) the
 # parameters' groups.  Three coefficients, the number of steps and eps of the iteration.
-muon_step_ = _native_op("muon_step_", lambda params, grads, momentum_buffers, group_of, hyper, lrs, coefficients, steps, eps: None)
+_muon_step_op = _native_op("muon_step_", lambda params, grads, momentum_buffers, group_of, hyper, lrs, coefficients, steps, eps: None)
+
+
+def muon_step_(*args):
+    """The operator with these arguments; its kernels' entry point at once where nothing looks on that would want the operator."""
+    if _observed() or not _lib.py_muon_step(args):
+        _muon_step_op(*args)
+
 
 # The matrices of tensors [..., m, n], each in its own shape and type.
 orthogonalize = _native_op("orthogonalize", lambda matrices, coefficients, steps, eps: [torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in matrices])
