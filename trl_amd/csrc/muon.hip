@@ -87,14 +87,18 @@ __global__ __launch_bounds__(64) void table_kernel(MatTable t) {
     for (int i = threadIdx.x; i < t.n; i += 64) t.to[i] = t.e[i];
 }
 
-// the matrix of piece w
+// The matrix of piece w, all lanes of the wave at it: 64 places at a time, two loads one after the other for up to 4096 matrices
+// (a search by halves, eight for 224 adapters: their two passes 30.5 and 29.5 us, so 28.6 and 28.4).
 template <typename F>
 __device__ __forceinline__ int mat_of(const Mat* e, int n, uint32_t w, F first) {
-    int lo = 0, hi = n;
-    while (hi - lo > 1) {
-        const int mid = (lo + hi) >> 1;
-        if (first(e[mid]) <= w) lo = mid;
-        else hi = mid;
+    const int lane = threadIdx.x & (kWave - 1);
+    int lo = 0, left = n;  // it is one of lo .. lo + left - 1
+    while (left > 1) {
+        const int step = (left + kWave - 1) / kWave, i = lane * step;
+        const uint64_t upto = __ballot(i < left && first(e[lo + min(i, left - 1)]) <= w);
+        const int k = (__popcll(upto) - 1) * step;
+        lo += k;
+        left = min(step, left - k);
     }
     return lo;
 }
@@ -750,7 +754,7 @@ __global__ __launch_bounds__(Tile::kThreads) __attribute__((amdgpu_waves_per_eu(
 //   P = a + b G + c G G,  T = P T,  G = P G P.
 // G squares the singular values: what X holds in 24 bits needs 48 in G, so all of this is in 64 bits (fp64 runs at full rate here, and there is
 // little of it).  Bound by the memory and by launches, three and the tables instead of the 18 of the larger matrices' way: 224 adapters of rank 16 with
-// 9 M entries 93 us, 30 of them G's sums, 10 the steps, 30 T X and the parameters, 17 the tables.
+// 9 M entries 93 us, 29 of them G's sums, 10 the steps, 28 T X and the parameters, 17 the tables.
 constexpr int kNarrow = 64;          // rows at most
 constexpr int kCols = 128;           // columns of u at a time in LDS, and of a workgroup that applies T
 constexpr int kSpan = 2 * kCols;     // of one that sums for G
