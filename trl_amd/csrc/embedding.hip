@@ -7,8 +7,8 @@
 // to a gradient that is there, reads and writes the rows that occur.  Atomics would make the sums' order, and their last bits, a
 // matter of chance, and in 16 bits round at every addition.  So the tokens are sorted by id (a stable radix sort of (id, position)
 // pairs, 9 bits a pass at most): the rows of one id are neighbours in the order of their positions, one wave adds them up in
-// registers and writes the table's row once.  1000 tokens into a table of 50257 x 1150 in fp16 30 us, 32768 into one of 151936 x 4096 in bf16 316 (209 of
-// them the table's zeros, at 5.9 TB/s); added, 8192 into one of 256000 x 2048 40.
+// registers and writes the table's row once.  1000 tokens into a table of 50257 x 1150 in fp16 28 us, 32768 into one of 151936 x 4096 in bf16 301 (192 of
+// them the table's zeros, at 6.5 TB/s); added, 8192 into one of 256000 x 2048 38.
 #include <algorithm>
 #include <atomic>
 
@@ -348,7 +348,9 @@ __global__ __launch_bounds__(kRankThreads) void rank_kernel(RankArgs a) {
 }
 
 // ---- the table's zeros --------------------------------------------------------------------------------------------------
-// 1.24 GB 214 us (5.8 TB/s); in workgroups of 1024, beside the sort, 250.
+// 4 KiB a workgroup, past the caches: 1.24 GB 187 us (6.7 TB/s), 0.54 GB 82.  Plain stores 183 and 78, but then what is left in the caches is written back
+// under the rows' sums (2000 tokens into 0.54 GB 99 us in all, with plain stores 114; 32768 into 1.24 GB, lookup and all, 374 and 389); four vectors a lane 211
+// and 91, workgroups of 1024 196 and 88.
 struct ZeroArgs {
     u32x4* p;
     int64_t vecs;
@@ -357,11 +359,7 @@ struct ZeroArgs {
 };
 __global__ __launch_bounds__(kThreads) void zero_kernel(ZeroArgs z) {
     const u32x4 zero = {0, 0, 0, 0};
-    for (int64_t at = int64_t(blockIdx.x) * kItems + threadIdx.x; at < z.vecs; at += int64_t(gridDim.x) * kItems) {
-#pragma unroll
-        for (int j = 0; j < kUnroll; ++j)
-            if (at + j * kThreads < z.vecs) __builtin_nontemporal_store(zero, z.p + at + j * kThreads);
-    }
+    for (int64_t at = int64_t(blockIdx.x) * kThreads + threadIdx.x; at < z.vecs; at += int64_t(gridDim.x) * kThreads) __builtin_nontemporal_store(zero, z.p + at);
     if (blockIdx.x == 0) {
         if (int(threadIdx.x) < z.head_bytes) z.head[threadIdx.x] = 0;
         if (int(threadIdx.x) < z.tail_bytes) z.tail[threadIdx.x] = 0;
@@ -784,7 +782,7 @@ extern "C" int trlk_embedding_bwd(const void* d_grad, int dtype, int64_t n, int6
     GradArgs a{};
     if (!accumulate) {
         const ZeroArgs z = zero_args(d_dweight, vocab * cols * int64_t(elem_size(out_dtype)));
-        const int64_t need = std::max<int64_t>(1, ceil_div(z.vecs, kItems));
+        const int64_t need = std::max<int64_t>(1, ceil_div(z.vecs, kThreads));
         zero_kernel<<<unsigned(std::min(need, kMaxGroups)), kThreads, 0, stream>>>(z);
     }
     if (n == 0) return launch_status("embedding_bwd");
