@@ -533,8 +533,8 @@ __device__ __forceinline__ int acc_turned_col(int wn, int j, int lane) { return 
 // Fewer a tiles (token counts below 8192) are put into even bands of at most 8; inside a band b is walked with the band's a
 // tiles innermost, and each XCD takes one eighth of that sequence: 4 to 8 a tiles beside 4 to 8 b tiles at a time.  Under
 // the rule for many a tiles an XCD has ONE a tile beside 32 b tiles when there are 8 to 15, and fetches 33 slabs where
-// 12 would do: 2300 tokens, H = 2048, V = 128256 forward 1140 -> 1107 us, with backward 3720 -> 3690 us; 3000 tokens, H =
-// 3072, V = 50257 866 -> 834 and 2713 -> 2664 us; 1000 tokens, H = 2048, V = 128256 (there the slices of dHidden) 1948 -> 1918 us.
+// 12 would do: 2300 tokens, H = 2048, V = 128256 forward 1140 -> 1107 us, with backward 3720 -> 3690 us; 1000 tokens,
+// H = 2048, V = 128256 (there the slices of dHidden) 1948 -> 1918 us.
 // The same for the last few of many a tiles loses (79 a tiles: forward 3653 -> 3735 us).
 // The caller skips ta >= n_a or tb >= n_b.
 __device__ __forceinline__ void xcd_patch(int w, int n_a, int n_b, int& ta, int& tb) {
