@@ -79,3 +79,46 @@ def test_shapes_for_tracers():
         rows = trl_amd.embedding(ids, weight)
         assert rows.shape == (2, 3, 8) and rows.dtype == torch.bfloat16
         assert trl_amd.ops.embedding_bwd(rows, ids, 50, 1.0, -1).shape == (50, 8)
+
+
+def scaled(name, **members):
+    """A class whose name ends as those of transformers' scaled embeddings do, with their forward unless `members` has another."""
+    def init(self, vocab, width, scale=3.0):
+        torch.nn.Embedding.__init__(self, vocab, width)
+        self.embed_scale = scale
+
+    def forward(self, input_ids):
+        return torch.nn.Embedding.forward(self, input_ids) * self.embed_scale
+
+    return type(name + "ScaledWordEmbedding", (torch.nn.Embedding,), dict(dict(__init__=init, forward=forward), **members))
+
+
+def test_patch_embedding_refuses_scaled_embeddings_that_do_more():
+    import trl_amd
+    from transformers.models.t5gemma2.modeling_t5gemma2 import T5Gemma2TextScaledWordEmbedding
+
+    def one_token_more(self, input_ids):
+        return torch.where(input_ids[..., None] == 7, 1.0, torch.nn.Embedding.forward(self, input_ids) * self.embed_scale)
+
+    def shifted(self, input_ids):
+        return torch.nn.Embedding.forward(self, input_ids) * self.embed_scale + 1.0
+
+    def rooted(self, input_ids):
+        return torch.nn.Embedding.forward(self, input_ids) * self.embed_scale**0.5
+
+    for module in (T5Gemma2TextScaledWordEmbedding(11, 6, 0, embed_scale=2.0, eoi_token_index=5), scaled("OneMore", forward=one_token_more)(11, 6),
+                   scaled("Shifted", forward=shifted)(11, 6), scaled("Rooted", forward=rooted)(11, 6)):
+        with pytest.raises(ValueError, match="ScaledWordEmbedding"):
+            trl_amd.patch_embedding(Model(module))
+        assert "forward" not in vars(module)
+    trl_amd.patch_embedding(Model(scaled("Plain")(11, 6)))
+
+
+def test_scaled_embeddings_of_the_installed_models_are_known():
+    import trl_amd
+    from transformers.models.bart.modeling_bart import BartScaledWordEmbedding
+    from transformers.models.gemma3.modeling_gemma3 import Gemma3TextScaledWordEmbedding
+
+    for kind in (BartScaledWordEmbedding, Gemma3TextScaledWordEmbedding):
+        for dtype in (torch.float32, torch.bfloat16):
+            trl_amd.patch_embedding(Model(kind(11, 6, 3, embed_scale=33.941).to(dtype)))

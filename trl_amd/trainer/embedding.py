@@ -1,6 +1,7 @@
 """The other end of the table that the fused head reads: the embedding of the tokens, times a scale, and its gradient from sorted tokens."""
 from __future__ import annotations
 
+import copy
 import types
 
 import torch
@@ -39,11 +40,30 @@ def embedding_grad_(grad_weight: Tensor, grad_output: Tensor, input_ids: Tensor,
     return grad_weight
 
 
+def _is_lookup_times_scale(module: torch.nn.Embedding) -> bool:
+    """Whether the module's forward is its table's rows times `embed_scale` and nothing else: it has no other parameter, and makes just that of every
+    token of a narrow table."""
+    scale = getattr(module, "embed_scale", None)
+    if scale is None or [name for name, _ in module.named_parameters()] != ["weight"]:
+        return False
+    device = "cpu" if module.weight.is_meta else module.weight.device
+    table = (torch.arange(module.num_embeddings, dtype=torch.float32, device=device)[:, None] % 1021 + 1.0) / 512
+    probe = copy.copy(module)
+    vars(probe)["_parameters"] = {"weight": torch.nn.Parameter(table, requires_grad=False)}
+    factor = float(scale.to(table.dtype)) if isinstance(scale, Tensor) else scale
+    try:
+        with torch.no_grad():
+            rows = type(module).forward(probe, torch.arange(module.num_embeddings, device=device)[None])
+    except Exception:
+        return False
+    return isinstance(rows, Tensor) and torch.equal(rows, (table * factor)[None])
+
+
 def _scale_of(module: torch.nn.Embedding) -> float:
     """The factor that the module's forward multiplies its rows by."""
     if type(module).forward is torch.nn.Embedding.forward:
         return 1.0
-    if not type(module).__name__.endswith("ScaledWordEmbedding") or not hasattr(module, "embed_scale"):
+    if not type(module).__name__.endswith("ScaledWordEmbedding") or not _is_lookup_times_scale(module):
         raise ValueError(f"{type(module).__name__} is not a lookup, or a scaled one, that patch_embedding knows")
     scale = module.embed_scale
     # (as a tensor it is rounded to the table's type before it is multiplied with, as a number it is not)
@@ -56,8 +76,8 @@ def _embedding_forward(self, input: Tensor) -> Tensor:
 
 def patch_embedding(model: torch.nn.Module) -> None:
     """Replaces the forward of `model.get_input_embeddings()` by `embedding`, with the module's own scale and padding index.  Takes
-    `torch.nn.Embedding` and the scaled embeddings of transformers' models; others, and embeddings with `max_norm`, `sparse` or
-    `scale_grad_by_freq`, raise ValueError."""
+    `torch.nn.Embedding` and the scaled embeddings of transformers' models whose forward is the rows times `embed_scale` and nothing else (it
+    is run once, on a narrow table); others, and embeddings with `max_norm`, `sparse` or `scale_grad_by_freq`, raise ValueError."""
     module = model.get_input_embeddings()
     if not isinstance(module, torch.nn.Embedding):
         raise ValueError(f"the model's input embeddings are a {type(module).__name__}, not a torch.nn.Embedding")
