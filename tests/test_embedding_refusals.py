@@ -122,3 +122,22 @@ def test_scaled_embeddings_of_the_installed_models_are_known():
     for kind in (BartScaledWordEmbedding, Gemma3TextScaledWordEmbedding):
         for dtype in (torch.float32, torch.bfloat16):
             trl_amd.patch_embedding(Model(kind(11, 6, 3, embed_scale=33.941).to(dtype)))
+
+
+def test_patch_embedding_refuses_a_forward_of_the_instance():
+    """A hook of another library around the forward, for instance: it would be lost."""
+    import trl_amd
+
+    module = torch.nn.Embedding(5, 4)
+    kept = module.forward
+
+    def around(input):
+        return kept(input) + 1
+
+    module.forward = around
+    with pytest.raises(ValueError, match="forward"):
+        trl_amd.patch_embedding(Model(module))
+    assert module.forward is around
+    plain = Model(torch.nn.Embedding(5, 4))
+    trl_amd.patch_embedding(plain)
+    trl_amd.patch_embedding(plain)  # its own is not another's

@@ -83,5 +83,8 @@ def patch_embedding(model: torch.nn.Module) -> None:
         raise ValueError(f"the model's input embeddings are a {type(module).__name__}, not a torch.nn.Embedding")
     if module.max_norm is not None or module.sparse or module.scale_grad_by_freq:
         raise ValueError("patch_embedding takes no max_norm, sparse or scale_grad_by_freq")
+    own = vars(module).get("forward")
+    if own is not None and getattr(own, "__func__", None) is not _embedding_forward:
+        raise ValueError("the input embeddings' forward has been replaced already, by a hook for instance: patch_embedding would drop it, call it first")
     module._trl_amd_scale = _scale_of(module)
     module.forward = types.MethodType(_embedding_forward, module)  # (a copy of the model gets one that is bound to its own table)
