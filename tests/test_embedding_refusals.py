@@ -141,3 +141,32 @@ def test_patch_embedding_refuses_a_forward_of_the_instance():
     plain = Model(torch.nn.Embedding(5, 4))
     trl_amd.patch_embedding(plain)
     trl_amd.patch_embedding(plain)  # its own is not another's
+
+
+def plain_embedding(input_ids, weight, *, scale=1.0, padding_idx=None):
+    return (weight.float()[input_ids] * scale).to(weight.dtype)
+
+
+def test_patched_modules_follow_their_scale(monkeypatch):
+    """The model is cast, and its scale is changed, after the patch: the rows stay those of the module's own forward."""
+    import sys
+
+    import trl_amd
+    from transformers.models.bart.modeling_bart import BartScaledWordEmbedding
+    from transformers.models.gemma3.modeling_gemma3 import Gemma3TextScaledWordEmbedding
+
+    monkeypatch.setattr(sys.modules["trl_amd.trainer.embedding"], "embedding", plain_embedding)
+    ids = torch.arange(11).view(1, 11)
+    for kind in (BartScaledWordEmbedding, Gemma3TextScaledWordEmbedding):
+        torch.manual_seed(0)
+        module = kind(11, 6, 0, embed_scale=1152**0.5)
+        trl_amd.patch_embedding(Model(module))
+        for dtype in (torch.float32, torch.bfloat16, torch.float32, torch.float16):
+            module.to(dtype)
+            for _ in range(2):
+                assert torch.equal(module(ids), kind.forward(module, ids)), (kind, dtype)
+        with torch.no_grad():
+            module.embed_scale *= 0.5  # (a tensor in place)
+        assert torch.equal(module(ids), kind.forward(module, ids))
+        with torch.inference_mode():
+            assert torch.equal(module(ids), kind.forward(module, ids))

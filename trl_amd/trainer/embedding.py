@@ -59,25 +59,41 @@ def _is_lookup_times_scale(module: torch.nn.Embedding) -> bool:
     return isinstance(rows, Tensor) and torch.equal(rows, (table * factor)[None])
 
 
-def _scale_of(module: torch.nn.Embedding) -> float:
-    """The factor that the module's forward multiplies its rows by."""
+def _is_scaled(module: torch.nn.Embedding) -> bool:
+    """Whether the module's forward multiplies its rows by `embed_scale`.  ValueError where it is neither that nor a lookup."""
     if type(module).forward is torch.nn.Embedding.forward:
-        return 1.0
+        return False
     if not type(module).__name__.endswith("ScaledWordEmbedding") or not _is_lookup_times_scale(module):
         raise ValueError(f"{type(module).__name__} is not a lookup, or a scaled one, that patch_embedding knows")
+    return True
+
+
+def _scale_of(module: torch.nn.Embedding) -> float:
+    """The factor that the module multiplies its rows by now.  As a tensor it is rounded to the table's type before it is multiplied with, and casts of the
+    model change both; its number is read again, which waits for the GPU, where the tensor is another one or has changed."""
     scale = module.embed_scale
-    # (as a tensor it is rounded to the table's type before it is multiplied with, as a number it is not)
-    return float(scale.to(module.weight.dtype)) if isinstance(scale, Tensor) else float(scale)
+    if not isinstance(scale, Tensor):
+        return float(scale)
+    seen = 0 if scale.is_inference() else scale._version, module.weight.dtype
+    held = vars(module).get("_trl_amd_scale")
+    if held is None or held[0] is not scale or held[1] != seen:
+        held = vars(module)["_trl_amd_scale"] = scale, seen, float(scale.detach().to(module.weight.dtype))
+    return held[2]
 
 
 def _embedding_forward(self, input: Tensor) -> Tensor:
-    return embedding(input, self.weight, scale=self._trl_amd_scale, padding_idx=self.padding_idx)
+    if not self._trl_amd_scaled:
+        return embedding(input, self.weight, padding_idx=self.padding_idx)
+    if torch.compiler.is_compiling() and isinstance(self.embed_scale, Tensor):  # (its number is not to be had while a graph is made)
+        return embedding(input, self.weight, padding_idx=self.padding_idx) * self.embed_scale.to(self.weight.dtype)
+    return embedding(input, self.weight, scale=_scale_of(self), padding_idx=self.padding_idx)
 
 
 def patch_embedding(model: torch.nn.Module) -> None:
-    """Replaces the forward of `model.get_input_embeddings()` by `embedding`, with the module's own scale and padding index.  Takes
+    """Replaces the forward of `model.get_input_embeddings()` by `embedding`, with the module's own scale (as it is at each call) and padding index.  Takes
     `torch.nn.Embedding` and the scaled embeddings of transformers' models whose forward is the rows times `embed_scale` and nothing else (it
-    is run once, on a narrow table); others, and embeddings with `max_norm`, `sparse` or `scale_grad_by_freq`, raise ValueError."""
+    is run once, on a narrow table); others, embeddings with `max_norm`, `sparse` or `scale_grad_by_freq`, and modules whose forward
+    has been replaced already, raise ValueError."""
     module = model.get_input_embeddings()
     if not isinstance(module, torch.nn.Embedding):
         raise ValueError(f"the model's input embeddings are a {type(module).__name__}, not a torch.nn.Embedding")
@@ -86,5 +102,7 @@ def patch_embedding(model: torch.nn.Module) -> None:
     own = vars(module).get("forward")
     if own is not None and getattr(own, "__func__", None) is not _embedding_forward:
         raise ValueError("the input embeddings' forward has been replaced already, by a hook for instance: patch_embedding would drop it, call it first")
-    module._trl_amd_scale = _scale_of(module)
+    module._trl_amd_scaled = _is_scaled(module)
+    if module._trl_amd_scaled:
+        _scale_of(module)  # (read now, not in the first forward)
     module.forward = types.MethodType(_embedding_forward, module)  # (a copy of the model gets one that is bound to its own table)
