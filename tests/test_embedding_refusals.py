@@ -170,3 +170,35 @@ def test_patched_modules_follow_their_scale(monkeypatch):
         assert torch.equal(module(ids), kind.forward(module, ids))
         with torch.inference_mode():
             assert torch.equal(module(ids), kind.forward(module, ids))
+
+
+def test_patched_modules_are_copied_and_pickled(monkeypatch):
+    """Each copy reads its own table and can be patched again."""
+    import copy
+    import io
+    import pickle
+    import sys
+
+    import trl_amd
+    from transformers.models.gemma3.modeling_gemma3 import Gemma3TextScaledWordEmbedding
+
+    monkeypatch.setattr(sys.modules["trl_amd.trainer.embedding"], "embedding", plain_embedding)
+    ids = torch.arange(11).view(1, 11)
+
+    def saved(model):
+        file = io.BytesIO()
+        torch.save(model, file)
+        file.seek(0)
+        return torch.load(file, weights_only=False)
+
+    for module in (torch.nn.Embedding(11, 6), Gemma3TextScaledWordEmbedding(11, 6, 0, embed_scale=1152**0.5)):
+        model = Model(module)
+        trl_amd.patch_embedding(model)
+        want = model.embed(ids)
+        for way in (copy.deepcopy, lambda m: pickle.loads(pickle.dumps(m)), saved, lambda m: saved(copy.deepcopy(m))):
+            other = way(model)
+            with torch.no_grad():
+                other.embed.weight.add_(1.0)
+            assert torch.equal(model.embed(ids), want) and not torch.equal(other.embed(ids), want)
+            assert torch.equal(other.to(torch.bfloat16).embed(ids), type(module).forward(other.embed, ids))
+            trl_amd.patch_embedding(other)

@@ -2,7 +2,7 @@
 from __future__ import annotations
 
 import copy
-import types
+import functools
 
 import torch
 from torch import Tensor
@@ -81,12 +81,12 @@ def _scale_of(module: torch.nn.Embedding) -> float:
     return held[2]
 
 
-def _embedding_forward(self, input: Tensor) -> Tensor:
-    if not self._trl_amd_scaled:
-        return embedding(input, self.weight, padding_idx=self.padding_idx)
-    if torch.compiler.is_compiling() and isinstance(self.embed_scale, Tensor):  # (its number is not to be had while a graph is made)
-        return embedding(input, self.weight, padding_idx=self.padding_idx) * self.embed_scale.to(self.weight.dtype)
-    return embedding(input, self.weight, scale=_scale_of(self), padding_idx=self.padding_idx)
+def _embedding_forward(module: torch.nn.Embedding, input: Tensor) -> Tensor:
+    if not module._trl_amd_scaled:
+        return embedding(input, module.weight, padding_idx=module.padding_idx)
+    if torch.compiler.is_compiling() and isinstance(module.embed_scale, Tensor):  # (its number is not to be had while a graph is made)
+        return embedding(input, module.weight, padding_idx=module.padding_idx) * module.embed_scale.to(module.weight.dtype)
+    return embedding(input, module.weight, scale=_scale_of(module), padding_idx=module.padding_idx)
 
 
 def patch_embedding(model: torch.nn.Module) -> None:
@@ -100,9 +100,10 @@ def patch_embedding(model: torch.nn.Module) -> None:
     if module.max_norm is not None or module.sparse or module.scale_grad_by_freq:
         raise ValueError("patch_embedding takes no max_norm, sparse or scale_grad_by_freq")
     own = vars(module).get("forward")
-    if own is not None and getattr(own, "__func__", None) is not _embedding_forward:
+    if own is not None and getattr(own, "func", None) is not _embedding_forward:
         raise ValueError("the input embeddings' forward has been replaced already, by a hook for instance: patch_embedding would drop it, call it first")
     module._trl_amd_scaled = _is_scaled(module)
     if module._trl_amd_scaled:
         _scale_of(module)  # (read now, not in the first forward)
-    module.forward = types.MethodType(_embedding_forward, module)  # (a copy of the model gets one that is bound to its own table)
+    # (a copy of the model gets one of its own table, and one that has been pickled, too, which a bound method does not survive)
+    module.forward = functools.partial(_embedding_forward, module)
