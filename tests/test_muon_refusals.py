@@ -172,3 +172,32 @@ def test_shapes_for_tracers():
     with FakeTensorMode():
         x = torch.empty((3, 50, 8), dtype=torch.bfloat16, device="cuda")
         assert trl_amd.orthogonalize(x).shape == x.shape and trl_amd.orthogonalize([x, x[0]])[1].shape == (50, 8)
+
+
+@pytest.mark.parametrize("way", ["mine", "theirs"])
+def test_loaded_moments_lie_as_their_parameters_do(way):
+    """A convolution's weight with its channels last, a transposed matrix: AdamW's step asks for moments in the parameter's order."""
+    import trl_amd
+
+    conv = torch.nn.Conv2d(3, 8, 4).to(memory_format=torch.channels_last)
+    turned = torch.nn.Parameter(torch.randn(6, 4).t())
+    matrix = torch.nn.Parameter(torch.randn(5, 4))
+    groups = [dict(params=[matrix]), dict(params=[conv.weight, turned], adamw=True)]
+    opt = trl_amd.Muon(copy.deepcopy(groups))
+    params = [p for g in opt.param_groups for p in g["params"]]
+    fresh = [opt._state_of(p, i > 0) for i, p in enumerate(params)]
+    gen = torch.Generator().manual_seed(0)
+    for s in fresh:
+        for t in s.values():
+            t.copy_(torch.randn(t.shape, generator=gen))
+    state = copy.deepcopy(opt.state_dict())
+    if way == "theirs":  # (saved without their layout)
+        state["state"] = {i: {k: t.contiguous() for k, t in s.items()} for i, s in state["state"].items()}
+    again = trl_amd.Muon(copy.deepcopy(groups))
+    again.load_state_dict(state)
+    for p, s in zip((p for g in again.param_groups for p in g["params"]), fresh):
+        assert set(again.state[p]) == set(s)
+        for k, t in s.items():
+            got = again.state[p][k]
+            assert torch.equal(got, t) and got.dtype == torch.float32 and got.device == p.device
+            assert k == "step" or got.stride() == p.stride() == t.stride(), k

@@ -202,7 +202,8 @@ class Muon(torch.optim.Optimizer):
             for k in ("step", "exp_avg", "exp_avg_sq") if group["adamw"] else ("momentum_buffer",):
                 if saved and k in saved:
                     t = torch.as_tensor(saved[k]).to(device=p.device, dtype=torch.float32, copy=True)
-                    self.state[p][k] = t if k == "step" else t.contiguous()
+                    # (in the parameter's order of entries, as the step asks for it, whatever it was saved in)
+                    self.state[p][k] = t if k == "step" else torch.empty_like(p, dtype=torch.float32, memory_format=torch.preserve_format).copy_(t)
 
 
 def muon_param_groups(model: torch.nn.Module) -> list[dict]:
