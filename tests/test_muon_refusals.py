@@ -201,3 +201,32 @@ def test_loaded_moments_lie_as_their_parameters_do(way):
             got = again.state[p][k]
             assert torch.equal(got, t) and got.dtype == torch.float32 and got.device == p.device
             assert k == "step" or got.stride() == p.stride() == t.stride(), k
+
+
+class Wrapper(torch.nn.Module):
+    """As a data-parallel wrapper has its model."""
+
+    def __init__(self, module):
+        super().__init__()
+        self.module = module
+
+
+def test_param_groups_of_wrapped_models_and_other_heads():
+    import transformers
+
+    import trl_amd
+
+    for tied in (False, True):
+        model = Small(tied)
+        matrices, rest = trl_amd.muon_param_groups(Wrapper(Wrapper(model)))
+        assert [id(p) for p in matrices["params"]] == [id(model.a.weight)]
+        assert id(model.lm_head.weight) in {id(p) for p in rest["params"]}
+    config = transformers.LlamaConfig(hidden_size=16, intermediate_size=32, num_hidden_layers=1, num_attention_heads=2, num_key_value_heads=2,
+                                      vocab_size=50, num_labels=2, pad_token_id=0)
+    for kind in (transformers.LlamaForCausalLM, transformers.LlamaForSequenceClassification, transformers.LlamaForTokenClassification,
+                 transformers.LlamaForQuestionAnswering):
+        for model in (kind(config), Wrapper(kind(config))):
+            matrices, rest = trl_amd.muon_param_groups(model)
+            names = {id(p): name for name, p in model.named_parameters()}
+            assert len(matrices["params"]) == 7 and all(".layers." in names[id(p)] for p in matrices["params"])
+            assert len(matrices["params"]) + len(rest["params"]) == len(names)

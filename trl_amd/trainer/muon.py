@@ -206,14 +206,27 @@ class Muon(torch.optim.Optimizer):
                     self.state[p][k] = t if k == "step" else torch.empty_like(p, dtype=torch.float32, memory_format=torch.preserve_format).copy_(t)
 
 
+_HEADS = ("lm_head", "score", "classifier", "qa_outputs")  # as transformers' models call what stands behind their last layer
+
+
+def _heads(model: torch.nn.Module):
+    """The output heads of the model, which may be wrapped (for data-parallel training, or by adapters)."""
+    for m in model.modules():
+        if m is not model and not hasattr(m, "get_output_embeddings") and not hasattr(m, "get_input_embeddings"):
+            continue
+        try:
+            yield m.get_output_embeddings() if hasattr(m, "get_output_embeddings") else None
+        except NotImplementedError:  # (of encoders without one)
+            pass
+        yield from (getattr(m, name, None) for name in _HEADS)
+
+
 def muon_param_groups(model: torch.nn.Module) -> list[dict]:
-    """Two groups for `Muon`: the model's trainable matrices, and with `adamw=True` its embeddings, its output head and whatever is no
-    matrix (convolutions' weights neither)."""
+    """Two groups for `Muon`: the model's trainable matrices, and with `adamw=True` its embeddings, its output head (of a language model, or a classifier's)
+    and whatever is no matrix (convolutions' weights neither)."""
     kinds = (torch.nn.Embedding, torch.nn.modules.conv._ConvNd)
     apart = {id(p) for m in model.modules() if isinstance(m, kinds) for p in m.parameters(recurse=False)}
-    head = model.get_output_embeddings() if hasattr(model, "get_output_embeddings") else getattr(model, "lm_head", None)
-    if isinstance(head, torch.nn.Module):
-        apart |= {id(p) for p in head.parameters()}
+    apart |= {id(p) for head in _heads(model) if isinstance(head, torch.nn.Module) for p in head.parameters()}
     params = [p for p in model.parameters() if p.requires_grad]
     matrices = [p for p in params if p.dim() >= 2 and id(p) not in apart]
     chosen = {id(p) for p in matrices}
