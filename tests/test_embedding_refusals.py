@@ -202,3 +202,17 @@ def test_patched_modules_are_copied_and_pickled(monkeypatch):
             assert torch.equal(model.embed(ids), want) and not torch.equal(other.embed(ids), want)
             assert torch.equal(other.to(torch.bfloat16).embed(ids), type(module).forward(other.embed, ids))
             trl_amd.patch_embedding(other)
+
+
+def test_a_scale_that_requires_a_gradient_is_refused():
+    import trl_amd
+
+    ids, weight = torch.zeros((2, 3), dtype=torch.int64), torch.zeros((5, 4))
+    scale = torch.tensor(2.0, requires_grad=True)
+    with pytest.raises(ValueError, match="scale"):
+        trl_amd.embedding(ids, weight, scale=scale)
+    for taken in (scale.detach(), 2.0):  # (as far as the tensors, which are on the CPU)
+        with pytest.raises(NotImplementedError):
+            trl_amd.embedding(ids, weight, scale=taken)
+    with torch.no_grad(), pytest.raises(NotImplementedError):
+        trl_amd.embedding(ids, weight, scale=scale)

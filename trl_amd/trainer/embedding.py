@@ -24,9 +24,12 @@ def _padding(padding_idx: int | None, vocab: int) -> int:
 def embedding(input_ids: Tensor, weight: Tensor, *, scale: float = 1.0, padding_idx: int | None = None) -> Tensor:
     """`scale * weight[input_ids]`, rounded once: `[..., H]` in the type of `weight` (`[V, H]`, fp32, bf16 or fp16, rows at any
     stride) for int64 or int32 ids `[...]`.  Differentiable w.r.t. `weight`: the gradient, dense, sums a token's rows in fp32 in
-    an order that depends on the ids alone (the same call gives the same bits) and is rounded once; tokens `padding_idx` have none.
+    an order that depends on the ids alone (the same call gives the same bits) and is rounded once; tokens `padding_idx` have none.  A scale that requires
+    a gradient raises.
 
     Ids outside [0, V) give NaN, have no gradient and are reported by `check_device_errors()`."""
+    if isinstance(scale, Tensor) and scale.requires_grad and torch.is_grad_enabled():
+        raise ValueError("embedding has no gradient for its scale")
     return ops.embedding(input_ids, weight, float(scale), _padding(padding_idx, weight.shape[0]))
 
 
