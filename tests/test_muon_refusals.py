@@ -230,3 +230,25 @@ def test_param_groups_of_wrapped_models_and_other_heads():
             names = {id(p): name for name, p in model.named_parameters()}
             assert len(matrices["params"]) == 7 and all(".layers." in names[id(p)] for p in matrices["params"])
             assert len(matrices["params"]) + len(rest["params"]) == len(names)
+
+
+def test_numbers_of_steps_are_whole_and_small(monkeypatch):
+    """2^32 + 5 is not 5, and neither is 5.9."""
+    import trl_amd
+
+    seen = []
+    monkeypatch.setattr(trl_amd.ops, "orthogonalize", lambda *args: seen.append(args) or list(args[0]))
+    monkeypatch.setattr(trl_amd.ops, "muon_step_", lambda *args: seen.append(args))
+    x = [torch.zeros((4, 5))]
+    for bad in (2**32 + 5, -(2**32) + 5, 0, 101):
+        for call in (lambda: trl_amd.orthogonalize(x[0], ns_steps=bad), lambda: trl_amd.muon_step_(x, x, x, ns_steps=bad),
+                     lambda: trl_amd.Muon([torch.nn.Parameter(x[0])], ns_steps=bad)):
+            with pytest.raises(ValueError, match="ns_steps"):
+                call()
+    for call in (lambda: trl_amd.orthogonalize(x[0], ns_steps=5.9), lambda: trl_amd.muon_step_(x, x, x, ns_steps=5.9),
+                 lambda: trl_amd.Muon([torch.nn.Parameter(x[0])], ns_steps=5.9)):
+        with pytest.raises(TypeError):
+            call()
+    assert not seen
+    trl_amd.orthogonalize(x[0], ns_steps=torch.tensor(100))
+    assert seen[0][2] == 100

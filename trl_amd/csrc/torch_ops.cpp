@@ -1035,7 +1035,10 @@ class MatrixTable {
     const char* op_;
     at::Device device_;
 };
-void check_coefficients(const char* op, at::ArrayRef<double> c) { TORCH_CHECK_VALUE(c.size() == 3, op, ": three coefficients are expected, got ", c.size()); }
+void check_iteration(const char* op, at::ArrayRef<double> c, int64_t steps) {
+    TORCH_CHECK_VALUE(c.size() == 3, op, ": three coefficients are expected, got ", c.size());
+    TORCH_CHECK_VALUE(steps >= 1 && steps <= 100, op, ": 1 to 100 steps, not ", steps);
+}
 
 template <typename List>
 void muon_step(const List& params, const List& grads_, const List& momenta, at::IntArrayRef group_of, at::ArrayRef<double> hyper, const List& lrs,
@@ -1045,7 +1048,7 @@ void muon_step(const List& params, const List& grads_, const List& momenta, at::
     TORCH_CHECK_VALUE(hyper.size() == 5 * n_groups && n_groups > 0 && (lrs.empty() || lrs.size() == n_groups),
                       "muon_step_: five numbers and one learning rate for each group are expected");
     TORCH_CHECK_VALUE(n > 0, "muon_step_: no parameters");
-    check_coefficients("muon_step_", coefficients);
+    check_iteration("muon_step_", coefficients, steps);
     const at::Device device = params[0].device();
     const at::NoGradGuard no_grad;
     const c10::DeviceGuard guard(device);
@@ -1071,7 +1074,9 @@ void muon_step(const List& params, const List& grads_, const List& momenta, at::
         TORCH_CHECK_VALUE(p.is_contiguous() && m.is_contiguous(), "muon_step_: parameter ", i, " or its momentum is not contiguous");
         Tensor g = grads_[i];
         if (!g.is_contiguous()) copies.push_back(g = g.contiguous());
-        matrices.add(i, p, g, &m, group_of.empty() ? 0 : int32_t(group_of[i]));
+        const int64_t group = group_of.empty() ? 0 : group_of[i];
+        TORCH_CHECK_VALUE(group >= 0 && size_t(group) < n_groups, "muon_step_: parameter ", i, " is in no group");
+        matrices.add(i, p, g, &m, int32_t(group));
         if (p.numel() == 0) continue;
         const size_t numel = size_t(p.numel());
         ranges.add(0, true, p, p.const_data_ptr(), numel * p.element_size());
@@ -1099,7 +1104,7 @@ void muon_step_(at::TensorList params, at::TensorList grads, at::TensorList mome
 
 std::vector<Tensor> orthogonalize(at::TensorList matrices, at::ArrayRef<double> coefficients, int64_t steps, double eps) {
     TORCH_CHECK_VALUE(!matrices.empty(), "orthogonalize: no matrices");
-    check_coefficients("orthogonalize", coefficients);
+    check_iteration("orthogonalize", coefficients, steps);
     const at::Device device = matrices[0].device();
     const c10::DeviceGuard guard(device);
     MatrixTable<at::TensorList> list("orthogonalize", device);

@@ -2,6 +2,7 @@
 takes the rest.  One call for all of them."""
 from __future__ import annotations
 
+import operator
 from collections.abc import Sequence
 
 import torch
@@ -18,7 +19,10 @@ _ADJUST = {None: 0, "original": 0, "match_rms_adamw": 1}
 def _numbers(ns_coefficients, ns_steps, eps) -> tuple[list[float], int, float]:
     if len(ns_coefficients) != 3:
         raise ValueError(f"ns_coefficients are three numbers, got {ns_coefficients}")
-    return [float(x) for x in ns_coefficients], int(ns_steps), float(eps)
+    steps = operator.index(ns_steps)
+    if not 1 <= steps <= 100:
+        raise ValueError(f"ns_steps must be 1 to 100, got {ns_steps}")
+    return [float(x) for x in ns_coefficients], steps, float(eps)
 
 
 def orthogonalize(matrices: Tensor | Sequence[Tensor], *, ns_coefficients: tuple[float, float, float] = NS_COEFFICIENTS, ns_steps: int = 5,
@@ -72,8 +76,8 @@ def _check_settings(group: dict) -> None:
         return
     if not 0.0 <= group["momentum"] < 1.0:
         raise ValueError(f"momentum must be in [0, 1), got {group['momentum']}")
-    if not 1e-30 <= group["eps"] <= 1.0 or not 1 <= group["ns_steps"] <= 100:
-        raise ValueError(f"eps must be in [1e-30, 1] and ns_steps 1 to 100, got {group['eps']}, {group['ns_steps']}")
+    if not 1e-30 <= group["eps"] <= 1.0:
+        raise ValueError(f"eps must be in [1e-30, 1], got {group['eps']}")
     _numbers(group["ns_coefficients"], group["ns_steps"], group["eps"])
     _adjustment(group["adjust_lr_fn"])
     for p in group["params"]:
@@ -127,7 +131,7 @@ class Muon(torch.optim.Optimizer):
             if group["adamw"]:
                 kind, hyper = None, [number, *map(float, group["betas"]), float(group["adamw_eps"]), float(group["weight_decay"])]
             else:
-                kind = (*map(float, group["ns_coefficients"]), int(group["ns_steps"]), float(group["eps"]))
+                kind = (*map(float, group["ns_coefficients"]), operator.index(group["ns_steps"]), float(group["eps"]))
                 hyper = [number, float(group["momentum"]), float(group["weight_decay"]), float(group["nesterov"]), float(_adjustment(group["adjust_lr_fn"]))]
             call = calls.setdefault(kind, dict(params=[], grads=[], states=[], of=[], hyper=[], lrs=[]))
             for p in group["params"]:
