@@ -927,6 +927,11 @@ __global__ __launch_bounds__(kThreads) void narrow_steps_kernel(const Mat* mats,
     __syncthreads();
     for (int k = threadIdx.x; k < MP * LD; k += kThreads) G[k] *= f * f;  // (the last column is nobody's)
     __syncthreads();
+    // The rounding of G's sums, some 2^-50 of its trace, takes eigenvalues of zero either way, and one below zero has no way back: it grows by a^2 a step and from
+    // size one on by its square (a matrix of rank one: 1e8 too large after 18 steps, NaN after 20).  2^-46 of the trace, more where more partial sums are
+    // added up, lifts all of them above zero; an eigenvalue s^2 of the matrix's own moves by less than the rounding of its entries to fp32 moves it.
+    if (threadIdx.x < MP) G[threadIdx.x * (LD + 1)] += trace * f * f * 0x1p-46 * (1.0 + chunks * 0x1p-10);
+    __syncthreads();
     for (int s = 0; s < steps; ++s) {
         square_product<MP>(G, G, P, [&](double x, int i, int j) { return c * x + b * G[i * LD + j] + (i == j ? a : 0.0); });
         if (s == 0) {
