@@ -26,6 +26,13 @@ def test_numbers_that_do_not_fit_are_refused():
     assert bool((x == 1).all()) and not m.any()
 
 
+def largest_value(a=A, b=B, c=C):
+    """Of a s + b s^3 + c s^5 for s up to 1.2: where a + 3 b s^2 + 5 c s^4 is zero for the first time, at s = 0.5545, it is 1.2024; its value there, at 1.2024, is 0.95
+    and at 1 it is 0.70."""
+    t = (-3 * b - math.sqrt(9 * b * b - 20 * a * c)) / (10 * c)
+    return math.sqrt(t) * (a + t * (b + c * t))
+
+
 def low_rank(shape, rank, gen, whole=False):
     draw = (lambda s: torch.randint(-8, 9, s, generator=gen, device=DEV).float()) if whole else (lambda s: torch.randn(s, generator=gen, device=DEV))
     return draw((shape[0], rank)) @ draw((rank, shape[1]))
@@ -47,7 +54,7 @@ def exact_of_rank(u, rank, steps, coefficients=(A, B, C), eps=1e-7):
 def test_narrow_matrices_of_low_rank_and_many_steps(shape, steps):
     """64 rows or fewer go by the Gram matrix, whose rounding moves eigenvalues of zero either way.  Whole numbers of rank one are exactly of that rank in every type:
     the result is u / |u| times one number, which 64 bits hold to 1e-12 after five steps and, the usual polynomial's cycle attracting, to 2e-7 after 100.  A direction
-    that is not the matrix's own is taken for one of size 2^-23, grows to size one and stays there (0.68 to 1.13): 1.7 2^23 in all, times the 64 2^-53 of
+    that is not the matrix's own is taken for one of size 2^-23, grows to size one and stays there (0.68 to 1.21): 1.8 2^23 in all, times the 64 2^-53 of
     the matrix that rounding leaves in it is 1e-7.  So 1e-5 has room for both."""
     import trl_amd
 
@@ -59,7 +66,70 @@ def test_narrow_matrices_of_low_rank_and_many_steps(shape, steps):
     # of rank four, rounded to fp32: what the rounding adds is at 2^-24, and comes up by itself from 12 steps on.  Then only the size is known.
     u = low_rank(shape, 4, gen)
     got = trl_amd.orthogonalize(u, ns_steps=steps)
-    assert float(torch.linalg.matrix_norm(got.double().cpu(), 2)) <= 1.1337 * 1.01  # the polynomial's largest value on its way
+    assert float(torch.linalg.matrix_norm(got.double().cpu(), 2)) <= largest_value() * 1.01
     if steps <= 12:
         want = exact(u, steps=steps)
         assert distance(got, want) <= 4 * distance(plain32(u, steps=steps), want) + 1e-6 * float(want.norm())
+
+
+def alike(kind, gen):
+    """Matrices whose entries or singular values are alike: roundings of their pieces go one way and do not average out."""
+    if kind == "ones":
+        return torch.ones((113, 120), device=DEV)
+    if kind == "signs":
+        return torch.sign(torch.randn((353, 1), generator=gen, device=DEV)) * torch.sign(torch.randn((1, 360), generator=gen, device=DEV))
+    if kind == "identity":
+        return torch.eye(353, device=DEV)
+    if kind == "orthogonal":
+        return torch.linalg.qr(torch.randn((353, 353), generator=gen, device=DEV).cpu())[0].to(DEV)
+    if kind == "hadamard":
+        x = torch.ones((1, 1), device=DEV)
+        for _ in range(9):
+            x = torch.cat([torch.cat([x, x], 1), torch.cat([x, -x], 1)])
+        return x[:, :100].contiguous()
+    return torch.randn((128, 512), generator=gen, device=DEV)
+
+
+KINDS = ["ones", "signs", "identity", "orthogonal", "hadamard", "even"]
+SENSITIVE = [(5, (A, B, C)), (10, (A, B, C)), (20, (A, B, C)), (5, (4.0848, -6.8946, 2.9270)), (7, (4.0848, -6.8946, 2.9270))]
+
+
+@pytest.mark.parametrize("dtype", list(DTYPES))
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("steps,coefficients", SENSITIVE)
+def test_a_result_is_as_near_as_fp32s(dtype, kind, steps, coefficients):
+    """Whatever the type: operands of 22 bits.  The rounding of a product in them, 2^-22 and the same for each piece left out, is made in each step and grows
+    by the slopes behind it; `growth` is the largest such growth of any singular value.  Twice over (X X^T and its square share it), and the result's rounding."""
+    import trl_amd
+
+    gen = torch.Generator(device=DEV).manual_seed(steps)
+    u = alike(kind, gen).to(DTYPES[dtype])
+    got, want = trl_amd.orthogonalize(u, ns_steps=steps, ns_coefficients=coefficients), exact(u, steps=steps, coefficients=coefficients)
+    assert distance(got, want) <= (2 * growth(steps, coefficients) * 2.0**-22 + half_step(got.dtype)) * float(want.norm()), distance(got, want) / float(want.norm())
+
+
+def growth(steps, coefficients):
+    """By how much a relative error of one made in b A + c A A of every step, has grown in the result, for the singular value where that is most."""
+    a, b, c = coefficients
+    s = torch.arange(1, 257, dtype=torch.float64) / 256
+    off = torch.zeros_like(s)
+    for _ in range(steps):
+        t = s * s
+        off = (a + 3 * b * t + 5 * c * t * t).abs() * off + (abs(b) * t + abs(c) * t * t) * s
+        s = s * (a + t * (b + c * t))
+    return float(off.max())
+
+
+@pytest.mark.parametrize("dtype", list(DTYPES))
+@pytest.mark.parametrize("shape", [(70, 70), (100, 260), (300, 129)])
+@pytest.mark.parametrize("steps", [5, 20, 100])
+def test_wide_matrices_of_low_rank_and_many_steps(dtype, shape, steps):
+    """What rounding adds to a matrix of low rank comes up by itself.  Its singular values stay under the polynomial's largest value on its way, but for
+    the rounding of each step and of the result: 2 per cent have room for both."""
+    import trl_amd
+
+    gen = torch.Generator(device=DEV).manual_seed(shape[0] + steps)
+    for rank in (1, 4):
+        u = low_rank(shape, rank, gen).to(DTYPES[dtype])
+        got = trl_amd.orthogonalize(u, ns_steps=steps)
+        assert float(torch.linalg.matrix_norm(got.double().cpu(), 2)) <= largest_value() * 1.02

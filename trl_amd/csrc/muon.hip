@@ -9,12 +9,13 @@
 // Bound by the matrix cores: m^2 n + m^3 + 2 m^2 n operations a step (X X^T and A A are symmetric, half of their tiles are computed and
 // written twice).  The products run on fp16 operands with fp32 sums.  X is held as two fp16 pieces, x = hi + lo, 22 bits, in units of 2^-14 (its
 // singular values stay under 1.3, so do its entries; the units keep what is 2^-28 of the largest out of fp16's subnormals), A and B in
-// units of 2^-13.  Parameters in 16 bits: the products take X's hi piece and A and B of one piece, and the term a X, which carries the small
-// singular values (they grow by a in each step), all 22 bits but for the last step's.  The largest entries of B are its diagonal's: what their rounding
-// leaves is kept in fp32 and multiplied with X's hi piece beside that term (66 rows: 1.96e-3 of the result -> 1.5e-3).  Against the exact
-// iteration that is off by 0.9 to 1.5e-3 of the result for matrices of independent entries and up to 1.8e-3 where few singular values are large; with one piece
-// everywhere those cases lose up to 4e-2, with bf16 operands 3e-1.  Parameters in fp32, and results in fp16, whose own rounding is 2e-4: A and B have two
-// pieces, too, and every product is three, lo hi + hi lo + hi hi, which is fp32's precision at a third of the rate.
+// units of 2^-13.  Results, and steps on parameters in fp32: A and B have two pieces, too, and every product is three, lo hi + hi lo + hi hi, which is fp32's
+// precision at a third of the rate (1e-6 of the result).  Steps on parameters in 16 bits: the products take X's hi piece and A and B of one piece, and the term a X, which
+// carries the small singular values (they grow by a in each step), all 22 bits but for the last step's.  The largest entries of B are its diagonal's: what their
+// rounding leaves is kept in fp32 and multiplied with X's hi piece beside that term (66 rows: 1.96e-3 of the update -> 1.5e-3).  Against the exact
+// iteration the update is then off by 0.9 to 1.5e-3 of its size for matrices of independent entries, up to 1.9e-3 where few singular values are large, and where
+// entries are alike but for their sign, whose roundings go one way, by up to 8e-3 (an identity); a parameter in 16 bits, rounded to 2^-9 of ITS size and moved by a
+// small part of that, does not show it.  With one piece for X as well those losses were up to 4e-2, with bf16 operands 3e-1.
 #include <math.h>
 
 #include <algorithm>
@@ -1009,8 +1010,8 @@ int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 int64_t up_to(int64_t n, int64_t unit) { return ceil_div(n, unit) * unit; }
 size_t up256(size_t n) { return (n + 255) / 256 * 256; }
 
-// (an fp16 result shows what one piece loses, a step's parameter does not)
-int pieces_of(const trlk_muon_matrix& x) { return x.dtype == TRLK_F32 || (x.dtype == TRLK_F16 && !x.d_momentum) ? 2 : 1; }
+// (a result shows what one piece loses, a step's parameter of 16 bits does not)
+int pieces_of(const trlk_muon_matrix& x) { return x.dtype == TRLK_F32 || !x.d_momentum ? 2 : 1; }
 // Rows that a narrow matrix is padded to, 0 for the others.
 int narrow_rows(const trlk_muon_matrix& x) {
     const int64_t m = std::min(x.rows, x.cols);
@@ -1272,9 +1273,8 @@ int run(const trlk_muon_matrix* x, int32_t n, const trlk_muon_group* groups, int
         const int dtype = x[g.each[0]].dtype;
         const trlk_muon_group* hyper = step ? groups : nullptr;
         const int rc = dtype == TRLK_F32    ? run_group<TRLK_F32, true>(g, x, hyper, num, ws, stream, what)
-                       : dtype == TRLK_BF16 ? run_group<TRLK_BF16, false>(g, x, hyper, num, ws, stream, what)
-                       : step               ? run_group<TRLK_F16, false>(g, x, hyper, num, ws, stream, what)
-                                            : run_group<TRLK_F16, true>(g, x, hyper, num, ws, stream, what);
+                       : dtype == TRLK_BF16 ? (step ? run_group<TRLK_BF16, false> : run_group<TRLK_BF16, true>)(g, x, hyper, num, ws, stream, what)
+                                            : (step ? run_group<TRLK_F16, false> : run_group<TRLK_F16, true>)(g, x, hyper, num, ws, stream, what);
         if (rc) return rc;
     }
     return launch_status(what);

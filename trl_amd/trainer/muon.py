@@ -31,9 +31,9 @@ def orthogonalize(matrices: Tensor | Sequence[Tensor], *, ns_coefficients: tuple
     `X = U / max(|U|, eps)` (Frobenius norm), `ns_steps` times `A = X X^T; X = a X + (b A + c A A) X`.  The singular vectors stay, each singular
     value s moves by `a s + b s^3 + c s^5`; the usual coefficients bring all but the smallest to between 0.7 and 1.2 in five steps.
 
-    `matrices` is one tensor `[..., m, n]` or a list of them (then a list is returned), in fp32, bf16 or fp16, all on one GPU: all in one call.  In bf16
-    the products round their operands to 11 bits and the result is within 2e-3 of the exact iteration's (2-norm) before it is rounded; in fp32 and fp16
-    they hold 22 bits.  A matrix of zeros gives zeros, one with a NaN or an infinity NaN.  Coefficients with which values of at most 1 would grow
+    `matrices` is one tensor `[..., m, n]` or a list of them (then a list is returned), in fp32, bf16 or fp16, all on one GPU: all in one call.  The
+    products hold 22 bits, whatever the type, and sum in fp32: the result is about as near to the exact iteration's as one in plain fp32, before it is rounded
+    to its type.  A matrix of zeros gives zeros, one with a NaN or an infinity NaN.  Coefficients with which values of at most 1 would grow
     past 2.5 raise.  Not differentiable."""
     numbers = _numbers(ns_coefficients, ns_steps, eps)
     if isinstance(matrices, Tensor):
