@@ -1010,8 +1010,6 @@ int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 int64_t up_to(int64_t n, int64_t unit) { return ceil_div(n, unit) * unit; }
 size_t up256(size_t n) { return (n + 255) / 256 * 256; }
 
-// (a result shows what one piece loses, a step's parameter of 16 bits does not)
-int pieces_of(const trlk_muon_matrix& x) { return x.dtype == TRLK_F32 || !x.d_momentum ? 2 : 1; }
 // Rows that a narrow matrix is padded to, 0 for the others.
 int narrow_rows(const trlk_muon_matrix& x) {
     const int64_t m = std::min(x.rows, x.cols);
@@ -1020,7 +1018,7 @@ int narrow_rows(const trlk_muon_matrix& x) {
 size_t matrix_bytes(const trlk_muon_matrix& x) {
     if (const int mp = narrow_rows(x)) return up256(size_t(ceil_div(std::max(x.rows, x.cols), kSpan) + 1) * mp * mp * sizeof(double));
     const int64_t m = up_to(std::min(x.rows, x.cols), BK), n = up_to(std::max(x.rows, x.cols), BK);
-    return up256(size_t(4 * m * n + 2 * pieces_of(x) * m * m) * 2 + size_t(m) * sizeof(float));
+    return up256(size_t(4 * m * n + 4 * m * m) * 2);  // (A and B in two pieces; of one, the rest of B's diagonal, too, lies in the other's place)
 }
 
 // Matrices that go through the launches together: of one type, narrow ones of one kind, as many as the workspace's share holds.
@@ -1216,6 +1214,24 @@ double largest_image(double top, double a, double b, double c) {
     return most;
 }
 
+// How far a relative error of one, made in b A + c A A of every step, has grown by the end (or before), for the singular value where that is most: each step
+// multiplies what is there by its polynomial's slope.  88 for five steps with the usual coefficients, 930 for ten of them, 870 for five with (4.0848, -6.8946, 2.9270),
+// under 2 for coefficients that converge.
+constexpr double kMostGrowth = 90.0;  // that one piece may have
+double error_growth(const Numbers& num) {
+    double most = 0.0;
+    for (int i = 1; i <= 64; ++i) {
+        double s = i / 64.0, off = 0.0;
+        for (int k = 0; k < num.steps && off <= kMostGrowth; ++k) {
+            const double t = s * s;
+            off = fabs(num.a + t * (3.0 * num.b + t * 5.0 * num.c)) * off + fabs(s * t) * (fabs(num.b) + fabs(num.c) * t);
+            s *= num.a + t * (num.b + t * num.c);
+        }
+        most = std::max(most, off);
+    }
+    return most;
+}
+
 int check_numbers(const Numbers& num, const char* what) {
     TRLK_REQUIRE(num.steps >= 1 && num.steps <= 100, TRLK_ERR_BAD_VALUE, "%s: 1 to 100 steps, not %d", what, num.steps);
     TRLK_REQUIRE(num.eps >= 1e-30 && num.eps <= 1.0, TRLK_ERR_BAD_VALUE, "%s: eps must be in [1e-30, 1]", what);
@@ -1269,12 +1285,14 @@ int run(const trlk_muon_matrix* x, int32_t n, const trlk_muon_group* groups, int
     TRLK_REQUIRE(aligned_to(d_workspace, 256), TRLK_ERR_WORKSPACE, "%s: misaligned workspace", what);
     const hipStream_t stream = static_cast<hipStream_t>(stream_);
     char* ws = static_cast<char*>(d_workspace);
+    // (a result shows what one piece loses, a step's parameter of 16 bits does not, unless the loss grows)
+    const bool one_piece = step && error_growth(num) <= kMostGrowth;
     for (const Group& g : all) {
         const int dtype = x[g.each[0]].dtype;
         const trlk_muon_group* hyper = step ? groups : nullptr;
         const int rc = dtype == TRLK_F32    ? run_group<TRLK_F32, true>(g, x, hyper, num, ws, stream, what)
-                       : dtype == TRLK_BF16 ? (step ? run_group<TRLK_BF16, false> : run_group<TRLK_BF16, true>)(g, x, hyper, num, ws, stream, what)
-                                            : (step ? run_group<TRLK_F16, false> : run_group<TRLK_F16, true>)(g, x, hyper, num, ws, stream, what);
+                       : dtype == TRLK_BF16 ? (one_piece ? run_group<TRLK_BF16, false> : run_group<TRLK_BF16, true>)(g, x, hyper, num, ws, stream, what)
+                                            : (one_piece ? run_group<TRLK_F16, false> : run_group<TRLK_F16, true>)(g, x, hyper, num, ws, stream, what);
         if (rc) return rc;
     }
     return launch_status(what);
