@@ -389,3 +389,30 @@ def test_patched_modules():
             torch.testing.assert_close(mine, grad, rtol=2e-2 if dtype == torch.bfloat16 else 1e-5, atol=0.25 if dtype == torch.bfloat16 else 1e-3)
             if type(model.embed) is torch.nn.Embedding and dtype == torch.float32:
                 assert torch.equal(mine, grad)  # whole numbers: exact
+
+
+def test_patched_modules_after_a_cast_and_compiled():
+    """A model that is cast after the patch, and one that is compiled, have the module's own rows, and gradients."""
+    import trl_amd
+    from transformers.models.bart.modeling_bart import BartScaledWordEmbedding
+    from transformers.models.gemma3.modeling_gemma3 import Gemma3TextScaledWordEmbedding
+
+    torch.manual_seed(0)
+    ids = torch.randint(0, 97, (3, 50), device=DEV)
+    for make in (lambda: torch.nn.Embedding(97, 72, padding_idx=4), lambda: Gemma3TextScaledWordEmbedding(97, 72, 4, embed_scale=1152**0.5),
+                 lambda: BartScaledWordEmbedding(97, 72, 4, embed_scale=1152**0.5)):
+        model = Tied(make())
+        trl_amd.patch_embedding(model)
+        for dtype in (torch.float32, torch.bfloat16):
+            model.to(DEV, dtype)
+            own = type(model.embed).forward
+            torch._dynamo.reset()
+            for call in (model, torch.compile(model, backend="aot_eager", fullgraph=True)):
+                want, got = own(model.embed, ids), call(ids)
+                assert torch.equal(got, want)
+                g = torch.randint(-8, 9, want.shape, device=DEV).to(dtype)
+                grads = [torch.autograd.grad(x, model.embed.weight, g)[0] for x in (want, got)]
+                # whole numbers times one factor: exact sums, but for the rounding of each product (half a step each, of 3 and more of one token)
+                step = 0.0 if type(model.embed) is torch.nn.Embedding else torch.finfo(dtype).eps
+                size = torch.autograd.grad(own(model.embed, ids), model.embed.weight, g.abs())[0].double()
+                assert bool(((grads[1].double() - grads[0].double()).abs() <= 2 * step * size).all())

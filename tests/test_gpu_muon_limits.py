@@ -153,3 +153,38 @@ def test_a_step_is_off_by_what_the_usual_five_are_at_most(dtype, kind, steps, co
     off = 12 * here * (2.0**-12 if here <= usual else 2.0**-22)
     most = 8e-3 if steps <= 5 and coefficients[0] == A else 1.0
     assert distance(p, want) <= (min(off, most) + half_step(p.dtype)) * float(want.norm()), distance(p, want) / float(want.norm())
+
+
+@pytest.mark.parametrize("size", [1e-30, 1e-18, 1e-11, 1e-9, 1.0, 1e18])
+@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
+def test_narrow_matrices_of_any_size(dtype, size):
+    """64 rows or fewer, in 64 bits, however far the norm is under eps: fp32's rounding of the result, and half a step.  (Zeros are not near.)"""
+    import trl_amd
+
+    gen = torch.Generator(device=DEV).manual_seed(3)
+    for shape in ((50, 60), (700, 13)):
+        u = (torch.randn(shape, generator=gen, device=DEV) * size).to(DTYPES[dtype])
+        got, want = trl_amd.orthogonalize(u), exact(u)
+        assert distance(got, want) <= (2.0**-22 + half_step(got.dtype)) * float(want.norm()), distance(got, want) / float(want.norm())
+
+
+@pytest.mark.parametrize("size", [1e-16, 1e-14, 1e-12, 1e-11, 1e-10, 1.0, 1e18])
+@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
+def test_wide_matrices_of_any_size(dtype, size):
+    """Of more rows X is a multiple of 2^-38 (fp16's least number, in X's units of 2^-14): half of that is lost at the start and in each step but the last, and grows by
+    3.4445 a step, 485 in all: 485 (1 + 1/3.4445 + ...) 2^-39 < 700 2^-39 in each entry.  The largest sizes have 22 bits (11 in a step) as elsewhere."""
+    import trl_amd
+
+    gen = torch.Generator(device=DEV).manual_seed(4)
+    for shape in ((300, 270), (70, 900)):
+        u = (torch.randn(shape, generator=gen, device=DEV) * size).to(DTYPES[dtype])
+        want = exact(u)
+        grain = 700 * 2.0**-39 * math.sqrt(u.numel())
+        got = trl_amd.orthogonalize(u)
+        assert distance(got, want) <= (12 * growth(5, (A, B, C)) * 2.0**-22 + half_step(got.dtype)) * float(want.norm()) + grain
+        p, m = torch.zeros_like(u), torch.zeros(shape, device=DEV)
+        trl_amd.muon_step_([p], [u], [m], lr=1.0, weight_decay=0.0, momentum=0.0, nesterov=False)
+        stretch = math.sqrt(max(1.0, shape[0] / shape[1]))
+        # (a norm under eps shows the small singular values: those are the term a X, of 22 bits but for the last step's 11)
+        bits = 12 * growth(5, (A, B, C)) * 2.0**-22 if got.dtype == torch.float32 else 8e-3
+        assert distance(p, -stretch * want) <= stretch * ((bits + half_step(p.dtype)) * float(want.norm()) + grain)
