@@ -188,3 +188,37 @@ def test_wide_matrices_of_any_size(dtype, size):
         # (a norm under eps shows the small singular values: those are the term a X, of 22 bits but for the last step's 11)
         bits = 12 * growth(5, (A, B, C)) * 2.0**-22 if got.dtype == torch.float32 else 8e-3
         assert distance(p, -stretch * want) <= stretch * ((bits + half_step(p.dtype)) * float(want.norm()) + grain)
+
+
+def test_a_resumed_run_steps_weights_in_another_order():
+    """A convolution's weight with its channels last, which AdamW steps: a run that is taken up is the run that was not."""
+    import copy
+
+    import trl_amd
+
+    def made():
+        torch.manual_seed(2)
+        model = torch.nn.Sequential(torch.nn.Conv2d(3, 8, 4), torch.nn.Flatten(), torch.nn.Linear(8, 16)).to(DEV, memory_format=torch.channels_last)
+        assert not model[0].weight.is_contiguous()
+        return model, trl_amd.Muon(trl_amd.muon_param_groups(model), lr=0.01)
+
+    def step(model, opt, seed):
+        gen = torch.Generator(device=DEV).manual_seed(seed)
+        x = torch.randn((6, 3, 4, 4), generator=gen, device=DEV).contiguous(memory_format=torch.channels_last)
+        opt.zero_grad()
+        model(x).square().sum().backward()
+        for p in model.parameters():  # (the library's gradients are no matter here)
+            p.grad = torch.randn(p.shape, generator=gen, device=DEV).contiguous(memory_format=torch.channels_last if p.dim() == 4 else torch.contiguous_format)
+        opt.step()
+
+    whole, opt = made()
+    for seed in range(4):
+        step(whole, opt, seed)
+        if seed == 1:
+            saved = copy.deepcopy((whole.state_dict(), opt.state_dict()))
+    other, again = made()
+    other.load_state_dict(saved[0])
+    again.load_state_dict(saved[1])
+    for seed in range(2, 4):
+        step(other, again, seed)
+    assert all(torch.equal(p, q) for p, q in zip(whole.parameters(), other.parameters()))
