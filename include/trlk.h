@@ -536,7 +536,7 @@ int trlk_adamw_state_values(const uint8_t* d_codes, const float* d_scales, int64
  * in fp32, in an order that depends on nothing but the ids; rounded once.  Tokens padding_idx (-1: none) count for nothing, and ids outside the
  * table neither (they set the flag).  accumulate 0: the whole table is written, dense; else the sums are added to what is there, and
  * rows of ids that do not occur are not touched.  The gradients' type, or fp32, is dweight's.
- * d_workspace: trlk_embedding_bwd_workspace_bytes(n, vocab, cols) bytes, 16-byte aligned.  n < 2^31, vocab < 2^31 - 1, cols <= 2^20. */
+ * d_workspace: trlk_embedding_bwd_workspace_bytes(n, vocab, cols) bytes, 16-byte aligned; over 1024 tokens an fp32 row for every 16 of them and more.  n < 2^31, vocab < 2^31 - 1, cols <= 2^20. */
 int trlk_embedding_fwd(const void* d_weight, int dtype, int64_t vocab, int64_t cols, int64_t row_stride, const void* d_ids,
                        int32_t id_bits, int64_t n, float scale, void* d_out, int32_t* d_error_flag, trlk_stream_t stream);
 size_t trlk_embedding_bwd_workspace_bytes(int64_t n, int64_t vocab, int64_t cols);
@@ -556,6 +556,7 @@ int trlk_embedding_bwd(const void* d_grad, int dtype, int64_t n, int64_t cols, i
  * alike but for their sign).  The tables are HOST memory, read before the call returns.  d_param, d_grad and d_momentum (fp32) are dense [rows, cols];
  * what is written shares no memory with anything else that is listed.  trlk_orthogonalize: d_param takes X, turned back, of d_grad (they may be
  * the same), d_momentum is NULL.  The smaller side is 32768 at most, the larger one 2^22, both 2^34 entries.  A matrix with a NaN or an infinity comes out as NaN.
+ * Of matrices with both sides over 64, what is under 2^-39 of max(|u|, eps) is lost, and the last bits may depend on what else is in the call.
  * Coefficients with which singular values of at most 1 grow past 2.5 on the way are refused.  eps in [1e-30, 1].
  * d_workspace: trlk_muon_workspace_bytes(...) bytes, 256-byte aligned: 8 GiB at most, unless one matrix needs more (several take turns in it). */
 enum trlk_muon_adjust { TRLK_MUON_ORIGINAL = 0, TRLK_MUON_MATCH_ADAMW = 1 };

@@ -15,7 +15,8 @@
 // rounding leaves is kept in fp32 and multiplied with X's hi piece beside that term (66 rows: 1.96e-3 of the update -> 1.5e-3).  Against the exact
 // iteration the update is then off by 0.9 to 1.5e-3 of its size for matrices of independent entries, up to 1.9e-3 where few singular values are large, and where
 // entries are alike but for their sign, whose roundings go one way, by up to 8e-3 (an identity); a parameter in 16 bits, rounded to 2^-9 of ITS size and moved by a
-// small part of that, does not show it.  More steps, or other coefficients, whose slopes would make more of the loss take two pieces, too (error_growth).  With one piece for X as well those losses were up to 4e-2, with bf16 operands 3e-1.
+// small part of that, does not show it.  More steps, or other coefficients, whose slopes would make more of the loss take two pieces, too (error_growth).  With one
+// piece for X as well those losses were up to 4e-2, with bf16 operands 3e-1.
 #include <math.h>
 
 #include <algorithm>
@@ -394,7 +395,7 @@ struct BigTile {
 // much less work, two on a CU.  Of 128 x 128 the bound is the LDS: a step of 64 k moves 96 KB in and out of it for 512 cycles of MFMAs,
 // and takes 0.58 us with one tile on a CU and 0.54 with two (165 and 180 GB/s a CU).  Four stages instead of two, which leave room for one
 // tile only, and tiles that come through registers two steps ahead were no faster (0.61 and 0.66 us).  Of 64 x 64 it is the transfers' latency: four stages
-// (one bf16 matrix of 1024 x 1024 151 us, with three 154, with two 174).  Layouts are those of the big tile's loop; a k-major stage has 64 k rows
+// (a step on one bf16 matrix of 1024 x 1024 151 us, with three 154, with two 174).  Layouts are those of the big tile's loop; a k-major stage has 64 k rows
 // of 256 or 128 bytes.
 template <int SIDE, int STAGES>
 struct SmallTileOf {
@@ -1102,7 +1103,7 @@ int launch_tiles(ProductArgs a, int64_t tiles, hipStream_t stream, const char* w
     return TRLK_OK;
 }
 // The size of tiles whose launch is done soonest, in units of a big tile's time.  A round is 256 big ones.  Of 128 x 128 two run on a CU, 512 take 0.6 of
-// that, 256 or fewer 0.36; of 64 x 64 two, too, 512 take 0.27, 256 or fewer 0.235.  Both sides in us: one bf16 matrix
+// that, 256 or fewer 0.36; of 64 x 64 two, too, 512 take 0.27, 256 or fewer 0.235.  Both sides in us: a step on one bf16 matrix
 // of 1024 x 1024 478 with 256 alone, 252 with 128, 150 with 64; 1408 x 1408 314 with 128, 212 with 64; 2048 x 2048 420 and 455, 432 with 64 for
 // the symmetric products only, 528 tiles; 8 of 512 x 512 189 and 154; fp32, 24 of 1150 x 2816: X X^T 468 with 256, 431 with 128, A A 222 and 195, X's own
 // product, 1320 tiles of 256, 660 and 697.

@@ -33,7 +33,7 @@ def orthogonalize(matrices: Tensor | Sequence[Tensor], *, ns_coefficients: tuple
 
     `matrices` is one tensor `[..., m, n]` or a list of them (then a list is returned), in fp32, bf16 or fp16, all on one GPU: all in one call.  The
     products hold 22 bits, whatever the type, and sum in fp32: the result is about as near to the exact iteration's as one in plain fp32, before it is rounded
-    to its type.  A matrix of zeros gives zeros, one with a NaN or an infinity NaN.  Coefficients with which values of at most 1 would grow
+    to its type; its last bits may depend on what else is in the call.  A matrix of zeros gives zeros, one with a NaN or an infinity NaN.  Coefficients with which values of at most 1 would grow
     past 2.5 raise.  Not differentiable."""
     numbers = _numbers(ns_coefficients, ns_steps, eps)
     if isinstance(matrices, Tensor):
