@@ -552,8 +552,8 @@ int trlk_embedding_bwd(const void* d_grad, int dtype, int64_t n, int64_t cols, i
  *   p = p (1 - lr weight_decay) - lr stretch X;   stretch = sqrt(max(1, rows / cols)), or 0.2 sqrt(max(rows, cols)) (MATCH_ADAMW)
  * Elementwise arithmetic and sums are fp32 (norms in 64 bits), p is rounded once to its type.  Products
  * hold 22 bits, and the result is about as near to the exact iteration's as one in plain fp32; a step on parameters of 16 bits rounds the products' operands to
- * 11 bits, unless errors grow by more in its iteration than in the usual one of five steps (its update is off by up to 2e-3 of its size, 8e-3 where entries are
- * alike but for their sign).  The tables are HOST memory, read before the call returns.  d_param, d_grad and d_momentum (fp32) are dense [rows, cols];
+ * 11 bits, unless errors grow by more in its iteration than in the usual one of five steps (its update is mostly within 2e-3 of its size, and within 1e-2
+ * where entries are alike but for their sign).  The tables are HOST memory, read before the call returns.  d_param, d_grad and d_momentum (fp32) are dense [rows, cols];
  * what is written shares no memory with anything else that is listed.  trlk_orthogonalize: d_param takes X, turned back, of d_grad (they may be
  * the same), d_momentum is NULL.  The smaller side is 32768 at most, the larger one 2^22, both 2^34 entries.  A matrix with a NaN or an infinity comes out as NaN.
  * Of matrices with both sides over 64, what is under 2^-39 of max(|u|, eps) is lost, and the last bits may depend on what else is in the call.

@@ -14,8 +14,8 @@
 // carries the small singular values (they grow by a in each step), all 22 bits but for the last step's.  The largest entries of B are its diagonal's: what their
 // rounding leaves is kept in fp32 and multiplied with X's hi piece beside that term (66 rows: 1.96e-3 of the update -> 1.5e-3).  Against the exact
 // iteration the update is then off by 0.9 to 1.5e-3 of its size for matrices of independent entries, up to 1.9e-3 where few singular values are large, and where
-// entries are alike but for their sign, whose roundings go one way, by up to 8e-3 (an identity); a parameter in 16 bits, rounded to 2^-9 of ITS size and moved by a
-// small part of that, does not show it.  More steps, or other coefficients, whose slopes would make more of the loss take two pieces, too (error_growth).  With one
+// entries are alike but for their sign, whose roundings go one way, by up to 1e-2 (ones of 383 x 4096 9.5e-3, an identity 7.7e-3); a parameter in 16 bits, rounded to 2^-9 of
+// ITS size and moved by a small part of that, does not show it.  More steps, or other coefficients, whose slopes would make more of the loss take two pieces, too (error_growth).  With one
 // piece for X as well those losses were up to 4e-2, with bf16 operands 3e-1.
 #include <math.h>
 

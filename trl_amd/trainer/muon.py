@@ -52,7 +52,7 @@ def muon_step_(params: list[Tensor], grads: list[Tensor], momentum_buffers: list
     `momentum_buffers` are fp32.  `stretch` is `sqrt(max(1, m / n))` (`adjust_lr_fn` None or "original") or `0.2 sqrt(max(m, n))`
     ("match_rms_adamw", with which learning rates are those of AdamW).  `lr` may be an fp32 number on the GPU.  Parameters are rounded once;
     those in fp32 take their update from products of 22 bits, those in 16 bits from ones of 11: that update is mostly within 2e-3 of the exact one's size, and
-    within 8e-3 where its entries are alike but for their sign.  More than five steps, or other coefficients, that would make more of the rounding
+    within 1e-2 where its entries are alike but for their sign.  More than five steps, or other coefficients, that would make more of the rounding
     take 22 bits, too.  Matrices of 64 rows (or columns) or fewer go by 64 bits.  Tensors that are written share
     no memory, with each other or with a gradient."""
     if not len(params):
