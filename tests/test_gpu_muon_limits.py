@@ -225,3 +225,91 @@ def test_a_resumed_run_steps_weights_in_another_order():
     for seed in range(2, 4):
         step(other, again, seed)
     assert all(torch.equal(p, q) for p, q in zip(whole.parameters(), other.parameters()))
+
+
+def test_the_optimizers_step_in_a_graph():
+    """Both kinds of groups, a learning rate on the GPU and one that is a number, replayed on new gradients with eager work between."""
+    import trl_amd
+
+    def made():
+        torch.manual_seed(3)
+        w = [torch.nn.Parameter(torch.randn(s, device=DEV).to(t) * 0.05) for s, t in (((90, 200), torch.bfloat16), ((16, 300), torch.float32), ((300, 70), torch.float32))]
+        rest = [torch.nn.Parameter(torch.randn(s, device=DEV)) for s in ((200,), (97, 40))]
+        lr = torch.tensor(0.01, device=DEV)
+        return w + rest, lr, trl_amd.Muon([dict(params=w[:2], lr=lr), dict(params=w[2:], ns_steps=3), dict(params=rest, adamw=True)], lr=0.02)
+
+    def fill(params, seed):
+        gen = torch.Generator(device=DEV).manual_seed(seed)
+        for p in params:
+            g = (torch.randn(p.shape, generator=gen, device=DEV) * 1e-2).to(p.dtype)
+            p.grad = g if p.grad is None else p.grad.copy_(g)
+
+    (params, lr, opt), (twins, their_lr, eager) = made(), made()
+    stream = torch.cuda.Stream()
+    fill(params, 0)
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(stream):
+        opt.step()
+    torch.cuda.current_stream().wait_stream(stream)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        opt.step()
+    fill(twins, 0)
+    eager.step()
+    for seed in range(1, 5):
+        fill(params, seed)
+        fill(twins, seed)
+        lr.fill_(0.01 / seed)
+        their_lr.fill_(0.01 / seed)
+        graph.replay()
+        eager.step()
+        torch.cuda.synchronize()
+        assert all(torch.equal(p, q) for p, q in zip(params, twins)), seed
+        assert all(torch.equal(x, y) for p, q in zip(params, twins) for x, y in zip(opt.state[p].values(), eager.state[q].values())), seed
+
+
+def test_calls_on_two_streams_at_once():
+    import trl_amd
+
+    gen = torch.Generator(device=DEV).manual_seed(5)
+    each = [torch.randn(s, generator=gen, device=DEV).to(t) for s, t in (((300, 500), torch.float32), ((700, 400), torch.bfloat16), ((12, 5000), torch.float32))]
+    ids = torch.randint(0, 900, (9000,), generator=gen, device=DEV)
+    g = torch.randn((9000, 130), generator=gen, device=DEV)
+    want = trl_amd.orthogonalize(each), trl_amd.ops.embedding_bwd(g, ids, 900, 1.0, -1)
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    results = []
+    for _ in range(4):
+        for s in streams:
+            with torch.cuda.stream(s):
+                results.append((trl_amd.orthogonalize(each), trl_amd.ops.embedding_bwd(g, ids, 900, 1.0, -1)))
+    torch.cuda.synchronize()
+    for xs, grad in results:
+        assert all(torch.equal(x, y) for x, y in zip(xs, want[0])) and torch.equal(grad, want[1])
+
+
+def test_a_patched_scaled_embedding_in_a_graph():
+    """Its tensor of a scale has been read when the patch was made: no wait for the GPU in the capture."""
+    import trl_amd
+    from transformers.models.gemma3.modeling_gemma3 import Gemma3TextScaledWordEmbedding
+
+    class Model(torch.nn.Module):
+        def __init__(self):
+            super().__init__()
+            self.embed = Gemma3TextScaledWordEmbedding(97, 72, 4, embed_scale=1152**0.5)
+
+        def get_input_embeddings(self):
+            return self.embed
+
+    model = Model().to(DEV, torch.bfloat16)
+    trl_amd.patch_embedding(model)
+    ids = torch.zeros((3, 50), dtype=torch.int64, device=DEV)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph), torch.no_grad():
+        rows = model.embed(ids)
+    gen = torch.Generator(device=DEV).manual_seed(1)
+    for _ in range(4):
+        ids.copy_(torch.randint(0, 97, ids.shape, generator=gen, device=DEV))
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(rows, Gemma3TextScaledWordEmbedding.forward(model.embed, ids))
